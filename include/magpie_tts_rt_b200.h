@@ -2,7 +2,7 @@
  * magpie_tts_rt_b200 -- B200 (sm_100a) implementation of MagpieTTS-RT's
  * per-frame Local AR + sampling hot path, behind the reference's C ABI.
  *
- * Five groups of entry points:
+ * Seven groups of entry points:
  *
  * 1. The plugin-library ABI the runtime dlopen()s
  *    (reference: include/magpie_tts_rt/magpie_tts_rt_plugin.h:70-152,
@@ -34,6 +34,12 @@
  * 5. The Main Decoder one-step (reference:
  *    tools/export/main_decoder_wrapper.py MainDecoderStepWrapper), batched
  *    over sessions: the decoder position between two Local AR frames.
+ *
+ * 6. The per-GPU session engine: the host side of the per-step loop.
+ *
+ * 7. A paged key/value cache (extend, fork, free, compact, store) and the
+ *    attention that reads it: sliding window with sinks, single-token and
+ *    prompt forms, and groups of sessions that share a prefix.
  *
  * Streams (`void* stream`) are cudaStream_t values; NULL is the legacy
  * default stream.
@@ -703,6 +709,142 @@ MTT_B200_API int mtt_b200_session_engine_step(mtt_b200_session_engine_t* engine)
 MTT_B200_API int mtt_b200_session_engine_collect(mtt_b200_session_engine_t* engine, int32_t n,
                                                  int64_t* codec_tokens, int32_t* end_frame_index,
                                                  int32_t* invalid_rows);
+
+/* ------------------------------------------------------------------------ */
+/* 7. Paged key/value cache and the attention that reads it (no reference     */
+/*    counterpart: its caches are one fixed block per session)                */
+/* ------------------------------------------------------------------------ */
+
+/*
+ * A pool of pages shared by `slots` token sequences.  A page holds page_size
+ * consecutive tokens' keys and values of every layer:
+ *   pool [pages][layers][2][kv_heads][page_size][head_dim]   (0 keys, 1 values)
+ * Slot i's token t lies in page page_table[i][t / page_size] at row
+ * t % page_size.  A page may belong to several slots (refs counts them); a
+ * page that is not full belongs to one slot only, so tokens are appended
+ * without looking at other slots.  Free pages are those with refs 0;
+ * allocation takes the lowest free page first, for the slots in order, so the
+ * state after any sequence of calls is determined by the calls alone.
+ *
+ * All state is caller-owned device memory, every call is stream-ordered with
+ * no host synchronisation, and returns MTT_B200_STATUS_*.  Page numbers
+ * outside [0, pages) stand for "no page" and lengths are read as at most
+ * table_pages * page_size, so no table content leads out of the pool.  The
+ * calls of one cache that change it must be ordered with each other and with
+ * its readers (one stream, or events).
+ *
+ * status[i] (may be NULL), written by fork and extend for each slot they are
+ * asked to change: 0 done; 1 a source slot or count out of range; 2 not
+ * enough free pages; with 1 and 2 the slot is left as it was.  store writes
+ * it only for rows it skips: 1 the slot's offsets do not fit, 3 the row would
+ * go to a page that other slots share, or to none.
+ */
+#define MTT_B200_DTYPE_BF16 0
+#define MTT_B200_DTYPE_F16 1
+
+typedef struct mtt_b200_paged_cache {
+  int32_t pages;
+  int32_t layers;
+  int32_t kv_heads;
+  int32_t page_size;   /* 16, 32, 64 or 128 */
+  int32_t head_dim;    /* 64 or 128 */
+  int32_t dtype;       /* MTT_B200_DTYPE_* of the pool, of keys, values, queries and outputs */
+  int32_t slots;       /* <= 16384 */
+  int32_t table_pages; /* page_table columns; table_pages * page_size < 2^31 */
+  void* pool;          /* 128-byte aligned */
+  int32_t* page_table; /* [slots][table_pages], -1 past a slot's pages */
+  int32_t* lengths;    /* [slots] tokens */
+  int32_t* refs;       /* [pages] */
+  int32_t* status;     /* [slots] or NULL */
+  int32_t* live;       /* [1] or NULL: pages in use, written by compact */
+} mtt_b200_paged_cache_t;
+
+/* Workspace bytes for any call on this cache with queries of q_heads heads (0
+ * for bad arguments).  256-byte aligned, zeroed once before its first use; one
+ * workspace serves one stream at a time. */
+MTT_B200_API size_t mtt_b200_paged_cache_workspace_size(const mtt_b200_paged_cache_t* cache, int32_t q_heads);
+
+/* lengths[i] += counts[i] (counts [slots] int32, >= 0), with the new pages
+ * that takes.  A slot's new pages are granted while the pages asked for by it
+ * and the slots before it are free. */
+MTT_B200_API int mtt_b200_launch_paged_cache_extend(const mtt_b200_paged_cache_t* cache, const int32_t* counts,
+                                                    void* workspace, size_t workspace_bytes, void* stream);
+
+/* For every slot d with source[d] >= 0 and != d: d's tokens become those that
+ * slot source[d] had before the call (all slots at once: a permutation
+ * reorders them), d's own pages are released.  Full pages are shared; a
+ * partial last page is copied.  deep != 0: every page is copied.  source[d]
+ * -1 or d: d stays.  The copies' pages come from those free before the call. */
+MTT_B200_API int mtt_b200_launch_paged_cache_fork(const mtt_b200_paged_cache_t* cache, const int32_t* source,
+                                                  int32_t deep, void* workspace, size_t workspace_bytes,
+                                                  void* stream);
+
+/* Releases the pages of every slot with mask[i] (mask [slots] bool): length 0, no pages. */
+MTT_B200_API int mtt_b200_launch_paged_cache_free(const mtt_b200_paged_cache_t* cache, const bool* mask,
+                                                  void* stream);
+
+/* Moves pages so that those in use are [0, live): the i-th page in use at or
+ * past `live` goes to the i-th free page before it; tables and refs follow. */
+MTT_B200_API int mtt_b200_launch_paged_cache_compact(const mtt_b200_paged_cache_t* cache, void* workspace,
+                                                     size_t workspace_bytes, void* stream);
+
+/* Writes the keys and values of the last tokens of each slot: rows
+ * [offsets[i], offsets[i + 1]) of k and v are slot i's last ones (offsets
+ * [slots + 1] int32, ascending, within [0, rows]); offsets NULL: row i is the
+ * last token of slot i (rows <= slots; empty slots skipped).  k and v:
+ * [n_layers][rows][kv_heads][head_dim] with strides in elements (multiples of
+ * 8, 16-byte aligned bases; heads contiguous), for layers [layer, layer +
+ * n_layers). */
+typedef struct mtt_b200_cache_rows {
+  int32_t layer;
+  int32_t n_layers;
+  int32_t rows;
+  int32_t reserved_0;
+  const void* k;
+  const void* v;
+  int64_t k_row_stride;
+  int64_t v_row_stride;
+  int64_t k_layer_stride;
+  int64_t v_layer_stride;
+  const int32_t* offsets;
+} mtt_b200_cache_rows_t;
+
+MTT_B200_API int mtt_b200_launch_paged_cache_store(const mtt_b200_paged_cache_t* cache,
+                                                   const mtt_b200_cache_rows_t* rows, void* stream);
+
+/* Attention of query rows over one layer of the cache.  A query at position p
+ * of its slot sees key j when j <= p and (window 0, p - j < window, or j <
+ * sinks) and key_mask[slot][j] (where given):
+ *   out = sum_j exp(scale q.k_j) v_j / sum_j exp(scale q.k_j)
+ *   lse = log sum_j exp(scale q.k_j)          (natural log, f32)
+ * with f32 sums; a row that sees no key gets out 0 and lse -inf.  Keys that
+ * no query may see (past the length, or masked) do not reach the result,
+ * whatever their bytes.  Query head h reads key head h / (q_heads / kv_heads).
+ *
+ * offsets NULL: row i is the last token of slot i (rows <= slots).  With
+ * offsets ([slots + 1] int32, as for store) slot i's rows are its last
+ * offsets[i + 1] - offsets[i] tokens, whose keys and values are already
+ * stored; the rows of a slot whose offsets do not fit get out 0 and lse -inf. */
+typedef struct mtt_b200_cache_attention {
+  int32_t layer;
+  int32_t q_heads;          /* a multiple of kv_heads, q_heads / kv_heads <= 64 */
+  int32_t rows;
+  int32_t window;           /* 0: no window */
+  int32_t sinks;            /* >= 0; no effect without a window */
+  float scale;
+  const void* q;            /* [rows][q_heads][head_dim], 16-byte aligned */
+  int64_t q_row_stride;     /* elements, a multiple of 8 */
+  void* out;                /* [rows][q_heads][head_dim], 16-byte aligned */
+  int64_t out_row_stride;   /* elements, a multiple of 8 */
+  float* lse;               /* [rows][q_heads] or NULL */
+  const int32_t* offsets;   /* [slots + 1] or NULL */
+  const bool* key_mask;     /* [slots][mask_stride] or NULL */
+  int64_t mask_stride;      /* >= table_pages * page_size */
+} mtt_b200_cache_attention_t;
+
+MTT_B200_API int mtt_b200_launch_paged_attention(const mtt_b200_paged_cache_t* cache,
+                                                 const mtt_b200_cache_attention_t* args, void* workspace,
+                                                 size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------ */
 /* Test hooks (no reference counterpart beyond launch_test_clamped_gumbel,   */

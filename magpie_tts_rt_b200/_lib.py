@@ -172,6 +172,28 @@ class SessionEngineBuffers(ctypes.Structure):
                                  "decoder_status")]
 
 
+DTYPE_BF16 = 0
+DTYPE_F16 = 1
+
+
+class PagedCache(ctypes.Structure):
+    _fields_ = [(n, I32) for n in ("pages", "layers", "kv_heads", "page_size", "head_dim", "dtype", "slots",
+                                   "table_pages")] + [(n, P) for n in ("pool", "page_table", "lengths", "refs",
+                                                                       "status", "live")]
+
+
+class CacheRows(ctypes.Structure):
+    _fields_ = [("layer", I32), ("n_layers", I32), ("rows", I32), ("reserved_0", I32), ("k", P), ("v", P),
+                ("k_row_stride", I64), ("v_row_stride", I64), ("k_layer_stride", I64), ("v_layer_stride", I64),
+                ("offsets", P)]
+
+
+class CacheAttention(ctypes.Structure):
+    _fields_ = [("layer", I32), ("q_heads", I32), ("rows", I32), ("window", I32), ("sinks", I32),
+                ("scale", ctypes.c_float), ("q", P), ("q_row_stride", I64), ("out", P), ("out_row_stride", I64),
+                ("lse", P), ("offsets", P), ("key_mask", P), ("mask_stride", I64)]
+
+
 # name -> (restype, argtypes)
 SIGNATURES = {
     "mtt_plugin_get_api_v1": (I32, [ctypes.POINTER(PluginApiV1)]),
@@ -202,6 +224,15 @@ SIGNATURES = {
     "mtt_b200_main_decoder_workspace_size": (SZ, [I32, I32]),
     "mtt_b200_launch_main_decoder_step": (
         I32, [ctypes.POINTER(MainDecoderWeights), ctypes.POINTER(MainDecoderBatch), P, SZ, P]),
+    "mtt_b200_paged_cache_workspace_size": (SZ, [ctypes.POINTER(PagedCache), I32]),
+    "mtt_b200_launch_paged_cache_extend": (I32, [ctypes.POINTER(PagedCache), P, P, SZ, P]),
+    "mtt_b200_launch_paged_cache_fork": (I32, [ctypes.POINTER(PagedCache), P, I32, P, SZ, P]),
+    "mtt_b200_launch_paged_cache_free": (I32, [ctypes.POINTER(PagedCache), P, P]),
+    "mtt_b200_launch_paged_cache_compact": (I32, [ctypes.POINTER(PagedCache), P, SZ, P]),
+    "mtt_b200_launch_paged_cache_store": (
+        I32, [ctypes.POINTER(PagedCache), ctypes.POINTER(CacheRows), P]),
+    "mtt_b200_launch_paged_attention": (
+        I32, [ctypes.POINTER(PagedCache), ctypes.POINTER(CacheAttention), P, SZ, P]),
     "mtt_b200_launch_test_clamped_gumbel": (I32, [P, P, SZ, P]),
     "mtt_b200_launch_test_log": (I32, [P, P, SZ, P]),
     "mtt_b200_launch_test_gemm": (I32, [P, P, P, I32, I32, I32, I32, I32, P, P]),

@@ -1,0 +1,532 @@
+// Upkeep of the paged key/value cache: extend, fork, free, compact, store.
+//
+// Every operator is a plan (which pages go where: integers, scanned over the
+// slots and over the pool's reference counts by one CTA, so the result does
+// not depend on timing) followed by the movement of whole pages or rows,
+// which is bound by HBM: each byte is read once and written once with
+// 16-byte accesses, enough of them in flight to cover the latency.
+#include <algorithm>
+#include <atomic>
+
+#include "paged_cache.cuh"
+
+namespace mtt {
+namespace {
+
+constexpr int kPlanThreads = 1024;
+constexpr int kMoveThreads = 256;
+
+// Workspace of one upkeep call, in 32-bit words.
+struct UpkeepSpace {
+  int32_t* free_list;  // [pages] free pages, ascending
+  int32_t* rank;       // [slots] index of the slot's first new page in free_list; -1 not granted
+  int32_t* len;        // [slots] forked lengths
+  int32_t* rows;       // [slots][table_pages] forked rows
+  int32_t* src;        // [pages] page copies: from
+  int32_t* dst;        // [pages] to
+  int32_t* map;        // [pages] compact: new number of each page
+  int32_t* counts;     // [4] 0 page copies
+};
+
+size_t upkeep_words(int64_t pages, int64_t slots, int64_t table_pages) {
+  return static_cast<size_t>(4 * pages + 2 * slots + slots * table_pages + 64);
+}
+
+UpkeepSpace upkeep_space(const PagedCache& c, void* ws) {
+  int32_t* p = static_cast<int32_t*>(ws);
+  UpkeepSpace u;
+  u.counts = p;
+  p += 64;
+  u.free_list = p;
+  p += c.pages;
+  u.src = p;
+  p += c.pages;
+  u.dst = p;
+  p += c.pages;
+  u.map = p;
+  p += c.pages;
+  u.rank = p;
+  p += c.slots;
+  u.len = p;
+  p += c.slots;
+  u.rows = p;
+  return u;
+}
+
+// Exclusive prefix sum over the block's threads; `total` gets the sum.
+__device__ __forceinline__ int block_scan(int v, int* total) {
+  __shared__ int warp_sum[kPlanThreads / 32];
+  __shared__ int all;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int inc = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int n = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += n;
+  }
+  if (lane == 31) warp_sum[warp] = inc;
+  __syncthreads();
+  if (warp == 0) {
+    int s = warp_sum[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int n = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += n;
+    }
+    warp_sum[lane] = s;
+    if (lane == 31) all = s;
+  }
+  __syncthreads();
+  const int before = (warp > 0 ? warp_sum[warp - 1] : 0) + inc - v;
+  *total = all;
+  __syncthreads();
+  return before;
+}
+
+// Lists the free pages in ascending order; returns how many there are.
+__device__ int list_free(const PagedCache& c, int32_t* list) {
+  int found = 0;
+  for (int base = 0; base < c.pages; base += 4 * kPlanThreads) {
+    const int p0 = base + 4 * threadIdx.x;
+    bool f[4];
+    int n = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      f[j] = p0 + j < c.pages && c.refs[p0 + j] == 0;
+      n += f[j];
+    }
+    int total;
+    int at = found + block_scan(n, &total);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (f[j]) list[at++] = p0 + j;
+    found += total;
+  }
+  __syncthreads();
+  return found;
+}
+
+// One CTA.  Grants the slots' new pages and writes them into the tables.
+__global__ void __launch_bounds__(kPlanThreads) extend_kernel(PagedCache c, const int32_t* counts, UpkeepSpace u) {
+  wait_prior_grid();
+  const int free_pages = list_free(c, u.free_list);
+  int asked = 0;
+  for (int base = 0; base < c.slots; base += kPlanThreads) {
+    const int i = base + threadIdx.x;
+    int need = 0, have = 0, add = 0, len = 0, st = 0;
+    if (i < c.slots) {
+      len = c.length(i);
+      add = counts[i];
+      have = (len + c.page_size - 1) >> c.page_shift;
+      // the sum is taken in 64 bits: a count near 2^31 is refused, not wrapped
+      const int64_t want = (static_cast<int64_t>(len) + add + c.page_size - 1) >> c.page_shift;
+      if (add < 0 || want > c.table_pages) {
+        st = 1;
+      } else {
+        need = static_cast<int>(want) - have;
+      }
+    }
+    int total;
+    const int rank = asked + block_scan(need, &total);
+    if (i < c.slots) {
+      if (st == 0 && need > 0 && rank + need > free_pages) st = 2;
+      if (st == 0 && add > 0) {
+        int32_t* row = c.table + static_cast<int64_t>(i) * c.table_pages + have;
+        for (int j = 0; j < need; ++j) {
+          const int p = u.free_list[rank + j];
+          row[j] = p;
+          c.refs[p] = 1;
+        }
+        c.lengths[i] = len + add;
+      }
+      if (c.status != nullptr && (add != 0 || st != 0)) c.status[i] = st;
+    }
+    asked += total;
+  }
+}
+
+// One CTA: which slots are forked, and their first private page's rank.
+__global__ void __launch_bounds__(kPlanThreads)
+    fork_plan_kernel(PagedCache c, const int32_t* source, int deep, UpkeepSpace u) {
+  wait_prior_grid();
+  const int free_pages = list_free(c, u.free_list);
+  int asked = 0, granted = 0;
+  for (int base = 0; base < c.slots; base += kPlanThreads) {
+    const int i = base + threadIdx.x;
+    int need = 0, s = -1, st = 0;
+    bool touch = false;
+    if (i < c.slots) {
+      s = source[i];
+      touch = s != -1 && s != i;
+      if (touch && (s < 0 || s >= c.slots)) st = 1;
+      if (touch && st == 0) {
+        const int len = c.length(s);
+        need = deep ? (len + c.page_size - 1) >> c.page_shift : ((len & (c.page_size - 1)) != 0 ? 1 : 0);
+      }
+    }
+    int total;
+    const int rank = asked + block_scan(need, &total);
+    const bool ok = touch && st == 0 && (need == 0 || rank + need <= free_pages);
+    int pages;
+    block_scan(ok ? need : 0, &pages);
+    if (i < c.slots) {
+      u.rank[i] = ok ? rank : -1;
+      if (touch && c.status != nullptr) c.status[i] = st != 0 ? st : (ok ? 0 : 2);
+    }
+    asked += total;
+    granted += pages;
+  }
+  if (threadIdx.x == 0) u.counts[0] = granted;
+}
+
+// Slot d (one CTA each): its new row, from its source's old one, and the page copies it asks for.
+__global__ void __launch_bounds__(kMoveThreads) fork_rows_kernel(PagedCache c, const int32_t* source, int deep,
+                                                                 UpkeepSpace u) {
+  wait_prior_grid();
+  const int d = blockIdx.x;
+  const int rank = u.rank[d];
+  if (rank < 0) return;
+  const int s = source[d];
+  const int len = c.length(s);
+  const int used = (len + c.page_size - 1) >> c.page_shift;
+  const int first_copy = deep ? 0 : len >> c.page_shift;
+  const int32_t* old = c.table + static_cast<int64_t>(s) * c.table_pages;
+  int32_t* row = u.rows + static_cast<int64_t>(d) * c.table_pages;
+  for (int j = threadIdx.x; j < c.table_pages; j += kMoveThreads) {
+    int p = j < used ? old[j] : -1;
+    if (j < used && j >= first_copy) {
+      const int to = u.free_list[rank + j - first_copy];
+      u.src[rank + j - first_copy] = p;
+      u.dst[rank + j - first_copy] = to;
+      p = to;
+    }
+    row[j] = p;
+    if (c.is_page(p)) atomicAdd(&c.refs[p], 1);
+  }
+  if (threadIdx.x == 0) u.len[d] = len;
+}
+
+// Part `part` of `parts` of one page, all layers.
+__device__ __forceinline__ void copy_page(const PagedCache& c, int from, int to, int part, int parts) {
+  const int64_t vecs = static_cast<int64_t>(c.layers) * 2 * c.kv_elems / 8;
+  const int64_t lo = vecs * part / parts, hi = vecs * (part + 1) / parts;
+  const uint4* s = reinterpret_cast<const uint4*>(c.pool) + from * vecs;
+  uint4* d = reinterpret_cast<uint4*>(c.pool) + to * vecs;
+  int64_t v = lo + threadIdx.x;
+  for (; v + 3 * kMoveThreads < hi; v += 4 * kMoveThreads) {
+    uint4 x[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = __ldcs(s + v + j * kMoveThreads);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) __stcs(d + v + j * kMoveThreads, x[j]);
+  }
+  for (; v < hi; v += kMoveThreads) __stcs(d + v, __ldcs(s + v));
+}
+
+// The plan's page copies, `parts` pieces each, dealt over the grid.
+__device__ __forceinline__ void copy_pairs(const PagedCache& c, const UpkeepSpace& u, int parts) {
+  const int64_t items = static_cast<int64_t>(u.counts[0]) * parts;
+  for (int64_t w = blockIdx.x; w < items; w += gridDim.x) {
+    const int pair = static_cast<int>(w / parts);
+    const int from = u.src[pair], to = u.dst[pair];
+    if (c.is_page(from) && c.is_page(to)) copy_page(c, from, to, static_cast<int>(w % parts), parts);
+  }
+}
+
+// The forked rows and lengths become the slots', the pages they had are released, partial pages copied.
+__global__ void __launch_bounds__(kMoveThreads) fork_commit_kernel(PagedCache c, UpkeepSpace u, int parts) {
+  wait_prior_grid();
+  for (int d = blockIdx.x; d < c.slots; d += gridDim.x) {
+    if (u.rank[d] < 0) continue;
+    int32_t* row = c.table + static_cast<int64_t>(d) * c.table_pages;
+    const int32_t* next = u.rows + static_cast<int64_t>(d) * c.table_pages;
+    for (int j = threadIdx.x; j < c.table_pages; j += kMoveThreads) {
+      const int p = row[j];
+      if (c.is_page(p)) atomicSub(&c.refs[p], 1);
+      row[j] = next[j];
+    }
+    if (threadIdx.x == 0) c.lengths[d] = u.len[d];
+  }
+  copy_pairs(c, u, parts);
+}
+
+// One warp per slot.
+__global__ void __launch_bounds__(kMoveThreads) free_kernel(PagedCache c, const bool* mask) {
+  wait_prior_grid();
+  const int i = blockIdx.x * (kMoveThreads / 32) + (threadIdx.x >> 5);
+  if (i >= c.slots || !mask[i]) return;
+  int32_t* row = c.table + static_cast<int64_t>(i) * c.table_pages;
+  for (int j = threadIdx.x & 31; j < c.table_pages; j += 32) {
+    const int p = row[j];
+    if (c.is_page(p)) atomicSub(&c.refs[p], 1);
+    row[j] = -1;
+  }
+  if ((threadIdx.x & 31) == 0) c.lengths[i] = 0;
+}
+
+// One CTA: live pages, and where those past the live count go.
+__global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(PagedCache c, UpkeepSpace u) {
+  wait_prior_grid();
+  const int live = c.pages - list_free(c, u.free_list);  // free pages below `live` come first in the list
+  int moved = 0;
+  for (int base = live & ~(4 * kPlanThreads - 1); base < c.pages; base += 4 * kPlanThreads) {
+    const int p0 = base + 4 * threadIdx.x;
+    bool f[4];
+    int n = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      f[j] = p0 + j >= live && p0 + j < c.pages && c.refs[p0 + j] != 0;
+      n += f[j];
+    }
+    int total;
+    int at = moved + block_scan(n, &total);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (f[j]) {
+        const int to = u.free_list[at];
+        u.src[at] = p0 + j;
+        u.dst[at] = to;
+        u.map[p0 + j] = to;
+        ++at;
+      }
+    }
+    moved += total;
+  }
+  if (threadIdx.x == 0) {
+    u.counts[0] = moved;
+    u.counts[1] = live;
+    if (c.live != nullptr) c.live[0] = live;
+  }
+}
+
+__global__ void __launch_bounds__(kMoveThreads) compact_move_kernel(PagedCache c, UpkeepSpace u, int parts) {
+  wait_prior_grid();
+  const int moved = u.counts[0], live = u.counts[1];
+  if (moved == 0) return;
+  const int64_t entries = static_cast<int64_t>(c.slots) * c.table_pages;
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * kMoveThreads;
+  const int64_t me = static_cast<int64_t>(blockIdx.x) * kMoveThreads + threadIdx.x;
+  for (int64_t e = me; e < entries; e += stride) {
+    const int p = c.table[e];
+    if (p >= live && p < c.pages) c.table[e] = u.map[p];
+  }
+  for (int64_t m = me; m < moved; m += stride) {
+    c.refs[u.dst[m]] = c.refs[u.src[m]];
+    c.refs[u.src[m]] = 0;
+  }
+  copy_pairs(c, u, parts);
+}
+
+struct Rows {
+  int layer, n_layers, rows;
+  const uint16_t *k, *v;
+  int64_t k_row, v_row, k_layer, v_layer;
+  const int32_t* offsets;
+};
+
+// Row blockIdx.x: its keys and values of every given layer to its slot's page.
+__global__ void __launch_bounds__(kMoveThreads) store_kernel(PagedCache c, Rows in) {
+  wait_prior_grid();
+  const int row = blockIdx.x;
+  int slot = row, count = 1, first = row;
+  if (in.offsets != nullptr) {
+    // the slot with offsets[slot] <= row < offsets[slot + 1]
+    int lo = 0, hi = c.slots;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (in.offsets[mid + 1] > row) hi = mid; else lo = mid + 1;
+    }
+    slot = lo;
+    if (slot >= c.slots) return;
+    first = in.offsets[slot];
+    count = in.offsets[slot + 1] - first;
+    if (first < 0 || first > row || in.offsets[slot + 1] > in.rows) {
+      if (threadIdx.x == 0 && c.status != nullptr) c.status[slot] = 1;
+      return;
+    }
+  }
+  const int len = c.length(slot);
+  if (in.offsets == nullptr && len == 0) return;
+  if (count > len) {
+    if (threadIdx.x == 0 && c.status != nullptr) c.status[slot] = 1;
+    return;
+  }
+  const int t = len - count + row - first;
+  const int page = c.table[static_cast<int64_t>(slot) * c.table_pages + (t >> c.page_shift)];
+  if (!c.is_page(page) || c.refs[page] > 1) {
+    if (threadIdx.x == 0 && c.status != nullptr) c.status[slot] = 3;
+    return;
+  }
+  const int hv = c.kv_heads * c.head_dim / 8;  // 16-byte pieces of one layer's keys
+  const int dv = c.head_dim / 8;
+  const int in_page = t & (c.page_size - 1);
+  for (int w = threadIdx.x; w < in.n_layers * 2 * hv; w += kMoveThreads) {
+    const int piece = w % hv, kv = (w / hv) & 1, l = w / (2 * hv);
+    const uint16_t* src = kv ? in.v + l * in.v_layer + row * in.v_row : in.k + l * in.k_layer + row * in.k_row;
+    const int h = piece / dv, e = piece % dv;
+    uint16_t* dst = c.pool + c.block(page, in.layer + l, kv) +
+                    (static_cast<int64_t>(h) * c.page_size + in_page) * c.head_dim + 8 * e;
+    *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(src + 8 * piece);
+  }
+}
+
+// Pieces a page copy is cut into: about 32 KB each, so that few large pages still occupy every SM.
+int copy_parts(const PagedCache& c) {
+  const int64_t bytes = static_cast<int64_t>(c.layers) * 4 * c.kv_elems;
+  return static_cast<int>(std::min<int64_t>(std::max<int64_t>((bytes + 32767) / 32768, 1), 4096));
+}
+
+}  // namespace
+
+int cache_sm_count() {
+  static std::atomic<int> known[64];  // by device ordinal; 0 not asked yet
+  int dev = -1, sms = 0;
+  if (cudaGetDevice(&dev) == cudaSuccess) {
+    if (dev >= 0 && dev < 64 && (sms = known[dev].load(std::memory_order_relaxed)) > 0) return sms;
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess) {
+      if (dev >= 0 && dev < 64) known[dev].store(sms, std::memory_order_relaxed);
+      return sms;
+    }
+  }
+  cudaGetLastError();
+  return 0;
+}
+
+int cache_call_status(cudaError_t e) {
+  if (e == cudaSuccess) e = cudaPeekAtLastError();
+  return e == cudaSuccess ? MTT_B200_STATUS_OK : MTT_B200_STATUS_CUDA_ERROR;
+}
+
+bool paged_cache_view(const mtt_b200_paged_cache_t* c, PagedCache* out) {
+  if (c == nullptr || c->pages < 1 || c->layers < 1 || c->kv_heads < 1 || c->slots < 1 || c->slots > kCacheMaxSlots ||
+      c->table_pages < 1 || (c->head_dim != 64 && c->head_dim != 128) ||
+      (c->page_size != 16 && c->page_size != 32 && c->page_size != 64 && c->page_size != 128) ||
+      (c->dtype != MTT_B200_DTYPE_BF16 && c->dtype != MTT_B200_DTYPE_F16))
+    return false;
+  // rows of the pool (one token's keys or values of one head) and tokens of a slot are counted in 31 bits
+  const double rows = static_cast<double>(c->pages) * c->layers * 2 * c->kv_heads * c->page_size;
+  if (rows >= 2147483648.0 || static_cast<int64_t>(c->table_pages) * c->page_size >= (int64_t{1} << 31)) return false;
+  if (c->pool == nullptr || c->page_table == nullptr || c->lengths == nullptr || c->refs == nullptr ||
+      (reinterpret_cast<uintptr_t>(c->pool) & 127u) != 0)
+    return false;
+  out->pages = c->pages;
+  out->layers = c->layers;
+  out->kv_heads = c->kv_heads;
+  out->page_size = c->page_size;
+  out->page_shift = c->page_size == 16 ? 4 : c->page_size == 32 ? 5 : c->page_size == 64 ? 6 : 7;
+  out->head_dim = c->head_dim;
+  out->slots = c->slots;
+  out->table_pages = c->table_pages;
+  out->kv_elems = static_cast<int64_t>(c->kv_heads) * c->page_size * c->head_dim;
+  out->pool = static_cast<uint16_t*>(c->pool);
+  out->table = c->page_table;
+  out->lengths = c->lengths;
+  out->refs = c->refs;
+  out->status = c->status;
+  out->live = c->live;
+  return true;
+}
+
+}  // namespace mtt
+
+using namespace mtt;
+
+namespace {
+
+size_t upkeep_bytes(const mtt_b200_paged_cache_t& c) {
+  return (4 * upkeep_words(c.pages, c.slots, c.table_pages) + 255) / 256 * 256;
+}
+
+// The upkeep words lie at the workspace's start.
+bool upkeep_checked(const mtt_b200_paged_cache_t* cache, void* ws, size_t bytes, PagedCache* c, UpkeepSpace* u) {
+  if (!paged_cache_view(cache, c) || ws == nullptr || !aligned16(ws) || bytes < upkeep_bytes(*cache)) return false;
+  *u = upkeep_space(*c, ws);
+  return true;
+}
+
+}  // namespace
+
+void* mtt::paged_attention_space(const mtt_b200_paged_cache_t& c, int q_heads, void* workspace, size_t bytes) {
+  const size_t up = upkeep_bytes(c);
+  if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0 ||
+      bytes < up + paged_attention_workspace(c, q_heads))
+    return nullptr;
+  return static_cast<char*>(workspace) + up;
+}
+
+extern "C" {
+
+size_t mtt_b200_paged_cache_workspace_size(const mtt_b200_paged_cache_t* cache, int32_t q_heads) {
+  PagedCache c;
+  if (!paged_cache_view(cache, &c) || q_heads < 1 || q_heads % c.kv_heads != 0 ||
+      q_heads / c.kv_heads > kCacheMaxGroup)
+    return 0;
+  return upkeep_bytes(*cache) + paged_attention_workspace(*cache, q_heads);
+}
+
+int mtt_b200_launch_paged_cache_extend(const mtt_b200_paged_cache_t* cache, const int32_t* counts, void* workspace,
+                                       size_t workspace_bytes, void* stream) {
+  PagedCache c;
+  UpkeepSpace u;
+  if (counts == nullptr || !upkeep_checked(cache, workspace, workspace_bytes, &c, &u))
+    return MTT_B200_STATUS_INVALID_ARGUMENT;
+  return cache_call_status(launch_serialized(extend_kernel, dim3(1), dim3(kPlanThreads), 0, static_cast<cudaStream_t>(stream), c,
+                                  counts, u));
+}
+
+int mtt_b200_launch_paged_cache_fork(const mtt_b200_paged_cache_t* cache, const int32_t* source, int32_t deep,
+                                     void* workspace, size_t workspace_bytes, void* stream) {
+  PagedCache c;
+  UpkeepSpace u;
+  const int sms = cache_sm_count();
+  if (source == nullptr || sms <= 0 || !upkeep_checked(cache, workspace, workspace_bytes, &c, &u))
+    return MTT_B200_STATUS_INVALID_ARGUMENT;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t e = launch_serialized(fork_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, c, source, deep, u);
+  if (e == cudaSuccess)
+    e = launch_serialized(fork_rows_kernel, dim3(c.slots), dim3(kMoveThreads), 0, s, c, source, deep, u);
+  if (e == cudaSuccess)
+    e = launch_serialized(fork_commit_kernel, dim3(8 * sms), dim3(kMoveThreads), 0, s, c, u, copy_parts(c));
+  return cache_call_status(e);
+}
+
+int mtt_b200_launch_paged_cache_free(const mtt_b200_paged_cache_t* cache, const bool* mask, void* stream) {
+  PagedCache c;
+  if (mask == nullptr || !paged_cache_view(cache, &c)) return MTT_B200_STATUS_INVALID_ARGUMENT;
+  constexpr int per = kMoveThreads / 32;
+  return cache_call_status(launch_serialized(free_kernel, dim3((c.slots + per - 1) / per), dim3(kMoveThreads), 0,
+                                  static_cast<cudaStream_t>(stream), c, mask));
+}
+
+int mtt_b200_launch_paged_cache_compact(const mtt_b200_paged_cache_t* cache, void* workspace, size_t workspace_bytes,
+                                        void* stream) {
+  PagedCache c;
+  UpkeepSpace u;
+  const int sms = cache_sm_count();
+  if (sms <= 0 || !upkeep_checked(cache, workspace, workspace_bytes, &c, &u)) return MTT_B200_STATUS_INVALID_ARGUMENT;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t e = launch_serialized(compact_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, c, u);
+  if (e == cudaSuccess)
+    e = launch_serialized(compact_move_kernel, dim3(8 * sms), dim3(kMoveThreads), 0, s, c, u, copy_parts(c));
+  return cache_call_status(e);
+}
+
+int mtt_b200_launch_paged_cache_store(const mtt_b200_paged_cache_t* cache, const mtt_b200_cache_rows_t* rows,
+                                      void* stream) {
+  PagedCache c;
+  if (rows == nullptr || !paged_cache_view(cache, &c) || rows->rows < 0 || rows->layer < 0 || rows->n_layers < 1 ||
+      rows->n_layers > c.layers - rows->layer)
+    return MTT_B200_STATUS_INVALID_ARGUMENT;
+  if (rows->rows == 0) return MTT_B200_STATUS_OK;
+  if (rows->k == nullptr || rows->v == nullptr || !aligned16(rows->k) || !aligned16(rows->v) ||
+      (rows->k_row_stride | rows->v_row_stride | rows->k_layer_stride | rows->v_layer_stride) % 8 != 0 ||
+      (rows->offsets == nullptr && rows->rows > c.slots))
+    return MTT_B200_STATUS_INVALID_ARGUMENT;
+  Rows in{rows->layer, rows->n_layers, rows->rows, static_cast<const uint16_t*>(rows->k),
+          static_cast<const uint16_t*>(rows->v), rows->k_row_stride, rows->v_row_stride, rows->k_layer_stride,
+          rows->v_layer_stride, rows->offsets};
+  return cache_call_status(launch_serialized(store_kernel, dim3(rows->rows), dim3(kMoveThreads), 0,
+                                  static_cast<cudaStream_t>(stream), c, in));
+}
+
+}  // extern "C"

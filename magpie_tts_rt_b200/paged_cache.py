@@ -1,0 +1,256 @@
+"""Paged key/value cache shared by many token sequences, and the attention
+that reads it (C ABI section 7 of include/magpie_tts_rt_b200.h).
+
+``PagedCache`` holds a pool of pages ``[pages, layers, 2, kv_heads, page_size,
+head_dim]`` (keys at index 0, values at 1), a page table and a length per
+slot, and a reference count per page, all on the device:
+
+* ``extend`` / ``store``: room for new tokens, and their keys and values;
+* ``fork``: slots take over other slots' tokens, full pages shared (sessions
+  started from one prefilled voice; reordering of slots);
+* ``free`` / ``compact``: slots closed, pages in use moved to the pool's start;
+* ``attend``: attention of each slot's newest token, or of runs of new tokens
+  (a prompt), with an optional sliding window and a few first tokens
+  (``sinks``) that stay visible.
+
+Every call is enqueued on the current (or given) CUDA stream and returns
+without waiting.  What a call cannot do on the device (no free page, offsets
+that do not fit) it reports in ``status``; what can be seen on the host
+(types, shapes, strides) raises ValueError before anything is launched.
+
+Calls that change a cache, and the calls that read it, must be ordered with
+each other by the caller when they use different streams.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional
+
+import torch
+
+from magpie_tts_rt_b200 import _lib as L
+
+PAGE_SIZES = (16, 32, 64, 128)
+HEAD_DIMS = (64, 128)
+MAX_SLOTS = 16384
+MAX_GROUP = 64
+_DTYPES = {torch.bfloat16: L.DTYPE_BF16, torch.float16: L.DTYPE_F16}
+
+
+def _check(ok: bool, what: str) -> None:
+    if not ok:
+        raise ValueError(what)
+
+
+class PagedCache:
+    def __init__(self, pool: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, refs: torch.Tensor):
+        """Adopts the tensors of a cache: pool [pages, layers, 2, kv_heads,
+        page_size, head_dim] bf16 or f16, page_table [slots, table_pages] int32
+        (-1: no page), lengths [slots] int32, refs [pages] int32; contiguous
+        and on one CUDA device."""
+        _check(pool.is_cuda, "the pool must be a CUDA tensor")
+        _check(pool.dim() == 6 and pool.shape[2] == 2, "pool must be [pages, layers, 2, kv_heads, page_size, head_dim]")
+        _check(pool.dtype in _DTYPES, "pool must be bfloat16 or float16")
+        pages, layers, _, kv_heads, page_size, head_dim = pool.shape
+        _check(min(pages, layers, kv_heads) >= 1, "a pool needs a page, a layer and a key head")
+        _check(page_size in PAGE_SIZES, f"page_size must be one of {PAGE_SIZES}")
+        _check(head_dim in HEAD_DIMS, f"head_dim must be one of {HEAD_DIMS}")
+        _check(page_table.dim() == 2 and min(page_table.shape) >= 1, "page_table must be [slots, table_pages]")
+        slots, table_pages = page_table.shape
+        _check(slots <= MAX_SLOTS, f"at most {MAX_SLOTS} slots")
+        _check(tuple(lengths.shape) == (slots,), "lengths must be [slots]")
+        _check(tuple(refs.shape) == (pages,), "refs must be [pages]")
+        for name, t in (("page_table", page_table), ("lengths", lengths), ("refs", refs)):
+            _check(t.dtype == torch.int32, f"{name} must be int32")
+        for name, t in (("pool", pool), ("page_table", page_table), ("lengths", lengths), ("refs", refs)):
+            _check(t.is_contiguous(), f"{name} must be contiguous")
+            _check(t.device == pool.device, f"{name} is on another device than the pool")
+        _check(pool.data_ptr() % 128 == 0, "the pool must be 128-byte aligned")
+        self.pool, self.page_table, self.lengths, self.refs = pool, page_table, lengths, refs
+        self.device = pool.device
+        self.dtype = pool.dtype
+        self.pages, self.layers, self.kv_heads, self.page_size, self.head_dim = (
+            pages, layers, kv_heads, page_size, head_dim)
+        self.slots, self.table_pages = slots, table_pages
+        self.status = torch.zeros(slots, dtype=torch.int32, device=self.device)
+        self.live = torch.zeros(1, dtype=torch.int32, device=self.device)
+        c = L.PagedCache()
+        c.pages, c.layers, c.kv_heads, c.page_size, c.head_dim = pages, layers, kv_heads, page_size, head_dim
+        c.dtype, c.slots, c.table_pages = _DTYPES[pool.dtype], slots, table_pages
+        c.pool, c.page_table, c.lengths, c.refs = (t.data_ptr() for t in (pool, page_table, lengths, refs))
+        c.status, c.live = self.status.data_ptr(), self.live.data_ptr()
+        self._c = c
+        self._ref = ctypes.byref(c)
+        self._spaces = {}  # (stream, query heads) -> workspace
+        _check(L.lib.mtt_b200_paged_cache_workspace_size(self._ref, kv_heads) > 0, "this cache is too large")
+
+    @staticmethod
+    def allocate(pages: int, slots: int, max_tokens: int, layers: int, kv_heads: int, head_dim: int,
+                 page_size: int = 16, dtype: torch.dtype = torch.bfloat16, device="cuda") -> "PagedCache":
+        """An empty cache: no slot has tokens, every page is free (the pool is not cleared)."""
+        _check(page_size in PAGE_SIZES, f"page_size must be one of {PAGE_SIZES}")
+        _check(max_tokens >= 1, "max_tokens must be at least 1")
+        table_pages = (max_tokens + page_size - 1) // page_size
+        i32 = dict(dtype=torch.int32, device=device)
+        return PagedCache(
+            pool=torch.empty(pages, layers, 2, kv_heads, page_size, head_dim, dtype=dtype, device=device),
+            page_table=torch.full((slots, table_pages), -1, **i32), lengths=torch.zeros(slots, **i32),
+            refs=torch.zeros(pages, **i32))
+
+    # -- plumbing -----------------------------------------------------------
+
+    def _stream(self, stream):
+        return torch.cuda.current_stream(self.device) if stream is None else stream
+
+    def _workspace(self, stream, q_heads: int) -> torch.Tensor:
+        """The workspace of calls on one stream: kept, as the streams' calls may overlap."""
+        key = (stream.cuda_stream, q_heads)
+        space = self._spaces.get(key)
+        if space is None:
+            size = L.lib.mtt_b200_paged_cache_workspace_size(self._ref, q_heads)
+            _check(size > 0, "q_heads must be a multiple of kv_heads, at most "
+                             f"{MAX_GROUP} query heads per key head")
+            with torch.cuda.stream(stream):
+                space = torch.zeros(size, dtype=torch.uint8, device=self.device)
+            self._spaces[key] = space
+        return space
+
+    def _vector(self, t: torch.Tensor, n: int, dtype: torch.dtype, name: str) -> int:
+        _check(t.dtype == dtype and t.dim() == 1 and t.shape[0] == n and t.is_contiguous(),
+               f"{name} must be a contiguous {dtype} vector of {n}")
+        _check(t.device == self.device, f"{name} is on another device than the pool")
+        return t.data_ptr()
+
+    @staticmethod
+    def _done(rc: int, what: str) -> None:
+        if rc != L.STATUS_OK:
+            raise RuntimeError(f"{what} failed with status {rc}")
+
+    # -- upkeep -------------------------------------------------------------
+
+    def extend(self, counts: torch.Tensor, stream=None) -> None:
+        """lengths += counts ([slots] int32), with the pages that takes."""
+        counts_ptr = self._vector(counts, self.slots, torch.int32, "counts")
+        stream = self._stream(stream)
+        ws = self._workspace(stream, self.kv_heads)
+        self._done(L.lib.mtt_b200_launch_paged_cache_extend(self._ref, counts_ptr, ws.data_ptr(), ws.numel(),
+                                                            stream.cuda_stream), "mtt_b200_launch_paged_cache_extend")
+
+    def fork(self, source: torch.Tensor, deep: bool = False, stream=None) -> None:
+        """Slot d takes over the tokens that slot source[d] had before the call
+        (source [slots] int32; -1 or d: slot d stays).  Full pages are shared
+        unless ``deep``, a partial last page is always copied."""
+        source_ptr = self._vector(source, self.slots, torch.int32, "source")
+        stream = self._stream(stream)
+        ws = self._workspace(stream, self.kv_heads)
+        self._done(L.lib.mtt_b200_launch_paged_cache_fork(self._ref, source_ptr, 1 if deep else 0, ws.data_ptr(),
+                                                          ws.numel(), stream.cuda_stream),
+                   "mtt_b200_launch_paged_cache_fork")
+
+    def free(self, mask: torch.Tensor, stream=None) -> None:
+        """Closes every slot with mask ([slots] bool): its pages are released."""
+        mask_ptr = self._vector(mask, self.slots, torch.bool, "mask")
+        self._done(L.lib.mtt_b200_launch_paged_cache_free(self._ref, mask_ptr, self._stream(stream).cuda_stream),
+                   "mtt_b200_launch_paged_cache_free")
+
+    def compact(self, stream=None) -> None:
+        """Moves the pages in use to [0, live); ``live`` [1] holds their number."""
+        stream = self._stream(stream)
+        ws = self._workspace(stream, self.kv_heads)
+        self._done(L.lib.mtt_b200_launch_paged_cache_compact(self._ref, ws.data_ptr(), ws.numel(),
+                                                             stream.cuda_stream), "mtt_b200_launch_paged_cache_compact")
+
+    def store(self, k: torch.Tensor, v: torch.Tensor, layer: Optional[int] = None,
+              offsets: Optional[torch.Tensor] = None, stream=None) -> None:
+        """Writes the keys and values of each slot's last tokens: rows
+        [offsets[i], offsets[i + 1]) are slot i's (offsets [slots + 1] int32), or,
+        without offsets, row i is slot i's last token.  With ``layer`` k and v are
+        [rows, kv_heads, head_dim]; without it [layers, rows, kv_heads, head_dim],
+        every layer at once.  The last two dimensions must be contiguous."""
+        _check(k.shape == v.shape and k.dim() == (3 if layer is not None else 4), "k and v must be [rows, kv_heads, "
+               "head_dim], or [layers, rows, kv_heads, head_dim] without a layer")
+        _check(tuple(k.shape[-2:]) == (self.kv_heads, self.head_dim), "k and v have other heads than the cache")
+        args = L.CacheRows()
+        if layer is None:
+            _check(k.shape[0] == self.layers, "k and v have other layers than the cache")
+            args.n_layers, args.k_layer_stride, args.v_layer_stride = self.layers, k.stride(0), v.stride(0)
+        else:
+            _check(0 <= layer < self.layers, "no such layer")
+            args.layer, args.n_layers = layer, 1
+        for t in (k, v):
+            _check(t.dtype == self.dtype and t.device == self.device, "k and v must have the pool's type and device")
+            _check(t.stride(-1) == 1 and t.stride(-2) == self.head_dim, "k and v must be contiguous in their heads")
+            _check(t.data_ptr() % 16 == 0 and t.stride(-3) % 8 == 0 and (layer is not None or t.stride(0) % 8 == 0),
+                   "rows of k and v must be 16-byte aligned")
+        args.rows = k.shape[-3]
+        args.k, args.v = k.data_ptr(), v.data_ptr()
+        args.k_row_stride, args.v_row_stride = k.stride(-3), v.stride(-3)
+        if offsets is not None:
+            args.offsets = self._vector(offsets, self.slots + 1, torch.int32, "offsets")
+        else:
+            _check(args.rows <= self.slots, "more rows than slots: offsets are needed")
+        self._done(L.lib.mtt_b200_launch_paged_cache_store(self._ref, ctypes.byref(args),
+                                                           self._stream(stream).cuda_stream),
+                   "mtt_b200_launch_paged_cache_store")
+
+    # -- attention ----------------------------------------------------------
+
+    def _attention(self, layer, q, out, window, sinks, scale, return_lse, stream):
+        """The fields that the attention calls share; (args, out, lse)."""
+        _check(q.dim() == 3 and q.shape[2] == self.head_dim, "q must be [rows, q_heads, head_dim]")
+        rows, q_heads, d = q.shape
+        _check(q_heads >= 1 and q_heads % self.kv_heads == 0 and q_heads // self.kv_heads <= MAX_GROUP,
+               f"q_heads must be a multiple of kv_heads, at most {MAX_GROUP} query heads per key head")
+        _check(0 <= layer < self.layers, "no such layer")
+        _check(window >= 0 and sinks >= 0, "window and sinks must not be negative")
+        if out is None:
+            with torch.cuda.stream(stream):
+                out = torch.empty(rows, q_heads, d, dtype=self.dtype, device=self.device)
+        else:
+            _check(out.shape == q.shape, "out must have q's shape")
+        for name, t in (("q", q), ("out", out)):
+            _check(t.dtype == self.dtype and t.device == self.device, f"{name} must have the pool's type and device")
+            _check(t.stride(2) == 1 and t.stride(1) == d, f"{name} must be contiguous in its heads")
+            _check(t.data_ptr() % 16 == 0 and t.stride(0) % 8 == 0, f"rows of {name} must be 16-byte aligned")
+        lse = None
+        args = L.CacheAttention()
+        if return_lse:
+            with torch.cuda.stream(stream):
+                lse = torch.empty(rows, q_heads, dtype=torch.float32, device=self.device)
+            args.lse = lse.data_ptr()
+        args.layer, args.q_heads, args.rows, args.window, args.sinks = layer, q_heads, rows, window, sinks
+        args.scale = d ** -0.5 if scale is None else scale
+        args.q, args.q_row_stride = q.data_ptr(), q.stride(0)
+        args.out, args.out_row_stride = out.data_ptr(), out.stride(0)
+        return args, out, lse
+
+    def attend(self, layer: int, q: torch.Tensor, out: Optional[torch.Tensor] = None, *,
+               offsets: Optional[torch.Tensor] = None, window: int = 0, sinks: int = 0,
+               scale: Optional[float] = None, key_mask: Optional[torch.Tensor] = None, return_lse: bool = False,
+               stream=None):
+        """Attention of q [rows, q_heads, head_dim] over one layer of the cache.
+
+        Without offsets row i is the last token of slot i (a decode step); with
+        offsets ([slots + 1] int32) rows [offsets[i], offsets[i + 1]) are slot i's
+        last tokens, whose keys and values are already stored (a prompt).  A
+        query sees the keys up to its own position, those less than ``window``
+        back (0: all) or among the first ``sinks``, and of these the ones with
+        key_mask ([slots, >= table_pages * page_size] bool).  A row that sees
+        none gets 0.  Returns out, or (out, lse) with the natural log of the sum
+        of exponentials ([rows, q_heads] f32, -inf for a row that sees none)."""
+        stream = self._stream(stream)
+        args, out, lse = self._attention(layer, q, out, window, sinks, scale, return_lse, stream)
+        if offsets is not None:
+            args.offsets = self._vector(offsets, self.slots + 1, torch.int32, "offsets")
+        else:
+            _check(args.rows <= self.slots, "more rows than slots: offsets are needed")
+        if key_mask is not None:
+            _check(key_mask.dtype == torch.bool and key_mask.dim() == 2 and key_mask.shape[0] == self.slots and
+                   key_mask.shape[1] >= self.table_pages * self.page_size and key_mask.stride(1) == 1 and
+                   key_mask.device == self.device and key_mask.stride(0) >= key_mask.shape[1],
+                   "key_mask must be a [slots, >= table_pages * page_size] bool tensor with contiguous rows")
+            args.key_mask, args.mask_stride = key_mask.data_ptr(), key_mask.stride(0)
+        ws = self._workspace(stream, args.q_heads)
+        self._done(L.lib.mtt_b200_launch_paged_attention(self._ref, ctypes.byref(args), ws.data_ptr(), ws.numel(),
+                                                         stream.cuda_stream), "mtt_b200_launch_paged_attention")
+        return (out, lse) if return_lse else out
