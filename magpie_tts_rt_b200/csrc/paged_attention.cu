@@ -1,34 +1,8 @@
 // Attention over the paged key/value cache (include/magpie_tts_rt_b200.h, group 7).
-#include "paged_cache.cuh"
+#include "paged_attention.cuh"
 
 namespace mtt {
 namespace {
-
-struct Attend {
-  int layer, q_heads, group, rows, window, sinks;
-  float scale;
-  const uint16_t* q;
-  int64_t q_row;
-  uint16_t* out;
-  int64_t out_row;
-  float* lse;
-  const int32_t* offsets;
-  const bool* key_mask;
-  int64_t mask_stride;
-};
-
-template <typename T>
-__device__ __forceinline__ float to_f(uint16_t b);
-template <>
-__device__ __forceinline__ float to_f<__nv_bfloat16>(uint16_t b) { return bits2f(b); }
-template <>
-__device__ __forceinline__ float to_f<__half>(uint16_t b) { return __half2float(__ushort_as_half(b)); }
-template <typename T>
-__device__ __forceinline__ uint16_t from_f(float v);
-template <>
-__device__ __forceinline__ uint16_t from_f<__nv_bfloat16>(float v) { return __bfloat16_as_ushort(__float2bfloat16_rn(v)); }
-template <>
-__device__ __forceinline__ uint16_t from_f<__half>(float v) { return __half_as_ushort(__float2half_rn(v)); }
 
 // One warp per (row, query head): keys one after the other, a running
 // maximum and sum, the head's dimensions over the lanes.
@@ -62,7 +36,7 @@ __global__ void __launch_bounds__(128) attend_rows_kernel(PagedCache c, Attend a
   float q[E], acc[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    q[e] = to_f<T>(a.q[row * a.q_row + static_cast<int64_t>(h) * D + lane * E + e]);
+    q[e] = Half16<T>::to_f(a.q[row * a.q_row + static_cast<int64_t>(h) * D + lane * E + e]);
     acc[e] = 0.f;
   }
   float m = -CUDART_INF_F, l = 0.f;
@@ -76,27 +50,27 @@ __global__ void __launch_bounds__(128) attend_rows_kernel(PagedCache c, Attend a
     const uint16_t* v = c.pool + c.block(page, a.layer, 1) + at;
     float s = 0.f;
 #pragma unroll
-    for (int e = 0; e < E; ++e) s = fmaf(q[e], to_f<T>(k[e]), s);
+    for (int e = 0; e < E; ++e) s = fmaf(q[e], Half16<T>::to_f(k[e]), s);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    s *= a.scale;
+    s *= a.scale2;
     const float mn = fmaxf(m, s);
-    const float keep = m == mn ? 1.f : __expf(m - mn), x = __expf(s - mn);
+    const float keep = m == mn ? 1.f : ex2(m - mn), x = ex2(s - mn);
     l = l * keep + x;
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = fmaf(x, to_f<T>(v[e]), acc[e] * keep);
+    for (int e = 0; e < E; ++e) acc[e] = fmaf(x, Half16<T>::to_f(v[e]), acc[e] * keep);
     m = mn;
   }
   const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
 #pragma unroll
   for (int e = 0; e < E; ++e)
-    a.out[row * a.out_row + static_cast<int64_t>(h) * D + lane * E + e] = from_f<T>(acc[e] * inv);
-  if (lane == 0 && a.lse != nullptr) a.lse[static_cast<int64_t>(row) * a.q_heads + h] = m + logf(l);
+    a.out[row * a.out_row + static_cast<int64_t>(h) * D + lane * E + e] = Half16<T>::one(acc[e] * inv);
+  if (lane == 0 && a.lse != nullptr) a.lse[static_cast<int64_t>(row) * a.q_heads + h] = (m + log2f(l)) * kLn2;
 }
 
 }  // namespace
 
-size_t paged_attention_workspace(const mtt_b200_paged_cache_t&, int) { return 256; }
+size_t paged_attention_workspace(const mtt_b200_paged_cache_t& c, int q_heads) { return step_workspace(c, q_heads); }
 
 }  // namespace mtt
 
@@ -107,6 +81,7 @@ extern "C" {
 int mtt_b200_launch_paged_attention(const mtt_b200_paged_cache_t* cache, const mtt_b200_cache_attention_t* args,
                                     void* workspace, size_t workspace_bytes, void* stream) {
   PagedCache c;
+  void* space = nullptr;
   if (args == nullptr || !paged_cache_view(cache, &c) || args->layer < 0 || args->layer >= c.layers ||
       args->q_heads < 1 || args->q_heads % c.kv_heads != 0 || args->q_heads / c.kv_heads > kCacheMaxGroup ||
       args->rows < 0 || args->window < 0 || args->sinks < 0)
@@ -116,11 +91,13 @@ int mtt_b200_launch_paged_attention(const mtt_b200_paged_cache_t* cache, const m
       args->q_row_stride % 8 != 0 || args->out_row_stride % 8 != 0 ||
       (args->offsets == nullptr && args->rows > c.slots) ||
       (args->key_mask != nullptr && args->mask_stride < static_cast<int64_t>(c.table_pages) * c.page_size) ||
-      paged_attention_space(*cache, args->q_heads, workspace, workspace_bytes) == nullptr)
+      (space = paged_attention_space(*cache, args->q_heads, workspace, workspace_bytes)) == nullptr)
     return MTT_B200_STATUS_INVALID_ARGUMENT;
-  Attend a{args->layer, args->q_heads, args->q_heads / c.kv_heads, args->rows, args->window, args->sinks, args->scale,
+  Attend a{args->layer, args->q_heads, args->q_heads / c.kv_heads, args->rows, args->window, args->sinks, args->scale * 1.4426950408889634f,
            static_cast<const uint16_t*>(args->q), args->q_row_stride, static_cast<uint16_t*>(args->out),
            args->out_row_stride, args->lse, args->offsets, args->key_mask, args->mask_stride};
+  if (a.offsets == nullptr)
+    return cache_call_status(launch_step(c, cache->dtype, a, space, static_cast<cudaStream_t>(stream)));
   const int64_t warps = static_cast<int64_t>(args->rows) * args->q_heads;
   auto* kernel = cache->dtype == MTT_B200_DTYPE_BF16
                      ? (c.head_dim == 64 ? attend_rows_kernel<__nv_bfloat16, 64> : attend_rows_kernel<__nv_bfloat16, 128>)

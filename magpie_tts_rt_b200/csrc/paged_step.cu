@@ -1,0 +1,406 @@
+// Attention of one new token per slot over the paged cache.
+//
+//   out = sum_j e^{s q.k_j} v_j / sum_j e^{s q.k_j} over the keys the window,
+//   the sinks and the mask leave: one pass with a running maximum and sum.
+//
+// Every key and value is used for one query row of each query head that
+// shares the key head, so HBM bounds it: 4 x head_dim bytes per key and key
+// head.  The design keeps those bytes in flight and everything else cheap:
+//  * Keys and values go from global memory straight into the registers that
+//    mma.sync reads, 16 bytes a load, with no shared memory between.  A
+//    warp's step is 16 keys (32 with head_dim 64).  Scores are S^T = K Q^T
+//    with the keys on the MMA's 16-row side and up to 8 query heads on its
+//    8-column side (a step of one query head costs no more).  The
+//    contraction's order is free, so a thread's A fragment is simply its 16
+//    bytes of the key row; two matrix transposes turn P^T into the B operand
+//    of O^T += V^T P^T, and V^T's fragments are byte permutes of two keys'
+//    16-byte pieces.  (tcgen05 would want the same bytes staged in shared
+//    memory for a tile of 128 rows of which 1 to 16 are real.)
+//  * The work is one line of 16-key tiles over all (slot, key head) units,
+//    cut into equal parts for a grid that fills the device, so ragged
+//    lengths balance by themselves.  A unit cut by a CTA boundary leaves
+//    (maximum, sum, weighted values) in the workspace; the CTA that arrives
+//    last joins them in the order of the CTAs, so the result does not depend
+//    on timing.
+#include "paged_attention.cuh"
+
+namespace mtt {
+namespace {
+
+constexpr int kStepWarps = 4;
+constexpr int kStepThreads = 32 * kStepWarps;
+
+template <int D>
+struct StepCfg {
+  static constexpr int kTiles = D == 64 ? 2 : 1;  // 16-key tiles per warp and step
+  static constexpr int kCtas = D == 64 ? 4 : 3;   // per SM (registers)
+};
+
+struct StepSpace {
+  int32_t* arrived;  // [slots * units]: CTAs that have left their part of a unit; 0 between calls
+  float* part;       // [CTAs][2][queries][D + 2]
+};
+
+// Not the read-only path: the launch before this one may have written the
+// cache, and this kernel may already have been scheduled by then.
+__device__ __forceinline__ uint4 load16(const uint16_t* p, bool on) {
+  uint4 v = make_uint4(0, 0, 0, 0);
+  if (on)
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "l"(p));
+  return v;
+}
+
+template <typename T, int D, int NB>
+__global__ void __launch_bounds__(kStepThreads, StepCfg<D>::kCtas)
+    step_kernel(PagedCache c, Attend a, StepSpace ws, int blocks, int min_tiles) {
+  constexpr int NT = StepCfg<D>::kTiles;
+  constexpr int NQ = 8 * NB;   // query rows of a unit
+  constexpr int KC = D / 32;   // 16-byte pieces of a key row per thread
+  constexpr int VC = D / 64;   // of a value row
+  extern __shared__ int tiles_before[];  // [rows + 1]: tiles of a key head of the slots before
+  __shared__ float s_m[kStepWarps][NQ], s_l[kStepWarps][NQ];
+  __shared__ float s_acc[kStepWarps][NQ][D];
+  __shared__ int s_last;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int t = lane & 3, g = lane >> 2;
+  wait_prior_grid();
+
+  // tiles of every slot, scanned
+  {
+    int run = 0;
+    for (int base = 0; base < a.rows; base += kStepThreads) {
+      const int i = base + tid;
+      const int n = i < a.rows ? SeenTiles(c.length(i), a.window, a.sinks, 0).n : 0;
+      int inc = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += x;
+      }
+      __shared__ int warp_sum[kStepWarps];
+      if (lane == 31) warp_sum[warp] = inc;
+      __syncthreads();
+      int before = run;
+#pragma unroll
+      for (int w = 0; w < kStepWarps; ++w) {
+        if (w < warp) before += warp_sum[w];
+        run += warp_sum[w];
+      }
+      if (i < a.rows) tiles_before[i] = before + inc - n;
+      __syncthreads();
+    }
+    if (tid == 0) tiles_before[a.rows] = run;
+    __syncthreads();
+  }
+  const int units = c.kv_heads * blocks;
+  const int64_t total = static_cast<int64_t>(tiles_before[a.rows]) * units;
+  const int64_t per = max((total + gridDim.x - 1) / gridDim.x, static_cast<int64_t>(min_tiles));
+
+  // slots without a key in reach
+  for (int i = blockIdx.x; i < a.rows; i += gridDim.x) {
+    if (tiles_before[i + 1] != tiles_before[i]) continue;
+    for (int e = tid; e < a.q_heads * D / 8; e += kStepThreads)
+      *reinterpret_cast<uint4*>(a.out + i * a.out_row + 8 * e) = make_uint4(0, 0, 0, 0);
+    if (a.lse != nullptr)
+      for (int h = tid; h < a.q_heads; h += kStepThreads) a.lse[static_cast<int64_t>(i) * a.q_heads + h] = -CUDART_INF_F;
+  }
+
+  int64_t x = static_cast<int64_t>(blockIdx.x) * per;
+  const int64_t x_end = min(total, x + per);
+  if (x >= x_end) return;
+  const int64_t x_first = x;
+  int slot;
+  {
+    int lo = 0, hi = a.rows;  // the last slot whose tiles begin at or before x
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (static_cast<int64_t>(tiles_before[mid]) * units <= x) lo = mid; else hi = mid;
+    }
+    slot = lo;
+  }
+  while (x < x_end) {
+    while (static_cast<int64_t>(tiles_before[slot + 1]) * units <= x) ++slot;
+    const SeenTiles seen(c.length(slot), a.window, a.sinks, 0);
+    const int64_t slot_x = static_cast<int64_t>(tiles_before[slot]) * units;
+    const int unit = static_cast<int>((x - slot_x) / seen.n);
+    const int64_t unit_x = slot_x + static_cast<int64_t>(unit) * seen.n;
+    const int t0 = static_cast<int>(x - unit_x);
+    const int t1 = static_cast<int>(min(static_cast<int64_t>(seen.n), x_end - unit_x));
+    const int head = unit / blocks, block = unit % blocks;
+    const int queries = min(NQ, a.group - block * NQ);
+    const int q_head = head * a.group + block * NQ;
+    const int32_t* row = c.table + static_cast<int64_t>(slot) * c.table_pages;
+    const bool* mask = a.key_mask != nullptr ? a.key_mask + slot * a.mask_stride : nullptr;
+    const int64_t head_at = static_cast<int64_t>(head) * c.page_size * D;
+
+    uint4 q[NB][KC];
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int k = 0; k < KC; ++k)
+        q[b][k] = load16(a.q + slot * a.q_row + static_cast<int64_t>(q_head + 8 * b + g) * D + 8 * (t + 4 * k),
+                         8 * b + g < queries);
+    float m[NB][2], l[NB][2], acc[NB][VC][4][4];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      m[b][0] = m[b][1] = -CUDART_INF_F;
+      l[b][0] = l[b][1] = 0.f;
+#pragma unroll
+      for (int v = 0; v < VC; ++v)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) acc[b][v][w][0] = acc[b][v][w][1] = acc[b][v][w][2] = acc[b][v][w][3] = 0.f;
+    }
+
+    int page[NT];
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+      const int tt = t0 + warp * NT + u;
+      page[u] = tt < t1 ? row[(16 * seen.tile(tt)) >> c.page_shift] : -1;
+    }
+    for (int base = t0 + warp * NT; base < t1; base += kStepWarps * NT) {
+      // keys in reach: one per lane
+      const int my_tile = base + (lane >> 4);
+      bool in = my_tile < t1 && (lane >> 4) < NT;
+      {
+        const int j = 16 * seen.tile(my_tile) + (lane & 15);
+        in = in && j < seen.len && (j >= seen.low || j < a.sinks);
+        if (in && mask != nullptr) in = mask[j];
+      }
+      const uint32_t bits = __ballot_sync(0xffffffffu, in);
+      uint4 kr[NT][2][KC], vr[NT][4][VC];
+      uint32_t on[NT];
+#pragma unroll
+      for (int u = 0; u < NT; ++u) {
+        on[u] = c.is_page(page[u]) ? (bits >> (16 * u)) & 0xffffu : 0u;
+        const int in_page = (16 * seen.tile(base + u)) & (c.page_size - 1);
+        const uint16_t* kp = c.pool + c.block(page[u], a.layer, 0) + head_at + static_cast<int64_t>(in_page) * D;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int k = 0; k < KC; ++k)
+            kr[u][h][k] = load16(kp + (g + 8 * h) * D + 8 * (t + 4 * k), (on[u] >> (g + 8 * h)) & 1u);
+        const uint16_t* vp = kp + c.kv_elems;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int key = 2 * t + (i & 1) + 8 * (i >> 1);
+#pragma unroll
+          for (int v = 0; v < VC; ++v) vr[u][i][v] = load16(vp + key * D + 8 * (g + 8 * v), (on[u] >> key) & 1u);
+        }
+      }
+      // the next step's pages, while this step's keys arrive
+#pragma unroll
+      for (int u = 0; u < NT; ++u) {
+        const int tt = base + kStepWarps * NT + u;
+        page[u] = tt < t1 ? row[(16 * seen.tile(tt)) >> c.page_shift] : -1;
+      }
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        float s[NT][4];
+        float top0 = m[b][0], top1 = m[b][1];
+#pragma unroll
+        for (int u = 0; u < NT; ++u) {
+          s[u][0] = s[u][1] = s[u][2] = s[u][3] = 0.f;
+#pragma unroll
+          for (int k = 0; k < KC; ++k) {
+            Half16<T>::mma(s[u], kr[u][0][k].x, kr[u][1][k].x, kr[u][0][k].y, kr[u][1][k].y, q[b][k].x, q[b][k].y);
+            Half16<T>::mma(s[u], kr[u][0][k].z, kr[u][1][k].z, kr[u][0][k].w, kr[u][1][k].w, q[b][k].z, q[b][k].w);
+          }
+          const bool lo = (on[u] >> g) & 1u, hi = (on[u] >> (g + 8)) & 1u;
+          s[u][0] = lo ? s[u][0] * a.scale2 : -CUDART_INF_F;
+          s[u][1] = lo ? s[u][1] * a.scale2 : -CUDART_INF_F;
+          s[u][2] = hi ? s[u][2] * a.scale2 : -CUDART_INF_F;
+          s[u][3] = hi ? s[u][3] * a.scale2 : -CUDART_INF_F;
+          top0 = fmaxf(top0, fmaxf(s[u][0], s[u][2]));
+          top1 = fmaxf(top1, fmaxf(s[u][1], s[u][3]));
+        }
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) {
+          top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, o));
+          top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, o));
+        }
+        const float z0 = top0 == -CUDART_INF_F ? 0.f : top0, z1 = top1 == -CUDART_INF_F ? 0.f : top1;
+        const float keep0 = ex2(m[b][0] - z0), keep1 = ex2(m[b][1] - z1);
+        m[b][0] = top0;
+        m[b][1] = top1;
+        l[b][0] *= keep0;
+        l[b][1] *= keep1;
+#pragma unroll
+        for (int v = 0; v < VC; ++v)
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            acc[b][v][w][0] *= keep0;
+            acc[b][v][w][1] *= keep1;
+            acc[b][v][w][2] *= keep0;
+            acc[b][v][w][3] *= keep1;
+          }
+#pragma unroll
+        for (int u = 0; u < NT; ++u) {
+          const float p0 = ex2(s[u][0] - z0), p1 = ex2(s[u][1] - z1), p2 = ex2(s[u][2] - z0), p3 = ex2(s[u][3] - z1);
+          // the sum keeps the unrounded probabilities; the values' weights are rounded to 16 bits once
+          l[b][0] += p0 + p2;
+          l[b][1] += p1 + p3;
+          const uint32_t b0 = transpose8x8(Half16<T>::pack(p0, p1)), b1 = transpose8x8(Half16<T>::pack(p2, p3));
+#pragma unroll
+          for (int v = 0; v < VC; ++v) {
+            const uint4 &x0 = vr[u][0][v], &x1 = vr[u][1][v], &x2 = vr[u][2][v], &x3 = vr[u][3][v];
+            Half16<T>::mma(acc[b][v][0], __byte_perm(x0.x, x1.x, 0x5410), __byte_perm(x0.x, x1.x, 0x7632),
+                           __byte_perm(x2.x, x3.x, 0x5410), __byte_perm(x2.x, x3.x, 0x7632), b0, b1);
+            Half16<T>::mma(acc[b][v][1], __byte_perm(x0.y, x1.y, 0x5410), __byte_perm(x0.y, x1.y, 0x7632),
+                           __byte_perm(x2.y, x3.y, 0x5410), __byte_perm(x2.y, x3.y, 0x7632), b0, b1);
+            Half16<T>::mma(acc[b][v][2], __byte_perm(x0.z, x1.z, 0x5410), __byte_perm(x0.z, x1.z, 0x7632),
+                           __byte_perm(x2.z, x3.z, 0x5410), __byte_perm(x2.z, x3.z, 0x7632), b0, b1);
+            Half16<T>::mma(acc[b][v][3], __byte_perm(x0.w, x1.w, 0x5410), __byte_perm(x0.w, x1.w, 0x7632),
+                           __byte_perm(x2.w, x3.w, 0x5410), __byte_perm(x2.w, x3.w, 0x7632), b0, b1);
+          }
+        }
+      }
+    }
+
+    // the four warps' parts
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) {
+        l[b][0] += __shfl_xor_sync(0xffffffffu, l[b][0], o);
+        l[b][1] += __shfl_xor_sync(0xffffffffu, l[b][1], o);
+      }
+      const int q0 = 8 * b + 2 * t;
+      if (g == 0) {
+        s_m[warp][q0] = m[b][0];
+        s_m[warp][q0 + 1] = m[b][1];
+        s_l[warp][q0] = l[b][0];
+        s_l[warp][q0 + 1] = l[b][1];
+      }
+#pragma unroll
+      for (int v = 0; v < VC; ++v)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const int d = 64 * v + 8 * g + 2 * w;
+          if (q0 < queries)
+            *reinterpret_cast<float2*>(&s_acc[warp][q0][d]) = make_float2(acc[b][v][w][0], acc[b][v][w][2]);
+          if (q0 + 1 < queries)
+            *reinterpret_cast<float2*>(&s_acc[warp][q0 + 1][d]) = make_float2(acc[b][v][w][1], acc[b][v][w][3]);
+        }
+    }
+    __syncthreads();
+    const bool whole = t0 == 0 && t1 == seen.n;
+    const int64_t part_size = static_cast<int64_t>(NQ) * (D + 2);
+    float* part = ws.part + (2 * static_cast<int64_t>(blockIdx.x) + (x == x_first ? 0 : 1)) * part_size;
+    for (int e = tid; e < queries * (D / 2); e += kStepThreads) {
+      const int qi = e / (D / 2), d = 2 * (e % (D / 2));
+      float top = s_m[0][qi];
+#pragma unroll
+      for (int w = 1; w < kStepWarps; ++w) top = fmaxf(top, s_m[w][qi]);
+      const float z = top == -CUDART_INF_F ? 0.f : top;
+      float sum = 0.f, o0 = 0.f, o1 = 0.f;
+#pragma unroll
+      for (int w = 0; w < kStepWarps; ++w) {
+        const float f = ex2(s_m[w][qi] - z);
+        const float2 y = *reinterpret_cast<const float2*>(&s_acc[w][qi][d]);
+        sum = fmaf(f, s_l[w][qi], sum);
+        o0 = fmaf(f, y.x, o0);
+        o1 = fmaf(f, y.y, o1);
+      }
+      if (whole) {
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        *reinterpret_cast<uint32_t*>(a.out + slot * a.out_row + static_cast<int64_t>(q_head + qi) * D + d) =
+            Half16<T>::pack(o0 * inv, o1 * inv);
+        if (d == 0 && a.lse != nullptr)
+          a.lse[static_cast<int64_t>(slot) * a.q_heads + q_head + qi] = (top + log2f(sum)) * kLn2;
+      } else {
+        *reinterpret_cast<float2*>(part + qi * (D + 2) + d) = make_float2(o0, o1);
+        if (d == 0) *reinterpret_cast<float2*>(part + qi * (D + 2) + D) = make_float2(top, sum);
+      }
+    }
+    if (!whole) {
+      const int first_cta = static_cast<int>(unit_x / per);
+      const int last_cta = static_cast<int>((unit_x + seen.n - 1) / per);
+      int32_t* arrived = ws.arrived + static_cast<int64_t>(slot) * units + unit;
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) s_last = atomicAdd(arrived, 1) == last_cta - first_cta;
+      __syncthreads();
+      if (s_last) {
+        __threadfence();
+        if (tid == 0) *arrived = 0;  // for the next call
+        for (int e = tid; e < queries * (D / 2); e += kStepThreads) {
+          const int qi = e / (D / 2), d = 2 * (e % (D / 2));
+          // the first CTA's part is its last one unless its share begins here
+          auto at = [&](int k) {
+            return ws.part + (2 * static_cast<int64_t>(k) + (k * per < unit_x ? 1 : 0)) * part_size + qi * (D + 2);
+          };
+          float top = -CUDART_INF_F;
+          for (int k = first_cta; k <= last_cta; ++k) top = fmaxf(top, __ldcg(at(k) + D));
+          const float z = top == -CUDART_INF_F ? 0.f : top;
+          float sum = 0.f, o0 = 0.f, o1 = 0.f;
+          for (int k = first_cta; k <= last_cta; ++k) {
+            const float* p = at(k);
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(p + D));
+            const float2 y = __ldcg(reinterpret_cast<const float2*>(p + d));
+            const float f = ex2(ml.x - z);
+            sum = fmaf(f, ml.y, sum);
+            o0 = fmaf(f, y.x, o0);
+            o1 = fmaf(f, y.y, o1);
+          }
+          const float inv = sum == 0.f ? 0.f : 1.f / sum;
+          *reinterpret_cast<uint32_t*>(a.out + slot * a.out_row + static_cast<int64_t>(q_head + qi) * D + d) =
+              Half16<T>::pack(o0 * inv, o1 * inv);
+          if (d == 0 && a.lse != nullptr)
+            a.lse[static_cast<int64_t>(slot) * a.q_heads + q_head + qi] = (top + log2f(sum)) * kLn2;
+        }
+      }
+    }
+    __syncthreads();  // s_* are free for the next unit
+    x = unit_x + t1;
+  }
+}
+
+int step_grid(int head_dim, int sms) { return sms * (head_dim == 64 ? StepCfg<64>::kCtas : StepCfg<128>::kCtas); }
+
+// 8-query blocks of a unit, and units per key head
+void step_blocks(int group, int* nb, int* blocks) {
+  *nb = group <= 8 ? 1 : 2;
+  *blocks = (group + 8 * *nb - 1) / (8 * *nb);
+}
+
+}  // namespace
+
+size_t step_workspace(const mtt_b200_paged_cache_t& c, int q_heads) {
+  int nb, blocks;
+  step_blocks(q_heads / c.kv_heads, &nb, &blocks);
+  const size_t arrived = (static_cast<size_t>(c.slots) * c.kv_heads * blocks * 4 + 255) / 256 * 256;
+  // sized for the largest device this library runs on, so that it does not depend on the current one
+  return arrived + static_cast<size_t>(step_grid(c.head_dim, 160)) * 2 * 8 * nb * (c.head_dim + 2) * 4;
+}
+
+cudaError_t launch_step(const PagedCache& c, int dtype, const Attend& a, void* space, cudaStream_t stream) {
+  int nb, blocks;
+  step_blocks(a.group, &nb, &blocks);
+  StepSpace ws;
+  ws.arrived = static_cast<int32_t*>(space);
+  ws.part = reinterpret_cast<float*>(static_cast<char*>(space) +
+                                     (static_cast<size_t>(c.slots) * c.kv_heads * blocks * 4 + 255) / 256 * 256);
+  const int sms = cache_sm_count();
+  if (sms <= 0 || sms > 160) return cudaErrorInvalidValue;
+  const size_t smem = 4 * (static_cast<size_t>(a.rows) + 1);
+  const int min_tiles = kStepWarps * (c.head_dim == 64 ? StepCfg<64>::kTiles : StepCfg<128>::kTiles);
+  auto go = [&](auto kernel) {
+    if (smem > 14 * 1024) {
+      const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                 4 * (kCacheMaxSlots + 1));
+      if (e != cudaSuccess) return e;
+    }
+    return launch_serialized(kernel, dim3(step_grid(c.head_dim, sms)), dim3(kStepThreads), smem, stream, c, a, ws,
+                             blocks, min_tiles);
+  };
+  auto pick = [&](auto type) {
+    using T = decltype(type);
+    if (c.head_dim == 64) return nb == 1 ? go(step_kernel<T, 64, 1>) : go(step_kernel<T, 64, 2>);
+    return nb == 1 ? go(step_kernel<T, 128, 1>) : go(step_kernel<T, 128, 2>);
+  };
+  return dtype == MTT_B200_DTYPE_BF16 ? pick(__nv_bfloat16{}) : pick(__half{});
+}
+
+}  // namespace mtt
