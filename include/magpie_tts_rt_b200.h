@@ -752,7 +752,7 @@ typedef struct mtt_b200_paged_cache {
   int32_t head_dim;    /* 64 or 128 */
   int32_t dtype;       /* MTT_B200_DTYPE_* of the pool, of keys, values, queries and outputs */
   int32_t slots;       /* <= 16384 */
-  int32_t table_pages; /* page_table columns; table_pages * page_size < 2^31 */
+  int32_t table_pages; /* page_table columns; table_pages * page_size < 2^30 */
   void* pool;          /* 128-byte aligned */
   int32_t* page_table; /* [slots][table_pages], -1 past a slot's pages */
   int32_t* lengths;    /* [slots] tokens */
@@ -761,10 +761,11 @@ typedef struct mtt_b200_paged_cache {
   int32_t* live;       /* [1] or NULL: pages in use, written by compact */
 } mtt_b200_paged_cache_t;
 
-/* Workspace bytes for any call on this cache with queries of q_heads heads (0
- * for bad arguments).  256-byte aligned, zeroed once before its first use; one
+/* Workspace bytes for any call on this cache with up to `rows` query rows of
+ * q_heads heads (0 for bad arguments).  256-byte aligned, zeroed once before its first use; one
  * workspace serves one stream at a time. */
-MTT_B200_API size_t mtt_b200_paged_cache_workspace_size(const mtt_b200_paged_cache_t* cache, int32_t q_heads);
+MTT_B200_API size_t mtt_b200_paged_cache_workspace_size(const mtt_b200_paged_cache_t* cache, int32_t q_heads,
+                                                        int32_t rows);
 
 /* lengths[i] += counts[i] (counts [slots] int32, >= 0), with the new pages
  * that takes.  A slot's new pages are granted while the pages asked for by it
@@ -819,21 +820,24 @@ MTT_B200_API int mtt_b200_launch_paged_cache_store(const mtt_b200_paged_cache_t*
  * sinks) and key_mask[slot][j] (where given):
  *   out = sum_j exp(scale q.k_j) v_j / sum_j exp(scale q.k_j)
  *   lse = log sum_j exp(scale q.k_j)          (natural log, f32)
- * with f32 sums; a row that sees no key gets out 0 and lse -inf.  Keys that
+ * with f32 sums and probabilities rounded once to the cache's type; a row that sees no key gets out 0 and lse -inf.  Keys that
  * no query may see (past the length, or masked) do not reach the result,
  * whatever their bytes.  Query head h reads key head h / (q_heads / kv_heads).
  *
  * offsets NULL: row i is the last token of slot i (rows <= slots).  With
  * offsets ([slots + 1] int32, as for store) slot i's rows are its last
  * offsets[i + 1] - offsets[i] tokens, whose keys and values are already
- * stored; the rows of a slot whose offsets do not fit get out 0 and lse -inf. */
+ * stored; a slot with more rows than tokens gets out 0 and lse -inf, offsets
+ * that are not ascending within [0, rows] leave their rows untouched.
+ * status[i] becomes 4 when a bounded wait inside the prompt kernel gave up
+ * (outputs unreliable). */
 typedef struct mtt_b200_cache_attention {
   int32_t layer;
   int32_t q_heads;          /* a multiple of kv_heads, q_heads / kv_heads <= 64 */
-  int32_t rows;
+  int32_t rows;             /* <= 2^22 */
   int32_t window;           /* 0: no window */
   int32_t sinks;            /* >= 0; no effect without a window */
-  float scale;
+  float scale;              /* > 0 */
   const void* q;            /* [rows][q_heads][head_dim], 16-byte aligned */
   int64_t q_row_stride;     /* elements, a multiple of 8 */
   void* out;                /* [rows][q_heads][head_dim], 16-byte aligned */

@@ -224,7 +224,7 @@ SIGNATURES = {
     "mtt_b200_main_decoder_workspace_size": (SZ, [I32, I32]),
     "mtt_b200_launch_main_decoder_step": (
         I32, [ctypes.POINTER(MainDecoderWeights), ctypes.POINTER(MainDecoderBatch), P, SZ, P]),
-    "mtt_b200_paged_cache_workspace_size": (SZ, [ctypes.POINTER(PagedCache), I32]),
+    "mtt_b200_paged_cache_workspace_size": (SZ, [ctypes.POINTER(PagedCache), I32, I32]),
     "mtt_b200_launch_paged_cache_extend": (I32, [ctypes.POINTER(PagedCache), P, P, SZ, P]),
     "mtt_b200_launch_paged_cache_fork": (I32, [ctypes.POINTER(PagedCache), P, I32, P, SZ, P]),
     "mtt_b200_launch_paged_cache_free": (I32, [ctypes.POINTER(PagedCache), P, P]),

@@ -92,4 +92,8 @@ struct SeenTiles {
 size_t step_workspace(const mtt_b200_paged_cache_t& c, int q_heads);
 cudaError_t launch_step(const PagedCache& c, int dtype, const Attend& a, void* space, cudaStream_t stream);
 
+// Workspace of the prompt attention for calls of up to `rows` query rows.
+size_t prompt_workspace(const mtt_b200_paged_cache_t& c, int q_heads, int rows);
+cudaError_t launch_prompt(const PagedCache& c, int dtype, const Attend& a, void* space, cudaStream_t stream);
+
 }  // namespace mtt

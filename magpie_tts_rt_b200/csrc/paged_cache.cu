@@ -405,7 +405,7 @@ bool paged_cache_view(const mtt_b200_paged_cache_t* c, PagedCache* out) {
     return false;
   // rows of the pool (one token's keys or values of one head) and tokens of a slot are counted in 31 bits
   const double rows = static_cast<double>(c->pages) * c->layers * 2 * c->kv_heads * c->page_size;
-  if (rows >= 2147483648.0 || static_cast<int64_t>(c->table_pages) * c->page_size >= (int64_t{1} << 31) ||
+  if (rows >= 2147483648.0 || static_cast<int64_t>(c->table_pages) * c->page_size >= (int64_t{1} << 30) ||
       static_cast<double>(c->slots) * c->table_pages * (c->page_size / 16) >= 2147483648.0)
     return false;
   if (c->pool == nullptr || c->page_table == nullptr || c->lengths == nullptr || c->refs == nullptr ||
@@ -448,22 +448,22 @@ bool upkeep_checked(const mtt_b200_paged_cache_t* cache, void* ws, size_t bytes,
 
 }  // namespace
 
-void* mtt::paged_attention_space(const mtt_b200_paged_cache_t& c, int q_heads, void* workspace, size_t bytes) {
+void* mtt::paged_attention_space(const mtt_b200_paged_cache_t& c, int q_heads, int rows, void* workspace, size_t bytes) {
   const size_t up = upkeep_bytes(c);
   if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0 ||
-      bytes < up + paged_attention_workspace(c, q_heads))
+      bytes < up + paged_attention_workspace(c, q_heads, rows))
     return nullptr;
   return static_cast<char*>(workspace) + up;
 }
 
 extern "C" {
 
-size_t mtt_b200_paged_cache_workspace_size(const mtt_b200_paged_cache_t* cache, int32_t q_heads) {
+size_t mtt_b200_paged_cache_workspace_size(const mtt_b200_paged_cache_t* cache, int32_t q_heads, int32_t rows) {
   PagedCache c;
   if (!paged_cache_view(cache, &c) || q_heads < 1 || q_heads % c.kv_heads != 0 ||
-      q_heads / c.kv_heads > kCacheMaxGroup)
+      q_heads / c.kv_heads > kCacheMaxGroup || rows < 0 || rows > kCacheMaxRows)
     return 0;
-  return upkeep_bytes(*cache) + paged_attention_workspace(*cache, q_heads);
+  return upkeep_bytes(*cache) + paged_attention_workspace(*cache, q_heads, rows);
 }
 
 int mtt_b200_launch_paged_cache_extend(const mtt_b200_paged_cache_t* cache, const int32_t* counts, void* workspace,

@@ -11,6 +11,7 @@ namespace mtt {
 
 constexpr int kCacheMaxSlots = 16384;
 constexpr int kCacheMaxGroup = 64;  // query heads per key head
+constexpr int kCacheMaxRows = 1 << 22;  // query rows of a call
 
 struct PagedCache {
   int pages, layers, kv_heads, page_size, page_shift, head_dim, slots, table_pages;
@@ -40,10 +41,10 @@ struct PagedCache {
 bool paged_cache_view(const mtt_b200_paged_cache_t* c, PagedCache* out);
 
 // Workspace bytes of the attention calls (they follow the upkeep's words).
-size_t paged_attention_workspace(const mtt_b200_paged_cache_t& c, int q_heads);
+size_t paged_attention_workspace(const mtt_b200_paged_cache_t& c, int q_heads, int rows);
 
 // Start of the attention's part of a workspace; null when the workspace is too small.
-void* paged_attention_space(const mtt_b200_paged_cache_t& c, int q_heads, void* workspace, size_t bytes);
+void* paged_attention_space(const mtt_b200_paged_cache_t& c, int q_heads, int rows, void* workspace, size_t bytes);
 
 // SMs of the current device (0: cannot be queried).
 int cache_sm_count();

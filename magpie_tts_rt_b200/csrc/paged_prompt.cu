@@ -1,0 +1,869 @@
+// Attention of runs of query rows over the paged cache on the tensor cores:
+// the prompt form (slot i's rows are its newest tokens, causal, with window,
+// sinks and key mask) and the prefix pass of groups of slots that share a
+// prefix (every member's newest token over the voice's pages).
+//
+//   S = Q K^T,  P = e^{scale S - m},  l += P 1,  O += P V     per 128-key tile
+//
+// with a running maximum m per row and O rescaled only when m grew by more
+// than a factor 2^8 (the f32 sums have room for it, and P in 16 bits keeps
+// its relative precision), so that rescaling is rare.
+//
+// A unit is a key head and two Q tiles of 128 rows; a tile's rows are the
+// group's query heads of consecutive tokens (128 / group of them), so shared
+// key heads fill the MMA's 128 rows and every key tile in shared memory is
+// used by both Q tiles.  Warp roles (320 threads, one CTA per SM):
+//   warps 0-3, 4-7  softmax of Q tile 0 / 1: one thread per row reads S from
+//                   tensor memory, writes P over it in 16 bits (the A operand
+//                   of the second product), rescales O when needed, and
+//                   stores the result;
+//   warp 8          issues the MMAs: S0, S1, then P0 V, next S0, P1 V, next
+//                   S1, ... so that one tile's products run under the other
+//                   tile's softmax; also clears value rows that no query may
+//                   see (page tails, masked keys: 0 times their bytes must be 0);
+//   warp 9          TMA: the pages of each 128-key tile, keys then values, into
+//                   a ring of stages (128-byte swizzle).
+// Tensor memory: S0, S1 (128 columns each), O0, O1 (head_dim each).
+//
+// The units' key tiles form one line that is cut into equal parts, one per
+// CTA; a unit cut by a boundary leaves (m, l, O) in the workspace for a
+// second kernel that joins the parts in order.  Every wait is bounded; one
+// that gives up marks the slot's status 4.
+#include "gemm_tc.cuh"
+#include "paged_attention.cuh"
+
+namespace mtt {
+namespace {
+
+constexpr int kTile = 128;          // rows of a Q tile, keys of a key tile
+constexpr int kPairRows = 2 * kTile;
+constexpr int kPromptThreads = 320;
+constexpr int kPromptPlanThreads = 1024;
+constexpr int kMinShare = 2;        // key tiles a CTA takes at least
+constexpr int kMaxSms = 160;        // workspaces are sized for the largest device
+
+template <int D>
+struct PromptCfg {
+  static constexpr int kStages = D == 64 ? 8 : 4;
+  static constexpr uint32_t kTileBytes = kTile * D * 2;
+  static constexpr size_t kSmem = 1024 + static_cast<size_t>(2 + kStages) * kTileBytes;
+};
+
+// Rows of the attention: tokens of slots, or members of prefix groups.
+struct PromptRows {
+  int n;                     // slots, or groups
+  int n_rows;                // rows in all (tokens, or members)
+  const int32_t* offsets;    // [n + 1]
+  const int32_t* members;    // prefix pass: slot of each member; null for prompts
+  const int32_t* voice;      // prefix pass: [n] slot that holds the prefix
+  const int32_t* tokens;     // prefix pass: [n] its length
+  float* state;              // prefix pass: [slots][q_heads][D + 2]: O, m, l of each member
+};
+
+// One pair of Q tiles: slot (or group), first token (or member), key tiles, key tiles of the pairs before.
+struct PromptSpace {
+  int64_t* head;       // [0] pairs, [1] key tiles of one key head, [2] key tiles per CTA
+  int32_t* cta_pair;   // [kMaxSms + 1] the pair that holds CTA c's first tile
+  int32_t* first;      // [n + 1] pairs of the slots before
+  int4* rec;           // [pairs]
+  float* part;         // [CTAs][2][D + 2][256]
+};
+
+// Where a pair's rows and keys are.
+struct PairGeom {
+  int count, len, row0, key_slot;
+  bool ok;
+  __device__ __forceinline__ PairGeom(const PagedCache& c, const PromptRows& r, int i) {
+    const int a = r.offsets[i], b = r.offsets[i + 1];
+    ok = a >= 0 && a <= b && b <= r.n_rows;
+    row0 = ok ? a : 0;
+    count = ok ? b - a : 0;
+    if (r.members != nullptr) {
+      key_slot = r.voice[i];
+      len = r.tokens[i];
+      ok = ok && key_slot >= 0 && key_slot < c.slots && len >= 0 && (len & (c.page_size - 1)) == 0;
+      ok = ok && c.length(ok ? key_slot : 0) >= len;
+    } else {
+      key_slot = i;
+      len = c.length(i);
+      ok = ok && count <= len;
+    }
+    if (!ok) {
+      len = 0;
+      key_slot = 0;
+    }
+  }
+};
+
+// The 128-key tiles that queries at positions [p0, p1] may see.
+struct KeySpan {
+  int sink_n, win0, n;
+  __device__ __forceinline__ KeySpan(int p0, int p1, int window, int sinks) {
+    const int low = window > 0 ? max(0, p0 - window + 1) : 0;
+    const int end = p1 / kTile + 1;
+    sink_n = low > 0 && sinks > 0 ? min((min(sinks - 1, p1)) / kTile + 1, end) : 0;
+    win0 = max(low / kTile, sink_n);
+    n = sink_n + max(0, end - win0);
+  }
+  __device__ __forceinline__ int tile(int t) const { return t < sink_n ? t : win0 + t - sink_n; }
+};
+
+// Whether any query at positions [p0, p1] sees a key of tile j.
+__device__ __forceinline__ bool tile_seen(int j, int p0, int p1, int window, int sinks) {
+  return p0 <= p1 && kTile * j <= p1 && (window == 0 || kTile * j + kTile - 1 > p0 - window || kTile * j < sinks);
+}
+// Whether every one of them sees every key of it.
+__device__ __forceinline__ bool tile_full(int j, int p0, int p1, int window, int sinks) {
+  return kTile * j + kTile - 1 <= p0 && (window == 0 || kTile * j > p1 - window || kTile * (j + 1) <= sinks);
+}
+
+// Positions [p0, p1] of the rows of tokens [t0, t1); empty when p1 < p0.  In
+// the prefix pass every row stands at the prefix's end.
+__device__ __forceinline__ void positions(const PairGeom& g, bool prefix, int t0, int t1, int* p0, int* p1) {
+  t1 = min(t1, g.count);
+  if (prefix) {
+    *p1 = g.len - 1;
+    *p0 = t0 < t1 && g.len > 0 ? g.len - 1 : g.len;
+  } else {
+    *p0 = g.len - g.count + t0;
+    *p1 = g.ok ? g.len - g.count + t1 - 1 : *p0 - 1;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// plan: one CTA lists the pairs and cuts the line of key tiles
+// ---------------------------------------------------------------------------
+
+__device__ __forceinline__ int plan_scan(int v, int* total) {
+  __shared__ int warp_sum[kPromptPlanThreads / 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int inc = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int n = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += n;
+  }
+  if (lane == 31) warp_sum[warp] = inc;
+  __syncthreads();
+  if (warp == 0) {
+    int s = warp_sum[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int n = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += n;
+    }
+    warp_sum[lane] = s;
+  }
+  __syncthreads();
+  const int before = (warp > 0 ? warp_sum[warp - 1] : 0) + inc - v;
+  *total = warp_sum[kPromptPlanThreads / 32 - 1];
+  __syncthreads();
+  return before;
+}
+
+__global__ void __launch_bounds__(kPromptPlanThreads)
+    prompt_plan_kernel(PagedCache c, PromptRows rows, PromptSpace ws, int window, int sinks, int tokens_per_pair,
+                       int ctas) {
+  wait_prior_grid();
+  const int tid = threadIdx.x;
+  const bool prefix = rows.members != nullptr;
+  // slots whose offsets overlap could ask for more pairs than there is room for
+  const int most = rows.n_rows / tokens_per_pair + rows.n;
+  int pairs = 0;
+  for (int base = 0; base < rows.n; base += kPromptPlanThreads) {
+    const int i = base + tid;
+    int n = 0;
+    if (i < rows.n) n = (PairGeom(c, rows, i).count + tokens_per_pair - 1) / tokens_per_pair;
+    int total;
+    const int before = pairs + plan_scan(n, &total);
+    if (i < rows.n) ws.first[i] = min(before, most);
+    pairs = min(pairs + total, most);
+  }
+  if (tid == 0) ws.first[rows.n] = pairs;
+  __syncthreads();
+  int tiles = 0;
+  for (int base = 0; base < pairs; base += kPromptPlanThreads) {
+    const int k = base + tid;
+    int n = 0, i = 0, tok0 = 0;
+    if (k < pairs) {
+      int lo = 0, hi = rows.n;  // the last slot whose pairs begin at or before k
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (ws.first[mid] <= k) lo = mid; else hi = mid;
+      }
+      i = lo;
+      tok0 = (k - ws.first[i]) * tokens_per_pair;
+      const PairGeom g(c, rows, i);
+      int p0, p1;
+      positions(g, prefix, tok0, tok0 + tokens_per_pair, &p0, &p1);
+      // rows that see nothing still need their zeros written: one tile without keys
+      n = p0 <= p1 ? KeySpan(p0, p1, window, sinks).n : (prefix ? 0 : 1);
+    }
+    int total;
+    const int before = tiles + plan_scan(n, &total);
+    if (k < pairs) ws.rec[k] = make_int4(i, tok0, n, before);
+    tiles += total;
+  }
+  __syncthreads();
+  const int64_t all = static_cast<int64_t>(tiles) * c.kv_heads;
+  const int64_t per = max((all + ctas - 1) / ctas, static_cast<int64_t>(kMinShare));
+  if (tid == 0) {
+    ws.head[0] = pairs;
+    ws.head[1] = tiles;
+    ws.head[2] = per;
+  }
+  if (tid < ctas && tid * per < all) {
+    const int x = static_cast<int>(tid * per % tiles);
+    int lo = 0, hi = pairs;  // the last pair that begins at or before x (pairs without tiles are never last)
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (ws.rec[mid].w <= x) lo = mid; else hi = mid;
+    }
+    ws.cta_pair[tid] = lo;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// a CTA's share, unit by unit
+// ---------------------------------------------------------------------------
+
+struct Walk {
+  int64_t x, end, per;
+  int tiles, pairs, head, pair;
+  int4 rec;
+  int t0, t1;       // key tiles of the unit in this share
+  int64_t unit_x;   // where the unit begins on the line
+  bool first;       // the share's first unit
+
+  __device__ __forceinline__ bool begin(const PromptSpace& ws, int kv_heads, int cta) {
+    pairs = static_cast<int>(ws.head[0]);
+    tiles = static_cast<int>(ws.head[1]);
+    per = ws.head[2];
+    const int64_t all = static_cast<int64_t>(tiles) * kv_heads;
+    x = cta * per;
+    end = min(all, x + per);
+    if (x >= end) return false;
+    head = static_cast<int>(x / tiles);
+    pair = ws.cta_pair[cta];
+    first = true;
+    load(ws);
+    return true;
+  }
+  __device__ __forceinline__ bool next(const PromptSpace& ws) {
+    x = unit_x + t1;
+    if (x >= end) return false;
+    first = false;
+    ++pair;
+    load(ws);
+    return true;
+  }
+  __device__ __forceinline__ void load(const PromptSpace& ws) {
+    while (true) {
+      if (pair >= pairs) {
+        pair = 0;
+        ++head;
+      }
+      rec = ws.rec[pair];
+      if (rec.z > 0) break;
+      ++pair;
+    }
+    unit_x = static_cast<int64_t>(head) * tiles + rec.w;
+    t0 = static_cast<int>(x - unit_x);
+    t1 = static_cast<int>(min(static_cast<int64_t>(rec.z), end - unit_x));
+  }
+  __device__ __forceinline__ bool whole() const { return t0 == 0 && t1 == rec.z; }
+};
+
+// 128-byte-swizzled MN-major operand (values: [keys][64 dims] rows of 128
+// bytes): 8-key groups 1024 bytes apart, the next 64 dims one 128-key block on.
+__device__ __forceinline__ uint64_t value_desc(uint32_t a) {
+  uint64_t d = static_cast<uint64_t>((a & 0x3FFFFu) >> 4);
+  d |= static_cast<uint64_t>((kTile * 128) >> 4) << 16;  // leading byte offset: 64 dims on
+  d |= static_cast<uint64_t>(1024 >> 4) << 32;           // stride byte offset: 8 keys on
+  d |= static_cast<uint64_t>(1) << 46;
+  d |= static_cast<uint64_t>(2) << 61;
+  return d;
+}
+
+template <typename T>
+__host__ __device__ constexpr uint32_t prompt_idesc(int n, bool b_mn_major);
+template <>
+__host__ __device__ constexpr uint32_t prompt_idesc<__nv_bfloat16>(int n, bool b_mn_major) {
+  return umma_idesc_bf16(kTile, n) | (b_mn_major ? 1u << 16 : 0u);
+}
+template <>
+__host__ __device__ constexpr uint32_t prompt_idesc<__half>(int n, bool b_mn_major) {
+  return (umma_idesc_bf16(kTile, n) & ~((1u << 7) | (1u << 10))) | (b_mn_major ? 1u << 16 : 0u);
+}
+
+// D[tmem] (+)= A[tmem] x B[smem desc], issued by one thread.
+__device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                        bool accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate ? 1u : 0u)
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
+      "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
+      "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      : "memory");
+}
+
+// Warp-uniform forms: a wait succeeds, and the CTA goes on, for all lanes or none.
+__device__ __forceinline__ bool wait_warp(unsigned long long* bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, mbar_wait_cta(bar, parity));
+}
+__device__ __forceinline__ bool alive(const volatile int* err) { return __all_sync(0xffffffffu, *err == 0); }
+
+// bits [lo, hi) of a 32-bit word
+__device__ __forceinline__ uint32_t bit_range(int lo, int hi) {
+  lo = max(lo, 0);
+  hi = min(hi, 32);
+  if (lo >= hi) return 0u;
+  const uint32_t up = hi == 32 ? 0xffffffffu : (1u << hi) - 1u;
+  return up & ~((1u << lo) - 1u);
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kPromptThreads, 1)
+    prompt_kernel(const __grid_constant__ CUtensorMap pool_map, PagedCache c, Attend a, PromptRows rows,
+                  PromptSpace ws) {
+  using C = PromptCfg<D>;
+  constexpr int S = C::kStages;
+  constexpr int DB = D / 64;  // 64-dim blocks of a tile
+  constexpr uint32_t kSCol = 0, kOCol = 2 * kTile;
+  extern __shared__ unsigned char prompt_smem[];
+  __shared__ unsigned long long kv_full[S], kv_empty[S], q_ready[2], s_full[2], p_full[2], o_full[2], fin;
+  __shared__ uint32_t tmem_base;
+  __shared__ int err;
+  const uint32_t pad = (1024u - (smem_addr(prompt_smem) & 1023u)) & 1023u;
+  unsigned char* q_smem = prompt_smem + pad;
+  unsigned char* ring = q_smem + 2 * C::kTileBytes;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const bool prefix = rows.members != nullptr;
+  const int tq = kTile / a.group;  // tokens of a Q tile
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&kv_full[s], 1);
+      mbar_init(&kv_empty[s], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_ready[i], 4);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&o_full[i], 1);
+    }
+    mbar_init(&fin, 1);
+    err = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 8) {
+    tmem_alloc(&tmem_base, 512);
+    tmem_relinquish();
+  }
+  if (warp == 9 && lane == 0)
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&pool_map)) : "memory");
+  tmem_fence_before_sync();
+  __syncthreads();
+  tmem_fence_after_sync();
+  const uint32_t tmem = tmem_base;
+  volatile int* errv = &err;
+  wait_prior_grid();
+
+  Walk w;
+  const bool any = w.begin(ws, c.kv_heads, blockIdx.x);
+
+  if (warp == 9) {
+    // ---- TMA producer: per key tile its keys, then its values
+    int it = 0;
+    const int boxes = kTile >> c.page_shift;  // pages per tile
+    const int beyond = c.pages * c.layers * 2 * c.kv_heads * c.page_size;  // a row past the pool: reads zeros
+    for (bool more = any; more && alive(errv); more = w.next(ws)) {
+      const PairGeom g(c, rows, w.rec.x);
+      int p0, p1;
+      positions(g, prefix, w.rec.y, w.rec.y + 2 * tq, &p0, &p1);
+      const KeySpan span(p0, max(p0, p1), a.window, a.sinks);
+      const int32_t* table = c.table + static_cast<int64_t>(g.key_slot) * c.table_pages;
+      for (int t = w.t0; t < w.t1; ++t) {
+        const int first_key = kTile * span.tile(t) + (lane << c.page_shift);
+        int page = -1;
+        if (lane < boxes && first_key < g.len) page = table[first_key >> c.page_shift];
+        for (int kv = 0; kv < 2; ++kv, ++it) {
+          const int s = it % S;
+          if (it >= S && !wait_warp(&kv_empty[s], ((it / S) - 1) & 1)) *errv = 1;
+          if (!alive(errv)) break;
+          if (lane == 0) mbar_expect_tx(&kv_full[s], C::kTileBytes);
+          __syncwarp();
+          if (lane < boxes) {
+            const int y = c.is_page(page)
+                              ? (((page * c.layers + a.layer) * 2 + kv) * c.kv_heads + w.head) * c.page_size
+                              : beyond;
+            unsigned char* dst = ring + static_cast<size_t>(s) * C::kTileBytes + (lane << (c.page_shift + 7));
+#pragma unroll
+            for (int b = 0; b < DB; ++b) tma_load_2d(dst + b * (kTile * 128), &pool_map, 64 * b, y, &kv_full[s]);
+          }
+        }
+        if (!alive(errv)) break;
+      }
+    }
+    // no copy may still be landing in shared memory when the CTA leaves
+    if (lane == 0)
+      for (int k = max(0, it - S); k < it; ++k) mbar_wait_cta(&kv_full[k % S], (k / S) & 1);
+  } else if (warp == 8) {
+    // ---- MMA issuer
+    int it = 0;                 // ring position of the next key tile
+    int p_uses[2] = {0, 0}, q_uses = 0;
+    const uint32_t idesc_s = prompt_idesc<T>(kTile, false), idesc_o = prompt_idesc<T>(D, true);
+    for (bool more = any; more && alive(errv); more = w.next(ws), ++q_uses) {
+      const PairGeom g(c, rows, w.rec.x);
+      int p0, p1, q0[2], q1[2];
+      positions(g, prefix, w.rec.y, w.rec.y + 2 * tq, &p0, &p1);
+      positions(g, prefix, w.rec.y, w.rec.y + tq, &q0[0], &q1[0]);
+      positions(g, prefix, w.rec.y + tq, w.rec.y + 2 * tq, &q0[1], &q1[1]);
+      const KeySpan span(p0, max(p0, p1), a.window, a.sinks);
+      const bool* mask = a.key_mask != nullptr ? a.key_mask + g.key_slot * a.mask_stride : nullptr;
+      bool ok = true, started[2] = {false, false};
+      int last[2] = {-1, -1};  // each Q tile's last key tile in this share
+      for (int i = 0; i < 2; ++i)
+        for (int t = w.t1 - 1; t >= w.t0 && last[i] < 0; --t)
+          if (tile_seen(span.tile(t), q0[i], q1[i], a.window, a.sinks)) last[i] = t;
+      auto scores = [&](int i, int s) {  // S_i = Q_i K^T
+        const unsigned char* q = q_smem + i * C::kTileBytes;
+        const unsigned char* k = ring + static_cast<size_t>(s) * C::kTileBytes;
+#pragma unroll
+        for (int b = 0; b < DB; ++b) {
+          const uint64_t qd = umma_desc_sw128(q + b * (kTile * 128)), kd = umma_desc_sw128(k + b * (kTile * 128));
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            umma_bf16(tmem + kSCol + i * kTile, qd + 2 * kk, kd + 2 * kk, idesc_s, (b | kk) != 0);
+        }
+        umma_commit(&s_full[i]);
+      };
+      auto key_tile = [&](int t, bool first) {  // wait for tile t's keys; the first also needs the queries
+        if (!wait_warp(&kv_full[it % S], (it / S) & 1)) return false;
+        if (first)
+          for (int i = 0; i < 2; ++i)
+            if (!wait_warp(&q_ready[i], q_uses & 1)) return false;
+        tmem_fence_after_sync();
+        return true;
+      };
+      ok = key_tile(w.t0, true);
+      if (ok && lane == 0) {
+        for (int i = 0; i < 2; ++i)
+          if (tile_seen(span.tile(w.t0), q0[i], q1[i], a.window, a.sinks)) scores(i, it % S);
+        // a Q tile without key tiles here waits too: its warps must not run ahead of this one
+        for (int i = 0; i < 2; ++i)
+          if (last[i] < 0) umma_commit(&o_full[i]);
+        umma_commit(&kv_empty[it % S]);
+      }
+      ++it;
+      for (int t = w.t0; ok && t < w.t1; ++t) {
+        const int vs = it % S;
+        ok = wait_warp(&kv_full[vs], (it / S) & 1);
+        if (!ok) break;
+        ++it;
+        const int base = kTile * span.tile(t);
+        // value rows that no query may see are cleared
+        if (mask != nullptr || (base + kTile > g.len && (g.len & (c.page_size - 1)) != 0)) {
+          unsigned char* v = ring + static_cast<size_t>(vs) * C::kTileBytes;
+          for (int r = lane; r < kTile; r += 32) {
+            const bool keep = base + r < g.len && (mask == nullptr || mask[base + r]);
+            if (!keep) {
+#pragma unroll
+              for (int b = 0; b < DB; ++b)
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                  *reinterpret_cast<uint4*>(v + b * (kTile * 128) + r * 128 + 16 * k) = make_uint4(0, 0, 0, 0);
+            }
+          }
+          fence_proxy_async();
+          __syncwarp();
+        }
+        const bool next = t + 1 < w.t1;
+        int ks = 0;
+        if (next) {
+          ks = it % S;
+          ok = key_tile(t + 1, false);
+          if (!ok) break;
+          ++it;
+        }
+        for (int i = 0; i < 2 && ok; ++i) {
+          if (tile_seen(span.tile(t), q0[i], q1[i], a.window, a.sinks)) {
+            ok = wait_warp(&p_full[i], p_uses[i] & 1);
+            ++p_uses[i];
+            if (!ok) break;
+            tmem_fence_after_sync();
+            if (lane == 0) {
+              const uint64_t vd = value_desc(smem_addr(ring + static_cast<size_t>(vs) * C::kTileBytes));
+#pragma unroll
+              for (int kk = 0; kk < kTile / 16; ++kk)
+                umma_ts(tmem + kOCol + i * D, tmem + kSCol + i * kTile + 8 * kk, vd + kk * (2048 >> 4), idesc_o,
+                        started[i] || kk != 0);
+            }
+            started[i] = true;
+            if (t == last[i] && lane == 0) umma_commit(&o_full[i]);
+          }
+          if (next && lane == 0 && tile_seen(span.tile(t + 1), q0[i], q1[i], a.window, a.sinks)) scores(i, ks);
+        }
+        if (ok && lane == 0) {
+          umma_commit(&kv_empty[vs]);
+          if (next) umma_commit(&kv_empty[ks]);
+        }
+      }
+      if (!ok) {
+        *errv = 1;
+        break;
+      }
+    }
+    // every MMA this thread issued has completed before tensor memory is freed
+    if (lane == 0) {
+      umma_commit(&fin);
+      mbar_wait_cta(&fin, 0);
+    }
+  } else {
+    // ---- softmax of Q tile i: thread r is its row r
+    const int i = warp >> 2, r = threadIdx.x & 127;
+    const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
+    const uint32_t s_col = tmem + kSCol + i * kTile + lanes, o_col = tmem + kOCol + i * D + lanes;
+    const int tok_in_tile = r / a.group, head_in_group = r % a.group;
+    int s_uses = 0, o_uses = 0;
+    for (bool more = any; more && alive(errv); more = w.next(ws)) {
+      const PairGeom g(c, rows, w.rec.x);
+      const int tok = w.rec.y + i * tq + tok_in_tile;
+      const bool valid = tok_in_tile < tq && tok < g.count;
+      int q_row = valid ? g.row0 + tok : 0;
+      if (prefix && valid) q_row = rows.members[q_row];
+      const bool there = valid && (!prefix || (q_row >= 0 && q_row < a.rows));
+      const int q_head = w.head * a.group + head_in_group;
+      {
+        const uint16_t* src = a.q + q_row * a.q_row + static_cast<int64_t>(q_head) * D;
+        unsigned char* dst = q_smem + i * C::kTileBytes + r * 128;
+#pragma unroll
+        for (int b = 0; b < DB; ++b) {
+          uint4 v[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            v[k] = there ? *reinterpret_cast<const uint4*>(src + 64 * b + 8 * k) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) *reinterpret_cast<uint4*>(dst + b * (kTile * 128) + 16 * (k ^ (r & 7))) = v[k];
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&q_ready[i]);
+      }
+      int p0, p1, q0, q1;
+      positions(g, prefix, w.rec.y, w.rec.y + 2 * tq, &p0, &p1);
+      positions(g, prefix, w.rec.y + i * tq, w.rec.y + (i + 1) * tq, &q0, &q1);
+      const KeySpan span(p0, max(p0, p1), a.window, a.sinks);
+      const int pos = prefix ? g.len - 1 : g.len - g.count + tok;
+      const bool* mask = a.key_mask != nullptr ? a.key_mask + g.key_slot * a.mask_stride : nullptr;
+      float m = -CUDART_INF_F, l = 0.f;
+      bool ok = true, started = false;
+      for (int t = w.t0; t < w.t1 && ok; ++t) {
+        const int j = span.tile(t);
+        if (!tile_seen(j, q0, q1, a.window, a.sinks)) continue;
+        const int base = kTile * j;
+        uint32_t see[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+        const bool all = mask == nullptr && tile_full(j, q0, q1, a.window, a.sinks) && base + kTile <= g.len;
+        if (!all) {
+          const int hi = min(pos + 1, g.len) - base;
+          const int lo = a.window > 0 ? max(max(pos + 1 - base, 0) - a.window, 0) : 0;
+          const int sk = min(a.sinks, kTile * (j + 1)) - base;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            see[x] = bit_range(0, hi - 32 * x) & (bit_range(lo - 32 * x, 32) | bit_range(0, sk - 32 * x));
+            if (mask != nullptr) {
+              const int k = base + 32 * x + lane;
+              see[x] &= __ballot_sync(0xffffffffu, k < g.len && mask[k]);
+            }
+          }
+        }
+        ok = wait_warp(&s_full[i], s_uses & 1);
+        ++s_uses;
+        if (!ok) break;
+        tmem_fence_after_sync();
+        uint32_t s[2][64];
+        tmem_ld64(s[0], s_col);
+        tmem_ld64(s[1], s_col + 64);
+        if (!all) {
+#pragma unroll
+          for (int k = 0; k < 128; ++k)
+            if (!((see[k >> 5] >> (k & 31)) & 1u)) s[k >> 6][k & 63] = 0xff800000u;
+        }
+        float top = m;
+#pragma unroll
+        for (int k = 0; k < 128; ++k) top = fmaxf(top, __uint_as_float(s[k >> 6][k & 63]));
+        // the maximum in use moves only when it must
+        const bool move = m == -CUDART_INF_F ? top > m : (top - m) * a.scale2 > 8.f;
+        if (__any_sync(0xffffffffu, move)) {
+          if (started && __any_sync(0xffffffffu, move && m != -CUDART_INF_F)) {
+            const float f = move && m != -CUDART_INF_F ? ex2((m - top) * a.scale2) : 1.f;
+            l *= f;
+#pragma unroll
+            for (int b = 0; b < D / 32; ++b) {
+              uint32_t o[32];
+              tmem_ld32(o, o_col + 32 * b);
+#pragma unroll
+              for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+              tmem_st32(o_col + 32 * b, o);
+            }
+          }
+          if (move) m = top;
+        }
+        const float off = m == -CUDART_INF_F ? 0.f : -m * a.scale2;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          uint32_t p[32];
+          float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+          for (int k = 0; k < 32; ++k) {
+            const float e0 = ex2(fmaf(__uint_as_float(s[x][2 * k]), a.scale2, off));
+            const float e1 = ex2(fmaf(__uint_as_float(s[x][2 * k + 1]), a.scale2, off));
+            // the sum keeps the unrounded probabilities; the values' weights are rounded to 16 bits once
+            s0 += e0;
+            s1 += e1;
+            p[k] = Half16<T>::pack(e0, e1);
+          }
+          l += s0 + s1;
+          tmem_st32(s_col + 32 * x, p);
+        }
+        tmem_wait_st();
+        tmem_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[i]);
+        started = true;
+      }
+      if (ok) {
+        ok = wait_warp(&o_full[i], o_uses & 1);
+        ++o_uses;
+        tmem_fence_after_sync();
+      }
+      if (!ok) {
+        *errv = 1;
+        break;
+      }
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const float m2 = m == -CUDART_INF_F ? m : m * a.scale2;
+      const bool whole = w.whole();
+      float* part = ws.part + (2 * static_cast<int64_t>(blockIdx.x) + (w.first ? 0 : 1)) * (D + 2) * kPairRows + i * kTile + r;
+      float* state = prefix && there ? rows.state + (static_cast<int64_t>(q_row) * a.q_heads + q_head) * (D + 2) : nullptr;
+      uint16_t* out = a.out + q_row * a.out_row + static_cast<int64_t>(q_head) * D;
+#pragma unroll
+      for (int b = 0; b < D / 32; ++b) {
+        uint32_t o[32];
+        tmem_ld32(o, o_col + 32 * b);
+        if (!started) {
+#pragma unroll
+          for (int k = 0; k < 32; ++k) o[k] = 0u;
+        }
+        if (!there) {
+        } else if (!whole) {
+#pragma unroll
+          for (int k = 0; k < 32; ++k) part[(32 * b + k) * kPairRows] = __uint_as_float(o[k]);
+        } else if (prefix) {
+#pragma unroll
+          for (int k = 0; k < 16; ++k)
+            *reinterpret_cast<uint2*>(state + 32 * b + 2 * k) = make_uint2(o[2 * k], o[2 * k + 1]);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            uint4 v;
+            v.x = Half16<T>::pack(__uint_as_float(o[8 * k]) * inv, __uint_as_float(o[8 * k + 1]) * inv);
+            v.y = Half16<T>::pack(__uint_as_float(o[8 * k + 2]) * inv, __uint_as_float(o[8 * k + 3]) * inv);
+            v.z = Half16<T>::pack(__uint_as_float(o[8 * k + 4]) * inv, __uint_as_float(o[8 * k + 5]) * inv);
+            v.w = Half16<T>::pack(__uint_as_float(o[8 * k + 6]) * inv, __uint_as_float(o[8 * k + 7]) * inv);
+            *reinterpret_cast<uint4*>(out + 32 * b + 8 * k) = v;
+          }
+        }
+        __syncwarp();
+      }
+      if (there) {
+        if (!whole) {
+          part[D * kPairRows] = m2;
+          part[(D + 1) * kPairRows] = l;
+        } else if (prefix) {
+          *reinterpret_cast<float2*>(state + D) = make_float2(m2, l);
+        } else if (a.lse != nullptr) {
+          a.lse[static_cast<int64_t>(q_row) * a.q_heads + q_head] = (m2 + log2f(l)) * kLn2;
+        }
+      }
+    }
+  }
+  tmem_fence_before_sync();
+  __syncthreads();
+  if (warp == 8) {
+    tmem_fence_after_sync();
+    tmem_dealloc(tmem, 512);
+  }
+  if (threadIdx.x == 0 && *errv != 0 && any && c.status != nullptr) {
+    const PairGeom g(c, rows, w.rec.x);
+    c.status[g.key_slot] = 4;
+  }
+}
+
+// Joins the parts of the units that a boundary between CTAs cut.  Block
+// (c - 1, chunk): the unit at the start of CTA c's share, if that is the first
+// boundary inside it; 32 of its rows.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) prompt_join_kernel(PagedCache c, Attend a, PromptRows rows, PromptSpace ws) {
+  wait_prior_grid();
+  const int cta = blockIdx.x + 1;
+  const int64_t tiles = ws.head[1], per = ws.head[2];
+  const int64_t x = cta * per;
+  if (x >= tiles * c.kv_heads) return;
+  const int head = static_cast<int>(x / tiles);
+  const int4 rec = ws.rec[ws.cta_pair[cta]];
+  const int64_t unit_x = head * tiles + rec.w;
+  if (unit_x == x || x - unit_x > per) return;  // not cut here, or cut before
+  const int last = static_cast<int>((unit_x + rec.z - 1) / per);
+  const PairGeom g(c, rows, rec.x);
+  const bool prefix = rows.members != nullptr;
+  const int tq = kTile / a.group;
+  const int r = 32 * blockIdx.y + (threadIdx.x & 31);
+  const int i = r / kTile, rr = r % kTile;
+  const int tok = rec.y + i * tq + rr / a.group;
+  if (rr / a.group >= tq || tok >= g.count) return;
+  int q_row = g.row0 + tok;
+  if (prefix) {
+    q_row = rows.members[q_row];
+    if (q_row < 0 || q_row >= a.rows) return;
+  }
+  const int q_head = head * a.group + rr % a.group;
+  constexpr int E = D / 8;  // dims per thread
+  const int d0 = E * (threadIdx.x >> 5);
+  auto part = [&](int k) {  // CTA cta - 1 holds the unit's beginning: its last unit unless its share begins there
+    const int64_t at = 2 * static_cast<int64_t>(k) + (k * per < unit_x ? 1 : 0);
+    return ws.part + at * (D + 2) * kPairRows + r;
+  };
+  float top = -CUDART_INF_F;
+  for (int k = cta - 1; k <= last; ++k) top = fmaxf(top, part(k)[D * kPairRows]);
+  const float z = top == -CUDART_INF_F ? 0.f : top;
+  float l = 0.f, o[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) o[e] = 0.f;
+  for (int k = cta - 1; k <= last; ++k) {
+    const float* p = part(k);
+    const float f = ex2(p[D * kPairRows] - z);
+    l = fmaf(f, p[(D + 1) * kPairRows], l);
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = fmaf(f, p[(d0 + e) * kPairRows], o[e]);
+  }
+  if (prefix) {
+    float* state = rows.state + (static_cast<int64_t>(q_row) * a.q_heads + q_head) * (D + 2);
+#pragma unroll
+    for (int e = 0; e < E; ++e) state[d0 + e] = o[e];
+    if (d0 == 0) *reinterpret_cast<float2*>(state + D) = make_float2(top, l);
+    return;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  uint16_t* out = a.out + q_row * a.out_row + static_cast<int64_t>(q_head) * D + d0;
+#pragma unroll
+  for (int e = 0; e < E; e += 8) {
+    uint4 v;
+    v.x = Half16<T>::pack(o[e] * inv, o[e + 1] * inv);
+    v.y = Half16<T>::pack(o[e + 2] * inv, o[e + 3] * inv);
+    v.z = Half16<T>::pack(o[e + 4] * inv, o[e + 5] * inv);
+    v.w = Half16<T>::pack(o[e + 6] * inv, o[e + 7] * inv);
+    *reinterpret_cast<uint4*>(out + e) = v;
+  }
+  if (d0 == 0 && a.lse != nullptr) a.lse[static_cast<int64_t>(q_row) * a.q_heads + q_head] = (top + log2f(l)) * kLn2;
+}
+
+// Bytes of the parts of a prompt call's workspace.
+struct PromptLayout {
+  size_t cta_pair, first, rec, part, bytes;
+  PromptLayout(int n, int rows, int group, int head_dim) {
+    const auto up = [](size_t v) { return (v + 255) / 256 * 256; };
+    const size_t pairs = static_cast<size_t>(rows) / (2 * (kTile / group)) + n + 1;
+    cta_pair = 256;
+    first = cta_pair + up(4 * (kMaxSms + 1));
+    rec = first + up(4 * (static_cast<size_t>(n) + 1));
+    part = rec + up(16 * pairs);
+    bytes = part + up(static_cast<size_t>(kMaxSms) * 2 * (head_dim + 2) * kPairRows * 4);
+  }
+};
+
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn find_encode() {
+  void* p = nullptr;
+  cudaDriverEntryPointQueryResult q{};
+  const bool ok = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+                  q == cudaDriverEntryPointSuccess;
+  cudaGetLastError();
+  return ok ? reinterpret_cast<EncodeTiledFn>(p) : nullptr;
+}
+
+// The pool as a matrix of rows (one token's keys or values of one head); a
+// box is one page's rows of one head, 64 dims wide.
+bool pool_map(const PagedCache& c, int dtype, CUtensorMap* map) {
+  static const EncodeTiledFn fn = find_encode();
+  if (fn == nullptr) return false;
+  const cuuint64_t rows = static_cast<cuuint64_t>(c.pages) * c.layers * 2 * c.kv_heads * c.page_size;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(c.head_dim), rows};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(c.head_dim) * 2};
+  const cuuint32_t box[2] = {64, static_cast<cuuint32_t>(c.page_size)};
+  const cuuint32_t elem[2] = {1, 1};
+  return fn(map,
+            dtype == MTT_B200_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+            c.pool, dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+cudaError_t run_prompt(const PagedCache& c, int dtype, const Attend& a, const PromptRows& rows, void* space,
+                       cudaStream_t stream) {
+  const int sms = cache_sm_count();
+  CUtensorMap map;
+  if (sms <= 0 || sms > kMaxSms || !pool_map(c, dtype, &map)) return cudaErrorInvalidValue;
+  const PromptLayout at(rows.n, rows.n_rows, a.group, c.head_dim);
+  char* base = static_cast<char*>(space);
+  PromptSpace ws;
+  ws.head = reinterpret_cast<int64_t*>(base);
+  ws.cta_pair = reinterpret_cast<int32_t*>(base + at.cta_pair);
+  ws.first = reinterpret_cast<int32_t*>(base + at.first);
+  ws.rec = reinterpret_cast<int4*>(base + at.rec);
+  ws.part = reinterpret_cast<float*>(base + at.part);
+  auto go = [&](auto kernel, auto join, size_t smem) {
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (e == cudaSuccess)
+      e = launch_serialized(prompt_plan_kernel, dim3(1), dim3(kPromptPlanThreads), 0, stream, c, rows, ws, a.window,
+                            a.sinks, 2 * (kTile / a.group), sms);
+    if (e == cudaSuccess) e = launch_serialized(kernel, dim3(sms), dim3(kPromptThreads), smem, stream, map, c, a, rows, ws);
+    if (e == cudaSuccess)
+      e = launch_serialized(join, dim3(sms - 1, kPairRows / 32), dim3(256), 0, stream, c, a, rows, ws);
+    return e;
+  };
+  auto pick = [&](auto type) {
+    using T = decltype(type);
+    return c.head_dim == 64 ? go(prompt_kernel<T, 64>, prompt_join_kernel<T, 64>, PromptCfg<64>::kSmem)
+                            : go(prompt_kernel<T, 128>, prompt_join_kernel<T, 128>, PromptCfg<128>::kSmem);
+  };
+  return dtype == MTT_B200_DTYPE_BF16 ? pick(__nv_bfloat16{}) : pick(__half{});
+}
+
+}  // namespace
+
+size_t prompt_workspace(const mtt_b200_paged_cache_t& c, int q_heads, int rows) {
+  return PromptLayout(c.slots, rows, q_heads / c.kv_heads, c.head_dim).bytes;
+}
+
+cudaError_t launch_prompt(const PagedCache& c, int dtype, const Attend& a, void* space, cudaStream_t stream) {
+  PromptRows rows{};
+  rows.n = c.slots;
+  rows.n_rows = a.rows;
+  rows.offsets = a.offsets;
+  return run_prompt(c, dtype, a, rows, space, stream);
+}
+
+}  // namespace mtt

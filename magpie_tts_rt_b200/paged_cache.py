@@ -23,6 +23,7 @@ each other by the caller when they use different streams.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from typing import Optional
 
@@ -34,6 +35,7 @@ PAGE_SIZES = (16, 32, 64, 128)
 HEAD_DIMS = (64, 128)
 MAX_SLOTS = 16384
 MAX_GROUP = 64
+MAX_ROWS = 1 << 22
 _DTYPES = {torch.bfloat16: L.DTYPE_BF16, torch.float16: L.DTYPE_F16}
 
 
@@ -82,7 +84,7 @@ class PagedCache:
         self._c = c
         self._ref = ctypes.byref(c)
         self._spaces = {}  # (stream, query heads) -> workspace
-        _check(L.lib.mtt_b200_paged_cache_workspace_size(self._ref, kv_heads) > 0, "this cache is too large")
+        _check(L.lib.mtt_b200_paged_cache_workspace_size(self._ref, kv_heads, 0) > 0, "this cache is too large")
 
     @staticmethod
     def allocate(pages: int, slots: int, max_tokens: int, layers: int, kv_heads: int, head_dim: int,
@@ -102,18 +104,24 @@ class PagedCache:
     def _stream(self, stream):
         return torch.cuda.current_stream(self.device) if stream is None else stream
 
-    def _workspace(self, stream, q_heads: int) -> torch.Tensor:
-        """The workspace of calls on one stream: kept, as the streams' calls may overlap."""
+    def _workspace(self, stream, q_heads: int, rows: int = 0) -> torch.Tensor:
+        """The workspace of calls on one stream: kept, and one for each stream, as the streams' calls may overlap."""
         key = (stream.cuda_stream, q_heads)
-        space = self._spaces.get(key)
-        if space is None:
-            size = L.lib.mtt_b200_paged_cache_workspace_size(self._ref, q_heads)
+        space, most = self._spaces.get(key, (None, -1))
+        if rows > most:
+            most = max(1024, 1 << (rows - 1).bit_length()) if rows else 0
+            size = L.lib.mtt_b200_paged_cache_workspace_size(self._ref, q_heads, most)
             _check(size > 0, "q_heads must be a multiple of kv_heads, at most "
                              f"{MAX_GROUP} query heads per key head")
             with torch.cuda.stream(stream):
                 space = torch.zeros(size, dtype=torch.uint8, device=self.device)
-            self._spaces[key] = space
+            self._spaces[key] = space, most
         return space
+
+    @staticmethod
+    def _on(stream, given):
+        """Where a call's own tensors are allocated: the stream that the caller gave, if any."""
+        return torch.cuda.stream(stream) if given else contextlib.nullcontext()
 
     def _vector(self, t: torch.Tensor, n: int, dtype: torch.dtype, name: str) -> int:
         _check(t.dtype == dtype and t.dim() == 1 and t.shape[0] == n and t.is_contiguous(),
@@ -201,10 +209,13 @@ class PagedCache:
         rows, q_heads, d = q.shape
         _check(q_heads >= 1 and q_heads % self.kv_heads == 0 and q_heads // self.kv_heads <= MAX_GROUP,
                f"q_heads must be a multiple of kv_heads, at most {MAX_GROUP} query heads per key head")
+        _check(rows <= MAX_ROWS, f"at most {MAX_ROWS} rows")
         _check(0 <= layer < self.layers, "no such layer")
         _check(window >= 0 and sinks >= 0, "window and sinks must not be negative")
+        _check(scale is None or 0 < scale < float("inf"), "scale must be positive")
+        given = stream is not None
         if out is None:
-            with torch.cuda.stream(stream):
+            with self._on(stream, given):
                 out = torch.empty(rows, q_heads, d, dtype=self.dtype, device=self.device)
         else:
             _check(out.shape == q.shape, "out must have q's shape")
@@ -215,7 +226,7 @@ class PagedCache:
         lse = None
         args = L.CacheAttention()
         if return_lse:
-            with torch.cuda.stream(stream):
+            with self._on(stream, given):
                 lse = torch.empty(rows, q_heads, dtype=torch.float32, device=self.device)
             args.lse = lse.data_ptr()
         args.layer, args.q_heads, args.rows, args.window, args.sinks = layer, q_heads, rows, window, sinks
@@ -238,8 +249,8 @@ class PagedCache:
         key_mask ([slots, >= table_pages * page_size] bool).  A row that sees
         none gets 0.  Returns out, or (out, lse) with the natural log of the sum
         of exponentials ([rows, q_heads] f32, -inf for a row that sees none)."""
-        stream = self._stream(stream)
         args, out, lse = self._attention(layer, q, out, window, sinks, scale, return_lse, stream)
+        stream = self._stream(stream)
         if offsets is not None:
             args.offsets = self._vector(offsets, self.slots + 1, torch.int32, "offsets")
         else:
@@ -250,7 +261,7 @@ class PagedCache:
                    key_mask.device == self.device and key_mask.stride(0) >= key_mask.shape[1],
                    "key_mask must be a [slots, >= table_pages * page_size] bool tensor with contiguous rows")
             args.key_mask, args.mask_stride = key_mask.data_ptr(), key_mask.stride(0)
-        ws = self._workspace(stream, args.q_heads)
+        ws = self._workspace(stream, args.q_heads, args.rows)
         self._done(L.lib.mtt_b200_launch_paged_attention(self._ref, ctypes.byref(args), ws.data_ptr(), ws.numel(),
                                                          stream.cuda_stream), "mtt_b200_launch_paged_attention")
         return (out, lse) if return_lse else out

@@ -282,6 +282,16 @@ def test_prompt_masks_and_nan_behind_them(pc, window, sinks, d, dtype):
                  dtype=dtype)
 
 
+@pytest.mark.parametrize("window,sinks,masked", [(0, 0, False), (300, 16, True), (64, 0, False)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_prompt_many_units_per_sm(pc, window, sinks, masked, d):
+    """More units than SMs, many with an empty second tile: every SM walks several, whole and cut."""
+    new = [1, 7, 130, 2, 255, 3, 40, 129, 5, 1, 300, 64] * 2
+    lengths = [n + (i * 97) % 500 for i, n in enumerate(new)]
+    cache = check_attend(pc, lengths, new, hkv=12, d=d, window=window, sinks=sinks, mask=holes if masked else None)
+    assert (cache.status == 0).all()
+
+
 def test_prompt_offsets_that_do_not_fit(pc):
     """More rows than tokens: those rows get 0 and -inf, the others are unharmed."""
     cache, pool, table = make(pc, [20, 40, 7])
