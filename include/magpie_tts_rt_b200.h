@@ -852,6 +852,35 @@ MTT_B200_API int mtt_b200_launch_paged_attention(const mtt_b200_paged_cache_t* c
                                                  const mtt_b200_cache_attention_t* args, void* workspace,
                                                  size_t workspace_bytes, void* stream);
 
+/* Groups of slots that share a prefix: members[offsets[g]..offsets[g + 1]) are
+ * the slots of group g, whose first tokens[g] tokens (a multiple of page_size)
+ * are those of slot voice[g], on the same pages, as fork leaves them.  A slot
+ * is in one group at most; slots in none are attended as usual. */
+typedef struct mtt_b200_prefix_groups {
+  int32_t n_groups;          /* <= slots */
+  int32_t n_members;         /* <= 2^22 */
+  const int32_t* voice;      /* [n_groups] */
+  const int32_t* tokens;     /* [n_groups] */
+  const int32_t* offsets;    /* [n_groups + 1] ascending, offsets[n_groups] = n_members */
+  const int32_t* members;    /* [n_members] slots */
+} mtt_b200_prefix_groups_t;
+
+/* Workspace bytes of the call below (0 for bad arguments); alignment and
+ * zeroing as above. */
+MTT_B200_API size_t mtt_b200_paged_shared_workspace_size(const mtt_b200_paged_cache_t* cache, int32_t q_heads,
+                                                         int32_t n_members);
+
+/* mtt_b200_launch_paged_attention's single-token form (args->offsets and
+ * args->key_mask NULL) with each group's prefix read and multiplied once for
+ * all its members.  The result is the same attention; a member is attended on
+ * its own when its slot or the voice's holds fewer than tokens[g] tokens, when
+ * its last prefix page is not the voice's, or when a window leaves some of the
+ * prefix out of sight (sinks < tokens[g]). */
+MTT_B200_API int mtt_b200_launch_paged_attention_shared(const mtt_b200_paged_cache_t* cache,
+                                                        const mtt_b200_cache_attention_t* args,
+                                                        const mtt_b200_prefix_groups_t* groups, void* workspace,
+                                                        size_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------------------------------ */
 /* Test hooks (no reference counterpart beyond launch_test_clamped_gumbel,   */
 /* plugins/local_ar_plugins.hpp:171-175)                                      */

@@ -194,6 +194,10 @@ class CacheAttention(ctypes.Structure):
                 ("lse", P), ("offsets", P), ("key_mask", P), ("mask_stride", I64)]
 
 
+class PrefixGroups(ctypes.Structure):
+    _fields_ = [("n_groups", I32), ("n_members", I32), ("voice", P), ("tokens", P), ("offsets", P), ("members", P)]
+
+
 # name -> (restype, argtypes)
 SIGNATURES = {
     "mtt_plugin_get_api_v1": (I32, [ctypes.POINTER(PluginApiV1)]),
@@ -233,6 +237,9 @@ SIGNATURES = {
         I32, [ctypes.POINTER(PagedCache), ctypes.POINTER(CacheRows), P]),
     "mtt_b200_launch_paged_attention": (
         I32, [ctypes.POINTER(PagedCache), ctypes.POINTER(CacheAttention), P, SZ, P]),
+    "mtt_b200_paged_shared_workspace_size": (SZ, [ctypes.POINTER(PagedCache), I32, I32]),
+    "mtt_b200_launch_paged_attention_shared": (
+        I32, [ctypes.POINTER(PagedCache), ctypes.POINTER(CacheAttention), ctypes.POINTER(PrefixGroups), P, SZ, P]),
     "mtt_b200_launch_test_clamped_gumbel": (I32, [P, P, SZ, P]),
     "mtt_b200_launch_test_log": (I32, [P, P, SZ, P]),
     "mtt_b200_launch_test_gemm": (I32, [P, P, P, I32, I32, I32, I32, I32, P, P]),

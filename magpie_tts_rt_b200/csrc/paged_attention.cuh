@@ -20,6 +20,12 @@ struct Attend {
   int64_t mask_stride;
 };
 
+// What the prefix pass leaves for the step kernel.
+struct SharedPrefix {
+  const int32_t* base;  // [rows] tokens of the slot's prefix that are already attended to (0: none); null: no groups
+  const float* state;   // [slots][q_heads][head_dim + 2]: weighted values, maximum (base 2), sum
+};
+
 constexpr float kLn2 = 0.6931471805599453f;
 
 __device__ __forceinline__ float ex2(float x) {
@@ -90,10 +96,15 @@ struct SeenTiles {
 
 // Workspace of the single-token attention.
 size_t step_workspace(const mtt_b200_paged_cache_t& c, int q_heads);
-cudaError_t launch_step(const PagedCache& c, int dtype, const Attend& a, void* space, cudaStream_t stream);
+cudaError_t launch_step(const PagedCache& c, int dtype, const Attend& a, const SharedPrefix& shared, void* space,
+                        cudaStream_t stream);
 
 // Workspace of the prompt attention for calls of up to `rows` query rows.
 size_t prompt_workspace(const mtt_b200_paged_cache_t& c, int q_heads, int rows);
 cudaError_t launch_prompt(const PagedCache& c, int dtype, const Attend& a, void* space, cudaStream_t stream);
+
+// The prefix pass of the shared-prefix attention: fills base and state.
+cudaError_t launch_prefix(const PagedCache& c, int dtype, const Attend& a, const mtt_b200_prefix_groups_t& groups,
+                          int32_t* base, float* state, void* space, cudaStream_t stream);
 
 }  // namespace mtt

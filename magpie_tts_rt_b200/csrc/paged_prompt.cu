@@ -57,6 +57,8 @@ struct PromptRows {
   const int32_t* members;    // prefix pass: slot of each member; null for prompts
   const int32_t* voice;      // prefix pass: [n] slot that holds the prefix
   const int32_t* tokens;     // prefix pass: [n] its length
+  int longest;               // prefix pass: longer prefixes are not shared (the window hides some of them)
+  int32_t* base;             // prefix pass: [slots] out, SharedPrefix::base
   float* state;              // prefix pass: [slots][q_heads][D + 2]: O, m, l of each member
 };
 
@@ -81,7 +83,7 @@ struct PairGeom {
     if (r.members != nullptr) {
       key_slot = r.voice[i];
       len = r.tokens[i];
-      ok = ok && key_slot >= 0 && key_slot < c.slots && len >= 0 && (len & (c.page_size - 1)) == 0;
+      ok = ok && key_slot >= 0 && key_slot < c.slots && len > 0 && len <= r.longest && (len & (c.page_size - 1)) == 0;
       ok = ok && c.length(ok ? key_slot : 0) >= len;
     } else {
       key_slot = i;
@@ -167,6 +169,24 @@ __global__ void __launch_bounds__(kPromptPlanThreads)
   wait_prior_grid();
   const int tid = threadIdx.x;
   const bool prefix = rows.members != nullptr;
+  if (prefix) {
+    for (int i = tid; i < c.slots; i += kPromptPlanThreads) rows.base[i] = 0;
+    __syncthreads();
+    for (int k = tid; k < rows.n_rows; k += kPromptPlanThreads) {
+      int lo = 0, hi = rows.n;  // the group whose members begin at or before k
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (rows.offsets[mid] <= k) lo = mid; else hi = mid;
+      }
+      const PairGeom g(c, rows, lo);
+      const int slot = rows.members[k];
+      if (!g.ok || k < g.row0 || k >= g.row0 + g.count || slot < 0 || slot >= c.slots || c.length(slot) < g.len) continue;
+      const int last = (g.len >> c.page_shift) - 1;
+      if (c.table[static_cast<int64_t>(slot) * c.table_pages + last] ==
+          c.table[static_cast<int64_t>(g.key_slot) * c.table_pages + last])
+        rows.base[slot] = g.len;
+    }
+  }
   // slots whose offsets overlap could ask for more pairs than there is room for
   const int most = rows.n_rows / tokens_per_pair + rows.n;
   int pairs = 0;
@@ -864,6 +884,23 @@ cudaError_t launch_prompt(const PagedCache& c, int dtype, const Attend& a, void*
   rows.n_rows = a.rows;
   rows.offsets = a.offsets;
   return run_prompt(c, dtype, a, rows, space, stream);
+}
+
+cudaError_t launch_prefix(const PagedCache& c, int dtype, const Attend& a, const mtt_b200_prefix_groups_t& groups,
+                          int32_t* base, float* state, void* space, cudaStream_t stream) {
+  PromptRows rows{};
+  rows.n = groups.n_groups;
+  rows.n_rows = groups.n_members;
+  rows.offsets = groups.offsets;
+  rows.members = groups.members;
+  rows.voice = groups.voice;
+  rows.tokens = groups.tokens;
+  rows.longest = a.window > 0 ? a.sinks : INT32_MAX;
+  rows.base = base;
+  rows.state = state;
+  Attend all = a;  // every member sees the whole prefix
+  all.window = all.sinks = 0;
+  return run_prompt(c, dtype, all, rows, space, stream);
 }
 
 }  // namespace mtt

@@ -54,7 +54,7 @@ __device__ __forceinline__ uint4 load16(const uint16_t* p, bool on) {
 
 template <typename T, int D, int NB>
 __global__ void __launch_bounds__(kStepThreads, StepCfg<D>::kCtas)
-    step_kernel(PagedCache c, Attend a, StepSpace ws, int blocks, int min_tiles) {
+    step_kernel(PagedCache c, Attend a, SharedPrefix shared, StepSpace ws, int blocks, int min_tiles) {
   constexpr int NT = StepCfg<D>::kTiles;
   constexpr int NQ = 8 * NB;   // query rows of a unit
   constexpr int KC = D / 32;   // 16-byte pieces of a key row per thread
@@ -67,44 +67,71 @@ __global__ void __launch_bounds__(kStepThreads, StepCfg<D>::kCtas)
   const int t = lane & 3, g = lane >> 2;
   wait_prior_grid();
 
-  // tiles of every slot, scanned
+  auto tiles_of = [&](int i) {
+    return SeenTiles(c.length(i), a.window, a.sinks, shared.base != nullptr ? shared.base[i] : 0);
+  };
+  // tiles of every slot, scanned: a thread's slots lie side by side
   {
-    int run = 0;
-    for (int base = 0; base < a.rows; base += kStepThreads) {
-      const int i = base + tid;
-      const int n = i < a.rows ? SeenTiles(c.length(i), a.window, a.sinks, 0).n : 0;
-      int inc = n;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int x = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += x;
-      }
-      __shared__ int warp_sum[kStepWarps];
-      if (lane == 31) warp_sum[warp] = inc;
-      __syncthreads();
-      int before = run;
-#pragma unroll
-      for (int w = 0; w < kStepWarps; ++w) {
-        if (w < warp) before += warp_sum[w];
-        run += warp_sum[w];
-      }
-      if (i < a.rows) tiles_before[i] = before + inc - n;
-      __syncthreads();
+    __shared__ int warp_sum[kStepWarps];
+    const int each = (a.rows + kStepThreads - 1) / kStepThreads;
+    const int i0 = min(a.rows, tid * each), i1 = min(a.rows, i0 + each);
+    int n = 0;
+#pragma unroll 8
+    for (int i = i0; i < i1; ++i) {
+      const int x = tiles_of(i).n;
+      tiles_before[i] = x;
+      n += x;
     }
-    if (tid == 0) tiles_before[a.rows] = run;
+    int inc = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += x;
+    }
+    if (lane == 31) warp_sum[warp] = inc;
+    __syncthreads();
+    int before = inc - n, all = 0;
+#pragma unroll
+    for (int w = 0; w < kStepWarps; ++w) {
+      if (w < warp) before += warp_sum[w];
+      all += warp_sum[w];
+    }
+    for (int i = i0; i < i1; ++i) {
+      const int x = tiles_before[i];
+      tiles_before[i] = before;
+      before += x;
+    }
+    if (tid == 0) tiles_before[a.rows] = all;
     __syncthreads();
   }
   const int units = c.kv_heads * blocks;
   const int64_t total = static_cast<int64_t>(tiles_before[a.rows]) * units;
   const int64_t per = max((total + gridDim.x - 1) / gridDim.x, static_cast<int64_t>(min_tiles));
 
-  // slots without a key in reach
+  // (maximum, sum, two dims of the weighted values) of a row to its output, with its prefix's where it has one
+  auto finish = [&](int slot, int h, int d, float top, float sum, float o0, float o1) {
+    if (shared.base != nullptr && shared.base[slot] > 0) {
+      const float* st = shared.state + (static_cast<int64_t>(slot) * a.q_heads + h) * (D + 2);
+      const float2 ml = *reinterpret_cast<const float2*>(st + D), y = *reinterpret_cast<const float2*>(st + d);
+      const float both = fmaxf(top, ml.x);
+      const float z = both == -CUDART_INF_F ? 0.f : both;
+      const float f0 = ex2(top - z), f1 = ex2(ml.x - z);
+      sum = fmaf(f0, sum, f1 * ml.y);
+      o0 = fmaf(f0, o0, f1 * y.x);
+      o1 = fmaf(f0, o1, f1 * y.y);
+      top = both;
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    *reinterpret_cast<uint32_t*>(a.out + slot * a.out_row + static_cast<int64_t>(h) * D + d) =
+        Half16<T>::pack(o0 * inv, o1 * inv);
+    if (d == 0 && a.lse != nullptr) a.lse[static_cast<int64_t>(slot) * a.q_heads + h] = (top + log2f(sum)) * kLn2;
+  };
+
+  // slots without a key in reach here
   for (int i = blockIdx.x; i < a.rows; i += gridDim.x) {
     if (tiles_before[i + 1] != tiles_before[i]) continue;
-    for (int e = tid; e < a.q_heads * D / 8; e += kStepThreads)
-      *reinterpret_cast<uint4*>(a.out + i * a.out_row + 8 * e) = make_uint4(0, 0, 0, 0);
-    if (a.lse != nullptr)
-      for (int h = tid; h < a.q_heads; h += kStepThreads) a.lse[static_cast<int64_t>(i) * a.q_heads + h] = -CUDART_INF_F;
+    for (int e = tid; e < a.q_heads * (D / 2); e += kStepThreads)
+      finish(i, e / (D / 2), 2 * (e % (D / 2)), -CUDART_INF_F, 0.f, 0.f, 0.f);
   }
 
   int64_t x = static_cast<int64_t>(blockIdx.x) * per;
@@ -122,7 +149,7 @@ __global__ void __launch_bounds__(kStepThreads, StepCfg<D>::kCtas)
   }
   while (x < x_end) {
     while (static_cast<int64_t>(tiles_before[slot + 1]) * units <= x) ++slot;
-    const SeenTiles seen(c.length(slot), a.window, a.sinks, 0);
+    const SeenTiles seen = tiles_of(slot);
     const int64_t slot_x = static_cast<int64_t>(tiles_before[slot]) * units;
     const int unit = static_cast<int>((x - slot_x) / seen.n);
     const int64_t unit_x = slot_x + static_cast<int64_t>(unit) * seen.n;
@@ -304,11 +331,7 @@ __global__ void __launch_bounds__(kStepThreads, StepCfg<D>::kCtas)
         o1 = fmaf(f, y.y, o1);
       }
       if (whole) {
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        *reinterpret_cast<uint32_t*>(a.out + slot * a.out_row + static_cast<int64_t>(q_head + qi) * D + d) =
-            Half16<T>::pack(o0 * inv, o1 * inv);
-        if (d == 0 && a.lse != nullptr)
-          a.lse[static_cast<int64_t>(slot) * a.q_heads + q_head + qi] = (top + log2f(sum)) * kLn2;
+        finish(slot, q_head + qi, d, top, sum, o0, o1);
       } else {
         *reinterpret_cast<float2*>(part + qi * (D + 2) + d) = make_float2(o0, o1);
         if (d == 0) *reinterpret_cast<float2*>(part + qi * (D + 2) + D) = make_float2(top, sum);
@@ -344,11 +367,7 @@ __global__ void __launch_bounds__(kStepThreads, StepCfg<D>::kCtas)
             o0 = fmaf(f, y.x, o0);
             o1 = fmaf(f, y.y, o1);
           }
-          const float inv = sum == 0.f ? 0.f : 1.f / sum;
-          *reinterpret_cast<uint32_t*>(a.out + slot * a.out_row + static_cast<int64_t>(q_head + qi) * D + d) =
-              Half16<T>::pack(o0 * inv, o1 * inv);
-          if (d == 0 && a.lse != nullptr)
-            a.lse[static_cast<int64_t>(slot) * a.q_heads + q_head + qi] = (top + log2f(sum)) * kLn2;
+          finish(slot, q_head + qi, d, top, sum, o0, o1);
         }
       }
     }
@@ -375,7 +394,8 @@ size_t step_workspace(const mtt_b200_paged_cache_t& c, int q_heads) {
   return arrived + static_cast<size_t>(step_grid(c.head_dim, 160)) * 2 * 8 * nb * (c.head_dim + 2) * 4;
 }
 
-cudaError_t launch_step(const PagedCache& c, int dtype, const Attend& a, void* space, cudaStream_t stream) {
+cudaError_t launch_step(const PagedCache& c, int dtype, const Attend& a, const SharedPrefix& shared, void* space,
+                        cudaStream_t stream) {
   int nb, blocks;
   step_blocks(a.group, &nb, &blocks);
   StepSpace ws;
@@ -392,7 +412,7 @@ cudaError_t launch_step(const PagedCache& c, int dtype, const Attend& a, void* s
                                                  4 * (kCacheMaxSlots + 1));
       if (e != cudaSuccess) return e;
     }
-    return launch_serialized(kernel, dim3(step_grid(c.head_dim, sms)), dim3(kStepThreads), smem, stream, c, a, ws,
+    return launch_serialized(kernel, dim3(step_grid(c.head_dim, sms)), dim3(kStepThreads), smem, stream, c, a, shared, ws,
                              blocks, min_tiles);
   };
   auto pick = [&](auto type) {

@@ -11,7 +11,9 @@ slot, and a reference count per page, all on the device:
 * ``free`` / ``compact``: slots closed, pages in use moved to the pool's start;
 * ``attend``: attention of each slot's newest token, or of runs of new tokens
   (a prompt), with an optional sliding window and a few first tokens
-  (``sinks``) that stay visible.
+  (``sinks``) that stay visible;
+* ``attend_shared``: the newest tokens' attention where groups of slots share a
+  prefix (``PrefixGroups``), computed once for each group.
 
 Every call is enqueued on the current (or given) CUDA stream and returns
 without waiting.  What a call cannot do on the device (no free page, offsets
@@ -265,3 +267,71 @@ class PagedCache:
         self._done(L.lib.mtt_b200_launch_paged_attention(self._ref, ctypes.byref(args), ws.data_ptr(), ws.numel(),
                                                          stream.cuda_stream), "mtt_b200_launch_paged_attention")
         return (out, lse) if return_lse else out
+
+    def attend_shared(self, layer: int, q: torch.Tensor, groups: "PrefixGroups", out: Optional[torch.Tensor] = None, *,
+                      window: int = 0, sinks: int = 0, scale: Optional[float] = None, return_lse: bool = False,
+                      stream=None):
+        """``attend`` without offsets for slots that share prefixes: the keys and
+        values of a group's prefix are read and multiplied once for all its
+        members.  Slots in no group, slots that no longer hold their group's
+        pages, and groups whose prefix is longer than ``sinks`` under a window
+        are attended one by one; the result is the same."""
+        _check(groups.cache is self, "these groups belong to another cache")
+        _check(q.dim() == 3 and q.shape[1] == groups.q_heads, "these groups were made for another number of heads")
+        _check(q.shape[0] <= self.slots, "more rows than slots")
+        args, out, lse = self._attention(layer, q, out, window, sinks, scale, return_lse, stream)
+        stream = self._stream(stream)
+        ws = groups._workspace(stream)
+        self._done(L.lib.mtt_b200_launch_paged_attention_shared(self._ref, ctypes.byref(args), groups._ref,
+                                                                ws.data_ptr(), ws.numel(), stream.cuda_stream),
+                   "mtt_b200_launch_paged_attention_shared")
+        return (out, lse) if return_lse else out
+
+
+class PrefixGroups:
+    """Which slots of a cache share which prefix, for ``attend_shared``: made
+    when sessions open or close, used for every layer of every step between.
+
+    groups: (voice, tokens, members) for each: the members' first ``tokens``
+    tokens are those of slot ``voice``, on the same pages (the members were
+    forked from it; the voice itself may be one of them).  ``tokens`` is
+    rounded down to full pages.  The voice must stay open while the groups are
+    used; a member whose slot has been closed or reopened since is attended on
+    its own."""
+
+    def __init__(self, cache: PagedCache, groups, q_heads: int):
+        _check(q_heads >= 1 and q_heads % cache.kv_heads == 0 and q_heads // cache.kv_heads <= MAX_GROUP,
+               f"q_heads must be a multiple of kv_heads, at most {MAX_GROUP} query heads per key head")
+        voices, tokens, offsets, members = [], [], [0], []
+        for voice, count, slots in groups:
+            _check(0 <= voice < cache.slots, "no such voice slot")
+            _check(0 <= count <= cache.table_pages * cache.page_size, "a prefix longer than a slot")
+            _check(all(0 <= s < cache.slots for s in slots), "no such member slot")
+            count = count // cache.page_size * cache.page_size
+            if count == 0 or len(slots) == 0:
+                continue
+            voices.append(voice)
+            tokens.append(count)
+            members.extend(slots)
+            offsets.append(len(members))
+        _check(len(set(members)) == len(members), "a slot can be in one group only")
+        self.cache, self.q_heads = cache, q_heads
+        self.n_members = len(members)
+        n = len(voices)
+        self._data = torch.tensor(voices + tokens + offsets + members, dtype=torch.int32).to(cache.device)
+        at = self._data.data_ptr()
+        c = L.PrefixGroups()
+        c.n_groups, c.n_members = n, len(members)
+        c.voice, c.tokens, c.offsets, c.members = at, at + 4 * n, at + 8 * n, at + 4 * (3 * n + 1)
+        self._c = c
+        self._ref = ctypes.byref(c)
+        self._spaces = {}
+
+    def _workspace(self, stream) -> torch.Tensor:
+        space = self._spaces.get(stream.cuda_stream)
+        if space is None:
+            size = L.lib.mtt_b200_paged_shared_workspace_size(self.cache._ref, self.q_heads, self.n_members)
+            with torch.cuda.stream(stream):
+                space = torch.zeros(size, dtype=torch.uint8, device=self.cache.device)
+            self._spaces[stream.cuda_stream] = space
+        return space

@@ -428,6 +428,124 @@ def test_in_a_cuda_graph(pc):
 
 
 # ---------------------------------------------------------------------------
+# shared prefixes
+# ---------------------------------------------------------------------------
+
+def voices_and_members(pc, prefixes, suffixes, hkv=2, d=64, ps=16, dtype=torch.bfloat16, seed=0):
+    """Slots: the voices, then for each voice its members, forked from it and
+    extended by suffixes[voice]; everything not stored is NaN."""
+    n = len(prefixes) + sum(len(s) for s in suffixes)
+    longest = max(p + max(s, default=0) for p, s in zip(prefixes, suffixes))
+    pages = sum(-(-p // ps) for p in prefixes) + sum(2 + x // ps for s in suffixes for x in s) + 4
+    cache = pc.PagedCache.allocate(pages, n, longest + 1, 1, hkv, d, ps, dtype)
+    cache.pool.fill_(float("nan"))
+    g = torch.Generator().manual_seed(seed)
+
+    def add(counts):
+        rows = sum(counts)
+        cache.extend(i32(counts))
+        k, v = (torch.randn(1, rows, hkv, d, generator=g).to(dtype).cuda() for _ in range(2))
+        cache.store(k, v, offsets=i32([0] + np.cumsum(counts).tolist()))
+
+    add(list(prefixes) + [0] * (n - len(prefixes)))
+    source, more, groups, at = [-1] * len(prefixes), [0] * len(prefixes), [], len(prefixes)
+    for v, s in enumerate(suffixes):
+        groups.append((v, prefixes[v], list(range(at, at + len(s)))))
+        source += [v] * len(s)
+        more += s
+        at += len(s)
+    cache.fork(i32(source))
+    add(more)
+    assert (cache.status == 0).all()
+    return cache, groups
+
+
+def check_shared(pc, cache, groups, group=1, window=0, sinks=0, rows=None, seed=5):
+    lengths = cache.lengths.cpu().tolist()
+    rows = len(lengths) if rows is None else rows
+    q = queries(rows, cache.kv_heads * group, cache.head_dim, cache.dtype, seed)
+    ref = O.attention(cache.pool.cpu(), cache.page_table.cpu(), lengths[:rows], 0, q, list(range(rows + 1)), window,
+                      sinks)
+    plan = pc.PrefixGroups(cache, groups, q_heads=q.shape[1])
+    for _ in range(2):
+        got, lse = cache.attend_shared(0, q.cuda(), plan, window=window, sinks=sinks, return_lse=True)
+        agree(got, lse, ref, cache.dtype, max(lengths))
+    assert (cache.status == 0).all()
+
+
+@pytest.mark.parametrize("prefixes,suffixes", [
+    ([208], [[1, 5, 17, 40, 100, 249, 3, 64]]), ([16], [[1]]), ([48], [[0, 0, 1]]), ([218, 37], [[1, 30], [2, 9, 200]]),
+    ([1000], [[7] * 3]), ([64, 128, 256], [[1 + i % 7 for i in range(130)], [3], [2] * 270]), ([5], [[1, 2, 3]])])
+@pytest.mark.parametrize("group,d,dtype", [(1, 64, torch.bfloat16), (4, 128, torch.float16)])
+def test_shared(pc, prefixes, suffixes, group, d, dtype):
+    cache, groups = voices_and_members(pc, prefixes, suffixes, d=d, dtype=dtype)
+    check_shared(pc, cache, groups, group)
+
+
+@pytest.mark.parametrize("hkv,group,d,ps", [(12, 1, 64, 16), (1, 13, 64, 32), (2, 64, 128, 128), (3, 3, 128, 64)])
+def test_shared_heads(pc, hkv, group, d, ps):
+    cache, groups = voices_and_members(pc, [3 * ps + 5, 640], [[1, 70, 9], [2, 33]], hkv=hkv, d=d, ps=ps)
+    check_shared(pc, cache, groups, group)
+
+
+def test_shared_long_prefix_is_cut(pc):
+    """Few members and a long prefix: the prefix's key tiles are dealt over the SMs and joined."""
+    cache, groups = voices_and_members(pc, [9000, 4096], [[1, 2, 3], [5] * 140], hkv=1, d=128)
+    check_shared(pc, cache, groups, group=2)
+
+
+@pytest.mark.parametrize("window,sinks", [(30, 208), (30, 300), (1, 218), (500, 208), (30, 100), (30, 0)])
+def test_shared_window(pc, window, sinks):
+    """sinks below the prefix's length: attended slot by slot."""
+    cache, groups = voices_and_members(pc, [218], [[1, 5, 40, 100, 249]])
+    check_shared(pc, cache, groups, group=2, window=window, sinks=sinks)
+
+
+def test_shared_slots_change_hands(pc):
+    """Members closed, reopened from another voice or too short, and a voice among its members."""
+    cache, groups = voices_and_members(pc, [64, 96], [[1, 5, 9], [2, 30, 4]])
+    n = cache.slots
+    groups = [(v, p, [v] + m) for v, p, m in groups]
+    check_shared(pc, cache, groups)
+    mask = torch.zeros(n, dtype=torch.bool, device="cuda")
+    mask[groups[0][2][1]] = True
+    mask[groups[1][2][2]] = True
+    cache.free(mask)
+    source = [-1] * n
+    source[groups[0][2][2]] = 1             # a member of voice 0 now speaks with voice 1
+    source[groups[1][2][3]] = 0             # and the other way round: shorter than its group's prefix
+    cache.fork(i32(source))
+    check_shared(pc, cache, groups)
+    check_shared(pc, cache, groups, rows=n - 2)
+    check_shared(pc, cache, groups[:1])
+    check_shared(pc, cache, [])
+    cache.compact()
+    check_shared(pc, cache, groups)
+    mask.zero_()
+    mask[1] = True                          # a voice closed under its members
+    cache.free(mask)
+    check_shared(pc, cache, groups)
+
+
+def test_shared_refusals(pc):
+    cache, groups = voices_and_members(pc, [64, 96], [[1, 5, 9], [2, 30, 4]])
+    other, _ = voices_and_members(pc, [64], [[1]])
+    plan = pc.PrefixGroups(cache, groups, q_heads=4)
+    q = queries(cache.slots, 4, 64, torch.bfloat16).cuda()
+    bad = [lambda: pc.PrefixGroups(cache, [(0, 64, [2, 3]), (1, 96, [3])], 4),
+           lambda: pc.PrefixGroups(cache, [(99, 64, [2])], 4), lambda: pc.PrefixGroups(cache, [(0, 64, [-1])], 4),
+           lambda: pc.PrefixGroups(cache, [(0, 64, [99])], 4), lambda: pc.PrefixGroups(cache, [(0, 1 << 20, [2])], 4),
+           lambda: pc.PrefixGroups(cache, groups, 3), lambda: other.attend_shared(0, q[:2], plan),
+           lambda: cache.attend_shared(0, q[:, :2], plan), lambda: cache.attend_shared(0, torch.cat([q, q]), plan),
+           lambda: cache.attend_shared(0, q, plan, window=-1), lambda: cache.attend_shared(1, q, plan),
+           lambda: cache.attend_shared(0, q, plan, scale=0.0)]
+    for n, call in enumerate(bad):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail(f"case {n} was accepted")
+
+
+# ---------------------------------------------------------------------------
 # refusals on the host
 # ---------------------------------------------------------------------------
 
