@@ -17,11 +17,13 @@
 //    16-byte pieces.  (tcgen05 would want the same bytes staged in shared
 //    memory for a tile of 128 rows of which 1 to 16 are real.)
 //  * The work is one line of 16-key tiles over all (slot, key head) units,
-//    cut into equal parts for a grid that fills the device, so ragged
-//    lengths balance by themselves.  A unit cut by a CTA boundary leaves
-//    (maximum, sum, weighted values) in the workspace; the CTA that arrives
-//    last joins them in the order of the CTAs, so the result does not depend
-//    on timing.
+//    cut into equal parts for the warps of a grid that fills the device, so
+//    ragged lengths balance by themselves and no warp waits for another.  A
+//    unit that a cut divides leaves (maximum, sum, weighted values) of each
+//    part in the workspace; a second kernel joins the parts in their order,
+//    so the result does not depend on timing.
+#include <algorithm>
+
 #include "paged_attention.cuh"
 
 namespace mtt {
@@ -30,16 +32,35 @@ namespace {
 constexpr int kStepWarps = 4;
 constexpr int kStepThreads = 32 * kStepWarps;
 
-template <int D>
-struct StepCfg {
-  static constexpr int kTiles = D == 64 ? 2 : 1;  // 16-key tiles per warp and step
-  static constexpr int kCtas = D == 64 ? 4 : 3;   // per SM (registers)
-};
+constexpr int step_tiles(int head_dim) { return head_dim == 64 ? 2 : 1; }  // 16-key tiles per warp and step
+constexpr int step_ctas(int head_dim, int nb) { return (head_dim == 64 ? 4 : 3) - (nb == 2 ? 1 : 0); }  // per SM (registers)
 
 struct StepSpace {
-  int32_t* arrived;  // [slots * units]: CTAs that have left their part of a unit; 0 between calls
-  float* part;       // [CTAs][2][queries][D + 2]
+  int4* cut;    // [warps]: the cut unit that begins in the warp's share: slot, unit, warps that hold it (0: none)
+  float* part;  // [warps][2][queries][D + 2]: of the share's first unit, and of a later one
 };
+
+// (maximum, sum, two dims of the weighted values) of a row to its output,
+// joined with its prefix's where it has one.
+template <typename T, int D>
+__device__ __forceinline__ void finish_row(const Attend& a, const SharedPrefix& shared, int slot, int h, int d,
+                                           float top, float sum, float o0, float o1) {
+  if (shared.base != nullptr && shared.base[slot] > 0) {
+    const float* st = shared.state + (static_cast<int64_t>(slot) * a.q_heads + h) * (D + 2);
+    const float2 ml = *reinterpret_cast<const float2*>(st + D), y = *reinterpret_cast<const float2*>(st + d);
+    const float both = fmaxf(top, ml.x);
+    const float z = both == -CUDART_INF_F ? 0.f : both;
+    const float f0 = ex2(top - z), f1 = ex2(ml.x - z);
+    sum = fmaf(f0, sum, f1 * ml.y);
+    o0 = fmaf(f0, o0, f1 * y.x);
+    o1 = fmaf(f0, o1, f1 * y.y);
+    top = both;
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  *reinterpret_cast<uint32_t*>(a.out + slot * a.out_row + static_cast<int64_t>(h) * D + d) =
+      Half16<T>::pack(o0 * inv, o1 * inv);
+  if (d == 0 && a.lse != nullptr) a.lse[static_cast<int64_t>(slot) * a.q_heads + h] = (top + log2f(sum)) * kLn2;
+}
 
 // Not the read-only path: the launch before this one may have written the
 // cache, and this kernel may already have been scheduled by then.
@@ -53,16 +74,13 @@ __device__ __forceinline__ uint4 load16(const uint16_t* p, bool on) {
 }
 
 template <typename T, int D, int NB>
-__global__ void __launch_bounds__(kStepThreads, StepCfg<D>::kCtas)
+__global__ void __launch_bounds__(kStepThreads, step_ctas(D, NB))
     step_kernel(PagedCache c, Attend a, SharedPrefix shared, StepSpace ws, int blocks, int min_tiles) {
-  constexpr int NT = StepCfg<D>::kTiles;
+  constexpr int NT = step_tiles(D);
   constexpr int NQ = 8 * NB;   // query rows of a unit
   constexpr int KC = D / 32;   // 16-byte pieces of a key row per thread
   constexpr int VC = D / 64;   // of a value row
   extern __shared__ int tiles_before[];  // [rows + 1]: tiles of a key head of the slots before
-  __shared__ float s_m[kStepWarps][NQ], s_l[kStepWarps][NQ];
-  __shared__ float s_acc[kStepWarps][NQ][D];
-  __shared__ int s_last;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int t = lane & 3, g = lane >> 2;
   wait_prior_grid();
@@ -106,36 +124,19 @@ __global__ void __launch_bounds__(kStepThreads, StepCfg<D>::kCtas)
   }
   const int units = c.kv_heads * blocks;
   const int64_t total = static_cast<int64_t>(tiles_before[a.rows]) * units;
-  const int64_t per = max((total + gridDim.x - 1) / gridDim.x, static_cast<int64_t>(min_tiles));
-
-  // (maximum, sum, two dims of the weighted values) of a row to its output, with its prefix's where it has one
-  auto finish = [&](int slot, int h, int d, float top, float sum, float o0, float o1) {
-    if (shared.base != nullptr && shared.base[slot] > 0) {
-      const float* st = shared.state + (static_cast<int64_t>(slot) * a.q_heads + h) * (D + 2);
-      const float2 ml = *reinterpret_cast<const float2*>(st + D), y = *reinterpret_cast<const float2*>(st + d);
-      const float both = fmaxf(top, ml.x);
-      const float z = both == -CUDART_INF_F ? 0.f : both;
-      const float f0 = ex2(top - z), f1 = ex2(ml.x - z);
-      sum = fmaf(f0, sum, f1 * ml.y);
-      o0 = fmaf(f0, o0, f1 * y.x);
-      o1 = fmaf(f0, o1, f1 * y.y);
-      top = both;
-    }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    *reinterpret_cast<uint32_t*>(a.out + slot * a.out_row + static_cast<int64_t>(h) * D + d) =
-        Half16<T>::pack(o0 * inv, o1 * inv);
-    if (d == 0 && a.lse != nullptr) a.lse[static_cast<int64_t>(slot) * a.q_heads + h] = (top + log2f(sum)) * kLn2;
-  };
+  const int shares = gridDim.x * kStepWarps, me = blockIdx.x * kStepWarps + warp;
+  const int64_t per = max((total + shares - 1) / shares, static_cast<int64_t>(min_tiles));
 
   // slots without a key in reach here
   for (int i = blockIdx.x; i < a.rows; i += gridDim.x) {
     if (tiles_before[i + 1] != tiles_before[i]) continue;
     for (int e = tid; e < a.q_heads * (D / 2); e += kStepThreads)
-      finish(i, e / (D / 2), 2 * (e % (D / 2)), -CUDART_INF_F, 0.f, 0.f, 0.f);
+      finish_row<T, D>(a, shared, i, e / (D / 2), 2 * (e % (D / 2)), -CUDART_INF_F, 0.f, 0.f, 0.f);
   }
 
-  int64_t x = static_cast<int64_t>(blockIdx.x) * per;
+  int64_t x = me * per;
   const int64_t x_end = min(total, x + per);
+  if (lane == 0) ws.cut[me] = make_int4(0, 0, 0, 0);
   if (x >= x_end) return;
   const int64_t x_first = x;
   int slot;
@@ -183,10 +184,10 @@ __global__ void __launch_bounds__(kStepThreads, StepCfg<D>::kCtas)
     int page[NT];
 #pragma unroll
     for (int u = 0; u < NT; ++u) {
-      const int tt = t0 + warp * NT + u;
+      const int tt = t0 + u;
       page[u] = tt < t1 ? row[(16 * seen.tile(tt)) >> c.page_shift] : -1;
     }
-    for (int base = t0 + warp * NT; base < t1; base += kStepWarps * NT) {
+    for (int base = t0; base < t1; base += NT) {
       // keys in reach: one per lane
       const int my_tile = base + (lane >> 4);
       bool in = my_tile < t1 && (lane >> 4) < NT;
@@ -219,7 +220,7 @@ __global__ void __launch_bounds__(kStepThreads, StepCfg<D>::kCtas)
       // the next step's pages, while this step's keys arrive
 #pragma unroll
       for (int u = 0; u < NT; ++u) {
-        const int tt = base + kStepWarps * NT + u;
+        const int tt = base + NT + u;
         page[u] = tt < t1 ? row[(16 * seen.tile(tt)) >> c.page_shift] : -1;
       }
 #pragma unroll
@@ -285,7 +286,9 @@ __global__ void __launch_bounds__(kStepThreads, StepCfg<D>::kCtas)
       }
     }
 
-    // the four warps' parts
+    // a thread holds queries 2t, 2t + 1 and dims 8g .. 8g + 7 of each 64
+    const bool whole = t0 == 0 && t1 == seen.n;
+    float* part = ws.part + (2 * static_cast<int64_t>(me) + (x == x_first ? 0 : 1)) * NQ * (D + 2);
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
 #pragma unroll
@@ -293,90 +296,68 @@ __global__ void __launch_bounds__(kStepThreads, StepCfg<D>::kCtas)
         l[b][0] += __shfl_xor_sync(0xffffffffu, l[b][0], o);
         l[b][1] += __shfl_xor_sync(0xffffffffu, l[b][1], o);
       }
-      const int q0 = 8 * b + 2 * t;
-      if (g == 0) {
-        s_m[warp][q0] = m[b][0];
-        s_m[warp][q0 + 1] = m[b][1];
-        s_l[warp][q0] = l[b][0];
-        s_l[warp][q0 + 1] = l[b][1];
-      }
 #pragma unroll
-      for (int v = 0; v < VC; ++v)
+      for (int i = 0; i < 2; ++i) {
+        const int qi = 8 * b + 2 * t + i;
+        if (qi >= queries) continue;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const int d = 64 * v + 8 * g + 2 * w;
-          if (q0 < queries)
-            *reinterpret_cast<float2*>(&s_acc[warp][q0][d]) = make_float2(acc[b][v][w][0], acc[b][v][w][2]);
-          if (q0 + 1 < queries)
-            *reinterpret_cast<float2*>(&s_acc[warp][q0 + 1][d]) = make_float2(acc[b][v][w][1], acc[b][v][w][3]);
-        }
-    }
-    __syncthreads();
-    const bool whole = t0 == 0 && t1 == seen.n;
-    const int64_t part_size = static_cast<int64_t>(NQ) * (D + 2);
-    float* part = ws.part + (2 * static_cast<int64_t>(blockIdx.x) + (x == x_first ? 0 : 1)) * part_size;
-    for (int e = tid; e < queries * (D / 2); e += kStepThreads) {
-      const int qi = e / (D / 2), d = 2 * (e % (D / 2));
-      float top = s_m[0][qi];
+        for (int v = 0; v < VC; ++v) {
 #pragma unroll
-      for (int w = 1; w < kStepWarps; ++w) top = fmaxf(top, s_m[w][qi]);
-      const float z = top == -CUDART_INF_F ? 0.f : top;
-      float sum = 0.f, o0 = 0.f, o1 = 0.f;
-#pragma unroll
-      for (int w = 0; w < kStepWarps; ++w) {
-        const float f = ex2(s_m[w][qi] - z);
-        const float2 y = *reinterpret_cast<const float2*>(&s_acc[w][qi][d]);
-        sum = fmaf(f, s_l[w][qi], sum);
-        o0 = fmaf(f, y.x, o0);
-        o1 = fmaf(f, y.y, o1);
-      }
-      if (whole) {
-        finish(slot, q_head + qi, d, top, sum, o0, o1);
-      } else {
-        *reinterpret_cast<float2*>(part + qi * (D + 2) + d) = make_float2(o0, o1);
-        if (d == 0) *reinterpret_cast<float2*>(part + qi * (D + 2) + D) = make_float2(top, sum);
-      }
-    }
-    if (!whole) {
-      const int first_cta = static_cast<int>(unit_x / per);
-      const int last_cta = static_cast<int>((unit_x + seen.n - 1) / per);
-      int32_t* arrived = ws.arrived + static_cast<int64_t>(slot) * units + unit;
-      __threadfence();
-      __syncthreads();
-      if (tid == 0) s_last = atomicAdd(arrived, 1) == last_cta - first_cta;
-      __syncthreads();
-      if (s_last) {
-        __threadfence();
-        if (tid == 0) *arrived = 0;  // for the next call
-        for (int e = tid; e < queries * (D / 2); e += kStepThreads) {
-          const int qi = e / (D / 2), d = 2 * (e % (D / 2));
-          // the first CTA's part is its last one unless its share begins here
-          auto at = [&](int k) {
-            return ws.part + (2 * static_cast<int64_t>(k) + (k * per < unit_x ? 1 : 0)) * part_size + qi * (D + 2);
-          };
-          float top = -CUDART_INF_F;
-          for (int k = first_cta; k <= last_cta; ++k) top = fmaxf(top, __ldcg(at(k) + D));
-          const float z = top == -CUDART_INF_F ? 0.f : top;
-          float sum = 0.f, o0 = 0.f, o1 = 0.f;
-          for (int k = first_cta; k <= last_cta; ++k) {
-            const float* p = at(k);
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(p + D));
-            const float2 y = __ldcg(reinterpret_cast<const float2*>(p + d));
-            const float f = ex2(ml.x - z);
-            sum = fmaf(f, ml.y, sum);
-            o0 = fmaf(f, y.x, o0);
-            o1 = fmaf(f, y.y, o1);
+          for (int w = 0; w < 4; ++w) {
+            const int d = 64 * v + 8 * g + 2 * w;
+            if (whole) {
+              finish_row<T, D>(a, shared, slot, q_head + qi, d, m[b][i], l[b][i], acc[b][v][w][i], acc[b][v][w][2 + i]);
+            } else {
+              *reinterpret_cast<float2*>(part + qi * (D + 2) + d) = make_float2(acc[b][v][w][i], acc[b][v][w][2 + i]);
+            }
           }
-          finish(slot, q_head + qi, d, top, sum, o0, o1);
         }
+        if (!whole && g == 0) *reinterpret_cast<float2*>(part + qi * (D + 2) + D) = make_float2(m[b][i], l[b][i]);
       }
     }
-    __syncthreads();  // s_* are free for the next unit
+    if (!whole && t0 == 0 && lane == 0)
+      ws.cut[me] = make_int4(slot, unit, static_cast<int>((unit_x + seen.n - 1) / per) - me + 1, x == x_first ? 0 : 1);
     x = unit_x + t1;
   }
 }
 
-int step_grid(int head_dim, int sms) { return sms * (head_dim == 64 ? StepCfg<64>::kCtas : StepCfg<128>::kCtas); }
+// Joins the parts of the units that a cut divided: `threads` threads (a
+// multiple of 32) for the unit that begins in one warp's share.
+template <typename T, int D>
+__global__ void __launch_bounds__(kStepThreads)
+    step_join_kernel(Attend a, SharedPrefix shared, StepSpace ws, int shares, int nq, int blocks, int threads) {
+  wait_prior_grid();
+  const int me = blockIdx.x * (kStepThreads / threads) + threadIdx.x / threads;
+  if (me >= shares) return;
+  const int4 cut = ws.cut[me];
+  if (cut.z == 0) return;
+  const int head = cut.y / blocks, block = cut.y % blocks;
+  const int queries = min(nq, a.group - block * nq);
+  // the first part lies where the warp left it, the others are their warps' first units
+  const int64_t stride = static_cast<int64_t>(nq) * (D + 2);
+  const float* first = ws.part + (2 * static_cast<int64_t>(me) + cut.w) * stride;
+  const float* rest = ws.part + 2 * static_cast<int64_t>(me) * stride;
+  for (int e = threadIdx.x % threads; e < queries * (D / 2); e += threads) {
+    const int qi = e / (D / 2), d = 2 * (e % (D / 2));
+    float2 ml = __ldcg(reinterpret_cast<const float2*>(first + qi * (D + 2) + D));
+    float2 y = __ldcg(reinterpret_cast<const float2*>(first + qi * (D + 2) + d));
+    float top = ml.x, sum = ml.y, o0 = y.x, o1 = y.y;
+#pragma unroll 4
+    for (int k = 1; k < cut.z; ++k) {
+      const float* p = rest + 2 * k * stride + qi * (D + 2);
+      ml = __ldcg(reinterpret_cast<const float2*>(p + D));
+      y = __ldcg(reinterpret_cast<const float2*>(p + d));
+      const float both = fmaxf(top, ml.x);
+      const float z = both == -CUDART_INF_F ? 0.f : both;
+      const float f0 = ex2(top - z), f1 = ex2(ml.x - z);
+      sum = fmaf(f0, sum, f1 * ml.y);
+      o0 = fmaf(f0, o0, f1 * y.x);
+      o1 = fmaf(f0, o1, f1 * y.y);
+      top = both;
+    }
+    finish_row<T, D>(a, shared, cut.x, head * a.group + block * nq + qi, d, top, sum, o0, o1);
+  }
+}
 
 // 8-query blocks of a unit, and units per key head
 void step_blocks(int group, int* nb, int* blocks) {
@@ -386,12 +367,18 @@ void step_blocks(int group, int* nb, int* blocks) {
 
 }  // namespace
 
+// cut records, then parts; sized for the largest device this library runs on
+// (kMaxSms SMs), so that the size does not depend on the current one
+constexpr int kMaxSms = 160;
+size_t cut_bytes(int head_dim, int nb) {
+  return static_cast<size_t>(kMaxSms) * step_ctas(head_dim, nb) * kStepWarps * sizeof(int4);
+}
+
 size_t step_workspace(const mtt_b200_paged_cache_t& c, int q_heads) {
   int nb, blocks;
   step_blocks(q_heads / c.kv_heads, &nb, &blocks);
-  const size_t arrived = (static_cast<size_t>(c.slots) * c.kv_heads * blocks * 4 + 255) / 256 * 256;
-  // sized for the largest device this library runs on, so that it does not depend on the current one
-  return arrived + static_cast<size_t>(step_grid(c.head_dim, 160)) * 2 * 8 * nb * (c.head_dim + 2) * 4;
+  const size_t shares = static_cast<size_t>(kMaxSms) * step_ctas(c.head_dim, nb) * kStepWarps;
+  return cut_bytes(c.head_dim, nb) + (shares * 2 * 8 * nb * (c.head_dim + 2) * 4 + 255) / 256 * 256;
 }
 
 cudaError_t launch_step(const PagedCache& c, int dtype, const Attend& a, const SharedPrefix& shared, void* space,
@@ -399,26 +386,35 @@ cudaError_t launch_step(const PagedCache& c, int dtype, const Attend& a, const S
   int nb, blocks;
   step_blocks(a.group, &nb, &blocks);
   StepSpace ws;
-  ws.arrived = static_cast<int32_t*>(space);
-  ws.part = reinterpret_cast<float*>(static_cast<char*>(space) +
-                                     (static_cast<size_t>(c.slots) * c.kv_heads * blocks * 4 + 255) / 256 * 256);
+  ws.cut = static_cast<int4*>(space);
+  ws.part = reinterpret_cast<float*>(static_cast<char*>(space) + cut_bytes(c.head_dim, nb));
   const int sms = cache_sm_count();
-  if (sms <= 0 || sms > 160) return cudaErrorInvalidValue;
+  if (sms <= 0 || sms > kMaxSms) return cudaErrorInvalidValue;
   const size_t smem = 4 * (static_cast<size_t>(a.rows) + 1);
-  const int min_tiles = kStepWarps * (c.head_dim == 64 ? StepCfg<64>::kTiles : StepCfg<128>::kTiles);
-  auto go = [&](auto kernel) {
-    if (smem > 14 * 1024) {
+  const int grid = sms * step_ctas(c.head_dim, nb), shares = grid * kStepWarps;
+  const int min_tiles = step_tiles(c.head_dim);
+  const int pairs = std::min(8 * nb, a.group) * c.head_dim / 2;
+  const int threads = pairs <= 32 ? 32 : pairs <= 64 ? 64 : 128;
+  auto go = [&](auto kernel, auto join) {
+    if (smem > 40 * 1024) {
       const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                  4 * (kCacheMaxSlots + 1));
       if (e != cudaSuccess) return e;
     }
-    return launch_serialized(kernel, dim3(step_grid(c.head_dim, sms)), dim3(kStepThreads), smem, stream, c, a, shared, ws,
-                             blocks, min_tiles);
+    cudaError_t e = launch_serialized(kernel, dim3(grid), dim3(kStepThreads), smem, stream, c, a, shared, ws, blocks,
+                                      min_tiles);
+    if (e != cudaSuccess) return e;
+    const int per_block = kStepThreads / threads;
+    return launch_serialized(join, dim3((shares + per_block - 1) / per_block), dim3(kStepThreads), 0, stream, a,
+                             shared, ws, shares, 8 * nb, blocks, threads);
   };
   auto pick = [&](auto type) {
     using T = decltype(type);
-    if (c.head_dim == 64) return nb == 1 ? go(step_kernel<T, 64, 1>) : go(step_kernel<T, 64, 2>);
-    return nb == 1 ? go(step_kernel<T, 128, 1>) : go(step_kernel<T, 128, 2>);
+    if (c.head_dim == 64)
+      return nb == 1 ? go(step_kernel<T, 64, 1>, step_join_kernel<T, 64>)
+                     : go(step_kernel<T, 64, 2>, step_join_kernel<T, 64>);
+    return nb == 1 ? go(step_kernel<T, 128, 1>, step_join_kernel<T, 128>)
+                   : go(step_kernel<T, 128, 2>, step_join_kernel<T, 128>);
   };
   return dtype == MTT_B200_DTYPE_BF16 ? pick(__nv_bfloat16{}) : pick(__half{});
 }
