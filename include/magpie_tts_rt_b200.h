@@ -733,7 +733,7 @@ MTT_B200_API int mtt_b200_session_engine_collect(mtt_b200_session_engine_t* engi
  * calls of one cache that change it must be ordered with each other and with
  * its readers (one stream, or events).
  *
- * slots * table_pages * page_size / 16 must be below 2^31.
+ * slots * table_pages * page_size / 16 must be below 2^31 - 2^17.
  *
  * status[i] (may be NULL), written by fork and extend for each slot they are
  * asked to change: 0 done; 1 a source slot or count out of range; 2 not

@@ -41,7 +41,7 @@ bool attend_args(const PagedCache& c, const mtt_b200_cache_attention_t* args, At
 // Bytes of the prefix pass's results: base and state (SharedPrefix).
 size_t base_bytes(const mtt_b200_paged_cache_t& c) { return (4 * static_cast<size_t>(c.slots) + 255) / 256 * 256; }
 size_t state_bytes(const mtt_b200_paged_cache_t& c, int q_heads) {
-  return (static_cast<size_t>(c.slots) * q_heads * (c.head_dim + 2) * 4 + 255) / 256 * 256;
+  return (static_cast<size_t>(c.slots) * q_heads * (c.head_dim + 4) * 4 + 255) / 256 * 256;
 }
 
 }  // namespace

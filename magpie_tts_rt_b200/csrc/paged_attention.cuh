@@ -23,7 +23,7 @@ struct Attend {
 // What the prefix pass leaves for the step kernel.
 struct SharedPrefix {
   const int32_t* base;  // [rows] tokens of the slot's prefix that are already attended to (0: none); null: no groups
-  const float* state;   // [slots][q_heads][head_dim + 2]: weighted values, maximum (base 2), sum
+  const float* state;   // [slots][q_heads][head_dim + 4]: weighted values, maximum (base 2), sum
 };
 
 constexpr float kLn2 = 0.6931471805599453f;

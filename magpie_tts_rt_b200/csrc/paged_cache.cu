@@ -406,7 +406,7 @@ bool paged_cache_view(const mtt_b200_paged_cache_t* c, PagedCache* out) {
   // rows of the pool (one token's keys or values of one head) and tokens of a slot are counted in 31 bits
   const double rows = static_cast<double>(c->pages) * c->layers * 2 * c->kv_heads * c->page_size;
   if (rows >= 2147483648.0 || static_cast<int64_t>(c->table_pages) * c->page_size >= (int64_t{1} << 30) ||
-      static_cast<double>(c->slots) * c->table_pages * (c->page_size / 16) >= 2147483648.0)
+      static_cast<double>(c->slots) * c->table_pages * (c->page_size / 16) >= 2147352576.0)
     return false;
   if (c->pool == nullptr || c->page_table == nullptr || c->lengths == nullptr || c->refs == nullptr ||
       (reinterpret_cast<uintptr_t>(c->pool) & 127u) != 0)

@@ -59,7 +59,7 @@ struct PromptRows {
   const int32_t* tokens;     // prefix pass: [n] its length
   int longest;               // prefix pass: longer prefixes are not shared (the window hides some of them)
   int32_t* base;             // prefix pass: [slots] out, SharedPrefix::base
-  float* state;              // prefix pass: [slots][q_heads][D + 2]: O, m, l of each member
+  float* state;              // prefix pass: [slots][q_heads][D + 4]: O, m, l of each member
 };
 
 // One pair of Q tiles: slot (or group), first token (or member), key tiles, key tiles of the pairs before.
@@ -675,7 +675,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       const float m2 = m == -CUDART_INF_F ? m : m * a.scale2;
       const bool whole = w.whole();
       float* part = ws.part + (2 * static_cast<int64_t>(blockIdx.x) + (w.first ? 0 : 1)) * (D + 2) * kPairRows + i * kTile + r;
-      float* state = prefix && there ? rows.state + (static_cast<int64_t>(q_row) * a.q_heads + q_head) * (D + 2) : nullptr;
+      float* state = prefix && there ? rows.state + (static_cast<int64_t>(q_row) * a.q_heads + q_head) * (D + 4) : nullptr;
       uint16_t* out = a.out + q_row * a.out_row + static_cast<int64_t>(q_head) * D;
 #pragma unroll
       for (int b = 0; b < D / 32; ++b) {
@@ -691,8 +691,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           for (int k = 0; k < 32; ++k) part[(32 * b + k) * kPairRows] = __uint_as_float(o[k]);
         } else if (prefix) {
 #pragma unroll
-          for (int k = 0; k < 16; ++k)
-            *reinterpret_cast<uint2*>(state + 32 * b + 2 * k) = make_uint2(o[2 * k], o[2 * k + 1]);
+          for (int k = 0; k < 8; ++k)
+            *reinterpret_cast<uint4*>(state + 32 * b + 4 * k) = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
         } else {
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
@@ -778,7 +778,7 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(PagedCache c, Attend a
     for (int e = 0; e < E; ++e) o[e] = fmaf(f, p[(d0 + e) * kPairRows], o[e]);
   }
   if (prefix) {
-    float* state = rows.state + (static_cast<int64_t>(q_row) * a.q_heads + q_head) * (D + 2);
+    float* state = rows.state + (static_cast<int64_t>(q_row) * a.q_heads + q_head) * (D + 4);
 #pragma unroll
     for (int e = 0; e < E; ++e) state[d0 + e] = o[e];
     if (d0 == 0) *reinterpret_cast<float2*>(state + D) = make_float2(top, l);

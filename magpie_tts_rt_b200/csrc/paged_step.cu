@@ -35,32 +35,67 @@ constexpr int kStepThreads = 32 * kStepWarps;
 constexpr int step_tiles(int head_dim) { return head_dim == 64 ? 2 : 1; }  // 16-key tiles per warp and step
 constexpr int step_ctas(int head_dim, int nb) { return (head_dim == 64 ? 4 : 3) - (nb == 2 ? 1 : 0); }  // per SM (registers)
 
+// A unit's place on the line: its tiles, and before them what entering and
+// leaving it costs, in tiles.  (2052 slots with 1 to 249 keys each, prefix pass
+// included: 134 us with 0, 96 with 2, 104 with 4, 116 with 8.)
+constexpr int kUnitCost = 2;
+
 struct StepSpace {
   int4* cut;    // [warps]: the cut unit that begins in the warp's share: slot, unit, warps that hold it (0: none)
   float* part;  // [warps][2][queries][D + 2]: of the share's first unit, and of a later one
 };
 
-// (maximum, sum, two dims of the weighted values) of a row to its output,
-// joined with its prefix's where it has one.
-template <typename T, int D>
-__device__ __forceinline__ void finish_row(const Attend& a, const SharedPrefix& shared, int slot, int h, int d,
-                                           float top, float sum, float o0, float o1) {
-  if (shared.base != nullptr && shared.base[slot] > 0) {
-    const float* st = shared.state + (static_cast<int64_t>(slot) * a.q_heads + h) * (D + 2);
-    const float2 ml = *reinterpret_cast<const float2*>(st + D), y = *reinterpret_cast<const float2*>(st + d);
-    const float both = fmaxf(top, ml.x);
-    const float z = both == -CUDART_INF_F ? 0.f : both;
-    const float f0 = ex2(top - z), f1 = ex2(ml.x - z);
-    sum = fmaf(f0, sum, f1 * ml.y);
-    o0 = fmaf(f0, o0, f1 * y.x);
-    o1 = fmaf(f0, o1, f1 * y.y);
-    top = both;
+// E consecutive dims of a row: weighted values, maximum (base 2) and sum.
+template <int E>
+struct RowPart {
+  float m, l, o[E];
+  __device__ __forceinline__ void none() {
+    m = -CUDART_INF_F;
+    l = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = 0.f;
   }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  *reinterpret_cast<uint32_t*>(a.out + slot * a.out_row + static_cast<int64_t>(h) * D + d) =
-      Half16<T>::pack(o0 * inv, o1 * inv);
-  if (d == 0 && a.lse != nullptr) a.lse[static_cast<int64_t>(slot) * a.q_heads + h] = (top + log2f(sum)) * kLn2;
-}
+  __device__ __forceinline__ void join(const RowPart& x) {
+    const float top = fmaxf(m, x.m);
+    const float z = top == -CUDART_INF_F ? 0.f : top;
+    const float f0 = ex2(m - z), f1 = ex2(x.m - z);
+    m = top;
+    l = fmaf(f0, l, f1 * x.l);
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = fmaf(f0, o[e], f1 * x.o[e]);
+  }
+  // what the prefix pass left for this row (nothing where `there` is false)
+  template <int D>
+  __device__ __forceinline__ void prefix(const SharedPrefix& s, int q_heads, int slot, int h, int d, bool there) {
+    none();
+    if (!there) return;
+    const float* st = s.state + (static_cast<int64_t>(slot) * q_heads + h) * (D + 4);
+    const float2 ml = *reinterpret_cast<const float2*>(st + D);
+    m = ml.x;
+    l = ml.y;
+#pragma unroll
+    for (int e = 0; e < E; e += 2) {
+      const float2 y = *reinterpret_cast<const float2*>(st + d + e);
+      o[e] = y.x;
+      o[e + 1] = y.y;
+    }
+  }
+  template <typename T, int D>
+  __device__ __forceinline__ void store(const Attend& a, int slot, int h, int d) const {
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    uint32_t y[E / 2];
+#pragma unroll
+    for (int e = 0; e < E / 2; ++e) y[e] = Half16<T>::pack(o[2 * e] * inv, o[2 * e + 1] * inv);
+    uint16_t* out = a.out + slot * a.out_row + static_cast<int64_t>(h) * D + d;
+    if constexpr (E == 8) {
+      *reinterpret_cast<uint4*>(out) = make_uint4(y[0], y[1], y[2], y[3]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < E / 2; ++e) *reinterpret_cast<uint32_t*>(out + 2 * e) = y[e];
+    }
+    if (d == 0 && a.lse != nullptr) a.lse[static_cast<int64_t>(slot) * a.q_heads + h] = (m + log2f(l)) * kLn2;
+  }
+};
 
 // Not the read-only path: the launch before this one may have written the
 // cache, and this kernel may already have been scheduled by then.
@@ -96,7 +131,8 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(D, NB))
     int n = 0;
 #pragma unroll 8
     for (int i = i0; i < i1; ++i) {
-      const int x = tiles_of(i).n;
+      const int tiles = tiles_of(i).n;
+      const int x = tiles > 0 ? tiles + kUnitCost : 0;
       tiles_before[i] = x;
       n += x;
     }
@@ -130,8 +166,12 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(D, NB))
   // slots without a key in reach here
   for (int i = blockIdx.x; i < a.rows; i += gridDim.x) {
     if (tiles_before[i + 1] != tiles_before[i]) continue;
-    for (int e = tid; e < a.q_heads * (D / 2); e += kStepThreads)
-      finish_row<T, D>(a, shared, i, e / (D / 2), 2 * (e % (D / 2)), -CUDART_INF_F, 0.f, 0.f, 0.f);
+    const bool there = shared.base != nullptr && shared.base[i] > 0;
+    for (int e = tid; e < a.q_heads * (D / 8); e += kStepThreads) {
+      RowPart<8> r;
+      r.prefix<D>(shared, a.q_heads, i, e / (D / 8), 8 * (e % (D / 8)), there);
+      r.store<T, D>(a, i, e / (D / 8), 8 * (e % (D / 8)));
+    }
   }
 
   int64_t x = me * per;
@@ -139,7 +179,8 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(D, NB))
   if (lane == 0) ws.cut[me] = make_int4(0, 0, 0, 0);
   if (x >= x_end) return;
   const int64_t x_first = x;
-  int slot;
+  int slot, head, block, t0, t1;
+  int64_t unit_x;  // where the unit begins on the line; its tile i lies at unit_x + kUnitCost + i
   {
     int lo = 0, hi = a.rows;  // the last slot whose tiles begin at or before x
     while (hi - lo > 1) {
@@ -147,29 +188,38 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(D, NB))
       if (static_cast<int64_t>(tiles_before[mid]) * units <= x) lo = mid; else hi = mid;
     }
     slot = lo;
-  }
-  while (x < x_end) {
-    while (static_cast<int64_t>(tiles_before[slot + 1]) * units <= x) ++slot;
-    const SeenTiles seen = tiles_of(slot);
     const int64_t slot_x = static_cast<int64_t>(tiles_before[slot]) * units;
-    const int unit = static_cast<int>((x - slot_x) / seen.n);
-    const int64_t unit_x = slot_x + static_cast<int64_t>(unit) * seen.n;
-    const int t0 = static_cast<int>(x - unit_x);
-    const int t1 = static_cast<int>(min(static_cast<int64_t>(seen.n), x_end - unit_x));
-    const int head = unit / blocks, block = unit % blocks;
+    const int n = tiles_before[slot + 1] - tiles_before[slot];
+    const int unit = static_cast<int>((x - slot_x) / n);
+    head = unit / blocks;
+    block = unit - head * blocks;
+    unit_x = slot_x + static_cast<int64_t>(unit) * n;
+  }
+  SeenTiles seen = tiles_of(slot);
+  int base_tokens = shared.base != nullptr ? shared.base[slot] : 0;
+  uint4 q[NB][KC];
+  int page[NT];
+  // the unit's share, its queries and its first pages
+  auto enter = [&] {
+    t0 = static_cast<int>(max(x - unit_x - kUnitCost, static_cast<int64_t>(0)));
+    t1 = static_cast<int>(max(min(static_cast<int64_t>(seen.n), x_end - unit_x - kUnitCost), static_cast<int64_t>(0)));
+    const int queries = min(NQ, a.group - block * NQ);
+    const int64_t q_at = slot * a.q_row + static_cast<int64_t>(head * a.group + block * NQ + g) * D + 8 * t;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int k = 0; k < KC; ++k) q[b][k] = load16(a.q + q_at + 8 * b * D + 32 * k, 8 * b + g < queries);
+    const int32_t* row = c.table + static_cast<int64_t>(slot) * c.table_pages;
+#pragma unroll
+    for (int u = 0; u < NT; ++u) page[u] = t0 + u < t1 ? row[(16 * seen.tile(t0 + u)) >> c.page_shift] : -1;
+  };
+  enter();
+  while (true) {
     const int queries = min(NQ, a.group - block * NQ);
     const int q_head = head * a.group + block * NQ;
     const int32_t* row = c.table + static_cast<int64_t>(slot) * c.table_pages;
     const bool* mask = a.key_mask != nullptr ? a.key_mask + slot * a.mask_stride : nullptr;
     const int64_t head_at = static_cast<int64_t>(head) * c.page_size * D;
-
-    uint4 q[NB][KC];
-#pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-      for (int k = 0; k < KC; ++k)
-        q[b][k] = load16(a.q + slot * a.q_row + static_cast<int64_t>(q_head + 8 * b + g) * D + 8 * (t + 4 * k),
-                         8 * b + g < queries);
     float m[NB][2], l[NB][2], acc[NB][VC][4][4];
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
@@ -181,12 +231,6 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(D, NB))
         for (int w = 0; w < 4; ++w) acc[b][v][w][0] = acc[b][v][w][1] = acc[b][v][w][2] = acc[b][v][w][3] = 0.f;
     }
 
-    int page[NT];
-#pragma unroll
-    for (int u = 0; u < NT; ++u) {
-      const int tt = t0 + u;
-      page[u] = tt < t1 ? row[(16 * seen.tile(tt)) >> c.page_shift] : -1;
-    }
     for (int base = t0; base < t1; base += NT) {
       // keys in reach: one per lane
       const int my_tile = base + (lane >> 4);
@@ -287,8 +331,39 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(D, NB))
     }
 
     // a thread holds queries 2t, 2t + 1 and dims 8g .. 8g + 7 of each 64
-    const bool whole = t0 == 0 && t1 == seen.n;
-    float* part = ws.part + (2 * static_cast<int64_t>(me) + (x == x_first ? 0 : 1)) * NQ * (D + 2);
+    const bool whole = t0 == 0 && t1 == seen.n, some = t0 < t1;
+    const bool there = base_tokens > 0 && whole;
+    RowPart<8> before[2][VC];  // of the first 8 queries: on their way while the next unit is entered
+    if (NB == 1) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int v = 0; v < VC; ++v)
+          before[i][v].template prefix<D>(shared, a.q_heads, slot, q_head + 2 * t + i, 64 * v + 8 * g,
+                                          there && 2 * t + i < queries);
+    }
+    // of a cut unit: the share's part 0 when the unit is its first, else part 1
+    const int my_part = x_first >= unit_x ? 0 : 1;
+    float* part = ws.part + (2 * static_cast<int64_t>(me) + my_part) * NQ * (D + 2);
+    if (t0 == 0 && some && !whole && lane == 0)
+      ws.cut[me] = make_int4(slot, head * blocks + block,
+                             static_cast<int>((unit_x + kUnitCost + seen.n - 1) / per) - me + 1, my_part);
+    const int my_slot = slot;
+    x = unit_x + kUnitCost + seen.n;
+    const bool more = x < x_end;
+    if (more) {
+      unit_x = x;
+      if (++block == blocks) {
+        block = 0;
+        if (++head == c.kv_heads) {
+          head = 0;
+          do ++slot; while (tiles_before[slot + 1] == tiles_before[slot]);
+          seen = tiles_of(slot);
+          base_tokens = shared.base != nullptr ? shared.base[slot] : 0;
+        }
+      }
+      enter();
+    }
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
 #pragma unroll
@@ -299,63 +374,93 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(D, NB))
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int qi = 8 * b + 2 * t + i;
-        if (qi >= queries) continue;
+        if (qi < queries && some) {
 #pragma unroll
-        for (int v = 0; v < VC; ++v) {
+          for (int v = 0; v < VC; ++v) {
+            const int d = 64 * v + 8 * g;
+            RowPart<8> r;
+            r.m = m[b][i];
+            r.l = l[b][i];
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const int d = 64 * v + 8 * g + 2 * w;
+            for (int w = 0; w < 4; ++w) {
+              r.o[2 * w] = acc[b][v][w][i];
+              r.o[2 * w + 1] = acc[b][v][w][2 + i];
+            }
             if (whole) {
-              finish_row<T, D>(a, shared, slot, q_head + qi, d, m[b][i], l[b][i], acc[b][v][w][i], acc[b][v][w][2 + i]);
+              if (there) {
+                if (NB > 1) before[i][v].template prefix<D>(shared, a.q_heads, my_slot, q_head + qi, d, true);
+                r.join(before[i][v]);
+              }
+              r.template store<T, D>(a, my_slot, q_head + qi, d);
             } else {
-              *reinterpret_cast<float2*>(part + qi * (D + 2) + d) = make_float2(acc[b][v][w][i], acc[b][v][w][2 + i]);
+#pragma unroll
+              for (int w = 0; w < 4; ++w)
+                *reinterpret_cast<float2*>(part + qi * (D + 2) + d + 2 * w) = make_float2(r.o[2 * w], r.o[2 * w + 1]);
+              if (d == 0) *reinterpret_cast<float2*>(part + qi * (D + 2) + D) = make_float2(r.m, r.l);
             }
           }
         }
-        if (!whole && g == 0) *reinterpret_cast<float2*>(part + qi * (D + 2) + D) = make_float2(m[b][i], l[b][i]);
       }
     }
-    if (!whole && t0 == 0 && lane == 0)
-      ws.cut[me] = make_int4(slot, unit, static_cast<int>((unit_x + seen.n - 1) / per) - me + 1, x == x_first ? 0 : 1);
-    x = unit_x + t1;
+    if (!more) break;
   }
 }
 
-// Joins the parts of the units that a cut divided: `threads` threads (a
-// multiple of 32) for the unit that begins in one warp's share.
+// Joins the parts of the units that a cut divided.  CTA x looks after the
+// units that begin in kJoinShares warps' shares, CTA y after 128 of their
+// (query, pair of dims).
+constexpr int kJoinShares = kStepWarps;
+constexpr int kJoinChunk = 16;  // parts on their way at a time
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kStepThreads)
-    step_join_kernel(Attend a, SharedPrefix shared, StepSpace ws, int shares, int nq, int blocks, int threads) {
+    step_join_kernel(Attend a, SharedPrefix shared, StepSpace ws, int nq, int blocks) {
   wait_prior_grid();
-  const int me = blockIdx.x * (kStepThreads / threads) + threadIdx.x / threads;
-  if (me >= shares) return;
-  const int4 cut = ws.cut[me];
-  if (cut.z == 0) return;
-  const int head = cut.y / blocks, block = cut.y % blocks;
-  const int queries = min(nq, a.group - block * nq);
-  // the first part lies where the warp left it, the others are their warps' first units
+  int4 cuts[kJoinShares];
+#pragma unroll
+  for (int s = 0; s < kJoinShares; ++s) cuts[s] = ws.cut[blockIdx.x * kJoinShares + s];
+  const int e = blockIdx.y * kStepThreads + threadIdx.x;
+  const int qi = e / (D / 2), d = 2 * (e % (D / 2));
   const int64_t stride = static_cast<int64_t>(nq) * (D + 2);
-  const float* first = ws.part + (2 * static_cast<int64_t>(me) + cut.w) * stride;
-  const float* rest = ws.part + 2 * static_cast<int64_t>(me) * stride;
-  for (int e = threadIdx.x % threads; e < queries * (D / 2); e += threads) {
-    const int qi = e / (D / 2), d = 2 * (e % (D / 2));
-    float2 ml = __ldcg(reinterpret_cast<const float2*>(first + qi * (D + 2) + D));
-    float2 y = __ldcg(reinterpret_cast<const float2*>(first + qi * (D + 2) + d));
-    float top = ml.x, sum = ml.y, o0 = y.x, o1 = y.y;
-#pragma unroll 4
-    for (int k = 1; k < cut.z; ++k) {
-      const float* p = rest + 2 * k * stride + qi * (D + 2);
-      ml = __ldcg(reinterpret_cast<const float2*>(p + D));
-      y = __ldcg(reinterpret_cast<const float2*>(p + d));
-      const float both = fmaxf(top, ml.x);
-      const float z = both == -CUDART_INF_F ? 0.f : both;
-      const float f0 = ex2(top - z), f1 = ex2(ml.x - z);
-      sum = fmaf(f0, sum, f1 * ml.y);
-      o0 = fmaf(f0, o0, f1 * y.x);
-      o1 = fmaf(f0, o1, f1 * y.y);
-      top = both;
+#pragma unroll
+  for (int s = 0; s < kJoinShares; ++s) {
+    const int4 cut = cuts[s];
+    const int head = cut.y / blocks, block = cut.y % blocks;
+    if (cut.z == 0 || qi >= min(nq, a.group - block * nq)) continue;
+    // the first part lies where the warp left it, the others are their warps' first units
+    const float* parts = ws.part + 2 * static_cast<int64_t>(blockIdx.x * kJoinShares + s) * stride + qi * (D + 2);
+    RowPart<2> r, before;
+    const int h = head * a.group + block * nq + qi;
+    before.prefix<D>(shared, a.q_heads, cut.x, h, d, shared.base != nullptr && shared.base[cut.x] > 0);
+    r.none();
+    for (int k0 = 0; k0 < cut.z; k0 += kJoinChunk) {
+      float2 ml[kJoinChunk], y[kJoinChunk];
+#pragma unroll
+      for (int k = 0; k < kJoinChunk; ++k) {
+        const float* p = parts + (k0 + k == 0 ? cut.w : 2 * (k0 + k)) * stride;
+        const bool on = k0 + k < cut.z;
+        ml[k] = on ? __ldcg(reinterpret_cast<const float2*>(p + D)) : make_float2(-CUDART_INF_F, 0.f);
+        y[k] = on ? __ldcg(reinterpret_cast<const float2*>(p + d)) : make_float2(0.f, 0.f);
+      }
+      float top = r.m;
+#pragma unroll
+      for (int k = 0; k < kJoinChunk; ++k) top = fmaxf(top, ml[k].x);
+      const float z = top == -CUDART_INF_F ? 0.f : top;
+      const float keep = ex2(r.m - z);
+      r.m = top;
+      r.l *= keep;
+      r.o[0] *= keep;
+      r.o[1] *= keep;
+#pragma unroll
+      for (int k = 0; k < kJoinChunk; ++k) {
+        const float f = ex2(ml[k].x - z);
+        r.l = fmaf(f, ml[k].y, r.l);
+        r.o[0] = fmaf(f, y[k].x, r.o[0]);
+        r.o[1] = fmaf(f, y[k].y, r.o[1]);
+      }
     }
-    finish_row<T, D>(a, shared, cut.x, head * a.group + block * nq + qi, d, top, sum, o0, o1);
+    r.join(before);
+    r.store<T, D>(a, cut.x, h, d);
   }
 }
 
@@ -392,9 +497,8 @@ cudaError_t launch_step(const PagedCache& c, int dtype, const Attend& a, const S
   if (sms <= 0 || sms > kMaxSms) return cudaErrorInvalidValue;
   const size_t smem = 4 * (static_cast<size_t>(a.rows) + 1);
   const int grid = sms * step_ctas(c.head_dim, nb), shares = grid * kStepWarps;
-  const int min_tiles = step_tiles(c.head_dim);
+  const int min_tiles = kUnitCost + step_tiles(c.head_dim);
   const int pairs = std::min(8 * nb, a.group) * c.head_dim / 2;
-  const int threads = pairs <= 32 ? 32 : pairs <= 64 ? 64 : 128;
   auto go = [&](auto kernel, auto join) {
     if (smem > 40 * 1024) {
       const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -404,9 +508,8 @@ cudaError_t launch_step(const PagedCache& c, int dtype, const Attend& a, const S
     cudaError_t e = launch_serialized(kernel, dim3(grid), dim3(kStepThreads), smem, stream, c, a, shared, ws, blocks,
                                       min_tiles);
     if (e != cudaSuccess) return e;
-    const int per_block = kStepThreads / threads;
-    return launch_serialized(join, dim3((shares + per_block - 1) / per_block), dim3(kStepThreads), 0, stream, a,
-                             shared, ws, shares, 8 * nb, blocks, threads);
+    return launch_serialized(join, dim3(shares / kJoinShares, (pairs + kStepThreads - 1) / kStepThreads),
+                             dim3(kStepThreads), 0, stream, a, shared, ws, 8 * nb, blocks);
   };
   auto pick = [&](auto type) {
     using T = decltype(type);
