@@ -12,7 +12,8 @@
 // A unit is a key head and two Q tiles of 128 rows; a tile's rows are the
 // group's query heads of consecutive tokens (128 / group of them), so shared
 // key heads fill the MMA's 128 rows and every key tile in shared memory is
-// used by both Q tiles.  Warp roles (320 threads, one CTA per SM):
+// used by both Q tiles.  Warp roles (384 threads, one CTA per SM; the softmax warps take registers over
+// from the others):
 //   warps 0-3, 4-7  softmax of Q tile 0 / 1: one thread per row reads S from
 //                   tensor memory, writes P over it in 16 bits (the A operand
 //                   of the second product), rescales O when needed, and
@@ -37,7 +38,7 @@ namespace {
 
 constexpr int kTile = 128;          // rows of a Q tile, keys of a key tile
 constexpr int kPairRows = 2 * kTile;
-constexpr int kPromptThreads = 320;
+constexpr int kPromptThreads = 384;
 constexpr int kPromptPlanThreads = 1024;
 constexpr int kMinShare = 2;        // key tiles a CTA takes at least
 constexpr int kMaxSms = 160;        // workspaces are sized for the largest device
@@ -62,18 +63,25 @@ struct PromptRows {
   float* state;              // prefix pass: [slots][q_heads][D + 4]: O, m, l of each member
 };
 
-// One pair of Q tiles: slot (or group), first token (or member), key tiles, key tiles of the pairs before.
+// A unit's place on the line: its key tiles, and before them what entering and
+// leaving it costs, in key tiles.
+constexpr int kPairCost = 2;
+
 struct PromptSpace {
-  int64_t* head;       // [0] pairs, [1] key tiles of one key head, [2] key tiles per CTA
-  int32_t* cta_pair;   // [kMaxSms + 1] the pair that holds CTA c's first tile
+  int64_t* head;       // [0] pairs, [1] length of one key head's line, [2] length of a share
+  int32_t* cta_pair;   // [kMaxSms + 1] the pair that holds the start of CTA c's share
   int32_t* first;      // [n + 1] pairs of the slots before
-  int4* rec;           // [pairs]
+  int4* rec;           // [2 * pairs]: first token (or member), 0, key tiles, place on the line; then Geom
   float* part;         // [CTAs][2][D + 2][256]
 };
 
-// Where a pair's rows and keys are.
-struct PairGeom {
-  int count, len, row0, key_slot;
+// Where a pair's rows and keys are: rows [row0, row0 + count) are the slot's
+// (or group's), its keys the first len tokens of key_slot.
+struct Geom {
+  int row0, count, len, key_slot;
+};
+
+struct PairGeom : Geom {
   bool ok;
   __device__ __forceinline__ PairGeom(const PagedCache& c, const PromptRows& r, int i) {
     const int a = r.offsets[i], b = r.offsets[i + 1];
@@ -121,14 +129,14 @@ __device__ __forceinline__ bool tile_full(int j, int p0, int p1, int window, int
 
 // Positions [p0, p1] of the rows of tokens [t0, t1); empty when p1 < p0.  In
 // the prefix pass every row stands at the prefix's end.
-__device__ __forceinline__ void positions(const PairGeom& g, bool prefix, int t0, int t1, int* p0, int* p1) {
+__device__ __forceinline__ void positions(const Geom& g, bool prefix, int t0, int t1, int* p0, int* p1) {
   t1 = min(t1, g.count);
   if (prefix) {
     *p1 = g.len - 1;
     *p0 = t0 < t1 && g.len > 0 ? g.len - 1 : g.len;
   } else {
     *p0 = g.len - g.count + t0;
-    *p1 = g.ok ? g.len - g.count + t1 - 1 : *p0 - 1;
+    *p1 = g.len >= g.count ? g.len - g.count + t1 - 1 : *p0 - 1;  // a slot with more rows than tokens: none
   }
 }
 
@@ -204,29 +212,32 @@ __global__ void __launch_bounds__(kPromptPlanThreads)
   int tiles = 0;
   for (int base = 0; base < pairs; base += kPromptPlanThreads) {
     const int k = base + tid;
-    int n = 0, i = 0, tok0 = 0;
+    int n = 0, tok0 = 0;
+    Geom geom{0, 0, 0, 0};
     if (k < pairs) {
       int lo = 0, hi = rows.n;  // the last slot whose pairs begin at or before k
       while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
         if (ws.first[mid] <= k) lo = mid; else hi = mid;
       }
-      i = lo;
-      tok0 = (k - ws.first[i]) * tokens_per_pair;
-      const PairGeom g(c, rows, i);
+      tok0 = (k - ws.first[lo]) * tokens_per_pair;
+      geom = PairGeom(c, rows, lo);
       int p0, p1;
-      positions(g, prefix, tok0, tok0 + tokens_per_pair, &p0, &p1);
+      positions(geom, prefix, tok0, tok0 + tokens_per_pair, &p0, &p1);
       // rows that see nothing still need their zeros written: one tile without keys
       n = p0 <= p1 ? KeySpan(p0, p1, window, sinks).n : (prefix ? 0 : 1);
     }
     int total;
-    const int before = tiles + plan_scan(n, &total);
-    if (k < pairs) ws.rec[k] = make_int4(i, tok0, n, before);
+    const int before = tiles + plan_scan(n > 0 ? n + kPairCost : 0, &total);
+    if (k < pairs) {
+      ws.rec[2 * k] = make_int4(tok0, 0, n, before);
+      ws.rec[2 * k + 1] = make_int4(geom.row0, geom.count, geom.len, geom.key_slot);
+    }
     tiles += total;
   }
   __syncthreads();
   const int64_t all = static_cast<int64_t>(tiles) * c.kv_heads;
-  const int64_t per = max((all + ctas - 1) / ctas, static_cast<int64_t>(kMinShare));
+  const int64_t per = max((all + ctas - 1) / ctas, static_cast<int64_t>(kMinShare + kPairCost));
   if (tid == 0) {
     ws.head[0] = pairs;
     ws.head[1] = tiles;
@@ -237,7 +248,7 @@ __global__ void __launch_bounds__(kPromptPlanThreads)
     int lo = 0, hi = pairs;  // the last pair that begins at or before x (pairs without tiles are never last)
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
-      if (ws.rec[mid].w <= x) lo = mid; else hi = mid;
+      if (ws.rec[2 * mid].w <= x) lo = mid; else hi = mid;
     }
     ws.cta_pair[tid] = lo;
   }
@@ -249,49 +260,53 @@ __global__ void __launch_bounds__(kPromptPlanThreads)
 
 struct Walk {
   int64_t x, end, per;
-  int tiles, pairs, head, pair;
-  int4 rec;
-  int t0, t1;       // key tiles of the unit in this share
-  int64_t unit_x;   // where the unit begins on the line
-  bool first;       // the share's first unit
+  int line, pairs, head, pair;
+  int tok0, n;      // the unit's first token (or member) and key tiles
+  Geom g;
+  int t0, t1;       // its key tiles in this share
+  int64_t unit_x;   // where it begins on the line
 
   __device__ __forceinline__ bool begin(const PromptSpace& ws, int kv_heads, int cta) {
     pairs = static_cast<int>(ws.head[0]);
-    tiles = static_cast<int>(ws.head[1]);
+    line = static_cast<int>(ws.head[1]);
     per = ws.head[2];
-    const int64_t all = static_cast<int64_t>(tiles) * kv_heads;
     x = cta * per;
-    end = min(all, x + per);
+    end = min(static_cast<int64_t>(line) * kv_heads, x + per);
     if (x >= end) return false;
-    head = static_cast<int>(x / tiles);
+    head = static_cast<int>(x / line);
     pair = ws.cta_pair[cta];
-    first = true;
-    load(ws);
-    return true;
+    return load(ws);
   }
   __device__ __forceinline__ bool next(const PromptSpace& ws) {
-    x = unit_x + t1;
+    x = unit_x + kPairCost + n;
     if (x >= end) return false;
-    first = false;
     ++pair;
-    load(ws);
-    return true;
+    return load(ws);
   }
-  __device__ __forceinline__ void load(const PromptSpace& ws) {
+  // false when the share ends before the unit's first key tile
+  __device__ __forceinline__ bool load(const PromptSpace& ws) {
+    int4 rec;
     while (true) {
       if (pair >= pairs) {
         pair = 0;
         ++head;
       }
-      rec = ws.rec[pair];
+      rec = ws.rec[2 * pair];
       if (rec.z > 0) break;
       ++pair;
     }
-    unit_x = static_cast<int64_t>(head) * tiles + rec.w;
-    t0 = static_cast<int>(x - unit_x);
-    t1 = static_cast<int>(min(static_cast<int64_t>(rec.z), end - unit_x));
+    const int4 at = ws.rec[2 * pair + 1];
+    tok0 = rec.x;
+    n = rec.z;
+    g = Geom{at.x, at.y, at.z, at.w};
+    unit_x = static_cast<int64_t>(head) * line + rec.w;
+    t0 = static_cast<int>(max(x - unit_x - kPairCost, static_cast<int64_t>(0)));
+    t1 = static_cast<int>(min(static_cast<int64_t>(n), end - unit_x - kPairCost));
+    return t1 > 0;
   }
-  __device__ __forceinline__ bool whole() const { return t0 == 0 && t1 == rec.z; }
+  __device__ __forceinline__ bool whole() const { return t0 == 0 && t1 == n; }
+  // which of its CTA's two parts a cut unit leaves
+  __device__ __forceinline__ int part(int cta) const { return cta * per >= unit_x ? 0 : 1; }
 };
 
 // 128-byte-swizzled MN-major operand (values: [keys][64 dims] rows of 128
@@ -337,6 +352,28 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32
       : "memory");
 }
 
+// Two f32 operations in one instruction.
+__device__ __forceinline__ uint64_t bits2(float2 v) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(v.x), "f"(v.y));
+  return r;
+}
+__device__ __forceinline__ float2 pair2(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(bits2(a)), "l"(bits2(b)), "l"(bits2(c)));
+  return pair2(d);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits2(a)), "l"(bits2(b)));
+  return pair2(d);
+}
+
 // Warp-uniform forms: a wait succeeds, and the CTA goes on, for all lanes or none.
 __device__ __forceinline__ bool wait_warp(unsigned long long* bar, uint32_t parity) {
   return __all_sync(0xffffffffu, mbar_wait_cta(bar, parity));
@@ -359,7 +396,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   using C = PromptCfg<D>;
   constexpr int S = C::kStages;
   constexpr int DB = D / 64;  // 64-dim blocks of a tile
-  constexpr uint32_t kSCol = 0, kOCol = 2 * kTile;
+  constexpr uint32_t kSCol = 0, kPCol = kTile / 2, kOCol = 2 * kTile;  // P over the second half of S
   extern __shared__ unsigned char prompt_smem[];
   __shared__ unsigned long long kv_full[S], kv_empty[S], q_ready[2], s_full[2], p_full[2], o_full[2], fin;
   __shared__ uint32_t tmem_base;
@@ -402,21 +439,28 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   Walk w;
   const bool any = w.begin(ws, c.kv_heads, blockIdx.x);
 
+  // registers: 384 threads x 168 at launch = 128 x 88 + 2 x 128 x 208
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
   if (warp == 9) {
     // ---- TMA producer: per key tile its keys, then its values
     int it = 0;
     const int boxes = kTile >> c.page_shift;  // pages per tile
     const int beyond = c.pages * c.layers * 2 * c.kv_heads * c.page_size;  // a row past the pool: reads zeros
     for (bool more = any; more && alive(errv); more = w.next(ws)) {
-      const PairGeom g(c, rows, w.rec.x);
+      const Geom g = w.g;
       int p0, p1;
-      positions(g, prefix, w.rec.y, w.rec.y + 2 * tq, &p0, &p1);
+      positions(g, prefix, w.tok0, w.tok0 + 2 * tq, &p0, &p1);
       const KeySpan span(p0, max(p0, p1), a.window, a.sinks);
       const int32_t* table = c.table + static_cast<int64_t>(g.key_slot) * c.table_pages;
-      for (int t = w.t0; t < w.t1; ++t) {
+      auto page_of = [&](int t) {
         const int first_key = kTile * span.tile(t) + (lane << c.page_shift);
-        int page = -1;
-        if (lane < boxes && first_key < g.len) page = table[first_key >> c.page_shift];
+        return lane < boxes && t < w.t1 && first_key < g.len ? table[first_key >> c.page_shift] : -1;
+      };
+      int ahead = page_of(w.t0);
+      for (int t = w.t0; t < w.t1; ++t) {
+        const int page = ahead;
+        ahead = page_of(t + 1);  // on its way while this tile's copies wait for their stage
         for (int kv = 0; kv < 2; ++kv, ++it) {
           const int s = it % S;
           if (it >= S && !wait_warp(&kv_empty[s], ((it / S) - 1) & 1)) *errv = 1;
@@ -444,11 +488,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     int p_uses[2] = {0, 0}, q_uses = 0;
     const uint32_t idesc_s = prompt_idesc<T>(kTile, false), idesc_o = prompt_idesc<T>(D, true);
     for (bool more = any; more && alive(errv); more = w.next(ws), ++q_uses) {
-      const PairGeom g(c, rows, w.rec.x);
+      const Geom g = w.g;
       int p0, p1, q0[2], q1[2];
-      positions(g, prefix, w.rec.y, w.rec.y + 2 * tq, &p0, &p1);
-      positions(g, prefix, w.rec.y, w.rec.y + tq, &q0[0], &q1[0]);
-      positions(g, prefix, w.rec.y + tq, w.rec.y + 2 * tq, &q0[1], &q1[1]);
+      positions(g, prefix, w.tok0, w.tok0 + 2 * tq, &p0, &p1);
+      positions(g, prefix, w.tok0, w.tok0 + tq, &q0[0], &q1[0]);
+      positions(g, prefix, w.tok0 + tq, w.tok0 + 2 * tq, &q0[1], &q1[1]);
       const KeySpan span(p0, max(p0, p1), a.window, a.sinks);
       const bool* mask = a.key_mask != nullptr ? a.key_mask + g.key_slot * a.mask_stride : nullptr;
       bool ok = true, started[2] = {false, false};
@@ -468,23 +512,17 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         }
         umma_commit(&s_full[i]);
       };
-      auto key_tile = [&](int t, bool first) {  // wait for tile t's keys; the first also needs the queries
-        if (!wait_warp(&kv_full[it % S], (it / S) & 1)) return false;
-        if (first)
-          for (int i = 0; i < 2; ++i)
-            if (!wait_warp(&q_ready[i], q_uses & 1)) return false;
+      ok = wait_warp(&kv_full[it % S], (it / S) & 1);
+      for (int i = 0; i < 2 && ok; ++i) {
+        ok = wait_warp(&q_ready[i], q_uses & 1);
         tmem_fence_after_sync();
-        return true;
-      };
-      ok = key_tile(w.t0, true);
-      if (ok && lane == 0) {
-        for (int i = 0; i < 2; ++i)
+        if (ok && lane == 0) {
           if (tile_seen(span.tile(w.t0), q0[i], q1[i], a.window, a.sinks)) scores(i, it % S);
-        // a Q tile without key tiles here waits too: its warps must not run ahead of this one
-        for (int i = 0; i < 2; ++i)
+          // a Q tile without key tiles here waits too: its warps must not run ahead of this one
           if (last[i] < 0) umma_commit(&o_full[i]);
-        umma_commit(&kv_empty[it % S]);
+        }
       }
+      if (ok && lane == 0) umma_commit(&kv_empty[it % S]);
       ++it;
       for (int t = w.t0; ok && t < w.t1; ++t) {
         const int vs = it % S;
@@ -512,8 +550,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         int ks = 0;
         if (next) {
           ks = it % S;
-          ok = key_tile(t + 1, false);
+          ok = wait_warp(&kv_full[ks], (it / S) & 1);
           if (!ok) break;
+          tmem_fence_after_sync();
           ++it;
         }
         for (int i = 0; i < 2 && ok; ++i) {
@@ -526,7 +565,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
               const uint64_t vd = value_desc(smem_addr(ring + static_cast<size_t>(vs) * C::kTileBytes));
 #pragma unroll
               for (int kk = 0; kk < kTile / 16; ++kk)
-                umma_ts(tmem + kOCol + i * D, tmem + kSCol + i * kTile + 8 * kk, vd + kk * (2048 >> 4), idesc_o,
+                umma_ts(tmem + kOCol + i * D, tmem + kSCol + i * kTile + kPCol + 8 * kk, vd + kk * (2048 >> 4), idesc_o,
                         started[i] || kk != 0);
             }
             started[i] = true;
@@ -549,46 +588,59 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       umma_commit(&fin);
       mbar_wait_cta(&fin, 0);
     }
+  }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     // ---- softmax of Q tile i: thread r is its row r
     const int i = warp >> 2, r = threadIdx.x & 127;
     const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
     const uint32_t s_col = tmem + kSCol + i * kTile + lanes, o_col = tmem + kOCol + i * D + lanes;
     const int tok_in_tile = r / a.group, head_in_group = r % a.group;
     int s_uses = 0, o_uses = 0;
-    for (bool more = any; more && alive(errv); more = w.next(ws)) {
-      const PairGeom g(c, rows, w.rec.x);
-      const int tok = w.rec.y + i * tq + tok_in_tile;
-      const bool valid = tok_in_tile < tq && tok < g.count;
-      int q_row = valid ? g.row0 + tok : 0;
-      if (prefix && valid) q_row = rows.members[q_row];
-      const bool there = valid && (!prefix || (q_row >= 0 && q_row < a.rows));
-      const int q_head = w.head * a.group + head_in_group;
-      {
-        const uint16_t* src = a.q + q_row * a.q_row + static_cast<int64_t>(q_head) * D;
-        unsigned char* dst = q_smem + i * C::kTileBytes + r * 128;
+    // this thread's row of unit u: q and out row, or -1
+    auto row_of = [&](const Walk& u) {
+      const int tok = u.tok0 + i * tq + tok_in_tile;
+      if (tok_in_tile >= tq || tok >= u.g.count) return -1;
+      const int row = u.g.row0 + tok;
+      if (!prefix) return row;
+      const int slot = rows.members[row];
+      return slot >= 0 && slot < a.rows ? slot : -1;
+    };
+    // its queries into shared memory, for the MMA warp
+    auto load_q = [&](const Walk& u, int row) {
+      const uint16_t* src = a.q + row * a.q_row + static_cast<int64_t>(u.head * a.group + head_in_group) * D;
+      unsigned char* dst = q_smem + i * C::kTileBytes + r * 128;
+      uint4 v[DB][8];
 #pragma unroll
-        for (int b = 0; b < DB; ++b) {
-          uint4 v[8];
+      for (int b = 0; b < DB; ++b)
 #pragma unroll
-          for (int k = 0; k < 8; ++k)
-            v[k] = there ? *reinterpret_cast<const uint4*>(src + 64 * b + 8 * k) : make_uint4(0, 0, 0, 0);
+        for (int k = 0; k < 8; ++k)
+          v[b][k] = row >= 0 ? *reinterpret_cast<const uint4*>(src + 64 * b + 8 * k) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) *reinterpret_cast<uint4*>(dst + b * (kTile * 128) + 16 * (k ^ (r & 7))) = v[k];
-        }
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&q_ready[i]);
-      }
+      for (int b = 0; b < DB; ++b)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) *reinterpret_cast<uint4*>(dst + b * (kTile * 128) + 16 * (k ^ (r & 7))) = v[b][k];
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_ready[i]);
+    };
+    int q_row = -1;
+    if (any) {
+      q_row = row_of(w);
+      load_q(w, q_row);
+    }
+    for (bool more = any; more && alive(errv);) {
+      const Geom g = w.g;
       int p0, p1, q0, q1;
-      positions(g, prefix, w.rec.y, w.rec.y + 2 * tq, &p0, &p1);
-      positions(g, prefix, w.rec.y + i * tq, w.rec.y + (i + 1) * tq, &q0, &q1);
+      positions(g, prefix, w.tok0, w.tok0 + 2 * tq, &p0, &p1);
+      positions(g, prefix, w.tok0 + i * tq, w.tok0 + (i + 1) * tq, &q0, &q1);
       const KeySpan span(p0, max(p0, p1), a.window, a.sinks);
-      const int pos = prefix ? g.len - 1 : g.len - g.count + tok;
+      const int pos = prefix ? g.len - 1 : g.len - g.count + w.tok0 + i * tq + tok_in_tile;
       const bool* mask = a.key_mask != nullptr ? a.key_mask + g.key_slot * a.mask_stride : nullptr;
-      float m = -CUDART_INF_F, l = 0.f;
+      float m = -CUDART_INF_F;
+      float2 l2 = make_float2(0.f, 0.f);
       bool ok = true, started = false;
-      for (int t = w.t0; t < w.t1 && ok; ++t) {
+      for (int t = w.t0; t < w.t1; ++t) {
         const int j = span.tile(t);
         if (!tile_seen(j, q0, q1, a.window, a.sinks)) continue;
         const int base = kTile * j;
@@ -611,58 +663,91 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         ++s_uses;
         if (!ok) break;
         tmem_fence_after_sync();
-        uint32_t s[2][64];
-        tmem_ld64(s[0], s_col);
-        tmem_ld64(s[1], s_col + 64);
-        if (!all) {
+        // 64 of the 128 scores at a time: the first half is read again after
+        // the maximum is known, which costs less than the registers to hold it
+        uint32_t s[64];
+        auto half = [&](int x) {
+          tmem_ld64(s, s_col + 64 * x);
+          if (!all) {
 #pragma unroll
-          for (int k = 0; k < 128; ++k)
-            if (!((see[k >> 5] >> (k & 31)) & 1u)) s[k >> 6][k & 63] = 0xff800000u;
+            for (int k = 0; k < 64; ++k)
+              if (!((see[2 * x + (k >> 5)] >> (k & 31)) & 1u)) s[k] = 0xff800000u;
+          }
+        };
+        float tops[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) tops[k] = m;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          half(x);
+#pragma unroll
+          for (int k = 0; k < 64; ++k) tops[k & 7] = fmaxf(tops[k & 7], __uint_as_float(s[k]));
         }
-        float top = m;
-#pragma unroll
-        for (int k = 0; k < 128; ++k) top = fmaxf(top, __uint_as_float(s[k >> 6][k & 63]));
+        const float top = fmaxf(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])),
+                                fmaxf(fmaxf(tops[4], tops[5]), fmaxf(tops[6], tops[7])));
         // the maximum in use moves only when it must
         const bool move = m == -CUDART_INF_F ? top > m : (top - m) * a.scale2 > 8.f;
         if (__any_sync(0xffffffffu, move)) {
           if (started && __any_sync(0xffffffffu, move && m != -CUDART_INF_F)) {
             const float f = move && m != -CUDART_INF_F ? ex2((m - top) * a.scale2) : 1.f;
-            l *= f;
+            l2.x *= f;
+            l2.y *= f;
 #pragma unroll
-            for (int b = 0; b < D / 32; ++b) {
-              uint32_t o[32];
-              tmem_ld32(o, o_col + 32 * b);
+            for (int b = 0; b < D / 16; ++b) {
+              uint32_t o[16];
+              tmem_ld16(o, o_col + 16 * b);
 #pragma unroll
-              for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-              tmem_st32(o_col + 32 * b, o);
+              for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+              tmem_st16(o_col + 16 * b, o);
             }
           }
           if (move) m = top;
         }
         const float off = m == -CUDART_INF_F ? 0.f : -m * a.scale2;
+        const float2 scale = make_float2(a.scale2, a.scale2), offs = make_float2(off, off);
+        float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        // the probabilities go over the second half's scores, which are in registers by now
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          uint32_t p[32];
-          float s0 = 0.f, s1 = 0.f;
+        for (int x = 1; x >= 0; --x) {
+          if (x == 0) half(0);
 #pragma unroll
-          for (int k = 0; k < 32; ++k) {
-            const float e0 = ex2(fmaf(__uint_as_float(s[x][2 * k]), a.scale2, off));
-            const float e1 = ex2(fmaf(__uint_as_float(s[x][2 * k + 1]), a.scale2, off));
-            // the sum keeps the unrounded probabilities; the values' weights are rounded to 16 bits once
-            s0 += e0;
-            s1 += e1;
-            p[k] = Half16<T>::pack(e0, e1);
+          for (int y = 0; y < 2; ++y) {
+            uint32_t p[16];
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+              const int e = 32 * y + 2 * k;
+              float2 v = fma2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), scale, offs);
+              v.x = ex2(v.x);
+              v.y = ex2(v.y);
+              // the sum keeps the unrounded probabilities; the values' weights are rounded to 16 bits once
+              sums[k & 1] = add2(sums[k & 1], v);
+              p[k] = Half16<T>::pack(v.x, v.y);
+            }
+            tmem_st16(s_col + kPCol + 32 * x + 16 * y, p);
           }
-          l += s0 + s1;
-          tmem_st32(s_col + 32 * x, p);
         }
+        l2 = add2(l2, add2(sums[0], sums[1]));
         tmem_wait_st();
         tmem_fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[i]);
         started = true;
       }
-      if (ok) {
+      // The next unit's queries go in before this one's result comes out: the
+      // scores that used the shared memory are done.  Not before the MMA warp
+      // has taken up this unit, though, which a tile's scores (or O) show.
+      if (ok && !started) {
+        ok = wait_warp(&o_full[i], o_uses & 1);
+        ++o_uses;
+      }
+      Walk v = w;
+      more = v.next(ws);
+      int next_row = -1;
+      if (ok && more) {
+        next_row = row_of(v);
+        load_q(v, next_row);
+      }
+      if (ok && started) {
         ok = wait_warp(&o_full[i], o_uses & 1);
         ++o_uses;
         tmem_fence_after_sync();
@@ -671,10 +756,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         *errv = 1;
         break;
       }
+      const float l = l2.x + l2.y;
       const float inv = l == 0.f ? 0.f : 1.f / l;
       const float m2 = m == -CUDART_INF_F ? m : m * a.scale2;
-      const bool whole = w.whole();
-      float* part = ws.part + (2 * static_cast<int64_t>(blockIdx.x) + (w.first ? 0 : 1)) * (D + 2) * kPairRows + i * kTile + r;
+      const bool whole = w.whole(), there = q_row >= 0;
+      const int q_head = w.head * a.group + head_in_group;
+      float* part = ws.part + (2 * static_cast<int64_t>(blockIdx.x) + w.part(blockIdx.x)) * (D + 2) * kPairRows +
+                    i * kTile + r;
       float* state = prefix && there ? rows.state + (static_cast<int64_t>(q_row) * a.q_heads + q_head) * (D + 4) : nullptr;
       uint16_t* out = a.out + q_row * a.out_row + static_cast<int64_t>(q_head) * D;
 #pragma unroll
@@ -696,12 +784,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         } else {
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            uint4 v;
-            v.x = Half16<T>::pack(__uint_as_float(o[8 * k]) * inv, __uint_as_float(o[8 * k + 1]) * inv);
-            v.y = Half16<T>::pack(__uint_as_float(o[8 * k + 2]) * inv, __uint_as_float(o[8 * k + 3]) * inv);
-            v.z = Half16<T>::pack(__uint_as_float(o[8 * k + 4]) * inv, __uint_as_float(o[8 * k + 5]) * inv);
-            v.w = Half16<T>::pack(__uint_as_float(o[8 * k + 6]) * inv, __uint_as_float(o[8 * k + 7]) * inv);
-            *reinterpret_cast<uint4*>(out + 32 * b + 8 * k) = v;
+            uint4 y;
+            y.x = Half16<T>::pack(__uint_as_float(o[8 * k]) * inv, __uint_as_float(o[8 * k + 1]) * inv);
+            y.y = Half16<T>::pack(__uint_as_float(o[8 * k + 2]) * inv, __uint_as_float(o[8 * k + 3]) * inv);
+            y.z = Half16<T>::pack(__uint_as_float(o[8 * k + 4]) * inv, __uint_as_float(o[8 * k + 5]) * inv);
+            y.w = Half16<T>::pack(__uint_as_float(o[8 * k + 6]) * inv, __uint_as_float(o[8 * k + 7]) * inv);
+            *reinterpret_cast<uint4*>(out + 32 * b + 8 * k) = y;
           }
         }
         __syncwarp();
@@ -716,6 +804,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           a.lse[static_cast<int64_t>(q_row) * a.q_heads + q_head] = (m2 + log2f(l)) * kLn2;
         }
       }
+      w = v;
+      q_row = next_row;
     }
   }
   tmem_fence_before_sync();
@@ -724,33 +814,33 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     tmem_fence_after_sync();
     tmem_dealloc(tmem, 512);
   }
-  if (threadIdx.x == 0 && *errv != 0 && any && c.status != nullptr) {
-    const PairGeom g(c, rows, w.rec.x);
-    c.status[g.key_slot] = 4;
-  }
+  if (threadIdx.x == 0 && *errv != 0 && any && c.status != nullptr) c.status[w.g.key_slot] = 4;
 }
 
 // Joins the parts of the units that a boundary between CTAs cut.  Block
-// (c - 1, chunk): the unit at the start of CTA c's share, if that is the first
-// boundary inside it; 32 of its rows.
+// (c - 1, row chunk, dim chunk): the unit at the start of CTA c's share, if
+// that is the first boundary between its key tiles; 32 of its rows, 32 dims.
+constexpr int kJoinParts = 8;  // parts on their way at a time
+
 template <typename T, int D>
 __global__ void __launch_bounds__(256) prompt_join_kernel(PagedCache c, Attend a, PromptRows rows, PromptSpace ws) {
   wait_prior_grid();
   const int cta = blockIdx.x + 1;
-  const int64_t tiles = ws.head[1], per = ws.head[2];
+  const int64_t line = ws.head[1], per = ws.head[2];
   const int64_t x = cta * per;
-  if (x >= tiles * c.kv_heads) return;
-  const int head = static_cast<int>(x / tiles);
-  const int4 rec = ws.rec[ws.cta_pair[cta]];
-  const int64_t unit_x = head * tiles + rec.w;
-  if (unit_x == x || x - unit_x > per) return;  // not cut here, or cut before
-  const int last = static_cast<int>((unit_x + rec.z - 1) / per);
-  const PairGeom g(c, rows, rec.x);
+  if (x >= line * c.kv_heads) return;
+  const int head = static_cast<int>(x / line);
+  const int pair = ws.cta_pair[cta];
+  const int4 rec = ws.rec[2 * pair], at = ws.rec[2 * pair + 1];
+  const Geom g{at.x, at.y, at.z, at.w};
+  const int64_t unit_x = head * line + rec.w, tile_x = unit_x + kPairCost;
+  if (x <= tile_x || x - per > tile_x) return;  // not cut here, or cut before
+  const int n = static_cast<int>((tile_x + rec.z - 1) / per) - cta + 2;  // parts, from CTA cta - 1 on
   const bool prefix = rows.members != nullptr;
   const int tq = kTile / a.group;
   const int r = 32 * blockIdx.y + (threadIdx.x & 31);
   const int i = r / kTile, rr = r % kTile;
-  const int tok = rec.y + i * tq + rr / a.group;
+  const int tok = rec.x + i * tq + rr / a.group;
   if (rr / a.group >= tq || tok >= g.count) return;
   int q_row = g.row0 + tok;
   if (prefix) {
@@ -758,43 +848,49 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(PagedCache c, Attend a
     if (q_row < 0 || q_row >= a.rows) return;
   }
   const int q_head = head * a.group + rr % a.group;
-  constexpr int E = D / 8;  // dims per thread
-  const int d0 = E * (threadIdx.x >> 5);
-  auto part = [&](int k) {  // CTA cta - 1 holds the unit's beginning: its last unit unless its share begins there
-    const int64_t at = 2 * static_cast<int64_t>(k) + (k * per < unit_x ? 1 : 0);
-    return ws.part + at * (D + 2) * kPairRows + r;
-  };
-  float top = -CUDART_INF_F;
-  for (int k = cta - 1; k <= last; ++k) top = fmaxf(top, part(k)[D * kPairRows]);
-  const float z = top == -CUDART_INF_F ? 0.f : top;
-  float l = 0.f, o[E];
+  constexpr int E = 4;  // dims per thread
+  const int d0 = 32 * blockIdx.z + E * (threadIdx.x >> 5);
+  const int64_t stride = static_cast<int64_t>(D + 2) * kPairRows;
+  const float* parts = ws.part + 2 * (cta - 1) * stride + r;
+  const int64_t first = ((cta - 1) * per >= unit_x ? 0 : 1) * stride;
+  float top = -CUDART_INF_F, l = 0.f, o[E] = {0.f, 0.f, 0.f, 0.f};
+  for (int k0 = 0; k0 < n; k0 += kJoinParts) {
+    float m[kJoinParts], s[kJoinParts], y[kJoinParts][E];
 #pragma unroll
-  for (int e = 0; e < E; ++e) o[e] = 0.f;
-  for (int k = cta - 1; k <= last; ++k) {
-    const float* p = part(k);
-    const float f = ex2(p[D * kPairRows] - z);
-    l = fmaf(f, p[(D + 1) * kPairRows], l);
+    for (int k = 0; k < kJoinParts; ++k) {
+      const bool on = k0 + k < n;
+      const float* p = parts + (k0 + k == 0 ? first : 2 * (k0 + k) * stride);
+      m[k] = on ? __ldcg(p + D * kPairRows) : -CUDART_INF_F;
+      s[k] = on ? __ldcg(p + (D + 1) * kPairRows) : 0.f;
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = fmaf(f, p[(d0 + e) * kPairRows], o[e]);
+      for (int e = 0; e < E; ++e) y[k][e] = on ? __ldcg(p + (d0 + e) * kPairRows) : 0.f;
+    }
+    float most = top;
+#pragma unroll
+    for (int k = 0; k < kJoinParts; ++k) most = fmaxf(most, m[k]);
+    const float z = most == -CUDART_INF_F ? 0.f : most;
+    const float keep = ex2(top - z);
+    top = most;
+    l *= keep;
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] *= keep;
+#pragma unroll
+    for (int k = 0; k < kJoinParts; ++k) {
+      const float f = ex2(m[k] - z);
+      l = fmaf(f, s[k], l);
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] = fmaf(f, y[k][e], o[e]);
+    }
   }
   if (prefix) {
     float* state = rows.state + (static_cast<int64_t>(q_row) * a.q_heads + q_head) * (D + 4);
-#pragma unroll
-    for (int e = 0; e < E; ++e) state[d0 + e] = o[e];
+    *reinterpret_cast<float4*>(state + d0) = make_float4(o[0], o[1], o[2], o[3]);
     if (d0 == 0) *reinterpret_cast<float2*>(state + D) = make_float2(top, l);
     return;
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  uint16_t* out = a.out + q_row * a.out_row + static_cast<int64_t>(q_head) * D + d0;
-#pragma unroll
-  for (int e = 0; e < E; e += 8) {
-    uint4 v;
-    v.x = Half16<T>::pack(o[e] * inv, o[e + 1] * inv);
-    v.y = Half16<T>::pack(o[e + 2] * inv, o[e + 3] * inv);
-    v.z = Half16<T>::pack(o[e + 4] * inv, o[e + 5] * inv);
-    v.w = Half16<T>::pack(o[e + 6] * inv, o[e + 7] * inv);
-    *reinterpret_cast<uint4*>(out + e) = v;
-  }
+  *reinterpret_cast<uint2*>(a.out + q_row * a.out_row + static_cast<int64_t>(q_head) * D + d0) =
+      make_uint2(Half16<T>::pack(o[0] * inv, o[1] * inv), Half16<T>::pack(o[2] * inv, o[3] * inv));
   if (d0 == 0 && a.lse != nullptr) a.lse[static_cast<int64_t>(q_row) * a.q_heads + q_head] = (top + log2f(l)) * kLn2;
 }
 
@@ -807,7 +903,7 @@ struct PromptLayout {
     cta_pair = 256;
     first = cta_pair + up(4 * (kMaxSms + 1));
     rec = first + up(4 * (static_cast<size_t>(n) + 1));
-    part = rec + up(16 * pairs);
+    part = rec + up(32 * pairs);
     bytes = part + up(static_cast<size_t>(kMaxSms) * 2 * (head_dim + 2) * kPairRows * 4);
   }
 };
@@ -861,7 +957,7 @@ cudaError_t run_prompt(const PagedCache& c, int dtype, const Attend& a, const Pr
                             a.sinks, 2 * (kTile / a.group), sms);
     if (e == cudaSuccess) e = launch_serialized(kernel, dim3(sms), dim3(kPromptThreads), smem, stream, map, c, a, rows, ws);
     if (e == cudaSuccess)
-      e = launch_serialized(join, dim3(sms - 1, kPairRows / 32), dim3(256), 0, stream, c, a, rows, ws);
+      e = launch_serialized(join, dim3(sms - 1, kPairRows / 32, c.head_dim / 32), dim3(256), 0, stream, c, a, rows, ws);
     return e;
   };
   auto pick = [&](auto type) {
