@@ -18,18 +18,21 @@
 //                   tensor memory, writes P over it in 16 bits (the A operand
 //                   of the second product), rescales O when needed, and
 //                   stores the result;
-//   warp 8          issues the MMAs: S0, S1, then P0 V, next S0, P1 V, next
-//                   S1, ... so that one tile's products run under the other
-//                   tile's softmax; also clears value rows that no query may
-//                   see (page tails, masked keys: 0 times their bytes must be 0);
+//   warp 8          one thread issues the MMAs: S0, S1, then P0 V, next S0,
+//                   P1 V, next S1, ... so that one tile's products run under
+//                   the other tile's softmax;
 //   warp 9          TMA: the pages of each 128-key tile, keys then values, into
-//                   a ring of stages (128-byte swizzle).
+//                   a ring of stages (128-byte swizzle);
+//   warp 10         clears value rows that no query may see (page tails,
+//                   masked keys), whose probability of 0 must not meet a NaN.
 // Tensor memory: S0, S1 (128 columns each), O0, O1 (head_dim each).
 //
 // The units' key tiles form one line that is cut into equal parts, one per
 // CTA; a unit cut by a boundary leaves (m, l, O) in the workspace for a
 // second kernel that joins the parts in order.  Every wait is bounded; one
 // that gives up marks the slot's status 4.
+#include <type_traits>
+
 #include "gemm_tc.cuh"
 #include "paged_attention.cuh"
 
@@ -118,10 +121,16 @@ struct KeySpan {
   __device__ __forceinline__ int tile(int t) const { return t < sink_n ? t : win0 + t - sink_n; }
 };
 
-// Whether any query at positions [p0, p1] sees a key of tile j.
-__device__ __forceinline__ bool tile_seen(int j, int p0, int p1, int window, int sinks) {
-  return p0 <= p1 && kTile * j <= p1 && (window == 0 || kTile * j + kTile - 1 > p0 - window || kTile * j < sinks);
-}
+// The key tiles of which a query at positions [p0, p1] sees anything.
+struct TilesSeen {
+  int low, high, sink;
+  __device__ __forceinline__ TilesSeen(int p0, int p1, int window, int sinks) {
+    low = window > 0 ? max(0, p0 - window + 1) / kTile : 0;
+    high = p0 <= p1 ? p1 / kTile : -1;
+    sink = (sinks > 0 ? (sinks - 1) / kTile : -1);
+  }
+  __device__ __forceinline__ bool at(int j) const { return j <= high && (j >= low || j <= sink); }
+};
 // Whether every one of them sees every key of it.
 __device__ __forceinline__ bool tile_full(int j, int p0, int p1, int window, int sinks) {
   return kTile * j + kTile - 1 <= p0 && (window == 0 || kTile * j > p1 - window || kTile * (j + 1) <= sinks);
@@ -331,13 +340,35 @@ __host__ __device__ constexpr uint32_t prompt_idesc<__half>(int n, bool b_mn_maj
   return (umma_idesc_bf16(kTile, n) & ~((1u << 7) | (1u << 10))) | (b_mn_major ? 1u << 16 : 0u);
 }
 
-// D[tmem] (+)= A[tmem] x B[smem desc], issued by one thread.
-__device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+// One thread of a converged warp, the same one every time: what it issued is
+// tracked by the commits it issues.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(one));
+  return one != 0;
+}
+
+// The high words of the two descriptor forms: stride 1024 bytes (8 rows of
+// 128), descriptor version 1, 128-byte swizzle.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+
+// D[tmem] (+)= A[smem desc] x B[smem desc]^T, given the descriptors' low words.
+__device__ __forceinline__ void umma_ss(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc,
                                         bool accumulate) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate ? 1u : 0u)
+      "{\n .reg .pred p;\n .reg .b64 da, db;\n setp.ne.b32 p, %5, 0;\n mov.b64 da, {%1, %3};\n mov.b64 db, {%2, %3};\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p;\n}\n" ::"r"(d_tmem),
+      "r"(a_lo), "r"(b_lo), "r"(kDescHigh), "r"(idesc), "r"(accumulate ? 1u : 0u)
+      : "memory");
+}
+
+// D[tmem] (+)= A[tmem] x B[smem desc].
+__device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc,
+                                        bool accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n .reg .b64 db;\n setp.ne.b32 p, %5, 0;\n mov.b64 db, {%2, %3};\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "r"(b_lo), "r"(kDescHigh), "r"(idesc), "r"(accumulate ? 1u : 0u)
       : "memory");
 }
 
@@ -374,6 +405,57 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return pair2(d);
 }
 
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// 2^x of two values on the FMA pipe: x = n + f with n the nearest whole number
+// (from the low bits of x + 1.5 * 2^23), 2^f by its minimax polynomial of
+// degree 4 on [-1/2, 1/2] (relative error 2.7e-6, far below the rounding of P),
+// n added to the exponent.  For x in [-126, 127]; smaller x gives 2^-126.
+constexpr int kPolyOf8 = 2;  // of 8 pairs of probabilities, those computed this way
+
+__device__ __forceinline__ float2 ex2_poly(float2 x) {
+  const float2 magic = make_float2(12582912.f, 12582912.f), back = make_float2(-12582912.f, -12582912.f);
+  const float2 minus = make_float2(-1.f, -1.f);
+  x.x = max_nan(x.x, -126.f);
+  x.y = max_nan(x.y, -126.f);
+  const float2 t = add2(x, magic);
+  const float2 f = fma2(add2(t, back), minus, x);
+  float2 p = make_float2(0x1.3997d6p-7f, 0x1.3997d6p-7f);
+  p = fma2(p, f, make_float2(0x1.ca1442p-5f, 0x1.ca1442p-5f));
+  p = fma2(p, f, make_float2(0x1.ec06dap-3f, 0x1.ec06dap-3f));
+  p = fma2(p, f, make_float2(0x1.62e0dcp-1f, 0x1.62e0dcp-1f));
+  p = fma2(p, f, make_float2(0x1.ffffe8p-1f, 0x1.ffffe8p-1f));
+  return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
+                     __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
+}
+
+// Starts a 32-column load; the registers are valid after tmem_ld_done names them.
+__device__ __forceinline__ void tmem_ld32_start(uint32_t (&v)[32], uint32_t taddr) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
+        "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
+        "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld_done(uint32_t (&v)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
+                 "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]),
+                 "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]),
+                 "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]),
+                 "+r"(v[30]), "+r"(v[31])
+               :
+               : "memory");
+}
+
 // Warp-uniform forms: a wait succeeds, and the CTA goes on, for all lanes or none.
 __device__ __forceinline__ bool wait_warp(unsigned long long* bar, uint32_t parity) {
   return __all_sync(0xffffffffu, mbar_wait_cta(bar, parity));
@@ -396,15 +478,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   using C = PromptCfg<D>;
   constexpr int S = C::kStages;
   constexpr int DB = D / 64;  // 64-dim blocks of a tile
-  constexpr uint32_t kSCol = 0, kPCol = kTile / 2, kOCol = 2 * kTile;  // P over the second half of S
+  constexpr uint32_t kSCol = 0, kOCol = 2 * kTile;
   extern __shared__ unsigned char prompt_smem[];
-  __shared__ unsigned long long kv_full[S], kv_empty[S], q_ready[2], s_full[2], p_full[2], o_full[2], fin;
+  __shared__ unsigned long long kv_full[S], kv_empty[S], v_ready[S], q_ready[2], s_full[2], p_full[2], o_full[2], fin;
   __shared__ uint32_t tmem_base;
   __shared__ int err;
   const uint32_t pad = (1024u - (smem_addr(prompt_smem) & 1023u)) & 1023u;
   unsigned char* q_smem = prompt_smem + pad;
   unsigned char* ring = q_smem + 2 * C::kTileBytes;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const bool prefix = rows.members != nullptr;
   const int tq = kTile / a.group;  // tokens of a Q tile
 
@@ -412,6 +494,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     for (int s = 0; s < S; ++s) {
       mbar_init(&kv_full[s], 1);
       mbar_init(&kv_empty[s], 1);
+      mbar_init(&v_ready[s], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_ready[i], 4);
@@ -482,57 +565,21 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     // no copy may still be landing in shared memory when the CTA leaves
     if (lane == 0)
       for (int k = max(0, it - S); k < it; ++k) mbar_wait_cta(&kv_full[k % S], (k / S) & 1);
-  } else if (warp == 8) {
-    // ---- MMA issuer
-    int it = 0;                 // ring position of the next key tile
-    int p_uses[2] = {0, 0}, q_uses = 0;
-    const uint32_t idesc_s = prompt_idesc<T>(kTile, false), idesc_o = prompt_idesc<T>(D, true);
-    for (bool more = any; more && alive(errv); more = w.next(ws), ++q_uses) {
+  } else if (warp == 10) {
+    // ---- value rows that no query may see are cleared before the MMA warp may use the tile
+    int it = 0;
+    for (bool more = any; more && alive(errv); more = w.next(ws)) {
       const Geom g = w.g;
-      int p0, p1, q0[2], q1[2];
+      int p0, p1;
       positions(g, prefix, w.tok0, w.tok0 + 2 * tq, &p0, &p1);
-      positions(g, prefix, w.tok0, w.tok0 + tq, &q0[0], &q1[0]);
-      positions(g, prefix, w.tok0 + tq, w.tok0 + 2 * tq, &q0[1], &q1[1]);
       const KeySpan span(p0, max(p0, p1), a.window, a.sinks);
       const bool* mask = a.key_mask != nullptr ? a.key_mask + g.key_slot * a.mask_stride : nullptr;
-      bool ok = true, started[2] = {false, false};
-      int last[2] = {-1, -1};  // each Q tile's last key tile in this share
-      for (int i = 0; i < 2; ++i)
-        for (int t = w.t1 - 1; t >= w.t0 && last[i] < 0; --t)
-          if (tile_seen(span.tile(t), q0[i], q1[i], a.window, a.sinks)) last[i] = t;
-      auto scores = [&](int i, int s) {  // S_i = Q_i K^T
-        const unsigned char* q = q_smem + i * C::kTileBytes;
-        const unsigned char* k = ring + static_cast<size_t>(s) * C::kTileBytes;
-#pragma unroll
-        for (int b = 0; b < DB; ++b) {
-          const uint64_t qd = umma_desc_sw128(q + b * (kTile * 128)), kd = umma_desc_sw128(k + b * (kTile * 128));
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            umma_bf16(tmem + kSCol + i * kTile, qd + 2 * kk, kd + 2 * kk, idesc_s, (b | kk) != 0);
-        }
-        umma_commit(&s_full[i]);
-      };
-      ok = wait_warp(&kv_full[it % S], (it / S) & 1);
-      for (int i = 0; i < 2 && ok; ++i) {
-        ok = wait_warp(&q_ready[i], q_uses & 1);
-        tmem_fence_after_sync();
-        if (ok && lane == 0) {
-          if (tile_seen(span.tile(w.t0), q0[i], q1[i], a.window, a.sinks)) scores(i, it % S);
-          // a Q tile without key tiles here waits too: its warps must not run ahead of this one
-          if (last[i] < 0) umma_commit(&o_full[i]);
-        }
-      }
-      if (ok && lane == 0) umma_commit(&kv_empty[it % S]);
-      ++it;
-      for (int t = w.t0; ok && t < w.t1; ++t) {
-        const int vs = it % S;
-        ok = wait_warp(&kv_full[vs], (it / S) & 1);
-        if (!ok) break;
-        ++it;
-        const int base = kTile * span.tile(t);
-        // value rows that no query may see are cleared
-        if (mask != nullptr || (base + kTile > g.len && (g.len & (c.page_size - 1)) != 0)) {
-          unsigned char* v = ring + static_cast<size_t>(vs) * C::kTileBytes;
+      bool ok = true;
+      for (int t = w.t0; ok && t < w.t1; ++t, it += 2) {
+        const int s = (it + 1) % S, base = kTile * span.tile(t);
+        ok = wait_warp(&kv_full[s], ((it + 1) / S) & 1);
+        if (ok && (mask != nullptr || (base + kTile > g.len && (g.len & (c.page_size - 1)) != 0))) {
+          unsigned char* v = ring + static_cast<size_t>(s) * C::kTileBytes;
           for (int r = lane; r < kTile; r += 32) {
             const bool keep = base + r < g.len && (mask == nullptr || mask[base + r]);
             if (!keep) {
@@ -546,48 +593,105 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           fence_proxy_async();
           __syncwarp();
         }
-        const bool next = t + 1 < w.t1;
-        int ks = 0;
-        if (next) {
-          ks = it % S;
-          ok = wait_warp(&kv_full[ks], (it / S) & 1);
-          if (!ok) break;
+        if (ok && lane == 0) mbar_arrive(&v_ready[s]);
+      }
+      if (!ok) *errv = 1;
+    }
+  } else if (warp == 8) {
+    // ---- MMA issuer.  The whole warp walks along, so that what the
+    // instructions are given stays in uniform registers; one elected thread
+    // issues them.  Only the descriptors' low words change.
+    int it = 0;  // ring position of the next key tile (its values follow)
+    int p_uses[2] = {0, 0}, q_uses = 0;
+    const uint32_t q_lo = static_cast<uint32_t>(umma_desc_sw128(q_smem));
+    const uint32_t k_lo = static_cast<uint32_t>(umma_desc_sw128(ring));
+    const uint32_t v_lo = static_cast<uint32_t>(value_desc(smem_addr(ring)));
+    constexpr uint32_t kTileStep = C::kTileBytes >> 4, kBlockStep = (kTile * 128) >> 4;
+    auto scores = [&](int i, int s) {  // S_i = Q_i K^T
+      const uint32_t qd = q_lo + i * kTileStep, kd = k_lo + s * kTileStep;
+      if (elect_one()) {
+#pragma unroll
+        for (int b = 0; b < DB; ++b)
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            umma_ss(tmem + kSCol + i * kTile, qd + b * kBlockStep + 2 * kk, kd + b * kBlockStep + 2 * kk,
+                    prompt_idesc<T>(kTile, false), (b | kk) != 0);
+        umma_commit(&s_full[i]);
+      }
+      __syncwarp();
+    };
+    auto commit = [&](unsigned long long* bar) {
+      if (elect_one()) umma_commit(bar);
+      __syncwarp();
+    };
+    bool more = any;
+    while (more && alive(errv)) {
+      int p0, p1, q0[2], q1[2];
+      positions(w.g, prefix, w.tok0, w.tok0 + 2 * tq, &p0, &p1);
+      positions(w.g, prefix, w.tok0, w.tok0 + tq, &q0[0], &q1[0]);
+      positions(w.g, prefix, w.tok0 + tq, w.tok0 + 2 * tq, &q0[1], &q1[1]);
+      const KeySpan span(p0, max(p0, p1), a.window, a.sinks);
+      const TilesSeen seen[2] = {TilesSeen(q0[0], q1[0], a.window, a.sinks), TilesSeen(q0[1], q1[1], a.window, a.sinks)};
+      bool started[2] = {false, false};
+      int last[2];  // each Q tile's last key tile in this share
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        last[i] = w.t1 - 1;
+        while (last[i] >= w.t0 && !seen[i].at(span.tile(last[i]))) --last[i];
+      }
+      const int t0 = w.t0, t1 = w.t1;
+      more = w.next(ws);  // its loads are on their way while this unit runs
+      bool ok = wait_warp(&kv_full[it % S], (it / S) & 1);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        ok = ok && wait_warp(&q_ready[i], q_uses & 1);
+        if (ok) {
           tmem_fence_after_sync();
-          ++it;
+          if (seen[i].at(span.tile(t0))) scores(i, it % S);
+          // a Q tile without key tiles here waits too: its warps must not run ahead of this one
+          if (last[i] < t0) commit(&o_full[i]);
         }
-        for (int i = 0; i < 2 && ok; ++i) {
-          if (tile_seen(span.tile(t), q0[i], q1[i], a.window, a.sinks)) {
+      }
+      ++q_uses;
+      if (ok) commit(&kv_empty[it % S]);
+      for (int t = t0; ok && t < t1; ++t) {
+        const int vs = (it + 1) % S, ks = (it + 2) % S;
+        const bool next = t + 1 < t1;
+        ok = wait_warp(&v_ready[vs], ((it + 1) / S) & 1);
+        if (next) ok = ok && wait_warp(&kv_full[ks], ((it + 2) / S) & 1);
+        const int j = span.tile(t), j1 = next ? span.tile(t + 1) : 0;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (ok && seen[i].at(j)) {
             ok = wait_warp(&p_full[i], p_uses[i] & 1);
             ++p_uses[i];
-            if (!ok) break;
-            tmem_fence_after_sync();
-            if (lane == 0) {
-              const uint64_t vd = value_desc(smem_addr(ring + static_cast<size_t>(vs) * C::kTileBytes));
+            if (ok) {
+              tmem_fence_after_sync();
+              const uint32_t vd = v_lo + vs * kTileStep;
+              if (elect_one()) {
 #pragma unroll
-              for (int kk = 0; kk < kTile / 16; ++kk)
-                umma_ts(tmem + kOCol + i * D, tmem + kSCol + i * kTile + kPCol + 8 * kk, vd + kk * (2048 >> 4), idesc_o,
-                        started[i] || kk != 0);
+                for (int kk = 0; kk < kTile / 16; ++kk)
+                  umma_ts(tmem + kOCol + i * D, tmem + kSCol + i * kTile + 8 * kk, vd + kk * (2048 >> 4),
+                          prompt_idesc<T>(D, true), started[i] || kk != 0);
+              }
+              __syncwarp();
+              started[i] = true;
+              if (t == last[i]) commit(&o_full[i]);
             }
-            started[i] = true;
-            if (t == last[i] && lane == 0) umma_commit(&o_full[i]);
           }
-          if (next && lane == 0 && tile_seen(span.tile(t + 1), q0[i], q1[i], a.window, a.sinks)) scores(i, ks);
+          if (ok && next && seen[i].at(j1)) scores(i, ks);
         }
-        if (ok && lane == 0) {
-          umma_commit(&kv_empty[vs]);
-          if (next) umma_commit(&kv_empty[ks]);
+        if (ok) {
+          commit(&kv_empty[vs]);
+          if (next) commit(&kv_empty[ks]);
+          it += 2;
         }
       }
-      if (!ok) {
-        *errv = 1;
-        break;
-      }
+      if (!ok) *errv = 1;
     }
-    // every MMA this thread issued has completed before tensor memory is freed
-    if (lane == 0) {
-      umma_commit(&fin);
-      mbar_wait_cta(&fin, 0);
-    }
+    // every MMA this warp issued has completed before tensor memory is freed
+    commit(&fin);
+    wait_warp(&fin, 0);
   }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
@@ -635,6 +739,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       positions(g, prefix, w.tok0, w.tok0 + 2 * tq, &p0, &p1);
       positions(g, prefix, w.tok0 + i * tq, w.tok0 + (i + 1) * tq, &q0, &q1);
       const KeySpan span(p0, max(p0, p1), a.window, a.sinks);
+      const TilesSeen seen(q0, q1, a.window, a.sinks);
       const int pos = prefix ? g.len - 1 : g.len - g.count + w.tok0 + i * tq + tok_in_tile;
       const bool* mask = a.key_mask != nullptr ? a.key_mask + g.key_slot * a.mask_stride : nullptr;
       float m = -CUDART_INF_F;
@@ -642,7 +747,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       bool ok = true, started = false;
       for (int t = w.t0; t < w.t1; ++t) {
         const int j = span.tile(t);
-        if (!tile_seen(j, q0, q1, a.window, a.sinks)) continue;
+        if (!seen.at(j)) continue;
         const int base = kTile * j;
         uint32_t see[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
         const bool all = mask == nullptr && tile_full(j, q0, q1, a.window, a.sinks) && base + kTile <= g.len;
@@ -663,30 +768,34 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         ++s_uses;
         if (!ok) break;
         tmem_fence_after_sync();
-        // 64 of the 128 scores at a time: the first half is read again after
-        // the maximum is known, which costs less than the registers to hold it
-        uint32_t s[64];
-        auto half = [&](int x) {
-          tmem_ld64(s, s_col + 64 * x);
-          if (!all) {
-#pragma unroll
-            for (int k = 0; k < 64; ++k)
-              if (!((see[2 * x + (k >> 5)] >> (k & 31)) & 1u)) s[k] = 0xff800000u;
-          }
-        };
-        float tops[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) tops[k] = m;
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          half(x);
-#pragma unroll
-          for (int k = 0; k < 64; ++k) tops[k & 7] = fmaxf(tops[k & 7], __uint_as_float(s[k]));
+        uint32_t s[128];
+        {
+          uint32_t(&s0)[32] = *reinterpret_cast<uint32_t(*)[32]>(s);
+          uint32_t(&s1)[32] = *reinterpret_cast<uint32_t(*)[32]>(s + 32);
+          uint32_t(&s2)[32] = *reinterpret_cast<uint32_t(*)[32]>(s + 64);
+          uint32_t(&s3)[32] = *reinterpret_cast<uint32_t(*)[32]>(s + 96);
+          tmem_ld32_start(s0, s_col);
+          tmem_ld32_start(s1, s_col + 32);
+          tmem_ld32_start(s2, s_col + 64);
+          tmem_ld32_start(s3, s_col + 96);
+          tmem_ld_done(s0);
+          tmem_ld_done(s1);
+          tmem_ld_done(s2);
+          tmem_ld_done(s3);
         }
-        const float top = fmaxf(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])),
-                                fmaxf(fmaxf(tops[4], tops[5]), fmaxf(tops[6], tops[7])));
+        if (!all) {
+#pragma unroll
+          for (int k = 0; k < 128; ++k)
+            if (!((see[k >> 5] >> (k & 31)) & 1u)) s[k] = 0xff800000u;
+        }
+        float tops[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) tops[k] = max_nan(m, __uint_as_float(s[k]));
+#pragma unroll
+        for (int k = 4; k < 128; ++k) tops[k & 3] = max_nan(tops[k & 3], __uint_as_float(s[k]));
+        const float top = max_nan(max_nan(tops[0], tops[1]), max_nan(tops[2], tops[3]));
         // the maximum in use moves only when it must
-        const bool move = m == -CUDART_INF_F ? top > m : (top - m) * a.scale2 > 8.f;
+        const bool move = m == -CUDART_INF_F ? !(top <= m) : !((top - m) * a.scale2 <= 8.f);  // a NaN moves it too
         if (__any_sync(0xffffffffu, move)) {
           if (started && __any_sync(0xffffffffu, move && m != -CUDART_INF_F)) {
             const float f = move && m != -CUDART_INF_F ? ex2((m - top) * a.scale2) : 1.f;
@@ -706,25 +815,32 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         const float off = m == -CUDART_INF_F ? 0.f : -m * a.scale2;
         const float2 scale = make_float2(a.scale2, a.scale2), offs = make_float2(off, off);
         float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-        // the probabilities go over the second half's scores, which are in registers by now
+        auto exps = [&](auto poly) {
 #pragma unroll
-        for (int x = 1; x >= 0; --x) {
-          if (x == 0) half(0);
-#pragma unroll
-          for (int y = 0; y < 2; ++y) {
+          for (int x = 0; x < 4; ++x) {
             uint32_t p[16];
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
-              const int e = 32 * y + 2 * k;
+              const int e = 32 * x + 2 * k;
               float2 v = fma2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), scale, offs);
-              v.x = ex2(v.x);
-              v.y = ex2(v.y);
+              if (decltype(poly)::value && (k & 7) < kPolyOf8) {
+                v = ex2_poly(v);
+              } else {
+                v.x = ex2(v.x);
+                v.y = ex2(v.y);
+              }
               // the sum keeps the unrounded probabilities; the values' weights are rounded to 16 bits once
               sums[k & 1] = add2(sums[k & 1], v);
               p[k] = Half16<T>::pack(v.x, v.y);
             }
-            tmem_st16(s_col + kPCol + 32 * x + 16 * y, p);
+            tmem_st16(s_col + 16 * x, p);
           }
+        };
+        // masked scores (-inf) must come out as exact zeros: the special function unit alone
+        if (all) {
+          exps(std::true_type{});
+        } else {
+          exps(std::false_type{});
         }
         l2 = add2(l2, add2(sums[0], sums[1]));
         tmem_wait_st();
