@@ -3,7 +3,7 @@
 // sinks and key mask) and the prefix pass of groups of slots that share a
 // prefix (every member's newest token over the voice's pages).
 //
-//   S = Q K^T,  P = e^{scale S - m},  l += P 1,  O += P V     per 128-key tile
+//   S = Q K^T,  P = e^{scale S - m},  l += P 1,  O += P V     per 64-key tile
 //
 // with a running maximum m per row and O rescaled only when m grew by more
 // than a factor 2^8 (the f32 sums have room for it, and P in 16 bits keeps
@@ -12,25 +12,29 @@
 // A unit is a key head and two Q tiles of 128 rows; a tile's rows are the
 // group's query heads of consecutive tokens (128 / group of them), so shared
 // key heads fill the MMA's 128 rows and every key tile in shared memory is
-// used by both Q tiles.  Warp roles (384 threads, one CTA per SM; the softmax warps take registers over
-// from the others):
+// used by both Q tiles.  Warp roles (384 threads, one CTA per SM; the softmax
+// warps take registers over from the others):
 //   warps 0-3, 4-7  softmax of Q tile 0 / 1: one thread per row reads S from
 //                   tensor memory, writes P over it in 16 bits (the A operand
 //                   of the second product), rescales O when needed, and
 //                   stores the result;
-//   warp 8          one thread issues the MMAs: S0, S1, then P0 V, next S0,
-//                   P1 V, next S1, ... so that one tile's products run under
-//                   the other tile's softmax;
-//   warp 9          TMA: the pages of each 128-key tile, keys then values, into
-//                   a ring of stages (128-byte swizzle);
+//   warps 8, 11     issue the MMAs of Q tile 0 / 1;
+//   warp 9          TMA: the pages of each key tile into a ring of stages
+//                   (128-byte swizzle);
 //   warp 10         clears value rows that no query may see (page tails,
 //                   masked keys), whose probability of 0 must not meet a NaN.
-// Tensor memory: S0, S1 (128 columns each), O0, O1 (head_dim each).
+// Tensor memory: two S buffers of 64 columns for each Q tile, O0, O1 (head_dim
+// each).  The scores of tile t + 2 are issued right after the product P V of
+// tile t, so a softmax warp finds its next scores waiting and is what bounds
+// the loop.  (128-key tiles with one buffer, whose softmax waited for both
+// products in between: 3150 SM cycles per 128 keys of both Q tiles at head_dim
+// 128, of which the MMAs take 2048.)
 //
 // The units' key tiles form one line that is cut into equal parts, one per
 // CTA; a unit cut by a boundary leaves (m, l, O) in the workspace for a
 // second kernel that joins the parts in order.  Every wait is bounded; one
 // that gives up marks the slot's status 4.
+#include <algorithm>
 #include <type_traits>
 
 #include "gemm_tc.cuh"
@@ -39,18 +43,20 @@
 namespace mtt {
 namespace {
 
-constexpr int kTile = 128;          // rows of a Q tile, keys of a key tile
+constexpr int kTile = 128;          // rows of a Q tile
+constexpr int kKeys = 64;           // keys of a key tile
 constexpr int kPairRows = 2 * kTile;
 constexpr int kPromptThreads = 384;
 constexpr int kPromptPlanThreads = 1024;
-constexpr int kMinShare = 2;        // key tiles a CTA takes at least
+constexpr int kMinShare = 4;        // key tiles a CTA takes at least
 constexpr int kMaxSms = 160;        // workspaces are sized for the largest device
 
 template <int D>
 struct PromptCfg {
-  static constexpr int kStages = D == 64 ? 8 : 4;
-  static constexpr uint32_t kTileBytes = kTile * D * 2;
-  static constexpr size_t kSmem = 1024 + static_cast<size_t>(2 + kStages) * kTileBytes;
+  static constexpr int kStages = D == 64 ? 16 : 8;
+  static constexpr uint32_t kQBytes = kTile * D * 2;
+  static constexpr uint32_t kTileBytes = kKeys * D * 2;
+  static constexpr size_t kSmem = 1024 + 2 * static_cast<size_t>(kQBytes) + kStages * static_cast<size_t>(kTileBytes);
 };
 
 // Rows of the attention: tokens of slots, or members of prefix groups.
@@ -68,7 +74,7 @@ struct PromptRows {
 
 // A unit's place on the line: its key tiles, and before them what entering and
 // leaving it costs, in key tiles.
-constexpr int kPairCost = 2;
+constexpr int kPairCost = 4;
 
 struct PromptSpace {
   int64_t* head;       // [0] pairs, [1] length of one key head's line, [2] length of a share
@@ -108,14 +114,14 @@ struct PairGeom : Geom {
   }
 };
 
-// The 128-key tiles that queries at positions [p0, p1] may see.
+// The key tiles that queries at positions [p0, p1] may see.
 struct KeySpan {
   int sink_n, win0, n;
   __device__ __forceinline__ KeySpan(int p0, int p1, int window, int sinks) {
     const int low = window > 0 ? max(0, p0 - window + 1) : 0;
-    const int end = p1 / kTile + 1;
-    sink_n = low > 0 && sinks > 0 ? min((min(sinks - 1, p1)) / kTile + 1, end) : 0;
-    win0 = max(low / kTile, sink_n);
+    const int end = p1 / kKeys + 1;
+    sink_n = low > 0 && sinks > 0 ? min((min(sinks - 1, p1)) / kKeys + 1, end) : 0;
+    win0 = max(low / kKeys, sink_n);
     n = sink_n + max(0, end - win0);
   }
   __device__ __forceinline__ int tile(int t) const { return t < sink_n ? t : win0 + t - sink_n; }
@@ -125,15 +131,15 @@ struct KeySpan {
 struct TilesSeen {
   int low, high, sink;
   __device__ __forceinline__ TilesSeen(int p0, int p1, int window, int sinks) {
-    low = window > 0 ? max(0, p0 - window + 1) / kTile : 0;
-    high = p0 <= p1 ? p1 / kTile : -1;
-    sink = (sinks > 0 ? (sinks - 1) / kTile : -1);
+    low = window > 0 ? max(0, p0 - window + 1) / kKeys : 0;
+    high = p0 <= p1 ? p1 / kKeys : -1;
+    sink = (sinks > 0 ? (sinks - 1) / kKeys : -1);
   }
   __device__ __forceinline__ bool at(int j) const { return j <= high && (j >= low || j <= sink); }
 };
 // Whether every one of them sees every key of it.
 __device__ __forceinline__ bool tile_full(int j, int p0, int p1, int window, int sinks) {
-  return kTile * j + kTile - 1 <= p0 && (window == 0 || kTile * j > p1 - window || kTile * (j + 1) <= sinks);
+  return kKeys * j + kKeys - 1 <= p0 && (window == 0 || kKeys * j > p1 - window || kKeys * (j + 1) <= sinks);
 }
 
 // Positions [p0, p1] of the rows of tokens [t0, t1); empty when p1 < p0.  In
@@ -319,10 +325,10 @@ struct Walk {
 };
 
 // 128-byte-swizzled MN-major operand (values: [keys][64 dims] rows of 128
-// bytes): 8-key groups 1024 bytes apart, the next 64 dims one 128-key block on.
+// bytes): 8-key groups 1024 bytes apart, the next 64 dims one block of kKeys rows on.
 __device__ __forceinline__ uint64_t value_desc(uint32_t a) {
   uint64_t d = static_cast<uint64_t>((a & 0x3FFFFu) >> 4);
-  d |= static_cast<uint64_t>((kTile * 128) >> 4) << 16;  // leading byte offset: 64 dims on
+  d |= static_cast<uint64_t>((kKeys * 128) >> 4) << 16;  // leading byte offset: 64 dims on
   d |= static_cast<uint64_t>(1024 >> 4) << 32;           // stride byte offset: 8 keys on
   d |= static_cast<uint64_t>(1) << 46;
   d |= static_cast<uint64_t>(2) << 61;
@@ -411,6 +417,12 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 // 2^x of two values on the FMA pipe: x = n + f with n the nearest whole number
 // (from the low bits of x + 1.5 * 2^23), 2^f by its minimax polynomial of
 // degree 4 on [-1/2, 1/2] (relative error 2.7e-6, far below the rounding of P),
@@ -478,14 +490,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   using C = PromptCfg<D>;
   constexpr int S = C::kStages;
   constexpr int DB = D / 64;  // 64-dim blocks of a tile
-  constexpr uint32_t kSCol = 0, kOCol = 2 * kTile;
+  constexpr uint32_t kSCol = 0, kOCol = 4 * kKeys;  // S of Q tile i, buffer b: column (2 i + b) kKeys
   extern __shared__ unsigned char prompt_smem[];
-  __shared__ unsigned long long kv_full[S], kv_empty[S], v_ready[S], q_ready[2], s_full[2], p_full[2], o_full[2], fin;
+  __shared__ unsigned long long kv_full[S], kv_empty[S], ready[S], q_ready[2], s_full[2][2], p_full[2][2], pv_done[2], skip[2], fin[2];
   __shared__ uint32_t tmem_base;
   __shared__ int err;
   const uint32_t pad = (1024u - (smem_addr(prompt_smem) & 1023u)) & 1023u;
   unsigned char* q_smem = prompt_smem + pad;
-  unsigned char* ring = q_smem + 2 * C::kTileBytes;
+  unsigned char* ring = q_smem + 2 * C::kQBytes;
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const bool prefix = rows.members != nullptr;
   const int tq = kTile / a.group;  // tokens of a Q tile
@@ -493,16 +505,19 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
       mbar_init(&kv_full[s], 1);
-      mbar_init(&kv_empty[s], 1);
-      mbar_init(&v_ready[s], 1);
+      mbar_init(&kv_empty[s], 2);  // both issuing warps
+      mbar_init(&ready[s], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_ready[i], 4);
-      mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 4);
-      mbar_init(&o_full[i], 1);
+      for (int b = 0; b < 2; ++b) {
+        mbar_init(&s_full[i][b], 1);
+        mbar_init(&p_full[i][b], 4);
+      }
+      mbar_init(&pv_done[i], 1);
+      mbar_init(&skip[i], 1);
+      mbar_init(&fin[i], 1);
     }
-    mbar_init(&fin, 1);
     err = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -526,9 +541,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
   if (warp == 9) {
-    // ---- TMA producer: per key tile its keys, then its values
+    // ---- TMA producer.  Order: keys 0, keys 1, then values t, keys t + 2, as they are used.
     int it = 0;
-    const int boxes = kTile >> c.page_shift;  // pages per tile
+    const int rows_per_box = min(kKeys, c.page_size), boxes = kKeys / rows_per_box;
     const int beyond = c.pages * c.layers * 2 * c.kv_heads * c.page_size;  // a row past the pool: reads zeros
     for (bool more = any; more && alive(errv); more = w.next(ws)) {
       const Geom g = w.g;
@@ -536,37 +551,46 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       positions(g, prefix, w.tok0, w.tok0 + 2 * tq, &p0, &p1);
       const KeySpan span(p0, max(p0, p1), a.window, a.sinks);
       const int32_t* table = c.table + static_cast<int64_t>(g.key_slot) * c.table_pages;
+      // the row of the pool, before the choice of keys or values, where lane's box of tile t begins
       auto page_of = [&](int t) {
-        const int first_key = kTile * span.tile(t) + (lane << c.page_shift);
-        return lane < boxes && t < w.t1 && first_key < g.len ? table[first_key >> c.page_shift] : -1;
+        const int key = kKeys * span.tile(t) + lane * rows_per_box;
+        return lane < boxes && t < w.t1 && key < g.len ? table[key >> c.page_shift] : -1;
       };
-      int ahead = page_of(w.t0);
-      for (int t = w.t0; t < w.t1; ++t) {
-        const int page = ahead;
-        ahead = page_of(t + 1);  // on its way while this tile's copies wait for their stage
-        for (int kv = 0; kv < 2; ++kv, ++it) {
-          const int s = it % S;
-          if (it >= S && !wait_warp(&kv_empty[s], ((it / S) - 1) & 1)) *errv = 1;
-          if (!alive(errv)) break;
-          if (lane == 0) mbar_expect_tx(&kv_full[s], C::kTileBytes);
-          __syncwarp();
-          if (lane < boxes) {
-            const int y = c.is_page(page)
-                              ? (((page * c.layers + a.layer) * 2 + kv) * c.kv_heads + w.head) * c.page_size
-                              : beyond;
-            unsigned char* dst = ring + static_cast<size_t>(s) * C::kTileBytes + (lane << (c.page_shift + 7));
+      auto copy = [&](int t, int page, int kv) {
+        const int s = it % S;
+        if (it >= S && !wait_warp(&kv_empty[s], ((it / S) - 1) & 1)) return false;
+        ++it;
+        if (lane == 0) mbar_expect_tx(&kv_full[s], C::kTileBytes);
+        __syncwarp();
+        if (lane < boxes) {
+          const int in_page = (kKeys * span.tile(t) + lane * rows_per_box) & (c.page_size - 1);
+          const int y = c.is_page(page) ? (((page * c.layers + a.layer) * 2 + kv) * c.kv_heads + w.head) * c.page_size + in_page
+                                        : beyond;
+          unsigned char* dst = ring + static_cast<size_t>(s) * C::kTileBytes + lane * rows_per_box * 128;
 #pragma unroll
-            for (int b = 0; b < DB; ++b) tma_load_2d(dst + b * (kTile * 128), &pool_map, 64 * b, y, &kv_full[s]);
-          }
+          for (int b = 0; b < DB; ++b) tma_load_2d(dst + b * (kKeys * 128), &pool_map, 64 * b, y, &kv_full[s]);
         }
-        if (!alive(errv)) break;
+        return true;
+      };
+      int page[3] = {page_of(w.t0), page_of(w.t0 + 1), page_of(w.t0 + 2)};  // of tiles t, t + 1, t + 2
+      bool ok = copy(w.t0, page[0], 0);
+      if (ok && w.t0 + 1 < w.t1) ok = copy(w.t0 + 1, page[1], 0);
+      for (int t = w.t0; ok && t < w.t1; ++t) {
+        const int ahead = page_of(t + 3);  // on its way while the copies wait for their stages
+        ok = copy(t, page[0], 1);
+        if (ok && t + 2 < w.t1) ok = copy(t + 2, page[2], 0);
+        page[0] = page[1];
+        page[1] = page[2];
+        page[2] = ahead;
       }
+      if (!ok) *errv = 1;
     }
     // no copy may still be landing in shared memory when the CTA leaves
     if (lane == 0)
       for (int k = max(0, it - S); k < it; ++k) mbar_wait_cta(&kv_full[k % S], (k / S) & 1);
   } else if (warp == 10) {
-    // ---- value rows that no query may see are cleared before the MMA warp may use the tile
+    // ---- value rows that no query may see are cleared before the MMA warp may use the tile.  Key tiles pass
+    // through too: so neither this warp nor the MMA warp is ever a round of the ring away from the other.
     int it = 0;
     for (bool more = any; more && alive(errv); more = w.next(ws)) {
       const Geom g = w.g;
@@ -574,133 +598,140 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       positions(g, prefix, w.tok0, w.tok0 + 2 * tq, &p0, &p1);
       const KeySpan span(p0, max(p0, p1), a.window, a.sinks);
       const bool* mask = a.key_mask != nullptr ? a.key_mask + g.key_slot * a.mask_stride : nullptr;
-      bool ok = true;
-      for (int t = w.t0; ok && t < w.t1; ++t, it += 2) {
-        const int s = (it + 1) % S, base = kTile * span.tile(t);
-        ok = wait_warp(&kv_full[s], ((it + 1) / S) & 1);
-        if (ok && (mask != nullptr || (base + kTile > g.len && (g.len & (c.page_size - 1)) != 0))) {
+      auto pass = [&](int t) {  // the ring's next tile: values of tile t, or keys (t < 0)
+        const int s = it % S;
+        if (!wait_warp(&kv_full[s], (it / S) & 1)) return false;
+        ++it;
+        const int base = t < 0 ? 0 : kKeys * span.tile(t);
+        if (t >= 0 && (mask != nullptr || (base + kKeys > g.len && (g.len & (c.page_size - 1)) != 0))) {
           unsigned char* v = ring + static_cast<size_t>(s) * C::kTileBytes;
-          for (int r = lane; r < kTile; r += 32) {
+          for (int r = lane; r < kKeys; r += 32) {
             const bool keep = base + r < g.len && (mask == nullptr || mask[base + r]);
             if (!keep) {
 #pragma unroll
               for (int b = 0; b < DB; ++b)
 #pragma unroll
                 for (int k = 0; k < 8; ++k)
-                  *reinterpret_cast<uint4*>(v + b * (kTile * 128) + r * 128 + 16 * k) = make_uint4(0, 0, 0, 0);
+                  *reinterpret_cast<uint4*>(v + b * (kKeys * 128) + r * 128 + 16 * k) = make_uint4(0, 0, 0, 0);
             }
           }
           fence_proxy_async();
           __syncwarp();
         }
-        if (ok && lane == 0) mbar_arrive(&v_ready[s]);
+        if (lane == 0) mbar_arrive(&ready[s]);
+        return true;
+      };
+      bool ok = pass(-1);
+      if (ok && w.t0 + 1 < w.t1) ok = pass(-1);
+      for (int t = w.t0; ok && t < w.t1; ++t) {
+        ok = pass(t);
+        if (ok && t + 2 < w.t1) ok = pass(-1);
       }
       if (!ok) *errv = 1;
     }
-  } else if (warp == 8) {
-    // ---- MMA issuer.  The whole warp walks along, so that what the
-    // instructions are given stays in uniform registers; one elected thread
-    // issues them.  Only the descriptors' low words change.
-    int it = 0;  // ring position of the next key tile (its values follow)
-    int p_uses[2] = {0, 0}, q_uses = 0;
-    const uint32_t q_lo = static_cast<uint32_t>(umma_desc_sw128(q_smem));
+  } else {
+    // ---- MMA issuer of Q tile i: warp 8 or 11.  The whole warp walks along, so
+    // that what the instructions are given stays in uniform registers; one
+    // elected thread issues them.  Only the descriptors' low words change.
+    // (One warp for both tiles left the tensor pipe idle between its bursts:
+    // its own waits and commits took as long as the products.)
+    const int i = warp == 8 ? 0 : 1;
+    int it = 0;  // ring position
+    int s_uses = 0, p_uses = 0, q_uses = 0;
+    const uint32_t q_lo = static_cast<uint32_t>(umma_desc_sw128(q_smem)) + i * (C::kQBytes >> 4);
     const uint32_t k_lo = static_cast<uint32_t>(umma_desc_sw128(ring));
     const uint32_t v_lo = static_cast<uint32_t>(value_desc(smem_addr(ring)));
-    constexpr uint32_t kTileStep = C::kTileBytes >> 4, kBlockStep = (kTile * 128) >> 4;
-    auto scores = [&](int i, int s) {  // S_i = Q_i K^T
-      const uint32_t qd = q_lo + i * kTileStep, kd = k_lo + s * kTileStep;
-      if (elect_one()) {
-#pragma unroll
-        for (int b = 0; b < DB; ++b)
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            umma_ss(tmem + kSCol + i * kTile, qd + b * kBlockStep + 2 * kk, kd + b * kBlockStep + 2 * kk,
-                    prompt_idesc<T>(kTile, false), (b | kk) != 0);
-        umma_commit(&s_full[i]);
-      }
-      __syncwarp();
-    };
+    const uint32_t s_tmem = tmem + kSCol + 2 * i * kKeys, o_tmem = tmem + kOCol + i * D;
+    constexpr uint32_t kTileStep = C::kTileBytes >> 4, kQBlock = (kTile * 128) >> 4, kKBlock = (kKeys * 128) >> 4;
     auto commit = [&](unsigned long long* bar) {
       if (elect_one()) umma_commit(bar);
       __syncwarp();
     };
+    // waits for the ring's next tile (keys); S = Q K^T into the next buffer if the tile is seen; lets the tile go
+    auto scores = [&](bool seen) {
+      const int s = it % S;
+      if (!wait_warp(&ready[s], (it / S) & 1)) return false;
+      ++it;
+      tmem_fence_after_sync();
+      const uint32_t kd = k_lo + s * kTileStep;
+      const int b = s_uses & 1;
+      if (seen) ++s_uses;
+      if (elect_one()) {
+        if (seen) {
+#pragma unroll
+          for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              umma_ss(s_tmem + b * kKeys, q_lo + d * kQBlock + 2 * kk, kd + d * kKBlock + 2 * kk,
+                      prompt_idesc<T>(kKeys, false), (d | kk) != 0);
+          umma_commit(&s_full[i][b]);
+        }
+        umma_commit(&kv_empty[s]);
+      }
+      __syncwarp();
+      return true;
+    };
     bool more = any;
     while (more && alive(errv)) {
-      int p0, p1, q0[2], q1[2];
+      int p0, p1, q0, q1;
       positions(w.g, prefix, w.tok0, w.tok0 + 2 * tq, &p0, &p1);
-      positions(w.g, prefix, w.tok0, w.tok0 + tq, &q0[0], &q1[0]);
-      positions(w.g, prefix, w.tok0 + tq, w.tok0 + 2 * tq, &q0[1], &q1[1]);
+      positions(w.g, prefix, w.tok0 + i * tq, w.tok0 + (i + 1) * tq, &q0, &q1);
       const KeySpan span(p0, max(p0, p1), a.window, a.sinks);
-      const TilesSeen seen[2] = {TilesSeen(q0[0], q1[0], a.window, a.sinks), TilesSeen(q0[1], q1[1], a.window, a.sinks)};
-      bool started[2] = {false, false};
-      int last[2];  // each Q tile's last key tile in this share
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        last[i] = w.t1 - 1;
-        while (last[i] >= w.t0 && !seen[i].at(span.tile(last[i]))) --last[i];
-      }
+      const TilesSeen seen(q0, q1, a.window, a.sinks);
+      bool started = false;
       const int t0 = w.t0, t1 = w.t1;
+      int last = t1 - 1;
+      while (last >= t0 && !seen.at(span.tile(last))) --last;
       more = w.next(ws);  // its loads are on their way while this unit runs
-      bool ok = wait_warp(&kv_full[it % S], (it / S) & 1);
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        ok = ok && wait_warp(&q_ready[i], q_uses & 1);
-        if (ok) {
-          tmem_fence_after_sync();
-          if (seen[i].at(span.tile(t0))) scores(i, it % S);
-          // a Q tile without key tiles here waits too: its warps must not run ahead of this one
-          if (last[i] < t0) commit(&o_full[i]);
-        }
-      }
+      bool ok = wait_warp(&q_ready[i], q_uses & 1);
       ++q_uses;
-      if (ok) commit(&kv_empty[it % S]);
+      // a Q tile without key tiles in this share: its warps must not run ahead of this one (a barrier of its own,
+      // since a warp may still be on its way to the last unit's pv_done)
+      if (ok && last < t0 && lane == 0) mbar_arrive(&skip[i]);
+      ok = ok && scores(seen.at(span.tile(t0)));
+      if (t0 + 1 < t1) ok = ok && scores(seen.at(span.tile(t0 + 1)));
       for (int t = t0; ok && t < t1; ++t) {
-        const int vs = (it + 1) % S, ks = (it + 2) % S;
-        const bool next = t + 1 < t1;
-        ok = wait_warp(&v_ready[vs], ((it + 1) / S) & 1);
-        if (next) ok = ok && wait_warp(&kv_full[ks], ((it + 2) / S) & 1);
-        const int j = span.tile(t), j1 = next ? span.tile(t + 1) : 0;
+        const int vs = it % S;
+        ok = wait_warp(&ready[vs], (it / S) & 1);
+        ++it;
+        const bool use = seen.at(span.tile(t));
+        if (use && ok) {
+          const int b = p_uses & 1;
+          ok = wait_warp(&p_full[i][b], (p_uses >> 1) & 1);
+          ++p_uses;
+          if (ok) {
+            tmem_fence_after_sync();
+            const uint32_t vd = v_lo + vs * kTileStep;
+            if (elect_one()) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          if (ok && seen[i].at(j)) {
-            ok = wait_warp(&p_full[i], p_uses[i] & 1);
-            ++p_uses[i];
-            if (ok) {
-              tmem_fence_after_sync();
-              const uint32_t vd = v_lo + vs * kTileStep;
-              if (elect_one()) {
-#pragma unroll
-                for (int kk = 0; kk < kTile / 16; ++kk)
-                  umma_ts(tmem + kOCol + i * D, tmem + kSCol + i * kTile + 8 * kk, vd + kk * (2048 >> 4),
-                          prompt_idesc<T>(D, true), started[i] || kk != 0);
-              }
-              __syncwarp();
-              started[i] = true;
-              if (t == last[i]) commit(&o_full[i]);
+              for (int kk = 0; kk < kKeys / 16; ++kk)
+                umma_ts(o_tmem, s_tmem + b * kKeys + 8 * kk, vd + kk * (2048 >> 4), prompt_idesc<T>(D, true),
+                        started || kk != 0);
+              umma_commit(&pv_done[i]);
+              umma_commit(&kv_empty[vs]);
             }
+            __syncwarp();
+            started = true;
           }
-          if (ok && next && seen[i].at(j1)) scores(i, ks);
-        }
-        if (ok) {
+        } else if (ok) {
           commit(&kv_empty[vs]);
-          if (next) commit(&kv_empty[ks]);
-          it += 2;
         }
+        if (t + 2 < t1) ok = ok && scores(seen.at(span.tile(t + 2)));
       }
       if (!ok) *errv = 1;
     }
     // every MMA this warp issued has completed before tensor memory is freed
-    commit(&fin);
-    wait_warp(&fin, 0);
+    commit(&fin[i]);
+    wait_warp(&fin[i], 0);
   }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     // ---- softmax of Q tile i: thread r is its row r
     const int i = warp >> 2, r = threadIdx.x & 127;
     const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
-    const uint32_t s_col = tmem + kSCol + i * kTile + lanes, o_col = tmem + kOCol + i * D + lanes;
+    const uint32_t s_cols = tmem + kSCol + 2 * i * kKeys + lanes, o_col = tmem + kOCol + i * D + lanes;
     const int tok_in_tile = r / a.group, head_in_group = r % a.group;
-    int s_uses = 0, o_uses = 0;
+    int s_uses = 0, pv_uses = 0, skips = 0;  // pv_uses: products asked for so far
     // this thread's row of unit u: q and out row, or -1
     auto row_of = [&](const Walk& u) {
       const int tok = u.tok0 + i * tq + tok_in_tile;
@@ -713,7 +744,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     // its queries into shared memory, for the MMA warp
     auto load_q = [&](const Walk& u, int row) {
       const uint16_t* src = a.q + row * a.q_row + static_cast<int64_t>(u.head * a.group + head_in_group) * D;
-      unsigned char* dst = q_smem + i * C::kTileBytes + r * 128;
+      unsigned char* dst = q_smem + i * C::kQBytes + r * 128;
       uint4 v[DB][8];
 #pragma unroll
       for (int b = 0; b < DB; ++b)
@@ -748,15 +779,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       for (int t = w.t0; t < w.t1; ++t) {
         const int j = span.tile(t);
         if (!seen.at(j)) continue;
-        const int base = kTile * j;
-        uint32_t see[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
-        const bool all = mask == nullptr && tile_full(j, q0, q1, a.window, a.sinks) && base + kTile <= g.len;
+        const int base = kKeys * j;
+        uint32_t see[2] = {0xffffffffu, 0xffffffffu};
+        const bool all = mask == nullptr && tile_full(j, q0, q1, a.window, a.sinks) && base + kKeys <= g.len;
         if (!all) {
           const int hi = min(pos + 1, g.len) - base;
           const int lo = a.window > 0 ? max(max(pos + 1 - base, 0) - a.window, 0) : 0;
-          const int sk = min(a.sinks, kTile * (j + 1)) - base;
+          const int sk = min(a.sinks, kKeys * (j + 1)) - base;
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
+          for (int x = 0; x < 2; ++x) {
             see[x] = bit_range(0, hi - 32 * x) & (bit_range(lo - 32 * x, 32) | bit_range(0, sk - 32 * x));
             if (mask != nullptr) {
               const int k = base + 32 * x + lane;
@@ -764,40 +795,35 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             }
           }
         }
-        ok = wait_warp(&s_full[i], s_uses & 1);
+        const int buf = s_uses & 1;
+        const uint32_t s_col = s_cols + buf * kKeys;
+        ok = wait_warp(&s_full[i][buf], (s_uses >> 1) & 1);
         ++s_uses;
         if (!ok) break;
         tmem_fence_after_sync();
-        uint32_t s[128];
-        {
-          uint32_t(&s0)[32] = *reinterpret_cast<uint32_t(*)[32]>(s);
-          uint32_t(&s1)[32] = *reinterpret_cast<uint32_t(*)[32]>(s + 32);
-          uint32_t(&s2)[32] = *reinterpret_cast<uint32_t(*)[32]>(s + 64);
-          uint32_t(&s3)[32] = *reinterpret_cast<uint32_t(*)[32]>(s + 96);
-          tmem_ld32_start(s0, s_col);
-          tmem_ld32_start(s1, s_col + 32);
-          tmem_ld32_start(s2, s_col + 64);
-          tmem_ld32_start(s3, s_col + 96);
-          tmem_ld_done(s0);
-          tmem_ld_done(s1);
-          tmem_ld_done(s2);
-          tmem_ld_done(s3);
-        }
+        uint32_t s[64];
+        tmem_ld64(s, s_col);
         if (!all) {
 #pragma unroll
-          for (int k = 0; k < 128; ++k)
+          for (int k = 0; k < 64; ++k)
             if (!((see[k >> 5] >> (k & 31)) & 1u)) s[k] = 0xff800000u;
         }
         float tops[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) tops[k] = max_nan(m, __uint_as_float(s[k]));
+        for (int k = 0; k < 4; ++k)
+          tops[k] = max_nan(m, __uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1]));
 #pragma unroll
-        for (int k = 4; k < 128; ++k) tops[k & 3] = max_nan(tops[k & 3], __uint_as_float(s[k]));
-        const float top = max_nan(max_nan(tops[0], tops[1]), max_nan(tops[2], tops[3]));
+        for (int k = 4; k < 32; ++k)
+          tops[k & 3] = max_nan(tops[k & 3], __uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1]));
+        const float top = max_nan(max_nan(tops[0], tops[1]), tops[2], tops[3]);
         // the maximum in use moves only when it must
         const bool move = m == -CUDART_INF_F ? !(top <= m) : !((top - m) * a.scale2 <= 8.f);  // a NaN moves it too
         if (__any_sync(0xffffffffu, move)) {
           if (started && __any_sync(0xffffffffu, move && m != -CUDART_INF_F)) {
+            // the product before this tile's must be in O (the one before that is: this tile's scores came after it)
+            ok = wait_warp(&pv_done[i], (pv_uses - 1) & 1);
+            if (!ok) break;
+            tmem_fence_after_sync();
             const float f = move && m != -CUDART_INF_F ? ex2((m - top) * a.scale2) : 1.f;
             l2.x *= f;
             l2.y *= f;
@@ -817,7 +843,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
         auto exps = [&](auto poly) {
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
+          for (int x = 0; x < 2; ++x) {
             uint32_t p[16];
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
@@ -845,17 +871,18 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         l2 = add2(l2, add2(sums[0], sums[1]));
         tmem_wait_st();
         tmem_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[i]);
+        // not before the product of the tile before is done: so pv_done is never two phases away from a wait for it
+        if (started) ok = wait_warp(&pv_done[i], (pv_uses - 1) & 1);
+        if (!ok) break;
+        if (lane == 0) mbar_arrive(&p_full[i][buf]);
+        ++pv_uses;
         started = true;
       }
       // The next unit's queries go in before this one's result comes out: the
       // scores that used the shared memory are done.  Not before the MMA warp
-      // has taken up this unit, though, which a tile's scores (or O) show.
-      if (ok && !started) {
-        ok = wait_warp(&o_full[i], o_uses & 1);
-        ++o_uses;
-      }
+      // has taken up this unit, though, which a tile's scores show, or
+      // `skip` for a Q tile without key tiles.
+      if (ok && !started) ok = wait_warp(&skip[i], skips++ & 1);
       Walk v = w;
       more = v.next(ws);
       int next_row = -1;
@@ -863,11 +890,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         next_row = row_of(v);
         load_q(v, next_row);
       }
-      if (ok && started) {
-        ok = wait_warp(&o_full[i], o_uses & 1);
-        ++o_uses;
-        tmem_fence_after_sync();
-      }
+      if (ok && started) ok = wait_warp(&pv_done[i], (pv_uses - 1) & 1);
+      tmem_fence_after_sync();
       if (!ok) {
         *errv = 1;
         break;
@@ -1038,14 +1062,14 @@ EncodeTiledFn find_encode() {
 }
 
 // The pool as a matrix of rows (one token's keys or values of one head); a
-// box is one page's rows of one head, 64 dims wide.
+// box is one page's rows of one head (at most a key tile's), 64 dims wide.
 bool pool_map(const PagedCache& c, int dtype, CUtensorMap* map) {
   static const EncodeTiledFn fn = find_encode();
   if (fn == nullptr) return false;
   const cuuint64_t rows = static_cast<cuuint64_t>(c.pages) * c.layers * 2 * c.kv_heads * c.page_size;
   const cuuint64_t dims[2] = {static_cast<cuuint64_t>(c.head_dim), rows};
   const cuuint64_t strides[1] = {static_cast<cuuint64_t>(c.head_dim) * 2};
-  const cuuint32_t box[2] = {64, static_cast<cuuint32_t>(c.page_size)};
+  const cuuint32_t box[2] = {64, static_cast<cuuint32_t>(std::min(c.page_size, kKeys))};
   const cuuint32_t elem[2] = {1, 1};
   return fn(map,
             dtype == MTT_B200_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,

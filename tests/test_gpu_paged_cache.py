@@ -292,6 +292,20 @@ def test_prompt_many_units_per_sm(pc, window, sinks, masked, d):
     assert (cache.status == 0).all()
 
 
+def test_prompt_calls_back_to_back(pc):
+    """Hundreds of calls of many units each: no wait inside the kernel gives up, the result never changes."""
+    new = [1, 7, 130, 2, 255, 3, 40, 129, 5, 1, 300, 64] * 2
+    lengths = [n + (i * 97) % 500 for i, n in enumerate(new)]
+    cache, _, _ = make(pc, lengths, 12)
+    q = queries(sum(new), 12, 64, torch.bfloat16).cuda()
+    offsets = i32([0] + np.cumsum(new).tolist())
+    out = torch.empty_like(q)
+    first = cache.attend(0, q, offsets=offsets, window=300, sinks=16).clone()
+    for _ in range(400):
+        cache.attend(0, q, out=out, offsets=offsets, window=300, sinks=16)
+    assert torch.equal(out, first) and (cache.status == 0).all()
+
+
 def test_prompt_offsets_that_do_not_fit(pc):
     """More rows than tokens: those rows get 0 and -inf, the others are unharmed."""
     cache, pool, table = make(pc, [20, 40, 7])
