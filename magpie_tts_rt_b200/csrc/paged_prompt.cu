@@ -3,11 +3,7 @@
 // sinks and key mask) and the prefix pass of groups of slots that share a
 // prefix (every member's newest token over the voice's pages).
 //
-//   S = Q K^T,  P = e^{scale S - m},  l += P 1,  O += P V     per 64-key tile
-//
-// with a running maximum m per row and O rescaled only when m grew by more
-// than a factor 2^8 (the f32 sums have room for it, and P in 16 bits keeps
-// its relative precision), so that rescaling is rare.
+//   S = Q K^T,  P = e^{scale S - m},  l += P 1,  O += P V     per 128-key tile
 //
 // A unit is a key head and two Q tiles of 128 rows; a tile's rows are the
 // group's query heads of consecutive tokens (128 / group of them), so shared
@@ -16,19 +12,23 @@
 // warps take registers over from the others):
 //   warps 0-3, 4-7  softmax of Q tile 0 / 1: one thread per row reads S from
 //                   tensor memory, writes P over it in 16 bits (the A operand
-//                   of the second product), rescales O when needed, and
-//                   stores the result;
-//   warps 8, 11     issue the MMAs of Q tile 0 / 1;
+//                   of the second product), half a tile at a time, and stores
+//                   the result;
+//   warp 8          issues the MMAs: S0, S1, then P0 V, next S0, P1 V, next S1,
+//                   ... so that one tile's products run under the other tile's
+//                   softmax;
 //   warp 9          TMA: the pages of each key tile into a ring of stages
 //                   (128-byte swizzle);
 //   warp 10         clears value rows that no query may see (page tails,
 //                   masked keys), whose probability of 0 must not meet a NaN.
-// Tensor memory: two S buffers of 64 columns for each Q tile, O0, O1 (head_dim
-// each).  The scores of tile t + 2 are issued right after the product P V of
-// tile t, so a softmax warp finds its next scores waiting and is what bounds
-// the loop.  (128-key tiles with one buffer, whose softmax waited for both
-// products in between: 3150 SM cycles per 128 keys of both Q tiles at head_dim
-// 128, of which the MMAs take 2048.)
+// Tensor memory: S0, S1 (128 columns each), O0, O1 (head_dim each), which at
+// head_dim 128 is all of it.
+//
+// m is not the maximum so far, but one found when it was last needed: as long
+// as a half tile's probabilities stay below 2^15 (where f16 ends; f32 sums and
+// any 16-bit type keep their relative precision up to there) nothing is
+// compared or rescaled.  Only when they do not, or when a row has seen no key
+// yet, is the maximum looked for, O and l rescaled, and the half taken again.
 //
 // The units' key tiles form one line that is cut into equal parts, one per
 // CTA; a unit cut by a boundary leaves (m, l, O) in the workspace for a
@@ -44,19 +44,22 @@ namespace mtt {
 namespace {
 
 constexpr int kTile = 128;          // rows of a Q tile
-constexpr int kKeys = 64;           // keys of a key tile
+constexpr int kKeys = 128;          // keys of a key tile
+constexpr int kHalf = kKeys / 2;    // keys whose probabilities are handed over together
 constexpr int kPairRows = 2 * kTile;
 constexpr int kPromptThreads = 384;
 constexpr int kPromptPlanThreads = 1024;
-constexpr int kMinShare = 4;        // key tiles a CTA takes at least
+constexpr int kMinShare = 2;        // key tiles a CTA takes at least
 constexpr int kMaxSms = 160;        // workspaces are sized for the largest device
 
 template <int D>
 struct PromptCfg {
-  static constexpr int kStages = D == 64 ? 16 : 8;
+  static constexpr int kStages = D == 64 ? 8 : 4;
   static constexpr uint32_t kQBytes = kTile * D * 2;
   static constexpr uint32_t kTileBytes = kKeys * D * 2;
-  static constexpr size_t kSmem = 1024 + 2 * static_cast<size_t>(kQBytes) + kStages * static_cast<size_t>(kTileBytes);
+  static constexpr uint32_t kOutBytes = 8 * 32 * 128;  // a 32 x 64 block of results per softmax warp, on its way out
+  static constexpr size_t kSmem =
+      1024 + 2 * static_cast<size_t>(kQBytes) + kStages * static_cast<size_t>(kTileBytes) + kOutBytes;
 };
 
 // Rows of the attention: tokens of slots, or members of prefix groups.
@@ -74,7 +77,7 @@ struct PromptRows {
 
 // A unit's place on the line: its key tiles, and before them what entering and
 // leaving it costs, in key tiles.
-constexpr int kPairCost = 4;
+constexpr int kPairCost = 2;
 
 struct PromptSpace {
   int64_t* head;       // [0] pairs, [1] length of one key head's line, [2] length of a share
@@ -417,6 +420,11 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 __device__ __forceinline__ float max_nan(float a, float b, float c) {
   float r;
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -426,14 +434,14 @@ __device__ __forceinline__ float max_nan(float a, float b, float c) {
 // 2^x of two values on the FMA pipe: x = n + f with n the nearest whole number
 // (from the low bits of x + 1.5 * 2^23), 2^f by its minimax polynomial of
 // degree 4 on [-1/2, 1/2] (relative error 2.7e-6, far below the rounding of P),
-// n added to the exponent.  For x in [-126, 127]; smaller x gives 2^-126.
+// n added to the exponent.  x is held to [-126, 127].
 constexpr int kPolyOf8 = 2;  // of 8 pairs of probabilities, those computed this way
 
 __device__ __forceinline__ float2 ex2_poly(float2 x) {
   const float2 magic = make_float2(12582912.f, 12582912.f), back = make_float2(-12582912.f, -12582912.f);
   const float2 minus = make_float2(-1.f, -1.f);
-  x.x = max_nan(x.x, -126.f);
-  x.y = max_nan(x.y, -126.f);
+  x.x = min_nan(max_nan(x.x, -126.f), 127.f);
+  x.y = min_nan(max_nan(x.y, -126.f), 127.f);
   const float2 t = add2(x, magic);
   const float2 f = fma2(add2(t, back), minus, x);
   float2 p = make_float2(0x1.3997d6p-7f, 0x1.3997d6p-7f);
@@ -443,29 +451,6 @@ __device__ __forceinline__ float2 ex2_poly(float2 x) {
   p = fma2(p, f, make_float2(0x1.ffffe8p-1f, 0x1.ffffe8p-1f));
   return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
                      __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
-}
-
-// Starts a 32-column load; the registers are valid after tmem_ld_done names them.
-__device__ __forceinline__ void tmem_ld32_start(uint32_t (&v)[32], uint32_t taddr) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
-      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
-        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
-        "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
-        "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
-      : "r"(taddr)
-      : "memory");
-}
-__device__ __forceinline__ void tmem_ld_done(uint32_t (&v)[32]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
-                 "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]),
-                 "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]),
-                 "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]),
-                 "+r"(v[30]), "+r"(v[31])
-               :
-               : "memory");
 }
 
 // Warp-uniform forms: a wait succeeds, and the CTA goes on, for all lanes or none.
@@ -490,14 +475,16 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   using C = PromptCfg<D>;
   constexpr int S = C::kStages;
   constexpr int DB = D / 64;  // 64-dim blocks of a tile
-  constexpr uint32_t kSCol = 0, kOCol = 4 * kKeys;  // S of Q tile i, buffer b: column (2 i + b) kKeys
+  constexpr uint32_t kSCol = 0, kOCol = 2 * kKeys;  // S of Q tile i: column i kKeys, O: kOCol + i D
   extern __shared__ unsigned char prompt_smem[];
-  __shared__ unsigned long long kv_full[S], kv_empty[S], ready[S], q_ready[2], s_full[2][2], p_full[2][2], pv_done[2], skip[2], fin[2];
+  __shared__ unsigned long long kv_full[S], kv_empty[S], ready[S], q_ready[2], s_full[2], p_full[2][2], half_done[2],
+      o_full[2], skip[2], fin;
   __shared__ uint32_t tmem_base;
   __shared__ int err;
   const uint32_t pad = (1024u - (smem_addr(prompt_smem) & 1023u)) & 1023u;
   unsigned char* q_smem = prompt_smem + pad;
   unsigned char* ring = q_smem + 2 * C::kQBytes;
+  unsigned char* out_smem = ring + static_cast<size_t>(S) * C::kTileBytes;
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const bool prefix = rows.members != nullptr;
   const int tq = kTile / a.group;  // tokens of a Q tile
@@ -505,19 +492,19 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
       mbar_init(&kv_full[s], 1);
-      mbar_init(&kv_empty[s], 2);  // both issuing warps
+      mbar_init(&kv_empty[s], 1);
       mbar_init(&ready[s], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_ready[i], 4);
-      for (int b = 0; b < 2; ++b) {
-        mbar_init(&s_full[i][b], 1);
-        mbar_init(&p_full[i][b], 4);
-      }
-      mbar_init(&pv_done[i], 1);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i][0], 4);
+      mbar_init(&p_full[i][1], 4);
+      mbar_init(&half_done[i], 1);
+      mbar_init(&o_full[i], 1);
       mbar_init(&skip[i], 1);
-      mbar_init(&fin[i], 1);
     }
+    mbar_init(&fin, 1);
     err = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -537,11 +524,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   Walk w;
   const bool any = w.begin(ws, c.kv_heads, blockIdx.x);
 
-  // registers: 384 threads x 168 at launch = 128 x 88 + 2 x 128 x 208
+  // registers: 384 threads x 168 at launch = 128 x 88 + 256 x 208
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
   if (warp == 9) {
-    // ---- TMA producer.  Order: keys 0, keys 1, then values t, keys t + 2, as they are used.
+    // ---- TMA producer.  Order: keys 0, then values t, keys t + 1, as they are used.
     int it = 0;
     const int rows_per_box = min(kKeys, c.page_size), boxes = kKeys / rows_per_box;
     const int beyond = c.pages * c.layers * 2 * c.kv_heads * c.page_size;  // a row past the pool: reads zeros
@@ -572,16 +559,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         }
         return true;
       };
-      int page[3] = {page_of(w.t0), page_of(w.t0 + 1), page_of(w.t0 + 2)};  // of tiles t, t + 1, t + 2
-      bool ok = copy(w.t0, page[0], 0);
-      if (ok && w.t0 + 1 < w.t1) ok = copy(w.t0 + 1, page[1], 0);
+      int page = page_of(w.t0), next_page = page_of(w.t0 + 1);
+      bool ok = copy(w.t0, page, 0);
       for (int t = w.t0; ok && t < w.t1; ++t) {
-        const int ahead = page_of(t + 3);  // on its way while the copies wait for their stages
-        ok = copy(t, page[0], 1);
-        if (ok && t + 2 < w.t1) ok = copy(t + 2, page[2], 0);
-        page[0] = page[1];
-        page[1] = page[2];
-        page[2] = ahead;
+        const int ahead = page_of(t + 2);  // on its way while the copies wait for their stages
+        ok = copy(t, page, 1);
+        if (ok && t + 1 < w.t1) ok = copy(t + 1, next_page, 0);
+        page = next_page;
+        next_page = ahead;
       }
       if (!ok) *errv = 1;
     }
@@ -622,116 +607,126 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         return true;
       };
       bool ok = pass(-1);
-      if (ok && w.t0 + 1 < w.t1) ok = pass(-1);
       for (int t = w.t0; ok && t < w.t1; ++t) {
         ok = pass(t);
-        if (ok && t + 2 < w.t1) ok = pass(-1);
+        if (ok && t + 1 < w.t1) ok = pass(-1);
       }
       if (!ok) *errv = 1;
     }
-  } else {
-    // ---- MMA issuer of Q tile i: warp 8 or 11.  The whole warp walks along, so
-    // that what the instructions are given stays in uniform registers; one
-    // elected thread issues them.  Only the descriptors' low words change.
-    // (One warp for both tiles left the tensor pipe idle between its bursts:
-    // its own waits and commits took as long as the products.)
-    const int i = warp == 8 ? 0 : 1;
+  } else if (warp == 8) {
+    // ---- MMA issuer.  The whole warp walks along, so that what the
+    // instructions are given stays in uniform registers (from a single thread's
+    // branch an MMA took 89 cycles to issue instead of 64); one elected thread
+    // issues them.  Only the descriptors' low words change.
     int it = 0;  // ring position
-    int s_uses = 0, p_uses = 0, q_uses = 0;
-    const uint32_t q_lo = static_cast<uint32_t>(umma_desc_sw128(q_smem)) + i * (C::kQBytes >> 4);
+    int p_uses[2] = {0, 0}, q_uses = 0;
+    const uint32_t q_lo = static_cast<uint32_t>(umma_desc_sw128(q_smem));
     const uint32_t k_lo = static_cast<uint32_t>(umma_desc_sw128(ring));
     const uint32_t v_lo = static_cast<uint32_t>(value_desc(smem_addr(ring)));
-    const uint32_t s_tmem = tmem + kSCol + 2 * i * kKeys, o_tmem = tmem + kOCol + i * D;
-    constexpr uint32_t kTileStep = C::kTileBytes >> 4, kQBlock = (kTile * 128) >> 4, kKBlock = (kKeys * 128) >> 4;
+    constexpr uint32_t kTileStep = C::kTileBytes >> 4, kBlock = (kTile * 128) >> 4;
+    auto scores = [&](int i, int s) {  // S_i = Q_i K^T
+      const uint32_t qd = q_lo + i * (C::kQBytes >> 4), kd = k_lo + s * kTileStep;
+      if (elect_one()) {
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            umma_ss(tmem + kSCol + i * kKeys, qd + d * kBlock + 2 * kk, kd + d * kBlock + 2 * kk,
+                    prompt_idesc<T>(kKeys, false), (d | kk) != 0);
+        umma_commit(&s_full[i]);
+      }
+      __syncwarp();
+    };
     auto commit = [&](unsigned long long* bar) {
       if (elect_one()) umma_commit(bar);
       __syncwarp();
     };
-    // waits for the ring's next tile (keys); S = Q K^T into the next buffer if the tile is seen; lets the tile go
-    auto scores = [&](bool seen) {
-      const int s = it % S;
-      if (!wait_warp(&ready[s], (it / S) & 1)) return false;
-      ++it;
-      tmem_fence_after_sync();
-      const uint32_t kd = k_lo + s * kTileStep;
-      const int b = s_uses & 1;
-      if (seen) ++s_uses;
-      if (elect_one()) {
-        if (seen) {
-#pragma unroll
-          for (int d = 0; d < DB; ++d)
-#pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-              umma_ss(s_tmem + b * kKeys, q_lo + d * kQBlock + 2 * kk, kd + d * kKBlock + 2 * kk,
-                      prompt_idesc<T>(kKeys, false), (d | kk) != 0);
-          umma_commit(&s_full[i][b]);
-        }
-        umma_commit(&kv_empty[s]);
-      }
-      __syncwarp();
-      return true;
-    };
     bool more = any;
     while (more && alive(errv)) {
-      int p0, p1, q0, q1;
+      int p0, p1, q0[2], q1[2];
       positions(w.g, prefix, w.tok0, w.tok0 + 2 * tq, &p0, &p1);
-      positions(w.g, prefix, w.tok0 + i * tq, w.tok0 + (i + 1) * tq, &q0, &q1);
+      positions(w.g, prefix, w.tok0, w.tok0 + tq, &q0[0], &q1[0]);
+      positions(w.g, prefix, w.tok0 + tq, w.tok0 + 2 * tq, &q0[1], &q1[1]);
       const KeySpan span(p0, max(p0, p1), a.window, a.sinks);
-      const TilesSeen seen(q0, q1, a.window, a.sinks);
-      bool started = false;
+      const TilesSeen seen[2] = {TilesSeen(q0[0], q1[0], a.window, a.sinks), TilesSeen(q0[1], q1[1], a.window, a.sinks)};
+      bool started[2] = {false, false};
       const int t0 = w.t0, t1 = w.t1;
-      int last = t1 - 1;
-      while (last >= t0 && !seen.at(span.tile(last))) --last;
-      more = w.next(ws);  // its loads are on their way while this unit runs
-      bool ok = wait_warp(&q_ready[i], q_uses & 1);
-      ++q_uses;
-      // a Q tile without key tiles in this share: its warps must not run ahead of this one (a barrier of its own,
-      // since a warp may still be on its way to the last unit's pv_done)
-      if (ok && last < t0 && lane == 0) mbar_arrive(&skip[i]);
-      ok = ok && scores(seen.at(span.tile(t0)));
-      if (t0 + 1 < t1) ok = ok && scores(seen.at(span.tile(t0 + 1)));
-      for (int t = t0; ok && t < t1; ++t) {
-        const int vs = it % S;
-        ok = wait_warp(&ready[vs], (it / S) & 1);
-        ++it;
-        const bool use = seen.at(span.tile(t));
-        if (use && ok) {
-          const int b = p_uses & 1;
-          ok = wait_warp(&p_full[i][b], (p_uses >> 1) & 1);
-          ++p_uses;
-          if (ok) {
-            tmem_fence_after_sync();
-            const uint32_t vd = v_lo + vs * kTileStep;
-            if (elect_one()) {
+      int last[2];  // each Q tile's last key tile in this share
 #pragma unroll
-              for (int kk = 0; kk < kKeys / 16; ++kk)
-                umma_ts(o_tmem, s_tmem + b * kKeys + 8 * kk, vd + kk * (2048 >> 4), prompt_idesc<T>(D, true),
-                        started || kk != 0);
-              umma_commit(&pv_done[i]);
-              umma_commit(&kv_empty[vs]);
-            }
-            __syncwarp();
-            started = true;
-          }
-        } else if (ok) {
-          commit(&kv_empty[vs]);
+      for (int i = 0; i < 2; ++i) {
+        last[i] = t1 - 1;
+        while (last[i] >= t0 && !seen[i].at(span.tile(last[i]))) --last[i];
+      }
+      more = w.next(ws);  // its loads are on their way while this unit runs
+      bool ok = wait_warp(&ready[it % S], (it / S) & 1);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        ok = ok && wait_warp(&q_ready[i], q_uses & 1);
+        if (ok) {
+          tmem_fence_after_sync();
+          if (seen[i].at(span.tile(t0))) scores(i, it % S);
+          // a Q tile without key tiles in this share: its warps must not run ahead of this one (a barrier of its
+          // own, since a warp may still be on its way to the last unit's o_full)
+          if (last[i] < t0 && lane == 0) mbar_arrive(&skip[i]);
         }
-        if (t + 2 < t1) ok = ok && scores(seen.at(span.tile(t + 2)));
+      }
+      ++q_uses;
+      if (ok) commit(&kv_empty[it % S]);
+      ++it;
+      for (int t = t0; ok && t < t1; ++t) {
+        const int vs = it % S, ks = (it + 1) % S;
+        const bool next = t + 1 < t1;
+        ok = wait_warp(&ready[vs], (it / S) & 1);
+        if (next) ok = ok && wait_warp(&ready[ks], ((it + 1) / S) & 1);
+        const int j = span.tile(t), j1 = next ? span.tile(t + 1) : 0;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (seen[i].at(j)) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              ok = ok && wait_warp(&p_full[i][h], p_uses[i] & 1);
+              if (ok) {
+                tmem_fence_after_sync();
+                const uint32_t vd = v_lo + vs * kTileStep + h * (kHalf * 128 >> 4);
+                if (elect_one()) {
+#pragma unroll
+                  for (int kk = 0; kk < kHalf / 16; ++kk)
+                    umma_ts(tmem + kOCol + i * D, tmem + kSCol + i * kKeys + h * (kHalf / 2) + 8 * kk, vd + kk * (2048 >> 4),
+                            prompt_idesc<T>(D, true), started[i] || (h | kk) != 0);
+                  if (h == 0) umma_commit(&half_done[i]);
+                }
+                __syncwarp();
+              }
+            }
+            ++p_uses[i];
+            started[i] = true;
+            if (ok && t == last[i]) commit(&o_full[i]);
+          }
+          if (ok && next && seen[i].at(j1)) scores(i, ks);
+        }
+        if (ok) {
+          commit(&kv_empty[vs]);
+          if (next) commit(&kv_empty[ks]);
+          it += next ? 2 : 1;
+        }
       }
       if (!ok) *errv = 1;
     }
     // every MMA this warp issued has completed before tensor memory is freed
-    commit(&fin[i]);
-    wait_warp(&fin[i], 0);
+    commit(&fin);
+    wait_warp(&fin, 0);
   }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     // ---- softmax of Q tile i: thread r is its row r
     const int i = warp >> 2, r = threadIdx.x & 127;
     const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
-    const uint32_t s_cols = tmem + kSCol + 2 * i * kKeys + lanes, o_col = tmem + kOCol + i * D + lanes;
+    const uint32_t s_col = tmem + kSCol + i * kKeys + lanes, o_col = tmem + kOCol + i * D + lanes;
     const int tok_in_tile = r / a.group, head_in_group = r % a.group;
-    int s_uses = 0, pv_uses = 0, skips = 0;  // pv_uses: products asked for so far
+    // Whole rows go to and from global memory: 8 lanes a 128-byte piece, 4 rows at a time (a thread per row would
+    // touch 32 sectors with every instruction, which took longer than several key tiles).
+    const int piece = lane & 7, sub_row = lane >> 3;
+    int s_uses = 0, o_uses = 0, skips = 0;
     // this thread's row of unit u: q and out row, or -1
     auto row_of = [&](const Walk& u) {
       const int tok = u.tok0 + i * tq + tok_in_tile;
@@ -741,20 +736,26 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       const int slot = rows.members[row];
       return slot >= 0 && slot < a.rows ? slot : -1;
     };
-    // its queries into shared memory, for the MMA warp
+    // the warp's 32 rows of queries into shared memory, for the MMA warp
     auto load_q = [&](const Walk& u, int row) {
-      const uint16_t* src = a.q + row * a.q_row + static_cast<int64_t>(u.head * a.group + head_in_group) * D;
-      unsigned char* dst = q_smem + i * C::kQBytes + r * 128;
-      uint4 v[DB][8];
+      const uint16_t* src = a.q + static_cast<int64_t>(u.head * a.group) * D + 8 * piece;
+      unsigned char* dst = q_smem + i * C::kQBytes + 32 * (warp & 3) * 128;
 #pragma unroll
-      for (int b = 0; b < DB; ++b)
+      for (int b = 0; b < DB; ++b) {
+        uint4 v[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-          v[b][k] = row >= 0 ? *reinterpret_cast<const uint4*>(src + 64 * b + 8 * k) : make_uint4(0, 0, 0, 0);
+        for (int k = 0; k < 8; ++k) {
+          const int from = 4 * k + sub_row;
+          const int q_row = __shfl_sync(0xffffffffu, row, from), h = __shfl_sync(0xffffffffu, head_in_group, from);
+          v[k] = q_row >= 0 ? *reinterpret_cast<const uint4*>(src + q_row * a.q_row + h * D + 64 * b)
+                            : make_uint4(0, 0, 0, 0);
+        }
 #pragma unroll
-      for (int b = 0; b < DB; ++b)
-#pragma unroll
-        for (int k = 0; k < 8; ++k) *reinterpret_cast<uint4*>(dst + b * (kTile * 128) + 16 * (k ^ (r & 7))) = v[b][k];
+        for (int k = 0; k < 8; ++k) {
+          const int to = 4 * k + sub_row;
+          *reinterpret_cast<uint4*>(dst + b * (kTile * 128) + to * 128 + 16 * (piece ^ (to & 7))) = v[k];
+        }
+      }
       fence_proxy_async();
       __syncwarp();
       if (lane == 0) mbar_arrive(&q_ready[i]);
@@ -765,117 +766,113 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       load_q(w, q_row);
     }
     for (bool more = any; more && alive(errv);) {
-      const Geom g = w.g;
       int p0, p1, q0, q1;
-      positions(g, prefix, w.tok0, w.tok0 + 2 * tq, &p0, &p1);
-      positions(g, prefix, w.tok0 + i * tq, w.tok0 + (i + 1) * tq, &q0, &q1);
+      positions(w.g, prefix, w.tok0, w.tok0 + 2 * tq, &p0, &p1);
+      positions(w.g, prefix, w.tok0 + i * tq, w.tok0 + (i + 1) * tq, &q0, &q1);
       const KeySpan span(p0, max(p0, p1), a.window, a.sinks);
       const TilesSeen seen(q0, q1, a.window, a.sinks);
-      const int pos = prefix ? g.len - 1 : g.len - g.count + w.tok0 + i * tq + tok_in_tile;
-      const bool* mask = a.key_mask != nullptr ? a.key_mask + g.key_slot * a.mask_stride : nullptr;
-      float m = -CUDART_INF_F;
-      float2 l2 = make_float2(0.f, 0.f);
+      const int len = w.g.len;
+      const int pos = prefix ? len - 1 : len - w.g.count + w.tok0 + i * tq + tok_in_tile;
+      const bool* mask = a.key_mask != nullptr ? a.key_mask + w.g.key_slot * a.mask_stride : nullptr;
+      float m = -CUDART_INF_F, l = 0.f;
       bool ok = true, started = false;
       for (int t = w.t0; t < w.t1; ++t) {
         const int j = span.tile(t);
         if (!seen.at(j)) continue;
         const int base = kKeys * j;
-        uint32_t see[2] = {0xffffffffu, 0xffffffffu};
-        const bool all = mask == nullptr && tile_full(j, q0, q1, a.window, a.sinks) && base + kKeys <= g.len;
+        uint32_t see[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+        const bool all = mask == nullptr && tile_full(j, q0, q1, a.window, a.sinks) && base + kKeys <= len;
         if (!all) {
-          const int hi = min(pos + 1, g.len) - base;
+          const int hi = min(pos + 1, len) - base;
           const int lo = a.window > 0 ? max(max(pos + 1 - base, 0) - a.window, 0) : 0;
-          const int sk = min(a.sinks, kKeys * (j + 1)) - base;
+          const int sk = min(a.sinks, base + kKeys) - base;
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
+          for (int x = 0; x < 4; ++x) {
             see[x] = bit_range(0, hi - 32 * x) & (bit_range(lo - 32 * x, 32) | bit_range(0, sk - 32 * x));
             if (mask != nullptr) {
               const int k = base + 32 * x + lane;
-              see[x] &= __ballot_sync(0xffffffffu, k < g.len && mask[k]);
+              see[x] &= __ballot_sync(0xffffffffu, k < len && mask[k]);
             }
           }
         }
-        const int buf = s_uses & 1;
-        const uint32_t s_col = s_cols + buf * kKeys;
-        ok = wait_warp(&s_full[i][buf], (s_uses >> 1) & 1);
-        ++s_uses;
+        ok = wait_warp(&s_full[i], s_uses & 1);
         if (!ok) break;
         tmem_fence_after_sync();
-        uint32_t s[64];
-        tmem_ld64(s, s_col);
+        uint32_t s[128];
+        tmem_ld64(*reinterpret_cast<uint32_t(*)[64]>(s), s_col);
+        tmem_ld64(*reinterpret_cast<uint32_t(*)[64]>(s + 64), s_col + 64);
         if (!all) {
 #pragma unroll
-          for (int k = 0; k < 64; ++k)
+          for (int k = 0; k < 128; ++k)
             if (!((see[k >> 5] >> (k & 31)) & 1u)) s[k] = 0xff800000u;
         }
-        float tops[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          tops[k] = max_nan(m, __uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1]));
+        for (int h = 0; h < 2; ++h) {
+          float sum;
+          auto probabilities = [&](auto poly) {
+            const float off = m == -CUDART_INF_F ? 0.f : -m * a.scale2;
+            const float2 scale = make_float2(a.scale2, a.scale2), offs = make_float2(off, off);
+            float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-        for (int k = 4; k < 32; ++k)
-          tops[k & 3] = max_nan(tops[k & 3], __uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1]));
-        const float top = max_nan(max_nan(tops[0], tops[1]), tops[2], tops[3]);
-        // the maximum in use moves only when it must
-        const bool move = m == -CUDART_INF_F ? !(top <= m) : !((top - m) * a.scale2 <= 8.f);  // a NaN moves it too
-        if (__any_sync(0xffffffffu, move)) {
-          if (started && __any_sync(0xffffffffu, move && m != -CUDART_INF_F)) {
-            // the product before this tile's must be in O (the one before that is: this tile's scores came after it)
-            ok = wait_warp(&pv_done[i], (pv_uses - 1) & 1);
-            if (!ok) break;
-            tmem_fence_after_sync();
-            const float f = move && m != -CUDART_INF_F ? ex2((m - top) * a.scale2) : 1.f;
-            l2.x *= f;
-            l2.y *= f;
+            for (int x = 0; x < 2; ++x) {
+              uint32_t p[16];
 #pragma unroll
-            for (int b = 0; b < D / 16; ++b) {
-              uint32_t o[16];
-              tmem_ld16(o, o_col + 16 * b);
-#pragma unroll
-              for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-              tmem_st16(o_col + 16 * b, o);
-            }
-          }
-          if (move) m = top;
-        }
-        const float off = m == -CUDART_INF_F ? 0.f : -m * a.scale2;
-        const float2 scale = make_float2(a.scale2, a.scale2), offs = make_float2(off, off);
-        float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-        auto exps = [&](auto poly) {
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            uint32_t p[16];
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {
-              const int e = 32 * x + 2 * k;
-              float2 v = fma2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), scale, offs);
-              if (decltype(poly)::value && (k & 7) < kPolyOf8) {
-                v = ex2_poly(v);
-              } else {
-                v.x = ex2(v.x);
-                v.y = ex2(v.y);
+              for (int k = 0; k < 16; ++k) {
+                const int e = kHalf * h + 32 * x + 2 * k;
+                float2 v = fma2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), scale, offs);
+                if (decltype(poly)::value && (k & 7) < kPolyOf8) {
+                  v = ex2_poly(v);
+                } else {
+                  v.x = ex2(v.x);
+                  v.y = ex2(v.y);
+                }
+                // the sum keeps the unrounded probabilities; the values' weights are rounded to 16 bits once
+                sums[k & 1] = add2(sums[k & 1], v);
+                p[k] = Half16<T>::pack(v.x, v.y);
               }
-              // the sum keeps the unrounded probabilities; the values' weights are rounded to 16 bits once
-              sums[k & 1] = add2(sums[k & 1], v);
-              p[k] = Half16<T>::pack(v.x, v.y);
+              tmem_st16(s_col + (kHalf / 2) * h + 16 * x, p);
             }
-            tmem_st16(s_col + 16 * x, p);
+            sums[0] = add2(sums[0], sums[1]);
+            sum = sums[0].x + sums[0].y;
+          };
+          bool again = h == 0 && !started;
+          if (!again) {
+            // masked scores (-inf) must come out as exact zeros: the special function unit alone
+            if (all) probabilities(std::true_type{}); else probabilities(std::false_type{});
+            again = __any_sync(0xffffffffu, !(sum <= 32768.f) || m == -CUDART_INF_F);
           }
-        };
-        // masked scores (-inf) must come out as exact zeros: the special function unit alone
-        if (all) {
-          exps(std::true_type{});
-        } else {
-          exps(std::false_type{});
+          if (again) {
+            float top = m;
+#pragma unroll
+            for (int k = 0; k < kHalf; k += 2)
+              top = max_nan(top, __uint_as_float(s[kHalf * h + k]), __uint_as_float(s[kHalf * h + k + 1]));
+            if (started || h == 1) {
+              // the products so far must be in O: those of the tiles before are (these scores came after them)
+              if (h == 1) ok = wait_warp(&half_done[i], s_uses & 1);
+              if (!ok) break;
+              tmem_fence_after_sync();
+              const float f = m == -CUDART_INF_F ? 1.f : ex2((m - top) * a.scale2);
+              l *= f;
+#pragma unroll
+              for (int b = 0; b < D / 16; ++b) {
+                uint32_t o[16];
+                tmem_ld16(o, o_col + 16 * b);
+#pragma unroll
+                for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+                tmem_st16(o_col + 16 * b, o);
+              }
+            }
+            m = top;
+            probabilities(std::false_type{});
+          }
+          l += sum;
+          tmem_wait_st();
+          tmem_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[i][h]);
         }
-        l2 = add2(l2, add2(sums[0], sums[1]));
-        tmem_wait_st();
-        tmem_fence_before_sync();
-        // not before the product of the tile before is done: so pv_done is never two phases away from a wait for it
-        if (started) ok = wait_warp(&pv_done[i], (pv_uses - 1) & 1);
         if (!ok) break;
-        if (lane == 0) mbar_arrive(&p_full[i][buf]);
-        ++pv_uses;
+        ++s_uses;
         started = true;
       }
       // The next unit's queries go in before this one's result comes out: the
@@ -890,13 +887,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         next_row = row_of(v);
         load_q(v, next_row);
       }
-      if (ok && started) ok = wait_warp(&pv_done[i], (pv_uses - 1) & 1);
-      tmem_fence_after_sync();
+      if (ok && started) ok = wait_warp(&o_full[i], o_uses++ & 1);
       if (!ok) {
         *errv = 1;
         break;
       }
-      const float l = l2.x + l2.y;
+      tmem_fence_after_sync();
       const float inv = l == 0.f ? 0.f : 1.f / l;
       const float m2 = m == -CUDART_INF_F ? m : m * a.scale2;
       const bool whole = w.whole(), there = q_row >= 0;
@@ -904,35 +900,54 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       float* part = ws.part + (2 * static_cast<int64_t>(blockIdx.x) + w.part(blockIdx.x)) * (D + 2) * kPairRows +
                     i * kTile + r;
       float* state = prefix && there ? rows.state + (static_cast<int64_t>(q_row) * a.q_heads + q_head) * (D + 4) : nullptr;
-      uint16_t* out = a.out + q_row * a.out_row + static_cast<int64_t>(q_head) * D;
+      unsigned char* stage = out_smem + warp * (32 * 128);
 #pragma unroll
-      for (int b = 0; b < D / 32; ++b) {
-        uint32_t o[32];
-        tmem_ld32(o, o_col + 32 * b);
-        if (!started) {
+      for (int b = 0; b < DB; ++b) {
 #pragma unroll
-          for (int k = 0; k < 32; ++k) o[k] = 0u;
-        }
-        if (!there) {
-        } else if (!whole) {
+        for (int half = 0; half < 2; ++half) {
+          uint32_t o[32];
+          tmem_ld32(o, o_col + 64 * b + 32 * half);
+          if (!started) {
 #pragma unroll
-          for (int k = 0; k < 32; ++k) part[(32 * b + k) * kPairRows] = __uint_as_float(o[k]);
-        } else if (prefix) {
-#pragma unroll
-          for (int k = 0; k < 8; ++k)
-            *reinterpret_cast<uint4*>(state + 32 * b + 4 * k) = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
-        } else {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            uint4 y;
-            y.x = Half16<T>::pack(__uint_as_float(o[8 * k]) * inv, __uint_as_float(o[8 * k + 1]) * inv);
-            y.y = Half16<T>::pack(__uint_as_float(o[8 * k + 2]) * inv, __uint_as_float(o[8 * k + 3]) * inv);
-            y.z = Half16<T>::pack(__uint_as_float(o[8 * k + 4]) * inv, __uint_as_float(o[8 * k + 5]) * inv);
-            y.w = Half16<T>::pack(__uint_as_float(o[8 * k + 6]) * inv, __uint_as_float(o[8 * k + 7]) * inv);
-            *reinterpret_cast<uint4*>(out + 32 * b + 8 * k) = y;
+            for (int k = 0; k < 32; ++k) o[k] = 0u;
           }
+          if (!whole) {
+            if (there) {
+#pragma unroll
+              for (int k = 0; k < 32; ++k) part[(64 * b + 32 * half + k) * kPairRows] = __uint_as_float(o[k]);
+            }
+          } else if (prefix) {
+            if (there) {
+#pragma unroll
+              for (int k = 0; k < 8; ++k)
+                *reinterpret_cast<uint4*>(state + 64 * b + 32 * half + 4 * k) =
+                    make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+            }
+          } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              uint4 y;
+              y.x = Half16<T>::pack(__uint_as_float(o[8 * k]) * inv, __uint_as_float(o[8 * k + 1]) * inv);
+              y.y = Half16<T>::pack(__uint_as_float(o[8 * k + 2]) * inv, __uint_as_float(o[8 * k + 3]) * inv);
+              y.z = Half16<T>::pack(__uint_as_float(o[8 * k + 4]) * inv, __uint_as_float(o[8 * k + 5]) * inv);
+              y.w = Half16<T>::pack(__uint_as_float(o[8 * k + 6]) * inv, __uint_as_float(o[8 * k + 7]) * inv);
+              *reinterpret_cast<uint4*>(stage + lane * 128 + 16 * ((4 * half + k) ^ (lane & 7))) = y;
+            }
+          }
+          __syncwarp();
         }
-        __syncwarp();
+        if (whole && !prefix) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int from = 4 * k + sub_row;
+            const int row = __shfl_sync(0xffffffffu, q_row, from), h = __shfl_sync(0xffffffffu, head_in_group, from);
+            const uint4 y = *reinterpret_cast<const uint4*>(stage + from * 128 + 16 * (piece ^ (from & 7)));
+            if (row >= 0)
+              *reinterpret_cast<uint4*>(a.out + row * a.out_row + static_cast<int64_t>(w.head * a.group + h) * D + 64 * b +
+                                        8 * piece) = y;
+          }
+          __syncwarp();
+        }
       }
       if (there) {
         if (!whole) {
@@ -944,6 +959,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           a.lse[static_cast<int64_t>(q_row) * a.q_heads + q_head] = (m2 + log2f(l)) * kLn2;
         }
       }
+      tmem_fence_before_sync();
       w = v;
       q_row = next_row;
     }

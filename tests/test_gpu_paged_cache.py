@@ -359,6 +359,24 @@ def test_large_scores_and_infinities(pc):
     agree(got, lse, ref, torch.bfloat16, 300)
 
 
+@pytest.mark.parametrize("d,dtype", [(64, torch.bfloat16), (128, torch.float16), (128, torch.bfloat16)])
+def test_prompt_scores_that_climb(pc, d, dtype):
+    """Scores that grow along the keys, slowly and in jumps far past the range of an f16 or an f32 exponential:
+    the running maximum has to move again and again."""
+    n = 700
+    cache, pool, table = make(pc, [n], 2, d, dtype=dtype)
+    rise = torch.cat([torch.linspace(0, 6, 400), torch.linspace(20, 60, 200), torch.full((100,), 200.0)])
+    for j in range(n):
+        pool[table[0, j // 16], :, 0, :, j % 16] = (pool[table[0, j // 16], :, 0, :, j % 16] * 0.1).to(dtype)
+        pool[table[0, j // 16], :, 0, :, j % 16, 0] = rise[j].to(dtype)
+    cache.pool.copy_(pool)
+    q = (0.1 * queries(n, 2, d, dtype).float()).to(dtype)
+    q[:, :, 0] = 2.0
+    ref = O.attention(pool, table, [n], 0, q, [0, n], scale=0.7)
+    got, lse = cache.attend(0, q.cuda(), offsets=i32([0, n]), scale=0.7, return_lse=True)
+    agree(got, lse, ref, dtype, n)
+
+
 def test_same_bits_every_time(pc):
     """Work is split and joined in an order that does not depend on timing."""
     cache, _, _ = make(pc, [3000, 17, 900, 2500], 2, seed=3)
