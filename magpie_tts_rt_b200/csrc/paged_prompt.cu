@@ -798,16 +798,17 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         ok = wait_warp(&s_full[i], s_uses & 1);
         if (!ok) break;
         tmem_fence_after_sync();
-        uint32_t s[128];
-        tmem_ld64(*reinterpret_cast<uint32_t(*)[64]>(s), s_col);
-        tmem_ld64(*reinterpret_cast<uint32_t(*)[64]>(s + 64), s_col + 64);
-        if (!all) {
-#pragma unroll
-          for (int k = 0; k < 128; ++k)
-            if (!((see[k >> 5] >> (k & 31)) & 1u)) s[k] = 0xff800000u;
-        }
+        // One half after the other, so that 64 scores are held and not 128: P of
+        // the first half goes over the first half's scores alone.
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
+          uint32_t s[kHalf];
+          tmem_ld64(s, s_col + kHalf * h);
+          if (!all) {
+#pragma unroll
+            for (int k = 0; k < kHalf; ++k)
+              if (!((see[2 * h + (k >> 5)] >> (k & 31)) & 1u)) s[k] = 0xff800000u;
+          }
           float sum;
           auto probabilities = [&](auto poly) {
             const float off = m == -CUDART_INF_F ? 0.f : -m * a.scale2;
@@ -818,7 +819,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
               uint32_t p[16];
 #pragma unroll
               for (int k = 0; k < 16; ++k) {
-                const int e = kHalf * h + 32 * x + 2 * k;
+                const int e = 32 * x + 2 * k;
                 float2 v = fma2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), scale, offs);
                 if (decltype(poly)::value && (k & 7) < kPolyOf8) {
                   v = ex2_poly(v);
@@ -845,7 +846,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             float top = m;
 #pragma unroll
             for (int k = 0; k < kHalf; k += 2)
-              top = max_nan(top, __uint_as_float(s[kHalf * h + k]), __uint_as_float(s[kHalf * h + k + 1]));
+              top = max_nan(top, __uint_as_float(s[k]), __uint_as_float(s[k + 1]));
             if (started || h == 1) {
               // the products so far must be in O: those of the tiles before are (these scores came after them)
               if (h == 1) ok = wait_warp(&half_done[i], s_uses & 1);
