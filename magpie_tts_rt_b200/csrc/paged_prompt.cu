@@ -8,8 +8,7 @@
 // A unit is a key head and two Q tiles of 128 rows; a tile's rows are the
 // group's query heads of consecutive tokens (128 / group of them), so shared
 // key heads fill the MMA's 128 rows and every key tile in shared memory is
-// used by both Q tiles.  Warp roles (384 threads, one CTA per SM; the softmax
-// warps take registers over from the others):
+// used by both Q tiles.  Warp roles (384 threads, one CTA per SM):
 //   warps 0-3, 4-7  softmax of Q tile 0 / 1: one thread per row reads S from
 //                   tensor memory, writes P over it in 16 bits (the A operand
 //                   of the second product), half a tile at a time, and stores
@@ -20,7 +19,10 @@
 //   warp 9          TMA: the pages of each key tile into a ring of stages
 //                   (128-byte swizzle);
 //   warp 10         clears value rows that no query may see (page tails,
-//                   masked keys), whose probability of 0 must not meet a NaN.
+//                   masked keys), whose probability of 0 must not meet a NaN;
+//   warp 11         TMA: the next unit's queries, as soon as the last scores
+//                   of this one are done (the prefix pass's rows lie apart, so
+//                   there the softmax warps copy them).
 // Tensor memory: S0, S1 (128 columns each), O0, O1 (head_dim each), which at
 // head_dim 128 is all of it.
 //
@@ -72,6 +74,7 @@ struct PromptRows {
   const int32_t* tokens;     // prefix pass: [n] its length
   int longest;               // prefix pass: longer prefixes are not shared (the window hides some of them)
   int32_t* base;             // prefix pass: [slots] out, SharedPrefix::base
+  bool q_mapped;             // the query map describes q: tiles come by TMA
   float* state;              // prefix pass: [slots][q_heads][D + 4]: O, m, l of each member
 };
 
@@ -276,28 +279,28 @@ __global__ void __launch_bounds__(kPromptPlanThreads)
 // a CTA's share, unit by unit
 // ---------------------------------------------------------------------------
 
+// Places are counted from the start of the CTA's share.
 struct Walk {
-  int64_t x, end, per;
-  int line, pairs, head, pair;
+  int end;          // of the share
+  int place;        // where the unit begins (before the share, when another CTA holds its beginning)
+  int pairs, head, pair;
   int tok0, n;      // the unit's first token (or member) and key tiles
   Geom g;
   int t0, t1;       // its key tiles in this share
-  int64_t unit_x;   // where it begins on the line
 
   __device__ __forceinline__ bool begin(const PromptSpace& ws, int kv_heads, int cta) {
     pairs = static_cast<int>(ws.head[0]);
-    line = static_cast<int>(ws.head[1]);
-    per = ws.head[2];
-    x = cta * per;
-    end = min(static_cast<int64_t>(line) * kv_heads, x + per);
-    if (x >= end) return false;
+    const int64_t line = ws.head[1], per = ws.head[2], x = cta * per;
+    if (x >= line * kv_heads) return false;
+    end = static_cast<int>(min(line * kv_heads - x, per));
     head = static_cast<int>(x / line);
     pair = ws.cta_pair[cta];
+    place = static_cast<int>(ws.rec[2 * pair].w - (x - head * line));
     return load(ws);
   }
   __device__ __forceinline__ bool next(const PromptSpace& ws) {
-    x = unit_x + kPairCost + n;
-    if (x >= end) return false;
+    place += kPairCost + n;
+    if (place >= end) return false;
     ++pair;
     return load(ws);
   }
@@ -317,14 +320,13 @@ struct Walk {
     tok0 = rec.x;
     n = rec.z;
     g = Geom{at.x, at.y, at.z, at.w};
-    unit_x = static_cast<int64_t>(head) * line + rec.w;
-    t0 = static_cast<int>(max(x - unit_x - kPairCost, static_cast<int64_t>(0)));
-    t1 = static_cast<int>(min(static_cast<int64_t>(n), end - unit_x - kPairCost));
+    t0 = max(-place - kPairCost, 0);
+    t1 = min(n, end - place - kPairCost);
     return t1 > 0;
   }
   __device__ __forceinline__ bool whole() const { return t0 == 0 && t1 == n; }
   // which of its CTA's two parts a cut unit leaves
-  __device__ __forceinline__ int part(int cta) const { return cta * per >= unit_x ? 0 : 1; }
+  __device__ __forceinline__ int part() const { return place <= 0 ? 0 : 1; }
 };
 
 // 128-byte-swizzled MN-major operand (values: [keys][64 dims] rows of 128
@@ -414,43 +416,19 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return pair2(d);
 }
 
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-
-__device__ __forceinline__ float min_nan(float a, float b) {
-  float r;
-  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
+// NaN if any of the three is.
 __device__ __forceinline__ float max_nan(float a, float b, float c) {
   float r;
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 
-// 2^x of two values on the FMA pipe: x = n + f with n the nearest whole number
-// (from the low bits of x + 1.5 * 2^23), 2^f by its minimax polynomial of
-// degree 4 on [-1/2, 1/2] (relative error 2.7e-6, far below the rounding of P),
-// n added to the exponent.  x is held to [-126, 127].
-constexpr int kPolyOf8 = 2;  // of 8 pairs of probabilities, those computed this way
-
-__device__ __forceinline__ float2 ex2_poly(float2 x) {
-  const float2 magic = make_float2(12582912.f, 12582912.f), back = make_float2(-12582912.f, -12582912.f);
-  const float2 minus = make_float2(-1.f, -1.f);
-  x.x = min_nan(max_nan(x.x, -126.f), 127.f);
-  x.y = min_nan(max_nan(x.y, -126.f), 127.f);
-  const float2 t = add2(x, magic);
-  const float2 f = fma2(add2(t, back), minus, x);
-  float2 p = make_float2(0x1.3997d6p-7f, 0x1.3997d6p-7f);
-  p = fma2(p, f, make_float2(0x1.ca1442p-5f, 0x1.ca1442p-5f));
-  p = fma2(p, f, make_float2(0x1.ec06dap-3f, 0x1.ec06dap-3f));
-  p = fma2(p, f, make_float2(0x1.62e0dcp-1f, 0x1.62e0dcp-1f));
-  p = fma2(p, f, make_float2(0x1.ffffe8p-1f, 0x1.ffffe8p-1f));
-  return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
-                     __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z,
+                                            unsigned long long* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+      ::"r"(smem_addr(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_addr(bar))
+      : "memory");
 }
 
 // Warp-uniform forms: a wait succeeds, and the CTA goes on, for all lanes or none.
@@ -468,9 +446,16 @@ __device__ __forceinline__ uint32_t bit_range(int lo, int hi) {
   return up & ~((1u << lo) - 1u);
 }
 
+// The key tiles of a unit: those that either of its Q tiles may see.
+__device__ __forceinline__ KeySpan unit_span(const Walk& w, bool prefix, int tq, const Attend& a) {
+  int p0, p1;
+  positions(w.g, prefix, w.tok0, w.tok0 + 2 * tq, &p0, &p1);
+  return KeySpan(p0, max(p0, p1), a.window, a.sinks);
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kPromptThreads, 1)
-    prompt_kernel(const __grid_constant__ CUtensorMap pool_map, PagedCache c, Attend a, PromptRows rows,
+    prompt_kernel(const __grid_constant__ CUtensorMap pool_map, const __grid_constant__ CUtensorMap q_map, PagedCache c, Attend a, PromptRows rows,
                   PromptSpace ws) {
   using C = PromptCfg<D>;
   constexpr int S = C::kStages;
@@ -478,9 +463,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   constexpr uint32_t kSCol = 0, kOCol = 2 * kKeys;  // S of Q tile i: column i kKeys, O: kOCol + i D
   extern __shared__ unsigned char prompt_smem[];
   __shared__ unsigned long long kv_full[S], kv_empty[S], ready[S], q_ready[2], s_full[2], p_full[2][2], half_done[2],
-      o_full[2], skip[2], fin;
+      o_full[2], q_free[2], fin;
   __shared__ uint32_t tmem_base;
-  __shared__ int err;
+  __shared__ int err, unit_slot;  // unit_slot: whose unit the softmax warps are at
   const uint32_t pad = (1024u - (smem_addr(prompt_smem) & 1023u)) & 1023u;
   unsigned char* q_smem = prompt_smem + pad;
   unsigned char* ring = q_smem + 2 * C::kQBytes;
@@ -496,16 +481,17 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       mbar_init(&ready[s], 1);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&q_ready[i], 4);
+      mbar_init(&q_ready[i], rows.q_mapped ? 1 : 4);
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i][0], 4);
       mbar_init(&p_full[i][1], 4);
       mbar_init(&half_done[i], 1);
       mbar_init(&o_full[i], 1);
-      mbar_init(&skip[i], 1);
+      mbar_init(&q_free[i], 1);
     }
     mbar_init(&fin, 1);
     err = 0;
+    unit_slot = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 8) {
@@ -524,9 +510,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   Walk w;
   const bool any = w.begin(ws, c.kv_heads, blockIdx.x);
 
-  // registers: 384 threads x 168 at launch = 128 x 88 + 256 x 208
-  if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
   if (warp == 9) {
     // ---- TMA producer.  Order: keys 0, then values t, keys t + 1, as they are used.
     int it = 0;
@@ -534,9 +517,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     const int beyond = c.pages * c.layers * 2 * c.kv_heads * c.page_size;  // a row past the pool: reads zeros
     for (bool more = any; more && alive(errv); more = w.next(ws)) {
       const Geom g = w.g;
-      int p0, p1;
-      positions(g, prefix, w.tok0, w.tok0 + 2 * tq, &p0, &p1);
-      const KeySpan span(p0, max(p0, p1), a.window, a.sinks);
+      const KeySpan span = unit_span(w, prefix, tq, a);
       const int32_t* table = c.table + static_cast<int64_t>(g.key_slot) * c.table_pages;
       // the row of the pool, before the choice of keys or values, where lane's box of tile t begins
       auto page_of = [&](int t) {
@@ -579,9 +560,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     int it = 0;
     for (bool more = any; more && alive(errv); more = w.next(ws)) {
       const Geom g = w.g;
-      int p0, p1;
-      positions(g, prefix, w.tok0, w.tok0 + 2 * tq, &p0, &p1);
-      const KeySpan span(p0, max(p0, p1), a.window, a.sinks);
+      const KeySpan span = unit_span(w, prefix, tq, a);
       const bool* mask = a.key_mask != nullptr ? a.key_mask + g.key_slot * a.mask_stride : nullptr;
       auto pass = [&](int t) {  // the ring's next tile: values of tile t, or keys (t < 0)
         const int s = it % S;
@@ -613,6 +592,27 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       }
       if (!ok) *errv = 1;
     }
+  } else if (warp == 11) {
+    // ---- queries: a box of 64 dims x the group's heads x the tile's tokens, whose rows are the tile's
+    int unit = 0;
+    for (bool more = any && rows.q_mapped; more && alive(errv); more = w.next(ws), ++unit) {
+      bool ok = true;
+      for (int i = 0; ok && i < 2; ++i) {
+        if (unit > 0) ok = wait_warp(&q_free[i], (unit - 1) & 1);
+        if (ok && lane == 0) {
+          mbar_expect_tx(&q_ready[i], static_cast<uint32_t>(tq * a.group * D * 2));
+#pragma unroll
+          for (int b = 0; b < DB; ++b)
+            tma_load_3d(q_smem + i * C::kQBytes + b * (kTile * 128), &q_map, 64 * b, w.head * a.group,
+                        w.g.row0 + w.tok0 + i * tq, &q_ready[i]);
+        }
+        __syncwarp();
+      }
+      if (!ok) *errv = 1;
+    }
+    // no copy may still be landing in shared memory when the CTA leaves
+    if (lane == 0 && unit > 0)
+      for (int i = 0; i < 2; ++i) mbar_wait_cta(&q_ready[i], (unit - 1) & 1);
   } else if (warp == 8) {
     // ---- MMA issuer.  The whole warp walks along, so that what the
     // instructions are given stays in uniform registers (from a single thread's
@@ -643,11 +643,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     };
     bool more = any;
     while (more && alive(errv)) {
-      int p0, p1, q0[2], q1[2];
-      positions(w.g, prefix, w.tok0, w.tok0 + 2 * tq, &p0, &p1);
+      int q0[2], q1[2];
       positions(w.g, prefix, w.tok0, w.tok0 + tq, &q0[0], &q1[0]);
       positions(w.g, prefix, w.tok0 + tq, w.tok0 + 2 * tq, &q0[1], &q1[1]);
-      const KeySpan span(p0, max(p0, p1), a.window, a.sinks);
+      const KeySpan span = unit_span(w, prefix, tq, a);
       const TilesSeen seen[2] = {TilesSeen(q0[0], q1[0], a.window, a.sinks), TilesSeen(q0[1], q1[1], a.window, a.sinks)};
       bool started[2] = {false, false};
       const int t0 = w.t0, t1 = w.t1;
@@ -665,9 +664,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         if (ok) {
           tmem_fence_after_sync();
           if (seen[i].at(span.tile(t0))) scores(i, it % S);
-          // a Q tile without key tiles in this share: its warps must not run ahead of this one (a barrier of its
-          // own, since a warp may still be on its way to the last unit's o_full)
-          if (last[i] < t0 && lane == 0) mbar_arrive(&skip[i]);
+          if (last[i] <= t0) commit(&q_free[i]);  // (a Q tile without key tiles in this share: at once)
         }
       }
       ++q_uses;
@@ -702,7 +699,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             started[i] = true;
             if (ok && t == last[i]) commit(&o_full[i]);
           }
-          if (ok && next && seen[i].at(j1)) scores(i, ks);
+          if (ok && next && seen[i].at(j1)) {
+            scores(i, ks);
+            if (t + 1 == last[i]) commit(&q_free[i]);
+          }
         }
         if (ok) {
           commit(&kv_empty[vs]);
@@ -715,28 +715,24 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     // every MMA this warp issued has completed before tensor memory is freed
     commit(&fin);
     wait_warp(&fin, 0);
-  }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     // ---- softmax of Q tile i: thread r is its row r
     const int i = warp >> 2, r = threadIdx.x & 127;
     const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
     const uint32_t s_col = tmem + kSCol + i * kKeys + lanes, o_col = tmem + kOCol + i * D + lanes;
     const int tok_in_tile = r / a.group, head_in_group = r % a.group;
-    // Whole rows go to and from global memory: 8 lanes a 128-byte piece, 4 rows at a time (a thread per row would
-    // touch 32 sectors with every instruction, which took longer than several key tiles).
+    // Whole rows go to global memory: 8 lanes a 128-byte piece, 4 rows at a time (a thread per row would touch 32
+    // sectors with every instruction, which took longer than several key tiles).
     const int piece = lane & 7, sub_row = lane >> 3;
-    int s_uses = 0, o_uses = 0, skips = 0;
+    int s_uses = 0, o_uses = 0, unit = 0;
     // this thread's row of unit u: q and out row, or -1
     auto row_of = [&](const Walk& u) {
       const int tok = u.tok0 + i * tq + tok_in_tile;
       if (tok_in_tile >= tq || tok >= u.g.count) return -1;
-      const int row = u.g.row0 + tok;
-      if (!prefix) return row;
-      const int slot = rows.members[row];
-      return slot >= 0 && slot < a.rows ? slot : -1;
+      const int row = prefix ? rows.members[u.g.row0 + tok] : u.g.row0 + tok;
+      return row >= 0 && row < a.rows ? row : -1;
     };
-    // the warp's 32 rows of queries into shared memory, for the MMA warp
+    // without a query map: the warp's 32 rows of queries into shared memory
     auto load_q = [&](const Walk& u, int row) {
       const uint16_t* src = a.q + static_cast<int64_t>(u.head * a.group) * D + 8 * piece;
       unsigned char* dst = q_smem + i * C::kQBytes + 32 * (warp & 3) * 128;
@@ -763,37 +759,35 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     int q_row = -1;
     if (any) {
       q_row = row_of(w);
-      load_q(w, q_row);
+      if (!rows.q_mapped) load_q(w, q_row);
     }
-    for (bool more = any; more && alive(errv);) {
-      int p0, p1, q0, q1;
-      positions(w.g, prefix, w.tok0, w.tok0 + 2 * tq, &p0, &p1);
+    for (bool more = any; more && alive(errv); ++unit) {
+      int q0, q1;
       positions(w.g, prefix, w.tok0 + i * tq, w.tok0 + (i + 1) * tq, &q0, &q1);
-      const KeySpan span(p0, max(p0, p1), a.window, a.sinks);
       const TilesSeen seen(q0, q1, a.window, a.sinks);
-      const int len = w.g.len;
+      const KeySpan span = unit_span(w, prefix, tq, a);
+      const int len = w.g.len, t0 = w.t0, t1 = w.t1, q_head = w.head * a.group + head_in_group;
       const int pos = prefix ? len - 1 : len - w.g.count + w.tok0 + i * tq + tok_in_tile;
       const bool* mask = a.key_mask != nullptr ? a.key_mask + w.g.key_slot * a.mask_stride : nullptr;
+      if (threadIdx.x == 0) unit_slot = w.g.key_slot;
+      const bool whole = w.whole();
+      const int part_at = 2 * static_cast<int>(blockIdx.x) + w.part();
+      more = w.next(ws);  // from here on w is the next unit: its loads are on their way while this one runs
+      const int next_row = more ? row_of(w) : -1;
       float m = -CUDART_INF_F, l = 0.f;
       bool ok = true, started = false;
-      for (int t = w.t0; t < w.t1; ++t) {
+      for (int t = t0; t < t1; ++t) {
         const int j = span.tile(t);
         if (!seen.at(j)) continue;
         const int base = kKeys * j;
-        uint32_t see[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
         const bool all = mask == nullptr && tile_full(j, q0, q1, a.window, a.sinks) && base + kKeys <= len;
-        if (!all) {
-          const int hi = min(pos + 1, len) - base;
-          const int lo = a.window > 0 ? max(max(pos + 1 - base, 0) - a.window, 0) : 0;
-          const int sk = min(a.sinks, base + kKeys) - base;
+        uint32_t kept[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+        if (mask != nullptr) {  // before the wait, which covers the loads
+          bool on[4];
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            see[x] = bit_range(0, hi - 32 * x) & (bit_range(lo - 32 * x, 32) | bit_range(0, sk - 32 * x));
-            if (mask != nullptr) {
-              const int k = base + 32 * x + lane;
-              see[x] &= __ballot_sync(0xffffffffu, k < len && mask[k]);
-            }
-          }
+          for (int x = 0; x < 4; ++x) on[x] = base + 32 * x + lane < len && mask[base + 32 * x + lane];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) kept[x] = __ballot_sync(0xffffffffu, on[x]);
         }
         ok = wait_warp(&s_full[i], s_uses & 1);
         if (!ok) break;
@@ -805,12 +799,21 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           uint32_t s[kHalf];
           tmem_ld64(s, s_col + kHalf * h);
           if (!all) {
+            const int from = base + kHalf * h;
+            const int hi = min(pos + 1, len) - from;
+            const int lo = a.window > 0 ? max(max(pos + 1 - from, 0) - a.window, 0) : 0;
+            const int sk = min(a.sinks, from + kHalf) - from;
 #pragma unroll
-            for (int k = 0; k < kHalf; ++k)
-              if (!((see[2 * h + (k >> 5)] >> (k & 31)) & 1u)) s[k] = 0xff800000u;
+            for (int x = 0; x < 2; ++x) {
+              const uint32_t see = kept[2 * h + x] & bit_range(0, hi - 32 * x) &
+                                   (bit_range(lo - 32 * x, 32) | bit_range(0, sk - 32 * x));
+#pragma unroll
+              for (int k = 0; k < 32; ++k)
+                if (!((see >> k) & 1u)) s[32 * x + k] = 0xff800000u;
+            }
           }
           float sum;
-          auto probabilities = [&](auto poly) {
+          auto probabilities = [&] {
             const float off = m == -CUDART_INF_F ? 0.f : -m * a.scale2;
             const float2 scale = make_float2(a.scale2, a.scale2), offs = make_float2(off, off);
             float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
@@ -821,12 +824,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
               for (int k = 0; k < 16; ++k) {
                 const int e = 32 * x + 2 * k;
                 float2 v = fma2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), scale, offs);
-                if (decltype(poly)::value && (k & 7) < kPolyOf8) {
-                  v = ex2_poly(v);
-                } else {
-                  v.x = ex2(v.x);
-                  v.y = ex2(v.y);
-                }
+                v.x = ex2(v.x);
+                v.y = ex2(v.y);
                 // the sum keeps the unrounded probabilities; the values' weights are rounded to 16 bits once
                 sums[k & 1] = add2(sums[k & 1], v);
                 p[k] = Half16<T>::pack(v.x, v.y);
@@ -836,36 +835,35 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             sums[0] = add2(sums[0], sums[1]);
             sum = sums[0].x + sums[0].y;
           };
-          bool again = h == 0 && !started;
-          if (!again) {
-            // masked scores (-inf) must come out as exact zeros: the special function unit alone
-            if (all) probabilities(std::true_type{}); else probabilities(std::false_type{});
-            again = __any_sync(0xffffffffu, !(sum <= 32768.f) || m == -CUDART_INF_F);
-          }
-          if (again) {
-            float top = m;
+          bool find = h == 0 && !started;
+          while (true) {
+            if (find) {
+              float top = m;
 #pragma unroll
-            for (int k = 0; k < kHalf; k += 2)
-              top = max_nan(top, __uint_as_float(s[k]), __uint_as_float(s[k + 1]));
-            if (started || h == 1) {
-              // the products so far must be in O: those of the tiles before are (these scores came after them)
-              if (h == 1) ok = wait_warp(&half_done[i], s_uses & 1);
-              if (!ok) break;
-              tmem_fence_after_sync();
-              const float f = m == -CUDART_INF_F ? 1.f : ex2((m - top) * a.scale2);
-              l *= f;
+              for (int k = 0; k < kHalf; k += 2) top = max_nan(top, __uint_as_float(s[k]), __uint_as_float(s[k + 1]));
+              if (started || h == 1) {
+                // the products so far must be in O: those of the tiles before are (these scores came after them)
+                if (h == 1) ok = wait_warp(&half_done[i], s_uses & 1);
+                if (!ok) break;
+                tmem_fence_after_sync();
+                const float f = m == -CUDART_INF_F ? 1.f : ex2((m - top) * a.scale2);
+                l *= f;
+#pragma unroll 1
+                for (int b = 0; b < D / 16; ++b) {
+                  uint32_t o[16];
+                  tmem_ld16(o, o_col + 16 * b);
 #pragma unroll
-              for (int b = 0; b < D / 16; ++b) {
-                uint32_t o[16];
-                tmem_ld16(o, o_col + 16 * b);
-#pragma unroll
-                for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-                tmem_st16(o_col + 16 * b, o);
+                  for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+                  tmem_st16(o_col + 16 * b, o);
+                }
               }
+              m = top;
             }
-            m = top;
-            probabilities(std::false_type{});
+            probabilities();
+            if (find || !__any_sync(0xffffffffu, q_row >= 0 && (!(sum <= 32768.f) || m == -CUDART_INF_F))) break;
+            find = true;
           }
+          if (!ok) break;
           l += sum;
           tmem_wait_st();
           tmem_fence_before_sync();
@@ -876,17 +874,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         ++s_uses;
         started = true;
       }
-      // The next unit's queries go in before this one's result comes out: the
-      // scores that used the shared memory are done.  Not before the MMA warp
-      // has taken up this unit, though, which a tile's scores show, or
-      // `skip` for a Q tile without key tiles.
-      if (ok && !started) ok = wait_warp(&skip[i], skips++ & 1);
-      Walk v = w;
-      more = v.next(ws);
-      int next_row = -1;
-      if (ok && more) {
-        next_row = row_of(v);
-        load_q(v, next_row);
+      if (ok && more && !rows.q_mapped) {  // before this unit's result comes out
+        ok = wait_warp(&q_free[i], unit & 1);
+        if (ok) load_q(w, next_row);
       }
       if (ok && started) ok = wait_warp(&o_full[i], o_uses++ & 1);
       if (!ok) {
@@ -896,12 +886,18 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       tmem_fence_after_sync();
       const float inv = l == 0.f ? 0.f : 1.f / l;
       const float m2 = m == -CUDART_INF_F ? m : m * a.scale2;
-      const bool whole = w.whole(), there = q_row >= 0;
-      const int q_head = w.head * a.group + head_in_group;
-      float* part = ws.part + (2 * static_cast<int64_t>(blockIdx.x) + w.part(blockIdx.x)) * (D + 2) * kPairRows +
-                    i * kTile + r;
+      const bool there = q_row >= 0;
+      float* part = ws.part + static_cast<int64_t>(part_at) * (D + 2) * kPairRows + i * kTile + r;
       float* state = prefix && there ? rows.state + (static_cast<int64_t>(q_row) * a.q_heads + q_head) * (D + 4) : nullptr;
       unsigned char* stage = out_smem + warp * (32 * 128);
+      // where the 8 rows whose pieces this lane stores go (null: nowhere)
+      uint16_t* to[8];
+      {
+        uint16_t* mine = there ? a.out + q_row * a.out_row + static_cast<int64_t>(q_head) * D : nullptr;
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          to[k] = reinterpret_cast<uint16_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine), 4 * k + sub_row));
+      }
 #pragma unroll
       for (int b = 0; b < DB; ++b) {
 #pragma unroll
@@ -941,11 +937,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
             const int from = 4 * k + sub_row;
-            const int row = __shfl_sync(0xffffffffu, q_row, from), h = __shfl_sync(0xffffffffu, head_in_group, from);
             const uint4 y = *reinterpret_cast<const uint4*>(stage + from * 128 + 16 * (piece ^ (from & 7)));
-            if (row >= 0)
-              *reinterpret_cast<uint4*>(a.out + row * a.out_row + static_cast<int64_t>(w.head * a.group + h) * D + 64 * b +
-                                        8 * piece) = y;
+            if (to[k] != nullptr) *reinterpret_cast<uint4*>(to[k] + 64 * b + 8 * piece) = y;
           }
           __syncwarp();
         }
@@ -961,7 +954,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         }
       }
       tmem_fence_before_sync();
-      w = v;
       q_row = next_row;
     }
   }
@@ -971,7 +963,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     tmem_fence_after_sync();
     tmem_dealloc(tmem, 512);
   }
-  if (threadIdx.x == 0 && *errv != 0 && any && c.status != nullptr) c.status[w.g.key_slot] = 4;
+  if (threadIdx.x == 0 && *errv != 0 && c.status != nullptr) c.status[unit_slot] = 4;
 }
 
 // Joins the parts of the units that a boundary between CTAs cut.  Block
@@ -1078,10 +1070,15 @@ EncodeTiledFn find_encode() {
   return ok ? reinterpret_cast<EncodeTiledFn>(p) : nullptr;
 }
 
+EncodeTiledFn encode_fn() {
+  static const EncodeTiledFn fn = find_encode();
+  return fn;
+}
+
 // The pool as a matrix of rows (one token's keys or values of one head); a
 // box is one page's rows of one head (at most a key tile's), 64 dims wide.
 bool pool_map(const PagedCache& c, int dtype, CUtensorMap* map) {
-  static const EncodeTiledFn fn = find_encode();
+  const EncodeTiledFn fn = encode_fn();
   if (fn == nullptr) return false;
   const cuuint64_t rows = static_cast<cuuint64_t>(c.pages) * c.layers * 2 * c.kv_heads * c.page_size;
   const cuuint64_t dims[2] = {static_cast<cuuint64_t>(c.head_dim), rows};
@@ -1094,11 +1091,30 @@ bool pool_map(const PagedCache& c, int dtype, CUtensorMap* map) {
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-cudaError_t run_prompt(const PagedCache& c, int dtype, const Attend& a, const PromptRows& rows, void* space,
+// The queries as [rows][heads][head_dim]; a box is a Q tile's tokens, its group's heads and 64 dims.
+bool query_map(const PagedCache& c, int dtype, const Attend& a, CUtensorMap* map) {
+  const EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr) return false;
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(c.head_dim), static_cast<cuuint64_t>(a.q_heads),
+                              static_cast<cuuint64_t>(a.rows)};
+  const cuuint64_t row = static_cast<cuuint64_t>(a.rows == 1 ? static_cast<int64_t>(a.q_heads) * c.head_dim : a.q_row) * 2;
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(c.head_dim) * 2, row};
+  const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(a.group), static_cast<cuuint32_t>(kTile / a.group)};
+  const cuuint32_t elem[3] = {1, 1, 1};
+  return row >= dims[0] * dims[1] * 2 &&
+         fn(map, dtype == MTT_B200_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+            const_cast<uint16_t*>(a.q), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) ==
+             CUDA_SUCCESS;
+}
+
+cudaError_t run_prompt(const PagedCache& c, int dtype, const Attend& a, PromptRows rows, void* space,
                        cudaStream_t stream) {
   const int sms = cache_sm_count();
-  CUtensorMap map;
+  CUtensorMap map, q_map;
   if (sms <= 0 || sms > kMaxSms || !pool_map(c, dtype, &map)) return cudaErrorInvalidValue;
+  rows.q_mapped = rows.members == nullptr && query_map(c, dtype, a, &q_map);
+  if (!rows.q_mapped) q_map = map;  // not read
   const PromptLayout at(rows.n, rows.n_rows, a.group, c.head_dim);
   char* base = static_cast<char*>(space);
   PromptSpace ws;
@@ -1112,7 +1128,7 @@ cudaError_t run_prompt(const PagedCache& c, int dtype, const Attend& a, const Pr
     if (e == cudaSuccess)
       e = launch_serialized(prompt_plan_kernel, dim3(1), dim3(kPromptPlanThreads), 0, stream, c, rows, ws, a.window,
                             a.sinks, 2 * (kTile / a.group), sms);
-    if (e == cudaSuccess) e = launch_serialized(kernel, dim3(sms), dim3(kPromptThreads), smem, stream, map, c, a, rows, ws);
+    if (e == cudaSuccess) e = launch_serialized(kernel, dim3(sms), dim3(kPromptThreads), smem, stream, map, q_map, c, a, rows, ws);
     if (e == cudaSuccess)
       e = launch_serialized(join, dim3(sms - 1, kPairRows / 32, c.head_dim / 32), dim3(256), 0, stream, c, a, rows, ws);
     return e;

@@ -338,6 +338,23 @@ def test_strided_rows_scale_and_out(pc):
     assert (wide[:, :4] == 7).all() and (wide[:, 16:] == 7).all()
 
 
+@pytest.mark.parametrize("group,d", [(1, 64), (3, 128), (4, 64)])
+def test_prompt_strided_and_repeated_rows(pc, group, d):
+    """Rows inside wider ones, and one row broadcast over all (a stride of 0)."""
+    lengths, new = [300, 40], [290, 33]
+    cache, pool, table = make(pc, lengths, 2, d)
+    rows, heads = sum(new), 2 * group
+    offsets = [0, 290, 323]
+    wide = queries(rows, heads + 5, d, torch.bfloat16)
+    ref = O.attention(pool, table, lengths, 0, wide[:, 2:2 + heads], offsets)
+    got = cache.attend(0, wide.cuda()[:, 2:2 + heads], offsets=i32(offsets))
+    agree(got, None, ref, torch.bfloat16, 300)
+    one = queries(1, heads, d, torch.bfloat16)
+    ref = O.attention(pool, table, lengths, 0, one.expand(rows, heads, d), offsets)
+    got = cache.attend(0, one.cuda().expand(rows, heads, d), offsets=i32(offsets))
+    agree(got, None, ref, torch.bfloat16, 300)
+
+
 def test_large_scores_and_infinities(pc):
     """Scores far apart (one key takes all), scores of the same huge size, and -inf and +inf among the values'
     masked neighbours."""
