@@ -46,6 +46,16 @@ def _check(ok: bool, what: str) -> None:
         raise ValueError(what)
 
 
+def _raw_stream(device: torch.device):
+    """A function that returns the handle of the device's current stream
+    (torch.cuda.current_stream builds a Stream object for it, which costs as
+    much as the rest of a small call)."""
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    if raw is None:
+        return lambda index: torch.cuda.current_stream(index).cuda_stream
+    return raw
+
+
 class PagedCache:
     def __init__(self, pool: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, refs: torch.Tensor):
         """Adopts the tensors of a cache: pool [pages, layers, 2, kv_heads,
@@ -72,6 +82,8 @@ class PagedCache:
         _check(pool.data_ptr() % 128 == 0, "the pool must be 128-byte aligned")
         self.pool, self.page_table, self.lengths, self.refs = pool, page_table, lengths, refs
         self.device = pool.device
+        self._index = pool.device.index
+        self._raw = _raw_stream(pool.device)
         self.dtype = pool.dtype
         self.pages, self.layers, self.kv_heads, self.page_size, self.head_dim = (
             pages, layers, kv_heads, page_size, head_dim)
@@ -85,6 +97,7 @@ class PagedCache:
         c.status, c.live = self.status.data_ptr(), self.live.data_ptr()
         self._c = c
         self._ref = ctypes.byref(c)
+        self._scale = head_dim ** -0.5
         self._spaces = {}  # (stream, query heads) -> workspace
         _check(L.lib.mtt_b200_paged_cache_workspace_size(self._ref, kv_heads, 0) > 0, "this cache is too large")
 
@@ -103,32 +116,30 @@ class PagedCache:
 
     # -- plumbing -----------------------------------------------------------
 
-    def _stream(self, stream):
-        return torch.cuda.current_stream(self.device) if stream is None else stream
+    def _handle(self, stream) -> int:
+        return self._raw(self._index) if stream is None else stream.cuda_stream
 
-    def _workspace(self, stream, q_heads: int, rows: int = 0) -> torch.Tensor:
-        """The workspace of calls on one stream: kept, and one for each stream, as the streams' calls may overlap."""
-        key = (stream.cuda_stream, q_heads)
-        space, most = self._spaces.get(key, (None, -1))
-        if rows > most:
+    def _workspace(self, handle: int, stream, q_heads: int, rows: int = 0):
+        """(address, bytes) of the workspace of calls on one stream: kept, and
+        one for each stream, as the streams' calls may overlap."""
+        space = self._spaces.get((handle, q_heads))
+        if space is None or rows > space[2]:
             most = max(1024, 1 << (rows - 1).bit_length()) if rows else 0
             size = L.lib.mtt_b200_paged_cache_workspace_size(self._ref, q_heads, most)
-            _check(size > 0, "q_heads must be a multiple of kv_heads, at most "
-                             f"{MAX_GROUP} query heads per key head")
-            with torch.cuda.stream(stream):
-                space = torch.zeros(size, dtype=torch.uint8, device=self.device)
-            self._spaces[key] = space, most
+            _check(size > 0, "this cache and number of heads or rows are not supported")
+            with self._on(stream):
+                data = torch.zeros(size, dtype=torch.uint8, device=self.device)
+            space = self._spaces[handle, q_heads] = (data.data_ptr(), size, most, data)
         return space
 
     @staticmethod
-    def _on(stream, given):
+    def _on(stream):
         """Where a call's own tensors are allocated: the stream that the caller gave, if any."""
-        return torch.cuda.stream(stream) if given else contextlib.nullcontext()
+        return contextlib.nullcontext() if stream is None else torch.cuda.stream(stream)
 
     def _vector(self, t: torch.Tensor, n: int, dtype: torch.dtype, name: str) -> int:
-        _check(t.dtype == dtype and t.dim() == 1 and t.shape[0] == n and t.is_contiguous(),
-               f"{name} must be a contiguous {dtype} vector of {n}")
-        _check(t.device == self.device, f"{name} is on another device than the pool")
+        if t.dtype is not dtype or t.shape != (n,) or t.get_device() != self._index or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous {dtype} vector of {n} on the pool's device")
         return t.data_ptr()
 
     @staticmethod
@@ -140,35 +151,34 @@ class PagedCache:
 
     def extend(self, counts: torch.Tensor, stream=None) -> None:
         """lengths += counts ([slots] int32), with the pages that takes."""
-        counts_ptr = self._vector(counts, self.slots, torch.int32, "counts")
-        stream = self._stream(stream)
-        ws = self._workspace(stream, self.kv_heads)
-        self._done(L.lib.mtt_b200_launch_paged_cache_extend(self._ref, counts_ptr, ws.data_ptr(), ws.numel(),
-                                                            stream.cuda_stream), "mtt_b200_launch_paged_cache_extend")
+        at = self._vector(counts, self.slots, torch.int32, "counts")
+        handle = self._handle(stream)
+        ws = self._workspace(handle, stream, self.kv_heads)
+        self._done(L.lib.mtt_b200_launch_paged_cache_extend(self._ref, at, ws[0], ws[1], handle),
+                   "mtt_b200_launch_paged_cache_extend")
 
     def fork(self, source: torch.Tensor, deep: bool = False, stream=None) -> None:
         """Slot d takes over the tokens that slot source[d] had before the call
         (source [slots] int32; -1 or d: slot d stays).  Full pages are shared
         unless ``deep``, a partial last page is always copied."""
-        source_ptr = self._vector(source, self.slots, torch.int32, "source")
-        stream = self._stream(stream)
-        ws = self._workspace(stream, self.kv_heads)
-        self._done(L.lib.mtt_b200_launch_paged_cache_fork(self._ref, source_ptr, 1 if deep else 0, ws.data_ptr(),
-                                                          ws.numel(), stream.cuda_stream),
+        at = self._vector(source, self.slots, torch.int32, "source")
+        handle = self._handle(stream)
+        ws = self._workspace(handle, stream, self.kv_heads)
+        self._done(L.lib.mtt_b200_launch_paged_cache_fork(self._ref, at, 1 if deep else 0, ws[0], ws[1], handle),
                    "mtt_b200_launch_paged_cache_fork")
 
     def free(self, mask: torch.Tensor, stream=None) -> None:
         """Closes every slot with mask ([slots] bool): its pages are released."""
-        mask_ptr = self._vector(mask, self.slots, torch.bool, "mask")
-        self._done(L.lib.mtt_b200_launch_paged_cache_free(self._ref, mask_ptr, self._stream(stream).cuda_stream),
+        at = self._vector(mask, self.slots, torch.bool, "mask")
+        self._done(L.lib.mtt_b200_launch_paged_cache_free(self._ref, at, self._handle(stream)),
                    "mtt_b200_launch_paged_cache_free")
 
     def compact(self, stream=None) -> None:
         """Moves the pages in use to [0, live); ``live`` [1] holds their number."""
-        stream = self._stream(stream)
-        ws = self._workspace(stream, self.kv_heads)
-        self._done(L.lib.mtt_b200_launch_paged_cache_compact(self._ref, ws.data_ptr(), ws.numel(),
-                                                             stream.cuda_stream), "mtt_b200_launch_paged_cache_compact")
+        handle = self._handle(stream)
+        ws = self._workspace(handle, stream, self.kv_heads)
+        self._done(L.lib.mtt_b200_launch_paged_cache_compact(self._ref, ws[0], ws[1], handle),
+                   "mtt_b200_launch_paged_cache_compact")
 
     def store(self, k: torch.Tensor, v: torch.Tensor, layer: Optional[int] = None,
               offsets: Optional[torch.Tensor] = None, stream=None) -> None:
@@ -177,65 +187,80 @@ class PagedCache:
         without offsets, row i is slot i's last token.  With ``layer`` k and v are
         [rows, kv_heads, head_dim]; without it [layers, rows, kv_heads, head_dim],
         every layer at once.  The last two dimensions must be contiguous."""
-        _check(k.shape == v.shape and k.dim() == (3 if layer is not None else 4), "k and v must be [rows, kv_heads, "
-               "head_dim], or [layers, rows, kv_heads, head_dim] without a layer")
-        _check(tuple(k.shape[-2:]) == (self.kv_heads, self.head_dim), "k and v have other heads than the cache")
+        shape, ks, vs = k.shape, k.stride(), v.stride()
+        if (len(shape) != (4 if layer is None else 3) or v.shape != shape or shape[-1] != self.head_dim or
+                shape[-2] != self.kv_heads):
+            raise ValueError("k and v must be [rows, kv_heads, head_dim], or [layers, rows, kv_heads, head_dim] without a "
+                             "layer, with the cache's heads")
         args = L.CacheRows()
         if layer is None:
-            _check(k.shape[0] == self.layers, "k and v have other layers than the cache")
-            args.n_layers, args.k_layer_stride, args.v_layer_stride = self.layers, k.stride(0), v.stride(0)
+            _check(shape[0] == self.layers, "k and v have other layers than the cache")
+            args.n_layers, args.k_layer_stride, args.v_layer_stride = self.layers, ks[0], vs[0]
         else:
             _check(0 <= layer < self.layers, "no such layer")
             args.layer, args.n_layers = layer, 1
-        for t in (k, v):
-            _check(t.dtype == self.dtype and t.device == self.device, "k and v must have the pool's type and device")
-            _check(t.stride(-1) == 1 and t.stride(-2) == self.head_dim, "k and v must be contiguous in their heads")
-            _check(t.data_ptr() % 16 == 0 and t.stride(-3) % 8 == 0 and (layer is not None or t.stride(0) % 8 == 0),
-                   "rows of k and v must be 16-byte aligned")
-        args.rows = k.shape[-3]
+        for t, st in ((k, ks), (v, vs)):
+            if t.dtype is not self.dtype or t.get_device() != self._index:
+                raise ValueError("k and v must have the pool's type and device")
+            if st[-1] != 1 or st[-2] != self.head_dim:
+                raise ValueError("k and v must be contiguous in their heads")
+            if t.data_ptr() % 16 or st[-3] % 8 or (layer is None and st[0] % 8):
+                raise ValueError("rows of k and v must be 16-byte aligned")
+        args.rows = shape[-3]
         args.k, args.v = k.data_ptr(), v.data_ptr()
-        args.k_row_stride, args.v_row_stride = k.stride(-3), v.stride(-3)
+        args.k_row_stride, args.v_row_stride = ks[-3], vs[-3]
         if offsets is not None:
             args.offsets = self._vector(offsets, self.slots + 1, torch.int32, "offsets")
         else:
             _check(args.rows <= self.slots, "more rows than slots: offsets are needed")
-        self._done(L.lib.mtt_b200_launch_paged_cache_store(self._ref, ctypes.byref(args),
-                                                           self._stream(stream).cuda_stream),
+        self._done(L.lib.mtt_b200_launch_paged_cache_store(self._ref, ctypes.byref(args), self._handle(stream)),
                    "mtt_b200_launch_paged_cache_store")
 
     # -- attention ----------------------------------------------------------
 
     def _attention(self, layer, q, out, window, sinks, scale, return_lse, stream):
         """The fields that the attention calls share; (args, out, lse)."""
-        _check(q.dim() == 3 and q.shape[2] == self.head_dim, "q must be [rows, q_heads, head_dim]")
-        rows, q_heads, d = q.shape
-        _check(q_heads >= 1 and q_heads % self.kv_heads == 0 and q_heads // self.kv_heads <= MAX_GROUP,
-               f"q_heads must be a multiple of kv_heads, at most {MAX_GROUP} query heads per key head")
-        _check(rows <= MAX_ROWS, f"at most {MAX_ROWS} rows")
-        _check(0 <= layer < self.layers, "no such layer")
-        _check(window >= 0 and sinks >= 0, "window and sinks must not be negative")
-        _check(scale is None or 0 < scale < float("inf"), "scale must be positive")
-        given = stream is not None
+        shape, st, d = q.shape, q.stride(), self.head_dim
+        if len(shape) != 3 or shape[2] != d:
+            raise ValueError("q must be [rows, q_heads, head_dim]")
+        rows, q_heads, _ = shape
+        if q_heads < 1 or q_heads % self.kv_heads or q_heads // self.kv_heads > MAX_GROUP:
+            raise ValueError(f"q_heads must be a multiple of kv_heads, at most {MAX_GROUP} query heads per key head")
+        if rows > MAX_ROWS:
+            raise ValueError(f"at most {MAX_ROWS} rows")
+        if not 0 <= layer < self.layers:
+            raise ValueError("no such layer")
+        if window < 0 or sinks < 0:
+            raise ValueError("window and sinks must not be negative")
+        if scale is None:
+            scale = self._scale
+        elif not 0 < scale < float("inf"):
+            raise ValueError("scale must be positive")
         if out is None:
-            with self._on(stream, given):
-                out = torch.empty(rows, q_heads, d, dtype=self.dtype, device=self.device)
+            with self._on(stream):
+                out = torch.empty(shape, dtype=self.dtype, device=self.device)
+            out_row = q_heads * d
         else:
-            _check(out.shape == q.shape, "out must have q's shape")
-        for name, t in (("q", q), ("out", out)):
-            _check(t.dtype == self.dtype and t.device == self.device, f"{name} must have the pool's type and device")
-            _check(t.stride(2) == 1 and t.stride(1) == d, f"{name} must be contiguous in its heads")
-            _check(t.data_ptr() % 16 == 0 and t.stride(0) % 8 == 0, f"rows of {name} must be 16-byte aligned")
+            if out.shape != shape:
+                raise ValueError("out must have q's shape")
+            self._rows_of(out, out.stride(), "out")
+            out_row = out.stride(0)
+        self._rows_of(q, st, "q")
         lse = None
-        args = L.CacheAttention()
+        args = L.CacheAttention(layer, q_heads, rows, window, sinks, scale, q.data_ptr(), st[0], out.data_ptr(), out_row)
         if return_lse:
-            with self._on(stream, given):
-                lse = torch.empty(rows, q_heads, dtype=torch.float32, device=self.device)
+            with self._on(stream):
+                lse = torch.empty((rows, q_heads), dtype=torch.float32, device=self.device)
             args.lse = lse.data_ptr()
-        args.layer, args.q_heads, args.rows, args.window, args.sinks = layer, q_heads, rows, window, sinks
-        args.scale = d ** -0.5 if scale is None else scale
-        args.q, args.q_row_stride = q.data_ptr(), q.stride(0)
-        args.out, args.out_row_stride = out.data_ptr(), out.stride(0)
         return args, out, lse
+
+    def _rows_of(self, t, st, name) -> None:
+        if t.dtype is not self.dtype or t.get_device() != self._index:
+            raise ValueError(f"{name} must have the pool's type and device")
+        if st[2] != 1 or st[1] != self.head_dim:
+            raise ValueError(f"{name} must be contiguous in its heads")
+        if t.data_ptr() % 16 or st[0] % 8:
+            raise ValueError(f"rows of {name} must be 16-byte aligned")
 
     def attend(self, layer: int, q: torch.Tensor, out: Optional[torch.Tensor] = None, *,
                offsets: Optional[torch.Tensor] = None, window: int = 0, sinks: int = 0,
@@ -252,20 +277,20 @@ class PagedCache:
         none gets 0.  Returns out, or (out, lse) with the natural log of the sum
         of exponentials ([rows, q_heads] f32, -inf for a row that sees none)."""
         args, out, lse = self._attention(layer, q, out, window, sinks, scale, return_lse, stream)
-        stream = self._stream(stream)
         if offsets is not None:
             args.offsets = self._vector(offsets, self.slots + 1, torch.int32, "offsets")
-        else:
-            _check(args.rows <= self.slots, "more rows than slots: offsets are needed")
+        elif args.rows > self.slots:
+            raise ValueError("more rows than slots: offsets are needed")
         if key_mask is not None:
-            _check(key_mask.dtype == torch.bool and key_mask.dim() == 2 and key_mask.shape[0] == self.slots and
+            _check(key_mask.dtype is torch.bool and key_mask.dim() == 2 and key_mask.shape[0] == self.slots and
                    key_mask.shape[1] >= self.table_pages * self.page_size and key_mask.stride(1) == 1 and
-                   key_mask.device == self.device and key_mask.stride(0) >= key_mask.shape[1],
+                   key_mask.get_device() == self._index and key_mask.stride(0) >= key_mask.shape[1],
                    "key_mask must be a [slots, >= table_pages * page_size] bool tensor with contiguous rows")
             args.key_mask, args.mask_stride = key_mask.data_ptr(), key_mask.stride(0)
-        ws = self._workspace(stream, args.q_heads, args.rows)
-        self._done(L.lib.mtt_b200_launch_paged_attention(self._ref, ctypes.byref(args), ws.data_ptr(), ws.numel(),
-                                                         stream.cuda_stream), "mtt_b200_launch_paged_attention")
+        handle = self._handle(stream)
+        ws = self._workspace(handle, stream, args.q_heads, args.rows)
+        self._done(L.lib.mtt_b200_launch_paged_attention(self._ref, ctypes.byref(args), ws[0], ws[1], handle),
+                   "mtt_b200_launch_paged_attention")
         return (out, lse) if return_lse else out
 
     def attend_shared(self, layer: int, q: torch.Tensor, groups: "PrefixGroups", out: Optional[torch.Tensor] = None, *,
@@ -277,14 +302,13 @@ class PagedCache:
         pages, and groups whose prefix is longer than ``sinks`` under a window
         are attended one by one; the result is the same."""
         _check(groups.cache is self, "these groups belong to another cache")
-        _check(q.dim() == 3 and q.shape[1] == groups.q_heads, "these groups were made for another number of heads")
-        _check(q.shape[0] <= self.slots, "more rows than slots")
         args, out, lse = self._attention(layer, q, out, window, sinks, scale, return_lse, stream)
-        stream = self._stream(stream)
-        ws = groups._workspace(stream)
-        self._done(L.lib.mtt_b200_launch_paged_attention_shared(self._ref, ctypes.byref(args), groups._ref,
-                                                                ws.data_ptr(), ws.numel(), stream.cuda_stream),
-                   "mtt_b200_launch_paged_attention_shared")
+        _check(args.q_heads == groups.q_heads, "these groups were made for another number of heads")
+        _check(args.rows <= self.slots, "more rows than slots")
+        handle = self._handle(stream)
+        ws = groups._workspace(handle, stream)
+        self._done(L.lib.mtt_b200_launch_paged_attention_shared(self._ref, ctypes.byref(args), groups._ref, ws[0], ws[1],
+                                                                handle), "mtt_b200_launch_paged_attention_shared")
         return (out, lse) if return_lse else out
 
 
@@ -327,11 +351,11 @@ class PrefixGroups:
         self._ref = ctypes.byref(c)
         self._spaces = {}
 
-    def _workspace(self, stream) -> torch.Tensor:
-        space = self._spaces.get(stream.cuda_stream)
+    def _workspace(self, handle: int, stream):
+        space = self._spaces.get(handle)
         if space is None:
             size = L.lib.mtt_b200_paged_shared_workspace_size(self.cache._ref, self.q_heads, self.n_members)
-            with torch.cuda.stream(stream):
-                space = torch.zeros(size, dtype=torch.uint8, device=self.cache.device)
-            self._spaces[stream.cuda_stream] = space
+            with PagedCache._on(stream):
+                data = torch.zeros(size, dtype=torch.uint8, device=self.cache.device)
+            space = self._spaces[handle] = (data.data_ptr(), size, data)
         return space
