@@ -195,7 +195,8 @@ class CacheAttention(ctypes.Structure):
 
 
 class PrefixGroups(ctypes.Structure):
-    _fields_ = [("n_groups", I32), ("n_members", I32), ("voice", P), ("tokens", P), ("offsets", P), ("members", P)]
+    _fields_ = [("n_groups", I32), ("n_members", I32), ("voice", P), ("tokens", P), ("offsets", P), ("members", P),
+                ("shared_tokens", I64)]
 
 
 # name -> (restype, argtypes)

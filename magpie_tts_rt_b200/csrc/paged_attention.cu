@@ -38,6 +38,14 @@ bool attend_args(const PagedCache& c, const mtt_b200_cache_attention_t* args, At
   return true;
 }
 
+// Keys and values of all members' prefixes from which on the prefix pass pays:
+// it adds about 20 us of launches and dependent steps, while those bytes read
+// slot by slot come at 8 to 10 TB/s, mostly from L2.  Measured, each slot on its
+// own against shared: 101 MB (12 heads of 64, 1024 tokens, 32 slots) 20 against
+// 32 us; 134 MB (8 of 128, 16384, 2) 37 / 45; 302 MB (12 of 64, 192, 512) 55 / 47;
+// 403 MB (12 of 64, 16384, 8) 58 / 42; 2.1 GB (8 of 128, 4096, 128) 243 / 54.
+constexpr double kSharedBytesWorth = 220e6;
+
 // Bytes of the prefix pass's results: base and state (SharedPrefix).
 size_t base_bytes(const mtt_b200_paged_cache_t& c) { return (4 * static_cast<size_t>(c.slots) + 255) / 256 * 256; }
 size_t state_bytes(const mtt_b200_paged_cache_t& c, int q_heads) {
@@ -83,7 +91,9 @@ int mtt_b200_launch_paged_attention_shared(const mtt_b200_paged_cache_t* cache, 
     return MTT_B200_STATUS_INVALID_ARGUMENT;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   SharedPrefix shared{};
-  if (groups->n_groups > 0 && groups->n_members > 0) {
+  const double shared_bytes = 4.0 * groups->shared_tokens * c.kv_heads * c.head_dim;
+  if (groups->n_groups > 0 && groups->n_members > 0 &&
+      (groups->shared_tokens <= 0 || shared_bytes >= kSharedBytesWorth)) {
     if (groups->voice == nullptr || groups->tokens == nullptr || groups->offsets == nullptr ||
         groups->members == nullptr)
       return MTT_B200_STATUS_INVALID_ARGUMENT;

@@ -108,7 +108,7 @@ __device__ int list_free(const PagedCache& c, int32_t* list) {
 
 // One CTA.  Grants the slots' new pages and writes them into the tables.
 __global__ void __launch_bounds__(kPlanThreads) extend_kernel(PagedCache c, const int32_t* counts, UpkeepSpace u) {
-  wait_prior_grid();
+  take_turn();
   const int free_pages = list_free(c, u.free_list);
   int asked = 0;
   for (int base = 0; base < c.slots; base += kPlanThreads) {
@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(kPlanThreads) extend_kernel(PagedCache c, cons
 // One CTA: which slots are forked, and their first private page's rank.
 __global__ void __launch_bounds__(kPlanThreads)
     fork_plan_kernel(PagedCache c, const int32_t* source, int deep, UpkeepSpace u) {
-  wait_prior_grid();
+  take_turn();
   const int free_pages = list_free(c, u.free_list);
   int asked = 0, granted = 0;
   for (int base = 0; base < c.slots; base += kPlanThreads) {
@@ -182,7 +182,7 @@ __global__ void __launch_bounds__(kPlanThreads)
 // Slot d (one CTA each): its new row, from its source's old one, and the page copies it asks for.
 __global__ void __launch_bounds__(kMoveThreads) fork_rows_kernel(PagedCache c, const int32_t* source, int deep,
                                                                  UpkeepSpace u) {
-  wait_prior_grid();
+  take_turn();
   const int d = blockIdx.x;
   const int rank = u.rank[d];
   if (rank < 0) return;
@@ -235,7 +235,7 @@ __device__ __forceinline__ void copy_pairs(const PagedCache& c, const UpkeepSpac
 
 // The forked rows and lengths become the slots', the pages they had are released, partial pages copied.
 __global__ void __launch_bounds__(kMoveThreads) fork_commit_kernel(PagedCache c, UpkeepSpace u, int parts) {
-  wait_prior_grid();
+  take_turn();
   for (int d = blockIdx.x; d < c.slots; d += gridDim.x) {
     if (u.rank[d] < 0) continue;
     int32_t* row = c.table + static_cast<int64_t>(d) * c.table_pages;
@@ -252,7 +252,7 @@ __global__ void __launch_bounds__(kMoveThreads) fork_commit_kernel(PagedCache c,
 
 // One warp per slot.
 __global__ void __launch_bounds__(kMoveThreads) free_kernel(PagedCache c, const bool* mask) {
-  wait_prior_grid();
+  take_turn();
   const int i = blockIdx.x * (kMoveThreads / 32) + (threadIdx.x >> 5);
   if (i >= c.slots || !mask[i]) return;
   int32_t* row = c.table + static_cast<int64_t>(i) * c.table_pages;
@@ -266,7 +266,7 @@ __global__ void __launch_bounds__(kMoveThreads) free_kernel(PagedCache c, const 
 
 // One CTA: live pages, and where those past the live count go.
 __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(PagedCache c, UpkeepSpace u) {
-  wait_prior_grid();
+  take_turn();
   const int live = c.pages - list_free(c, u.free_list);  // free pages below `live` come first in the list
   int moved = 0;
   for (int base = live & ~(4 * kPlanThreads - 1); base < c.pages; base += 4 * kPlanThreads) {
@@ -300,7 +300,7 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(PagedCache c
 }
 
 __global__ void __launch_bounds__(kMoveThreads) compact_move_kernel(PagedCache c, UpkeepSpace u, int parts) {
-  wait_prior_grid();
+  take_turn();
   const int moved = u.counts[0], live = u.counts[1];
   if (moved == 0) return;
   const int64_t entries = static_cast<int64_t>(c.slots) * c.table_pages;
@@ -326,7 +326,7 @@ struct Rows {
 
 // Row blockIdx.x: its keys and values of every given layer to its slot's page.
 __global__ void __launch_bounds__(kMoveThreads) store_kernel(PagedCache c, Rows in) {
-  wait_prior_grid();
+  take_turn();
   const int row = blockIdx.x;
   int slot = row, count = 1, first = row;
   if (in.offsets != nullptr) {

@@ -37,6 +37,14 @@ struct PagedCache {
   }
 };
 
+// The first statement of every kernel here (before its first global access):
+// the next launch on the stream may be scheduled from now on, and waits in
+// turn for this grid; this one waits for the launch before it.
+__device__ __forceinline__ void take_turn() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  wait_prior_grid();
+}
+
 // Checks a caller's cache and fills the device view; false for bad arguments.
 bool paged_cache_view(const mtt_b200_paged_cache_t* c, PagedCache* out);
 

@@ -37,7 +37,7 @@
 // second kernel that joins the parts in order.  Every wait is bounded; one
 // that gives up marks the slot's status 4.
 #include <algorithm>
-#include <type_traits>
+#include <atomic>
 
 #include "gemm_tc.cuh"
 #include "paged_attention.cuh"
@@ -195,7 +195,7 @@ __device__ __forceinline__ int plan_scan(int v, int* total) {
 __global__ void __launch_bounds__(kPromptPlanThreads)
     prompt_plan_kernel(PagedCache c, PromptRows rows, PromptSpace ws, int window, int sinks, int tokens_per_pair,
                        int ctas) {
-  wait_prior_grid();
+  take_turn();
   const int tid = threadIdx.x;
   const bool prefix = rows.members != nullptr;
   if (prefix) {
@@ -505,7 +505,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   tmem_fence_after_sync();
   const uint32_t tmem = tmem_base;
   volatile int* errv = &err;
-  wait_prior_grid();
+  take_turn();
 
   Walk w;
   const bool any = w.begin(ws, c.kv_heads, blockIdx.x);
@@ -973,7 +973,7 @@ constexpr int kJoinParts = 8;  // parts on their way at a time
 
 template <typename T, int D>
 __global__ void __launch_bounds__(256) prompt_join_kernel(PagedCache c, Attend a, PromptRows rows, PromptSpace ws) {
-  wait_prior_grid();
+  take_turn();
   const int cta = blockIdx.x + 1;
   const int64_t line = ws.head[1], per = ws.head[2];
   const int64_t x = cta * per;
@@ -1123,20 +1123,28 @@ cudaError_t run_prompt(const PagedCache& c, int dtype, const Attend& a, PromptRo
   ws.first = reinterpret_cast<int32_t*>(base + at.first);
   ws.rec = reinterpret_cast<int4*>(base + at.rec);
   ws.part = reinterpret_cast<float*>(base + at.part);
-  auto go = [&](auto kernel, auto join, size_t smem) {
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  auto go = [&](auto type, auto dim) {
+    using T = decltype(type);
+    constexpr int D = decltype(dim)::value;
+    const auto kernel = prompt_kernel<T, D>;
+    constexpr size_t smem = PromptCfg<D>::kSmem;
+    static std::atomic<uint64_t> opted_in;  // devices on which this kernel has its shared memory
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess && (dev > 63 || !(opted_in.load(std::memory_order_relaxed) >> dev & 1))) {
+      e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+      if (e == cudaSuccess && dev < 64) opted_in.fetch_or(uint64_t{1} << dev, std::memory_order_relaxed);
+    }
     if (e == cudaSuccess)
       e = launch_serialized(prompt_plan_kernel, dim3(1), dim3(kPromptPlanThreads), 0, stream, c, rows, ws, a.window,
                             a.sinks, 2 * (kTile / a.group), sms);
     if (e == cudaSuccess) e = launch_serialized(kernel, dim3(sms), dim3(kPromptThreads), smem, stream, map, q_map, c, a, rows, ws);
     if (e == cudaSuccess)
-      e = launch_serialized(join, dim3(sms - 1, kPairRows / 32, c.head_dim / 32), dim3(256), 0, stream, c, a, rows, ws);
+      e = launch_serialized(prompt_join_kernel<T, D>, dim3(sms - 1, kPairRows / 32, c.head_dim / 32), dim3(256), 0, stream, c, a, rows, ws);
     return e;
   };
   auto pick = [&](auto type) {
-    using T = decltype(type);
-    return c.head_dim == 64 ? go(prompt_kernel<T, 64>, prompt_join_kernel<T, 64>, PromptCfg<64>::kSmem)
-                            : go(prompt_kernel<T, 128>, prompt_join_kernel<T, 128>, PromptCfg<128>::kSmem);
+    return c.head_dim == 64 ? go(type, std::integral_constant<int, 64>{}) : go(type, std::integral_constant<int, 128>{});
   };
   return dtype == MTT_B200_DTYPE_BF16 ? pick(__nv_bfloat16{}) : pick(__half{});
 }

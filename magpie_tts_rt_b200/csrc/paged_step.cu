@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(D, NB))
   extern __shared__ int tiles_before[];  // [rows + 1]: tiles of a key head of the slots before
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int t = lane & 3, g = lane >> 2;
-  wait_prior_grid();
+  take_turn();
 
   auto tiles_of = [&](int i) {
     return SeenTiles(c.length(i), a.window, a.sinks, shared.base != nullptr ? shared.base[i] : 0);
@@ -406,29 +406,24 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(D, NB))
   }
 }
 
-// Joins the parts of the units that a cut divided.  CTA x looks after the
-// units that begin in kJoinShares warps' shares, CTA y after 128 of their
-// (query, pair of dims).
-constexpr int kJoinShares = kStepWarps;
+// Joins the parts of the units that a cut divided.  `threads` threads (32, 64
+// or 128) look after the unit that begins in one warp's share, a pair of dims of
+// one query each; CTA y after the y-th 128 of them.
 constexpr int kJoinChunk = 16;  // parts on their way at a time
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kStepThreads)
-    step_join_kernel(Attend a, SharedPrefix shared, StepSpace ws, int nq, int blocks) {
-  wait_prior_grid();
-  int4 cuts[kJoinShares];
-#pragma unroll
-  for (int s = 0; s < kJoinShares; ++s) cuts[s] = ws.cut[blockIdx.x * kJoinShares + s];
-  const int e = blockIdx.y * kStepThreads + threadIdx.x;
+    step_join_kernel(Attend a, SharedPrefix shared, StepSpace ws, int nq, int blocks, int threads) {
+  take_turn();
+  const int me = (blockIdx.x * kStepThreads + threadIdx.x) / threads;
+  const int e = blockIdx.y * kStepThreads + threadIdx.x % threads;
   const int qi = e / (D / 2), d = 2 * (e % (D / 2));
   const int64_t stride = static_cast<int64_t>(nq) * (D + 2);
-#pragma unroll
-  for (int s = 0; s < kJoinShares; ++s) {
-    const int4 cut = cuts[s];
-    const int head = cut.y / blocks, block = cut.y % blocks;
-    if (cut.z == 0 || qi >= min(nq, a.group - block * nq)) continue;
+  const int4 cut = ws.cut[me];
+  const int head = cut.y / blocks, block = cut.y % blocks;
+  if (cut.z > 0 && qi < min(nq, a.group - block * nq)) {
     // the first part lies where the warp left it, the others are their warps' first units
-    const float* parts = ws.part + 2 * static_cast<int64_t>(blockIdx.x * kJoinShares + s) * stride + qi * (D + 2);
+    const float* parts = ws.part + 2 * static_cast<int64_t>(me) * stride + qi * (D + 2);
     RowPart<2> r, before;
     const int h = head * a.group + block * nq + qi;
     before.prefix<D>(shared, a.q_heads, cut.x, h, d, shared.base != nullptr && shared.base[cut.x] > 0);
@@ -508,8 +503,9 @@ cudaError_t launch_step(const PagedCache& c, int dtype, const Attend& a, const S
     cudaError_t e = launch_serialized(kernel, dim3(grid), dim3(kStepThreads), smem, stream, c, a, shared, ws, blocks,
                                       min_tiles);
     if (e != cudaSuccess) return e;
-    return launch_serialized(join, dim3(shares / kJoinShares, (pairs + kStepThreads - 1) / kStepThreads),
-                             dim3(kStepThreads), 0, stream, a, shared, ws, 8 * nb, blocks);
+    const int threads = pairs <= 32 ? 32 : pairs <= 64 ? 64 : kStepThreads;
+    return launch_serialized(join, dim3(shares / (kStepThreads / threads), (pairs + kStepThreads - 1) / kStepThreads),
+                             dim3(kStepThreads), 0, stream, a, shared, ws, 8 * nb, blocks, threads);
   };
   auto pick = [&](auto type) {
     using T = decltype(type);

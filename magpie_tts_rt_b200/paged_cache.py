@@ -347,6 +347,7 @@ class PrefixGroups:
         c = L.PrefixGroups()
         c.n_groups, c.n_members = n, len(members)
         c.voice, c.tokens, c.offsets, c.members = at, at + 4 * n, at + 8 * n, at + 4 * (3 * n + 1)
+        c.shared_tokens = sum(t * (b - a) for t, a, b in zip(tokens, offsets, offsets[1:]))
         self._c = c
         self._ref = ctypes.byref(c)
         self._spaces = {}

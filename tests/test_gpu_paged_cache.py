@@ -516,7 +516,8 @@ def check_shared(pc, cache, groups, group=1, window=0, sinks=0, rows=None, seed=
     ref = O.attention(cache.pool.cpu(), cache.page_table.cpu(), lengths[:rows], 0, q, list(range(rows + 1)), window,
                       sinks)
     plan = pc.PrefixGroups(cache, groups, q_heads=q.shape[1])
-    for _ in range(2):
+    for shared_tokens in (plan._c.shared_tokens, 0):    # by the rule on sizes, and shared in any case
+        plan._c.shared_tokens = shared_tokens
         got, lse = cache.attend_shared(0, q.cuda(), plan, window=window, sinks=sinks, return_lse=True)
         agree(got, lse, ref, cache.dtype, max(lengths))
     assert (cache.status == 0).all()
