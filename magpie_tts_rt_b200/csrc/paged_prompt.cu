@@ -198,24 +198,8 @@ __global__ void __launch_bounds__(kPromptPlanThreads)
   take_turn();
   const int tid = threadIdx.x;
   const bool prefix = rows.members != nullptr;
-  if (prefix) {
+  if (prefix)
     for (int i = tid; i < c.slots; i += kPromptPlanThreads) rows.base[i] = 0;
-    __syncthreads();
-    for (int k = tid; k < rows.n_rows; k += kPromptPlanThreads) {
-      int lo = 0, hi = rows.n;  // the group whose members begin at or before k
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (rows.offsets[mid] <= k) lo = mid; else hi = mid;
-      }
-      const PairGeom g(c, rows, lo);
-      const int slot = rows.members[k];
-      if (!g.ok || k < g.row0 || k >= g.row0 + g.count || slot < 0 || slot >= c.slots || c.length(slot) < g.len) continue;
-      const int last = (g.len >> c.page_shift) - 1;
-      if (c.table[static_cast<int64_t>(slot) * c.table_pages + last] ==
-          c.table[static_cast<int64_t>(g.key_slot) * c.table_pages + last])
-        rows.base[slot] = g.len;
-    }
-  }
   // slots whose offsets overlap could ask for more pairs than there is room for
   const int most = rows.n_rows / tokens_per_pair + rows.n;
   int pairs = 0;
@@ -966,6 +950,24 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   if (threadIdx.x == 0 && *errv != 0 && c.status != nullptr) c.status[unit_slot] = 4;
 }
 
+// Prefix pass: how many of each member's tokens it has attended to (base is 0 so far).
+__device__ void member_bases(const PagedCache& c, const PromptRows& rows) {
+  for (int k = blockIdx.x * blockDim.x + threadIdx.x; k < rows.n_rows; k += gridDim.x * blockDim.x) {
+    int lo = 0, hi = rows.n;  // the group whose members begin at or before k
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (rows.offsets[mid] <= k) lo = mid; else hi = mid;
+    }
+    const PairGeom g(c, rows, lo);
+    const int slot = rows.members[k];
+    if (!g.ok || k < g.row0 || k >= g.row0 + g.count || slot < 0 || slot >= c.slots || c.length(slot) < g.len) continue;
+    const int last = (g.len >> c.page_shift) - 1;
+    if (c.table[static_cast<int64_t>(slot) * c.table_pages + last] ==
+        c.table[static_cast<int64_t>(g.key_slot) * c.table_pages + last])
+      rows.base[slot] = g.len;
+  }
+}
+
 // Joins the parts of the units that a boundary between CTAs cut.  Block
 // (c - 1, row chunk, dim chunk): the unit at the start of CTA c's share, if
 // that is the first boundary between its key tiles; 32 of its rows, 32 dims.
@@ -974,6 +976,7 @@ constexpr int kJoinParts = 8;  // parts on their way at a time
 template <typename T, int D>
 __global__ void __launch_bounds__(256) prompt_join_kernel(PagedCache c, Attend a, PromptRows rows, PromptSpace ws) {
   take_turn();
+  if (rows.members != nullptr && blockIdx.y == 0 && blockIdx.z == 0) member_bases(c, rows);
   const int cta = blockIdx.x + 1;
   const int64_t line = ws.head[1], per = ws.head[2];
   const int64_t x = cta * per;
