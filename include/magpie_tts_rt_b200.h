@@ -756,7 +756,7 @@ typedef struct mtt_b200_paged_cache {
   void* pool;          /* 128-byte aligned */
   int32_t* page_table; /* [slots][table_pages], -1 past a slot's pages */
   int32_t* lengths;    /* [slots] tokens */
-  int32_t* refs;       /* [pages] */
+  int32_t* refs;       /* [pages], 16-byte aligned */
   int32_t* status;     /* [slots] or NULL */
   int32_t* live;       /* [1] or NULL: pages in use, written by compact */
 } mtt_b200_paged_cache_t;

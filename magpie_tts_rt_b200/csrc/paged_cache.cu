@@ -83,100 +83,122 @@ __device__ __forceinline__ int block_scan(int v, int* total) {
   return before;
 }
 
-// Lists the free pages in ascending order; returns how many there are.
-__device__ int list_free(const PagedCache& c, int32_t* list) {
+// Lists the free pages in ascending order, at least `want` of them if there
+// are that many; returns how many were found.  A thread looks at 16 pages a
+// round: what a round costs is its latency, and a pool may have 100,000s.
+__device__ int list_free(const PagedCache& c, int32_t* list, int want) {
+  constexpr int kEach = 16;
   int found = 0;
-  for (int base = 0; base < c.pages; base += 4 * kPlanThreads) {
-    const int p0 = base + 4 * threadIdx.x;
-    bool f[4];
-    int n = 0;
+  for (int64_t base = 0; base < c.pages && found < want; base += kEach * kPlanThreads) {
+    const int64_t p0 = base + kEach * threadIdx.x;
+    uint32_t free = 0;
+    if (p0 + kEach <= c.pages) {
+      int4 r[kEach / 4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      f[j] = p0 + j < c.pages && c.refs[p0 + j] == 0;
-      n += f[j];
+      for (int j = 0; j < kEach / 4; ++j) r[j] = *reinterpret_cast<const int4*>(c.refs + p0 + 4 * j);
+#pragma unroll
+      for (int j = 0; j < kEach / 4; ++j)
+        free |= ((r[j].x == 0 ? 1u : 0u) | (r[j].y == 0 ? 2u : 0u) | (r[j].z == 0 ? 4u : 0u) | (r[j].w == 0 ? 8u : 0u))
+                << (4 * j);
+    } else {
+      for (int j = 0; j < kEach; ++j)
+        if (p0 + j < c.pages && c.refs[p0 + j] == 0) free |= 1u << j;
     }
     int total;
-    int at = found + block_scan(n, &total);
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (f[j]) list[at++] = p0 + j;
+    int at = found + block_scan(__popc(free), &total);
+    for (; free != 0; free &= free - 1) list[at++] = static_cast<int32_t>(p0) + __ffs(free) - 1;
     found += total;
   }
   __syncthreads();
   return found;
 }
 
+// What each slot asks for, and the sum over the slots before it (at most
+// INT_MAX): of the thread's first slot in registers, of further ones (more than
+// kPlanThreads slots) in the workspace.
+struct Asked {
+  int need, rank, all;
+  template <typename Need>
+  __device__ __forceinline__ Asked(const PagedCache& c, const UpkeepSpace& u, Need need_of) {
+    int64_t before = 0;
+    for (int base = 0; base < c.slots; base += kPlanThreads) {
+      const int i = base + threadIdx.x;
+      const int n = i < c.slots ? need_of(i) : -1;
+      int total;
+      const int r = static_cast<int>(min(before + block_scan(max(n, 0), &total), static_cast<int64_t>(INT32_MAX)));
+      if (base == 0) {
+        need = n;
+        rank = r;
+      } else if (i < c.slots) {
+        u.rank[i] = r;
+        u.len[i] = n;
+      }
+      before += total;
+    }
+    all = static_cast<int>(min(before, static_cast<int64_t>(INT32_MAX)));
+  }
+  __device__ __forceinline__ void load(const UpkeepSpace& u, int i) {
+    if (i < kPlanThreads) return;
+    need = u.len[i];
+    rank = u.rank[i];
+  }
+  // whether its pages are among the `free` ones; no more are granted after one is not
+  __device__ __forceinline__ bool granted(int free) const {
+    return need == 0 || (need > 0 && static_cast<int64_t>(rank) + need <= free);
+  }
+};
+
 // One CTA.  Grants the slots' new pages and writes them into the tables.
 __global__ void __launch_bounds__(kPlanThreads) extend_kernel(PagedCache c, const int32_t* counts, UpkeepSpace u) {
   take_turn();
-  const int free_pages = list_free(c, u.free_list);
-  int asked = 0;
-  for (int base = 0; base < c.slots; base += kPlanThreads) {
-    const int i = base + threadIdx.x;
-    int need = 0, have = 0, add = 0, len = 0, st = 0;
-    if (i < c.slots) {
-      len = c.length(i);
-      add = counts[i];
-      have = (len + c.page_size - 1) >> c.page_shift;
-      // the sum is taken in 64 bits: a count near 2^31 is refused, not wrapped
-      const int64_t want = (static_cast<int64_t>(len) + add + c.page_size - 1) >> c.page_shift;
-      if (add < 0 || want > c.table_pages) {
-        st = 1;
-      } else {
-        need = static_cast<int>(want) - have;
+  Asked a(c, u, [&](int i) {  // pages; -1: the count is out of range
+    const int len = c.length(i), add = counts[i];
+    // the sum is taken in 64 bits: a count near 2^31 is refused, not wrapped
+    const int64_t want = (static_cast<int64_t>(len) + add + c.page_size - 1) >> c.page_shift;
+    if (add < 0 || want > c.table_pages) return -1;
+    return static_cast<int>(want) - ((len + c.page_size - 1) >> c.page_shift);
+  });
+  const int free_pages = list_free(c, u.free_list, a.all);
+  for (int i = threadIdx.x; i < c.slots; i += kPlanThreads) {
+    a.load(u, i);
+    const int len = c.length(i), add = counts[i];
+    const bool ok = a.granted(free_pages);
+    if (ok && add > 0) {
+      int32_t* row = c.table + static_cast<int64_t>(i) * c.table_pages + ((len + c.page_size - 1) >> c.page_shift);
+      for (int j = 0; j < a.need; ++j) {
+        const int p = u.free_list[a.rank + j];
+        row[j] = p;
+        c.refs[p] = 1;
       }
+      c.lengths[i] = len + add;
     }
-    int total;
-    const int rank = asked + block_scan(need, &total);
-    if (i < c.slots) {
-      if (st == 0 && need > 0 && rank + need > free_pages) st = 2;
-      if (st == 0 && add > 0) {
-        int32_t* row = c.table + static_cast<int64_t>(i) * c.table_pages + have;
-        for (int j = 0; j < need; ++j) {
-          const int p = u.free_list[rank + j];
-          row[j] = p;
-          c.refs[p] = 1;
-        }
-        c.lengths[i] = len + add;
-      }
-      if (c.status != nullptr && (add != 0 || st != 0)) c.status[i] = st;
-    }
-    asked += total;
+    if (c.status != nullptr && add != 0) c.status[i] = ok ? 0 : (a.need < 0 ? 1 : 2);
   }
 }
 
 // One CTA: which slots are forked, and their first private page's rank.
 __global__ void __launch_bounds__(kPlanThreads)
     fork_plan_kernel(PagedCache c, const int32_t* source, int deep, UpkeepSpace u) {
+  __shared__ int copies;
+  if (threadIdx.x == 0) copies = 0;
   take_turn();
-  const int free_pages = list_free(c, u.free_list);
-  int asked = 0, granted = 0;
-  for (int base = 0; base < c.slots; base += kPlanThreads) {
-    const int i = base + threadIdx.x;
-    int need = 0, s = -1, st = 0;
-    bool touch = false;
-    if (i < c.slots) {
-      s = source[i];
-      touch = s != -1 && s != i;
-      if (touch && (s < 0 || s >= c.slots)) st = 1;
-      if (touch && st == 0) {
-        const int len = c.length(s);
-        need = deep ? (len + c.page_size - 1) >> c.page_shift : ((len & (c.page_size - 1)) != 0 ? 1 : 0);
-      }
-    }
-    int total;
-    const int rank = asked + block_scan(need, &total);
-    const bool ok = touch && st == 0 && (need == 0 || rank + need <= free_pages);
-    int pages;
-    block_scan(ok ? need : 0, &pages);
-    if (i < c.slots) {
-      u.rank[i] = ok ? rank : -1;
-      if (touch && c.status != nullptr) c.status[i] = st != 0 ? st : (ok ? 0 : 2);
-    }
-    asked += total;
-    granted += pages;
+  Asked a(c, u, [&](int i) {  // pages; -1: it stays as it is; -2: no such source
+    const int s = source[i];
+    if (s == -1 || s == i) return -1;
+    if (s < 0 || s >= c.slots) return -2;
+    const int len = c.length(s);
+    return deep ? (len + c.page_size - 1) >> c.page_shift : ((len & (c.page_size - 1)) != 0 ? 1 : 0);
+  });
+  const int free_pages = list_free(c, u.free_list, a.all);
+  for (int i = threadIdx.x; i < c.slots; i += kPlanThreads) {
+    a.load(u, i);
+    const bool ok = a.granted(free_pages);
+    u.rank[i] = ok ? a.rank : -1;
+    if (ok && a.need > 0) atomicMax(&copies, a.rank + a.need);
+    if (a.need != -1 && c.status != nullptr) c.status[i] = a.need == -2 ? 1 : (ok ? 0 : 2);
   }
-  if (threadIdx.x == 0) u.counts[0] = granted;
+  __syncthreads();
+  if (threadIdx.x == 0) u.counts[0] = copies;
 }
 
 // Slot d (one CTA each): its new row, from its source's old one, and the page copies it asks for.
@@ -267,7 +289,7 @@ __global__ void __launch_bounds__(kMoveThreads) free_kernel(PagedCache c, const 
 // One CTA: live pages, and where those past the live count go.
 __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(PagedCache c, UpkeepSpace u) {
   take_turn();
-  const int live = c.pages - list_free(c, u.free_list);  // free pages below `live` come first in the list
+  const int live = c.pages - list_free(c, u.free_list, INT32_MAX);  // free pages below `live` come first in the list
   int moved = 0;
   for (int base = live & ~(4 * kPlanThreads - 1); base < c.pages; base += 4 * kPlanThreads) {
     const int p0 = base + 4 * threadIdx.x;
@@ -357,16 +379,33 @@ __global__ void __launch_bounds__(kMoveThreads) store_kernel(PagedCache c, Rows 
     if (threadIdx.x == 0 && c.status != nullptr) c.status[slot] = 3;
     return;
   }
+  // A thread keeps its piece of the heads and walks over (layer, keys or
+  // values), several rows of threads side by side where the heads are few.
   const int hv = c.kv_heads * c.head_dim / 8;  // 16-byte pieces of one layer's keys
-  const int dv = c.head_dim / 8;
-  const int in_page = t & (c.page_size - 1);
-  for (int w = threadIdx.x; w < in.n_layers * 2 * hv; w += kMoveThreads) {
-    const int piece = w % hv, kv = (w / hv) & 1, l = w / (2 * hv);
-    const uint16_t* src = kv ? in.v + l * in.v_layer + row * in.v_row : in.k + l * in.k_layer + row * in.k_row;
-    const int h = piece / dv, e = piece % dv;
-    uint16_t* dst = c.pool + c.block(page, in.layer + l, kv) +
-                    (static_cast<int64_t>(h) * c.page_size + in_page) * c.head_dim + 8 * e;
-    *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(src + 8 * piece);
+  const int dv_shift = c.head_dim == 64 ? 3 : 4;
+  const int side = max(1, kMoveThreads / hv), blocks = 2 * in.n_layers;
+  const int mine = static_cast<int>(threadIdx.x) / min(hv, kMoveThreads);
+  if (mine >= side) return;
+  const int64_t in_page = static_cast<int64_t>(t & (c.page_size - 1)) * c.head_dim;
+  for (int piece = hv < kMoveThreads ? threadIdx.x - mine * hv : threadIdx.x; piece < hv; piece += kMoveThreads) {
+    const int h = piece >> dv_shift, e = piece & ((1 << dv_shift) - 1);
+    uint16_t* dst = c.pool + c.block(page, in.layer, 0) + static_cast<int64_t>(h) * c.page_size * c.head_dim + in_page + 8 * e;
+    const uint16_t* k = in.k + row * in.k_row + 8 * piece;
+    const uint16_t* v = in.v + row * in.v_row + 8 * piece;
+    constexpr int kAhead = 4;
+    for (int b = mine; b < blocks; b += kAhead * side) {
+      uint4 x[kAhead];
+#pragma unroll
+      for (int n = 0; n < kAhead; ++n) {
+        const int at = b + n * side, l = at >> 1;
+        if (at < blocks) x[n] = __ldcs(reinterpret_cast<const uint4*>((at & 1) ? v + l * in.v_layer : k + l * in.k_layer));
+      }
+#pragma unroll
+      for (int n = 0; n < kAhead; ++n) {
+        const int at = b + n * side;
+        if (at < blocks) *reinterpret_cast<uint4*>(dst + at * c.kv_elems) = x[n];
+      }
+    }
   }
 }
 
@@ -409,7 +448,7 @@ bool paged_cache_view(const mtt_b200_paged_cache_t* c, PagedCache* out) {
       static_cast<double>(c->slots) * c->table_pages * (c->page_size / 16) >= 2147352576.0)
     return false;
   if (c->pool == nullptr || c->page_table == nullptr || c->lengths == nullptr || c->refs == nullptr ||
-      (reinterpret_cast<uintptr_t>(c->pool) & 127u) != 0)
+      (reinterpret_cast<uintptr_t>(c->pool) & 127u) != 0 || !aligned16(c->refs))
     return false;
   out->pages = c->pages;
   out->layers = c->layers;

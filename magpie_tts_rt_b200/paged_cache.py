@@ -79,7 +79,8 @@ class PagedCache:
         for name, t in (("pool", pool), ("page_table", page_table), ("lengths", lengths), ("refs", refs)):
             _check(t.is_contiguous(), f"{name} must be contiguous")
             _check(t.device == pool.device, f"{name} is on another device than the pool")
-        _check(pool.data_ptr() % 128 == 0, "the pool must be 128-byte aligned")
+        _check(pool.data_ptr() % 128 == 0 and refs.data_ptr() % 16 == 0,
+               "the pool must be 128-byte aligned, refs 16-byte aligned")
         self.pool, self.page_table, self.lengths, self.refs = pool, page_table, lengths, refs
         self.device = pool.device
         self._index = pool.device.index
