@@ -228,7 +228,10 @@ __global__ void __launch_bounds__(kMoveThreads) fork_rows_kernel(PagedCache c, c
   if (threadIdx.x == 0) u.len[d] = len;
 }
 
-// Part `part` of `parts` of one page, all layers.
+// Part `part` of `parts` of one page, all layers.  kAgain: other copies read the
+// same page (a voice's partial page goes to every session forked from it), so
+// it stays in L2.
+template <bool kAgain>
 __device__ __forceinline__ void copy_page(const PagedCache& c, int from, int to, int part, int parts) {
   const int64_t vecs = static_cast<int64_t>(c.layers) * 2 * c.kv_elems / 8;
   const int64_t lo = vecs * part / parts, hi = vecs * (part + 1) / parts;
@@ -238,7 +241,7 @@ __device__ __forceinline__ void copy_page(const PagedCache& c, int from, int to,
   for (; v + 3 * kMoveThreads < hi; v += 4 * kMoveThreads) {
     uint4 x[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = __ldcs(s + v + j * kMoveThreads);
+    for (int j = 0; j < 4; ++j) x[j] = kAgain ? __ldcg(s + v + j * kMoveThreads) : __ldcs(s + v + j * kMoveThreads);
 #pragma unroll
     for (int j = 0; j < 4; ++j) __stcs(d + v + j * kMoveThreads, x[j]);
   }
@@ -246,12 +249,13 @@ __device__ __forceinline__ void copy_page(const PagedCache& c, int from, int to,
 }
 
 // The plan's page copies, `parts` pieces each, dealt over the grid.
+template <bool kAgain>
 __device__ __forceinline__ void copy_pairs(const PagedCache& c, const UpkeepSpace& u, int parts) {
   const int64_t items = static_cast<int64_t>(u.counts[0]) * parts;
   for (int64_t w = blockIdx.x; w < items; w += gridDim.x) {
     const int pair = static_cast<int>(w / parts);
     const int from = u.src[pair], to = u.dst[pair];
-    if (c.is_page(from) && c.is_page(to)) copy_page(c, from, to, static_cast<int>(w % parts), parts);
+    if (c.is_page(from) && c.is_page(to)) copy_page<kAgain>(c, from, to, static_cast<int>(w % parts), parts);
   }
 }
 
@@ -269,7 +273,7 @@ __global__ void __launch_bounds__(kMoveThreads) fork_commit_kernel(PagedCache c,
     }
     if (threadIdx.x == 0) c.lengths[d] = u.len[d];
   }
-  copy_pairs(c, u, parts);
+  copy_pairs<true>(c, u, parts);
 }
 
 // One warp per slot.
@@ -336,7 +340,7 @@ __global__ void __launch_bounds__(kMoveThreads) compact_move_kernel(PagedCache c
     c.refs[u.dst[m]] = c.refs[u.src[m]];
     c.refs[u.src[m]] = 0;
   }
-  copy_pairs(c, u, parts);
+  copy_pairs<false>(c, u, parts);
 }
 
 struct Rows {
