@@ -762,8 +762,8 @@ typedef struct mtt_b200_paged_cache {
 } mtt_b200_paged_cache_t;
 
 /* Workspace bytes for any call on this cache with up to `rows` query rows of
- * q_heads heads (0 for bad arguments).  256-byte aligned, zeroed once before its first use; one
- * workspace serves one stream at a time. */
+ * q_heads heads (0 for bad arguments).  256-byte aligned; nothing is kept in it
+ * from one call to the next, and one workspace serves one stream at a time. */
 MTT_B200_API size_t mtt_b200_paged_cache_workspace_size(const mtt_b200_paged_cache_t* cache, int32_t q_heads,
                                                         int32_t rows);
 
@@ -820,9 +820,12 @@ MTT_B200_API int mtt_b200_launch_paged_cache_store(const mtt_b200_paged_cache_t*
  * sinks) and key_mask[slot][j] (where given):
  *   out = sum_j exp(scale q.k_j) v_j / sum_j exp(scale q.k_j)
  *   lse = log sum_j exp(scale q.k_j)          (natural log, f32)
- * with f32 sums and probabilities rounded once to the cache's type; a row that sees no key gets out 0 and lse -inf.  Keys that
- * no query may see (past the length, or masked) do not reach the result,
- * whatever their bytes.  Query head h reads key head h / (q_heads / kv_heads).
+ * with f32 sums and probabilities rounded once to the cache's type (relative
+ * to that, 2^-8 or 2^-11, the result is off by less than sum_j p_j |v_j| + |out|); a row that sees no key gets out 0 and lse -inf.  Keys that
+ * no query of the slot may see (past the length, or masked) do not reach the
+ * result, whatever their bytes; a value that is not finite makes those of the
+ * slot's queries not finite that see it, and may make earlier ones of the same
+ * call so.  Query head h reads key head h / (q_heads / kv_heads).
  *
  * offsets NULL: row i is the last token of slot i (rows <= slots).  With
  * offsets ([slots + 1] int32, as for store) slot i's rows are its last
@@ -868,8 +871,7 @@ typedef struct mtt_b200_prefix_groups {
                                 every slot is attended on its own. */
 } mtt_b200_prefix_groups_t;
 
-/* Workspace bytes of the call below (0 for bad arguments); alignment and
- * zeroing as above. */
+/* Workspace bytes of the call below (0 for bad arguments); aligned as above. */
 MTT_B200_API size_t mtt_b200_paged_shared_workspace_size(const mtt_b200_paged_cache_t* cache, int32_t q_heads,
                                                          int32_t n_members);
 

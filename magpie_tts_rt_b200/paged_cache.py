@@ -16,7 +16,7 @@ slot, and a reference count per page, all on the device:
   prefix (``PrefixGroups``), computed once for each group.
 
 Every call is enqueued on the current (or given) CUDA stream and returns
-without waiting.  What a call cannot do on the device (no free page, offsets
+without waiting; no gradient is recorded (this is a decoder's cache).  What a call cannot do on the device (no free page, offsets
 that do not fit) it reports in ``status``; what can be seen on the host
 (types, shapes, strides) raises ValueError before anything is launched.
 
@@ -129,7 +129,7 @@ class PagedCache:
             size = L.lib.mtt_b200_paged_cache_workspace_size(self._ref, q_heads, most)
             _check(size > 0, "this cache and number of heads or rows are not supported")
             with self._on(stream):
-                data = torch.zeros(size, dtype=torch.uint8, device=self.device)
+                data = torch.empty(size, dtype=torch.uint8, device=self.device)
             space = self._spaces[handle, q_heads] = (data.data_ptr(), size, most, data)
         return space
 
@@ -358,6 +358,6 @@ class PrefixGroups:
         if space is None:
             size = L.lib.mtt_b200_paged_shared_workspace_size(self.cache._ref, self.q_heads, self.n_members)
             with PagedCache._on(stream):
-                data = torch.zeros(size, dtype=torch.uint8, device=self.cache.device)
+                data = torch.empty(size, dtype=torch.uint8, device=self.cache.device)
             space = self._spaces[handle] = (data.data_ptr(), size, data)
         return space
