@@ -787,7 +787,8 @@ MTT_B200_API int mtt_b200_launch_paged_cache_free(const mtt_b200_paged_cache_t* 
                                                   void* stream);
 
 /* Moves pages so that those in use are [0, live): the i-th page in use at or
- * past `live` goes to the i-th free page before it; tables and refs follow. */
+ * past `live` goes to the i-th free page before it; tables and refs follow
+ * (a page in use is one with refs, whether or not a slot's table names it). */
 MTT_B200_API int mtt_b200_launch_paged_cache_compact(const mtt_b200_paged_cache_t* cache, void* workspace,
                                                      size_t workspace_bytes, void* stream);
 

@@ -21,7 +21,9 @@ that do not fit) it reports in ``status``; what can be seen on the host
 (types, shapes, strides) raises ValueError before anything is launched.
 
 Calls that change a cache, and the calls that read it, must be ordered with
-each other by the caller when they use different streams.
+each other by the caller when they use different streams.  Every call can be
+captured into a CUDA graph after one such call on the capturing stream (which
+makes that stream's workspace).
 """
 from __future__ import annotations
 
@@ -100,6 +102,7 @@ class PagedCache:
         self._ref = ctypes.byref(c)
         self._scale = head_dim ** -0.5
         self._spaces = {}  # (stream, query heads) -> workspace
+        self._outgrown = []
         _check(L.lib.mtt_b200_paged_cache_workspace_size(self._ref, kv_heads, 0) > 0, "this cache is too large")
 
     @staticmethod
@@ -130,6 +133,8 @@ class PagedCache:
             _check(size > 0, "this cache and number of heads or rows are not supported")
             with self._on(stream):
                 data = torch.empty(size, dtype=torch.uint8, device=self.device)
+            if space is not None:
+                self._outgrown.append(space)  # a CUDA graph captured with it may still replay
             space = self._spaces[handle, q_heads] = (data.data_ptr(), size, most, data)
         return space
 
