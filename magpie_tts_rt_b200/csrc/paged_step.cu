@@ -22,14 +22,17 @@
 //    unit that a cut divides leaves (maximum, sum, weighted values) of each
 //    part in the workspace; a second kernel joins the parts in their order,
 //    so the result does not depend on timing.
-// Measured, both kernels: 512 slots of 12 heads of 64, up to 1242 of 2048 keys in
+//  * Few slots, whose call is launches and latency, take clusters instead
+//    (step_few_kernel): one launch.
+// Measured, line and join: 512 slots of 12 heads of 64, up to 1242 of 2048 keys in
 // reach, 162 us (6.7 TB/s of the keys and values in reach; 974 MB from DRAM); 8
-// slots of 30,001 to 65,536 keys, 32/8 heads of 128, 238 us (6.3 TB/s); 2 slots of
-// 467 keys 8 us, of which two launches are most.  What bounds it is DRAM; where
-// sequences are short (1 to 249 keys) a unit's chain of dependent loads (63 us
+// slots of 30,001 to 65,536 keys, 32/8 heads of 128, 238 us (6.3 TB/s).
+// Clusters: 2 slots of 467 keys, 12 heads of 64, 5.3 us (9.0 us as a line).  What
+// bounds the line is DRAM; where sequences are short (1 to 249 keys) a unit's chain of dependent loads (63 us
 // for 275 MB).  Tried: shares per CTA with the four warps of a CTA side by side
 // in a unit (187 and 247 us, 389 us for the short ones).
 #include <algorithm>
+#include <type_traits>
 
 #include "paged_attention.cuh"
 
@@ -104,6 +107,17 @@ struct RowPart {
   }
 };
 
+// Waits for the cluster's CTAs; what they wrote to shared memory before is visible.
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ float2 load_cluster(uint32_t at) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at));
+  return v;
+}
+
 // Not the read-only path: the launch before this one may have written the
 // cache, and this kernel may already have been scheduled by then.
 __device__ __forceinline__ uint4 load16(const uint16_t* p, bool on) {
@@ -115,13 +129,142 @@ __device__ __forceinline__ uint4 load16(const uint16_t* p, bool on) {
   return v;
 }
 
+// A thread's running maximum (base 2), sum and weighted values: queries 2t, 2t + 1
+// of each 8, dims 8g .. 8g + 7 of each 64.
+template <int D, int NB>
+struct StepSums {
+  float m[NB][2], l[NB][2], acc[NB][D / 64][4][4];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      m[b][0] = m[b][1] = -CUDART_INF_F;
+      l[b][0] = l[b][1] = 0.f;
+#pragma unroll
+      for (int v = 0; v < D / 64; ++v)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) acc[b][v][w][0] = acc[b][v][w][1] = acc[b][v][w][2] = acc[b][v][w][3] = 0.f;
+    }
+  }
+};
+
+// A warp's tiles t0 .. t1 - 1 of a unit.  `page` holds the pages of the first
+// step's tiles.
+template <typename T, int D, int NB>
+__device__ __forceinline__ void attend_tiles(const PagedCache& c, const Attend& a, const SeenTiles& seen,
+                                             const int32_t* row, const bool* mask, int64_t head_at, int t0, int t1,
+                                             const uint4 (&q)[NB][D / 32], int (&page)[step_tiles(D)],
+                                             StepSums<D, NB>& sums) {
+  constexpr int NT = step_tiles(D);
+  constexpr int KC = D / 32;  // 16-byte pieces of a key row per thread
+  constexpr int VC = D / 64;  // of a value row
+  const int lane = threadIdx.x & 31, t = lane & 3, g = lane >> 2;
+  auto& [m, l, acc] = sums;
+      for (int base = t0; base < t1; base += NT) {
+        // keys in reach: one per lane
+        const int my_tile = base + (lane >> 4);
+        bool in = my_tile < t1 && (lane >> 4) < NT;
+        {
+          const int j = 16 * seen.tile(my_tile) + (lane & 15);
+          in = in && j < seen.len && (j >= seen.low || j < a.sinks);
+          if (in && mask != nullptr) in = mask[j];
+        }
+        const uint32_t bits = __ballot_sync(0xffffffffu, in);
+        uint4 kr[NT][2][KC], vr[NT][4][VC];
+        uint32_t on[NT];
+  #pragma unroll
+        for (int u = 0; u < NT; ++u) {
+          on[u] = c.is_page(page[u]) ? (bits >> (16 * u)) & 0xffffu : 0u;
+          const int in_page = (16 * seen.tile(base + u)) & (c.page_size - 1);
+          const uint16_t* kp = c.pool + c.block(page[u], a.layer, 0) + head_at + static_cast<int64_t>(in_page) * D;
+  #pragma unroll
+          for (int h = 0; h < 2; ++h)
+  #pragma unroll
+            for (int k = 0; k < KC; ++k)
+              kr[u][h][k] = load16(kp + (g + 8 * h) * D + 8 * (t + 4 * k), (on[u] >> (g + 8 * h)) & 1u);
+          const uint16_t* vp = kp + c.kv_elems;
+  #pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int key = 2 * t + (i & 1) + 8 * (i >> 1);
+  #pragma unroll
+            for (int v = 0; v < VC; ++v) vr[u][i][v] = load16(vp + key * D + 8 * (g + 8 * v), (on[u] >> key) & 1u);
+          }
+        }
+        // the next step's pages, while this step's keys arrive
+  #pragma unroll
+        for (int u = 0; u < NT; ++u) {
+          const int tt = base + NT + u;
+          page[u] = tt < t1 ? row[(16 * seen.tile(tt)) >> c.page_shift] : -1;
+        }
+  #pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          float s[NT][4];
+          float top0 = m[b][0], top1 = m[b][1];
+  #pragma unroll
+          for (int u = 0; u < NT; ++u) {
+            s[u][0] = s[u][1] = s[u][2] = s[u][3] = 0.f;
+  #pragma unroll
+            for (int k = 0; k < KC; ++k) {
+              Half16<T>::mma(s[u], kr[u][0][k].x, kr[u][1][k].x, kr[u][0][k].y, kr[u][1][k].y, q[b][k].x, q[b][k].y);
+              Half16<T>::mma(s[u], kr[u][0][k].z, kr[u][1][k].z, kr[u][0][k].w, kr[u][1][k].w, q[b][k].z, q[b][k].w);
+            }
+            const bool lo = (on[u] >> g) & 1u, hi = (on[u] >> (g + 8)) & 1u;
+            s[u][0] = lo ? s[u][0] * a.scale2 : -CUDART_INF_F;
+            s[u][1] = lo ? s[u][1] * a.scale2 : -CUDART_INF_F;
+            s[u][2] = hi ? s[u][2] * a.scale2 : -CUDART_INF_F;
+            s[u][3] = hi ? s[u][3] * a.scale2 : -CUDART_INF_F;
+            top0 = fmaxf(top0, fmaxf(s[u][0], s[u][2]));
+            top1 = fmaxf(top1, fmaxf(s[u][1], s[u][3]));
+          }
+  #pragma unroll
+          for (int o = 4; o < 32; o <<= 1) {
+            top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, o));
+            top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, o));
+          }
+          const float z0 = top0 == -CUDART_INF_F ? 0.f : top0, z1 = top1 == -CUDART_INF_F ? 0.f : top1;
+          const float keep0 = ex2(m[b][0] - z0), keep1 = ex2(m[b][1] - z1);
+          m[b][0] = top0;
+          m[b][1] = top1;
+          l[b][0] *= keep0;
+          l[b][1] *= keep1;
+  #pragma unroll
+          for (int v = 0; v < VC; ++v)
+  #pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              acc[b][v][w][0] *= keep0;
+              acc[b][v][w][1] *= keep1;
+              acc[b][v][w][2] *= keep0;
+              acc[b][v][w][3] *= keep1;
+            }
+  #pragma unroll
+          for (int u = 0; u < NT; ++u) {
+            const float p0 = ex2(s[u][0] - z0), p1 = ex2(s[u][1] - z1), p2 = ex2(s[u][2] - z0), p3 = ex2(s[u][3] - z1);
+            // the sum keeps the unrounded probabilities; the values' weights are rounded to 16 bits once
+            l[b][0] += p0 + p2;
+            l[b][1] += p1 + p3;
+            const uint32_t b0 = transpose8x8(Half16<T>::pack(p0, p1)), b1 = transpose8x8(Half16<T>::pack(p2, p3));
+  #pragma unroll
+            for (int v = 0; v < VC; ++v) {
+              const uint4 &x0 = vr[u][0][v], &x1 = vr[u][1][v], &x2 = vr[u][2][v], &x3 = vr[u][3][v];
+              Half16<T>::mma(acc[b][v][0], __byte_perm(x0.x, x1.x, 0x5410), __byte_perm(x0.x, x1.x, 0x7632),
+                             __byte_perm(x2.x, x3.x, 0x5410), __byte_perm(x2.x, x3.x, 0x7632), b0, b1);
+              Half16<T>::mma(acc[b][v][1], __byte_perm(x0.y, x1.y, 0x5410), __byte_perm(x0.y, x1.y, 0x7632),
+                             __byte_perm(x2.y, x3.y, 0x5410), __byte_perm(x2.y, x3.y, 0x7632), b0, b1);
+              Half16<T>::mma(acc[b][v][2], __byte_perm(x0.z, x1.z, 0x5410), __byte_perm(x0.z, x1.z, 0x7632),
+                             __byte_perm(x2.z, x3.z, 0x5410), __byte_perm(x2.z, x3.z, 0x7632), b0, b1);
+              Half16<T>::mma(acc[b][v][3], __byte_perm(x0.w, x1.w, 0x5410), __byte_perm(x0.w, x1.w, 0x7632),
+                             __byte_perm(x2.w, x3.w, 0x5410), __byte_perm(x2.w, x3.w, 0x7632), b0, b1);
+            }
+          }
+        }
+      }
+}
+
 template <typename T, int D, int NB>
 __global__ void __launch_bounds__(kStepThreads, step_ctas(D, NB))
     step_kernel(PagedCache c, Attend a, SharedPrefix shared, StepSpace ws, int blocks, int min_tiles) {
   constexpr int NT = step_tiles(D);
   constexpr int NQ = 8 * NB;   // query rows of a unit
-  constexpr int KC = D / 32;   // 16-byte pieces of a key row per thread
-  constexpr int VC = D / 64;   // of a value row
+  constexpr int KC = D / 32, VC = D / 64;
   extern __shared__ int tiles_before[];  // [rows + 1]: tiles of a key head of the slots before
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int t = lane & 3, g = lane >> 2;
@@ -227,115 +370,10 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(D, NB))
     const int32_t* row = c.table + static_cast<int64_t>(slot) * c.table_pages;
     const bool* mask = a.key_mask != nullptr ? a.key_mask + slot * a.mask_stride : nullptr;
     const int64_t head_at = static_cast<int64_t>(head) * c.page_size * D;
-    float m[NB][2], l[NB][2], acc[NB][VC][4][4];
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      m[b][0] = m[b][1] = -CUDART_INF_F;
-      l[b][0] = l[b][1] = 0.f;
-#pragma unroll
-      for (int v = 0; v < VC; ++v)
-#pragma unroll
-        for (int w = 0; w < 4; ++w) acc[b][v][w][0] = acc[b][v][w][1] = acc[b][v][w][2] = acc[b][v][w][3] = 0.f;
-    }
-
-    for (int base = t0; base < t1; base += NT) {
-      // keys in reach: one per lane
-      const int my_tile = base + (lane >> 4);
-      bool in = my_tile < t1 && (lane >> 4) < NT;
-      {
-        const int j = 16 * seen.tile(my_tile) + (lane & 15);
-        in = in && j < seen.len && (j >= seen.low || j < a.sinks);
-        if (in && mask != nullptr) in = mask[j];
-      }
-      const uint32_t bits = __ballot_sync(0xffffffffu, in);
-      uint4 kr[NT][2][KC], vr[NT][4][VC];
-      uint32_t on[NT];
-#pragma unroll
-      for (int u = 0; u < NT; ++u) {
-        on[u] = c.is_page(page[u]) ? (bits >> (16 * u)) & 0xffffu : 0u;
-        const int in_page = (16 * seen.tile(base + u)) & (c.page_size - 1);
-        const uint16_t* kp = c.pool + c.block(page[u], a.layer, 0) + head_at + static_cast<int64_t>(in_page) * D;
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int k = 0; k < KC; ++k)
-            kr[u][h][k] = load16(kp + (g + 8 * h) * D + 8 * (t + 4 * k), (on[u] >> (g + 8 * h)) & 1u);
-        const uint16_t* vp = kp + c.kv_elems;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int key = 2 * t + (i & 1) + 8 * (i >> 1);
-#pragma unroll
-          for (int v = 0; v < VC; ++v) vr[u][i][v] = load16(vp + key * D + 8 * (g + 8 * v), (on[u] >> key) & 1u);
-        }
-      }
-      // the next step's pages, while this step's keys arrive
-#pragma unroll
-      for (int u = 0; u < NT; ++u) {
-        const int tt = base + NT + u;
-        page[u] = tt < t1 ? row[(16 * seen.tile(tt)) >> c.page_shift] : -1;
-      }
-#pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        float s[NT][4];
-        float top0 = m[b][0], top1 = m[b][1];
-#pragma unroll
-        for (int u = 0; u < NT; ++u) {
-          s[u][0] = s[u][1] = s[u][2] = s[u][3] = 0.f;
-#pragma unroll
-          for (int k = 0; k < KC; ++k) {
-            Half16<T>::mma(s[u], kr[u][0][k].x, kr[u][1][k].x, kr[u][0][k].y, kr[u][1][k].y, q[b][k].x, q[b][k].y);
-            Half16<T>::mma(s[u], kr[u][0][k].z, kr[u][1][k].z, kr[u][0][k].w, kr[u][1][k].w, q[b][k].z, q[b][k].w);
-          }
-          const bool lo = (on[u] >> g) & 1u, hi = (on[u] >> (g + 8)) & 1u;
-          s[u][0] = lo ? s[u][0] * a.scale2 : -CUDART_INF_F;
-          s[u][1] = lo ? s[u][1] * a.scale2 : -CUDART_INF_F;
-          s[u][2] = hi ? s[u][2] * a.scale2 : -CUDART_INF_F;
-          s[u][3] = hi ? s[u][3] * a.scale2 : -CUDART_INF_F;
-          top0 = fmaxf(top0, fmaxf(s[u][0], s[u][2]));
-          top1 = fmaxf(top1, fmaxf(s[u][1], s[u][3]));
-        }
-#pragma unroll
-        for (int o = 4; o < 32; o <<= 1) {
-          top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, o));
-          top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, o));
-        }
-        const float z0 = top0 == -CUDART_INF_F ? 0.f : top0, z1 = top1 == -CUDART_INF_F ? 0.f : top1;
-        const float keep0 = ex2(m[b][0] - z0), keep1 = ex2(m[b][1] - z1);
-        m[b][0] = top0;
-        m[b][1] = top1;
-        l[b][0] *= keep0;
-        l[b][1] *= keep1;
-#pragma unroll
-        for (int v = 0; v < VC; ++v)
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            acc[b][v][w][0] *= keep0;
-            acc[b][v][w][1] *= keep1;
-            acc[b][v][w][2] *= keep0;
-            acc[b][v][w][3] *= keep1;
-          }
-#pragma unroll
-        for (int u = 0; u < NT; ++u) {
-          const float p0 = ex2(s[u][0] - z0), p1 = ex2(s[u][1] - z1), p2 = ex2(s[u][2] - z0), p3 = ex2(s[u][3] - z1);
-          // the sum keeps the unrounded probabilities; the values' weights are rounded to 16 bits once
-          l[b][0] += p0 + p2;
-          l[b][1] += p1 + p3;
-          const uint32_t b0 = transpose8x8(Half16<T>::pack(p0, p1)), b1 = transpose8x8(Half16<T>::pack(p2, p3));
-#pragma unroll
-          for (int v = 0; v < VC; ++v) {
-            const uint4 &x0 = vr[u][0][v], &x1 = vr[u][1][v], &x2 = vr[u][2][v], &x3 = vr[u][3][v];
-            Half16<T>::mma(acc[b][v][0], __byte_perm(x0.x, x1.x, 0x5410), __byte_perm(x0.x, x1.x, 0x7632),
-                           __byte_perm(x2.x, x3.x, 0x5410), __byte_perm(x2.x, x3.x, 0x7632), b0, b1);
-            Half16<T>::mma(acc[b][v][1], __byte_perm(x0.y, x1.y, 0x5410), __byte_perm(x0.y, x1.y, 0x7632),
-                           __byte_perm(x2.y, x3.y, 0x5410), __byte_perm(x2.y, x3.y, 0x7632), b0, b1);
-            Half16<T>::mma(acc[b][v][2], __byte_perm(x0.z, x1.z, 0x5410), __byte_perm(x0.z, x1.z, 0x7632),
-                           __byte_perm(x2.z, x3.z, 0x5410), __byte_perm(x2.z, x3.z, 0x7632), b0, b1);
-            Half16<T>::mma(acc[b][v][3], __byte_perm(x0.w, x1.w, 0x5410), __byte_perm(x0.w, x1.w, 0x7632),
-                           __byte_perm(x2.w, x3.w, 0x5410), __byte_perm(x2.w, x3.w, 0x7632), b0, b1);
-          }
-        }
-      }
-    }
+    StepSums<D, NB> sums;
+    sums.clear();
+    attend_tiles<T, D, NB>(c, a, seen, row, mask, head_at, t0, t1, q, page, sums);
+    auto& [m, l, acc] = sums;
 
     // a thread holds queries 2t, 2t + 1 and dims 8g .. 8g + 7 of each 64
     const bool whole = t0 == 0 && t1 == seen.n, some = t0 < t1;
@@ -466,6 +504,159 @@ __global__ void __launch_bounds__(kStepThreads)
   }
 }
 
+// Few slots: a cluster of 1 to 8 CTAs for each unit, its tiles dealt to the
+// cluster's warps, which join their parts through shared memory: one launch and
+// no workspace.  The largest cluster is taken with which all units run at once
+// (8 CTAs of 8 warps only where a slot can have more than one step for each of 32
+// warps), if a slot cannot be longer than kFewSteps steps of each of its warps.
+// There this saves the scan, the second launch and the parts' way through L2;
+// past either limit the line of tiles is faster, as it fills the device and
+// balances it.  GPU time of a call in us, line / clusters, bf16, all slots of the
+// same length (in brackets what is not taken):
+//   heads  dim  slots    128 keys      467         1000         2000         8000
+//   12/12   64    2     8.7 /  6.4  11.7 /  7.0  13.2 /  7.6  14.7 /  8.5  22.5 / 16.7
+//   12/12   64    9    11.2 /  7.3  13.2 /  8.2  15.7 / 13.1  19.5 / 17.4
+//   12/12   64   24    12.5 /  7.1  13.9 / 11.9  20.8 / 18.5 (32.6 / 29.4)
+//   32/8   128    4    14.3 /  7.5  15.4 /  8.6  17.1 / 10.4  20.9 / 15.1 (36.0 / 34.8)
+//   32/8   128   16    15.5 /  8.2  18.3 / 13.4  24.3 / 19.5 (34.8 / 30.8)
+//   32/8   128   48    17.4 / 12.0 (29.1 / 27.4) (45.9 / 48.6)
+//   16/1   128    6    21.3 /  7.7  21.9 /  8.4  23.7 /  9.1  25.2 / 11.1
+constexpr int kMaxSpread = 8, kFewSteps = 4;
+
+template <typename T, int D, int NB, int W>
+__global__ void __launch_bounds__(32 * W) step_few_kernel(PagedCache c, Attend a, int blocks, int spread) {
+  constexpr int NT = step_tiles(D);
+  constexpr int NQ = 8 * NB, KC = D / 32, VC = D / 64;
+  constexpr int kRow = D + 2;  // weighted values, maximum, sum
+  extern __shared__ float few_smem[];
+  auto parts = reinterpret_cast<float (*)[NQ][kRow]>(few_smem);  // [W]
+  auto& joined = parts[W];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int t = lane & 3, g = lane >> 2;
+  const int rank = blockIdx.x % spread, unit = blockIdx.x / spread;
+  const int block = unit % blocks, head = unit / blocks % c.kv_heads, slot = unit / blocks / c.kv_heads;
+  const int queries = min(NQ, a.group - block * NQ), q_head = head * a.group + block * NQ;
+  take_turn();
+
+  const SeenTiles seen(c.length(slot), a.window, a.sinks, 0);
+  // steps of NT tiles, dealt evenly
+  const int warps = spread * W;
+  const int steps = (seen.n + NT - 1) / NT, me = rank * W + warp;
+  const int t0 = NT * static_cast<int>(static_cast<int64_t>(steps) * me / warps);
+  const int t1 = min(seen.n, NT * static_cast<int>(static_cast<int64_t>(steps) * (me + 1) / warps));
+  const int32_t* row = c.table + static_cast<int64_t>(slot) * c.table_pages;
+  uint4 q[NB][KC];
+  int page[NT];
+#pragma unroll
+  for (int u = 0; u < NT; ++u) page[u] = t0 + u < t1 ? row[(16 * seen.tile(t0 + u)) >> c.page_shift] : -1;
+  const int64_t q_at = slot * a.q_row + static_cast<int64_t>(q_head + g) * D + 8 * t;
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int k = 0; k < KC; ++k) q[b][k] = load16(a.q + q_at + 8 * b * D + 32 * k, 8 * b + g < queries);
+  StepSums<D, NB> sums;
+  sums.clear();
+  attend_tiles<T, D, NB>(c, a, seen, row, a.key_mask != nullptr ? a.key_mask + slot * a.mask_stride : nullptr,
+                         static_cast<int64_t>(head) * c.page_size * D, t0, t1, q, page, sums);
+  auto& [m, l, acc] = sums;
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) l[b][i] += __shfl_xor_sync(0xffffffffu, l[b][i], o);
+      float* part = parts[warp][8 * b + 2 * t + i];
+#pragma unroll
+      for (int v = 0; v < VC; ++v)
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+          *reinterpret_cast<float2*>(part + 64 * v + 8 * g + 2 * w) = make_float2(acc[b][v][w][i], acc[b][v][w][2 + i]);
+      if (g == 0) *reinterpret_cast<float2*>(part + D) = make_float2(m[b][i], l[b][i]);
+    }
+  __syncthreads();
+  const int pairs = queries * (D / 2);  // of dims
+  auto join = [&](int n, auto at) {  // of n parts, in order
+    RowPart<2> r;
+    r.none();
+    float2 ml[kMaxSpread], y[kMaxSpread];
+#pragma unroll
+    for (int k = 0; k < kMaxSpread; ++k)
+      if (k < n) at(k, &ml[k], &y[k]);
+#pragma unroll
+    for (int k = 0; k < kMaxSpread; ++k)
+      if (k < n) {
+        RowPart<2> x;
+        x.m = ml[k].x;
+        x.l = ml[k].y;
+        x.o[0] = y[k].x;
+        x.o[1] = y[k].y;
+        r.join(x);
+      }
+    return r;
+  };
+  for (int e = tid; e < pairs; e += 32 * W) {
+    const int qi = e / (D / 2), d = 2 * (e % (D / 2));
+    const RowPart<2> r = join(W, [&](int k, float2* ml, float2* y) {
+      *ml = *reinterpret_cast<const float2*>(&parts[k][qi][D]);
+      *y = *reinterpret_cast<const float2*>(&parts[k][qi][d]);
+    });
+    *reinterpret_cast<float2*>(&joined[qi][d]) = make_float2(r.o[0], r.o[1]);
+    if (d == 0) *reinterpret_cast<float2*>(&joined[qi][D]) = make_float2(r.m, r.l);
+  }
+  cluster_sync();
+  const int each = pairs / spread;  // D / 2 is a multiple of it
+  for (int e = rank * each + tid; e < (rank + 1) * each; e += 32 * W) {
+    const int qi = e / (D / 2), d = 2 * (e % (D / 2));
+    const RowPart<2> r = join(spread, [&](int k, float2* ml, float2* y) {
+      *ml = load_cluster(cluster_addr(&joined[qi][D], k));
+      *y = load_cluster(cluster_addr(&joined[qi][d], k));
+    });
+    r.store<T, D>(a, slot, q_head + qi, d);
+  }
+  cluster_sync();  // the others may still be reading this CTA's shared memory
+}
+
+constexpr size_t few_bytes(int head_dim, int nb, int warps) {
+  return static_cast<size_t>(warps + 1) * 8 * nb * (head_dim + 2) * 4;
+}
+
+// Launch of step_few_kernel with clusters of `spread` CTAs.
+struct FewLaunch {
+  cudaLaunchAttribute attr[2];
+  cudaLaunchConfig_t cfg{};
+  FewLaunch(int units, int spread, int warps, size_t smem, cudaStream_t stream) {
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = spread;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3(units * spread);
+    cfg.blockDim = dim3(32 * warps);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+  }
+};
+
+// Clusters of `Spread` CTAs of the kernel that the current device runs at once.
+template <typename T, int D, int NB, int W, int Spread>
+int few_clusters() {
+  static PerDeviceInt cache;  // the opt-in below is per device context
+  return cache.get([] {
+    const auto kernel = step_few_kernel<T, D, NB, W>;
+    int clusters = 0;
+    FewLaunch launch(1, Spread, W, few_bytes(D, NB, W), nullptr);
+    launch.cfg.numAttrs = 1;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(few_bytes(D, NB, W))) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&clusters, kernel, &launch.cfg) != cudaSuccess)
+      clusters = 0;
+    cudaGetLastError();
+    return clusters;
+  });
+}
+
 // 8-query blocks of a unit, and units per key head
 void step_blocks(int group, int* nb, int* blocks) {
   *nb = group <= 8 ? 1 : 2;
@@ -514,13 +705,37 @@ cudaError_t launch_step(const PagedCache& c, int dtype, const Attend& a, const S
     return launch_serialized(join, dim3(shares / (kStepThreads / threads), (pairs + kStepThreads - 1) / kStepThreads),
                              dim3(kStepThreads), 0, stream, a, shared, ws, 8 * nb, blocks, threads);
   };
-  auto pick = [&](auto type) {
+  const int64_t units = static_cast<int64_t>(a.rows) * c.kv_heads * blocks;
+  // the most keys that a row can see (a run of tiles has up to 15 keys more at each end)
+  int64_t reach = static_cast<int64_t>(c.table_pages) * c.page_size;
+  if (a.window > 0) reach = std::min(reach, static_cast<int64_t>(a.window) + a.sinks + 32);
+  auto few = [&](auto kernel, int warps, int spread) {
+    const FewLaunch launch(static_cast<int>(units), spread, warps, few_bytes(c.head_dim, nb, warps), stream);
+    return cudaLaunchKernelEx(&launch.cfg, kernel, c, a, blocks, spread);
+  };
+  auto run = [&](auto type, auto dim, auto bs) {
     using T = decltype(type);
+    constexpr int D = decltype(dim)::value, NB = decltype(bs)::value;
+    auto fits = [&](int warps, int clusters) {
+      return units <= clusters && reach <= static_cast<int64_t>(kFewSteps) * warps * 16 * step_tiles(D);
+    };
+    if (shared.base == nullptr) {
+      if (reach > 32 * 16 * step_tiles(D) && fits(64, few_clusters<T, D, NB, 8, 8>()))
+        return few(step_few_kernel<T, D, NB, 8>, 8, 8);
+      if (fits(32, few_clusters<T, D, NB, 4, 8>())) return few(step_few_kernel<T, D, NB, 4>, 4, 8);
+      if (fits(16, few_clusters<T, D, NB, 4, 4>())) return few(step_few_kernel<T, D, NB, 4>, 4, 4);
+      if (fits(8, few_clusters<T, D, NB, 4, 2>())) return few(step_few_kernel<T, D, NB, 4>, 4, 2);
+      if (fits(4, few_clusters<T, D, NB, 4, 1>())) return few(step_few_kernel<T, D, NB, 4>, 4, 1);
+    }
+    return go(step_kernel<T, D, NB>, step_join_kernel<T, D>);
+  };
+  auto pick = [&](auto type) {
+    using std::integral_constant;
     if (c.head_dim == 64)
-      return nb == 1 ? go(step_kernel<T, 64, 1>, step_join_kernel<T, 64>)
-                     : go(step_kernel<T, 64, 2>, step_join_kernel<T, 64>);
-    return nb == 1 ? go(step_kernel<T, 128, 1>, step_join_kernel<T, 128>)
-                   : go(step_kernel<T, 128, 2>, step_join_kernel<T, 128>);
+      return nb == 1 ? run(type, integral_constant<int, 64>{}, integral_constant<int, 1>{})
+                     : run(type, integral_constant<int, 64>{}, integral_constant<int, 2>{});
+    return nb == 1 ? run(type, integral_constant<int, 128>{}, integral_constant<int, 1>{})
+                   : run(type, integral_constant<int, 128>{}, integral_constant<int, 2>{});
   };
   return dtype == MTT_B200_DTYPE_BF16 ? pick(__nv_bfloat16{}) : pick(__half{});
 }

@@ -258,6 +258,35 @@ def test_step_masks_and_nan_behind_them(pc, window, sinks, d, dtype):
     check_attend(pc, [50, 130, 467, 41, 300], mask=holes, window=window, sinks=sinks, d=d, dtype=dtype, group=2)
 
 
+# few slots: clusters of 64, 32, 16, 8 and 4 warps for each unit, up to and past their longest caches; many slots
+FORMS = [([480, 33, 0, 1, 511], 2, 1, 64), ([1000, 33, 0, 1, 513], 2, 1, 64), ([8000, 130, 0, 1], 1, 1, 64),
+         ([8192, 17], 1, 1, 64), ([300, 0, 1, 257], 2, 4, 128), ([3900, 33, 64, 1], 2, 4, 128), ([4097, 5], 1, 3, 128),
+         ([2100, 33, 0, 1], 1, 16, 128), ([2500, 40], 2, 13, 64), ([700, 33, 0, 1, 64, 257, 16], 12, 1, 64),
+         ([700, 33, 0, 1, 64, 257] * 4, 12, 1, 64), ([90, 33, 0, 1, 64, 257] * 8, 6, 2, 128),
+         ([90, 33, 0, 1, 64, 240] * 16, 3, 1, 128), ([90, 33, 0, 1, 64, 500] * 16, 2, 16, 64),
+         ([90, 33, 0, 1, 64, 300] * 16, 6, 1, 64), ([90, 33, 0, 1, 64, 700] * 16, 6, 1, 64)]
+
+
+@pytest.mark.parametrize("lengths,hkv,group,d", FORMS)
+@pytest.mark.parametrize("window,sinks,masked", [(0, 0, False), (40, 20, True), (0, 0, True)])
+def test_step_forms(pc, lengths, hkv, group, d, window, sinks, masked):
+    check_attend(pc, lengths, hkv=hkv, group=group, d=d, window=window, sinks=sinks, mask=holes if masked else None)
+
+
+def test_step_forms_agree(pc):
+    """Slot 0's row alone, among few slots and among many: the same up to the order of its sums, and each form's bits
+    are the same in every call."""
+    lengths = [467, 40] + [100 + i for i in range(30)]
+    cache, pool, table = make(pc, lengths, hkv=12)
+    q = queries(32, 12, 64, torch.bfloat16)
+    ref = O.attention(pool, table, lengths, 1, q, list(range(33)))
+    for rows in (1, 2, 32):
+        got = [cache.attend(1, q[:rows].cuda()) for _ in range(3)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(got[0], g) for g in got)
+        agree(got[0], None, tuple(r[:rows] for r in ref), torch.bfloat16, 467)
+
+
 PROMPTS = [([1], [1]), ([218], [218]), ([128], [128]), ([129], [1]), ([300, 0, 17, 64], [257, 0, 17, 1]),
            ([1000, 33, 513], [3, 33, 400]), ([131] * 5, [131, 130, 129, 128, 127])]
 
