@@ -321,6 +321,14 @@ def test_prompt_many_units_per_sm(pc, window, sinks, masked, d):
     assert (cache.status == 0).all()
 
 
+@pytest.mark.parametrize("slots", [383, 384, 1100])
+def test_prompt_many_slots(pc, slots):
+    """Up to as many pairs of Q tiles as the kernel has threads, and more."""
+    new = [(7 * i) % 23 for i in range(slots)]
+    cache = check_attend(pc, [n + (5 * i) % 40 for i, n in enumerate(new)], new, hkv=1)
+    assert (cache.status == 0).all()
+
+
 def test_prompt_calls_back_to_back(pc):
     """Hundreds of calls of many units each: no wait inside the kernel gives up, the result never changes."""
     new = [1, 7, 130, 2, 255, 3, 40, 129, 5, 1, 300, 64] * 2
@@ -559,6 +567,12 @@ def check_shared(pc, cache, groups, group=1, window=0, sinks=0, rows=None, seed=
 def test_shared(pc, prefixes, suffixes, group, d, dtype):
     cache, groups = voices_and_members(pc, prefixes, suffixes, d=d, dtype=dtype)
     check_shared(pc, cache, groups, group)
+
+
+def test_shared_many_groups(pc):
+    """More groups than the prefix pass's kernel has threads."""
+    cache, groups = voices_and_members(pc, [16 + 16 * (i % 3) for i in range(400)], [[1 + i % 5] for i in range(400)])
+    check_shared(pc, cache, groups)
 
 
 @pytest.mark.parametrize("hkv,group,d,ps", [(12, 1, 64, 16), (1, 13, 64, 32), (2, 64, 128, 128), (3, 3, 128, 64)])
