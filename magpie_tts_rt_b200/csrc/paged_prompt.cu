@@ -1006,82 +1006,111 @@ __device__ void member_bases(const PagedCache& c, const PromptRows& rows) {
   }
 }
 
-// Joins the parts of the units that a boundary between CTAs cut.  Block
-// (c - 1, row chunk, dim chunk): the unit at the start of CTA c's share, if
-// that is the first boundary between its key tiles; 32 of its rows, 32 dims.
+// Joins the parts of the units that a boundary between CTAs cut.  Every CTA
+// lists these units (by the CTA in whose share the first boundary between their
+// key tiles falls) and takes its share of their blocks of 32 rows and 32 dims.
+// (A CTA for each boundary and block, most without work: 65 slots over
+// 32,768 tokens 111.0 us a call instead of 106.7.)
 constexpr int kJoinParts = 8;  // parts on their way at a time
+constexpr int kJoinThreads = 256;  // more than there are boundaries
+static_assert(kJoinThreads >= kMaxSms);
 
 template <typename T, int D>
-__global__ void __launch_bounds__(256) prompt_join_kernel(PagedCache c, Attend a, PromptRows rows, PromptSpace ws) {
+__global__ void __launch_bounds__(kJoinThreads)
+    prompt_join_kernel(PagedCache c, Attend a, PromptRows rows, PromptSpace ws, int ctas) {
+  __shared__ int cut[kJoinThreads], warp_cuts[kJoinThreads / 32];
   take_turn();
-  if (rows.members != nullptr && blockIdx.y == 0 && blockIdx.z == 0) member_bases(c, rows);
-  const int cta = blockIdx.x + 1;
+  if (rows.members != nullptr) member_bases(c, rows);
   const int64_t line = ws.head[1], per = ws.head[2];
-  const int64_t x = cta * per;
-  if (x >= line * c.kv_heads) return;
-  const int head = static_cast<int>(x / line);
-  const int pair = ws.cta_pair[cta];
-  const int4 rec = ws.rec[2 * pair], at = ws.rec[2 * pair + 1];
-  const Geom g{at.x, at.y, at.z, at.w};
-  const int64_t unit_x = head * line + pair_place(rec), tile_x = unit_x + kPairCost;
-  if (x <= tile_x || x - per > tile_x) return;  // not cut here, or cut before
-  const int n = static_cast<int>((tile_x + rec.z - 1) / per) - cta + 2;  // parts, from CTA cta - 1 on
+  int cuts = 0;
+  {
+    const int cta = threadIdx.x + 1, warp = threadIdx.x >> 5;
+    const int64_t x = cta * per;
+    bool mine = false;
+    if (cta < ctas && x < line * c.kv_heads) {
+      const int4 rec = ws.rec[2 * ws.cta_pair[cta]];
+      const int64_t tile_x = x / line * line + pair_place(rec) + kPairCost;
+      mine = x > tile_x && x - per <= tile_x;
+    }
+    const uint32_t votes = __ballot_sync(0xffffffffu, mine);
+    if ((threadIdx.x & 31) == 0) warp_cuts[warp] = __popc(votes);
+    __syncthreads();
+    int before = 0;
+#pragma unroll
+    for (int k = 0; k < kJoinThreads / 32; ++k) {
+      if (k < warp) before += warp_cuts[k];
+      cuts += warp_cuts[k];
+    }
+    if (mine) cut[before + __popc(votes & ((1u << (threadIdx.x & 31)) - 1u))] = cta;
+    __syncthreads();
+  }
   const bool prefix = rows.members != nullptr;
   const int tq = kTile / a.group;
-  const int r = 32 * blockIdx.y + (threadIdx.x & 31);
-  const int i = r / kTile, rr = r % kTile;
-  const int tok = rec.x + i * tq + rr / a.group;
-  if (rr / a.group >= tq || tok >= g.count) return;
-  int q_row = g.row0 + tok;
-  if (prefix) {
-    q_row = rows.members[q_row];
-    if (q_row < 0 || q_row >= a.rows) return;
-  }
-  const int q_head = head * a.group + rr % a.group;
-  constexpr int E = 4;  // dims per thread
-  const int d0 = 32 * blockIdx.z + E * (threadIdx.x >> 5);
-  const int64_t stride = static_cast<int64_t>(D + 2) * kPairRows;
-  const float* parts = ws.part + 2 * (cta - 1) * stride + r;
-  const int64_t first = ((cta - 1) * per >= unit_x ? 0 : 1) * stride;
-  float top = -CUDART_INF_F, l = 0.f, o[E] = {0.f, 0.f, 0.f, 0.f};
-  for (int k0 = 0; k0 < n; k0 += kJoinParts) {
-    float m[kJoinParts], s[kJoinParts], y[kJoinParts][E];
-#pragma unroll
-    for (int k = 0; k < kJoinParts; ++k) {
-      const bool on = k0 + k < n;
-      const float* p = parts + (k0 + k == 0 ? first : 2 * (k0 + k) * stride);
-      m[k] = on ? __ldcg(p + D * kPairRows) : -CUDART_INF_F;
-      s[k] = on ? __ldcg(p + (D + 1) * kPairRows) : 0.f;
-#pragma unroll
-      for (int e = 0; e < E; ++e) y[k][e] = on ? __ldcg(p + (d0 + e) * kPairRows) : 0.f;
+  constexpr int kBlocks = (kPairRows / 32) * (D / 32);
+  for (int item = blockIdx.x; item < cuts * kBlocks; item += gridDim.x) {
+    const int cta = cut[item / kBlocks];
+    const int64_t x = cta * per;
+    const int head = static_cast<int>(x / line);
+    const int pair = ws.cta_pair[cta];
+    const int4 rec = ws.rec[2 * pair], at = ws.rec[2 * pair + 1];
+    const Geom g{at.x, at.y, at.z, at.w};
+    const int64_t unit_x = head * line + pair_place(rec), tile_x = unit_x + kPairCost;
+    const int n = static_cast<int>((tile_x + rec.z - 1) / per) - cta + 2;  // parts, from CTA cta - 1 on
+    const int r = 32 * (item % kBlocks / (D / 32)) + (threadIdx.x & 31);
+    const int i = r / kTile, rr = r % kTile;
+    const int tok = rec.x + i * tq + rr / a.group;
+    if (rr / a.group >= tq || tok >= g.count) continue;
+    int q_row = g.row0 + tok;
+    if (prefix) {
+      q_row = rows.members[q_row];
+      if (q_row < 0 || q_row >= a.rows) continue;
     }
-    float most = top;
-#pragma unroll
-    for (int k = 0; k < kJoinParts; ++k) most = fmaxf(most, m[k]);
-    const float z = most == -CUDART_INF_F ? 0.f : most;
-    const float keep = ex2(top - z);
-    top = most;
-    l *= keep;
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] *= keep;
-#pragma unroll
-    for (int k = 0; k < kJoinParts; ++k) {
-      const float f = ex2(m[k] - z);
-      l = fmaf(f, s[k], l);
-#pragma unroll
-      for (int e = 0; e < E; ++e) o[e] = fmaf(f, y[k][e], o[e]);
+    const int q_head = head * a.group + rr % a.group;
+    constexpr int E = 4;  // dims per thread
+    const int d0 = 32 * (item % (D / 32)) + E * (threadIdx.x >> 5);
+    const int64_t stride = static_cast<int64_t>(D + 2) * kPairRows;
+    const float* parts = ws.part + 2 * (cta - 1) * stride + r;
+    const int64_t first = ((cta - 1) * per >= unit_x ? 0 : 1) * stride;
+    float top = -CUDART_INF_F, l = 0.f, o[E] = {0.f, 0.f, 0.f, 0.f};
+    for (int k0 = 0; k0 < n; k0 += kJoinParts) {
+      float m[kJoinParts], s[kJoinParts], y[kJoinParts][E];
+  #pragma unroll
+      for (int k = 0; k < kJoinParts; ++k) {
+        const bool on = k0 + k < n;
+        const float* p = parts + (k0 + k == 0 ? first : 2 * (k0 + k) * stride);
+        m[k] = on ? __ldcg(p + D * kPairRows) : -CUDART_INF_F;
+        s[k] = on ? __ldcg(p + (D + 1) * kPairRows) : 0.f;
+  #pragma unroll
+        for (int e = 0; e < E; ++e) y[k][e] = on ? __ldcg(p + (d0 + e) * kPairRows) : 0.f;
+      }
+      float most = top;
+  #pragma unroll
+      for (int k = 0; k < kJoinParts; ++k) most = fmaxf(most, m[k]);
+      const float z = most == -CUDART_INF_F ? 0.f : most;
+      const float keep = ex2(top - z);
+      top = most;
+      l *= keep;
+  #pragma unroll
+      for (int e = 0; e < E; ++e) o[e] *= keep;
+  #pragma unroll
+      for (int k = 0; k < kJoinParts; ++k) {
+        const float f = ex2(m[k] - z);
+        l = fmaf(f, s[k], l);
+  #pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = fmaf(f, y[k][e], o[e]);
+      }
     }
+    if (prefix) {
+      float* state = rows.state + (static_cast<int64_t>(q_row) * a.q_heads + q_head) * (D + 4);
+      *reinterpret_cast<float4*>(state + d0) = make_float4(o[0], o[1], o[2], o[3]);
+      if (d0 == 0) *reinterpret_cast<float2*>(state + D) = make_float2(top, l);
+      continue;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    *reinterpret_cast<uint2*>(a.out + q_row * a.out_row + static_cast<int64_t>(q_head) * D + d0) =
+        make_uint2(Half16<T>::pack(o[0] * inv, o[1] * inv), Half16<T>::pack(o[2] * inv, o[3] * inv));
+    if (d0 == 0 && a.lse != nullptr) a.lse[static_cast<int64_t>(q_row) * a.q_heads + q_head] = (top + log2f(l)) * kLn2;
   }
-  if (prefix) {
-    float* state = rows.state + (static_cast<int64_t>(q_row) * a.q_heads + q_head) * (D + 4);
-    *reinterpret_cast<float4*>(state + d0) = make_float4(o[0], o[1], o[2], o[3]);
-    if (d0 == 0) *reinterpret_cast<float2*>(state + D) = make_float2(top, l);
-    return;
-  }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  *reinterpret_cast<uint2*>(a.out + q_row * a.out_row + static_cast<int64_t>(q_head) * D + d0) =
-      make_uint2(Half16<T>::pack(o[0] * inv, o[1] * inv), Half16<T>::pack(o[2] * inv, o[3] * inv));
-  if (d0 == 0 && a.lse != nullptr) a.lse[static_cast<int64_t>(q_row) * a.q_heads + q_head] = (top + log2f(l)) * kLn2;
 }
 
 // Bytes of the parts of a prompt call's workspace.
@@ -1183,7 +1212,7 @@ cudaError_t run_prompt(const PagedCache& c, int dtype, const Attend& a, PromptRo
                             a.sinks, tokens_per_pair, sms);
     if (e == cudaSuccess) e = launch_serialized(kernel, dim3(sms), dim3(kPromptThreads), smem, stream, map, q_map, c, a, rows, ws);
     if (e == cudaSuccess)
-      e = launch_serialized(prompt_join_kernel<T, D>, dim3(sms - 1, kPairRows / 32, c.head_dim / 32), dim3(256), 0, stream, c, a, rows, ws);
+      e = launch_serialized(prompt_join_kernel<T, D>, dim3(4 * sms), dim3(kJoinThreads), 0, stream, c, a, rows, ws, sms);
     return e;
   };
   auto pick = [&](auto type) {
