@@ -28,9 +28,10 @@
 // reach, 162 us (6.7 TB/s of the keys and values in reach; 974 MB from DRAM); 8
 // slots of 30,001 to 65,536 keys, 32/8 heads of 128, 238 us (6.3 TB/s).
 // Clusters: 2 slots of 467 keys, 12 heads of 64, 5.3 us (9.0 us as a line).  What
-// bounds the line is DRAM; where sequences are short (1 to 249 keys) a unit's chain of dependent loads (63 us
-// for 275 MB).  Tried: shares per CTA with the four warps of a CTA side by side
-// in a unit (187 and 247 us, 389 us for the short ones).
+// bounds the line is DRAM; where sequences are short (1 to 249 keys) a unit's chain
+// of dependent loads (63 us for 275 MB).  Tried: shares per CTA with the four warps of a CTA side by side
+// in a unit (187 and 247 us, 389 us for the short ones); a unit's further tiles
+// prefetched into L2 when it is entered (249 -> 253 us, the short ones 10 us more).
 #include <algorithm>
 #include <type_traits>
 
