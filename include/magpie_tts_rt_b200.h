@@ -833,8 +833,9 @@ MTT_B200_API int mtt_b200_launch_paged_cache_store(const mtt_b200_paged_cache_t*
  * offsets[i + 1] - offsets[i] tokens, whose keys and values are already
  * stored; a slot with more rows than tokens gets out 0 and lse -inf, offsets
  * that are not ascending within [0, rows] leave their rows untouched.
- * status[i] becomes 4 when a bounded wait inside the prompt kernel gave up
- * (outputs unreliable). */
+ * status[i] becomes 4 when a bounded wait inside the prompt kernel gave up (the
+ * bounds grow with the keys that the call has to read): the outputs of slot i's
+ * rows are then not to be used. */
 typedef struct mtt_b200_cache_attention {
   int32_t layer;
   int32_t q_heads;          /* a multiple of kv_heads, q_heads / kv_heads <= 64 */
@@ -881,7 +882,9 @@ MTT_B200_API size_t mtt_b200_paged_shared_workspace_size(const mtt_b200_paged_ca
  * all its members.  The result is the same attention; a member is attended on
  * its own when its slot or the voice's holds fewer than tokens[g] tokens, when
  * its last prefix page is not the voice's, or when a window leaves some of the
- * prefix out of sight (sinks < tokens[g]). */
+ * prefix out of sight (sinks < tokens[g]).  When a bounded wait
+ * inside the prefix pass gave up, all members are attended on their own and their
+ * status becomes 4; the result is right all the same. */
 MTT_B200_API int mtt_b200_launch_paged_attention_shared(const mtt_b200_paged_cache_t* cache,
                                                         const mtt_b200_cache_attention_t* args,
                                                         const mtt_b200_prefix_groups_t* groups, void* workspace,
@@ -897,6 +900,14 @@ MTT_B200_API int mtt_b200_launch_test_clamped_gumbel(const float* uniform, float
                                                      void* stream);
 /* out[i] = the device's correctly rounded natural log of x[i]. */
 MTT_B200_API int mtt_b200_launch_test_log(const float* x, float* out, size_t count, void* stream);
+
+/* Section 7's attention calls (groups NULL: mtt_b200_launch_paged_attention) with
+ * wait_ns in place of the part of the prompt kernel's bounds that does not grow
+ * with the keys; starve != 0: the kernel gets no keys and gives up. */
+MTT_B200_API int mtt_b200_launch_test_paged_attention(const mtt_b200_paged_cache_t* cache,
+                                                      const mtt_b200_cache_attention_t* args,
+                                                      const mtt_b200_prefix_groups_t* groups, uint32_t wait_ns,
+                                                      int32_t starve, void* workspace, size_t workspace_bytes, void* stream);
 
 /* The projection GEMM of the Main Decoder step on its own (for numerics tests
  * and timing): Y[rows][n] = bf16(X[rows][k] W[n][k]^T) with f32 accumulation

@@ -243,6 +243,8 @@ SIGNATURES = {
         I32, [ctypes.POINTER(PagedCache), ctypes.POINTER(CacheAttention), ctypes.POINTER(PrefixGroups), P, SZ, P]),
     "mtt_b200_launch_test_clamped_gumbel": (I32, [P, P, SZ, P]),
     "mtt_b200_launch_test_log": (I32, [P, P, SZ, P]),
+    "mtt_b200_launch_test_paged_attention": (
+        I32, [ctypes.POINTER(PagedCache), ctypes.POINTER(CacheAttention), ctypes.POINTER(PrefixGroups), ctypes.c_uint32, I32, P, SZ, P]),
     "mtt_b200_launch_test_gemm": (I32, [P, P, P, I32, I32, I32, I32, I32, P, P]),
     "mtt_b200_test_umma_cycles": (I32, [I32, I32, I32, I32, P, P]),
     "mtt_b200_test_dsmem_cycles": (I32, [I32, I32, I32, P, P]),

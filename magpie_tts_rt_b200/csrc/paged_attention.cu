@@ -52,12 +52,8 @@ size_t state_bytes(const mtt_b200_paged_cache_t& c, int q_heads) {
   return (static_cast<size_t>(c.slots) * q_heads * (c.head_dim + 4) * 4 + 255) / 256 * 256;
 }
 
-}  // namespace
-
-extern "C" {
-
-int mtt_b200_launch_paged_attention(const mtt_b200_paged_cache_t* cache, const mtt_b200_cache_attention_t* args,
-                                    void* workspace, size_t workspace_bytes, void* stream) {
+int attend(const mtt_b200_paged_cache_t* cache, const mtt_b200_cache_attention_t* args, void* workspace,
+           size_t workspace_bytes, const Waits& waits, void* stream) {
   PagedCache c;
   Attend a;
   if (!paged_cache_view(cache, &c) || !attend_args(c, args, &a)) return MTT_B200_STATUS_INVALID_ARGUMENT;
@@ -67,17 +63,12 @@ int mtt_b200_launch_paged_attention(const mtt_b200_paged_cache_t* cache, const m
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (a.offsets == nullptr) return cache_call_status(launch_step(c, cache->dtype, a, SharedPrefix{}, space, s));
   return cache_call_status(
-      launch_prompt(c, cache->dtype, a, static_cast<char*>(space) + step_workspace(*cache, a.q_heads), s));
+      launch_prompt(c, cache->dtype, a, static_cast<char*>(space) + step_workspace(*cache, a.q_heads), waits, s));
 }
 
-size_t mtt_b200_paged_shared_workspace_size(const mtt_b200_paged_cache_t* cache, int32_t q_heads, int32_t n_members) {
-  const size_t plain = mtt_b200_paged_cache_workspace_size(cache, q_heads, n_members);
-  return plain == 0 ? 0 : (plain + 255) / 256 * 256 + base_bytes(*cache) + state_bytes(*cache, q_heads);
-}
-
-int mtt_b200_launch_paged_attention_shared(const mtt_b200_paged_cache_t* cache, const mtt_b200_cache_attention_t* args,
-                                           const mtt_b200_prefix_groups_t* groups, void* workspace,
-                                           size_t workspace_bytes, void* stream) {
+int attend_shared(const mtt_b200_paged_cache_t* cache, const mtt_b200_cache_attention_t* args,
+                  const mtt_b200_prefix_groups_t* groups, void* workspace, size_t workspace_bytes,
+                  const Waits& waits, void* stream) {
   PagedCache c;
   Attend a;
   if (!paged_cache_view(cache, &c) || !attend_args(c, args, &a) || a.offsets != nullptr || a.key_mask != nullptr ||
@@ -100,12 +91,40 @@ int mtt_b200_launch_paged_attention_shared(const mtt_b200_paged_cache_t* cache, 
     int32_t* base = reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + plain);
     float* state = reinterpret_cast<float*>(static_cast<char*>(workspace) + plain + base_bytes(*cache));
     const cudaError_t e = launch_prefix(c, cache->dtype, a, *groups, base, state,
-                                        static_cast<char*>(space) + step_workspace(*cache, a.q_heads), s);
+                                        static_cast<char*>(space) + step_workspace(*cache, a.q_heads), waits, s);
     if (e != cudaSuccess) return cache_call_status(e);
     shared.base = base;
     shared.state = state;
   }
   return cache_call_status(launch_step(c, cache->dtype, a, shared, space, s));
+}
+
+}  // namespace
+
+extern "C" {
+
+int mtt_b200_launch_paged_attention(const mtt_b200_paged_cache_t* cache, const mtt_b200_cache_attention_t* args,
+                                    void* workspace, size_t workspace_bytes, void* stream) {
+  return attend(cache, args, workspace, workspace_bytes, Waits{}, stream);
+}
+
+size_t mtt_b200_paged_shared_workspace_size(const mtt_b200_paged_cache_t* cache, int32_t q_heads, int32_t n_members) {
+  const size_t plain = mtt_b200_paged_cache_workspace_size(cache, q_heads, n_members);
+  return plain == 0 ? 0 : (plain + 255) / 256 * 256 + base_bytes(*cache) + state_bytes(*cache, q_heads);
+}
+
+int mtt_b200_launch_paged_attention_shared(const mtt_b200_paged_cache_t* cache, const mtt_b200_cache_attention_t* args,
+                                           const mtt_b200_prefix_groups_t* groups, void* workspace,
+                                           size_t workspace_bytes, void* stream) {
+  return attend_shared(cache, args, groups, workspace, workspace_bytes, Waits{}, stream);
+}
+
+int mtt_b200_launch_test_paged_attention(const mtt_b200_paged_cache_t* cache, const mtt_b200_cache_attention_t* args,
+                                         const mtt_b200_prefix_groups_t* groups, uint32_t wait_ns, int32_t starve,
+                                         void* workspace, size_t workspace_bytes, void* stream) {
+  const Waits waits{wait_ns, Waits{}.tile_ns, starve != 0};
+  return groups == nullptr ? attend(cache, args, workspace, workspace_bytes, waits, stream)
+                           : attend_shared(cache, args, groups, workspace, workspace_bytes, waits, stream);
 }
 
 }  // extern "C"

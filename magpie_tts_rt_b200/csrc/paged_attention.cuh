@@ -99,12 +99,20 @@ size_t step_workspace(const mtt_b200_paged_cache_t& c, int q_heads);
 cudaError_t launch_step(const PagedCache& c, int dtype, const Attend& a, const SharedPrefix& shared, void* space,
                         cudaStream_t stream);
 
+// How long the prompt kernel's waits may last: ns, and tile_ns for each key tile
+// of a CTA's share (which takes it some 2 us).
+struct Waits {
+  uint32_t ns = 200000000, tile_ns = 50000;
+  bool starve = false;  // tests: no key tile ever arrives
+};
+
 // Workspace of the prompt attention for calls of up to `rows` query rows.
 size_t prompt_workspace(const mtt_b200_paged_cache_t& c, int q_heads, int rows);
-cudaError_t launch_prompt(const PagedCache& c, int dtype, const Attend& a, void* space, cudaStream_t stream);
+cudaError_t launch_prompt(const PagedCache& c, int dtype, const Attend& a, void* space, const Waits& waits,
+                          cudaStream_t stream);
 
 // The prefix pass of the shared-prefix attention: fills base and state.
 cudaError_t launch_prefix(const PagedCache& c, int dtype, const Attend& a, const mtt_b200_prefix_groups_t& groups,
-                          int32_t* base, float* state, void* space, cudaStream_t stream);
+                          int32_t* base, float* state, void* space, const Waits& waits, cudaStream_t stream);
 
 }  // namespace mtt

@@ -34,8 +34,15 @@
 //
 // The units' key tiles form one line that is cut into equal parts, one per
 // CTA; a unit cut by a boundary leaves (m, l, O) in the workspace for a
-// second kernel that joins the parts in order.  Every wait is bounded; one
-// that gives up marks the slot's status 4.
+// second kernel that joins the parts in order.
+//
+// Every wait is bounded.  Some last as long as a unit's part in a share (the
+// next unit's queries wait for this one's last scores, a Q tile without rows
+// for the next unit), so the bound grows with the key tiles of the CTA's share:
+// 50 us for each, some twenty times what it takes, and 0.2 s beside.  A CTA in
+// which a wait gives up says so in the workspace and leaves; the join marks the
+// slots of its share with status 4 (and lets the members of a prefix pass be
+// attended on their own).
 //
 // Measured: 8192 tokens, 32/8 heads of 128, causal, 484 us alone and 555 us back
 // to back, where the board's power holds the clock near 1.4 GHz (1.14 and 0.99
@@ -99,8 +106,10 @@ struct PromptSpace {
   int64_t* head;       // [0] pairs, [1] length of one key head's line, [2] length of a share
   int32_t* cta_pair;   // [kMaxSms + 1] the pair that holds the start of CTA c's share
   int32_t* first;      // [n + 1] pairs of the slots before
+  int32_t* gave_up;    // [kMaxSms] whether a wait of CTA c ran out
   int4* rec;           // [2 * pairs]: first token (or member), place (high), key tiles, place (low); then Geom
   float* part;         // [CTAs][2][D + 2][256]
+  Waits waits;
 };
 
 // A pair's place on its key head's line.
@@ -447,10 +456,25 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, i
       : "memory");
 }
 
-// Warp-uniform forms: a wait succeeds, and the CTA goes on, for all lanes or none.
-__device__ __forceinline__ bool wait_warp(unsigned long long* bar, uint32_t parity) {
-  return __all_sync(0xffffffffu, mbar_wait_cta(bar, parity));
-}
+// A wait of up to *limit ns, for all lanes of the warp or none.
+struct Patience {
+  const volatile unsigned long long* limit;  // in shared memory: looked at only by a wait that has to
+  __device__ __forceinline__ bool wait(unsigned long long* bar, uint32_t parity) const {
+    const uint32_t at = smem_addr(bar);
+    bool ok = mbar_try_cta(at, parity);
+    if (!ok) {
+      const unsigned long long end = global_ns() + *limit;
+      do ok = mbar_try_cta(at, parity);
+      while (!ok && global_ns() <= end);
+    }
+    return __all_sync(0xffffffffu, ok);
+  }
+};
+
+// For what is certain to come, before the CTA leaves: its own copies in flight, its MMAs.
+constexpr unsigned long long kDrainNs = 1000000000ull;
+__device__ __forceinline__ void drain(unsigned long long* bar, uint32_t parity) { mbar_wait_cta(bar, parity, kDrainNs); }
+
 __device__ __forceinline__ bool alive(const volatile int* err) { return __all_sync(0xffffffffu, *err == 0); }
 
 // bits [lo, hi) of a 32-bit word
@@ -481,7 +505,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   __shared__ unsigned long long kv_full[S], kv_empty[S], ready[S], q_ready[2], s_full[2], p_full[2][2], half_done[2],
       o_full[2], q_free[2], fin;
   __shared__ uint32_t tmem_base;
-  __shared__ int err, unit_slot;  // unit_slot: whose unit the softmax warps are at
+  __shared__ unsigned long long wait_limit;
+  __shared__ int err;
   const uint32_t pad = (1024u - (smem_addr(prompt_smem) & 1023u)) & 1023u;
   unsigned char* q_smem = prompt_smem + pad;
   unsigned char* ring = q_smem + 2 * C::kQBytes;
@@ -507,7 +532,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     }
     mbar_init(&fin, 1);
     err = 0;
-    unit_slot = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 8) {
@@ -531,13 +555,16 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 
   Walk w;
   const bool any = w.begin(ws, c.kv_heads, blockIdx.x);
+  const Patience patience{&wait_limit};
+  if (threadIdx.x == 0) wait_limit = ws.waits.ns + static_cast<unsigned long long>(ws.waits.tile_ns) * (any ? w.end : 0);
+  __syncthreads();
 
   if (warp == 9) {
     // ---- TMA producer.  Order: keys 0, then values t, keys t + 1, as they are used.
     int it = 0;
     const int rows_per_box = min(kKeys, c.page_size), boxes = kKeys / rows_per_box;
     const int beyond = c.pages * c.layers * 2 * c.kv_heads * c.page_size;  // a row past the pool: reads zeros
-    for (bool more = any; more && alive(errv); more = w.next(ws)) {
+    for (bool more = any && !ws.waits.starve; more && alive(errv); more = w.next(ws)) {
       const Geom g = w.g;
       const KeySpan span = unit_span(w, prefix, tq, a);
       const int32_t* table = c.table + static_cast<int64_t>(g.key_slot) * c.table_pages;
@@ -548,7 +575,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       };
       auto copy = [&](int t, int page, int kv) {
         const int s = it % S;
-        if (it >= S && !wait_warp(&kv_empty[s], ((it / S) - 1) & 1)) return false;
+        if (it >= S && !patience.wait(&kv_empty[s], ((it / S) - 1) & 1)) return false;
         ++it;
         if (lane == 0) mbar_expect_tx(&kv_full[s], C::kTileBytes);
         __syncwarp();
@@ -575,7 +602,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     }
     // no copy may still be landing in shared memory when the CTA leaves
     if (lane == 0)
-      for (int k = max(0, it - S); k < it; ++k) mbar_wait_cta(&kv_full[k % S], (k / S) & 1);
+      for (int k = max(0, it - S); k < it; ++k) drain(&kv_full[k % S], (k / S) & 1);
   } else if (warp == 10) {
     // ---- value rows that no query may see are cleared before the MMA warp may use the tile.  Key tiles pass
     // through too: so neither this warp nor the MMA warp is ever a round of the ring away from the other.
@@ -586,7 +613,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       const bool* mask = a.key_mask != nullptr ? a.key_mask + g.key_slot * a.mask_stride : nullptr;
       auto pass = [&](int t) {  // the ring's next tile: values of tile t, or keys (t < 0)
         const int s = it % S;
-        if (!wait_warp(&kv_full[s], (it / S) & 1)) return false;
+        if (!patience.wait(&kv_full[s], (it / S) & 1)) return false;
         ++it;
         const int base = t < 0 ? 0 : kKeys * span.tile(t);
         if (t >= 0 && (mask != nullptr || (base + kKeys > g.len && (g.len & (c.page_size - 1)) != 0))) {
@@ -616,11 +643,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     }
   } else if (warp == 11) {
     // ---- queries: a box of 64 dims x the group's heads x the tile's tokens, whose rows are the tile's
-    int unit = 0;
-    for (bool more = any && rows.q_mapped; more && alive(errv); more = w.next(ws), ++unit) {
+    int units[2] = {0, 0};  // whose queries have been asked for
+    for (bool more = any && rows.q_mapped; more && alive(errv); more = w.next(ws)) {
       bool ok = true;
-      for (int i = 0; ok && i < 2; ++i) {
-        if (unit > 0) ok = wait_warp(&q_free[i], (unit - 1) & 1);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (units[i] > 0) ok = ok && patience.wait(&q_free[i], (units[i] - 1) & 1);
+        if (ok) ++units[i];
         if (ok && lane == 0) {
           mbar_expect_tx(&q_ready[i], static_cast<uint32_t>(tq * a.group * D * 2));
 #pragma unroll
@@ -633,8 +662,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       if (!ok) *errv = 1;
     }
     // no copy may still be landing in shared memory when the CTA leaves
-    if (lane == 0 && unit > 0)
-      for (int i = 0; i < 2; ++i) mbar_wait_cta(&q_ready[i], (unit - 1) & 1);
+    if (lane == 0) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (units[i] > 0) drain(&q_ready[i], (units[i] - 1) & 1);
+    }
   } else if (warp == 8) {
     // ---- MMA issuer.  The whole warp walks along, so that what the
     // instructions are given stays in uniform registers (from a single thread's
@@ -675,14 +707,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       int last[2];  // each Q tile's last key tile in this share
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        last[i] = t1 - 1;
+        last[i] = seen[i].high < 0 ? t0 - 1 : t1 - 1;
         while (last[i] >= t0 && !seen[i].at(span.tile(last[i]))) --last[i];
       }
       more = w.next(ws);  // its loads are on their way while this unit runs
-      bool ok = wait_warp(&ready[it % S], (it / S) & 1);
+      bool ok = patience.wait(&ready[it % S], (it / S) & 1);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        ok = ok && wait_warp(&q_ready[i], q_uses & 1);
+        ok = ok && patience.wait(&q_ready[i], q_uses & 1);
         if (ok) {
           tmem_fence_after_sync();
           if (seen[i].at(span.tile(t0))) scores(i, it % S);
@@ -695,15 +727,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       for (int t = t0; ok && t < t1; ++t) {
         const int vs = it % S, ks = (it + 1) % S;
         const bool next = t + 1 < t1;
-        ok = wait_warp(&ready[vs], (it / S) & 1);
-        if (next) ok = ok && wait_warp(&ready[ks], ((it + 1) / S) & 1);
+        ok = patience.wait(&ready[vs], (it / S) & 1);
+        if (next) ok = ok && patience.wait(&ready[ks], ((it + 1) / S) & 1);
         const int j = span.tile(t), j1 = next ? span.tile(t + 1) : 0;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           if (seen[i].at(j)) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              ok = ok && wait_warp(&p_full[i][h], p_uses[i] & 1);
+              ok = ok && patience.wait(&p_full[i][h], p_uses[i] & 1);
               if (ok) {
                 tmem_fence_after_sync();
                 const uint32_t vd = v_lo + vs * kTileStep + h * (kHalf * 128 >> 4);
@@ -736,7 +768,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     }
     // every MMA this warp issued has completed before tensor memory is freed
     commit(&fin);
-    wait_warp(&fin, 0);
+    drain(&fin, 0);
   } else {
     // ---- softmax of Q tile i: thread r is its row r
     const int i = warp >> 2, r = threadIdx.x & 127;
@@ -791,7 +823,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       const int len = w.g.len, t0 = w.t0, t1 = w.t1, q_head = w.head * a.group + head_in_group;
       const int pos = prefix ? len - 1 : len - w.g.count + w.tok0 + i * tq + tok_in_tile;
       const bool* mask = a.key_mask != nullptr ? a.key_mask + w.g.key_slot * a.mask_stride : nullptr;
-      if (threadIdx.x == 0) unit_slot = w.g.key_slot;
       const bool whole = w.whole();
       const int part_at = 2 * static_cast<int>(blockIdx.x) + w.part();
       more = w.next(ws);  // from here on w is the next unit: its loads are on their way while this one runs
@@ -811,7 +842,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 #pragma unroll
           for (int x = 0; x < 4; ++x) kept[x] = __ballot_sync(0xffffffffu, on[x]);
         }
-        ok = wait_warp(&s_full[i], s_uses & 1);
+        ok = patience.wait(&s_full[i], s_uses & 1);
         if (!ok) break;
         tmem_fence_after_sync();
         // One half after the other, so that 64 scores are held and not 128: P of
@@ -865,7 +896,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
               for (int k = 0; k < kHalf; k += 2) top = max_nan(top, __uint_as_float(s[k]), __uint_as_float(s[k + 1]));
               if (started || h == 1) {
                 // the products so far must be in O: those of the tiles before are (these scores came after them)
-                if (h == 1) ok = wait_warp(&half_done[i], s_uses & 1);
+                if (h == 1) ok = patience.wait(&half_done[i], s_uses & 1);
                 if (!ok) break;
                 tmem_fence_after_sync();
                 const float f = m == -CUDART_INF_F ? 1.f : ex2((m - top) * a.scale2);
@@ -897,10 +928,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         started = true;
       }
       if (ok && more && !rows.q_mapped) {  // before this unit's result comes out
-        ok = wait_warp(&q_free[i], unit & 1);
+        ok = patience.wait(&q_free[i], unit & 1);
         if (ok) load_q(w, next_row);
       }
-      if (ok && started) ok = wait_warp(&o_full[i], o_uses++ & 1);
+      if (ok && started) ok = patience.wait(&o_full[i], o_uses++ & 1);
       if (!ok) {
         *errv = 1;
         break;
@@ -978,6 +1009,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       tmem_fence_before_sync();
       q_row = next_row;
     }
+    tmem_wait_st();  // also where a wait ran out between a store and its use
   }
   tmem_fence_before_sync();
   __syncthreads();
@@ -985,7 +1017,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     tmem_fence_after_sync();
     tmem_dealloc(tmem, 512);
   }
-  if (threadIdx.x == 0 && *errv != 0 && c.status != nullptr) c.status[unit_slot] = 4;
+  if (threadIdx.x == 0) ws.gave_up[blockIdx.x] = *errv;
 }
 
 // Prefix pass: how many of each member's tokens it has attended to (base is 0 so far).
@@ -1006,6 +1038,20 @@ __device__ void member_bases(const PagedCache& c, const PromptRows& rows) {
   }
 }
 
+// Status 4: of a prompt's slots, those with units in the shares of the CTAs that
+// gave up (thread c's says whether CTA c did); of a prefix pass, all members.
+__device__ void mark_lost(const PagedCache& c, const PromptRows& rows, const PromptSpace& ws, bool gave_up) {
+  if (rows.members != nullptr) {
+    for (int k = blockIdx.x * blockDim.x + threadIdx.x; k < rows.n_rows; k += gridDim.x * blockDim.x) {
+      const int slot = rows.members[k];
+      if (slot >= 0 && slot < c.slots) c.status[slot] = 4;
+    }
+  } else if (gave_up && blockIdx.x == 0) {
+    Walk w;
+    for (bool more = w.begin(ws, c.kv_heads, threadIdx.x); more; more = w.next(ws)) c.status[w.g.key_slot] = 4;
+  }
+}
+
 // Joins the parts of the units that a boundary between CTAs cut.  Every CTA
 // lists these units (by the CTA in whose share the first boundary between their
 // key tiles falls) and takes its share of their blocks of 32 rows and 32 dims.
@@ -1020,7 +1066,8 @@ __global__ void __launch_bounds__(kJoinThreads)
     prompt_join_kernel(PagedCache c, Attend a, PromptRows rows, PromptSpace ws, int ctas) {
   __shared__ int cut[kJoinThreads], warp_cuts[kJoinThreads / 32];
   take_turn();
-  if (rows.members != nullptr) member_bases(c, rows);
+  const bool prefix = rows.members != nullptr;
+  const bool mine_gave_up = threadIdx.x < ctas && ws.gave_up[threadIdx.x] != 0;
   const int64_t line = ws.head[1], per = ws.head[2];
   int cuts = 0;
   {
@@ -1034,7 +1081,9 @@ __global__ void __launch_bounds__(kJoinThreads)
     }
     const uint32_t votes = __ballot_sync(0xffffffffu, mine);
     if ((threadIdx.x & 31) == 0) warp_cuts[warp] = __popc(votes);
-    __syncthreads();
+    const bool gave_up = __syncthreads_or(mine_gave_up);
+    if (prefix && !gave_up) member_bases(c, rows);
+    if (gave_up && c.status != nullptr) mark_lost(c, rows, ws, mine_gave_up);
     int before = 0;
 #pragma unroll
     for (int k = 0; k < kJoinThreads / 32; ++k) {
@@ -1044,7 +1093,6 @@ __global__ void __launch_bounds__(kJoinThreads)
     if (mine) cut[before + __popc(votes & ((1u << (threadIdx.x & 31)) - 1u))] = cta;
     __syncthreads();
   }
-  const bool prefix = rows.members != nullptr;
   const int tq = kTile / a.group;
   constexpr int kBlocks = (kPairRows / 32) * (D / 32);
   for (int item = blockIdx.x; item < cuts * kBlocks; item += gridDim.x) {
@@ -1115,12 +1163,13 @@ __global__ void __launch_bounds__(kJoinThreads)
 
 // Bytes of the parts of a prompt call's workspace.
 struct PromptLayout {
-  size_t cta_pair, first, rec, part, bytes;
+  size_t cta_pair, gave_up, first, rec, part, bytes;
   PromptLayout(int n, int rows, int group, int head_dim) {
     const auto up = [](size_t v) { return (v + 255) / 256 * 256; };
     const size_t pairs = static_cast<size_t>(rows) / (2 * (kTile / group)) + n + 1;
     cta_pair = 256;
-    first = cta_pair + up(4 * (kMaxSms + 1));
+    gave_up = cta_pair + up(4 * (kMaxSms + 1));
+    first = gave_up + up(4 * kMaxSms);
     rec = first + up(4 * (static_cast<size_t>(n) + 1));
     part = rec + up(32 * pairs);
     bytes = part + up(static_cast<size_t>(kMaxSms) * 2 * (head_dim + 2) * kPairRows * 4);
@@ -1179,7 +1228,7 @@ bool query_map(const PagedCache& c, int dtype, const Attend& a, CUtensorMap* map
 }
 
 cudaError_t run_prompt(const PagedCache& c, int dtype, const Attend& a, PromptRows rows, void* space,
-                       cudaStream_t stream) {
+                       const Waits& waits, cudaStream_t stream) {
   const int sms = cache_sm_count();
   CUtensorMap map, q_map;
   if (sms <= 0 || sms > kMaxSms || !pool_map(c, dtype, &map)) return cudaErrorInvalidValue;
@@ -1192,9 +1241,11 @@ cudaError_t run_prompt(const PagedCache& c, int dtype, const Attend& a, PromptRo
   PromptSpace ws;
   ws.head = reinterpret_cast<int64_t*>(base);
   ws.cta_pair = reinterpret_cast<int32_t*>(base + at.cta_pair);
+  ws.gave_up = reinterpret_cast<int32_t*>(base + at.gave_up);
   ws.first = reinterpret_cast<int32_t*>(base + at.first);
   ws.rec = reinterpret_cast<int4*>(base + at.rec);
   ws.part = reinterpret_cast<float*>(base + at.part);
+  ws.waits = waits;
   auto go = [&](auto type, auto dim) {
     using T = decltype(type);
     constexpr int D = decltype(dim)::value;
@@ -1227,16 +1278,17 @@ size_t prompt_workspace(const mtt_b200_paged_cache_t& c, int q_heads, int rows) 
   return PromptLayout(c.slots, rows, q_heads / c.kv_heads, c.head_dim).bytes;
 }
 
-cudaError_t launch_prompt(const PagedCache& c, int dtype, const Attend& a, void* space, cudaStream_t stream) {
+cudaError_t launch_prompt(const PagedCache& c, int dtype, const Attend& a, void* space, const Waits& waits,
+                          cudaStream_t stream) {
   PromptRows rows{};
   rows.n = c.slots;
   rows.n_rows = a.rows;
   rows.offsets = a.offsets;
-  return run_prompt(c, dtype, a, rows, space, stream);
+  return run_prompt(c, dtype, a, rows, space, waits, stream);
 }
 
 cudaError_t launch_prefix(const PagedCache& c, int dtype, const Attend& a, const mtt_b200_prefix_groups_t& groups,
-                          int32_t* base, float* state, void* space, cudaStream_t stream) {
+                          int32_t* base, float* state, void* space, const Waits& waits, cudaStream_t stream) {
   PromptRows rows{};
   rows.n = groups.n_groups;
   rows.n_rows = groups.n_members;
@@ -1249,7 +1301,7 @@ cudaError_t launch_prefix(const PagedCache& c, int dtype, const Attend& a, const
   rows.state = state;
   Attend all = a;  // every member sees the whole prefix
   all.window = all.sinks = 0;
-  return run_prompt(c, dtype, all, rows, space, stream);
+  return run_prompt(c, dtype, all, rows, space, waits, stream);
 }
 
 }  // namespace mtt
