@@ -726,8 +726,8 @@ MTT_B200_API int mtt_b200_session_engine_collect(mtt_b200_session_engine_t* engi
  * allocation takes the lowest free page first, for the slots in order, so the
  * state after any sequence of calls is determined by the calls alone.
  *
- * All state is caller-owned device memory, every call is stream-ordered with
- * no host synchronisation, and returns MTT_B200_STATUS_*.  Page numbers
+ * All state is caller-owned memory of the current device, every call is
+ * stream-ordered with no host synchronisation, and returns MTT_B200_STATUS_*.  Page numbers
  * outside [0, pages) stand for "no page" and lengths are read as at most
  * table_pages * page_size, so no table content leads out of the pool.  The
  * calls of one cache that change it must be ordered with each other and with

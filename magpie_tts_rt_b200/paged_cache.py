@@ -15,8 +15,8 @@ slot, and a reference count per page, all on the device:
 * ``attend_shared``: the newest tokens' attention where groups of slots share a
   prefix (``PrefixGroups``), computed once for each group.
 
-Every call is enqueued on the current (or given) CUDA stream and returns
-without waiting; no gradient is recorded (this is a decoder's cache).  What a call cannot do on the device (no free page, offsets
+Every call is enqueued on the current (or given) CUDA stream of the pool's
+device and returns without waiting; no gradient is recorded (this is a decoder's cache).  What a call cannot do on the device (no free page, offsets
 that do not fit) it reports in ``status``; what can be seen on the host
 (types, shapes, strides) raises ValueError before anything is launched.
 
@@ -46,6 +46,10 @@ _DTYPES = {torch.bfloat16: L.DTYPE_BF16, torch.float16: L.DTYPE_F16}
 def _check(ok: bool, what: str) -> None:
     if not ok:
         raise ValueError(what)
+
+
+# the current device's index (torch.cuda.current_device takes several times as long)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _raw_stream(device: torch.device):
@@ -121,7 +125,11 @@ class PagedCache:
     # -- plumbing -----------------------------------------------------------
 
     def _handle(self, stream) -> int:
-        return self._raw(self._index) if stream is None else stream.cuda_stream
+        if stream is None:
+            return self._raw(self._index)
+        if stream.device.index != self._index:
+            raise ValueError("the stream belongs to another device than the pool")
+        return stream.cuda_stream
 
     def _workspace(self, handle: int, stream, q_heads: int, rows: int = 0):
         """(address, bytes) of the workspace of calls on one stream: kept, and
@@ -148,10 +156,16 @@ class PagedCache:
             raise ValueError(f"{name} must be a contiguous {dtype} vector of {n} on the pool's device")
         return t.data_ptr()
 
-    @staticmethod
-    def _done(rc: int, what: str) -> None:
+    def _call(self, name: str, *args) -> None:
+        """One launch, on the pool's device whichever is current."""
+        call = getattr(L.lib, name)
+        if _current_device() == self._index:
+            rc = call(*args)
+        else:
+            with torch.cuda.device(self._index):
+                rc = call(*args)
         if rc != L.STATUS_OK:
-            raise RuntimeError(f"{what} failed with status {rc}")
+            raise RuntimeError(f"{name} failed with status {rc}")
 
     # -- upkeep -------------------------------------------------------------
 
@@ -160,8 +174,7 @@ class PagedCache:
         at = self._vector(counts, self.slots, torch.int32, "counts")
         handle = self._handle(stream)
         ws = self._workspace(handle, stream, self.kv_heads)
-        self._done(L.lib.mtt_b200_launch_paged_cache_extend(self._ref, at, ws[0], ws[1], handle),
-                   "mtt_b200_launch_paged_cache_extend")
+        self._call("mtt_b200_launch_paged_cache_extend", self._ref, at, ws[0], ws[1], handle)
 
     def fork(self, source: torch.Tensor, deep: bool = False, stream=None) -> None:
         """Slot d takes over the tokens that slot source[d] had before the call
@@ -170,21 +183,18 @@ class PagedCache:
         at = self._vector(source, self.slots, torch.int32, "source")
         handle = self._handle(stream)
         ws = self._workspace(handle, stream, self.kv_heads)
-        self._done(L.lib.mtt_b200_launch_paged_cache_fork(self._ref, at, 1 if deep else 0, ws[0], ws[1], handle),
-                   "mtt_b200_launch_paged_cache_fork")
+        self._call("mtt_b200_launch_paged_cache_fork", self._ref, at, 1 if deep else 0, ws[0], ws[1], handle)
 
     def free(self, mask: torch.Tensor, stream=None) -> None:
         """Closes every slot with mask ([slots] bool): its pages are released."""
         at = self._vector(mask, self.slots, torch.bool, "mask")
-        self._done(L.lib.mtt_b200_launch_paged_cache_free(self._ref, at, self._handle(stream)),
-                   "mtt_b200_launch_paged_cache_free")
+        self._call("mtt_b200_launch_paged_cache_free", self._ref, at, self._handle(stream))
 
     def compact(self, stream=None) -> None:
         """Moves the pages in use to [0, live); ``live`` [1] holds their number."""
         handle = self._handle(stream)
         ws = self._workspace(handle, stream, self.kv_heads)
-        self._done(L.lib.mtt_b200_launch_paged_cache_compact(self._ref, ws[0], ws[1], handle),
-                   "mtt_b200_launch_paged_cache_compact")
+        self._call("mtt_b200_launch_paged_cache_compact", self._ref, ws[0], ws[1], handle)
 
     def store(self, k: torch.Tensor, v: torch.Tensor, layer: Optional[int] = None,
               offsets: Optional[torch.Tensor] = None, stream=None) -> None:
@@ -219,8 +229,7 @@ class PagedCache:
             args.offsets = self._vector(offsets, self.slots + 1, torch.int32, "offsets")
         else:
             _check(args.rows <= self.slots, "more rows than slots: offsets are needed")
-        self._done(L.lib.mtt_b200_launch_paged_cache_store(self._ref, ctypes.byref(args), self._handle(stream)),
-                   "mtt_b200_launch_paged_cache_store")
+        self._call("mtt_b200_launch_paged_cache_store", self._ref, ctypes.byref(args), self._handle(stream))
 
     # -- attention ----------------------------------------------------------
 
@@ -295,8 +304,7 @@ class PagedCache:
             args.key_mask, args.mask_stride = key_mask.data_ptr(), key_mask.stride(0)
         handle = self._handle(stream)
         ws = self._workspace(handle, stream, args.q_heads, args.rows)
-        self._done(L.lib.mtt_b200_launch_paged_attention(self._ref, ctypes.byref(args), ws[0], ws[1], handle),
-                   "mtt_b200_launch_paged_attention")
+        self._call("mtt_b200_launch_paged_attention", self._ref, ctypes.byref(args), ws[0], ws[1], handle)
         return (out, lse) if return_lse else out
 
     def attend_shared(self, layer: int, q: torch.Tensor, groups: "PrefixGroups", out: Optional[torch.Tensor] = None, *,
@@ -313,8 +321,8 @@ class PagedCache:
         _check(args.rows <= self.slots, "more rows than slots")
         handle = self._handle(stream)
         ws = groups._workspace(handle, stream)
-        self._done(L.lib.mtt_b200_launch_paged_attention_shared(self._ref, ctypes.byref(args), groups._ref, ws[0], ws[1],
-                                                                handle), "mtt_b200_launch_paged_attention_shared")
+        self._call("mtt_b200_launch_paged_attention_shared", self._ref, ctypes.byref(args), groups._ref, ws[0], ws[1],
+                   handle)
         return (out, lse) if return_lse else out
 
 

@@ -1,0 +1,85 @@
+"""The Python side of the paged cache without a GPU: on which device its calls
+are made.  The library is a stand-in that notes each call, the tensors are on
+the CPU."""
+import types
+
+import pytest
+import torch
+
+from magpie_tts_rt_b200 import paged_cache as pc
+
+HOST = -1  # the index that tensors on the CPU report
+
+
+class Library:
+    """Notes (call, device current at it)."""
+
+    def __init__(self):
+        self.calls, self.device = [], 0
+
+    def __getattr__(self, name):
+        def call(*args):
+            if name.endswith("_size"):
+                return 256
+            self.calls.append((name, self.device))
+            return pc.L.STATUS_OK
+        return call
+
+
+@pytest.fixture
+def lib(monkeypatch):
+    lib = Library()
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.before, lib.device = lib.device, self.index
+
+        def __exit__(self, *exc):
+            lib.device = self.before
+
+    monkeypatch.setattr(pc.L, "lib", lib)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(pc, "_current_device", lambda: lib.device, raising=False)
+    return lib
+
+
+def on_host(slots=3, pages=4, layers=2, heads=2, ps=16, d=64):
+    cache = pc.PagedCache.__new__(pc.PagedCache)
+    cache.pool = torch.zeros(pages, layers, 2, heads, ps, d, dtype=torch.bfloat16)
+    cache.device, cache._index, cache._raw, cache.dtype = torch.device("cpu"), HOST, lambda index: 0, torch.bfloat16
+    cache.pages, cache.layers, cache.kv_heads, cache.page_size, cache.head_dim = pages, layers, heads, ps, d
+    cache.slots, cache.table_pages, cache._scale = slots, 2, d ** -0.5
+    cache._c = pc.L.PagedCache()
+    cache._ref = pc.ctypes.byref(cache._c)
+    cache._spaces, cache._outgrown = {}, []
+    return cache
+
+
+def every_call(cache, stream=None):
+    """The public calls that launch something."""
+    i32 = torch.zeros(cache.slots, dtype=torch.int32)
+    kv = torch.zeros(cache.slots, cache.kv_heads, cache.head_dim, dtype=torch.bfloat16)
+    groups = pc.PrefixGroups(cache, [(0, 16, [1, 2])], q_heads=cache.kv_heads)
+    return [lambda: cache.extend(i32, stream=stream), lambda: cache.fork(i32, stream=stream),
+            lambda: cache.free(i32.bool(), stream=stream), lambda: cache.compact(stream=stream),
+            lambda: cache.store(kv, kv, layer=0, stream=stream), lambda: cache.attend(0, kv, stream=stream),
+            lambda: cache.attend_shared(0, kv, groups, stream=stream)]
+
+
+@pytest.mark.parametrize("call", range(7))
+def test_calls_are_made_on_the_pools_device(lib, call):
+    """Another device is current: each launch is made with the pool's, and the other is current again after it."""
+    every_call(on_host())[call]()
+    assert len(lib.calls) == 1 and lib.calls[0][1] == HOST
+    assert lib.device == 0
+
+
+@pytest.mark.parametrize("call", range(7))
+def test_streams_of_another_device_are_refused(lib, call):
+    stream = types.SimpleNamespace(device=torch.device("cuda", 1), cuda_stream=7)
+    with pytest.raises(ValueError):
+        every_call(on_host(), stream)[call]()
+    assert lib.calls == []
