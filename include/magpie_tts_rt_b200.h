@@ -740,6 +740,12 @@ MTT_B200_API int mtt_b200_session_engine_collect(mtt_b200_session_engine_t* engi
  * enough free pages; with 1 and 2 the slot is left as it was.  store writes
  * it only for rows it skips: 1 the slot's offsets do not fit, 3 the row would
  * go to a page that other slots share, or to none.
+ *
+ * refused[i] (may be NULL): extend sets it, for every slot, to whether it
+ * refused the slot's tokens; a fork of the slot or its release clears it.
+ * store writes no row of a slot whose tokens were refused, since its last rows
+ * are then older tokens' (their status stays extend's).  Without refused a
+ * caller has to look at status between extend and store.
  */
 #define MTT_B200_DTYPE_BF16 0
 #define MTT_B200_DTYPE_F16 1
@@ -759,6 +765,7 @@ typedef struct mtt_b200_paged_cache {
   int32_t* refs;       /* [pages], 16-byte aligned */
   int32_t* status;     /* [slots] or NULL */
   int32_t* live;       /* [1] or NULL: pages in use, written by compact */
+  int32_t* refused;    /* [slots] or NULL: tokens are still missing (see above) */
 } mtt_b200_paged_cache_t;
 
 /* Workspace bytes for any call on this cache with up to `rows` query rows of

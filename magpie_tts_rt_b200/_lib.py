@@ -179,7 +179,7 @@ DTYPE_F16 = 1
 class PagedCache(ctypes.Structure):
     _fields_ = [(n, I32) for n in ("pages", "layers", "kv_heads", "page_size", "head_dim", "dtype", "slots",
                                    "table_pages")] + [(n, P) for n in ("pool", "page_table", "lengths", "refs",
-                                                                       "status", "live")]
+                                                                       "status", "live", "refused")]
 
 
 class CacheRows(ctypes.Structure):

@@ -175,6 +175,7 @@ __global__ void __launch_bounds__(kPlanThreads) extend_kernel(PagedCache c, cons
       c.lengths[i] = len + add;
     }
     if (c.status != nullptr && add != 0) c.status[i] = ok ? 0 : (a.need < 0 ? 1 : 2);
+    if (c.refused != nullptr) c.refused[i] = add != 0 && !ok;
   }
 }
 
@@ -273,7 +274,10 @@ __global__ void __launch_bounds__(kMoveThreads) fork_commit_kernel(PagedCache c,
       if (c.is_page(p)) atomicSub(&c.refs[p], 1);
       row[j] = next[j];
     }
-    if (threadIdx.x == 0) c.lengths[d] = u.len[d];
+    if (threadIdx.x == 0) {
+      c.lengths[d] = u.len[d];
+      if (c.refused != nullptr) c.refused[d] = 0;
+    }
   }
   copy_pairs<true>(c, u, parts);
 }
@@ -289,7 +293,10 @@ __global__ void __launch_bounds__(kMoveThreads) free_kernel(PagedCache c, const 
     if (c.is_page(p)) atomicSub(&c.refs[p], 1);
     row[j] = -1;
   }
-  if ((threadIdx.x & 31) == 0) c.lengths[i] = 0;
+  if ((threadIdx.x & 31) == 0) {
+    c.lengths[i] = 0;
+    if (c.refused != nullptr) c.refused[i] = 0;
+  }
 }
 
 // One CTA: live pages, and where those past the live count go.
@@ -375,6 +382,7 @@ __global__ void __launch_bounds__(kMoveThreads) store_kernel(PagedCache c, Rows 
   }
   const int len = c.length(slot);
   if (in.offsets == nullptr && len == 0) return;
+  if (c.refused != nullptr && c.refused[slot] != 0) return;  // its last tokens are not the rows'
   if (count > len) {
     if (threadIdx.x == 0 && c.status != nullptr) c.status[slot] = 1;
     return;
@@ -471,6 +479,7 @@ bool paged_cache_view(const mtt_b200_paged_cache_t* c, PagedCache* out) {
   out->refs = c->refs;
   out->status = c->status;
   out->live = c->live;
+  out->refused = c->refused;
   return true;
 }
 

@@ -22,6 +22,7 @@ struct PagedCache {
   int32_t* refs;
   int32_t* status;
   int32_t* live;
+  int32_t* refused;
 
   // tokens of a slot, as far as its table can hold them
   __device__ __forceinline__ int length(int slot) const {

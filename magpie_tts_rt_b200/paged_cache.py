@@ -97,11 +97,12 @@ class PagedCache:
         self.slots, self.table_pages = slots, table_pages
         self.status = torch.zeros(slots, dtype=torch.int32, device=self.device)
         self.live = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self.refused = torch.zeros(slots, dtype=torch.int32, device=self.device)
         c = L.PagedCache()
         c.pages, c.layers, c.kv_heads, c.page_size, c.head_dim = pages, layers, kv_heads, page_size, head_dim
         c.dtype, c.slots, c.table_pages = _DTYPES[pool.dtype], slots, table_pages
         c.pool, c.page_table, c.lengths, c.refs = (t.data_ptr() for t in (pool, page_table, lengths, refs))
-        c.status, c.live = self.status.data_ptr(), self.live.data_ptr()
+        c.status, c.live, c.refused = (t.data_ptr() for t in (self.status, self.live, self.refused))
         self._c = c
         self._ref = ctypes.byref(c)
         self._scale = head_dim ** -0.5
@@ -170,7 +171,9 @@ class PagedCache:
     # -- upkeep -------------------------------------------------------------
 
     def extend(self, counts: torch.Tensor, stream=None) -> None:
-        """lengths += counts ([slots] int32), with the pages that takes."""
+        """lengths += counts ([slots] int32), with the pages that takes.  A slot
+        that does not get them stays as it is, and ``store`` leaves it alone until
+        the next ``extend`` (``refused`` [slots])."""
         at = self._vector(counts, self.slots, torch.int32, "counts")
         handle = self._handle(stream)
         ws = self._workspace(handle, stream, self.kv_heads)
@@ -202,7 +205,8 @@ class PagedCache:
         [offsets[i], offsets[i + 1]) are slot i's (offsets [slots + 1] int32), or,
         without offsets, row i is slot i's last token.  With ``layer`` k and v are
         [rows, kv_heads, head_dim]; without it [layers, rows, kv_heads, head_dim],
-        every layer at once.  The last two dimensions must be contiguous."""
+        every layer at once.  The last two dimensions must be contiguous.  Rows of
+        slots whose tokens ``extend`` has refused are not written."""
         shape, ks, vs = k.shape, k.stride(), v.stride()
         if (len(shape) != (4 if layer is None else 3) or v.shape != shape or shape[-1] != self.head_dim or
                 shape[-2] != self.kv_heads):

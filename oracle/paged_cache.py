@@ -16,6 +16,7 @@ class ListCache:
         self.rows = [[] for _ in range(slots)]
         self.lengths = [0] * slots
         self.status = [0] * slots
+        self.refused = [False] * slots
         self.table_pages = table_pages
 
     @property
@@ -42,14 +43,16 @@ class ListCache:
     def free(self, mask):
         for i, m in enumerate(mask):
             if m:
-                self.rows[i], self.lengths[i] = [], 0
+                self.rows[i], self.lengths[i], self.refused[i] = [], 0, False
 
     def extend(self, counts):
         free = sorted(set(range(self.pages)) - self.used())
         asked = 0
         for i, c in enumerate(counts):
+            self.refused[i] = False
             if c == 0:
                 continue
+            self.refused[i] = True
             want = -(-(self.lengths[i] + c) // self.page_size)
             if c < 0 or want > self.table_pages:
                 self.status[i] = 1
@@ -59,7 +62,7 @@ class ListCache:
             if need and asked > len(free):
                 self.status[i] = 2
                 continue
-            self.status[i] = 0
+            self.status[i], self.refused[i] = 0, False
             self.rows[i] += free[asked - need:asked]
             self.lengths[i] += c
 
@@ -85,7 +88,7 @@ class ListCache:
             for old, new in zip(before[s][first:], fresh):
                 self.data[new] = self.data[old]
             self.rows[d] = before[s][:first] + fresh
-            self.lengths[d] = lengths[s]
+            self.lengths[d], self.refused[d] = lengths[s], False
 
     def compact(self):
         used = sorted(self.used())
@@ -102,6 +105,8 @@ class ListCache:
         refs = self.refs()
         for i in range(len(self.rows)):
             a, b = offsets[i], offsets[i + 1]
+            if self.refused[i]:
+                continue
             if b - a > self.lengths[i]:
                 self.status[i] = 1
                 continue
