@@ -21,9 +21,12 @@ that do not fit) it reports in ``status``; what can be seen on the host
 (types, shapes, strides) raises ValueError before anything is launched.
 
 Calls that change a cache, and the calls that read it, must be ordered with
-each other by the caller when they use different streams.  Every call can be
-captured into a CUDA graph after one such call on the capturing stream (which
-makes that stream's workspace).
+each other by the caller when they use different streams; a tensor given to a
+call on another stream than its own is the caller's to keep until the call is
+done.  Every call can be captured into a CUDA graph after one such call on the
+capturing stream (which makes that stream's workspace).  A graph goes on using
+that workspace: its replays must be ordered with that stream's other calls, and
+with the replays of other graphs captured on it.
 """
 from __future__ import annotations
 
@@ -106,6 +109,7 @@ class PagedCache:
         self._c = c
         self._ref = ctypes.byref(c)
         self._scale = head_dim ** -0.5
+        self._streams = set()  # that calls were made on
         self._spaces = {}  # (stream, query heads) -> workspace
         self._outgrown = []
         _check(L.lib.mtt_b200_paged_cache_workspace_size(self._ref, kv_heads, 0) > 0, "this cache is too large")
@@ -127,10 +131,24 @@ class PagedCache:
 
     def _handle(self, stream) -> int:
         if stream is None:
-            return self._raw(self._index)
-        if stream.device.index != self._index:
+            handle = self._raw(self._index)
+        elif stream.device.index == self._index:
+            handle = stream.cuda_stream
+        else:
             raise ValueError("the stream belongs to another device than the pool")
-        return stream.cuda_stream
+        if handle not in self._streams:
+            self._keep(stream, self.pool, self.page_table, self.lengths, self.refs, self.status, self.live, self.refused)
+            self._streams.add(handle)
+        return handle
+
+    def _keep(self, stream, *tensors) -> None:
+        """Tensors that calls on this stream use, whichever stream they were made
+        on: when they are dropped, their memory is not reused before those calls
+        are done."""
+        if stream is None:
+            stream = torch.cuda.current_stream(self.device)
+        for t in tensors:
+            t.record_stream(stream)
 
     def _workspace(self, handle: int, stream, q_heads: int, rows: int = 0):
         """(address, bytes) of the workspace of calls on one stream: kept, and
@@ -339,7 +357,8 @@ class PrefixGroups:
     forked from it; the voice itself may be one of them).  ``tokens`` is
     rounded down to full pages.  The voice must stay open while the groups are
     used; a member whose slot has been closed or reopened since is attended on
-    its own."""
+    its own.  Groups may be dropped while calls that use them are still queued, but
+    must outlive CUDA graphs captured with them."""
 
     def __init__(self, cache: PagedCache, groups, q_heads: int):
         _check(q_heads >= 1 and q_heads % cache.kv_heads == 0 and q_heads // cache.kv_heads <= MAX_GROUP,
@@ -376,5 +395,6 @@ class PrefixGroups:
             size = L.lib.mtt_b200_paged_shared_workspace_size(self.cache._ref, self.q_heads, self.n_members)
             with PagedCache._on(stream):
                 data = torch.empty(size, dtype=torch.uint8, device=self.cache.device)
+            self.cache._keep(stream, self._data)
             space = self._spaces[handle] = (data.data_ptr(), size, data)
         return space

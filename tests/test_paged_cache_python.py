@@ -54,7 +54,8 @@ def on_host(slots=3, pages=4, layers=2, heads=2, ps=16, d=64):
     cache.slots, cache.table_pages, cache._scale = slots, 2, d ** -0.5
     cache._c = pc.L.PagedCache()
     cache._ref = pc.ctypes.byref(cache._c)
-    cache._spaces, cache._outgrown = {}, []
+    cache._streams, cache._spaces, cache._outgrown = {0, 7}, {}, []
+    cache._keep = lambda stream, *tensors: None     # a matter of CUDA memory
     return cache
 
 
