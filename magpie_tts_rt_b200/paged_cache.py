@@ -233,20 +233,18 @@ class PagedCache:
         args = L.CacheRows()
         if layer is None:
             _check(shape[0] == self.layers, "k and v have other layers than the cache")
-            args.n_layers, args.k_layer_stride, args.v_layer_stride = self.layers, ks[0], vs[0]
+            args.n_layers = self.layers
         else:
             _check(0 <= layer < self.layers, "no such layer")
             args.layer, args.n_layers = layer, 1
-        for t, st in ((k, ks), (v, vs)):
-            if t.dtype is not self.dtype or t.get_device() != self._index:
-                raise ValueError("k and v must have the pool's type and device")
-            if st[-1] != 1 or st[-2] != self.head_dim:
-                raise ValueError("k and v must be contiguous in their heads")
-            if t.data_ptr() % 16 or st[-3] % 8 or (layer is None and st[0] % 8):
-                raise ValueError("rows of k and v must be 16-byte aligned")
         args.rows = shape[-3]
         args.k, args.v = k.data_ptr(), v.data_ptr()
-        args.k_row_stride, args.v_row_stride = ks[-3], vs[-3]
+        args.k_row_stride = self._rows_of(k, shape[-3:], ks[-3:], "k")
+        args.v_row_stride = self._rows_of(v, shape[-3:], vs[-3:], "v")
+        if layer is None and shape[0] > 1:  # the stride of a dimension of one has no meaning
+            args.k_layer_stride, args.v_layer_stride = ks[0], vs[0]
+            if ks[0] % 8 or vs[0] % 8:
+                raise ValueError("layers of k and v must be 16-byte aligned")
         if offsets is not None:
             args.offsets = self._vector(offsets, self.slots + 1, torch.int32, "offsets")
         else:
@@ -280,24 +278,27 @@ class PagedCache:
         else:
             if out.shape != shape:
                 raise ValueError("out must have q's shape")
-            self._rows_of(out, out.stride(), "out")
-            out_row = out.stride(0)
-        self._rows_of(q, st, "q")
+            out_row = self._rows_of(out, shape, out.stride(), "out")
+        q_row = self._rows_of(q, shape, st, "q")
         lse = None
-        args = L.CacheAttention(layer, q_heads, rows, window, sinks, scale, q.data_ptr(), st[0], out.data_ptr(), out_row)
+        args = L.CacheAttention(layer, q_heads, rows, window, sinks, scale, q.data_ptr(), q_row, out.data_ptr(), out_row)
         if return_lse:
             with self._on(stream):
                 lse = torch.empty((rows, q_heads), dtype=torch.float32, device=self.device)
             args.lse = lse.data_ptr()
         return args, out, lse
 
-    def _rows_of(self, t, st, name) -> None:
+    def _rows_of(self, t, shape, st, name) -> int:
+        """The stride of t's rows [rows, heads, head_dim]; that of a dimension of
+        one has no meaning and is not looked at."""
         if t.dtype is not self.dtype or t.get_device() != self._index:
             raise ValueError(f"{name} must have the pool's type and device")
-        if st[2] != 1 or st[1] != self.head_dim:
+        if st[2] != 1 or (st[1] != self.head_dim and shape[1] > 1):
             raise ValueError(f"{name} must be contiguous in its heads")
-        if t.data_ptr() % 16 or st[0] % 8:
+        row = st[0] if shape[0] > 1 else shape[1] * self.head_dim
+        if t.data_ptr() % 16 or row % 8:
             raise ValueError(f"rows of {name} must be 16-byte aligned")
+        return row
 
     def attend(self, layer: int, q: torch.Tensor, out: Optional[torch.Tensor] = None, *,
                offsets: Optional[torch.Tensor] = None, window: int = 0, sinks: int = 0,
@@ -321,9 +322,10 @@ class PagedCache:
         if key_mask is not None:
             _check(key_mask.dtype is torch.bool and key_mask.dim() == 2 and key_mask.shape[0] == self.slots and
                    key_mask.shape[1] >= self.table_pages * self.page_size and key_mask.stride(1) == 1 and
-                   key_mask.get_device() == self._index and key_mask.stride(0) >= key_mask.shape[1],
+                   key_mask.get_device() == self._index and
+                   (self.slots == 1 or key_mask.stride(0) >= key_mask.shape[1]),
                    "key_mask must be a [slots, >= table_pages * page_size] bool tensor with contiguous rows")
-            args.key_mask, args.mask_stride = key_mask.data_ptr(), key_mask.stride(0)
+            args.key_mask, args.mask_stride = key_mask.data_ptr(), max(key_mask.stride(0), key_mask.shape[1])
         handle = self._handle(stream)
         ws = self._workspace(handle, stream, args.q_heads, args.rows)
         self._call("mtt_b200_launch_paged_attention", self._ref, ctypes.byref(args), ws[0], ws[1], handle)

@@ -49,3 +49,49 @@ def test_refused_tokens_are_not_stored(pc, ps, layer):
         sim.store(k[None], v[None], [0, 1, 2, 3, 4, 5] if sim.lengths[2] else [0, 1, 2, 2, 2, 3], [1])
         cache.store(k.cuda(), v.cuda(), layer=1, offsets=None if sim.lengths[2] else i32([0, 1, 2, 2, 2, 3]))
         same(cache, sim)
+
+
+def odd(t, *sizes):
+    """t's values with other strides: dimensions of one with sizes[i] as theirs."""
+    st = list(t.stride())
+    for dim, stride in sizes:
+        assert t.shape[dim] == 1
+        st[dim] = stride
+    return torch.as_strided(t, t.shape, st)
+
+
+@pytest.mark.parametrize("prompt", [False, True])
+def test_one_head_and_one_row_of_any_stride(pc, prompt):
+    """A single head's stride, a single row's, a single layer's and a single slot's have no meaning."""
+    lengths = [40, 57, 3]
+    cache, pool, table = make(pc, lengths, hkv=1, layers=1)
+    q = queries(3, 1, 64, torch.bfloat16)
+    offsets = [0, 1, 2, 3]
+    ref = O.attention(pool, table, lengths, 0, q, offsets)
+    args = dict(offsets=i32(offsets)) if prompt else {}
+    got, lse = cache.attend(0, odd(q.cuda(), (1, 7)), out=odd(torch.empty(3, 1, 64, dtype=q.dtype, device="cuda"), (1, 3)),
+                            return_lse=True, **args)
+    agree(got, lse, ref, torch.bfloat16, 57)
+    one, pool, table = make(pc, [57], hkv=2, layers=1)
+    q = queries(1, 4, 64, torch.bfloat16)
+    mask = torch.rand(1, one.table_pages * 16, generator=torch.Generator().manual_seed(1)) < 0.5
+    ref = O.attention(pool, table, [57], 0, q, [0, 1], key_mask=mask)
+    args = dict(offsets=i32([0, 1])) if prompt else {}
+    got, lse = one.attend(0, odd(q.cuda(), (0, 3)), key_mask=odd(mask.cuda(), (0, 5)), return_lse=True, **args)
+    agree(got, lse, ref, torch.bfloat16, 57)
+
+
+@pytest.mark.parametrize("hkv,rows,form", [(1, 3, "layer"), (2, 1, "layer"), (1, 3, "all"), (2, 1, "all")])
+def test_stores_of_any_stride(pc, hkv, rows, form):
+    cache, sim = paired(pc, 8, rows, 64, layers=1, hkv=hkv)
+    sim.extend([5] * rows)
+    cache.extend(i32([5] * rows))
+    k, v = queries(rows, hkv, 64, cache.dtype, 3), queries(rows, hkv, 64, cache.dtype, 4)
+    sim.store(k[None], v[None], list(range(rows + 1)), [0])
+    dims = [(1, 9)] if hkv == 1 else [(0, 11)]
+    if form == "layer":
+        cache.store(odd(k.cuda(), *dims), odd(v.cuda(), *dims), layer=0)
+    else:
+        dims = [(0, 13)] + [(d + 1, s) for d, s in dims]
+        cache.store(odd(k.cuda()[None], *dims), odd(v.cuda()[None], *dims))
+    same(cache, sim)
