@@ -838,8 +838,10 @@ MTT_B200_API int mtt_b200_launch_paged_cache_store(const mtt_b200_paged_cache_t*
  * offsets NULL: row i is the last token of slot i (rows <= slots).  With
  * offsets ([slots + 1] int32, as for store) slot i's rows are its last
  * offsets[i + 1] - offsets[i] tokens, whose keys and values are already
- * stored; a slot with more rows than tokens gets out 0 and lse -inf, offsets
- * that are not ascending within [0, rows] leave their rows untouched.
+ * stored; a slot with more rows than tokens gets out 0 and lse -inf, as do rows
+ * before the first slot's and after the last one's.  Offsets that are not
+ * ascending within [0, rows] are not to be given: which rows are then written is
+ * not said (none outside [0, rows]).
  * status[i] becomes 4 when a bounded wait inside the prompt kernel gave up (the
  * bounds grow with the keys that the call has to read): the outputs of slot i's
  * rows are then not to be used. */

@@ -1055,6 +1055,7 @@ __device__ void mark_lost(const PagedCache& c, const PromptRows& rows, const Pro
 // Joins the parts of the units that a boundary between CTAs cut.  Every CTA
 // lists these units (by the CTA in whose share the first boundary between their
 // key tiles falls) and takes its share of their blocks of 32 rows and 32 dims.
+// Also gives rows that no slot has their zeros.
 // (A CTA for each boundary and block, most without work: 65 slots over
 // 32,768 tokens 111.0 us a call instead of 106.7.)
 constexpr int kJoinParts = 8;  // parts on their way at a time
@@ -1068,6 +1069,7 @@ __global__ void __launch_bounds__(kJoinThreads)
   take_turn();
   const bool prefix = rows.members != nullptr;
   const bool mine_gave_up = threadIdx.x < ctas && ws.gave_up[threadIdx.x] != 0;
+  const int row0 = rows.offsets[0], row1 = rows.offsets[rows.n];  // slots have the rows between
   const int64_t line = ws.head[1], per = ws.head[2];
   int cuts = 0;
   {
@@ -1158,6 +1160,16 @@ __global__ void __launch_bounds__(kJoinThreads)
     *reinterpret_cast<uint2*>(a.out + q_row * a.out_row + static_cast<int64_t>(q_head) * D + d0) =
         make_uint2(Half16<T>::pack(o[0] * inv, o[1] * inv), Half16<T>::pack(o[2] * inv, o[3] * inv));
     if (d0 == 0 && a.lse != nullptr) a.lse[static_cast<int64_t>(q_row) * a.q_heads + q_head] = (top + log2f(l)) * kLn2;
+  }
+  // rows that no slot has see nothing
+  if (!prefix && row0 >= 0 && row0 <= row1 && row1 <= a.rows && row1 - row0 < a.rows) {
+    const int64_t pieces = static_cast<int64_t>(a.q_heads) * (D / 8), all = (row0 + a.rows - row1) * pieces;
+    for (int64_t e = blockIdx.x * kJoinThreads + threadIdx.x; e < all; e += gridDim.x * kJoinThreads) {
+      const int k = static_cast<int>(e / pieces), at = static_cast<int>(e % pieces);
+      const int64_t row = k < row0 ? k : row1 + k - row0;
+      *reinterpret_cast<uint4*>(a.out + row * a.out_row + 8 * at) = make_uint4(0, 0, 0, 0);
+      if (at % (D / 8) == 0 && a.lse != nullptr) a.lse[row * a.q_heads + at / (D / 8)] = -CUDART_INF_F;
+    }
   }
 }
 

@@ -312,7 +312,8 @@ class PagedCache:
         query sees the keys up to its own position, those less than ``window``
         back (0: all) or among the first ``sinks``, and of these the ones with
         key_mask ([slots, >= table_pages * page_size] bool).  A row that sees
-        none gets 0.  Returns out, or (out, lse) with the natural log of the sum
+        none gets 0, and so does one that no slot has (offsets may end before the
+        last row, or begin after the first).  Returns out, or (out, lse) with the natural log of the sum
         of exponentials ([rows, q_heads] f32, -inf for a row that sees none)."""
         args, out, lse = self._attention(layer, q, out, window, sinks, scale, return_lse, stream)
         if offsets is not None:

@@ -95,3 +95,26 @@ def test_stores_of_any_stride(pc, hkv, rows, form):
         dims = [(0, 13)] + [(d + 1, s) for d, s in dims]
         cache.store(odd(k.cuda()[None], *dims), odd(v.cuda()[None], *dims))
     same(cache, sim)
+
+
+@pytest.mark.parametrize("d,group", [(64, 1), (128, 3)])
+@pytest.mark.parametrize("before,after", [(0, 5), (300, 0), (3, 700), (0, 0)])
+def test_rows_that_no_slot_has(pc, before, after, d, group):
+    """Offsets that begin after the first row or end before the last: those rows get 0 and -inf, whatever was there."""
+    lengths, new = [300, 40, 0, 9], [290, 0, 0, 9]
+    cache, pool, table = make(pc, lengths, 2, d)
+    offsets = (before + np.cumsum([0] + new)).tolist()
+    rows = offsets[-1] + after
+    q = queries(rows, 2 * group, d, torch.bfloat16)
+    ref = O.attention(pool, table, lengths, 0, q, offsets)
+    out = torch.full((rows, 2 * group + 1, d), float("nan"), dtype=q.dtype, device="cuda")
+    trash = torch.full((rows, 2 * group), 7.0, device="cuda")   # where the call's lse will probably lie
+    del trash
+    got, lse = cache.attend(0, q.cuda(), out=out[:, :2 * group], offsets=i32(offsets), return_lse=True)
+    agree(got, lse, ref, torch.bfloat16, 300)
+    assert torch.isnan(out[:, 2 * group]).all()
+    free = torch.ones(rows, dtype=torch.bool)
+    free[before:offsets[-1]] = False
+    assert (got.cpu()[free] == 0).all() and (lse.cpu()[free] == float("-inf")).all()
+    none = cache.attend(0, q.cuda(), offsets=i32([rows] * 5))
+    assert (none == 0).all()
