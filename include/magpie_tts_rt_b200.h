@@ -830,10 +830,10 @@ MTT_B200_API int mtt_b200_launch_paged_cache_store(const mtt_b200_paged_cache_t*
  *   lse = log sum_j exp(scale q.k_j)          (natural log, f32)
  * with f32 sums and probabilities rounded once to the cache's type (relative
  * to that, 2^-8 or 2^-11, the result is off by less than sum_j p_j |v_j| + |out|); a row that sees no key gets out 0 and lse -inf.  Keys that
- * no query of the slot may see (past the length, or masked) do not reach the
- * result, whatever their bytes; a value that is not finite makes those of the
- * slot's queries not finite that see it, and may make earlier ones of the same
- * call so.  Query head h reads key head h / (q_heads / kv_heads).
+ * no query of the slot's may see (past the length, masked, or out of every
+ * query's window) do not reach the result, whatever their bytes; a value that is
+ * not finite makes those of the slot's queries not finite that see it, and may
+ * make others of its rows in the same call so.  Query head h reads key head h / (q_heads / kv_heads).
  *
  * offsets NULL: row i is the last token of slot i (rows <= slots).  With
  * offsets ([slots + 1] int32, as for store) slot i's rows are its last

@@ -18,8 +18,9 @@
 //                   softmax;
 //   warp 9          TMA: the pages of each key tile into a ring of stages
 //                   (128-byte swizzle);
-//   warp 10         clears value rows that no query may see (page tails,
-//                   masked keys), whose probability of 0 must not meet a NaN;
+//   warp 10         clears value rows that no query of the unit may see (page
+//                   tails, masked keys, later keys, those that the window has left
+//                   behind), whose probability of 0 must not meet a NaN;
 //   warp 11         TMA: the next unit's queries, as soon as the last scores
 //                   of this one are done (the prefix pass's rows lie apart, so
 //                   there the softmax warps copy them).
@@ -604,22 +605,28 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     if (lane == 0)
       for (int k = max(0, it - S); k < it; ++k) drain(&kv_full[k % S], (k / S) & 1);
   } else if (warp == 10) {
-    // ---- value rows that no query may see are cleared before the MMA warp may use the tile.  Key tiles pass
+    // ---- value rows that no query of the unit may see are cleared before the MMA warp may use the tile.  Key tiles pass
     // through too: so neither this warp nor the MMA warp is ever a round of the ring away from the other.
     int it = 0;
     for (bool more = any; more && alive(errv); more = w.next(ws)) {
       const Geom g = w.g;
       const KeySpan span = unit_span(w, prefix, tq, a);
       const bool* mask = a.key_mask != nullptr ? a.key_mask + g.key_slot * a.mask_stride : nullptr;
+      int p0, p1;
+      positions(g, prefix, w.tok0, w.tok0 + 2 * tq, &p0, &p1);
+      const bool zero_tail = p1 + 1 == g.len && (g.len & (c.page_size - 1)) == 0;  // keys past it came as zeros
       auto pass = [&](int t) {  // the ring's next tile: values of tile t, or keys (t < 0)
         const int s = it % S;
         if (!patience.wait(&kv_full[s], (it / S) & 1)) return false;
         ++it;
         const int base = t < 0 ? 0 : kKeys * span.tile(t);
-        if (t >= 0 && (mask != nullptr || (base + kKeys > g.len && (g.len & (c.page_size - 1)) != 0))) {
+        if (t >= 0 && (mask != nullptr || (base + kKeys > p1 + 1 && !zero_tail) ||
+                       (a.window > 0 && base <= p0 - a.window && base + kKeys > a.sinks))) {
           unsigned char* v = ring + static_cast<size_t>(s) * C::kTileBytes;
           for (int r = lane; r < kKeys; r += 32) {
-            const bool keep = base + r < g.len && (mask == nullptr || mask[base + r]);
+            const int j = base + r;
+            const bool keep =
+                j <= p1 && (a.window == 0 || j > p0 - a.window || j < a.sinks) && (mask == nullptr || mask[j]);
             if (!keep) {
 #pragma unroll
               for (int b = 0; b < DB; ++b)
