@@ -828,8 +828,11 @@ MTT_B200_API int mtt_b200_launch_paged_cache_store(const mtt_b200_paged_cache_t*
  * sinks) and key_mask[slot][j] (where given):
  *   out = sum_j exp(scale q.k_j) v_j / sum_j exp(scale q.k_j)
  *   lse = log sum_j exp(scale q.k_j)          (natural log, f32)
- * with f32 sums and probabilities rounded once to the cache's type (relative
- * to that, 2^-8 or 2^-11, the result is off by less than sum_j p_j |v_j| + |out|); a row that sees no key gets out 0 and lse -inf.  Keys that
+ * with f32 sums.  Prompts, and the shared part of a prefix, round the
+ * probabilities p_j once to the cache's type: the result is off by less than u
+ * (sum_j p_j |v_j| + |out|), u = 2^-8 (bf16) or 2^-11 (f16).  Single tokens hold
+ * them in two numbers of that type: u |out| + 2^-16 sum_j p_j |v_j|.  A row that
+ * sees no key gets out 0 and lse -inf.  Keys that
  * no query of the slot's may see (past the length, masked, or out of every
  * query's window) do not reach the result, whatever their bytes; a value that is
  * not finite makes those of the slot's queries not finite that see it, and may

@@ -42,8 +42,11 @@ struct Half16<__nv_bfloat16> {
     const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
   }
-  static __device__ __forceinline__ uint16_t one(float v) { return __bfloat16_as_ushort(__float2bfloat16_rn(v)); }
-  static __device__ __forceinline__ float to_f(uint16_t b) { return bits2f(b); }
+  // the pair, and what its rounding leaves of the two
+  static __device__ __forceinline__ uint2 split(float lo, float hi) {
+    const uint32_t h = pack(lo, hi);
+    return make_uint2(h, pack(lo - __uint_as_float(h << 16), hi - __uint_as_float(h & 0xffff0000u)));
+  }
   static __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                              uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -57,8 +60,11 @@ struct Half16<__half> {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
   }
-  static __device__ __forceinline__ uint16_t one(float v) { return __half_as_ushort(__float2half_rn(v)); }
-  static __device__ __forceinline__ float to_f(uint16_t b) { return __half2float(__ushort_as_half(b)); }
+  static __device__ __forceinline__ uint2 split(float lo, float hi) {
+    const uint32_t h = pack(lo, hi);
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+    return make_uint2(h, pack(lo - f.x, hi - f.y));
+  }
   static __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                              uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"

@@ -12,8 +12,8 @@
 //    with the keys on the MMA's 16-row side and up to 8 query heads on its
 //    8-column side (a step of one query head costs no more).  The
 //    contraction's order is free, so a thread's A fragment is simply its 16
-//    bytes of the key row; two matrix transposes turn P^T into the B operand
-//    of O^T += V^T P^T, and V^T's fragments are byte permutes of two keys'
+//    bytes of the key row; matrix transposes turn P^T into the B operand of
+//    O^T += V^T P^T (once for its 16-bit rounding, once for the rest), and V^T's fragments are byte permutes of two keys'
 //    16-byte pieces.  (tcgen05 would want the same bytes staged in shared
 //    memory for a tile of 128 rows of which 1 to 16 are real.)
 //  * The work is one line of 16-key tiles over all (slot, key head) units,
@@ -239,21 +239,30 @@ __device__ __forceinline__ void attend_tiles(const PagedCache& c, const Attend& 
   #pragma unroll
           for (int u = 0; u < NT; ++u) {
             const float p0 = ex2(s[u][0] - z0), p1 = ex2(s[u][1] - z1), p2 = ex2(s[u][2] - z0), p3 = ex2(s[u][3] - z1);
-            // the sum keeps the unrounded probabilities; the values' weights are rounded to 16 bits once
+            // the sum keeps the unrounded probabilities; the values' weights are two 16-bit numbers each, of whose sum
+            // 16 bits (bf16) or 22 (f16) are right: the second products cost no bytes, and HBM is what bounds this
             l[b][0] += p0 + p2;
             l[b][1] += p1 + p3;
-            const uint32_t b0 = transpose8x8(Half16<T>::pack(p0, p1)), b1 = transpose8x8(Half16<T>::pack(p2, p3));
+            const uint2 w0 = Half16<T>::split(p0, p1), w1 = Half16<T>::split(p2, p3);
+            const uint32_t b0 = transpose8x8(w0.x), b1 = transpose8x8(w1.x);
+            const uint32_t rest0 = transpose8x8(w0.y), rest1 = transpose8x8(w1.y);
   #pragma unroll
             for (int v = 0; v < VC; ++v) {
               const uint4 &x0 = vr[u][0][v], &x1 = vr[u][1][v], &x2 = vr[u][2][v], &x3 = vr[u][3][v];
-              Half16<T>::mma(acc[b][v][0], __byte_perm(x0.x, x1.x, 0x5410), __byte_perm(x0.x, x1.x, 0x7632),
-                             __byte_perm(x2.x, x3.x, 0x5410), __byte_perm(x2.x, x3.x, 0x7632), b0, b1);
-              Half16<T>::mma(acc[b][v][1], __byte_perm(x0.y, x1.y, 0x5410), __byte_perm(x0.y, x1.y, 0x7632),
-                             __byte_perm(x2.y, x3.y, 0x5410), __byte_perm(x2.y, x3.y, 0x7632), b0, b1);
-              Half16<T>::mma(acc[b][v][2], __byte_perm(x0.z, x1.z, 0x5410), __byte_perm(x0.z, x1.z, 0x7632),
-                             __byte_perm(x2.z, x3.z, 0x5410), __byte_perm(x2.z, x3.z, 0x7632), b0, b1);
-              Half16<T>::mma(acc[b][v][3], __byte_perm(x0.w, x1.w, 0x5410), __byte_perm(x0.w, x1.w, 0x7632),
-                             __byte_perm(x2.w, x3.w, 0x5410), __byte_perm(x2.w, x3.w, 0x7632), b0, b1);
+              const uint32_t vt[4][4] = {
+                  {__byte_perm(x0.x, x1.x, 0x5410), __byte_perm(x0.x, x1.x, 0x7632), __byte_perm(x2.x, x3.x, 0x5410),
+                   __byte_perm(x2.x, x3.x, 0x7632)},
+                  {__byte_perm(x0.y, x1.y, 0x5410), __byte_perm(x0.y, x1.y, 0x7632), __byte_perm(x2.y, x3.y, 0x5410),
+                   __byte_perm(x2.y, x3.y, 0x7632)},
+                  {__byte_perm(x0.z, x1.z, 0x5410), __byte_perm(x0.z, x1.z, 0x7632), __byte_perm(x2.z, x3.z, 0x5410),
+                   __byte_perm(x2.z, x3.z, 0x7632)},
+                  {__byte_perm(x0.w, x1.w, 0x5410), __byte_perm(x0.w, x1.w, 0x7632), __byte_perm(x2.w, x3.w, 0x5410),
+                   __byte_perm(x2.w, x3.w, 0x7632)}};
+#pragma unroll
+              for (int w = 0; w < 4; ++w) {
+                Half16<T>::mma(acc[b][v][w], vt[w][0], vt[w][1], vt[w][2], vt[w][3], b0, b1);
+                Half16<T>::mma(acc[b][v][w], vt[w][0], vt[w][1], vt[w][2], vt[w][3], rest0, rest1);
+              }
             }
           }
         }
