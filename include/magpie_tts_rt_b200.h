@@ -831,8 +831,9 @@ MTT_B200_API int mtt_b200_launch_paged_cache_store(const mtt_b200_paged_cache_t*
  * with f32 sums.  Prompts, and the shared part of a prefix, round the
  * probabilities p_j once to the cache's type: the result is off by less than u
  * (sum_j p_j |v_j| + |out|), u = 2^-8 (bf16) or 2^-11 (f16).  Single tokens hold
- * them in two numbers of that type: u |out| + 2^-16 sum_j p_j |v_j|.  A row that
- * sees no key gets out 0 and lse -inf.  Keys that
+ * them in two numbers of that type: u |out| + 2^-16 sum_j p_j |v_j|.  An f16
+ * probability below 2^-22 of the largest loses up to 2^-33 of that one in a
+ * prompt, 2^-40 for a single token.  A row that sees no key gets out 0 and lse -inf.  Keys that
  * no query of the slot's may see (past the length, masked, or out of every
  * query's window) do not reach the result, whatever their bytes; a value that is
  * not finite makes those of the slot's queries not finite that see it, and may

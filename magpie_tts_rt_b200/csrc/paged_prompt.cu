@@ -30,7 +30,8 @@
 // m is not the maximum so far, but one found when it was last needed: as long
 // as a half tile's probabilities stay below 2^15 (where f16 ends; f32 sums and
 // any 16-bit type keep their relative precision up to there) nothing is
-// compared or rescaled.  Only when they do not, or when a row has seen no key
+// compared or rescaled.  (For f16 they are held 2^8 times as large from the start,
+// so that what is small beside the largest stays in that type's range too.)  Only when they do not, or when a row has seen no key
 // yet, is the maximum looked for, O and l rescaled, and the half taken again.
 //
 // The units' key tiles form one line that is cut into equal parts, one per
@@ -58,6 +59,7 @@
 // the FMA pipe (5 to 10%: it is instructions that bound the loop).
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "gemm_tc.cuh"
 #include "paged_attention.cuh"
@@ -71,6 +73,9 @@ constexpr int kHalf = kKeys / 2;    // keys whose probabilities are handed over 
 constexpr int kPairRows = 2 * kTile;
 constexpr int kPromptThreads = 384;
 constexpr int kPromptPlanThreads = 1024;
+// e^{scale S - m} is held times 2^this (see above); l and O share the factor
+template <typename T>
+constexpr float kPromptBias = std::is_same_v<T, __half> ? 8.f : 0.f;
 constexpr int kMinShare = 2;        // key tiles a CTA takes at least
 constexpr int kMaxSms = 160;        // workspaces are sized for the largest device
 
@@ -874,7 +879,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           }
           float sum;
           auto probabilities = [&] {
-            const float off = m == -CUDART_INF_F ? 0.f : -m * a.scale2;
+            const float off = m == -CUDART_INF_F ? 0.f : fmaf(-m, a.scale2, kPromptBias<T>);
             const float2 scale = make_float2(a.scale2, a.scale2), offs = make_float2(off, off);
             float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
@@ -945,7 +950,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       }
       tmem_fence_after_sync();
       const float inv = l == 0.f ? 0.f : 1.f / l;
-      const float m2 = m == -CUDART_INF_F ? m : m * a.scale2;
+      const float m2 = m == -CUDART_INF_F ? m : fmaf(m, a.scale2, -kPromptBias<T>);
       const bool there = q_row >= 0;
       float* part = ws.part + static_cast<int64_t>(part_at) * (D + 2) * kPairRows + i * kTile + r;
       float* state = prefix && there ? rows.state + (static_cast<int64_t>(q_row) * a.q_heads + q_head) * (D + 4) : nullptr;

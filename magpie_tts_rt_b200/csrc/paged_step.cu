@@ -51,6 +51,12 @@ constexpr int step_ctas(int head_dim, int nb) { return (head_dim == 64 ? 4 : 3) 
 // included: 134 us with 0, 96 with 2, 104 with 4, 116 with 8.)
 constexpr int kUnitCost = 2;
 
+// Probabilities are held 2^15 times as large where the cache is f16, so that what
+// is small beside the largest (1) stays in that type's range; sums and weighted
+// values share the factor, and the maximum that goes with them is less by 15.
+template <typename T>
+constexpr float kStepBias = std::is_same_v<T, __half> ? 15.f : 0.f;
+
 struct StepSpace {
   int4* cut;    // [warps]: the cut unit that begins in the warp's share: slot, unit, warps that hold it (0: none)
   float* part;  // [warps][2][queries][D + 2]: of the share's first unit, and of a later one
@@ -149,7 +155,7 @@ struct StepSums {
 };
 
 // A warp's tiles t0 .. t1 - 1 of a unit.  `page` holds the pages of the first
-// step's tiles.
+// step's tiles.  Called once for `sums`.
 template <typename T, int D, int NB>
 __device__ __forceinline__ void attend_tiles(const PagedCache& c, const Attend& a, const SeenTiles& seen,
                                              const int32_t* row, const bool* mask, int64_t head_at, int t0, int t1,
@@ -222,6 +228,7 @@ __device__ __forceinline__ void attend_tiles(const PagedCache& c, const Attend& 
             top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, o));
           }
           const float z0 = top0 == -CUDART_INF_F ? 0.f : top0, z1 = top1 == -CUDART_INF_F ? 0.f : top1;
+          const float y0 = z0 - kStepBias<T>, y1 = z1 - kStepBias<T>;
           const float keep0 = ex2(m[b][0] - z0), keep1 = ex2(m[b][1] - z1);
           m[b][0] = top0;
           m[b][1] = top1;
@@ -238,7 +245,7 @@ __device__ __forceinline__ void attend_tiles(const PagedCache& c, const Attend& 
             }
   #pragma unroll
           for (int u = 0; u < NT; ++u) {
-            const float p0 = ex2(s[u][0] - z0), p1 = ex2(s[u][1] - z1), p2 = ex2(s[u][2] - z0), p3 = ex2(s[u][3] - z1);
+            const float p0 = ex2(s[u][0] - y0), p1 = ex2(s[u][1] - y1), p2 = ex2(s[u][2] - y0), p3 = ex2(s[u][3] - y1);
             // the sum keeps the unrounded probabilities; the values' weights are two 16-bit numbers each, of whose sum
             // 16 bits (bf16) or 22 (f16) are right: the second products cost no bytes, and HBM is what bounds this
             l[b][0] += p0 + p2;
@@ -267,6 +274,11 @@ __device__ __forceinline__ void attend_tiles(const PagedCache& c, const Attend& 
           }
         }
       }
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    m[b][0] -= kStepBias<T>;
+    m[b][1] -= kStepBias<T>;
+  }
 }
 
 template <typename T, int D, int NB>

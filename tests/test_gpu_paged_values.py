@@ -52,3 +52,40 @@ def test_step_weights_are_finer_than_the_caches_type(pc, keys, slots, dtype, d, 
     err = (got.cpu().double() - out).abs()
     assert (err <= tol).all(), (err / tol).max().item()
     assert (lse.cpu().double() - ref_lse).abs().max().item() <= 5e-4
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("bits", [6.4, 13.4, 20.4, 24.4, 27.4])
+@pytest.mark.parametrize("form,slots", [("step", 2), ("step", 1200), ("prompt", 1200), ("shared", 400)])
+@pytest.mark.parametrize("sink_at", [0, 40000])
+def test_many_small_probabilities(pc, dtype, bits, form, slots, sink_at):
+    """One key whose value is zero takes nearly all, 65,536 others 2^-bits of it each: the result is theirs alone.  Slots
+    enough that most keep their keys together (each part of a slot has a largest probability of its own).
+    Tolerance: the formulas of agree(), without its allowance for small f16 probabilities but with the 2^-33 of the
+    largest that such a one may lose below 2^-22 of it, and the smallest step of the result's type."""
+    n, d, ps = 65536, 64, 128
+    g = torch.Generator().manual_seed(int(bits))
+    pool = torch.zeros(n // ps, 1, 2, 1, ps, d)
+    pool[:, :, 1] = 1 + torch.rand(pool[:, :, 1].shape, generator=g)
+    pool[sink_at // ps, 0, 0, 0, sink_at % ps, 0] = bits * 0.6931 / 8
+    pool[sink_at // ps, 0, 1, 0, sink_at % ps] = 0
+    pool = pool.to(dtype)
+    table = torch.arange(n // ps, dtype=torch.int32).expand(slots, n // ps).contiguous()    # all slots hold all pages
+    cache = pc.PagedCache(pool.cuda(), table.cuda(), i32([n] * slots), i32([slots] * (n // ps)))
+    q = torch.zeros(slots, 1, d, dtype=dtype)
+    q[:, :, 0] = 8
+    out, ref_lse, weight = O.attention(pool, table[:1], [n], 0, q[:1], [0, 1], scale=1.0)
+    if form == "shared":
+        plan = pc.PrefixGroups(cache, [(0, n, [i]) for i in range(slots)], q_heads=1)
+        plan._c.shared_tokens = 0
+        got, lse = cache.attend_shared(0, q.cuda(), plan, scale=1.0, return_lse=True)
+    else:
+        offsets = i32(list(range(slots + 1))) if form == "prompt" else None
+        got, lse = cache.attend(0, q.cuda(), offsets=offsets, scale=1.0, return_lse=True)
+    tol = 1.1 * U[dtype] * (out.abs() + weight)
+    if dtype == torch.float16:
+        tol += 2.0 ** -33 * 2 * n + 2.0 ** -25
+    err = (got.cpu().double() - out).abs()
+    assert (err <= tol).all(), (err / tol).max().item()
+    assert (lse.cpu().double() - ref_lse).abs().max().item() <= 5e-4
+    assert (cache.status == 0).all()
