@@ -881,8 +881,9 @@ typedef struct mtt_b200_prefix_groups {
   const int32_t* tokens;     /* [n_groups] */
   const int32_t* offsets;    /* [n_groups + 1] ascending, offsets[n_groups] = n_members */
   const int32_t* members;    /* [n_members] slots */
-  int64_t shared_tokens;     /* sum over groups of members x tokens, if the caller knows it (0: not known).
-                                Where it is known and small, sharing costs more than it saves and
+  int64_t shared_tokens;     /* sum over groups of members x tokens, if the caller knows it (0: not known);
+                                under a window over the groups with tokens <= sinks, and if there are
+                                none, n_groups 0 saves a pass over prefixes that are not shared.  Where it is known and small, sharing costs more than it saves and
                                 every slot is attended on its own. */
 } mtt_b200_prefix_groups_t;
 

@@ -30,8 +30,10 @@ with the replays of other graphs captured on it.
 """
 from __future__ import annotations
 
+import bisect
 import contextlib
 import ctypes
+import itertools
 from typing import Optional
 
 import torch
@@ -346,8 +348,8 @@ class PagedCache:
         _check(args.rows <= self.slots, "more rows than slots")
         handle = self._handle(stream)
         ws = groups._workspace(handle, stream)
-        self._call("mtt_b200_launch_paged_attention_shared", self._ref, ctypes.byref(args), groups._ref, ws[0], ws[1],
-                   handle)
+        self._call("mtt_b200_launch_paged_attention_shared", self._ref, ctypes.byref(args), groups._seen(window, sinks),
+                   ws[0], ws[1], handle)
         return (out, lse) if return_lse else out
 
 
@@ -391,6 +393,24 @@ class PrefixGroups:
         self._c = c
         self._ref = ctypes.byref(c)
         self._spaces = {}
+        # prefix lengths in order, and the members' tokens of the groups up to each
+        sizes = sorted((t, t * (b - a)) for t, a, b in zip(tokens, offsets, offsets[1:]))
+        self._lengths = [t for t, _ in sizes]
+        self._shared_up_to = [0] + list(itertools.accumulate(n for _, n in sizes))
+
+    def _seen(self, window: int, sinks: int):
+        """The groups for a call: under a window only prefixes among the sinks are
+        shared, so only these speak for the prefix pass, and without one there is
+        none."""
+        n = len(self._lengths) if window == 0 else bisect.bisect_right(self._lengths, sinks)
+        if n == len(self._lengths):
+            return self._ref
+        c = L.PrefixGroups.from_buffer_copy(self._c)
+        if n == 0:
+            c.n_groups = c.n_members = 0
+        elif c.shared_tokens > 0:
+            c.shared_tokens = self._shared_up_to[n]
+        return ctypes.byref(c)
 
     def _workspace(self, handle: int, stream):
         space = self._spaces.get(handle)

@@ -84,3 +84,25 @@ def test_streams_of_another_device_are_refused(lib, call):
     with pytest.raises(ValueError):
         every_call(on_host(), stream)[call]()
     assert lib.calls == []
+
+
+@pytest.mark.parametrize("window,sinks,groups,shared", [
+    (0, 0, 3, 16 * 2 + 48 * 3 + 96 * 1), (9, 96, 3, 16 * 2 + 48 * 3 + 96 * 1), (9, 95, 3, 16 * 2 + 48 * 3),
+    (9, 48, 3, 16 * 2 + 48 * 3), (9, 16, 3, 16 * 2), (9, 15, 0, None), (9, 0, 0, None), (0, 15, 3, 16 * 2 + 48 * 3 + 96 * 1)])
+@pytest.mark.parametrize("known", [True, False])
+def test_groups_that_a_window_does_not_share(lib, monkeypatch, window, sinks, groups, shared, known):
+    """The prefix pass is asked for by the groups that it can serve: those whose prefix is among the sinks."""
+    cache = on_host(slots=8)
+    cache.table_pages = 8
+    plan = pc.PrefixGroups(cache, [(0, 50, [1, 2, 3]), (0, 16, [4, 5]), (0, 96, [6]), (0, 7, [7])], q_heads=2)
+    if not known:
+        plan._c.shared_tokens = 0
+    seen = []
+    monkeypatch.setattr(cache, "_call", lambda name, *args: seen.append(args[2]._obj))
+    q = torch.zeros(8, 2, 64, dtype=torch.bfloat16)
+    cache.attend_shared(0, q, plan, window=window, sinks=sinks)
+    assert seen[0].n_groups == groups
+    if groups:
+        assert seen[0].shared_tokens == (shared if known else 0) and seen[0].n_members == 6
+        assert [getattr(seen[0], f) for f in ("voice", "tokens", "offsets", "members")] == [
+            getattr(plan._c, f) for f in ("voice", "tokens", "offsets", "members")]
