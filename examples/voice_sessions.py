@@ -93,19 +93,20 @@ class VoiceServer:
                                                if self.open[s] and self.voice[s] == v])
                 for v in range(2) for r in range(2)]
         self.groups = PrefixGroups(self.cache, rows, q_heads=HEADS)
-        self.one_more = self._slots([0] * 4 + [1 if self.open[s // 2] else 0 for s in range(2 * self.sessions)])
+        one_more = [0] * 4 + [1 if self.open[s // 2] else 0 for s in range(2 * self.sessions)]
+        self.one_more = self._slots(one_more)
+        # rows of the voices themselves store nothing: their last tokens are shared pages or already there
+        self.live = self._slots([s for s, n in enumerate(one_more) if n], torch.int64)
+        self.offsets = self._slots([sum(one_more[:s]) for s in range(len(one_more) + 1)])
 
     def step(self, x: torch.Tensor) -> torch.Tensor:
         """x [slots, 768]: one token's input per slot (closed slots' rows are ignored)."""
         self.cache.extend(self.one_more)
         sinks = REFERENCE_PREFIX if self.window else 0
-        # rows of the voices themselves store nothing: their last tokens are shared pages or already there
-        offsets = torch.cat([torch.zeros(1, dtype=torch.int32, device="cuda"), self.one_more.cumsum(0, dtype=torch.int32)])
-        live = self.one_more.bool().nonzero()[:, 0]
         for layer in range(self.layers):
             x = self._layer(x, layer,
                             lambda l, q: self.cache.attend_shared(l, q, self.groups, window=self.window, sinks=sinks),
-                            lambda k, v, l: self.cache.store(k[live], v[live], layer=l, offsets=offsets))
+                            lambda k, v, l: self.cache.store(k[self.live], v[self.live], layer=l, offsets=self.offsets))
         return x
 
 
