@@ -45,6 +45,7 @@ HEAD_DIMS = (64, 128)
 MAX_SLOTS = 16384
 MAX_GROUP = 64
 MAX_ROWS = 1 << 22
+MAX_TOKENS = 1 << 30  # more than a slot can have
 _DTYPES = {torch.bfloat16: L.DTYPE_BF16, torch.float16: L.DTYPE_F16}
 
 
@@ -269,6 +270,7 @@ class PagedCache:
             raise ValueError("no such layer")
         if window < 0 or sinks < 0:
             raise ValueError("window and sinks must not be negative")
+        window, sinks = min(window, MAX_TOKENS), min(sinks, MAX_TOKENS)  # the struct's fields would wrap
         if scale is None:
             scale = self._scale
         elif not 0 < scale < float("inf"):

@@ -106,3 +106,14 @@ def test_groups_that_a_window_does_not_share(lib, monkeypatch, window, sinks, gr
         assert seen[0].shared_tokens == (shared if known else 0) and seen[0].n_members == 6
         assert [getattr(seen[0], f) for f in ("voice", "tokens", "offsets", "members")] == [
             getattr(plan._c, f) for f in ("voice", "tokens", "offsets", "members")]
+
+
+@pytest.mark.parametrize("value", [2 ** 31 - 1, 2 ** 31, 2 ** 32, 2 ** 32 + 5, 2 ** 63 - 1, 2 ** 70])
+@pytest.mark.parametrize("name", ["window", "sinks"])
+def test_windows_past_32_bits(lib, monkeypatch, name, value):
+    """A window or number of sinks that no slot reaches is all of a slot, however large it is given."""
+    cache = on_host()
+    seen = []
+    monkeypatch.setattr(cache, "_call", lambda call, *args: seen.append(args[1]._obj))
+    cache.attend(0, torch.zeros(3, 2, 64, dtype=torch.bfloat16), **{name: value})
+    assert getattr(seen[0], name) >= 1 << 30
