@@ -33,6 +33,7 @@
 // in a unit (187 and 247 us, 389 us for the short ones); a unit's further tiles
 // prefetched into L2 when it is entered (249 -> 253 us, the short ones 10 us more).
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "paged_attention.cuh"
@@ -661,22 +662,26 @@ struct FewLaunch {
   }
 };
 
-// Clusters of `Spread` CTAs of the kernel that the current device runs at once.
+// Clusters of `Spread` CTAs of the kernel that the current device runs at once
+// (0: cannot be queried).  Nothing here allocates or throws.
 template <typename T, int D, int NB, int W, int Spread>
 int few_clusters() {
-  static PerDeviceInt cache;  // the opt-in below is per device context
-  return cache.get([] {
+  static std::atomic<int> known[64];  // by device ordinal, plus 1; the opt-in below is per device
+  int dev = -1, clusters = 0;
+  if (cudaGetDevice(&dev) == cudaSuccess) {
+    if (dev >= 0 && dev < 64 && (clusters = known[dev].load(std::memory_order_relaxed)) > 0) return clusters - 1;
     const auto kernel = step_few_kernel<T, D, NB, W>;
-    int clusters = 0;
     FewLaunch launch(1, Spread, W, few_bytes(D, NB, W), nullptr);
     launch.cfg.numAttrs = 1;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(few_bytes(D, NB, W))) != cudaSuccess ||
-        cudaOccupancyMaxActiveClusters(&clusters, kernel, &launch.cfg) != cudaSuccess)
-      clusters = 0;
-    cudaGetLastError();
-    return clusters;
-  });
+                             static_cast<int>(few_bytes(D, NB, W))) == cudaSuccess &&
+        cudaOccupancyMaxActiveClusters(&clusters, kernel, &launch.cfg) == cudaSuccess) {
+      if (dev >= 0 && dev < 64) known[dev].store(clusters + 1, std::memory_order_relaxed);
+      return clusters;
+    }
+  }
+  cudaGetLastError();
+  return 0;
 }
 
 // 8-query blocks of a unit, and units per key head
