@@ -13,8 +13,8 @@
 //    8-column side (a step of one query head costs no more).  The
 //    contraction's order is free, so a thread's A fragment is simply its 16
 //    bytes of the key row; matrix transposes turn P^T into the B operand of
-//    O^T += V^T P^T (once for its 16-bit rounding, once for the rest), and V^T's fragments are byte permutes of two keys'
-//    16-byte pieces.  (tcgen05 would want the same bytes staged in shared
+//    O^T += V^T P^T (once for its 16-bit rounding, once for the rest), and
+//    V^T's fragments are byte permutes of two keys' 16-byte pieces.  (tcgen05 would want the same bytes staged in shared
 //    memory for a tile of 128 rows of which 1 to 16 are real.)
 //  * The work is one line of 16-key tiles over all (slot, key head) units,
 //    cut into equal parts for the warps of a grid that fills the device, so
@@ -25,13 +25,15 @@
 //  * Few slots, whose call is launches and latency, take clusters instead
 //    (step_few_kernel): one launch.
 // Measured, line and join: 512 slots of 12 heads of 64, up to 1242 of 2048 keys in
-// reach, 162 us (6.7 TB/s of the keys and values in reach; 974 MB from DRAM); 8
-// slots of 30,001 to 65,536 keys, 32/8 heads of 128, 238 us (6.3 TB/s).
-// Clusters: 2 slots of 467 keys, 12 heads of 64, 5.3 us (9.0 us as a line).  What
-// bounds the line is DRAM; where sequences are short (1 to 249 keys) a unit's chain
-// of dependent loads (63 us for 275 MB).  Tried: shares per CTA with the four warps of a CTA side by side
-// in a unit (187 and 247 us, 389 us for the short ones); a unit's further tiles
-// prefetched into L2 when it is entered (249 -> 253 us, the short ones 10 us more).
+// reach, 164 us (974 MB from DRAM, where masked keys are not read: 5.9 TB/s); 8
+// slots of 30,001 to 65,536 keys, 32/8 heads of 128, 239 to 251 us from one GPU to
+// another (6.3 to 6.0 TB/s).  Clusters: 2 slots of 467 keys, 12 heads of 64, 5.4 us
+// (9.0 us as a line).  What bounds the line is DRAM; where sequences are short (1
+// to 249 keys) a unit's chain of dependent loads (65 us for 275 MB).  The second
+// product of the values costs 1%.  Tried, before it: shares per CTA with the four
+// warps of a CTA side by side in a unit (187 and 247 us, 389 us for the short ones,
+// when the line took 162 and 238); a unit's further tiles prefetched into L2 when
+// it is entered (249 -> 253 us, the short ones 10 us more).
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -534,20 +536,25 @@ __global__ void __launch_bounds__(kStepThreads)
 // warps), if a slot cannot be longer than kFewSteps steps of each of its warps.
 // There this saves the scan, the second launch and the parts' way through L2;
 // past either limit the line of tiles is faster, as it fills the device and
-// balances it.  GPU time of a call in us, line / clusters, bf16, all slots of the
-// same length (in brackets what is not taken):
+// balances it.  How long a slot can be is the table's width, which the host knows,
+// not its length, which it does not: a short slot in a wide table takes the line.
+// GPU time of a call in us, line / clusters, bf16, all slots of the
+// same length (in brackets what is not taken, as it was with one product of the
+// values):
 //   heads  dim  slots    128 keys      467         1000         2000         8000
-//   12/12   64    2     8.7 /  6.4  11.7 /  7.0  13.2 /  7.6  14.7 /  8.5  22.5 / 16.7
-//   12/12   64    9    11.2 /  7.3  13.2 /  8.2  15.7 / 13.1  19.5 / 17.4
-//   12/12   64   24    12.5 /  7.1  13.9 / 11.9  20.8 / 18.5 (32.6 / 29.4)
-//   32/8   128    4    14.3 /  7.5  15.4 /  8.6  17.1 / 10.4  20.9 / 15.1 (36.0 / 34.8)
-//   32/8   128   16    15.5 /  8.2  18.3 / 13.4  24.3 / 19.5 (34.8 / 30.8)
-//   32/8   128   48    17.4 / 12.0 (29.1 / 27.4) (45.9 / 48.6)
-//   16/1   128    6    21.3 /  7.7  21.9 /  8.4  23.7 /  9.1  25.2 / 11.1
+//   12/12   64    2     8.5 /  5.6   9.2 /  5.8  11.9 /  7.4  14.3 /  7.5  20.8 / 16.0
+//   12/12   64    9    10.5 /  6.3  13.4 /  8.2  15.6 / 12.0  20.2 / 18.2
+//   12/12   64   24    12.0 /  6.7  13.6 / 12.2  21.8 / 19.0 (32.6 / 29.4)
+//   32/8   128    4    12.6 /  6.2  14.0 /  8.2  16.6 / 10.1  20.8 / 13.5 (36.0 / 34.8)
+//   32/8   128   16    14.5 /  7.4  17.8 / 12.0  23.7 / 18.3 (34.8 / 30.8)
+//   32/8   128   48    18.3 / 12.5 (29.1 / 27.4) (45.9 / 48.6)
+//   16/1   128    6    21.2 /  7.9  21.8 /  8.1  22.8 /  9.9  27.1 / 14.8
 constexpr int kMaxSpread = 8, kFewSteps = 4;
 
+// 4 CTAs of 4 warps an SM, as head_dim 64 has by itself: 132 registers instead of
+// 128 would let one cluster in four go.
 template <typename T, int D, int NB, int W>
-__global__ void __launch_bounds__(32 * W) step_few_kernel(PagedCache c, Attend a, int blocks, int spread) {
+__global__ void __launch_bounds__(32 * W, D == 128 && NB == 1 && W == 4 ? 4 : 0) step_few_kernel(PagedCache c, Attend a, int blocks, int spread) {
   constexpr int NT = step_tiles(D);
   constexpr int NQ = 8 * NB, KC = D / 32, VC = D / 64;
   constexpr int kRow = D + 2;  // weighted values, maximum, sum
