@@ -40,10 +40,10 @@ bool attend_args(const PagedCache& c, const mtt_b200_cache_attention_t* args, At
 
 // Keys and values of all members' prefixes from which on the prefix pass pays:
 // it adds about 20 us of launches and dependent steps, while those bytes read
-// slot by slot come at 8 to 10 TB/s, mostly from L2.  Measured, each slot on its
-// own against shared: 101 MB (12 heads of 64, 1024 tokens, 32 slots) 20 against
-// 32 us; 134 MB (8 of 128, 16384, 2) 37 / 45; 302 MB (12 of 64, 192, 512) 55 / 47;
-// 403 MB (12 of 64, 16384, 8) 58 / 42; 2.1 GB (8 of 128, 4096, 128) 243 / 54.
+// slot by slot come at 4 to 9 TB/s, mostly from L2.  Measured, each slot on its
+// own against shared: 101 MB (12 heads of 64, 1024 tokens, 32 slots) 19 against
+// 30 us; 134 MB (8 of 128, 16384, 2) 38 / 62; 302 MB (12 of 64, 192, 512) 43 / 34;
+// 403 MB (12 of 64, 16384, 8) 66 / 60; 2.1 GB (8 of 128, 4096, 128) 244 / 43.
 constexpr double kSharedBytesWorth = 220e6;
 
 // Bytes of the prefix pass's results: base and state (SharedPrefix).

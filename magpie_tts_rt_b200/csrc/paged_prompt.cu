@@ -31,8 +31,9 @@
 // as a half tile's probabilities stay below 2^15 (where f16 ends; f32 sums and
 // any 16-bit type keep their relative precision up to there) nothing is
 // compared or rescaled.  (For f16 they are held 2^8 times as large from the start,
-// so that what is small beside the largest stays in that type's range too.)  Only when they do not, or when a row has seen no key
-// yet, is the maximum looked for, O and l rescaled, and the half taken again.
+// so that what is small beside the largest stays in that type's range too.)  Only
+// when they do not, or when a row has seen no key yet, is the maximum looked for, O
+// and l rescaled, and the half taken again.
 //
 // The units' key tiles form one line that is cut into equal parts, one per
 // CTA; a unit cut by a boundary leaves (m, l, O) in the workspace for a
@@ -46,9 +47,13 @@
 // slots of its share with status 4 (and lets the members of a prefix pass be
 // attended on their own).
 //
-// Measured: 8192 tokens, 32/8 heads of 128, causal, 484 us alone and 555 us back
-// to back, where the board's power holds the clock near 1.4 GHz (1.14 and 0.99
-// PFLOP/s); the tensor pipe and the special function unit are each busy 59% of
+// Probabilities are rounded once to the cache's type because P is the tensor
+// core's A operand: to multiply the rounding's remainder as well would take a key
+// tile's MMAs from 2048 to 3072 cycles of the 3100 that it takes.
+//
+// Measured: 8192 tokens, 32/8 heads of 128, causal, 484 us alone and 550 to 562 us
+// back to back, where the board's power holds the clock near 1.4 GHz (1.14 and
+// 0.99 PFLOP/s); the tensor pipe and the special function unit are each busy 59% of
 // the time.  A key tile takes both Q tiles about 3100 SM cycles: 2048 of MMA, as
 // many of exponentials, and what bounds it is a softmax warp's own chain: 500
 // cycles for a half's 64 exponentials a row, 300 for loads, packing, stores and
