@@ -16,9 +16,11 @@ slot, and a reference count per page, all on the device:
   prefix (``PrefixGroups``), computed once for each group.
 
 Every call is enqueued on the current (or given) CUDA stream of the pool's
-device and returns without waiting; no gradient is recorded (this is a decoder's cache).  What a call cannot do on the device (no free page, offsets
-that do not fit) it reports in ``status``; what can be seen on the host
-(types, shapes, strides) raises ValueError before anything is launched.
+device and returns without waiting; no gradient is recorded (this is a decoder's
+cache).  What an upkeep call cannot do on the device (no free page, rows that do
+not fit) it reports in ``status``; what can be seen on the host (types, shapes,
+strides, streams of another device) raises ValueError before anything is
+launched.
 
 Calls that change a cache, and the calls that read it, must be ordered with
 each other by the caller when they use different streams; a tensor given to a
