@@ -18,7 +18,8 @@ The 4-bit format: 64 dims of a token's head share a (step, low) pair of the cach
 value = low + step * code, code 0..15; low is the smallest of the 64, step the spread / 15, and the
 code is chosen in single precision: rint((x - low) * (1 / step)).  A block (page, layer, keys or
 values, head) of the pool [pages, layers, 2, kv_heads, page_size, head_dim / 2 + head_dim / 16]
-bytes holds the codes of its page_size tokens (dim 2 i in the low half of byte i), then their pairs.
+bytes holds the codes of its page_size tokens, then their pairs.  Every 8 dims are a 32-bit word: the
+codes of dims 0, 2, 4, 6, then those of 1, 3, 5, 7, from the lowest bits up.
 
 With ``own`` false every operator is computed in its plain form (elementary torch operations
 in 32 bits, rounded once at the end); with ``own`` true by the framework's kernels.
@@ -409,13 +410,15 @@ def _quantised(x):
 
 
 def _packed(codes):
-    return codes[..., 0::2] | codes[..., 1::2] << 4
+    c = codes.unflatten(-1, (-1, 4, 2)).transpose(-1, -2).flatten(-2)      # of each 8: 0, 2, 4, 6, 1, 3, 5, 7
+    return (c[..., 0::2] | c[..., 1::2] << 4).flatten(-2)
 
 
 def _unpacked(blocks, ps, d, dtype):
     """blocks [..., bytes] -> values [..., ps, d] in f32."""
     codes = blocks[..., :ps * d // 2].unflatten(-1, (ps, d // 2))
     codes = torch.stack([codes & 15, codes >> 4], -1).flatten(-2)
+    codes = codes.unflatten(-1, (-1, 2, 4)).transpose(-1, -2).flatten(-3)
     pairs = blocks[..., ps * d // 2:].contiguous().view(dtype).unflatten(-1, (ps, d // GROUP, 2)).float()
     values = codes.unflatten(-1, (-1, GROUP)).float()
     return values.mul_(pairs[..., 0:1]).add_(pairs[..., 1:2]).flatten(-2)
@@ -560,7 +563,8 @@ def _held(case, blocks):
     n, h = blocks.shape[:2]
     byte = blocks[..., :ps * d // 2].reshape(n, h, ps, d // 2).long()
     code = torch.empty(n, h, ps, d, dtype=torch.float64, device=blocks.device)
-    code[..., 0::2], code[..., 1::2] = (byte % 16).double(), (byte // 16).double()
+    for dim, (b, above) in enumerate([(0, 1), (2, 1), (0, 16), (2, 16), (1, 1), (3, 1), (1, 16), (3, 16)]):
+        code[..., dim::8] = (byte[..., b::4] // above % 16).double()
     pair = blocks[..., ps * d // 2:].contiguous().view(DTYPES[case["dtype"]]).double().reshape(n, h, ps, d // GROUP, 2)
     return pair[..., 1].repeat_interleave(GROUP, -1) + pair[..., 0].repeat_interleave(GROUP, -1) * code
 
