@@ -750,13 +750,32 @@ MTT_B200_API int mtt_b200_session_engine_collect(mtt_b200_session_engine_t* engi
 #define MTT_B200_DTYPE_BF16 0
 #define MTT_B200_DTYPE_F16 1
 
+/*
+ * Or'ed into a cache's dtype: the pool holds keys and values in 4 bits.  The
+ * dtype below it stays that of keys, values, queries and outputs in the calls.
+ * 64 dims of a token's head (a group) share a pair (step, low) of that type:
+ *   low = the smallest of the 64,  step = their spread / 15,
+ *   code = rint((x - low) * (1 / step)) in 0..15 (0 where step is below 2^-126),
+ *   value = low + step * code,
+ * with spread, spread / 15 and the code's operations each rounded to single
+ * precision, and step then to the type.  A group with a value that is not
+ * finite, or a spread that single precision does not hold, reads as NaN.
+ *   pool [pages][layers][2][kv_heads] blocks of page_size * (head_dim / 2 +
+ *   head_dim / 16) bytes: the codes of the block's tokens (head_dim / 2 bytes
+ *   each), then their pairs, step first ([page_size][head_dim / 64][2]).  Every
+ *   8 dims are a 32-bit word: the codes of dims 0, 2, 4, 6, then those of 1, 3,
+ *   5, 7, from the lowest bits up.
+ */
+#define MTT_B200_CACHE_4BIT 0x100
+
 typedef struct mtt_b200_paged_cache {
   int32_t pages;
   int32_t layers;
   int32_t kv_heads;
   int32_t page_size;   /* 16, 32, 64 or 128 */
   int32_t head_dim;    /* 64 or 128 */
-  int32_t dtype;       /* MTT_B200_DTYPE_* of the pool, of keys, values, queries and outputs */
+  int32_t dtype;       /* MTT_B200_DTYPE_* of the pool, of keys, values, queries and outputs;
+                          or MTT_B200_CACHE_4BIT | that of all but the pool */
   int32_t slots;       /* <= 16384 */
   int32_t table_pages; /* page_table columns; table_pages * page_size < 2^30 */
   void* pool;          /* 128-byte aligned */
@@ -823,6 +842,67 @@ typedef struct mtt_b200_cache_rows {
 MTT_B200_API int mtt_b200_launch_paged_cache_store(const mtt_b200_paged_cache_t* cache,
                                                    const mtt_b200_cache_rows_t* rows, void* stream);
 
+/* The reverse of store: reads the keys and values of each slot's last tokens
+ * into rows of k and v (written; the same fields).  A row that no slot has, or
+ * whose slot has fewer tokens than rows, gets zeros, and so does one without a
+ * page.  Of a 4-bit cache it gives the values that the codes stand for, rounded
+ * once to the type. */
+MTT_B200_API int mtt_b200_launch_paged_cache_load(const mtt_b200_paged_cache_t* cache,
+                                                  const mtt_b200_cache_rows_t* rows, void* stream);
+
+/* Position rotation of queries and keys, with a norm of each head before it:
+ *   y = x / sqrt(mean(x^2) + eps) * weight            (where a weight is given)
+ *   (y_a, y_b) <- (y_a cos t - y_b sin t, y_b cos t + y_a sin t),  t = 2 pi turns[i] position
+ * for i in [0, rotary_dim / 2), a = i, b = i + rotary_dim / 2, or, interleaved,
+ * a = 2 i, b = 2 i + 1; dims from rotary_dim on are not turned.  The angle is
+ * taken in 64 bits and reduced to one turn, the rest is f32, and each result is
+ * rounded once. */
+typedef struct mtt_b200_rotation {
+  int32_t head_dim;        /* 64 or 128 */
+  int32_t rotary_dim;      /* a multiple of 16, at most head_dim */
+  int32_t interleaved;
+  int32_t dtype;           /* MTT_B200_DTYPE_* */
+  const double* turns;     /* [rotary_dim / 2] turns per position */
+  const float* q_weight;   /* [head_dim], 16-byte aligned, or NULL: queries are not normed */
+  const float* k_weight;   /* [head_dim], 16-byte aligned, or NULL: keys are not normed */
+  float eps;               /* >= 0 */
+  int32_t reserved_0;
+} mtt_b200_rotation_t;
+
+/* Rows of queries, keys and values [rows][heads][head_dim], strides in elements
+ * (multiples of 8; 16-byte aligned bases; heads contiguous). */
+typedef struct mtt_b200_rotate_rows {
+  int32_t rows;              /* <= 2^22 */
+  int32_t q_heads;           /* 0: no queries; at most 2^16 heads of each */
+  int32_t kv_heads;          /* 0: no keys (rotate only) */
+  int32_t layer;             /* append only */
+  const void* q;
+  const void* k;
+  const void* v;             /* append only */
+  void* q_out;               /* may be q (with its stride) */
+  void* k_out;               /* rotate only; may be k (with its stride) */
+  int64_t q_row_stride;
+  int64_t k_row_stride;
+  int64_t v_row_stride;
+  int64_t q_out_row_stride;
+  int64_t k_out_row_stride;
+  const int32_t* positions;  /* [rows]; append: or NULL, a token's place in its slot */
+  const int32_t* offsets;    /* append only: as for store */
+} mtt_b200_rotate_rows_t;
+
+/* q_out, k_out = norm and rotation of q, k. */
+MTT_B200_API int mtt_b200_launch_rotate_heads(const mtt_b200_rotation_t* rotation, const mtt_b200_rotate_rows_t* rows,
+                                              void* stream);
+
+/* store with norm and rotation on the way: keys are normed, turned and written
+ * to their pages with their values, queries normed and turned into q_out.  It
+ * leaves what mtt_b200_launch_rotate_heads and store would, bit for bit.  A row
+ * that no slot has, or whose slot was refused its tokens or has fewer than
+ * rows, gets zeros in q_out; status as for store. */
+MTT_B200_API int mtt_b200_launch_paged_cache_append(const mtt_b200_paged_cache_t* cache,
+                                                    const mtt_b200_rotation_t* rotation,
+                                                    const mtt_b200_rotate_rows_t* rows, void* stream);
+
 /* Attention of query rows over one layer of the cache.  A query at position p
  * of its slot sees key j when j <= p and (window 0, p - j < window, or j <
  * sinks) and key_mask[slot][j] (where given):
@@ -846,6 +926,10 @@ MTT_B200_API int mtt_b200_launch_paged_cache_store(const mtt_b200_paged_cache_t*
  * before the first slot's and after the last one's.  Offsets that are not
  * ascending within [0, rows] are not to be given: which rows are then written is
  * not said (none outside [0, rows]).
+ * A 4-bit cache is attended to as if it held the values its codes stand for;
+ * single tokens take them as they are, prompts and shared prefixes round each
+ * once to the cache's type (a further u sum_j p_j |v_j|, and u scale sum_d |q_d
+ * k_jd| in a score).
  * status[i] becomes 4 when a bounded wait inside the prompt kernel gave up (the
  * bounds grow with the keys that the call has to read): the outputs of slot i's
  * rows are then not to be used. */

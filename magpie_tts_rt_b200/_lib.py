@@ -174,6 +174,7 @@ class SessionEngineBuffers(ctypes.Structure):
 
 DTYPE_BF16 = 0
 DTYPE_F16 = 1
+CACHE_4BIT = 0x100
 
 
 class PagedCache(ctypes.Structure):
@@ -186,6 +187,17 @@ class CacheRows(ctypes.Structure):
     _fields_ = [("layer", I32), ("n_layers", I32), ("rows", I32), ("reserved_0", I32), ("k", P), ("v", P),
                 ("k_row_stride", I64), ("v_row_stride", I64), ("k_layer_stride", I64), ("v_layer_stride", I64),
                 ("offsets", P)]
+
+
+class Rotation(ctypes.Structure):
+    _fields_ = [("head_dim", I32), ("rotary_dim", I32), ("interleaved", I32), ("dtype", I32), ("turns", P), ("q_weight", P),
+                ("k_weight", P), ("eps", ctypes.c_float), ("reserved_0", I32)]
+
+
+class RotateRows(ctypes.Structure):
+    _fields_ = [("rows", I32), ("q_heads", I32), ("kv_heads", I32), ("layer", I32), ("q", P), ("k", P), ("v", P),
+                ("q_out", P), ("k_out", P), ("q_row_stride", I64), ("k_row_stride", I64), ("v_row_stride", I64),
+                ("q_out_row_stride", I64), ("k_out_row_stride", I64), ("positions", P), ("offsets", P)]
 
 
 class CacheAttention(ctypes.Structure):
@@ -236,6 +248,11 @@ SIGNATURES = {
     "mtt_b200_launch_paged_cache_compact": (I32, [ctypes.POINTER(PagedCache), P, SZ, P]),
     "mtt_b200_launch_paged_cache_store": (
         I32, [ctypes.POINTER(PagedCache), ctypes.POINTER(CacheRows), P]),
+    "mtt_b200_launch_paged_cache_load": (
+        I32, [ctypes.POINTER(PagedCache), ctypes.POINTER(CacheRows), P]),
+    "mtt_b200_launch_rotate_heads": (I32, [ctypes.POINTER(Rotation), ctypes.POINTER(RotateRows), P]),
+    "mtt_b200_launch_paged_cache_append": (
+        I32, [ctypes.POINTER(PagedCache), ctypes.POINTER(Rotation), ctypes.POINTER(RotateRows), P]),
     "mtt_b200_launch_paged_attention": (
         I32, [ctypes.POINTER(PagedCache), ctypes.POINTER(CacheAttention), P, SZ, P]),
     "mtt_b200_paged_shared_workspace_size": (SZ, [ctypes.POINTER(PagedCache), I32, I32]),

@@ -1,0 +1,168 @@
+// The 4-bit form of the paged cache's pool (MTT_B200_CACHE_4BIT): where a
+// token's codes and (step, low) pairs lie, and how they are made from 16-bit
+// values and turned back into them.
+#pragma once
+
+#include "paged_attention.cuh"
+
+namespace mtt {
+
+constexpr int kGroup4 = 64;  // dims that share a pair
+
+// Bytes of one head's block in a page; of them the codes' come first.
+__device__ __forceinline__ int block4_bytes(const PagedCache& c) { return c.page_size * 9 * c.head_dim / 16; }
+__device__ __forceinline__ int block4_codes(const PagedCache& c) { return c.page_size * c.head_dim / 2; }
+
+// The block of (page, layer, keys or values, head).
+__device__ __forceinline__ unsigned char* block4(const PagedCache& c, int page, int layer, int kv, int head) {
+  return reinterpret_cast<unsigned char*>(c.pool + c.block(page, layer, kv)) + static_cast<int64_t>(head) * block4_bytes(c);
+}
+
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t v);
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v) {
+  return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+}
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t v) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&v));
+}
+
+// Two 16-bit minima or maxima; NaN if either is.
+template <typename T>
+__device__ __forceinline__ uint32_t min2(uint32_t a, uint32_t b);
+template <typename T>
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b);
+template <>
+__device__ __forceinline__ uint32_t min2<__nv_bfloat16>(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+template <>
+__device__ __forceinline__ uint32_t max2<__nv_bfloat16>(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+template <>
+__device__ __forceinline__ uint32_t min2<__half>(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+template <>
+__device__ __forceinline__ uint32_t max2<__half>(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
+// Smallest and largest of a group so far, in two lanes of 16 bits each.
+template <typename T>
+struct Extent4 {
+  uint32_t low, high;
+  __device__ __forceinline__ void take(const uint4& x) {
+    low = min2<T>(low, min2<T>(min2<T>(x.x, x.y), min2<T>(x.z, x.w)));
+    high = max2<T>(high, max2<T>(max2<T>(x.x, x.y), max2<T>(x.z, x.w)));
+  }
+  __device__ __forceinline__ void join(int lanes) {  // with the lanes that differ in these bits of their number
+    for (int o = 1; o < lanes; o <<= 1) {
+      low = min2<T>(low, __shfl_xor_sync(0xffffffffu, low, o));
+      high = max2<T>(high, __shfl_xor_sync(0xffffffffu, high, o));
+    }
+  }
+  static __device__ __forceinline__ Extent4 of(const uint4& x) {
+    return {min2<T>(min2<T>(x.x, x.y), min2<T>(x.z, x.w)), max2<T>(max2<T>(x.x, x.y), max2<T>(x.z, x.w))};
+  }
+};
+
+// A group's pair, and what its codes are chosen with.  Every operation is
+// rounded as the format says (no contraction): the codes do not depend on which
+// kernel stores a token.
+template <typename T>
+struct Pair4 {
+  float low, inverse;
+  uint32_t bits;  // step, low
+  __device__ __forceinline__ explicit Pair4(const Extent4<T>& e) {
+    low = unpack2<T>(min2<T>(e.low, e.low >> 16 | e.low << 16)).x;
+    const float high = unpack2<T>(max2<T>(e.high, e.high >> 16 | e.high << 16)).x;
+    const float spread = __fsub_rn(high, low);
+    // not finite: the whole group reads as NaN
+    const float wide = spread <= 3.402823466e38f ? __fdiv_rn(spread, 15.f) : CUDART_NAN_F;
+    bits = Half16<T>::pack(wide, low);
+    const float step = unpack2<T>(bits).x;
+    inverse = step >= 1.17549435e-38f ? __frcp_rn(step) : 0.f;
+  }
+  // the codes of 8 values
+  __device__ __forceinline__ uint32_t codes(const uint4& x) const {
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    uint32_t r = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 v = unpack2<T>(w[i]);
+      r |= code(v.x) << (4 * i) | code(v.y) << (4 * i + 16);
+    }
+    return r;
+  }
+  __device__ __forceinline__ uint32_t code(float x) const {
+    const float at = fminf(fmaxf(__fmul_rn(__fsub_rn(x, low), inverse), 0.f), 15.f);  // 0 for a NaN
+    return __float_as_uint(__fadd_rn(at, 12582912.f)) & 15u;  // 1.5 * 2^23: rounds to a whole number, half to even
+  }
+};
+
+// The values of 8 codes, rounded to 16 bits.
+template <typename T>
+__device__ __forceinline__ uint4 values4(uint32_t codes, uint32_t pair) {
+  const float2 p = unpack2<T>(pair);
+  uint32_t r[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    r[i] = Half16<T>::pack(fmaf(static_cast<float>((codes >> (4 * i)) & 15u), p.x, p.y),
+                           fmaf(static_cast<float>((codes >> (4 * i + 16)) & 15u), p.x, p.y));
+  return make_uint4(r[0], r[1], r[2], r[3]);
+}
+
+// Codes of dims 2 I and 2 I + 1 of the eight in w, as 16 + code in 16 bits each:
+// the code goes into the upper mantissa bits of 16.0, so that it takes a shift and
+// one three-input operation, and nothing is rounded.
+template <typename T, int I>
+__device__ __forceinline__ uint32_t codes2(uint32_t w) {
+  if constexpr (std::is_same_v<T, __half>) {
+    const uint32_t x = I == 0 ? w << 6 : I == 1 ? w << 2 : w >> (4 * I - 6);
+    return (x & 0x03c003c0u) | 0x4c004c00u;
+  } else {
+    const uint32_t x = I == 0 ? w << 3 : w >> (4 * I - 3);
+    return (x & 0x00780078u) | 0x41804180u;
+  }
+}
+
+// value = low + step * (codes2 - 16), two at a time: the subtraction is exact, the
+// rest rounded once.  step2, low2: step and low twice.
+template <typename T>
+__device__ __forceinline__ uint32_t value2(uint32_t c16, uint32_t step2, uint32_t low2);
+template <>
+__device__ __forceinline__ uint32_t value2<__nv_bfloat16>(uint32_t c16, uint32_t step2, uint32_t low2) {
+  uint32_t r;
+  asm("{\n .reg .b32 c;\n add.rn.bf16x2 c, %1, %4;\n fma.rn.bf16x2 %0, c, %2, %3;\n}\n"
+      : "=r"(r) : "r"(c16), "r"(step2), "r"(low2), "r"(0xc180c180u));
+  return r;
+}
+template <>
+__device__ __forceinline__ uint32_t value2<__half>(uint32_t c16, uint32_t step2, uint32_t low2) {
+  uint32_t r;
+  asm("{\n .reg .b32 c;\n add.rn.f16x2 c, %1, %4;\n fma.rn.f16x2 %0, c, %2, %3;\n}\n"
+      : "=r"(r) : "r"(c16), "r"(step2), "r"(low2), "r"(0xcc00cc00u));
+  return r;
+}
+
+// Where a token's 8 dims from 8 * piece on, and the pair of its group, lie in its block.
+__device__ __forceinline__ uint32_t* codes_at(const PagedCache& c, unsigned char* block, int in_page, int piece) {
+  return reinterpret_cast<uint32_t*>(block + in_page * (c.head_dim / 2)) + piece;
+}
+__device__ __forceinline__ uint32_t* pair_at(const PagedCache& c, unsigned char* block, int in_page, int group) {
+  return reinterpret_cast<uint32_t*>(block + block4_codes(c)) + in_page * (c.head_dim / kGroup4) + group;
+}
+
+}  // namespace mtt

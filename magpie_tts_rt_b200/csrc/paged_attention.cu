@@ -61,9 +61,9 @@ int attend(const mtt_b200_paged_cache_t* cache, const mtt_b200_cache_attention_t
   void* space = paged_attention_space(*cache, a.q_heads, a.rows, workspace, workspace_bytes);
   if (space == nullptr) return MTT_B200_STATUS_INVALID_ARGUMENT;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (a.offsets == nullptr) return cache_call_status(launch_step(c, cache->dtype, a, SharedPrefix{}, space, s));
+  if (a.offsets == nullptr) return cache_call_status(launch_step(c, c.dtype, a, SharedPrefix{}, space, s));
   return cache_call_status(
-      launch_prompt(c, cache->dtype, a, static_cast<char*>(space) + step_workspace(*cache, a.q_heads), waits, s));
+      launch_prompt(c, c.dtype, a, static_cast<char*>(space) + step_workspace(*cache, a.q_heads), waits, s));
 }
 
 int attend_shared(const mtt_b200_paged_cache_t* cache, const mtt_b200_cache_attention_t* args,
@@ -90,13 +90,13 @@ int attend_shared(const mtt_b200_paged_cache_t* cache, const mtt_b200_cache_atte
       return MTT_B200_STATUS_INVALID_ARGUMENT;
     int32_t* base = reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + plain);
     float* state = reinterpret_cast<float*>(static_cast<char*>(workspace) + plain + base_bytes(*cache));
-    const cudaError_t e = launch_prefix(c, cache->dtype, a, *groups, base, state,
+    const cudaError_t e = launch_prefix(c, c.dtype, a, *groups, base, state,
                                         static_cast<char*>(space) + step_workspace(*cache, a.q_heads), waits, s);
     if (e != cudaSuccess) return cache_call_status(e);
     shared.base = base;
     shared.state = state;
   }
-  return cache_call_status(launch_step(c, cache->dtype, a, shared, space, s));
+  return cache_call_status(launch_step(c, c.dtype, a, shared, space, s));
 }
 
 }  // namespace

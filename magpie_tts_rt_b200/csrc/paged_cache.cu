@@ -363,31 +363,14 @@ struct Rows {
 __global__ void __launch_bounds__(kMoveThreads) store_kernel(PagedCache c, Rows in) {
   take_turn();
   const int row = blockIdx.x;
-  int slot = row, count = 1, first = row;
-  if (in.offsets != nullptr) {
-    // the slot with offsets[slot] <= row < offsets[slot + 1]
-    int lo = 0, hi = c.slots;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (in.offsets[mid + 1] > row) hi = mid; else lo = mid + 1;
-    }
-    slot = lo;
-    if (slot >= c.slots) return;
-    first = in.offsets[slot];
-    count = in.offsets[slot + 1] - first;
-    if (first < 0 || first > row || in.offsets[slot + 1] > in.rows) {
-      if (threadIdx.x == 0 && c.status != nullptr) c.status[slot] = 1;
-      return;
-    }
-  }
-  const int len = c.length(slot);
-  if (in.offsets == nullptr && len == 0) return;
-  if (c.refused != nullptr && c.refused[slot] != 0) return;  // its last tokens are not the rows'
-  if (count > len) {
+  const RowPlace at(c, in.offsets, in.rows, row);
+  const int slot = at.slot, t = at.pos;
+  if (t < 0 && at.unfit == 0) return;
+  if (at.unfit != 2 && c.refused != nullptr && c.refused[slot] != 0) return;  // its last tokens are not the rows'
+  if (at.unfit != 0) {
     if (threadIdx.x == 0 && c.status != nullptr) c.status[slot] = 1;
     return;
   }
-  const int t = len - count + row - first;
   const int page = c.table[static_cast<int64_t>(slot) * c.table_pages + (t >> c.page_shift)];
   if (!c.is_page(page) || c.refs[page] > 1) {
     if (threadIdx.x == 0 && c.status != nullptr) c.status[slot] = 3;
@@ -454,7 +437,7 @@ bool paged_cache_view(const mtt_b200_paged_cache_t* c, PagedCache* out) {
   if (c == nullptr || c->pages < 1 || c->layers < 1 || c->kv_heads < 1 || c->slots < 1 || c->slots > kCacheMaxSlots ||
       c->table_pages < 1 || (c->head_dim != 64 && c->head_dim != 128) ||
       (c->page_size != 16 && c->page_size != 32 && c->page_size != 64 && c->page_size != 128) ||
-      (c->dtype != MTT_B200_DTYPE_BF16 && c->dtype != MTT_B200_DTYPE_F16))
+      ((c->dtype & ~MTT_B200_CACHE_4BIT) != MTT_B200_DTYPE_BF16 && (c->dtype & ~MTT_B200_CACHE_4BIT) != MTT_B200_DTYPE_F16))
     return false;
   // rows of the pool (one token's keys or values of one head) and tokens of a slot are counted in 31 bits
   const double rows = static_cast<double>(c->pages) * c->layers * 2 * c->kv_heads * c->page_size;
@@ -472,7 +455,10 @@ bool paged_cache_view(const mtt_b200_paged_cache_t* c, PagedCache* out) {
   out->head_dim = c->head_dim;
   out->slots = c->slots;
   out->table_pages = c->table_pages;
-  out->kv_elems = static_cast<int64_t>(c->kv_heads) * c->page_size * c->head_dim;
+  out->dtype = c->dtype & ~MTT_B200_CACHE_4BIT;
+  out->bits = out->dtype == c->dtype ? 16 : 4;
+  // of 4 bits: 9 bytes for 16 dims (codes, and a pair for every 64)
+  out->kv_elems = static_cast<int64_t>(c->kv_heads) * c->page_size * (out->bits == 16 ? c->head_dim : 9 * c->head_dim / 32);
   out->pool = static_cast<uint16_t*>(c->pool);
   out->table = c->page_table;
   out->lengths = c->lengths;
@@ -570,14 +556,9 @@ int mtt_b200_launch_paged_cache_compact(const mtt_b200_paged_cache_t* cache, voi
 int mtt_b200_launch_paged_cache_store(const mtt_b200_paged_cache_t* cache, const mtt_b200_cache_rows_t* rows,
                                       void* stream) {
   PagedCache c;
-  if (rows == nullptr || !paged_cache_view(cache, &c) || rows->rows < 0 || rows->layer < 0 || rows->n_layers < 1 ||
-      rows->n_layers > c.layers - rows->layer)
-    return MTT_B200_STATUS_INVALID_ARGUMENT;
+  if (rows == nullptr || !paged_cache_view(cache, &c) || !rows_checked(c, rows)) return MTT_B200_STATUS_INVALID_ARGUMENT;
   if (rows->rows == 0) return MTT_B200_STATUS_OK;
-  if (rows->k == nullptr || rows->v == nullptr || !aligned16(rows->k) || !aligned16(rows->v) ||
-      (rows->k_row_stride | rows->v_row_stride | rows->k_layer_stride | rows->v_layer_stride) % 8 != 0 ||
-      (rows->offsets == nullptr && rows->rows > c.slots))
-    return MTT_B200_STATUS_INVALID_ARGUMENT;
+  if (c.bits == 4) return store4(c, *rows, static_cast<cudaStream_t>(stream));
   Rows in{rows->layer, rows->n_layers, rows->rows, static_cast<const uint16_t*>(rows->k),
           static_cast<const uint16_t*>(rows->v), rows->k_row_stride, rows->v_row_stride, rows->k_layer_stride,
           rows->v_layer_stride, rows->offsets};

@@ -66,8 +66,8 @@
 #include <atomic>
 #include <type_traits>
 
+#include "cache4.cuh"
 #include "gemm_tc.cuh"
-#include "paged_attention.cuh"
 
 namespace mtt {
 namespace {
@@ -493,7 +493,49 @@ __device__ __forceinline__ KeySpan unit_span(const Walk& w, bool prefix, int tq,
   return KeySpan(p0, max(p0, p1), a.window, a.sinks);
 }
 
+// Converter of one half of the ring's tiles (keys or values) of a 4-bit pool: a
+// warp reads 16 tokens' codes at a time, two lanes a token, makes 16-bit values of
+// them and writes them as TMA would have (128-byte swizzle).  A piece of 16 tokens is
+// asked for a whole tile before it is converted.
 template <typename T, int D>
+struct Convert4 {
+  static constexpr int DB = D / 64, kPieces = kKeys / 16;
+  uint4 codes[kPieces][DB];
+  uint32_t pair[kPieces][DB];
+
+  // tokens 16 * piece .. of the tile at key `base`, from the page that holds them;
+  // `keep`: whether the lane's token is to be read
+  __device__ __forceinline__ void ask(const PagedCache& c, int piece, int page, int layer, int kv, int head, int base, bool keep) {
+    const int lane = threadIdx.x & 31, in_page = (base + 16 * piece + (lane >> 1)) & (c.page_size - 1);
+    const unsigned char* block = block4(c, page, layer, kv, head);
+    keep = keep && c.is_page(page);
+#pragma unroll
+    for (int b = 0; b < DB; ++b) {
+      codes[piece][b] = make_uint4(0, 0, 0, 0);
+      pair[piece][b] = 0;
+      if (keep) {
+        codes[piece][b] = *reinterpret_cast<const uint4*>(block + in_page * (D / 2) + 32 * b + 16 * (lane & 1));
+        pair[piece][b] = *(reinterpret_cast<const uint32_t*>(block + block4_codes(c)) + in_page * DB + b);
+      }
+    }
+  }
+  __device__ __forceinline__ void put(int piece, unsigned char* tile) const {
+    const int lane = threadIdx.x & 31, row = 16 * piece + (lane >> 1);
+#pragma unroll
+    for (int b = 0; b < DB; ++b) {
+      const uint32_t step2 = __byte_perm(pair[piece][b], 0, 0x1010), low2 = __byte_perm(pair[piece][b], 0, 0x3232);
+      const uint32_t w[4] = {codes[piece][b].x, codes[piece][b].y, codes[piece][b].z, codes[piece][b].w};
+      unsigned char* to = tile + b * (kKeys * 128) + row * 128;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        *reinterpret_cast<uint4*>(to + 16 * ((4 * (lane & 1) + k) ^ (row & 7))) =
+            make_uint4(value2<T>(codes2<T, 0>(w[k]), step2, low2), value2<T>(codes2<T, 1>(w[k]), step2, low2),
+                       value2<T>(codes2<T, 2>(w[k]), step2, low2), value2<T>(codes2<T, 3>(w[k]), step2, low2));
+    }
+  }
+};
+
+template <typename T, int D, int Bits>
 __global__ void __launch_bounds__(kPromptThreads, 1)
     prompt_kernel(const __grid_constant__ CUtensorMap pool_map, const __grid_constant__ CUtensorMap q_map, PagedCache c, Attend a, PromptRows rows,
                   PromptSpace ws) {
@@ -538,7 +580,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     tmem_alloc(&tmem_base, 512);
     tmem_relinquish();
   }
-  if (warp == 9 && lane == 0)
+  if (Bits == 16 && warp == 9 && lane == 0)
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&pool_map)) : "memory");
   tmem_fence_before_sync();
   __syncthreads();
@@ -559,7 +601,53 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   if (threadIdx.x == 0) wait_limit = ws.waits.ns + static_cast<unsigned long long>(ws.waits.tile_ns) * (any ? w.end : 0);
   __syncthreads();
 
-  if (warp == 9) {
+  if (Bits == 4 && (warp == 9 || warp == 10)) {
+    // ---- 4-bit pool: warp 9 fills the ring's key tiles (the even places), warp 10 its value tiles.  Values that no query
+    // of the unit may see are zeros.
+    const int kv = warp - 9;
+    int it = kv;
+    for (bool more = any && !ws.waits.starve; more && alive(errv); more = w.next(ws)) {
+      const Geom g = w.g;
+      const KeySpan span = unit_span(w, prefix, tq, a);
+      const int32_t* table = c.table + static_cast<int64_t>(g.key_slot) * c.table_pages;
+      const bool* mask = a.key_mask != nullptr ? a.key_mask + g.key_slot * a.mask_stride : nullptr;
+      int p0, p1;
+      positions(g, prefix, w.tok0, w.tok0 + 2 * tq, &p0, &p1);
+      Convert4<T, D> x;
+      // the page of lane's 16 tokens of tile t
+      auto page_of = [&](int t) {
+        const int key = kKeys * span.tile(t) + 16 * lane;
+        return lane < x.kPieces && t < w.t1 && key < g.len ? table[key >> c.page_shift] : -1;
+      };
+      auto ask = [&](int piece, int t, int page) {
+        const int base = kKeys * span.tile(t), j = base + 16 * piece + (lane >> 1);
+        bool keep = j < g.len;
+        if (kv == 1) keep = j <= p1 && (a.window == 0 || j > p0 - a.window || j < a.sinks) && (mask == nullptr || mask[j]);
+        x.ask(c, piece, __shfl_sync(0xffffffffu, page, piece), a.layer, kv, w.head, base, keep);
+      };
+      int page = page_of(w.t0), next_page = page_of(w.t0 + 1);
+#pragma unroll
+      for (int i = 0; i < x.kPieces; ++i) ask(i, w.t0, page);
+      bool ok = true;
+      for (int t = w.t0; ok && t < w.t1; ++t, it += 2) {
+        page = next_page;
+        next_page = page_of(t + 2);
+        const int s = it % S;
+        ok = it < S || patience.wait(&kv_empty[s], ((it / S) - 1) & 1);
+        if (!ok) break;
+        unsigned char* tile = ring + static_cast<size_t>(s) * C::kTileBytes;
+#pragma unroll
+        for (int i = 0; i < x.kPieces; ++i) {
+          x.put(i, tile);
+          ask(i, t + 1, page);
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ready[s]);
+      }
+      if (!ok) *errv = 1;
+    }
+  } else if (warp == 9) {
     // ---- TMA producer.  Order: keys 0, then values t, keys t + 1, as they are used.
     int it = 0;
     const int rows_per_box = min(kKeys, c.page_size), boxes = kKeys / rows_per_box;
@@ -1248,10 +1336,9 @@ bool query_map(const PagedCache& c, int dtype, const Attend& a, CUtensorMap* map
 cudaError_t run_prompt(const PagedCache& c, int dtype, const Attend& a, PromptRows rows, void* space,
                        const Waits& waits, cudaStream_t stream) {
   const int sms = cache_sm_count();
-  CUtensorMap map, q_map;
-  if (sms <= 0 || sms > kMaxSms || !pool_map(c, dtype, &map)) return cudaErrorInvalidValue;
+  CUtensorMap map{}, q_map{};  // one that is not made is not read
+  if (sms <= 0 || sms > kMaxSms || (c.bits == 16 && !pool_map(c, dtype, &map))) return cudaErrorInvalidValue;
   rows.q_mapped = rows.members == nullptr && query_map(c, dtype, a, &q_map);
-  if (!rows.q_mapped) q_map = map;  // not read
   const int tokens_per_pair = 2 * (kTile / a.group);
   rows.own_plan = rows.n_rows / tokens_per_pair + rows.n <= kPromptThreads;
   const PromptLayout at(rows.n, rows.n_rows, a.group, c.head_dim);
@@ -1264,10 +1351,10 @@ cudaError_t run_prompt(const PagedCache& c, int dtype, const Attend& a, PromptRo
   ws.rec = reinterpret_cast<int4*>(base + at.rec);
   ws.part = reinterpret_cast<float*>(base + at.part);
   ws.waits = waits;
-  auto go = [&](auto type, auto dim) {
+  auto go = [&](auto type, auto dim, auto bits) {
     using T = decltype(type);
-    constexpr int D = decltype(dim)::value;
-    const auto kernel = prompt_kernel<T, D>;
+    constexpr int D = decltype(dim)::value, Bits = decltype(bits)::value;
+    const auto kernel = prompt_kernel<T, D, Bits>;
     constexpr size_t smem = PromptCfg<D>::kSmem;
     static std::atomic<uint64_t> opted_in;  // devices on which this kernel has its shared memory
     int dev = 0;
@@ -1284,10 +1371,14 @@ cudaError_t run_prompt(const PagedCache& c, int dtype, const Attend& a, PromptRo
       e = launch_serialized(prompt_join_kernel<T, D>, dim3(4 * sms), dim3(kJoinThreads), 0, stream, c, a, rows, ws, sms);
     return e;
   };
-  auto pick = [&](auto type) {
-    return c.head_dim == 64 ? go(type, std::integral_constant<int, 64>{}) : go(type, std::integral_constant<int, 128>{});
+  auto pick = [&](auto type, auto bits) {
+    return c.head_dim == 64 ? go(type, std::integral_constant<int, 64>{}, bits)
+                            : go(type, std::integral_constant<int, 128>{}, bits);
   };
-  return dtype == MTT_B200_DTYPE_BF16 ? pick(__nv_bfloat16{}) : pick(__half{});
+  auto with_bits = [&](auto type) {
+    return c.bits == 4 ? pick(type, std::integral_constant<int, 4>{}) : pick(type, std::integral_constant<int, 16>{});
+  };
+  return dtype == MTT_B200_DTYPE_BF16 ? with_bits(__nv_bfloat16{}) : with_bits(__half{});
 }
 
 }  // namespace

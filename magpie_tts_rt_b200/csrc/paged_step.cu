@@ -38,7 +38,7 @@
 #include <atomic>
 #include <type_traits>
 
-#include "paged_attention.cuh"
+#include "cache4.cuh"
 
 namespace mtt {
 namespace {
@@ -46,7 +46,8 @@ namespace {
 constexpr int kStepWarps = 4;
 constexpr int kStepThreads = 32 * kStepWarps;
 
-constexpr int step_tiles(int head_dim) { return head_dim == 64 ? 2 : 1; }  // 16-key tiles per warp and step
+// 16-key tiles per warp and step
+constexpr int step_tiles(int head_dim, int bits) { return (head_dim == 64 ? 2 : 1) * (bits == 4 ? 2 : 1); }
 constexpr int step_ctas(int head_dim, int nb) { return (head_dim == 64 ? 4 : 3) - (nb == 2 ? 1 : 0); }  // per SM (registers)
 
 // A unit's place on the line: its tiles, and before them what entering and
@@ -162,9 +163,9 @@ struct StepSums {
 template <typename T, int D, int NB>
 __device__ __forceinline__ void attend_tiles(const PagedCache& c, const Attend& a, const SeenTiles& seen,
                                              const int32_t* row, const bool* mask, int64_t head_at, int t0, int t1,
-                                             const uint4 (&q)[NB][D / 32], int (&page)[step_tiles(D)],
+                                             const uint4 (&q)[NB][D / 32], int (&page)[step_tiles(D, 16)],
                                              StepSums<D, NB>& sums) {
-  constexpr int NT = step_tiles(D);
+  constexpr int NT = step_tiles(D, 16);
   constexpr int KC = D / 32;  // 16-byte pieces of a key row per thread
   constexpr int VC = D / 64;  // of a value row
   const int lane = threadIdx.x & 31, t = lane & 3, g = lane >> 2;
@@ -284,10 +285,234 @@ __device__ __forceinline__ void attend_tiles(const PagedCache& c, const Attend& 
   }
 }
 
+// 4 or 8 bytes, as load16.
+__device__ __forceinline__ uint32_t load4(const unsigned char* p, bool on) {
+  uint32_t v = 0;
+  if (on) asm volatile("ld.global.L1::no_allocate.u32 %0, [%1];" : "=r"(v) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint2 load8(const unsigned char* p, bool on) {
+  uint2 v = make_uint2(0, 0);
+  if (on) asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  return v;
+}
+
+// step, and what belongs to 16 + code: value = step (16 + code) + off
+__device__ __forceinline__ float2 step_off(float2 pair) { return make_float2(pair.x, fmaf(-16.f, pair.x, pair.y)); }
+
+// The first of the 8 dims that piece k of a thread's queries holds, as its keys do.
+template <int Bits>
+__device__ __forceinline__ int step_dims(int t, int k) {
+  return Bits == 16 ? 32 * k + 8 * t : 64 * (k >> 1) + 16 * t + 8 * (k & 1);
+}
+
+// attend_tiles for a cache in 4 bits.  Nothing is rounded on the way into the
+// products: a code is a small whole number, exact in either 16-bit type, and the
+// pairs come in afterwards, in f32,
+//   q.k = sum over groups: step (q.(16 + c)) + off sum q,   off = low - 16 step;
+// the values' weights are p step, in two bf16 numbers each (their range is not
+// f16's), and p off is summed by itself.
 template <typename T, int D, int NB>
+__device__ __forceinline__ void attend_tiles4(const PagedCache& c, const Attend& a, const SeenTiles& seen,
+                                              const int32_t* row, const bool* mask, int head, int t0, int t1,
+                                              const uint4 (&q)[NB][D / 32], int (&page)[step_tiles(D, 4)],
+                                              StepSums<D, NB>& sums) {
+  using B = __nv_bfloat16;
+  constexpr int NT = step_tiles(D, 4);
+  constexpr int G = D / kGroup4;
+  const int lane = threadIdx.x & 31, t = lane & 3, g = lane >> 2;
+  auto& [m, l, acc] = sums;
+  // the queries' sums over each group
+  float qs[NB][G][2], rest[NB][G][2];
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int v = 0; v < G; ++v) {
+      float sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const uint4& x = q[b][2 * v + k];
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 f = unpack2<T>(w[i]);
+          sum += f.x + f.y;
+        }
+      }
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        qs[b][v][i] = __shfl_sync(0xffffffffu, sum, 4 * (2 * t + i));
+        rest[b][v][i] = 0.f;
+      }
+    }
+  for (int base = t0; base < t1; base += NT) {
+    // keys in reach: one per lane and pair of tiles
+    uint32_t bits[NT / 2];
+#pragma unroll
+    for (int u = 0; u < NT / 2; ++u) {
+      const int my_tile = base + 2 * u + (lane >> 4), j = 16 * seen.tile(my_tile) + (lane & 15);
+      bool in = my_tile < t1 && j < seen.len && (j >= seen.low || j < a.sinks);
+      if (in && mask != nullptr) in = mask[j];
+      bits[u] = __ballot_sync(0xffffffffu, in);
+    }
+    uint2 kr[NT][2][G];
+    uint32_t vr[NT][4][G], kp[NT][2][G], vp[NT][2][G], on[NT];
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+      on[u] = c.is_page(page[u]) ? (bits[u >> 1] >> (16 * (u & 1))) & 0xffffu : 0u;
+      const int in_page = (16 * seen.tile(base + u)) & (c.page_size - 1);
+      const unsigned char* kb = block4(c, page[u], a.layer, 0, head);
+      const unsigned char* vb = kb + 2 * c.kv_elems;
+      const int pairs = block4_codes(c);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int key = in_page + g + 8 * h;
+        const bool there = (on[u] >> (g + 8 * h)) & 1u;
+#pragma unroll
+        for (int v = 0; v < G; ++v) kr[u][h][v] = load8(kb + key * (D / 2) + 32 * v + 8 * t, there);
+        if constexpr (G == 1) {
+          kp[u][h][0] = load4(kb + pairs + 4 * key, there);
+          vp[u][h][0] = load4(vb + pairs + 4 * key, there);
+        } else {
+          const uint2 x = load8(kb + pairs + 8 * key, there), y = load8(vb + pairs + 8 * key, there);
+          kp[u][h][0] = x.x;
+          kp[u][h][1] = x.y;
+          vp[u][h][0] = y.x;
+          vp[u][h][1] = y.y;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = 2 * t + (i & 1) + 8 * (i >> 1);
+#pragma unroll
+        for (int v = 0; v < G; ++v) vr[u][i][v] = load4(vb + (in_page + key) * (D / 2) + 32 * v + 4 * g, (on[u] >> key) & 1u);
+      }
+    }
+    // the next step's pages, while this step's keys arrive
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+      const int tt = base + NT + u;
+      page[u] = tt < t1 ? row[(16 * seen.tile(tt)) >> c.page_shift] : -1;
+    }
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      float s[NT][4];
+      float top0 = m[b][0], top1 = m[b][1];
+#pragma unroll
+      for (int u = 0; u < NT; ++u) {
+        s[u][0] = s[u][1] = s[u][2] = s[u][3] = 0.f;
+#pragma unroll
+        for (int v = 0; v < G; ++v) {
+          float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const uint32_t w0 = k == 0 ? kr[u][0][v].x : kr[u][0][v].y, w1 = k == 0 ? kr[u][1][v].x : kr[u][1][v].y;
+            const uint4& y = q[b][2 * v + k];
+            Half16<T>::mma(x, codes2<T, 0>(w0), codes2<T, 0>(w1), codes2<T, 1>(w0), codes2<T, 1>(w1), y.x, y.y);
+            Half16<T>::mma(x, codes2<T, 2>(w0), codes2<T, 2>(w1), codes2<T, 3>(w0), codes2<T, 3>(w1), y.z, y.w);
+          }
+          const float2 lo = step_off(unpack2<T>(kp[u][0][v])), hi = step_off(unpack2<T>(kp[u][1][v]));
+          s[u][0] = fmaf(lo.x, x[0], fmaf(lo.y, qs[b][v][0], s[u][0]));
+          s[u][1] = fmaf(lo.x, x[1], fmaf(lo.y, qs[b][v][1], s[u][1]));
+          s[u][2] = fmaf(hi.x, x[2], fmaf(hi.y, qs[b][v][0], s[u][2]));
+          s[u][3] = fmaf(hi.x, x[3], fmaf(hi.y, qs[b][v][1], s[u][3]));
+        }
+        const bool lo = (on[u] >> g) & 1u, hi = (on[u] >> (g + 8)) & 1u;
+        s[u][0] = lo ? s[u][0] * a.scale2 : -CUDART_INF_F;
+        s[u][1] = lo ? s[u][1] * a.scale2 : -CUDART_INF_F;
+        s[u][2] = hi ? s[u][2] * a.scale2 : -CUDART_INF_F;
+        s[u][3] = hi ? s[u][3] * a.scale2 : -CUDART_INF_F;
+        top0 = fmaxf(top0, fmaxf(s[u][0], s[u][2]));
+        top1 = fmaxf(top1, fmaxf(s[u][1], s[u][3]));
+      }
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) {
+        top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, o));
+        top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, o));
+      }
+      const float z0 = top0 == -CUDART_INF_F ? 0.f : top0, z1 = top1 == -CUDART_INF_F ? 0.f : top1;
+      const float keep0 = ex2(m[b][0] - z0), keep1 = ex2(m[b][1] - z1);
+      m[b][0] = top0;
+      m[b][1] = top1;
+      l[b][0] *= keep0;
+      l[b][1] *= keep1;
+#pragma unroll
+      for (int v = 0; v < G; ++v) {
+        rest[b][v][0] *= keep0;
+        rest[b][v][1] *= keep1;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          acc[b][v][w][0] *= keep0;
+          acc[b][v][w][1] *= keep1;
+          acc[b][v][w][2] *= keep0;
+          acc[b][v][w][3] *= keep1;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < NT; ++u) {
+        const float p0 = ex2(s[u][0] - z0), p1 = ex2(s[u][1] - z1), p2 = ex2(s[u][2] - z0), p3 = ex2(s[u][3] - z1);
+        l[b][0] += p0 + p2;
+        l[b][1] += p1 + p3;
+#pragma unroll
+        for (int v = 0; v < G; ++v) {
+          const float2 lo = step_off(unpack2<T>(vp[u][0][v])), hi = step_off(unpack2<T>(vp[u][1][v]));
+          rest[b][v][0] = fmaf(p0, lo.y, fmaf(p2, hi.y, rest[b][v][0]));
+          rest[b][v][1] = fmaf(p1, lo.y, fmaf(p3, hi.y, rest[b][v][1]));
+          const uint2 w0 = Half16<B>::split(p0 * lo.x, p1 * lo.x), w1 = Half16<B>::split(p2 * hi.x, p3 * hi.x);
+          const uint32_t b0 = transpose8x8(w0.x), b1 = transpose8x8(w1.x);
+          const uint32_t rest0 = transpose8x8(w0.y), rest1 = transpose8x8(w1.y);
+          const uint32_t near[2] = {__byte_perm(vr[u][0][v], vr[u][1][v], 0x5410), __byte_perm(vr[u][0][v], vr[u][1][v], 0x7632)};
+          const uint32_t far[2] = {__byte_perm(vr[u][2][v], vr[u][3][v], 0x5410), __byte_perm(vr[u][2][v], vr[u][3][v], 0x7632)};
+          auto dims = [&](auto w) {  // 8g + 2w (row g of the product) and 8g + 2w + 1 (row g + 8)
+            constexpr int W = decltype(w)::value;
+            const uint32_t v0 = codes2<B, W>(near[0]), v1 = codes2<B, W>(near[1]);
+            const uint32_t v2 = codes2<B, W>(far[0]), v3 = codes2<B, W>(far[1]);
+            Half16<B>::mma(acc[b][v][W], v0, v1, v2, v3, b0, b1);
+            Half16<B>::mma(acc[b][v][W], v0, v1, v2, v3, rest0, rest1);
+          };
+          dims(std::integral_constant<int, 0>{});
+          dims(std::integral_constant<int, 1>{});
+          dims(std::integral_constant<int, 2>{});
+          dims(std::integral_constant<int, 3>{});
+        }
+      }
+    }
+  }
+  // the weights' part that belongs to no code is the same for all dims of a group
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int v = 0; v < G; ++v)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float x = rest[b][v][i];
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          acc[b][v][w][i] += x;
+          acc[b][v][w][2 + i] += x;
+        }
+      }
+}
+
+template <typename T, int D, int NB, int Bits>
+__device__ __forceinline__ void attend_tiles_of(const PagedCache& c, const Attend& a, const SeenTiles& seen,
+                                                const int32_t* row, const bool* mask, int head, int t0, int t1,
+                                                const uint4 (&q)[NB][D / 32], int (&page)[step_tiles(D, Bits)],
+                                                StepSums<D, NB>& sums) {
+  if constexpr (Bits == 4)
+    attend_tiles4<T, D, NB>(c, a, seen, row, mask, head, t0, t1, q, page, sums);
+  else
+    attend_tiles<T, D, NB>(c, a, seen, row, mask, static_cast<int64_t>(head) * c.page_size * D, t0, t1, q, page, sums);
+}
+
+template <typename T, int D, int NB, int Bits>
 __global__ void __launch_bounds__(kStepThreads, step_ctas(D, NB))
     step_kernel(PagedCache c, Attend a, SharedPrefix shared, StepSpace ws, int blocks, int min_tiles) {
-  constexpr int NT = step_tiles(D);
+  constexpr int NT = step_tiles(D, Bits);
   constexpr int NQ = 8 * NB;   // query rows of a unit
   constexpr int KC = D / 32, VC = D / 64;
   extern __shared__ int tiles_before[];  // [rows + 1]: tiles of a key head of the slots before
@@ -379,11 +604,11 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(D, NB))
     t0 = static_cast<int>(max(x - unit_x - kUnitCost, static_cast<int64_t>(0)));
     t1 = static_cast<int>(max(min(static_cast<int64_t>(seen.n), x_end - unit_x - kUnitCost), static_cast<int64_t>(0)));
     const int queries = min(NQ, a.group - block * NQ);
-    const int64_t q_at = slot * a.q_row + static_cast<int64_t>(head * a.group + block * NQ + g) * D + 8 * t;
+    const int64_t q_at = slot * a.q_row + static_cast<int64_t>(head * a.group + block * NQ + g) * D;
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
-      for (int k = 0; k < KC; ++k) q[b][k] = load16(a.q + q_at + 8 * b * D + 32 * k, 8 * b + g < queries);
+      for (int k = 0; k < KC; ++k) q[b][k] = load16(a.q + q_at + 8 * b * D + step_dims<Bits>(t, k), 8 * b + g < queries);
     const int32_t* row = c.table + static_cast<int64_t>(slot) * c.table_pages;
 #pragma unroll
     for (int u = 0; u < NT; ++u) page[u] = t0 + u < t1 ? row[(16 * seen.tile(t0 + u)) >> c.page_shift] : -1;
@@ -394,10 +619,9 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(D, NB))
     const int q_head = head * a.group + block * NQ;
     const int32_t* row = c.table + static_cast<int64_t>(slot) * c.table_pages;
     const bool* mask = a.key_mask != nullptr ? a.key_mask + slot * a.mask_stride : nullptr;
-    const int64_t head_at = static_cast<int64_t>(head) * c.page_size * D;
     StepSums<D, NB> sums;
     sums.clear();
-    attend_tiles<T, D, NB>(c, a, seen, row, mask, head_at, t0, t1, q, page, sums);
+    attend_tiles_of<T, D, NB, Bits>(c, a, seen, row, mask, head, t0, t1, q, page, sums);
     auto& [m, l, acc] = sums;
 
     // a thread holds queries 2t, 2t + 1 and dims 8g .. 8g + 7 of each 64
@@ -553,9 +777,9 @@ constexpr int kMaxSpread = 8, kFewSteps = 4;
 
 // 4 CTAs of 4 warps an SM, as head_dim 64 has by itself: 132 registers instead of
 // 128 would let one cluster in four go.
-template <typename T, int D, int NB, int W>
+template <typename T, int D, int NB, int W, int Bits>
 __global__ void __launch_bounds__(32 * W, D == 128 && NB == 1 && W == 4 ? 4 : 0) step_few_kernel(PagedCache c, Attend a, int blocks, int spread) {
-  constexpr int NT = step_tiles(D);
+  constexpr int NT = step_tiles(D, Bits);
   constexpr int NQ = 8 * NB, KC = D / 32, VC = D / 64;
   constexpr int kRow = D + 2;  // weighted values, maximum, sum
   extern __shared__ float few_smem[];
@@ -579,15 +803,15 @@ __global__ void __launch_bounds__(32 * W, D == 128 && NB == 1 && W == 4 ? 4 : 0)
   int page[NT];
 #pragma unroll
   for (int u = 0; u < NT; ++u) page[u] = t0 + u < t1 ? row[(16 * seen.tile(t0 + u)) >> c.page_shift] : -1;
-  const int64_t q_at = slot * a.q_row + static_cast<int64_t>(q_head + g) * D + 8 * t;
+  const int64_t q_at = slot * a.q_row + static_cast<int64_t>(q_head + g) * D;
 #pragma unroll
   for (int b = 0; b < NB; ++b)
 #pragma unroll
-    for (int k = 0; k < KC; ++k) q[b][k] = load16(a.q + q_at + 8 * b * D + 32 * k, 8 * b + g < queries);
+    for (int k = 0; k < KC; ++k) q[b][k] = load16(a.q + q_at + 8 * b * D + step_dims<Bits>(t, k), 8 * b + g < queries);
   StepSums<D, NB> sums;
   sums.clear();
-  attend_tiles<T, D, NB>(c, a, seen, row, a.key_mask != nullptr ? a.key_mask + slot * a.mask_stride : nullptr,
-                         static_cast<int64_t>(head) * c.page_size * D, t0, t1, q, page, sums);
+  attend_tiles_of<T, D, NB, Bits>(c, a, seen, row, a.key_mask != nullptr ? a.key_mask + slot * a.mask_stride : nullptr, head,
+                                  t0, t1, q, page, sums);
   auto& [m, l, acc] = sums;
 #pragma unroll
   for (int b = 0; b < NB; ++b)
@@ -671,13 +895,13 @@ struct FewLaunch {
 
 // Clusters of `Spread` CTAs of the kernel that the current device runs at once
 // (0: cannot be queried).  Nothing here allocates or throws.
-template <typename T, int D, int NB, int W, int Spread>
+template <typename T, int D, int NB, int W, int Spread, int Bits>
 int few_clusters() {
   static std::atomic<int> known[64];  // by device ordinal, plus 1; the opt-in below is per device
   int dev = -1, clusters = 0;
   if (cudaGetDevice(&dev) == cudaSuccess) {
     if (dev >= 0 && dev < 64 && (clusters = known[dev].load(std::memory_order_relaxed)) > 0) return clusters - 1;
-    const auto kernel = step_few_kernel<T, D, NB, W>;
+    const auto kernel = step_few_kernel<T, D, NB, W, Bits>;
     FewLaunch launch(1, Spread, W, few_bytes(D, NB, W), nullptr);
     launch.cfg.numAttrs = 1;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -724,7 +948,7 @@ cudaError_t launch_step(const PagedCache& c, int dtype, const Attend& a, const S
   if (sms <= 0 || sms > kMaxSms) return cudaErrorInvalidValue;
   const size_t smem = 4 * (static_cast<size_t>(a.rows) + 1);
   const int grid = sms * step_ctas(c.head_dim, nb), shares = grid * kStepWarps;
-  const int min_tiles = kUnitCost + step_tiles(c.head_dim);
+  const int min_tiles = kUnitCost + step_tiles(c.head_dim, c.bits);
   const int pairs = std::min(8 * nb, a.group) * c.head_dim / 2;
   auto go = [&](auto kernel, auto join) {
     if (smem > 40 * 1024) {
@@ -747,21 +971,25 @@ cudaError_t launch_step(const PagedCache& c, int dtype, const Attend& a, const S
     const FewLaunch launch(static_cast<int>(units), spread, warps, few_bytes(c.head_dim, nb, warps), stream);
     return cudaLaunchKernelEx(&launch.cfg, kernel, c, a, blocks, spread);
   };
-  auto run = [&](auto type, auto dim, auto bs) {
+  auto with_bits = [&](auto type, auto dim, auto bs, auto bits) {
     using T = decltype(type);
-    constexpr int D = decltype(dim)::value, NB = decltype(bs)::value;
+    constexpr int D = decltype(dim)::value, NB = decltype(bs)::value, Bits = decltype(bits)::value;
     auto fits = [&](int warps, int clusters) {
-      return units <= clusters && reach <= static_cast<int64_t>(kFewSteps) * warps * 16 * step_tiles(D);
+      return units <= clusters && reach <= static_cast<int64_t>(kFewSteps) * warps * 16 * step_tiles(D, Bits);
     };
     if (shared.base == nullptr) {
-      if (reach > 32 * 16 * step_tiles(D) && fits(64, few_clusters<T, D, NB, 8, 8>()))
-        return few(step_few_kernel<T, D, NB, 8>, 8, 8);
-      if (fits(32, few_clusters<T, D, NB, 4, 8>())) return few(step_few_kernel<T, D, NB, 4>, 4, 8);
-      if (fits(16, few_clusters<T, D, NB, 4, 4>())) return few(step_few_kernel<T, D, NB, 4>, 4, 4);
-      if (fits(8, few_clusters<T, D, NB, 4, 2>())) return few(step_few_kernel<T, D, NB, 4>, 4, 2);
-      if (fits(4, few_clusters<T, D, NB, 4, 1>())) return few(step_few_kernel<T, D, NB, 4>, 4, 1);
+      if (reach > 32 * 16 * step_tiles(D, Bits) && fits(64, few_clusters<T, D, NB, 8, 8, Bits>()))
+        return few(step_few_kernel<T, D, NB, 8, Bits>, 8, 8);
+      if (fits(32, few_clusters<T, D, NB, 4, 8, Bits>())) return few(step_few_kernel<T, D, NB, 4, Bits>, 4, 8);
+      if (fits(16, few_clusters<T, D, NB, 4, 4, Bits>())) return few(step_few_kernel<T, D, NB, 4, Bits>, 4, 4);
+      if (fits(8, few_clusters<T, D, NB, 4, 2, Bits>())) return few(step_few_kernel<T, D, NB, 4, Bits>, 4, 2);
+      if (fits(4, few_clusters<T, D, NB, 4, 1, Bits>())) return few(step_few_kernel<T, D, NB, 4, Bits>, 4, 1);
     }
-    return go(step_kernel<T, D, NB>, step_join_kernel<T, D>);
+    return go(step_kernel<T, D, NB, Bits>, step_join_kernel<T, D>);
+  };
+  auto run = [&](auto type, auto dim, auto bs) {
+    return c.bits == 4 ? with_bits(type, dim, bs, std::integral_constant<int, 4>{})
+                       : with_bits(type, dim, bs, std::integral_constant<int, 16>{});
   };
   auto pick = [&](auto type) {
     using std::integral_constant;

@@ -5,7 +5,10 @@ that reads it (C ABI section 7 of include/magpie_tts_rt_b200.h).
 head_dim]`` (keys at index 0, values at 1), a page table and a length per
 slot, and a reference count per page, all on the device:
 
-* ``extend`` / ``store``: room for new tokens, and their keys and values;
+* ``extend`` / ``store`` / ``load``: room for new tokens, their keys and values
+  in, and out again;
+* ``append``: ``store`` with a norm of each head and the position rotation
+  (``rotary.Rotation``) on the way;
 * ``fork``: slots take over other slots' tokens, full pages shared (sessions
   started from one prefilled voice; reordering of slots);
 * ``free`` / ``compact``: slots closed, pages in use moved to the pool's start;
@@ -14,6 +17,11 @@ slot, and a reference count per page, all on the device:
   (``sinks``) that stay visible;
 * ``attend_shared``: the newest tokens' attention where groups of slots share a
   prefix (``PrefixGroups``), computed once for each group.
+
+With ``bits=4`` the pool holds keys and values in 4 bits: 64 dims of a token's
+head share a (step, low) pair of the cache's 16-bit type and are held as
+low + step * code, code 0..15 (4.5 bits a value in all).  Every call above works
+on such a cache.
 
 Every call is enqueued on the current (or given) CUDA stream of the pool's
 device and returns without waiting; no gradient is recorded (this is a decoder's
@@ -48,6 +56,7 @@ MAX_SLOTS = 16384
 MAX_GROUP = 64
 MAX_ROWS = 1 << 22
 MAX_TOKENS = 1 << 30  # more than a slot can have
+GROUP_4BIT = 64  # dims that share a pair in a 4-bit pool
 _DTYPES = {torch.bfloat16: L.DTYPE_BF16, torch.float16: L.DTYPE_F16}
 
 
@@ -70,16 +79,50 @@ def _raw_stream(device: torch.device):
     return raw
 
 
+def _rows_of(t, shape, st, name, dtype, index) -> int:
+    """The stride of t's rows [rows, heads, head_dim]; that of a dimension of
+    one has no meaning and is not looked at."""
+    if t.dtype is not dtype or t.get_device() != index:
+        raise ValueError(f"{name} must have the type and device of the call's other tensors")
+    if st[2] != 1 or (st[1] != shape[2] and shape[1] > 1):
+        raise ValueError(f"{name} must be contiguous in its heads")
+    row = st[0] if shape[0] > 1 else shape[1] * shape[2]
+    if t.data_ptr() % 16 or row % 8:
+        raise ValueError(f"rows of {name} must be 16-byte aligned")
+    return row
+
+
+def _token_bytes(head_dim: int) -> int:
+    """Of one token's keys, or values, of one head in a 4-bit pool."""
+    return head_dim // 2 + head_dim // 16
+
+
 class PagedCache:
-    def __init__(self, pool: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, refs: torch.Tensor):
+    bits = 16  # of a value in the pool
+
+    def __init__(self, pool: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, refs: torch.Tensor,
+                 dtype: Optional[torch.dtype] = None):
         """Adopts the tensors of a cache: pool [pages, layers, 2, kv_heads,
         page_size, head_dim] bf16 or f16, page_table [slots, table_pages] int32
         (-1: no page), lengths [slots] int32, refs [pages] int32; contiguous
-        and on one CUDA device."""
+        and on one CUDA device.  A uint8 pool is one in 4 bits, [pages, layers, 2,
+        kv_heads, page_size, head_dim / 2 + head_dim / 16]: its last two dimensions
+        are a block that holds the codes of its tokens, then their pairs (the
+        header has the order); dtype is then that of keys, values, queries and
+        outputs."""
         _check(pool.is_cuda, "the pool must be a CUDA tensor")
         _check(pool.dim() == 6 and pool.shape[2] == 2, "pool must be [pages, layers, 2, kv_heads, page_size, head_dim]")
-        _check(pool.dtype in _DTYPES, "pool must be bfloat16 or float16")
         pages, layers, _, kv_heads, page_size, head_dim = pool.shape
+        if pool.dtype is torch.uint8:
+            self.bits = 4
+            _check(dtype in _DTYPES, "a 4-bit cache needs a dtype, bfloat16 or float16")
+            _check(any(head_dim == _token_bytes(d) for d in HEAD_DIMS),
+                   "the last dimension of a 4-bit pool must be head_dim / 2 + head_dim / 16")
+            head_dim = head_dim * 16 // 9
+        else:
+            _check(pool.dtype in _DTYPES, "pool must be bfloat16 or float16, or uint8 for 4 bits")
+            _check(dtype is None or dtype is pool.dtype, "dtype must be the pool's")
+            dtype = pool.dtype
         _check(min(pages, layers, kv_heads) >= 1, "a pool needs a page, a layer and a key head")
         _check(page_size in PAGE_SIZES, f"page_size must be one of {PAGE_SIZES}")
         _check(head_dim in HEAD_DIMS, f"head_dim must be one of {HEAD_DIMS}")
@@ -99,7 +142,7 @@ class PagedCache:
         self.device = pool.device
         self._index = pool.device.index
         self._raw = _raw_stream(pool.device)
-        self.dtype = pool.dtype
+        self.dtype = dtype
         self.pages, self.layers, self.kv_heads, self.page_size, self.head_dim = (
             pages, layers, kv_heads, page_size, head_dim)
         self.slots, self.table_pages = slots, table_pages
@@ -108,7 +151,7 @@ class PagedCache:
         self.refused = torch.zeros(slots, dtype=torch.int32, device=self.device)
         c = L.PagedCache()
         c.pages, c.layers, c.kv_heads, c.page_size, c.head_dim = pages, layers, kv_heads, page_size, head_dim
-        c.dtype, c.slots, c.table_pages = _DTYPES[pool.dtype], slots, table_pages
+        c.dtype, c.slots, c.table_pages = _DTYPES[dtype] | (L.CACHE_4BIT if self.bits == 4 else 0), slots, table_pages
         c.pool, c.page_table, c.lengths, c.refs = (t.data_ptr() for t in (pool, page_table, lengths, refs))
         c.status, c.live, c.refused = (t.data_ptr() for t in (self.status, self.live, self.refused))
         self._c = c
@@ -121,14 +164,17 @@ class PagedCache:
 
     @staticmethod
     def allocate(pages: int, slots: int, max_tokens: int, layers: int, kv_heads: int, head_dim: int,
-                 page_size: int = 16, dtype: torch.dtype = torch.bfloat16, device="cuda") -> "PagedCache":
+                 page_size: int = 16, dtype: torch.dtype = torch.bfloat16, device="cuda", bits: int = 16) -> "PagedCache":
         """An empty cache: no slot has tokens, every page is free (the pool is not cleared)."""
+        _check(bits in (4, 16), "bits must be 4 or 16")
+        _check(bits == 16 or head_dim in HEAD_DIMS, f"head_dim must be one of {HEAD_DIMS}")
         _check(page_size in PAGE_SIZES, f"page_size must be one of {PAGE_SIZES}")
         _check(max_tokens >= 1, "max_tokens must be at least 1")
         table_pages = (max_tokens + page_size - 1) // page_size
         i32 = dict(dtype=torch.int32, device=device)
         return PagedCache(
-            pool=torch.empty(pages, layers, 2, kv_heads, page_size, head_dim, dtype=dtype, device=device),
+            pool=torch.empty(pages, layers, 2, kv_heads, page_size, head_dim if bits == 16 else _token_bytes(head_dim),
+                             dtype=dtype if bits == 16 else torch.uint8, device=device), dtype=dtype,
             page_table=torch.full((slots, table_pages), -1, **i32), lengths=torch.zeros(slots, **i32),
             refs=torch.zeros(pages, **i32))
 
@@ -230,6 +276,63 @@ class PagedCache:
         [rows, kv_heads, head_dim]; without it [layers, rows, kv_heads, head_dim],
         every layer at once.  The last two dimensions must be contiguous.  Rows of
         slots whose tokens ``extend`` has refused are not written."""
+        args = self._cache_rows(k, v, layer, offsets)
+        self._call("mtt_b200_launch_paged_cache_store", self._ref, ctypes.byref(args), self._handle(stream))
+
+    def load(self, rows: int, layer: Optional[int] = None, offsets: Optional[torch.Tensor] = None, k: Optional[torch.Tensor] = None,
+             v: Optional[torch.Tensor] = None, stream=None):
+        """(k, v): the keys and values of each slot's last tokens, in rows laid out
+        as for ``store`` (of a 4-bit cache the values its codes stand for).  A row
+        that no slot has, or whose slot has fewer tokens than rows, is 0.  k and v:
+        where they go, if given."""
+        _check((k is None) == (v is None), "k and v are given together")
+        if k is None:
+            _check(0 <= rows <= MAX_ROWS, f"at most {MAX_ROWS} rows")
+            shape = (rows, self.kv_heads, self.head_dim) if layer is not None else (self.layers, rows, self.kv_heads, self.head_dim)
+            with self._on(stream):
+                k, v = torch.empty((2, *shape), dtype=self.dtype, device=self.device)
+        args = self._cache_rows(k, v, layer, offsets)
+        _check(args.rows == rows, "k and v have other rows than asked for")
+        self._call("mtt_b200_launch_paged_cache_load", self._ref, ctypes.byref(args), self._handle(stream))
+        return k, v
+
+    def append(self, layer: int, q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, rotation, q_out: Optional[torch.Tensor] = None,
+               *, offsets: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None, stream=None):
+        """``store`` of one layer with ``rotation`` (a rotary.Rotation) on the way:
+        keys are normed and turned, queries q [rows, q_heads, head_dim] too, which
+        are returned (q may be None; q_out may be q).  The result is that of
+        ``rotation.rotate`` and ``store``, bit for bit, in one pass.  A token's
+        position is its place in its slot, or positions [rows] int32.  A row that no
+        slot has, or whose tokens ``extend`` has refused, gets a query of 0."""
+        _check(rotation._index == self._index and rotation.head_dim == self.head_dim,
+               "the rotation is for another head_dim or device than the cache")
+        rows = L.RotateRows()
+        args = self._cache_rows(k, v, layer, offsets)
+        rows.rows, rows.kv_heads, rows.layer, rows.k, rows.v = args.rows, self.kv_heads, layer, args.k, args.v
+        rows.k_row_stride, rows.v_row_stride, rows.offsets = args.k_row_stride, args.v_row_stride, args.offsets
+        _check(args.rows <= MAX_ROWS, f"at most {MAX_ROWS} rows")
+        if positions is not None:
+            rows.positions = self._vector(positions, args.rows, torch.int32, "positions")
+        if q is not None:
+            shape = q.shape
+            if len(shape) != 3 or shape[0] != args.rows or shape[2] != self.head_dim or not 1 <= shape[1] <= MAX_GROUP * self.kv_heads:
+                raise ValueError("q must be [rows, q_heads, head_dim], with the rows of k and v")
+            rows.q_heads, rows.q, rows.q_row_stride = shape[1], q.data_ptr(), self._rows_of(q, shape, q.stride(), "q")
+            if q_out is None:
+                with self._on(stream):
+                    q_out = torch.empty(shape, dtype=self.dtype, device=self.device)
+            elif q_out.shape != shape:
+                raise ValueError("q_out must have q's shape")
+            rows.q_out, rows.q_out_row_stride = q_out.data_ptr(), self._rows_of(q_out, shape, q_out.stride(), "q_out")
+        else:
+            _check(q_out is None, "q_out without q")
+        handle = self._handle(stream)
+        rotation._on_stream(handle, stream)
+        self._call("mtt_b200_launch_paged_cache_append", self._ref, rotation._c[self.dtype][1], ctypes.byref(rows), handle)
+        return q_out
+
+    def _cache_rows(self, k, v, layer, offsets):
+        """The fields of the calls that move rows."""
         shape, ks, vs = k.shape, k.stride(), v.stride()
         if (len(shape) != (4 if layer is None else 3) or v.shape != shape or shape[-1] != self.head_dim or
                 shape[-2] != self.kv_heads):
@@ -254,7 +357,7 @@ class PagedCache:
             args.offsets = self._vector(offsets, self.slots + 1, torch.int32, "offsets")
         else:
             _check(args.rows <= self.slots, "more rows than slots: offsets are needed")
-        self._call("mtt_b200_launch_paged_cache_store", self._ref, ctypes.byref(args), self._handle(stream))
+        return args
 
     # -- attention ----------------------------------------------------------
 
@@ -295,16 +398,7 @@ class PagedCache:
         return args, out, lse
 
     def _rows_of(self, t, shape, st, name) -> int:
-        """The stride of t's rows [rows, heads, head_dim]; that of a dimension of
-        one has no meaning and is not looked at."""
-        if t.dtype is not self.dtype or t.get_device() != self._index:
-            raise ValueError(f"{name} must have the pool's type and device")
-        if st[2] != 1 or (st[1] != self.head_dim and shape[1] > 1):
-            raise ValueError(f"{name} must be contiguous in its heads")
-        row = st[0] if shape[0] > 1 else shape[1] * self.head_dim
-        if t.data_ptr() % 16 or row % 8:
-            raise ValueError(f"rows of {name} must be 16-byte aligned")
-        return row
+        return _rows_of(t, shape, st, name, self.dtype, self._index)
 
     def attend(self, layer: int, q: torch.Tensor, out: Optional[torch.Tensor] = None, *,
                offsets: Optional[torch.Tensor] = None, window: int = 0, sinks: int = 0,

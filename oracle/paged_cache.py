@@ -1,6 +1,7 @@
 """Plain restatement of the paged key/value cache and its attention (test
 infrastructure): page bookkeeping with Python lists and sets, attention in 64
-bits, one query row at a time."""
+bits, one query row at a time; the 4-bit form of the pool, and the position
+rotation of heads."""
 from __future__ import annotations
 
 import numpy as np
@@ -11,8 +12,9 @@ class ListCache:
     """The cache's state as lists: rows[i] the pages of slot i, lengths[i] its
     tokens, data [pages, layers, 2, kv_heads, page_size, head_dim]."""
 
-    def __init__(self, data, slots, table_pages):
-        self.data = data
+    def __init__(self, data, slots, table_pages, dtype=None):
+        """dtype: the 16-bit type beside a 4-bit pool (data uint8, its last two dimensions a block)."""
+        self.data, self.dtype = data, dtype
         self.rows = [[] for _ in range(slots)]
         self.lengths = [0] * slots
         self.status = [0] * slots
@@ -117,8 +119,73 @@ class ListCache:
                     self.status[i] = 3
                     continue
                 for n, layer in enumerate(layers):
-                    self.data[page, layer, 0, :, t % self.page_size] = k[n, r]
-                    self.data[page, layer, 1, :, t % self.page_size] = v[n, r]
+                    for kv, x in enumerate((k, v)):
+                        if self.dtype is None:
+                            self.data[page, layer, kv, :, t % self.page_size] = x[n, r]
+                        else:
+                            put4(self.data[page, layer, kv], t % self.page_size, x[n, r])
+
+
+GROUP = 64
+ORDER = (0, 2, 4, 6, 1, 3, 5, 7)  # of every 8 dims, from the word's lowest bits up
+
+
+def quantised(x):
+    """(codes, step, low) of x [..., d]: codes int64, step and low [..., groups] of x's type.  Single precision where the
+    format says so, one operation at a time."""
+    g = x.reshape(*x.shape[:-1], -1, GROUP).float().numpy()
+    low, high = g.min(-1), g.max(-1)
+    with np.errstate(all="ignore"):
+        spread = high - low
+        step = torch.from_numpy(np.where(np.isfinite(spread), spread / np.float32(15), np.float32("nan"))).to(x.dtype)
+        s32 = step.float().numpy()
+        inverse = np.where(s32 >= np.float32(2.0 ** -126), np.float32(1) / s32, np.float32(0))
+        at = (g - low[..., None]) * inverse[..., None]
+    codes = np.rint(np.clip(np.nan_to_num(at, nan=0.0, posinf=15.0, neginf=0.0), 0, 15))
+    return torch.from_numpy(codes).long().reshape(x.shape), step, torch.from_numpy(low).to(x.dtype)
+
+
+def put4(blocks, t, x):
+    """Token t's x [heads, d] into blocks [heads, page_size, bytes]."""
+    heads, ps, _ = blocks.shape
+    d = x.shape[-1]
+    codes, step, low = quantised(x)
+    flat = blocks.view(heads, -1)
+    words = codes.reshape(heads, -1, 8)[..., list(ORDER)]
+    flat[:, t * d // 2:(t + 1) * d // 2] = (words[..., 0::2] + 16 * words[..., 1::2]).reshape(heads, -1).to(torch.uint8)
+    pairs = torch.stack([step, low], -1).reshape(heads, -1).contiguous().view(torch.uint8)
+    at = ps * d // 2 + t * d // 16
+    flat[:, at:at + d // 16] = pairs
+
+
+def held(data, dtype):
+    """The values of a 4-bit pool, in 64 bits: [pages, layers, 2, kv_heads, page_size, head_dim]."""
+    ps, d = data.shape[4], data.shape[5] * 16 // 9
+    flat = data.reshape(*data.shape[:4], -1)
+    byte = flat[..., :ps * d // 2].reshape(*data.shape[:4], ps, d // 8, 4).long()
+    words = torch.stack([byte % 16, byte // 16], -1).reshape(*data.shape[:4], ps, d // 8, 8)
+    codes = torch.empty_like(words)
+    codes[..., list(ORDER)] = words
+    pairs = flat[..., ps * d // 2:].contiguous().view(dtype).double().reshape(*data.shape[:4], ps, d // GROUP, 2)
+    step, low = (pairs[..., i].repeat_interleave(GROUP, -1) for i in range(2))
+    return low + step * codes.reshape(*data.shape[:4], ps, d).double()
+
+
+def rotated(x, positions, rotary_dim, frequencies, interleaved=False, weight=None, eps=1e-6):
+    """(y, size) in 64 bits: the heads x [rows, heads, d] normed and turned, one pair at a time; size is |a| + |b| of each
+    pair before the turn (|x| past rotary_dim), which rounding errors are measured by."""
+    y = x.double()
+    if weight is not None:
+        y = y / torch.sqrt((y * y).mean(-1, keepdim=True) + eps) * weight.double()
+    out, size = y.clone(), y.abs()
+    for i in range(rotary_dim // 2):
+        a, b = (2 * i, 2 * i + 1) if interleaved else (i, i + rotary_dim // 2)
+        t = positions.double() * float(frequencies[i])
+        cos, sin = torch.cos(t)[:, None], torch.sin(t)[:, None]
+        out[..., a] = y[..., a] * cos - y[..., b] * sin
+        out[..., b] = y[..., b] * cos + y[..., a] * sin
+        size[..., a] = size[..., b] = y[..., a].abs() + y[..., b].abs()
+    return out, size
 
 
 def attention(pool, table, lengths, layer, q, offsets, window=0, sinks=0, scale=None, key_mask=None):
