@@ -927,9 +927,9 @@ MTT_B200_API int mtt_b200_launch_paged_cache_append(const mtt_b200_paged_cache_t
  * ascending within [0, rows] are not to be given: which rows are then written is
  * not said (none outside [0, rows]).
  * A 4-bit cache is attended to as if it held the values its codes stand for;
- * single tokens take them as they are, prompts and shared prefixes round each
- * once to the cache's type (a further u sum_j p_j |v_j|, and u scale sum_d |q_d
- * k_jd| in a score).
+ * keys as they are, and values too for single tokens; prompts and shared
+ * prefixes round each value once to the cache's type (a further u sum_j p_j
+ * |v_j|).
  * status[i] becomes 4 when a bounded wait inside the prompt kernel gave up (the
  * bounds grow with the keys that the call has to read): the outputs of slot i's
  * rows are then not to be used. */

@@ -138,6 +138,9 @@ __device__ __forceinline__ uint32_t codes2(uint32_t w) {
   }
 }
 
+// step, and what belongs to 16 + code: value = step (16 + code) + off
+__device__ __forceinline__ float2 step_off(float2 pair) { return make_float2(pair.x, fmaf(-16.f, pair.x, pair.y)); }
+
 // value = low + step * (codes2 - 16), two at a time: the subtraction is exact, the
 // rest rounded once.  step2, low2: step and low twice.
 template <typename T>

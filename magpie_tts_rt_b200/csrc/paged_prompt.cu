@@ -84,14 +84,19 @@ constexpr float kPromptBias = std::is_same_v<T, __half> ? 8.f : 0.f;
 constexpr int kMinShare = 2;        // key tiles a CTA takes at least
 constexpr int kMaxSms = 160;        // workspaces are sized for the largest device
 
-template <int D>
+template <int D, int Bits>
 struct PromptCfg {
   static constexpr int kStages = D == 64 ? 8 : 4;
   static constexpr uint32_t kQBytes = kTile * D * 2;
   static constexpr uint32_t kTileBytes = kKeys * D * 2;
-  static constexpr uint32_t kOutBytes = 8 * 32 * 128;  // a 32 x 64 block of results per softmax warp, on its way out
+  // a 32 x 64 block of results per softmax warp on its way out; 4-bit pool: 32 x 32, for room
+  static constexpr int kOutRow = Bits == 4 ? 64 : 128;
+  static constexpr uint32_t kOutBytes = 8 * 32 * kOutRow;
+  // 4-bit pool: step and off of each key and group, for each stage that holds keys
+  static constexpr int kKeyFloats = 2 * (D / kGroup4) * kKeys;
+  static constexpr uint32_t kKeyBytes = Bits == 4 ? kStages / 2 * kKeyFloats * 4 : 0;
   static constexpr size_t kSmem =
-      1024 + 2 * static_cast<size_t>(kQBytes) + kStages * static_cast<size_t>(kTileBytes) + kOutBytes;
+      1024 + 2 * static_cast<size_t>(kQBytes) + kStages * static_cast<size_t>(kTileBytes) + kOutBytes + kKeyBytes;
 };
 
 // Rows of the attention: tokens of slots, or members of prefix groups.
@@ -441,6 +446,12 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return pair2(d);
 }
 
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits2(a)), "l"(bits2(b)));
+  return pair2(d);
+}
+
 // NaN if any of the three is.
 __device__ __forceinline__ float max_nan(float a, float b, float c) {
   float r;
@@ -493,10 +504,10 @@ __device__ __forceinline__ KeySpan unit_span(const Walk& w, bool prefix, int tq,
   return KeySpan(p0, max(p0, p1), a.window, a.sinks);
 }
 
-// Converter of one half of the ring's tiles (keys or values) of a 4-bit pool: a
-// warp reads 16 tokens' codes at a time, two lanes a token, makes 16-bit values of
-// them and writes them as TMA would have (128-byte swizzle).  A piece of 16 tokens is
-// asked for a whole tile before it is converted.
+// A converter warp of a 4-bit pool fills the ring's key tiles or its value tiles.
+// It reads 16 tokens' codes at a time, two lanes a token, and asks for each piece a
+// whole tile before it is used.  Values become 16-bit values, keys 16 + code, which is
+// exact: what belongs to them, step and off, goes beside the tile.
 template <typename T, int D>
 struct Convert4 {
   static constexpr int DB = D / 64, kPieces = kKeys / 16;
@@ -519,18 +530,34 @@ struct Convert4 {
       }
     }
   }
-  __device__ __forceinline__ void put(int piece, unsigned char* tile) const {
+  // into the tile as TMA would have (128-byte swizzle)
+  template <typename F>
+  __device__ __forceinline__ void put(int piece, int b, unsigned char* tile, F word) const {
     const int lane = threadIdx.x & 31, row = 16 * piece + (lane >> 1);
+    const uint32_t w[4] = {codes[piece][b].x, codes[piece][b].y, codes[piece][b].z, codes[piece][b].w};
+    unsigned char* to = tile + b * (kKeys * 128) + row * 128;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) *reinterpret_cast<uint4*>(to + 16 * ((4 * (lane & 1) + k) ^ (row & 7))) = word(w[k]);
+  }
+  __device__ __forceinline__ void values(int piece, unsigned char* tile) const {
 #pragma unroll
     for (int b = 0; b < DB; ++b) {
       const uint32_t step2 = __byte_perm(pair[piece][b], 0, 0x1010), low2 = __byte_perm(pair[piece][b], 0, 0x3232);
-      const uint32_t w[4] = {codes[piece][b].x, codes[piece][b].y, codes[piece][b].z, codes[piece][b].w};
-      unsigned char* to = tile + b * (kKeys * 128) + row * 128;
+      put(piece, b, tile, [&](uint32_t w) {
+        return make_uint4(value2<T>(codes2<T, 0>(w), step2, low2), value2<T>(codes2<T, 1>(w), step2, low2),
+                          value2<T>(codes2<T, 2>(w), step2, low2), value2<T>(codes2<T, 3>(w), step2, low2));
+      });
+    }
+  }
+  __device__ __forceinline__ void keys(int piece, unsigned char* tile, float* beside) const {
+    const int lane = threadIdx.x & 31, row = 16 * piece + (lane >> 1);
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        *reinterpret_cast<uint4*>(to + 16 * ((4 * (lane & 1) + k) ^ (row & 7))) =
-            make_uint4(value2<T>(codes2<T, 0>(w[k]), step2, low2), value2<T>(codes2<T, 1>(w[k]), step2, low2),
-                       value2<T>(codes2<T, 2>(w[k]), step2, low2), value2<T>(codes2<T, 3>(w[k]), step2, low2));
+    for (int b = 0; b < DB; ++b) {
+      put(piece, b, tile, [&](uint32_t w) {
+        return make_uint4(codes2<T, 0>(w), codes2<T, 1>(w), codes2<T, 2>(w), codes2<T, 3>(w));
+      });
+      const float2 so = step_off(unpack2<T>(pair[piece][b]));
+      beside[(2 * b + (lane & 1)) * kKeys + row] = (lane & 1) == 0 ? so.x : so.y;
     }
   }
 };
@@ -539,7 +566,7 @@ template <typename T, int D, int Bits>
 __global__ void __launch_bounds__(kPromptThreads, 1)
     prompt_kernel(const __grid_constant__ CUtensorMap pool_map, const __grid_constant__ CUtensorMap q_map, PagedCache c, Attend a, PromptRows rows,
                   PromptSpace ws) {
-  using C = PromptCfg<D>;
+  using C = PromptCfg<D, Bits>;
   constexpr int S = C::kStages;
   constexpr int DB = D / 64;  // 64-dim blocks of a tile
   constexpr uint32_t kSCol = 0, kOCol = 2 * kKeys;  // S of Q tile i: column i kKeys, O: kOCol + i D
@@ -553,6 +580,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   unsigned char* q_smem = prompt_smem + pad;
   unsigned char* ring = q_smem + 2 * C::kQBytes;
   unsigned char* out_smem = ring + static_cast<size_t>(S) * C::kTileBytes;
+  float* key_pairs = reinterpret_cast<float*>(out_smem + C::kOutBytes);
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const bool prefix = rows.members != nullptr;
   const int tq = kTile / a.group;  // tokens of a Q tile
@@ -560,7 +588,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
       mbar_init(&kv_full[s], 1);
-      mbar_init(&kv_empty[s], 1);
+      mbar_init(&kv_empty[s], Bits == 4 && s % 2 == 0 ? 1 + 8 : 1);  // keys in 4 bits: the softmax warps too
       mbar_init(&ready[s], 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -570,7 +598,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       mbar_init(&p_full[i][1], 4);
       mbar_init(&half_done[i], 1);
       mbar_init(&o_full[i], 1);
-      mbar_init(&q_free[i], 1);
+      mbar_init(&q_free[i], Bits == 4 ? 1 + 4 : 1);
     }
     mbar_init(&fin, 1);
     err = 0;
@@ -638,7 +666,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         unsigned char* tile = ring + static_cast<size_t>(s) * C::kTileBytes;
 #pragma unroll
         for (int i = 0; i < x.kPieces; ++i) {
-          x.put(i, tile);
+          if (kv == 0)
+            x.keys(i, tile, key_pairs + s / 2 * C::kKeyFloats);
+          else
+            x.values(i, tile);
           ask(i, t + 1, page);
         }
         fence_proxy_async();
@@ -789,6 +820,20 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       if (elect_one()) umma_commit(bar);
       __syncwarp();
     };
+    // 4-bit pool: a product for each group of dims, for 64 keys
+    auto scores4 = [&](int i, int s, int h) {
+      const uint32_t qd = q_lo + i * (C::kQBytes >> 4), kd = k_lo + s * kTileStep + h * (kHalf * 128 >> 4);
+      if (elect_one()) {
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            umma_ss(tmem + kSCol + i * kKeys + d * kHalf, qd + d * kBlock + 2 * kk, kd + d * kBlock + 2 * kk,
+                    prompt_idesc<T>(kHalf, false), kk != 0);
+        umma_commit(&s_full[i]);
+      }
+      __syncwarp();
+    };
     bool more = any;
     while (more && alive(errv)) {
       int q0[2], q1[2];
@@ -811,11 +856,59 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         ok = ok && patience.wait(&q_ready[i], q_uses & 1);
         if (ok) {
           tmem_fence_after_sync();
-          if (seen[i].at(span.tile(t0))) scores(i, it % S);
-          if (last[i] <= t0) commit(&q_free[i]);  // (a Q tile without key tiles in this share: at once)
+          if constexpr (Bits == 4) {
+            if (seen[i].at(span.tile(t0))) scores4(i, it % S, 0);
+            if (last[i] < t0) commit(&q_free[i]);
+          } else {
+            if (seen[i].at(span.tile(t0))) scores(i, it % S);
+            if (last[i] <= t0) commit(&q_free[i]);  // (a Q tile without key tiles in this share: at once)
+          }
         }
       }
       ++q_uses;
+      if constexpr (Bits == 4) {
+        for (int t = t0; ok && t < t1; ++t, it += 2) {
+          const int ks = it % S, vs = (it + 1) % S, next_ks = (it + 2) % S;
+          const bool next = t + 1 < t1;
+          const int j = span.tile(t), j1 = next ? span.tile(t + 1) : 0;
+          ok = patience.wait(&ready[vs], ((it + 1) / S) & 1);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              if (seen[i].at(j)) {
+                ok = ok && patience.wait(&p_full[i][h], p_uses[i] & 1);
+                if (ok) {
+                  tmem_fence_after_sync();
+                  const uint32_t vd = v_lo + vs * kTileStep + h * (kHalf * 128 >> 4);
+                  if (elect_one()) {
+#pragma unroll
+                    for (int kk = 0; kk < kHalf / 16; ++kk)
+                      umma_ts(tmem + kOCol + i * D, tmem + kSCol + i * kKeys + 8 * kk, vd + kk * (2048 >> 4),
+                              prompt_idesc<T>(D, true), started[i] || kk != 0);
+                  }
+                  __syncwarp();
+                }
+                started[i] = true;
+                if (h == 1) {
+                  ++p_uses[i];
+                  if (ok && t == last[i]) commit(&o_full[i]);
+                } else if (ok) {
+                  scores4(i, ks, 1);
+                  if (t == last[i]) commit(&q_free[i]);
+                }
+              }
+              if (h == 1 && next) {
+                if (i == 0) ok = ok && patience.wait(&ready[next_ks], ((it + 2) / S) & 1);
+                if (ok && seen[i].at(j1)) scores4(i, next_ks, 0);
+              }
+            }
+            if (ok) commit(h == 0 ? &kv_empty[ks] : &kv_empty[vs]);
+          }
+        }
+        if (!ok) *errv = 1;
+        continue;
+      }
       if (ok) commit(&kv_empty[it % S]);
       ++it;
       for (int t = t0; ok && t < t1; ++t) {
@@ -873,6 +966,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     // sectors with every instruction, which took longer than several key tiles).
     const int piece = lane & 7, sub_row = lane >> 3;
     int s_uses = 0, o_uses = 0, unit = 0;
+    int key_it = 0;  // 4-bit pool: the ring's place of the next key tile
     // this thread's row of unit u: q and out row, or -1
     auto row_of = [&](const Walk& u) {
       const int tok = u.tok0 + i * tq + tok_in_tile;
@@ -923,9 +1017,34 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       const int next_row = more ? row_of(w) : -1;
       float m = -CUDART_INF_F, l = 0.f;
       bool ok = true, started = false;
-      for (int t = t0; t < t1; ++t) {
+      float q_sum[DB] = {};  // 4-bit pool: of the row's queries, over each group
+      if constexpr (Bits == 4) {
+        ok = patience.wait(&q_ready[i], unit & 1);
+        if (ok) {
+          const unsigned char* mine = q_smem + i * C::kQBytes + r * 128;
+#pragma unroll
+          for (int b = 0; b < DB; ++b)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const uint4 x = *reinterpret_cast<const uint4*>(mine + b * (kTile * 128) + 16 * (k ^ (r & 7)));
+              const float2 f0 = unpack2<T>(x.x), f1 = unpack2<T>(x.y), f2 = unpack2<T>(x.z), f3 = unpack2<T>(x.w);
+              q_sum[b] += ((f0.x + f0.y) + (f1.x + f1.y)) + ((f2.x + f2.y) + (f3.x + f3.y));
+            }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&q_free[i]);
+        }
+      }
+      for (int t = t0; ok && t < t1; ++t) {
         const int j = span.tile(t);
-        if (!seen.at(j)) continue;
+        const int ks = key_it % S, k_round = (key_it / S) & 1;
+        key_it += 2;
+        if (!seen.at(j)) {
+          if constexpr (Bits == 4) {  // (not before the tile is there: it would count for the one before it)
+            ok = patience.wait(&ready[ks], k_round);
+            if (ok && lane == 0) mbar_arrive(&kv_empty[ks]);
+          }
+          continue;
+        }
         const int base = kKeys * j;
         const bool all = mask == nullptr && tile_full(j, q0, q1, a.window, a.sinks) && base + kKeys <= len;
         uint32_t kept[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
@@ -936,15 +1055,52 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 #pragma unroll
           for (int x = 0; x < 4; ++x) kept[x] = __ballot_sync(0xffffffffu, on[x]);
         }
-        ok = patience.wait(&s_full[i], s_uses & 1);
+        if constexpr (Bits == 4) {
+          ok = patience.wait(&ready[ks], k_round);
+        } else {
+          ok = patience.wait(&s_full[i], s_uses & 1);
+        }
         if (!ok) break;
-        tmem_fence_after_sync();
+        if constexpr (Bits == 16) tmem_fence_after_sync();
         // One half after the other, so that 64 scores are held and not 128: P of
         // the first half goes over the first half's scores alone.
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           uint32_t s[kHalf];
-          tmem_ld64(s, s_col + kHalf * h);
+          if constexpr (Bits == 4) {
+            // scores of 64 keys: of each group step (q.(16 + c)) + off sum q
+            ok = patience.wait(&s_full[i], s_uses++ & 1);
+            if (!ok) break;
+            tmem_fence_after_sync();
+            tmem_ld64(s, s_col);
+            const float* beside = key_pairs + ks / 2 * C::kKeyFloats + kHalf * h;
+#pragma unroll
+            for (int b = 0; b < DB; ++b) {
+              const float2 sum = make_float2(q_sum[b], q_sum[b]);
+#pragma unroll
+              for (int x = 0; x < kHalf; x += 16) {
+                uint32_t y[16];
+                if (b > 0) tmem_ld16(y, s_col + kHalf * b + x);
+#pragma unroll
+                for (int k = 0; k < 16; k += 2) {
+                  const int e = x + k;
+                  const float2 step = *reinterpret_cast<const float2*>(beside + 2 * b * kKeys + e);
+                  const float2 off = *reinterpret_cast<const float2*>(beside + (2 * b + 1) * kKeys + e);
+                  float2 v = make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1]));
+                  v = b == 0 ? fma2(v, step, mul2(sum, off))
+                             : fma2(make_float2(__uint_as_float(y[k]), __uint_as_float(y[k + 1])), step, fma2(sum, off, v));
+                  s[e] = __float_as_uint(v.x);
+                  s[e + 1] = __float_as_uint(v.y);
+                }
+              }
+            }
+            if (h == 1) {
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&kv_empty[ks]);
+            }
+          } else {
+            tmem_ld64(s, s_col + kHalf * h);
+          }
           if (!all) {
             const int from = base + kHalf * h;
             const int hi = min(pos + 1, len) - from;
@@ -977,7 +1133,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                 sums[k & 1] = add2(sums[k & 1], v);
                 p[k] = Half16<T>::pack(v.x, v.y);
               }
-              tmem_st16(s_col + (kHalf / 2) * h + 16 * x, p);
+              tmem_st16(s_col + (Bits == 4 ? 0 : (kHalf / 2) * h) + 16 * x, p);
             }
             sums[0] = add2(sums[0], sums[1]);
             sum = sums[0].x + sums[0].y;
@@ -990,7 +1146,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
               for (int k = 0; k < kHalf; k += 2) top = max_nan(top, __uint_as_float(s[k]), __uint_as_float(s[k + 1]));
               if (started || h == 1) {
                 // the products so far must be in O: those of the tiles before are (these scores came after them)
-                if (h == 1) ok = patience.wait(&half_done[i], s_uses & 1);
+                if (Bits == 16 && h == 1) ok = patience.wait(&half_done[i], s_uses & 1);
                 if (!ok) break;
                 tmem_fence_after_sync();
                 const float f = m == -CUDART_INF_F ? 1.f : ex2((m - top) * a.scale2);
@@ -1018,7 +1174,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           if (lane == 0) mbar_arrive(&p_full[i][h]);
         }
         if (!ok) break;
-        ++s_uses;
+        if (Bits == 16) ++s_uses;
         started = true;
       }
       if (ok && more && !rows.q_mapped) {  // before this unit's result comes out
@@ -1036,14 +1192,16 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       const bool there = q_row >= 0;
       float* part = ws.part + static_cast<int64_t>(part_at) * (D + 2) * kPairRows + i * kTile + r;
       float* state = prefix && there ? rows.state + (static_cast<int64_t>(q_row) * a.q_heads + q_head) * (D + 4) : nullptr;
-      unsigned char* stage = out_smem + warp * (32 * 128);
-      // where the 8 rows whose pieces this lane stores go (null: nowhere)
-      uint16_t* to[8];
+      unsigned char* stage = out_smem + warp * (32 * C::kOutRow);
+      // where the rows whose pieces this lane stores go (null: nowhere)
+      constexpr int kOuts = Bits == 4 ? 4 : 8;
+      auto out_row = [&](int k) { return Bits == 4 ? 8 * k + (lane >> 2) : 4 * k + sub_row; };
+      uint16_t* to[kOuts];
       {
         uint16_t* mine = there ? a.out + q_row * a.out_row + static_cast<int64_t>(q_head) * D : nullptr;
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-          to[k] = reinterpret_cast<uint16_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine), 4 * k + sub_row));
+        for (int k = 0; k < kOuts; ++k)
+          to[k] = reinterpret_cast<uint16_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine), out_row(k)));
       }
 #pragma unroll
       for (int b = 0; b < DB; ++b) {
@@ -1075,12 +1233,24 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
               y.y = Half16<T>::pack(__uint_as_float(o[8 * k + 2]) * inv, __uint_as_float(o[8 * k + 3]) * inv);
               y.z = Half16<T>::pack(__uint_as_float(o[8 * k + 4]) * inv, __uint_as_float(o[8 * k + 5]) * inv);
               y.w = Half16<T>::pack(__uint_as_float(o[8 * k + 6]) * inv, __uint_as_float(o[8 * k + 7]) * inv);
-              *reinterpret_cast<uint4*>(stage + lane * 128 + 16 * ((4 * half + k) ^ (lane & 7))) = y;
+              if constexpr (Bits == 4)
+                *reinterpret_cast<uint4*>(stage + lane * 64 + 16 * (k ^ (lane >> 1 & 3))) = y;
+              else
+                *reinterpret_cast<uint4*>(stage + lane * 128 + 16 * ((4 * half + k) ^ (lane & 7))) = y;
             }
           }
           __syncwarp();
+          if (Bits == 4 && whole && !prefix) {
+#pragma unroll
+            for (int k = 0; k < kOuts; ++k) {
+              const int from = out_row(k);
+              const uint4 y = *reinterpret_cast<const uint4*>(stage + from * 64 + 16 * ((lane & 3) ^ (from >> 1 & 3)));
+              if (to[k] != nullptr) *reinterpret_cast<uint4*>(to[k] + 64 * b + 32 * half + 8 * (lane & 3)) = y;
+            }
+            __syncwarp();
+          }
         }
-        if (whole && !prefix) {
+        if (Bits == 16 && whole && !prefix) {
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
             const int from = 4 * k + sub_row;
@@ -1355,7 +1525,7 @@ cudaError_t run_prompt(const PagedCache& c, int dtype, const Attend& a, PromptRo
     using T = decltype(type);
     constexpr int D = decltype(dim)::value, Bits = decltype(bits)::value;
     const auto kernel = prompt_kernel<T, D, Bits>;
-    constexpr size_t smem = PromptCfg<D>::kSmem;
+    constexpr size_t smem = PromptCfg<D, Bits>::kSmem;
     static std::atomic<uint64_t> opted_in;  // devices on which this kernel has its shared memory
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);

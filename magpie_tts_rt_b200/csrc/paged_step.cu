@@ -297,9 +297,6 @@ __device__ __forceinline__ uint2 load8(const unsigned char* p, bool on) {
   return v;
 }
 
-// step, and what belongs to 16 + code: value = step (16 + code) + off
-__device__ __forceinline__ float2 step_off(float2 pair) { return make_float2(pair.x, fmaf(-16.f, pair.x, pair.y)); }
-
 // The first of the 8 dims that piece k of a thread's queries holds, as its keys do.
 template <int Bits>
 __device__ __forceinline__ int step_dims(int t, int k) {

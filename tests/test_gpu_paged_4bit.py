@@ -11,8 +11,9 @@ The result is rounded once: u |o|, u = finfo.eps / 2.  Sums in f32 and the
 exponential's own error (2^-22 each) are allowed for by n 2^-22 of the weight for n
 keys, n at most 64 (parts are summed pairwise by warps and joined), and a tenth.
 
-Prompts round the held values once to the cache's type before anything else;
-rounded so, they are held to the tolerance of a 16-bit cache."""
+Prompts take keys as they are held, too, and round the held values once to the
+cache's type: with values rounded so, they are held to the tolerance of a 16-bit
+cache."""
 import math
 
 import numpy as np
@@ -60,6 +61,12 @@ def make4(pc, lengths, hkv=2, d=64, ps=16, layers=2, dtype=torch.bfloat16, seed=
         refs[p] += 1
     cache = pc.PagedCache(pool.cuda(), table.cuda(), i32(lengths), refs.cuda(), dtype=dtype)
     return cache, pool, table
+
+
+def values_rounded(held, dtype):
+    held = held.clone()
+    held[:, :, 1] = held[:, :, 1].to(dtype).double()
+    return held
 
 
 def spoil(cache, table, i, j, value=0xff):
@@ -113,7 +120,7 @@ def check(pc, lengths, new=None, group=1, hkv=2, d=64, ps=16, dtype=torch.bfloat
                     spoil(cache, table, i, j)
     held = O.held(pool, dtype)
     if new is not None:
-        held = held.to(dtype)
+        held = values_rounded(held, dtype)
     ref = O.attention(held, table, lengths, 1, q, offsets, window, sinks, scale, key_mask)
     got, lse = cache.attend(1, q.cuda(), offsets=None if new is None else i32(offsets), window=window, sinks=sinks,
                             scale=scale, key_mask=None if key_mask is None else key_mask.cuda(), return_lse=True)
@@ -380,9 +387,9 @@ def test_shared_prefix(pc, d, group, known):
     torch.cuda.synchronize()
     held = O.held(cache.pool.cpu(), dtype)
     lengths, table = cache.lengths.tolist(), cache.page_table.cpu()
-    ref = O.attention(held.to(dtype), table, lengths, 1, q, list(range(10)))
+    ref = O.attention(values_rounded(held, dtype), table, lengths, 1, q, list(range(10)))
     plain = O.attention(held, table, lengths, 1, q, list(range(10)))
-    # prefix keys and values rounded once, the others not at all: between the two references, which differ by that rounding
+    # a prefix's values are rounded once, the others not at all: between the two references, which differ by that rounding
     out, ref_lse, weight = ref
     tol = 1.1 * 2.0 ** -8 * (out.abs() + weight) + (plain[0] - out).abs() * 2 + 1e-4
     assert ((got.cpu().double() - out).abs() <= tol).all()
