@@ -95,8 +95,10 @@ struct PromptCfg {
   // 4-bit pool: step and off of each key and group, for each stage that holds keys
   static constexpr int kKeyFloats = 2 * (D / kGroup4) * kKeys;
   static constexpr uint32_t kKeyBytes = Bits == 4 ? kStages / 2 * kKeyFloats * 4 : 0;
+  static constexpr uint32_t kRawBytes = Bits == 4 ? 2 * 4 * (D / kGroup4) * 32 * 20 : 0;  // the converters' (Convert4::Raw)
   static constexpr size_t kSmem =
-      1024 + 2 * static_cast<size_t>(kQBytes) + kStages * static_cast<size_t>(kTileBytes) + kOutBytes + kKeyBytes;
+      1024 + 2 * static_cast<size_t>(kQBytes) + kStages * static_cast<size_t>(kTileBytes) + kOutBytes + kKeyBytes +
+      kRawBytes;
 };
 
 // Rows of the attention: tokens of slots, or members of prefix groups.
@@ -505,58 +507,66 @@ __device__ __forceinline__ KeySpan unit_span(const Walk& w, bool prefix, int tq,
 }
 
 // A converter warp of a 4-bit pool fills the ring's key tiles or its value tiles.
-// It reads 16 tokens' codes at a time, two lanes a token, and asks for each piece a
-// whole tile before it is used.  Values become 16-bit values, keys 16 + code, which is
-// exact: what belongs to them, step and off, goes beside the tile.
+// It takes 16 tokens at a time, two lanes a token: their codes and pairs are copied to
+// shared memory (each lane its own, kRaw pieces ahead) and from there converted into
+// the tile as TMA would have written it (128-byte swizzle).  Values become 16-bit
+// values, keys 16 + code, which is exact: what belongs to them, step and off, goes
+// beside the tile.  Everything is in rolled loops, so that it fits the instruction
+// cache beside the softmax.
+constexpr int kRaw = 4;
+
 template <typename T, int D>
 struct Convert4 {
   static constexpr int DB = D / 64, kPieces = kKeys / 16;
-  uint4 codes[kPieces][DB];
-  uint32_t pair[kPieces][DB];
+  struct Raw {
+    uint4 codes[kRaw][DB][32];
+    uint32_t pair[kRaw][DB][32];
+  };
+  Raw* raw;
 
-  // tokens 16 * piece .. of the tile at key `base`, from the page that holds them;
-  // `keep`: whether the lane's token is to be read
-  __device__ __forceinline__ void ask(const PagedCache& c, int piece, int page, int layer, int kv, int head, int base, bool keep) {
-    const int lane = threadIdx.x & 31, in_page = (base + 16 * piece + (lane >> 1)) & (c.page_size - 1);
-    const unsigned char* block = block4(c, page, layer, kv, head);
+  // the lane's token `key`, from the page that holds it; zeros if it is not to be read
+  __device__ __forceinline__ void ask(const PagedCache& c, int slot, int page, int layer, int kv, int head, int key, bool keep) const {
+    const int lane = threadIdx.x & 31, in_page = key & (c.page_size - 1);
     keep = keep && c.is_page(page);
+    const unsigned char* block = block4(c, keep ? page : 0, layer, kv, head);
 #pragma unroll
     for (int b = 0; b < DB; ++b) {
-      codes[piece][b] = make_uint4(0, 0, 0, 0);
-      pair[piece][b] = 0;
-      if (keep) {
-        codes[piece][b] = *reinterpret_cast<const uint4*>(block + in_page * (D / 2) + 32 * b + 16 * (lane & 1));
-        pair[piece][b] = *(reinterpret_cast<const uint32_t*>(block + block4_codes(c)) + in_page * DB + b);
-      }
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(&raw->codes[slot][b][lane])),
+                   "l"(block + in_page * (D / 2) + 32 * b + 16 * (lane & 1)), "r"(keep ? 16 : 0)
+                   : "memory");
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_addr(&raw->pair[slot][b][lane])),
+                   "l"(block + block4_codes(c) + (in_page * DB + b) * 4), "r"(keep ? 4 : 0)
+                   : "memory");
     }
   }
-  // into the tile as TMA would have (128-byte swizzle)
   template <typename F>
-  __device__ __forceinline__ void put(int piece, int b, unsigned char* tile, F word) const {
-    const int lane = threadIdx.x & 31, row = 16 * piece + (lane >> 1);
-    const uint32_t w[4] = {codes[piece][b].x, codes[piece][b].y, codes[piece][b].z, codes[piece][b].w};
+  __device__ __forceinline__ void put(int slot, int b, int row, unsigned char* tile, F word) const {
+    const int lane = threadIdx.x & 31;
+    const uint4 x = raw->codes[slot][b][lane];
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
     unsigned char* to = tile + b * (kKeys * 128) + row * 128;
 #pragma unroll
     for (int k = 0; k < 4; ++k) *reinterpret_cast<uint4*>(to + 16 * ((4 * (lane & 1) + k) ^ (row & 7))) = word(w[k]);
   }
-  __device__ __forceinline__ void values(int piece, unsigned char* tile) const {
-#pragma unroll
+  __device__ __forceinline__ void values(int slot, int row, unsigned char* tile) const {
+#pragma unroll 1
     for (int b = 0; b < DB; ++b) {
-      const uint32_t step2 = __byte_perm(pair[piece][b], 0, 0x1010), low2 = __byte_perm(pair[piece][b], 0, 0x3232);
-      put(piece, b, tile, [&](uint32_t w) {
+      const uint32_t p = raw->pair[slot][b][threadIdx.x & 31];
+      const uint32_t step2 = __byte_perm(p, 0, 0x1010), low2 = __byte_perm(p, 0, 0x3232);
+      put(slot, b, row, tile, [&](uint32_t w) {
         return make_uint4(value2<T>(codes2<T, 0>(w), step2, low2), value2<T>(codes2<T, 1>(w), step2, low2),
                           value2<T>(codes2<T, 2>(w), step2, low2), value2<T>(codes2<T, 3>(w), step2, low2));
       });
     }
   }
-  __device__ __forceinline__ void keys(int piece, unsigned char* tile, float* beside) const {
-    const int lane = threadIdx.x & 31, row = 16 * piece + (lane >> 1);
-#pragma unroll
+  __device__ __forceinline__ void keys(int slot, int row, unsigned char* tile, float* beside) const {
+    const int lane = threadIdx.x & 31;
+#pragma unroll 1
     for (int b = 0; b < DB; ++b) {
-      put(piece, b, tile, [&](uint32_t w) {
+      put(slot, b, row, tile, [&](uint32_t w) {
         return make_uint4(codes2<T, 0>(w), codes2<T, 1>(w), codes2<T, 2>(w), codes2<T, 3>(w));
       });
-      const float2 so = step_off(unpack2<T>(pair[piece][b]));
+      const float2 so = step_off(unpack2<T>(raw->pair[slot][b][lane]));
       beside[(2 * b + (lane & 1)) * kKeys + row] = (lane & 1) == 0 ? so.x : so.y;
     }
   }
@@ -633,6 +643,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     // ---- 4-bit pool: warp 9 fills the ring's key tiles (the even places), warp 10 its value tiles.  Values that no query
     // of the unit may see are zeros.
     const int kv = warp - 9;
+    const Convert4<T, D> x{reinterpret_cast<typename Convert4<T, D>::Raw*>(key_pairs + C::kKeyBytes / 4) + kv};
+    static_assert(Bits == 16 || 2 * sizeof(typename Convert4<T, D>::Raw) == C::kRawBytes);
     int it = kv;
     for (bool more = any && !ws.waits.starve; more && alive(errv); more = w.next(ws)) {
       const Geom g = w.g;
@@ -641,42 +653,51 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       const bool* mask = a.key_mask != nullptr ? a.key_mask + g.key_slot * a.mask_stride : nullptr;
       int p0, p1;
       positions(g, prefix, w.tok0, w.tok0 + 2 * tq, &p0, &p1);
-      Convert4<T, D> x;
       // the page of lane's 16 tokens of tile t
       auto page_of = [&](int t) {
         const int key = kKeys * span.tile(t) + 16 * lane;
         return lane < x.kPieces && t < w.t1 && key < g.len ? table[key >> c.page_shift] : -1;
       };
-      auto ask = [&](int piece, int t, int page) {
-        const int base = kKeys * span.tile(t), j = base + 16 * piece + (lane >> 1);
-        bool keep = j < g.len;
-        if (kv == 1) keep = j <= p1 && (a.window == 0 || j > p0 - a.window || j < a.sinks) && (mask == nullptr || mask[j]);
-        x.ask(c, piece, __shfl_sync(0xffffffffu, page, piece), a.layer, kv, w.head, base, keep);
+      // piece p of tile t into a slot of the raw ring
+      auto ask = [&](int slot, int t, int p, int page) {
+        const int j = kKeys * span.tile(t) + 16 * p + (lane >> 1);
+        page = __shfl_sync(0xffffffffu, page, p);
+        if (t < w.t1) {
+          bool keep = j < g.len;
+          if (kv == 1) keep = j <= p1 && (a.window == 0 || j > p0 - a.window || j < a.sinks) && (mask == nullptr || mask[j]);
+          x.ask(c, slot, page, a.layer, kv, w.head, j, keep);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
       };
       int page = page_of(w.t0), next_page = page_of(w.t0 + 1);
-#pragma unroll
-      for (int i = 0; i < x.kPieces; ++i) ask(i, w.t0, page);
+#pragma unroll 1
+      for (int p = 0; p < kRaw; ++p) ask(p, w.t0, p, page);
       bool ok = true;
       for (int t = w.t0; ok && t < w.t1; ++t, it += 2) {
-        page = next_page;
-        next_page = page_of(t + 2);
+        const int ahead = page_of(t + 2);
         const int s = it % S;
         ok = it < S || patience.wait(&kv_empty[s], ((it / S) - 1) & 1);
         if (!ok) break;
         unsigned char* tile = ring + static_cast<size_t>(s) * C::kTileBytes;
-#pragma unroll
-        for (int i = 0; i < x.kPieces; ++i) {
+#pragma unroll 1
+        for (int p = 0; p < x.kPieces; ++p) {
+          asm volatile("cp.async.wait_group %0;" ::"n"(kRaw - 1) : "memory");
+          const int row = 16 * p + (lane >> 1);
           if (kv == 0)
-            x.keys(i, tile, key_pairs + s / 2 * C::kKeyFloats);
+            x.keys(p % kRaw, row, tile, key_pairs + s / 2 * C::kKeyFloats);
           else
-            x.values(i, tile);
-          ask(i, t + 1, page);
+            x.values(p % kRaw, row, tile);
+          const bool same = p + kRaw < x.kPieces;
+          ask(p % kRaw, same ? t : t + 1, (p + kRaw) % x.kPieces, same ? page : next_page);
         }
+        page = next_page;
+        next_page = ahead;
         fence_proxy_async();
         __syncwarp();
         if (lane == 0) mbar_arrive(&ready[s]);
       }
       if (!ok) *errv = 1;
+      cp_async_wait_all();
     }
   } else if (warp == 9) {
     // ---- TMA producer.  Order: keys 0, then values t, keys t + 1, as they are used.
@@ -872,7 +893,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           const bool next = t + 1 < t1;
           const int j = span.tile(t), j1 = next ? span.tile(t + 1) : 0;
           ok = patience.wait(&ready[vs], ((it + 1) / S) & 1);
-#pragma unroll
+#pragma unroll 1
           for (int h = 0; h < 2; ++h) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
@@ -1056,126 +1077,213 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           for (int x = 0; x < 4; ++x) kept[x] = __ballot_sync(0xffffffffu, on[x]);
         }
         if constexpr (Bits == 4) {
+          // 32 keys at a time, in one copy of the code: beside the converter warps' it has to fit the instruction cache (with
+          // 64 and two copies 8192 tokens took 2.5 ms, in which the converters had half a tile's time to wait for
+          // instructions)
           ok = patience.wait(&ready[ks], k_round);
-        } else {
-          ok = patience.wait(&s_full[i], s_uses & 1);
-        }
-        if (!ok) break;
-        if constexpr (Bits == 16) tmem_fence_after_sync();
-        // One half after the other, so that 64 scores are held and not 128: P of
-        // the first half goes over the first half's scores alone.
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t s[kHalf];
-          if constexpr (Bits == 4) {
-            // scores of 64 keys: of each group step (q.(16 + c)) + off sum q
+          if (!ok) break;
+          const float* beside = key_pairs + ks / 2 * C::kKeyFloats;
+#pragma unroll 1
+          for (int h = 0; h < 2; ++h) {
             ok = patience.wait(&s_full[i], s_uses++ & 1);
             if (!ok) break;
             tmem_fence_after_sync();
-            tmem_ld64(s, s_col);
-            const float* beside = key_pairs + ks / 2 * C::kKeyFloats + kHalf * h;
-#pragma unroll
-            for (int b = 0; b < DB; ++b) {
-              const float2 sum = make_float2(q_sum[b], q_sum[b]);
-#pragma unroll
-              for (int x = 0; x < kHalf; x += 16) {
-                uint32_t y[16];
-                if (b > 0) tmem_ld16(y, s_col + kHalf * b + x);
-#pragma unroll
-                for (int k = 0; k < 16; k += 2) {
-                  const int e = x + k;
-                  const float2 step = *reinterpret_cast<const float2*>(beside + 2 * b * kKeys + e);
-                  const float2 off = *reinterpret_cast<const float2*>(beside + (2 * b + 1) * kKeys + e);
-                  float2 v = make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1]));
-                  v = b == 0 ? fma2(v, step, mul2(sum, off))
-                             : fma2(make_float2(__uint_as_float(y[k]), __uint_as_float(y[k + 1])), step, fma2(sum, off, v));
-                  s[e] = __float_as_uint(v.x);
-                  s[e + 1] = __float_as_uint(v.y);
-                }
-              }
-            }
-            if (h == 1) {
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&kv_empty[ks]);
-            }
-          } else {
-            tmem_ld64(s, s_col + kHalf * h);
-          }
-          if (!all) {
-            const int from = base + kHalf * h;
-            const int hi = min(pos + 1, len) - from;
-            const int lo = a.window > 0 ? max(max(pos + 1 - from, 0) - a.window, 0) : 0;
-            const int sk = min(a.sinks, from + kHalf) - from;
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              const uint32_t see = kept[2 * h + x] & bit_range(0, hi - 32 * x) &
-                                   (bit_range(lo - 32 * x, 32) | bit_range(0, sk - 32 * x));
-#pragma unroll
-              for (int k = 0; k < 32; ++k)
-                if (!((see >> k) & 1u)) s[32 * x + k] = 0xff800000u;
-            }
-          }
-          float sum;
-          auto probabilities = [&] {
-            const float off = m == -CUDART_INF_F ? 0.f : fmaf(-m, a.scale2, kPromptBias<T>);
-            const float2 scale = make_float2(a.scale2, a.scale2), offs = make_float2(off, off);
-            float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              uint32_t p[16];
-#pragma unroll
-              for (int k = 0; k < 16; ++k) {
-                const int e = 32 * x + 2 * k;
-                float2 v = fma2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), scale, offs);
-                v.x = ex2(v.x);
-                v.y = ex2(v.y);
-                // the sum keeps the unrounded probabilities; the values' weights are rounded to 16 bits once
-                sums[k & 1] = add2(sums[k & 1], v);
-                p[k] = Half16<T>::pack(v.x, v.y);
-              }
-              tmem_st16(s_col + (Bits == 4 ? 0 : (kHalf / 2) * h) + 16 * x, p);
-            }
-            sums[0] = add2(sums[0], sums[1]);
-            sum = sums[0].x + sums[0].y;
-          };
-          bool find = h == 0 && !started;
-          while (true) {
-            if (find) {
-              float top = m;
-#pragma unroll
-              for (int k = 0; k < kHalf; k += 2) top = max_nan(top, __uint_as_float(s[k]), __uint_as_float(s[k + 1]));
-              if (started || h == 1) {
-                // the products so far must be in O: those of the tiles before are (these scores came after them)
-                if (Bits == 16 && h == 1) ok = patience.wait(&half_done[i], s_uses & 1);
-                if (!ok) break;
-                tmem_fence_after_sync();
-                const float f = m == -CUDART_INF_F ? 1.f : ex2((m - top) * a.scale2);
-                l *= f;
 #pragma unroll 1
-                for (int b = 0; b < D / 16; ++b) {
-                  uint32_t o[16];
-                  tmem_ld16(o, o_col + 16 * b);
+            for (int x = 0; x < kHalf; x += 32) {
+              const int e0 = kHalf * h + x;  // the chunk's first key in the tile
+              uint32_t s[32];
+              tmem_ld32(s, s_col + x);
+              // of each group step (q.(16 + c)) + off sum q
 #pragma unroll
-                  for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-                  tmem_st16(o_col + 16 * b, o);
+              for (int b = 0; b < DB; ++b) {
+                const float2 of = make_float2(q_sum[b], q_sum[b]);
+#pragma unroll
+                for (int y0 = 0; y0 < 32; y0 += 16) {
+                  uint32_t y[16];
+                  if (b > 0) tmem_ld16(y, s_col + kHalf * b + x + y0);
+#pragma unroll
+                  for (int k = 0; k < 16; k += 4) {
+                    const int e = y0 + k;
+                    const float4 step = *reinterpret_cast<const float4*>(beside + 2 * b * kKeys + e0 + e);
+                    const float4 off = *reinterpret_cast<const float4*>(beside + (2 * b + 1) * kKeys + e0 + e);
+                    float2 v0 = make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1]));
+                    float2 v1 = make_float2(__uint_as_float(s[e + 2]), __uint_as_float(s[e + 3]));
+                    if (b == 0) {
+                      v0 = fma2(v0, make_float2(step.x, step.y), mul2(of, make_float2(off.x, off.y)));
+                      v1 = fma2(v1, make_float2(step.z, step.w), mul2(of, make_float2(off.z, off.w)));
+                    } else {
+                      v0 = fma2(of, make_float2(off.x, off.y), v0);
+                      v1 = fma2(of, make_float2(off.z, off.w), v1);
+                      v0 = fma2(make_float2(__uint_as_float(y[k]), __uint_as_float(y[k + 1])), make_float2(step.x, step.y), v0);
+                      v1 = fma2(make_float2(__uint_as_float(y[k + 2]), __uint_as_float(y[k + 3])), make_float2(step.z, step.w), v1);
+                    }
+                    s[e] = __float_as_uint(v0.x);
+                    s[e + 1] = __float_as_uint(v0.y);
+                    s[e + 2] = __float_as_uint(v1.x);
+                    s[e + 3] = __float_as_uint(v1.y);
+                  }
                 }
               }
-              m = top;
+              if (!all) {
+                const int from = base + e0;
+                const int hi = min(pos + 1, len) - from;
+                const int lo = a.window > 0 ? max(max(pos + 1 - from, 0) - a.window, 0) : 0;
+                const uint32_t there = x == 0 ? (h == 0 ? kept[0] : kept[2]) : (h == 0 ? kept[1] : kept[3]);
+                const uint32_t see = there & bit_range(0, hi) & (bit_range(lo, 32) | bit_range(0, a.sinks - from));
+#pragma unroll
+                for (int k = 0; k < 32; ++k)
+                  if (!((see >> k) & 1u)) s[k] = 0xff800000u;
+              }
+              float sum;
+              bool find = e0 == 0 && !started;
+              while (true) {
+                if (find) {
+                  float top = m;
+#pragma unroll
+                  for (int k = 0; k < 32; k += 2) top = max_nan(top, __uint_as_float(s[k]), __uint_as_float(s[k + 1]));
+                  // the products so far are in O: these scores came after them
+                  const float f = m == -CUDART_INF_F ? 1.f : ex2((m - top) * a.scale2);
+                  l *= f;
+                  if (started || h == 1) {
+#pragma unroll 1
+                    for (int b = 0; b < D / 16; ++b) {
+                      uint32_t o[16];
+                      tmem_ld16(o, o_col + 16 * b);
+#pragma unroll
+                      for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+                      tmem_st16(o_col + 16 * b, o);
+                    }
+                  }
+                  if (x > 0) {  // the chunk before, whose weights wait in P: at most 2^-15 of these, so that rounding them again is nothing
+                    uint32_t p[16];
+                    tmem_wait_st();
+                    tmem_ld16(p, s_col);
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                      const float2 v = unpack2<T>(p[k]);
+                      p[k] = Half16<T>::pack(v.x * f, v.y * f);
+                    }
+                    tmem_st16(s_col, p);
+                  }
+                  m = top;
+                }
+                const float off = m == -CUDART_INF_F ? 0.f : fmaf(-m, a.scale2, kPromptBias<T>);
+                const float2 scale = make_float2(a.scale2, a.scale2), offs = make_float2(off, off);
+                float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+                uint32_t p[16];
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                  float2 v = fma2(make_float2(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1])), scale, offs);
+                  v.x = ex2(v.x);
+                  v.y = ex2(v.y);
+                  // the sum keeps the unrounded probabilities; the values' weights are rounded to 16 bits once
+                  sums[k & 1] = add2(sums[k & 1], v);
+                  p[k] = Half16<T>::pack(v.x, v.y);
+                }
+                tmem_st16(s_col + x / 2, p);
+                sums[0] = add2(sums[0], sums[1]);
+                sum = sums[0].x + sums[0].y;
+                if (find || !__any_sync(0xffffffffu, q_row >= 0 && (!(sum <= 32768.f) || m == -CUDART_INF_F))) break;
+                find = true;
+              }
+              l += sum;
             }
-            probabilities();
-            if (find || !__any_sync(0xffffffffu, q_row >= 0 && (!(sum <= 32768.f) || m == -CUDART_INF_F))) break;
-            find = true;
+            tmem_wait_st();
+            tmem_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) {
+              if (h == 1) mbar_arrive(&kv_empty[ks]);
+              mbar_arrive(&p_full[i][h]);
+            }
           }
           if (!ok) break;
-          l += sum;
-          tmem_wait_st();
-          tmem_fence_before_sync();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&p_full[i][h]);
+          started = true;
+        } else {
+          ok = patience.wait(&s_full[i], s_uses & 1);
+          if (!ok) break;
+          tmem_fence_after_sync();
+          // One half after the other, so that 64 scores are held and not 128: P of
+          // the first half goes over the first half's scores alone.
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t s[kHalf];
+            tmem_ld64(s, s_col + kHalf * h);
+            if (!all) {
+              const int from = base + kHalf * h;
+              const int hi = min(pos + 1, len) - from;
+              const int lo = a.window > 0 ? max(max(pos + 1 - from, 0) - a.window, 0) : 0;
+              const int sk = min(a.sinks, from + kHalf) - from;
+#pragma unroll
+              for (int x = 0; x < 2; ++x) {
+                const uint32_t see = kept[2 * h + x] & bit_range(0, hi - 32 * x) &
+                                     (bit_range(lo - 32 * x, 32) | bit_range(0, sk - 32 * x));
+#pragma unroll
+                for (int k = 0; k < 32; ++k)
+                  if (!((see >> k) & 1u)) s[32 * x + k] = 0xff800000u;
+              }
+            }
+            float sum;
+            auto probabilities = [&] {
+              const float off = m == -CUDART_INF_F ? 0.f : fmaf(-m, a.scale2, kPromptBias<T>);
+              const float2 scale = make_float2(a.scale2, a.scale2), offs = make_float2(off, off);
+              float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+              for (int x = 0; x < 2; ++x) {
+                uint32_t p[16];
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                  const int e = 32 * x + 2 * k;
+                  float2 v = fma2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), scale, offs);
+                  v.x = ex2(v.x);
+                  v.y = ex2(v.y);
+                  // the sum keeps the unrounded probabilities; the values' weights are rounded to 16 bits once
+                  sums[k & 1] = add2(sums[k & 1], v);
+                  p[k] = Half16<T>::pack(v.x, v.y);
+                }
+                tmem_st16(s_col + (kHalf / 2) * h + 16 * x, p);
+              }
+              sums[0] = add2(sums[0], sums[1]);
+              sum = sums[0].x + sums[0].y;
+            };
+            bool find = h == 0 && !started;
+            while (true) {
+              if (find) {
+                float top = m;
+#pragma unroll
+                for (int k = 0; k < kHalf; k += 2) top = max_nan(top, __uint_as_float(s[k]), __uint_as_float(s[k + 1]));
+                if (started || h == 1) {
+                  // the products so far must be in O: those of the tiles before are (these scores came after them)
+                  if (h == 1) ok = patience.wait(&half_done[i], s_uses & 1);
+                  if (!ok) break;
+                  tmem_fence_after_sync();
+                  const float f = m == -CUDART_INF_F ? 1.f : ex2((m - top) * a.scale2);
+                  l *= f;
+#pragma unroll 1
+                  for (int b = 0; b < D / 16; ++b) {
+                    uint32_t o[16];
+                    tmem_ld16(o, o_col + 16 * b);
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+                    tmem_st16(o_col + 16 * b, o);
+                  }
+                }
+                m = top;
+              }
+              probabilities();
+              if (find || !__any_sync(0xffffffffu, q_row >= 0 && (!(sum <= 32768.f) || m == -CUDART_INF_F))) break;
+              find = true;
+            }
+            if (!ok) break;
+            l += sum;
+            tmem_wait_st();
+            tmem_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[i][h]);
+          }
+          if (!ok) break;
+          ++s_uses;
+          started = true;
         }
-        if (!ok) break;
-        if (Bits == 16) ++s_uses;
-        started = true;
       }
       if (ok && more && !rows.q_mapped) {  // before this unit's result comes out
         ok = patience.wait(&q_free[i], unit & 1);
