@@ -86,6 +86,7 @@ constexpr int kMaxSms = 160;        // workspaces are sized for the largest devi
 
 template <int D, int Bits>
 struct PromptCfg {
+  static constexpr int kThreads = kPromptThreads + (Bits == 4 ? 128 : 0);
   static constexpr int kStages = D == 64 ? 8 : 4;
   static constexpr uint32_t kQBytes = kTile * D * 2;
   static constexpr uint32_t kTileBytes = kKeys * D * 2;
@@ -95,7 +96,9 @@ struct PromptCfg {
   // 4-bit pool: step and off of each key and group, for each stage that holds keys
   static constexpr int kKeyFloats = 2 * (D / kGroup4) * kKeys;
   static constexpr uint32_t kKeyBytes = Bits == 4 ? kStages / 2 * kKeyFloats * 4 : 0;
-  static constexpr uint32_t kRawBytes = Bits == 4 ? 2 * 4 * (D / kGroup4) * 32 * 20 : 0;  // the converters' (Convert4::Raw)
+  // ... and its converter warps: of keys and of values, and what is on its way to one (Convert4::Raw)
+  static constexpr int kKeyWarps = 2, kValueWarps = 4;
+  static constexpr uint32_t kRawBytes = Bits == 4 ? (kKeyWarps + kValueWarps) * 2 * (D / kGroup4) * (32 * 16 + 16 * 4) : 0;
   static constexpr size_t kSmem =
       1024 + 2 * static_cast<size_t>(kQBytes) + kStages * static_cast<size_t>(kTileBytes) + kOutBytes + kKeyBytes +
       kRawBytes;
@@ -508,19 +511,19 @@ __device__ __forceinline__ KeySpan unit_span(const Walk& w, bool prefix, int tq,
 
 // A converter warp of a 4-bit pool fills the ring's key tiles or its value tiles.
 // It takes 16 tokens at a time, two lanes a token: their codes and pairs are copied to
-// shared memory (each lane its own, kRaw pieces ahead) and from there converted into
+// shared memory (kRaw pieces ahead) and from there converted into
 // the tile as TMA would have written it (128-byte swizzle).  Values become 16-bit
 // values, keys 16 + code, which is exact: what belongs to them, step and off, goes
 // beside the tile.  Everything is in rolled loops, so that it fits the instruction
 // cache beside the softmax.
-constexpr int kRaw = 4;
+constexpr int kRaw = 2;
 
 template <typename T, int D>
 struct Convert4 {
   static constexpr int DB = D / 64, kPieces = kKeys / 16;
   struct Raw {
     uint4 codes[kRaw][DB][32];
-    uint32_t pair[kRaw][DB][32];
+    uint32_t pair[kRaw][DB][16];
   };
   Raw* raw;
 
@@ -534,9 +537,10 @@ struct Convert4 {
       asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(&raw->codes[slot][b][lane])),
                    "l"(block + in_page * (D / 2) + 32 * b + 16 * (lane & 1)), "r"(keep ? 16 : 0)
                    : "memory");
-      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_addr(&raw->pair[slot][b][lane])),
-                   "l"(block + block4_codes(c) + (in_page * DB + b) * 4), "r"(keep ? 4 : 0)
-                   : "memory");
+      if ((lane & 1) == 0)
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_addr(&raw->pair[slot][b][lane >> 1])),
+                     "l"(block + block4_codes(c) + (in_page * DB + b) * 4), "r"(keep ? 4 : 0)
+                     : "memory");
     }
   }
   template <typename F>
@@ -551,7 +555,7 @@ struct Convert4 {
   __device__ __forceinline__ void values(int slot, int row, unsigned char* tile) const {
 #pragma unroll 1
     for (int b = 0; b < DB; ++b) {
-      const uint32_t p = raw->pair[slot][b][threadIdx.x & 31];
+      const uint32_t p = raw->pair[slot][b][(threadIdx.x & 31) >> 1];
       const uint32_t step2 = __byte_perm(p, 0, 0x1010), low2 = __byte_perm(p, 0, 0x3232);
       put(slot, b, row, tile, [&](uint32_t w) {
         return make_uint4(value2<T>(codes2<T, 0>(w), step2, low2), value2<T>(codes2<T, 1>(w), step2, low2),
@@ -566,14 +570,14 @@ struct Convert4 {
       put(slot, b, row, tile, [&](uint32_t w) {
         return make_uint4(codes2<T, 0>(w), codes2<T, 1>(w), codes2<T, 2>(w), codes2<T, 3>(w));
       });
-      const float2 so = step_off(unpack2<T>(raw->pair[slot][b][lane]));
+      const float2 so = step_off(unpack2<T>(raw->pair[slot][b][lane >> 1]));
       beside[(2 * b + (lane & 1)) * kKeys + row] = (lane & 1) == 0 ? so.x : so.y;
     }
   }
 };
 
 template <typename T, int D, int Bits>
-__global__ void __launch_bounds__(kPromptThreads, 1)
+__global__ void __launch_bounds__(PromptCfg<D, Bits>::kThreads, 1)
     prompt_kernel(const __grid_constant__ CUtensorMap pool_map, const __grid_constant__ CUtensorMap q_map, PagedCache c, Attend a, PromptRows rows,
                   PromptSpace ws) {
   using C = PromptCfg<D, Bits>;
@@ -599,7 +603,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     for (int s = 0; s < S; ++s) {
       mbar_init(&kv_full[s], 1);
       mbar_init(&kv_empty[s], Bits == 4 && s % 2 == 0 ? 1 + 8 : 1);  // keys in 4 bits: the softmax warps too
-      mbar_init(&ready[s], 1);
+      mbar_init(&ready[s], Bits == 16 ? 1 : s % 2 == 0 ? C::kKeyWarps : C::kValueWarps);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_ready[i], rows.q_mapped ? 1 : 4);
@@ -628,8 +632,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   take_turn();
   if (rows.own_plan) {  // all CTAs write the same plan
     if (prefix)
-      for (int k = blockIdx.x * kPromptThreads + threadIdx.x; k < c.slots; k += gridDim.x * kPromptThreads) rows.base[k] = 0;
-    make_plan<kPromptThreads>(c, rows, ws, a.window, a.sinks, 2 * tq, gridDim.x, blockIdx.x, blockIdx.x + 1);
+      for (int k = blockIdx.x * C::kThreads + threadIdx.x; k < c.slots; k += gridDim.x * C::kThreads) rows.base[k] = 0;
+    make_plan<C::kThreads>(c, rows, ws, a.window, a.sinks, 2 * tq, gridDim.x, blockIdx.x, blockIdx.x + 1);
     __syncthreads();
   }
 
@@ -639,12 +643,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   if (threadIdx.x == 0) wait_limit = ws.waits.ns + static_cast<unsigned long long>(ws.waits.tile_ns) * (any ? w.end : 0);
   __syncthreads();
 
-  if (Bits == 4 && (warp == 9 || warp == 10)) {
-    // ---- 4-bit pool: warp 9 fills the ring's key tiles (the even places), warp 10 its value tiles.  Values that no query
-    // of the unit may see are zeros.
-    const int kv = warp - 9;
-    const Convert4<T, D> x{reinterpret_cast<typename Convert4<T, D>::Raw*>(key_pairs + C::kKeyBytes / 4) + kv};
-    static_assert(Bits == 16 || 2 * sizeof(typename Convert4<T, D>::Raw) == C::kRawBytes);
+  if (Bits == 4 && warp > 8 && warp != 11) {
+    // ---- 4-bit pool: warps 9 and 10 fill the ring's key tiles (the even places), 12 to 15 its value tiles.  Values that no
+    // query of the unit may see are zeros.
+    const int me = warp < 11 ? warp - 9 : warp - 10, kv = me < C::kKeyWarps ? 0 : 1;
+    using X = Convert4<T, D>;
+    const X x{reinterpret_cast<typename X::Raw*>(key_pairs + C::kKeyBytes / 4) + me};
+    static_assert(Bits == 16 || (C::kKeyWarps + C::kValueWarps) * sizeof(typename X::Raw) == C::kRawBytes);
+    // this warp's pieces of a tile
+    const int pieces = X::kPieces / (kv == 0 ? C::kKeyWarps : C::kValueWarps), first = (kv == 0 ? me : me - C::kKeyWarps) * pieces;
     int it = kv;
     for (bool more = any && !ws.waits.starve; more && alive(errv); more = w.next(ws)) {
       const Geom g = w.g;
@@ -656,7 +663,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       // the page of lane's 16 tokens of tile t
       auto page_of = [&](int t) {
         const int key = kKeys * span.tile(t) + 16 * lane;
-        return lane < x.kPieces && t < w.t1 && key < g.len ? table[key >> c.page_shift] : -1;
+        return lane < X::kPieces && t < w.t1 && key < g.len ? table[key >> c.page_shift] : -1;
       };
       // piece p of tile t into a slot of the raw ring
       auto ask = [&](int slot, int t, int p, int page) {
@@ -671,7 +678,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       };
       int page = page_of(w.t0), next_page = page_of(w.t0 + 1);
 #pragma unroll 1
-      for (int p = 0; p < kRaw; ++p) ask(p, w.t0, p, page);
+      for (int p = 0; p < kRaw; ++p) ask(p, w.t0, first + p, page);
       bool ok = true;
       for (int t = w.t0; ok && t < w.t1; ++t, it += 2) {
         const int ahead = page_of(t + 2);
@@ -680,15 +687,17 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         if (!ok) break;
         unsigned char* tile = ring + static_cast<size_t>(s) * C::kTileBytes;
 #pragma unroll 1
-        for (int p = 0; p < x.kPieces; ++p) {
+        for (int p = 0; p < pieces; ++p) {
           asm volatile("cp.async.wait_group %0;" ::"n"(kRaw - 1) : "memory");
-          const int row = 16 * p + (lane >> 1);
+          __syncwarp();
+          const int row = 16 * (first + p) + (lane >> 1);
           if (kv == 0)
             x.keys(p % kRaw, row, tile, key_pairs + s / 2 * C::kKeyFloats);
           else
             x.values(p % kRaw, row, tile);
-          const bool same = p + kRaw < x.kPieces;
-          ask(p % kRaw, same ? t : t + 1, (p + kRaw) % x.kPieces, same ? page : next_page);
+          __syncwarp();
+          const bool same = p + kRaw < pieces;
+          ask(p % kRaw, same ? t : t + 1, first + (same ? p + kRaw : p + kRaw - pieces), same ? page : next_page);
         }
         page = next_page;
         next_page = ahead;
@@ -1644,7 +1653,7 @@ cudaError_t run_prompt(const PagedCache& c, int dtype, const Attend& a, PromptRo
     if (e == cudaSuccess && !rows.own_plan)
       e = launch_serialized(prompt_plan_kernel, dim3(1), dim3(kPromptPlanThreads), 0, stream, c, rows, ws, a.window,
                             a.sinks, tokens_per_pair, sms);
-    if (e == cudaSuccess) e = launch_serialized(kernel, dim3(sms), dim3(kPromptThreads), smem, stream, map, q_map, c, a, rows, ws);
+    if (e == cudaSuccess) e = launch_serialized(kernel, dim3(sms), dim3(PromptCfg<D, Bits>::kThreads), smem, stream, map, q_map, c, a, rows, ws);
     if (e == cudaSuccess)
       e = launch_serialized(prompt_join_kernel<T, D>, dim3(4 * sms), dim3(kJoinThreads), 0, stream, c, a, rows, ws, sms);
     return e;
