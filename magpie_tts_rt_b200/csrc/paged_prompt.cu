@@ -93,7 +93,7 @@ struct PromptCfg {
   // a 32 x 64 block of results per softmax warp on its way out; 4-bit pool: 32 x 32, for room
   static constexpr int kOutRow = Bits == 4 ? 64 : 128;
   static constexpr uint32_t kOutBytes = 8 * 32 * kOutRow;
-  // 4-bit pool: step and off of each key and group, for each stage that holds keys
+  // 4-bit pool: step and off of each key and group, times scale2, for each stage that holds keys
   static constexpr int kKeyFloats = 2 * (D / kGroup4) * kKeys;
   static constexpr uint32_t kKeyBytes = Bits == 4 ? kStages / 2 * kKeyFloats * 4 : 0;
   // ... and its converter warps: of keys and of values, and what is on its way to one (Convert4::Raw)
@@ -563,7 +563,7 @@ struct Convert4 {
       });
     }
   }
-  __device__ __forceinline__ void keys(int slot, int row, unsigned char* tile, float* beside) const {
+  __device__ __forceinline__ void keys(int slot, int row, unsigned char* tile, float* beside, float scale2) const {
     const int lane = threadIdx.x & 31;
 #pragma unroll 1
     for (int b = 0; b < DB; ++b) {
@@ -571,7 +571,7 @@ struct Convert4 {
         return make_uint4(codes2<T, 0>(w), codes2<T, 1>(w), codes2<T, 2>(w), codes2<T, 3>(w));
       });
       const float2 so = step_off(unpack2<T>(raw->pair[slot][b][lane >> 1]));
-      beside[(2 * b + (lane & 1)) * kKeys + row] = (lane & 1) == 0 ? so.x : so.y;
+      beside[(2 * b + (lane & 1)) * kKeys + row] = ((lane & 1) == 0 ? so.x : so.y) * scale2;
     }
   }
 };
@@ -692,7 +692,7 @@ __global__ void __launch_bounds__(PromptCfg<D, Bits>::kThreads, 1)
           __syncwarp();
           const int row = 16 * (first + p) + (lane >> 1);
           if (kv == 0)
-            x.keys(p % kRaw, row, tile, key_pairs + s / 2 * C::kKeyFloats);
+            x.keys(p % kRaw, row, tile, key_pairs + s / 2 * C::kKeyFloats, a.scale2);
           else
             x.values(p % kRaw, row, tile);
           __syncwarp();
@@ -1100,38 +1100,33 @@ __global__ void __launch_bounds__(PromptCfg<D, Bits>::kThreads, 1)
 #pragma unroll 1
             for (int x = 0; x < kHalf; x += 32) {
               const int e0 = kHalf * h + x;  // the chunk's first key in the tile
-              uint32_t s[32];
-              tmem_ld32(s, s_col + x);
-              // of each group step (q.(16 + c)) + off sum q
+              // Of each group step (q.(16 + c)) + off sum q, in base 2 and less the maximum: four additions and products a
+              // score at head_dim 128.
+              const float less = m == -CUDART_INF_F ? 0.f : kPromptBias<T> - m;
+              uint32_t s[32], y[32];
+              if constexpr (DB == 2)
+                tmem_ld32x2(s, y, s_col + x, s_col + kHalf + x);
+              else
+                tmem_ld32(s, s_col + x);
+              const float2 less2 = make_float2(less, less);
 #pragma unroll
-              for (int b = 0; b < DB; ++b) {
-                const float2 of = make_float2(q_sum[b], q_sum[b]);
+              for (int e = 0; e < 32; e += 4) {
+                float2 v0 = less2, v1 = less2;
 #pragma unroll
-                for (int y0 = 0; y0 < 32; y0 += 16) {
-                  uint32_t y[16];
-                  if (b > 0) tmem_ld16(y, s_col + kHalf * b + x + y0);
-#pragma unroll
-                  for (int k = 0; k < 16; k += 4) {
-                    const int e = y0 + k;
-                    const float4 step = *reinterpret_cast<const float4*>(beside + 2 * b * kKeys + e0 + e);
-                    const float4 off = *reinterpret_cast<const float4*>(beside + (2 * b + 1) * kKeys + e0 + e);
-                    float2 v0 = make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1]));
-                    float2 v1 = make_float2(__uint_as_float(s[e + 2]), __uint_as_float(s[e + 3]));
-                    if (b == 0) {
-                      v0 = fma2(v0, make_float2(step.x, step.y), mul2(of, make_float2(off.x, off.y)));
-                      v1 = fma2(v1, make_float2(step.z, step.w), mul2(of, make_float2(off.z, off.w)));
-                    } else {
-                      v0 = fma2(of, make_float2(off.x, off.y), v0);
-                      v1 = fma2(of, make_float2(off.z, off.w), v1);
-                      v0 = fma2(make_float2(__uint_as_float(y[k]), __uint_as_float(y[k + 1])), make_float2(step.x, step.y), v0);
-                      v1 = fma2(make_float2(__uint_as_float(y[k + 2]), __uint_as_float(y[k + 3])), make_float2(step.z, step.w), v1);
-                    }
-                    s[e] = __float_as_uint(v0.x);
-                    s[e + 1] = __float_as_uint(v0.y);
-                    s[e + 2] = __float_as_uint(v1.x);
-                    s[e + 3] = __float_as_uint(v1.y);
-                  }
+                for (int b = 0; b < DB; ++b) {
+                  const uint32_t(&z)[32] = b == 0 ? s : y;
+                  const float2 of = make_float2(q_sum[b], q_sum[b]);
+                  const float4 step = *reinterpret_cast<const float4*>(beside + 2 * b * kKeys + e0 + e);
+                  const float4 off = *reinterpret_cast<const float4*>(beside + (2 * b + 1) * kKeys + e0 + e);
+                  v0 = fma2(of, make_float2(off.x, off.y), v0);
+                  v1 = fma2(of, make_float2(off.z, off.w), v1);
+                  v0 = fma2(make_float2(__uint_as_float(z[e]), __uint_as_float(z[e + 1])), make_float2(step.x, step.y), v0);
+                  v1 = fma2(make_float2(__uint_as_float(z[e + 2]), __uint_as_float(z[e + 3])), make_float2(step.z, step.w), v1);
                 }
+                s[e] = __float_as_uint(v0.x);
+                s[e + 1] = __float_as_uint(v0.y);
+                s[e + 2] = __float_as_uint(v1.x);
+                s[e + 3] = __float_as_uint(v1.y);
               }
               if (!all) {
                 const int from = base + e0;
@@ -1147,11 +1142,15 @@ __global__ void __launch_bounds__(PromptCfg<D, Bits>::kThreads, 1)
               bool find = e0 == 0 && !started;
               while (true) {
                 if (find) {
-                  float top = m;
+                  float top = -CUDART_INF_F;
 #pragma unroll
                   for (int k = 0; k < 32; k += 2) top = max_nan(top, __uint_as_float(s[k]), __uint_as_float(s[k + 1]));
+                  top = max_nan(m, top - less, top - less);
+                  const float more = (top == -CUDART_INF_F ? 0.f : kPromptBias<T> - top) - less;
+#pragma unroll
+                  for (int k = 0; k < 32; ++k) s[k] = __float_as_uint(__uint_as_float(s[k]) + more);
                   // the products so far are in O: these scores came after them
-                  const float f = m == -CUDART_INF_F ? 1.f : ex2((m - top) * a.scale2);
+                  const float f = m == -CUDART_INF_F ? 1.f : ex2(m - top);
                   l *= f;
                   if (started || h == 1) {
 #pragma unroll 1
@@ -1176,15 +1175,11 @@ __global__ void __launch_bounds__(PromptCfg<D, Bits>::kThreads, 1)
                   }
                   m = top;
                 }
-                const float off = m == -CUDART_INF_F ? 0.f : fmaf(-m, a.scale2, kPromptBias<T>);
-                const float2 scale = make_float2(a.scale2, a.scale2), offs = make_float2(off, off);
                 float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
                 uint32_t p[16];
 #pragma unroll
                 for (int k = 0; k < 16; ++k) {
-                  float2 v = fma2(make_float2(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1])), scale, offs);
-                  v.x = ex2(v.x);
-                  v.y = ex2(v.y);
+                  const float2 v = make_float2(ex2(__uint_as_float(s[2 * k])), ex2(__uint_as_float(s[2 * k + 1])));
                   // the sum keeps the unrounded probabilities; the values' weights are rounded to 16 bits once
                   sums[k & 1] = add2(sums[k & 1], v);
                   p[k] = Half16<T>::pack(v.x, v.y);
@@ -1305,7 +1300,7 @@ __global__ void __launch_bounds__(PromptCfg<D, Bits>::kThreads, 1)
       }
       tmem_fence_after_sync();
       const float inv = l == 0.f ? 0.f : 1.f / l;
-      const float m2 = m == -CUDART_INF_F ? m : fmaf(m, a.scale2, -kPromptBias<T>);
+      const float m2 = Bits == 4 || m == -CUDART_INF_F ? m - kPromptBias<T> : fmaf(m, a.scale2, -kPromptBias<T>);
       const bool there = q_row >= 0;
       float* part = ws.part + static_cast<int64_t>(part_at) * (D + 2) * kPairRows + i * kTile + r;
       float* state = prefix && there ? rows.state + (static_cast<int64_t>(q_row) * a.q_heads + q_head) * (D + 4) : nullptr;
