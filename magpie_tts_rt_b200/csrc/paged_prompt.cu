@@ -93,15 +93,11 @@ struct PromptCfg {
   // a 32 x 64 block of results per softmax warp on its way out; 4-bit pool: 32 x 32, for room
   static constexpr int kOutRow = Bits == 4 ? 64 : 128;
   static constexpr uint32_t kOutBytes = 8 * 32 * kOutRow;
-  // 4-bit pool: step and off of each key and group, times scale2, for each stage that holds keys
-  static constexpr int kKeyFloats = 2 * (D / kGroup4) * kKeys;
-  static constexpr uint32_t kKeyBytes = Bits == 4 ? kStages / 2 * kKeyFloats * 4 : 0;
-  // ... and its converter warps: of keys and of values, and what is on its way to one (Convert4::Raw)
-  static constexpr int kKeyWarps = 2, kValueWarps = 4;
-  static constexpr uint32_t kRawBytes = Bits == 4 ? (kKeyWarps + kValueWarps) * 2 * (D / kGroup4) * (32 * 16 + 16 * 4) : 0;
+  // 4-bit pool: what is on its way to each of the converter warps (Convert4::Raw)
+  static constexpr int kConverters = 6, kRaw = D == 64 ? 2 : 4;
+  static constexpr uint32_t kRawBytes = Bits == 4 ? kConverters * kRaw * (32 * 16 + 16 * 4) : 0;
   static constexpr size_t kSmem =
-      1024 + 2 * static_cast<size_t>(kQBytes) + kStages * static_cast<size_t>(kTileBytes) + kOutBytes + kKeyBytes +
-      kRawBytes;
+      1024 + 2 * static_cast<size_t>(kQBytes) + kStages * static_cast<size_t>(kTileBytes) + kOutBytes + kRawBytes;
 };
 
 // Rows of the attention: tokens of slots, or members of prefix groups.
@@ -509,69 +505,75 @@ __device__ __forceinline__ KeySpan unit_span(const Walk& w, bool prefix, int tq,
   return KeySpan(p0, max(p0, p1), a.window, a.sinks);
 }
 
-// A converter warp of a 4-bit pool fills the ring's key tiles or its value tiles.
-// It takes 16 tokens at a time, two lanes a token: their codes and pairs are copied to
-// shared memory (kRaw pieces ahead) and from there converted into
-// the tile as TMA would have written it (128-byte swizzle).  Values become 16-bit
-// values, keys 16 + code, which is exact: what belongs to them, step and off, goes
-// beside the tile.  Everything is in rolled loops, so that it fits the instruction
-// cache beside the softmax.
-constexpr int kRaw = 2;
-
+// The converter warps of a 4-bit pool fill the ring: a stage holds a key tile's
+// values, or half a tile's keys.  Values are rounded to 16 bits.  Keys are written as
+// two 16-bit numbers each, the second one what rounding leaves of the first, which a
+// second pass of the product adds: a score is then right to 2^-16 of its terms, as
+// rounding keys once (2^-8) would show in every log-sum-exp.
+// A piece is 16 tokens' 64 dims of a group, two lanes a token.  Its codes and pairs are
+// copied to shared memory (kRaw pieces ahead) and from there converted into the stage,
+// laid out as TMA would have written it (128-byte swizzle).  Everything is in rolled
+// loops: beside the softmax's code it has to fit the instruction cache (unrolled, 8192
+// tokens took 2.5 ms, in which the warps waited for instructions).
 template <typename T, int D>
 struct Convert4 {
-  static constexpr int DB = D / 64, kPieces = kKeys / 16;
+  static constexpr int DB = D / 64, kRaw = PromptCfg<D, 4>::kRaw;
   struct Raw {
-    uint4 codes[kRaw][DB][32];
-    uint32_t pair[kRaw][DB][16];
+    uint4 codes[kRaw][32];
+    uint32_t pair[kRaw][16];
   };
   Raw* raw;
 
   // the lane's token `key`, from the page that holds it; zeros if it is not to be read
-  __device__ __forceinline__ void ask(const PagedCache& c, int slot, int page, int layer, int kv, int head, int key, bool keep) const {
+  __device__ __forceinline__ void ask(const PagedCache& c, int slot, int page, int layer, int kv, int head, int b, int key,
+                                      bool keep) const {
     const int lane = threadIdx.x & 31, in_page = key & (c.page_size - 1);
     keep = keep && c.is_page(page);
     const unsigned char* block = block4(c, keep ? page : 0, layer, kv, head);
-#pragma unroll
-    for (int b = 0; b < DB; ++b) {
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(&raw->codes[slot][b][lane])),
-                   "l"(block + in_page * (D / 2) + 32 * b + 16 * (lane & 1)), "r"(keep ? 16 : 0)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(&raw->codes[slot][lane])),
+                 "l"(block + in_page * (D / 2) + 32 * b + 16 * (lane & 1)), "r"(keep ? 16 : 0)
+                 : "memory");
+    if ((lane & 1) == 0)
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_addr(&raw->pair[slot][lane >> 1])),
+                   "l"(block + block4_codes(c) + (in_page * DB + b) * 4), "r"(keep ? 4 : 0)
                    : "memory");
-      if ((lane & 1) == 0)
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_addr(&raw->pair[slot][b][lane >> 1])),
-                     "l"(block + block4_codes(c) + (in_page * DB + b) * 4), "r"(keep ? 4 : 0)
-                     : "memory");
-    }
   }
-  template <typename F>
-  __device__ __forceinline__ void put(int slot, int b, int row, unsigned char* tile, F word) const {
+  // `block`: 128-byte rows of the stage
+  __device__ __forceinline__ void values(int slot, int row, unsigned char* block) const {
     const int lane = threadIdx.x & 31;
-    const uint4 x = raw->codes[slot][b][lane];
-    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-    unsigned char* to = tile + b * (kKeys * 128) + row * 128;
+    const uint4 x = raw->codes[slot][lane];
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w}, p = raw->pair[slot][lane >> 1];
+    const uint32_t step2 = __byte_perm(p, 0, 0x1010), low2 = __byte_perm(p, 0, 0x3232);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) *reinterpret_cast<uint4*>(to + 16 * ((4 * (lane & 1) + k) ^ (row & 7))) = word(w[k]);
+    for (int k = 0; k < 4; ++k)
+      *reinterpret_cast<uint4*>(block + row * 128 + 16 * ((4 * (lane & 1) + k) ^ (row & 7))) =
+          make_uint4(value2<T>(codes2<T, 0>(w[k]), step2, low2), value2<T>(codes2<T, 1>(w[k]), step2, low2),
+                     value2<T>(codes2<T, 2>(w[k]), step2, low2), value2<T>(codes2<T, 3>(w[k]), step2, low2));
   }
-  __device__ __forceinline__ void values(int slot, int row, unsigned char* tile) const {
-#pragma unroll 1
-    for (int b = 0; b < DB; ++b) {
-      const uint32_t p = raw->pair[slot][b][(threadIdx.x & 31) >> 1];
-      const uint32_t step2 = __byte_perm(p, 0, 0x1010), low2 = __byte_perm(p, 0, 0x3232);
-      put(slot, b, row, tile, [&](uint32_t w) {
-        return make_uint4(value2<T>(codes2<T, 0>(w), step2, low2), value2<T>(codes2<T, 1>(w), step2, low2),
-                          value2<T>(codes2<T, 2>(w), step2, low2), value2<T>(codes2<T, 3>(w), step2, low2));
-      });
-    }
-  }
-  __device__ __forceinline__ void keys(int slot, int row, unsigned char* tile, float* beside, float scale2) const {
+  // the rounded keys into `block`, the rest into the block `rest` bytes on
+  __device__ __forceinline__ void keys(int slot, int row, unsigned char* block, int rest) const {
     const int lane = threadIdx.x & 31;
-#pragma unroll 1
-    for (int b = 0; b < DB; ++b) {
-      put(slot, b, row, tile, [&](uint32_t w) {
-        return make_uint4(codes2<T, 0>(w), codes2<T, 1>(w), codes2<T, 2>(w), codes2<T, 3>(w));
-      });
-      const float2 so = step_off(unpack2<T>(raw->pair[slot][b][lane >> 1]));
-      beside[(2 * b + (lane & 1)) * kKeys + row] = ((lane & 1) == 0 ? so.x : so.y) * scale2;
+    const uint4 x = raw->codes[slot][lane];
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    const float2 so = step_off(unpack2<T>(raw->pair[slot][lane >> 1]));
+    const float2 step = make_float2(so.x, so.x), off = make_float2(so.y, so.y);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        // 16 + code in f32, as in codes2
+        const uint32_t a = i == 0 ? w[k] << 19 : i == 1 ? w[k] << 15 : i == 2 ? w[k] << 11 : w[k] << 7;
+        const uint32_t b = i == 0 ? w[k] << 3 : w[k] >> (4 * i - 3);
+        const float2 v = fma2(make_float2(__uint_as_float((a & 0x00780000u) | 0x41800000u),
+                                          __uint_as_float((b & 0x00780000u) | 0x41800000u)), step, off);
+        hi[i] = Half16<T>::pack(v.x, v.y);
+        const float2 h = unpack2<T>(hi[i]), r = add2(v, make_float2(-h.x, -h.y));
+        lo[i] = Half16<T>::pack(r.x, r.y);
+      }
+      unsigned char* to = block + row * 128 + 16 * ((4 * (lane & 1) + k) ^ (row & 7));
+      *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+      *reinterpret_cast<uint4*>(to + rest) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     }
   }
 };
@@ -587,6 +589,7 @@ __global__ void __launch_bounds__(PromptCfg<D, Bits>::kThreads, 1)
   extern __shared__ unsigned char prompt_smem[];
   __shared__ unsigned long long kv_full[S], kv_empty[S], ready[S], q_ready[2], s_full[2], p_full[2][2], half_done[2],
       o_full[2], q_free[2], fin;
+  __shared__ unsigned long long s_half[2][2], pv_done[2][2];  // 4-bit pool: of each half of a key tile
   __shared__ uint32_t tmem_base;
   __shared__ unsigned long long wait_limit;
   __shared__ int err;
@@ -594,7 +597,6 @@ __global__ void __launch_bounds__(PromptCfg<D, Bits>::kThreads, 1)
   unsigned char* q_smem = prompt_smem + pad;
   unsigned char* ring = q_smem + 2 * C::kQBytes;
   unsigned char* out_smem = ring + static_cast<size_t>(S) * C::kTileBytes;
-  float* key_pairs = reinterpret_cast<float*>(out_smem + C::kOutBytes);
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const bool prefix = rows.members != nullptr;
   const int tq = kTile / a.group;  // tokens of a Q tile
@@ -602,8 +604,8 @@ __global__ void __launch_bounds__(PromptCfg<D, Bits>::kThreads, 1)
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
       mbar_init(&kv_full[s], 1);
-      mbar_init(&kv_empty[s], Bits == 4 && s % 2 == 0 ? 1 + 8 : 1);  // keys in 4 bits: the softmax warps too
-      mbar_init(&ready[s], Bits == 16 ? 1 : s % 2 == 0 ? C::kKeyWarps : C::kValueWarps);
+      mbar_init(&kv_empty[s], 1);
+      mbar_init(&ready[s], Bits == 4 ? C::kConverters : 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_ready[i], rows.q_mapped ? 1 : 4);
@@ -612,7 +614,11 @@ __global__ void __launch_bounds__(PromptCfg<D, Bits>::kThreads, 1)
       mbar_init(&p_full[i][1], 4);
       mbar_init(&half_done[i], 1);
       mbar_init(&o_full[i], 1);
-      mbar_init(&q_free[i], Bits == 4 ? 1 + 4 : 1);
+      mbar_init(&q_free[i], 1);
+      for (int h = 0; h < 2; ++h) {
+        mbar_init(&s_half[i][h], 1);
+        mbar_init(&pv_done[i][h], 1);
+      }
     }
     mbar_init(&fin, 1);
     err = 0;
@@ -644,15 +650,16 @@ __global__ void __launch_bounds__(PromptCfg<D, Bits>::kThreads, 1)
   __syncthreads();
 
   if (Bits == 4 && warp > 8 && warp != 11) {
-    // ---- 4-bit pool: warps 9 and 10 fill the ring's key tiles (the even places), 12 to 15 its value tiles.  Values that no
-    // query of the unit may see are zeros.
-    const int me = warp < 11 ? warp - 9 : warp - 10, kv = me < C::kKeyWarps ? 0 : 1;
+    // ---- 4-bit pool: converters.  The ring's order: both halves of a tile's keys, its values.  A tile's pieces are dealt
+    // to the warps in turn.  Values that no query of the unit may see are zeros.
     using X = Convert4<T, D>;
-    const X x{reinterpret_cast<typename X::Raw*>(key_pairs + C::kKeyBytes / 4) + me};
-    static_assert(Bits == 16 || (C::kKeyWarps + C::kValueWarps) * sizeof(typename X::Raw) == C::kRawBytes);
-    // this warp's pieces of a tile
-    const int pieces = X::kPieces / (kv == 0 ? C::kKeyWarps : C::kValueWarps), first = (kv == 0 ? me : me - C::kKeyWarps) * pieces;
-    int it = kv;
+    const int me = warp < 11 ? warp - 9 : warp - 10;
+    const X x{reinterpret_cast<typename X::Raw*>(out_smem + C::kOutBytes) + me};
+    static_assert(Bits == 16 || C::kConverters * sizeof(typename X::Raw) == C::kRawBytes);
+    constexpr int kHalfPieces = kHalf / 16 * DB, kTilePieces = 4 * kHalfPieces;  // keys' halves, then values
+    constexpr int kAhead = C::kConverters * C::kRaw;
+    static_assert(kAhead <= kTilePieces);
+    int it = 0;
     for (bool more = any && !ws.waits.starve; more && alive(errv); more = w.next(ws)) {
       const Geom g = w.g;
       const KeySpan span = unit_span(w, prefix, tq, a);
@@ -663,47 +670,56 @@ __global__ void __launch_bounds__(PromptCfg<D, Bits>::kThreads, 1)
       // the page of lane's 16 tokens of tile t
       auto page_of = [&](int t) {
         const int key = kKeys * span.tile(t) + 16 * lane;
-        return lane < X::kPieces && t < w.t1 && key < g.len ? table[key >> c.page_shift] : -1;
+        return lane < kKeys / 16 && t < w.t1 && key < g.len ? table[key >> c.page_shift] : -1;
       };
-      // piece p of tile t into a slot of the raw ring
-      auto ask = [&](int slot, int t, int p, int page) {
-        const int j = kKeys * span.tile(t) + 16 * p + (lane >> 1);
-        page = __shfl_sync(0xffffffffu, page, p);
+      // piece n of a tile into a slot of the raw ring
+      auto ask = [&](int slot, int t, int n, int page) {
+        const int kv = n >= 2 * kHalfPieces ? 1 : 0, sub = n - 2 * kHalfPieces * kv, rows = sub / DB;
+        const int j = kKeys * span.tile(t) + 16 * rows + (lane >> 1);
+        page = __shfl_sync(0xffffffffu, page, rows);
         if (t < w.t1) {
           bool keep = j < g.len;
           if (kv == 1) keep = j <= p1 && (a.window == 0 || j > p0 - a.window || j < a.sinks) && (mask == nullptr || mask[j]);
-          x.ask(c, slot, page, a.layer, kv, w.head, j, keep);
+          x.ask(c, slot, page, a.layer, kv, w.head, sub % DB, j, keep);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
       };
       int page = page_of(w.t0), next_page = page_of(w.t0 + 1);
+      int n = me, slot = 0;  // this warp's next piece of the tile
 #pragma unroll 1
-      for (int p = 0; p < kRaw; ++p) ask(p, w.t0, first + p, page);
+      for (int k = 0; k < C::kRaw; ++k) ask(k, w.t0, me + C::kConverters * k, page);
       bool ok = true;
-      for (int t = w.t0; ok && t < w.t1; ++t, it += 2) {
+      for (int t = w.t0; ok && t < w.t1; ++t) {
         const int ahead = page_of(t + 2);
-        const int s = it % S;
-        ok = it < S || patience.wait(&kv_empty[s], ((it / S) - 1) & 1);
-        if (!ok) break;
-        unsigned char* tile = ring + static_cast<size_t>(s) * C::kTileBytes;
 #pragma unroll 1
-        for (int p = 0; p < pieces; ++p) {
-          asm volatile("cp.async.wait_group %0;" ::"n"(kRaw - 1) : "memory");
+        for (int e = 0; e < 3; ++e, ++it) {
+          const int s = it % S, end = (e == 2 ? 4 : e + 1) * kHalfPieces;
+          ok = it < S || patience.wait(&kv_empty[s], ((it / S) - 1) & 1);
+          if (!ok) break;
+          unsigned char* stage = ring + static_cast<size_t>(s) * C::kTileBytes;
+#pragma unroll 1
+          for (; n < end; n += C::kConverters) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(C::kRaw - 1) : "memory");
+            __syncwarp();
+            if (e < 2) {
+              const int sub = n - kHalfPieces * e;
+              x.keys(slot, 16 * (sub / DB) + (lane >> 1), stage + sub % DB * (kHalf * 128), DB * kHalf * 128);
+            } else {
+              const int sub = n - 2 * kHalfPieces;
+              x.values(slot, 16 * (sub / DB) + (lane >> 1), stage + sub % DB * (kKeys * 128));
+            }
+            __syncwarp();
+            const int then = n + kAhead;
+            ask(slot, then < kTilePieces ? t : t + 1, then & (kTilePieces - 1), then < kTilePieces ? page : next_page);
+            slot = (slot + 1) & (C::kRaw - 1);
+          }
+          fence_proxy_async();
           __syncwarp();
-          const int row = 16 * (first + p) + (lane >> 1);
-          if (kv == 0)
-            x.keys(p % kRaw, row, tile, key_pairs + s / 2 * C::kKeyFloats, a.scale2);
-          else
-            x.values(p % kRaw, row, tile);
-          __syncwarp();
-          const bool same = p + kRaw < pieces;
-          ask(p % kRaw, same ? t : t + 1, first + (same ? p + kRaw : p + kRaw - pieces), same ? page : next_page);
+          if (lane == 0) mbar_arrive(&ready[s]);
         }
+        n -= kTilePieces;
         page = next_page;
         next_page = ahead;
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&ready[s]);
       }
       if (!ok) *errv = 1;
       cp_async_wait_all();
@@ -850,17 +866,17 @@ __global__ void __launch_bounds__(PromptCfg<D, Bits>::kThreads, 1)
       if (elect_one()) umma_commit(bar);
       __syncwarp();
     };
-    // 4-bit pool: a product for each group of dims, for 64 keys
+    // 4-bit pool: 64 keys, each in two numbers, into half h of the Q tile's columns
     auto scores4 = [&](int i, int s, int h) {
-      const uint32_t qd = q_lo + i * (C::kQBytes >> 4), kd = k_lo + s * kTileStep + h * (kHalf * 128 >> 4);
+      const uint32_t qd = q_lo + i * (C::kQBytes >> 4), kd = k_lo + s * kTileStep;
       if (elect_one()) {
 #pragma unroll
-        for (int d = 0; d < DB; ++d)
+        for (int d = 0; d < 2 * DB; ++d)
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)
-            umma_ss(tmem + kSCol + i * kKeys + d * kHalf, qd + d * kBlock + 2 * kk, kd + d * kBlock + 2 * kk,
-                    prompt_idesc<T>(kHalf, false), kk != 0);
-        umma_commit(&s_full[i]);
+            umma_ss(tmem + kSCol + i * kKeys + h * kHalf, qd + d % DB * kBlock + 2 * kk, kd + d * (kHalf * 128 >> 4) + 2 * kk,
+                    prompt_idesc<T>(kHalf, false), (d | kk) != 0);
+        umma_commit(&s_half[i][h]);
       }
       __syncwarp();
     };
@@ -888,7 +904,6 @@ __global__ void __launch_bounds__(PromptCfg<D, Bits>::kThreads, 1)
           tmem_fence_after_sync();
           if constexpr (Bits == 4) {
             if (seen[i].at(span.tile(t0))) scores4(i, it % S, 0);
-            if (last[i] < t0) commit(&q_free[i]);
           } else {
             if (seen[i].at(span.tile(t0))) scores(i, it % S);
             if (last[i] <= t0) commit(&q_free[i]);  // (a Q tile without key tiles in this share: at once)
@@ -897,13 +912,30 @@ __global__ void __launch_bounds__(PromptCfg<D, Bits>::kThreads, 1)
       }
       ++q_uses;
       if constexpr (Bits == 4) {
-        for (int t = t0; ok && t < t1; ++t, it += 2) {
-          const int ks = it % S, vs = (it + 1) % S, next_ks = (it + 2) % S;
+        // The ring holds K0 K1 V of each tile (halves of its keys, its values).  A half's scores have columns of their own,
+        // so that the next tile's are made as soon as P V of the same half is under way.
+        if (ok) commit(&kv_empty[it % S]);
+        ++it;
+        ok = ok && patience.wait(&ready[it % S], (it / S) & 1);
+        if (ok) {
+          tmem_fence_after_sync();
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            if (seen[i].at(span.tile(t0))) scores4(i, it % S, 1);
+            if (last[i] <= t0) commit(&q_free[i]);  // (a Q tile without key tiles in this share: at once)
+          }
+          commit(&kv_empty[it % S]);
+        }
+        ++it;
+        for (int t = t0; ok && t < t1; ++t) {
+          const int vs = it % S;
           const bool next = t + 1 < t1;
           const int j = span.tile(t), j1 = next ? span.tile(t + 1) : 0;
-          ok = patience.wait(&ready[vs], ((it + 1) / S) & 1);
+          ok = patience.wait(&ready[vs], (it / S) & 1);
+          ++it;
 #pragma unroll 1
           for (int h = 0; h < 2; ++h) {
+            const int ks = it % S;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               if (seen[i].at(j)) {
@@ -914,8 +946,9 @@ __global__ void __launch_bounds__(PromptCfg<D, Bits>::kThreads, 1)
                   if (elect_one()) {
 #pragma unroll
                     for (int kk = 0; kk < kHalf / 16; ++kk)
-                      umma_ts(tmem + kOCol + i * D, tmem + kSCol + i * kKeys + 8 * kk, vd + kk * (2048 >> 4),
+                      umma_ts(tmem + kOCol + i * D, tmem + kSCol + i * kKeys + h * kHalf + 8 * kk, vd + kk * (2048 >> 4),
                               prompt_idesc<T>(D, true), started[i] || kk != 0);
+                    umma_commit(&pv_done[i][h]);
                   }
                   __syncwarp();
                 }
@@ -923,18 +956,23 @@ __global__ void __launch_bounds__(PromptCfg<D, Bits>::kThreads, 1)
                 if (h == 1) {
                   ++p_uses[i];
                   if (ok && t == last[i]) commit(&o_full[i]);
-                } else if (ok) {
-                  scores4(i, ks, 1);
-                  if (t == last[i]) commit(&q_free[i]);
                 }
               }
-              if (h == 1 && next) {
-                if (i == 0) ok = ok && patience.wait(&ready[next_ks], ((it + 2) / S) & 1);
-                if (ok && seen[i].at(j1)) scores4(i, next_ks, 0);
+              if (next) {
+                if (i == 0) {
+                  ok = ok && patience.wait(&ready[ks], (it / S) & 1);
+                  if (ok) tmem_fence_after_sync();
+                }
+                if (ok && seen[i].at(j1)) {
+                  scores4(i, ks, h);
+                  if (h == 1 && t + 1 == last[i]) commit(&q_free[i]);
+                }
               }
             }
-            if (ok) commit(h == 0 ? &kv_empty[ks] : &kv_empty[vs]);
+            if (ok && next) commit(&kv_empty[ks]);
+            if (next) ++it;
           }
+          if (ok) commit(&kv_empty[vs]);
         }
         if (!ok) *errv = 1;
         continue;
@@ -996,7 +1034,6 @@ __global__ void __launch_bounds__(PromptCfg<D, Bits>::kThreads, 1)
     // sectors with every instruction, which took longer than several key tiles).
     const int piece = lane & 7, sub_row = lane >> 3;
     int s_uses = 0, o_uses = 0, unit = 0;
-    int key_it = 0;  // 4-bit pool: the ring's place of the next key tile
     // this thread's row of unit u: q and out row, or -1
     auto row_of = [&](const Walk& u) {
       const int tok = u.tok0 + i * tq + tok_in_tile;
@@ -1047,34 +1084,9 @@ __global__ void __launch_bounds__(PromptCfg<D, Bits>::kThreads, 1)
       const int next_row = more ? row_of(w) : -1;
       float m = -CUDART_INF_F, l = 0.f;
       bool ok = true, started = false;
-      float q_sum[DB] = {};  // 4-bit pool: of the row's queries, over each group
-      if constexpr (Bits == 4) {
-        ok = patience.wait(&q_ready[i], unit & 1);
-        if (ok) {
-          const unsigned char* mine = q_smem + i * C::kQBytes + r * 128;
-#pragma unroll
-          for (int b = 0; b < DB; ++b)
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              const uint4 x = *reinterpret_cast<const uint4*>(mine + b * (kTile * 128) + 16 * (k ^ (r & 7)));
-              const float2 f0 = unpack2<T>(x.x), f1 = unpack2<T>(x.y), f2 = unpack2<T>(x.z), f3 = unpack2<T>(x.w);
-              q_sum[b] += ((f0.x + f0.y) + (f1.x + f1.y)) + ((f2.x + f2.y) + (f3.x + f3.y));
-            }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&q_free[i]);
-        }
-      }
-      for (int t = t0; ok && t < t1; ++t) {
+      for (int t = t0; t < t1; ++t) {
         const int j = span.tile(t);
-        const int ks = key_it % S, k_round = (key_it / S) & 1;
-        key_it += 2;
-        if (!seen.at(j)) {
-          if constexpr (Bits == 4) {  // (not before the tile is there: it would count for the one before it)
-            ok = patience.wait(&ready[ks], k_round);
-            if (ok && lane == 0) mbar_arrive(&kv_empty[ks]);
-          }
-          continue;
-        }
+        if (!seen.at(j)) continue;
         const int base = kKeys * j;
         const bool all = mask == nullptr && tile_full(j, q0, q1, a.window, a.sinks) && base + kKeys <= len;
         uint32_t kept[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
@@ -1086,48 +1098,18 @@ __global__ void __launch_bounds__(PromptCfg<D, Bits>::kThreads, 1)
           for (int x = 0; x < 4; ++x) kept[x] = __ballot_sync(0xffffffffu, on[x]);
         }
         if constexpr (Bits == 4) {
-          // 32 keys at a time, in one copy of the code: beside the converter warps' it has to fit the instruction cache (with
-          // 64 and two copies 8192 tokens took 2.5 ms, in which the converters had half a tile's time to wait for
-          // instructions)
-          ok = patience.wait(&ready[ks], k_round);
-          if (!ok) break;
-          const float* beside = key_pairs + ks / 2 * C::kKeyFloats;
+          // 32 keys at a time, in one copy of the code (see Convert4)
 #pragma unroll 1
           for (int h = 0; h < 2; ++h) {
-            ok = patience.wait(&s_full[i], s_uses++ & 1);
+            ok = patience.wait(&s_half[i][h], s_uses & 1);
             if (!ok) break;
             tmem_fence_after_sync();
+            const uint32_t h_col = s_col + kHalf * h;
 #pragma unroll 1
             for (int x = 0; x < kHalf; x += 32) {
               const int e0 = kHalf * h + x;  // the chunk's first key in the tile
-              // Of each group step (q.(16 + c)) + off sum q, in base 2 and less the maximum: four additions and products a
-              // score at head_dim 128.
-              const float less = m == -CUDART_INF_F ? 0.f : kPromptBias<T> - m;
-              uint32_t s[32], y[32];
-              if constexpr (DB == 2)
-                tmem_ld32x2(s, y, s_col + x, s_col + kHalf + x);
-              else
-                tmem_ld32(s, s_col + x);
-              const float2 less2 = make_float2(less, less);
-#pragma unroll
-              for (int e = 0; e < 32; e += 4) {
-                float2 v0 = less2, v1 = less2;
-#pragma unroll
-                for (int b = 0; b < DB; ++b) {
-                  const uint32_t(&z)[32] = b == 0 ? s : y;
-                  const float2 of = make_float2(q_sum[b], q_sum[b]);
-                  const float4 step = *reinterpret_cast<const float4*>(beside + 2 * b * kKeys + e0 + e);
-                  const float4 off = *reinterpret_cast<const float4*>(beside + (2 * b + 1) * kKeys + e0 + e);
-                  v0 = fma2(of, make_float2(off.x, off.y), v0);
-                  v1 = fma2(of, make_float2(off.z, off.w), v1);
-                  v0 = fma2(make_float2(__uint_as_float(z[e]), __uint_as_float(z[e + 1])), make_float2(step.x, step.y), v0);
-                  v1 = fma2(make_float2(__uint_as_float(z[e + 2]), __uint_as_float(z[e + 3])), make_float2(step.z, step.w), v1);
-                }
-                s[e] = __float_as_uint(v0.x);
-                s[e + 1] = __float_as_uint(v0.y);
-                s[e + 2] = __float_as_uint(v1.x);
-                s[e + 3] = __float_as_uint(v1.y);
-              }
+              uint32_t s[32];
+              tmem_ld32(s, h_col + x);
               if (!all) {
                 const int from = base + e0;
                 const int hi = min(pos + 1, len) - from;
@@ -1142,17 +1124,16 @@ __global__ void __launch_bounds__(PromptCfg<D, Bits>::kThreads, 1)
               bool find = e0 == 0 && !started;
               while (true) {
                 if (find) {
-                  float top = -CUDART_INF_F;
+                  float top = m;
 #pragma unroll
                   for (int k = 0; k < 32; k += 2) top = max_nan(top, __uint_as_float(s[k]), __uint_as_float(s[k + 1]));
-                  top = max_nan(m, top - less, top - less);
-                  const float more = (top == -CUDART_INF_F ? 0.f : kPromptBias<T> - top) - less;
-#pragma unroll
-                  for (int k = 0; k < 32; ++k) s[k] = __float_as_uint(__uint_as_float(s[k]) + more);
-                  // the products so far are in O: these scores came after them
-                  const float f = m == -CUDART_INF_F ? 1.f : ex2(m - top);
+                  const float f = m == -CUDART_INF_F ? 1.f : ex2((m - top) * a.scale2);
                   l *= f;
                   if (started || h == 1) {
+                    // the products so far must be in O: the last are those of the other half, of this tile or of the one before
+                    ok = patience.wait(&pv_done[i][h ^ 1], (h == 1 ? s_uses : s_uses + 1) & 1);
+                    if (!ok) break;
+                    tmem_fence_after_sync();
 #pragma unroll 1
                     for (int b = 0; b < D / 16; ++b) {
                       uint32_t o[16];
@@ -1165,42 +1146,46 @@ __global__ void __launch_bounds__(PromptCfg<D, Bits>::kThreads, 1)
                   if (x > 0) {  // the chunk before, whose weights wait in P: at most 2^-15 of these, so that rounding them again is nothing
                     uint32_t p[16];
                     tmem_wait_st();
-                    tmem_ld16(p, s_col);
+                    tmem_ld16(p, h_col);
 #pragma unroll
                     for (int k = 0; k < 16; ++k) {
                       const float2 v = unpack2<T>(p[k]);
                       p[k] = Half16<T>::pack(v.x * f, v.y * f);
                     }
-                    tmem_st16(s_col, p);
+                    tmem_st16(h_col, p);
                   }
                   m = top;
                 }
+                const float off = m == -CUDART_INF_F ? 0.f : fmaf(-m, a.scale2, kPromptBias<T>);
+                const float2 scale = make_float2(a.scale2, a.scale2), offs = make_float2(off, off);
                 float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
                 uint32_t p[16];
 #pragma unroll
                 for (int k = 0; k < 16; ++k) {
-                  const float2 v = make_float2(ex2(__uint_as_float(s[2 * k])), ex2(__uint_as_float(s[2 * k + 1])));
+                  float2 v = fma2(make_float2(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1])), scale, offs);
+                  v.x = ex2(v.x);
+                  v.y = ex2(v.y);
                   // the sum keeps the unrounded probabilities; the values' weights are rounded to 16 bits once
                   sums[k & 1] = add2(sums[k & 1], v);
                   p[k] = Half16<T>::pack(v.x, v.y);
                 }
-                tmem_st16(s_col + x / 2, p);
+                tmem_st16(h_col + x / 2, p);
                 sums[0] = add2(sums[0], sums[1]);
                 sum = sums[0].x + sums[0].y;
                 if (find || !__any_sync(0xffffffffu, q_row >= 0 && (!(sum <= 32768.f) || m == -CUDART_INF_F))) break;
                 find = true;
               }
+              if (!ok) break;
               l += sum;
             }
+            if (!ok) break;
             tmem_wait_st();
             tmem_fence_before_sync();
             __syncwarp();
-            if (lane == 0) {
-              if (h == 1) mbar_arrive(&kv_empty[ks]);
-              mbar_arrive(&p_full[i][h]);
-            }
+            if (lane == 0) mbar_arrive(&p_full[i][h]);
           }
           if (!ok) break;
+          ++s_uses;
           started = true;
         } else {
           ok = patience.wait(&s_full[i], s_uses & 1);
@@ -1300,7 +1285,7 @@ __global__ void __launch_bounds__(PromptCfg<D, Bits>::kThreads, 1)
       }
       tmem_fence_after_sync();
       const float inv = l == 0.f ? 0.f : 1.f / l;
-      const float m2 = Bits == 4 || m == -CUDART_INF_F ? m - kPromptBias<T> : fmaf(m, a.scale2, -kPromptBias<T>);
+      const float m2 = m == -CUDART_INF_F ? m : fmaf(m, a.scale2, -kPromptBias<T>);
       const bool there = q_row >= 0;
       float* part = ws.part + static_cast<int64_t>(part_at) * (D + 2) * kPairRows + i * kTile + r;
       float* state = prefix && there ? rows.state + (static_cast<int64_t>(q_row) * a.q_heads + q_head) * (D + 4) : nullptr;
