@@ -94,8 +94,8 @@ struct PromptCfg {
   static constexpr int kOutRow = Bits == 4 ? 64 : 128;
   static constexpr uint32_t kOutBytes = 8 * 32 * kOutRow;
   // 4-bit pool: what is on its way to each of the converter warps (Convert4::Raw)
-  static constexpr int kConverters = 6, kRaw = D == 64 ? 2 : 4;
-  static constexpr uint32_t kRawBytes = Bits == 4 ? kConverters * kRaw * (32 * 16 + 16 * 4) : 0;
+  static constexpr int kConverters = 6, kRaw = 2;
+  static constexpr uint32_t kRawBytes = Bits == 4 ? kConverters * kRaw * (D / 64) * (32 * 16 + 16 * 4) : 0;
   static constexpr size_t kSmem =
       1024 + 2 * static_cast<size_t>(kQBytes) + kStages * static_cast<size_t>(kTileBytes) + kOutBytes + kRawBytes;
 };
@@ -510,7 +510,7 @@ __device__ __forceinline__ KeySpan unit_span(const Walk& w, bool prefix, int tq,
 // two 16-bit numbers each, the second one what rounding leaves of the first, which a
 // second pass of the product adds: a score is then right to 2^-16 of its terms, as
 // rounding keys once (2^-8) would show in every log-sum-exp.
-// A piece is 16 tokens' 64 dims of a group, two lanes a token.  Its codes and pairs are
+// A piece is 16 tokens, two lanes each.  Its codes and pairs are
 // copied to shared memory (kRaw pieces ahead) and from there converted into the stage,
 // laid out as TMA would have written it (128-byte swizzle).  Everything is in rolled
 // loops: beside the softmax's code it has to fit the instruction cache (unrolled, 8192
@@ -519,61 +519,74 @@ template <typename T, int D>
 struct Convert4 {
   static constexpr int DB = D / 64, kRaw = PromptCfg<D, 4>::kRaw;
   struct Raw {
-    uint4 codes[kRaw][32];
-    uint32_t pair[kRaw][16];
+    uint4 codes[kRaw][DB][32];
+    uint32_t pair[kRaw][DB][16];
   };
   Raw* raw;
 
   // the lane's token `key`, from the page that holds it; zeros if it is not to be read
-  __device__ __forceinline__ void ask(const PagedCache& c, int slot, int page, int layer, int kv, int head, int b, int key,
+  __device__ __forceinline__ void ask(const PagedCache& c, int slot, int page, int layer, int kv, int head, int key,
                                       bool keep) const {
     const int lane = threadIdx.x & 31, in_page = key & (c.page_size - 1);
     keep = keep && c.is_page(page);
     const unsigned char* block = block4(c, keep ? page : 0, layer, kv, head);
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(&raw->codes[slot][lane])),
-                 "l"(block + in_page * (D / 2) + 32 * b + 16 * (lane & 1)), "r"(keep ? 16 : 0)
-                 : "memory");
-    if ((lane & 1) == 0)
-      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_addr(&raw->pair[slot][lane >> 1])),
-                   "l"(block + block4_codes(c) + (in_page * DB + b) * 4), "r"(keep ? 4 : 0)
+    const unsigned char* codes = block + in_page * (D / 2) + 16 * (lane & 1);
+    const unsigned char* pairs = block + block4_codes(c) + in_page * (4 * DB);
+#pragma unroll
+    for (int b = 0; b < DB; ++b) {
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(&raw->codes[slot][b][lane])),
+                   "l"(codes + 32 * b), "r"(keep ? 16 : 0)
                    : "memory");
+      if ((lane & 1) == 0)
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_addr(&raw->pair[slot][b][lane >> 1])),
+                     "l"(pairs + 4 * b), "r"(keep ? 4 : 0)
+                     : "memory");
+    }
   }
-  // `block`: 128-byte rows of the stage
-  __device__ __forceinline__ void values(int slot, int row, unsigned char* block) const {
+  // into row `row` of the stage's blocks of 128-byte rows
+  __device__ __forceinline__ void values(int slot, int row, unsigned char* stage) const {
     const int lane = threadIdx.x & 31;
-    const uint4 x = raw->codes[slot][lane];
-    const uint32_t w[4] = {x.x, x.y, x.z, x.w}, p = raw->pair[slot][lane >> 1];
-    const uint32_t step2 = __byte_perm(p, 0, 0x1010), low2 = __byte_perm(p, 0, 0x3232);
+#pragma unroll 1
+    for (int b = 0; b < DB; ++b) {
+      const uint4 x = raw->codes[slot][b][lane];
+      const uint32_t w[4] = {x.x, x.y, x.z, x.w}, p = raw->pair[slot][b][lane >> 1];
+      const uint32_t step2 = __byte_perm(p, 0, 0x1010), low2 = __byte_perm(p, 0, 0x3232);
+      unsigned char* to = stage + b * (kKeys * 128) + row * 128;
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      *reinterpret_cast<uint4*>(block + row * 128 + 16 * ((4 * (lane & 1) + k) ^ (row & 7))) =
-          make_uint4(value2<T>(codes2<T, 0>(w[k]), step2, low2), value2<T>(codes2<T, 1>(w[k]), step2, low2),
-                     value2<T>(codes2<T, 2>(w[k]), step2, low2), value2<T>(codes2<T, 3>(w[k]), step2, low2));
+      for (int k = 0; k < 4; ++k)
+        *reinterpret_cast<uint4*>(to + 16 * ((4 * (lane & 1) + k) ^ (row & 7))) =
+            make_uint4(value2<T>(codes2<T, 0>(w[k]), step2, low2), value2<T>(codes2<T, 1>(w[k]), step2, low2),
+                       value2<T>(codes2<T, 2>(w[k]), step2, low2), value2<T>(codes2<T, 3>(w[k]), step2, low2));
+    }
   }
-  // the rounded keys into `block`, the rest into the block `rest` bytes on
-  __device__ __forceinline__ void keys(int slot, int row, unsigned char* block, int rest) const {
+  // the rounded keys, and DB blocks on what that leaves
+  __device__ __forceinline__ void keys(int slot, int row, unsigned char* stage) const {
     const int lane = threadIdx.x & 31;
-    const uint4 x = raw->codes[slot][lane];
-    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-    const float2 so = step_off(unpack2<T>(raw->pair[slot][lane >> 1]));
-    const float2 step = make_float2(so.x, so.x), off = make_float2(so.y, so.y);
+#pragma unroll 1
+    for (int b = 0; b < DB; ++b) {
+      const uint4 x = raw->codes[slot][b][lane];
+      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+      const float2 so = step_off(unpack2<T>(raw->pair[slot][b][lane >> 1]));
+      const float2 step = make_float2(so.x, so.x), off = make_float2(so.y, so.y);
+      unsigned char* to = stage + b * (kHalf * 128) + row * 128;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      uint32_t hi[4], lo[4];
+      for (int k = 0; k < 4; ++k) {
+        uint32_t hi[4], lo[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        // 16 + code in f32, as in codes2
-        const uint32_t a = i == 0 ? w[k] << 19 : i == 1 ? w[k] << 15 : i == 2 ? w[k] << 11 : w[k] << 7;
-        const uint32_t b = i == 0 ? w[k] << 3 : w[k] >> (4 * i - 3);
-        const float2 v = fma2(make_float2(__uint_as_float((a & 0x00780000u) | 0x41800000u),
-                                          __uint_as_float((b & 0x00780000u) | 0x41800000u)), step, off);
-        hi[i] = Half16<T>::pack(v.x, v.y);
-        const float2 h = unpack2<T>(hi[i]), r = add2(v, make_float2(-h.x, -h.y));
-        lo[i] = Half16<T>::pack(r.x, r.y);
+        for (int i = 0; i < 4; ++i) {
+          // 16 + code in f32, as in codes2
+          const uint32_t c0 = i == 0 ? w[k] << 19 : i == 1 ? w[k] << 15 : i == 2 ? w[k] << 11 : w[k] << 7;
+          const uint32_t c1 = i == 0 ? w[k] << 3 : w[k] >> (4 * i - 3);
+          const float2 v = fma2(make_float2(__uint_as_float((c0 & 0x00780000u) | 0x41800000u),
+                                            __uint_as_float((c1 & 0x00780000u) | 0x41800000u)), step, off);
+          hi[i] = Half16<T>::pack(v.x, v.y);
+          const float2 r = fma2(unpack2<T>(hi[i]), make_float2(-1.f, -1.f), v);
+          lo[i] = Half16<T>::pack(r.x, r.y);
+        }
+        const int at = 16 * ((4 * (lane & 1) + k) ^ (row & 7));
+        *reinterpret_cast<uint4*>(to + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<uint4*>(to + DB * kHalf * 128 + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
       }
-      unsigned char* to = block + row * 128 + 16 * ((4 * (lane & 1) + k) ^ (row & 7));
-      *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-      *reinterpret_cast<uint4*>(to + rest) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     }
   }
 };
@@ -656,7 +669,7 @@ __global__ void __launch_bounds__(PromptCfg<D, Bits>::kThreads, 1)
     const int me = warp < 11 ? warp - 9 : warp - 10;
     const X x{reinterpret_cast<typename X::Raw*>(out_smem + C::kOutBytes) + me};
     static_assert(Bits == 16 || C::kConverters * sizeof(typename X::Raw) == C::kRawBytes);
-    constexpr int kHalfPieces = kHalf / 16 * DB, kTilePieces = 4 * kHalfPieces;  // keys' halves, then values
+    constexpr int kHalfPieces = kHalf / 16, kTilePieces = 4 * kHalfPieces;  // keys' halves, then values
     constexpr int kAhead = C::kConverters * C::kRaw;
     static_assert(kAhead <= kTilePieces);
     int it = 0;
@@ -674,13 +687,13 @@ __global__ void __launch_bounds__(PromptCfg<D, Bits>::kThreads, 1)
       };
       // piece n of a tile into a slot of the raw ring
       auto ask = [&](int slot, int t, int n, int page) {
-        const int kv = n >= 2 * kHalfPieces ? 1 : 0, sub = n - 2 * kHalfPieces * kv, rows = sub / DB;
+        const int kv = n >= 2 * kHalfPieces ? 1 : 0, rows = n - 2 * kHalfPieces * kv;
         const int j = kKeys * span.tile(t) + 16 * rows + (lane >> 1);
         page = __shfl_sync(0xffffffffu, page, rows);
         if (t < w.t1) {
           bool keep = j < g.len;
           if (kv == 1) keep = j <= p1 && (a.window == 0 || j > p0 - a.window || j < a.sinks) && (mask == nullptr || mask[j]);
-          x.ask(c, slot, page, a.layer, kv, w.head, sub % DB, j, keep);
+          x.ask(c, slot, page, a.layer, kv, w.head, j, keep);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
       };
@@ -701,13 +714,11 @@ __global__ void __launch_bounds__(PromptCfg<D, Bits>::kThreads, 1)
           for (; n < end; n += C::kConverters) {
             asm volatile("cp.async.wait_group %0;" ::"n"(C::kRaw - 1) : "memory");
             __syncwarp();
-            if (e < 2) {
-              const int sub = n - kHalfPieces * e;
-              x.keys(slot, 16 * (sub / DB) + (lane >> 1), stage + sub % DB * (kHalf * 128), DB * kHalf * 128);
-            } else {
-              const int sub = n - 2 * kHalfPieces;
-              x.values(slot, 16 * (sub / DB) + (lane >> 1), stage + sub % DB * (kKeys * 128));
-            }
+            const int row = 16 * (n - kHalfPieces * e) + (lane >> 1);
+            if (e < 2)
+              x.keys(slot, row, stage);
+            else
+              x.values(slot, row, stage);
             __syncwarp();
             const int then = n + kAhead;
             ask(slot, then < kTilePieces ? t : t + 1, then & (kTilePieces - 1), then < kTilePieces ? page : next_page);
