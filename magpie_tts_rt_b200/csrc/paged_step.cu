@@ -46,8 +46,12 @@ namespace {
 constexpr int kStepWarps = 4;
 constexpr int kStepThreads = 32 * kStepWarps;
 
+// Forms of the kernels: 16 for a pool in 16 bits; for one in 4 bits how many query
+// heads a key head has at most: 1, 4 or more (8).
+constexpr int step_form(int bits, int group) { return bits == 16 ? 16 : group == 1 ? 1 : group <= 4 ? 4 : 8; }
+
 // 16-key tiles per warp and step
-constexpr int step_tiles(int head_dim, int bits) { return (head_dim == 64 ? 2 : 1) * (bits == 4 ? 2 : 1); }
+constexpr int step_tiles(int head_dim, int form) { return (head_dim == 64 ? 2 : 1) * (form == 16 ? 1 : 2); }
 constexpr int step_ctas(int head_dim, int nb) { return (head_dim == 64 ? 4 : 3) - (nb == 2 ? 1 : 0); }  // per SM (registers)
 
 // A unit's place on the line: its tiles, and before them what entering and
@@ -298,29 +302,43 @@ __device__ __forceinline__ uint2 load8(const unsigned char* p, bool on) {
 }
 
 // The first of the 8 dims that piece k of a thread's queries holds, as its keys do.
-template <int Bits>
+template <int Form>
 __device__ __forceinline__ int step_dims(int t, int k) {
-  return Bits == 16 ? 32 * k + 8 * t : 64 * (k >> 1) + 16 * t + 8 * (k & 1);
+  return Form == 16 ? 32 * k + 8 * t : 64 * (k >> 1) + 16 * t + 8 * (k & 1);
+}
+// The query of a product's column.
+template <int Form>
+__device__ __forceinline__ int step_column(int g) {
+  return Form == 16 || Form == 8 ? g : g & 3;
 }
 
-// attend_tiles for a cache in 4 bits.  Nothing is rounded on the way into the
+// attend_tiles for a pool in 4 bits.  Nothing is rounded on the way into the
 // products: a code is a small whole number, exact in either 16-bit type, and the
 // pairs come in afterwards, in f32,
 //   q.k = sum over groups: step (q.(16 + c)) + off sum q,   off = low - 16 step;
 // the values' weights are p step, in two bf16 numbers each (their range is not
-// f16's), and p off is summed by itself.
-template <typename T, int D, int NB>
+// f16's), and p off is summed by itself.  Up to four queries take the product's
+// columns twice, the weights' first numbers in columns 0 to 3 and what their
+// rounding leaves in 4 to 7: one product for both, the halves added at the end.
+//
+// What bounds it is instructions, a third of them the codes' way into 16 bits, so
+// the rest is kept few: addresses are one sum a tile, all 16 keys of a tile are
+// loaded (a masked key's pair is taken as zero), and the maximum is looked after
+// only when a key passes it.
+template <typename T, int D, int NB, int Form>
 __device__ __forceinline__ void attend_tiles4(const PagedCache& c, const Attend& a, const SeenTiles& seen,
                                               const int32_t* row, const bool* mask, int head, int t0, int t1,
-                                              const uint4 (&q)[NB][D / 32], int (&page)[step_tiles(D, 4)],
+                                              const uint4 (&q)[NB][D / 32], int (&page)[step_tiles(D, Form)],
                                               StepSums<D, NB>& sums) {
   using B = __nv_bfloat16;
-  constexpr int NT = step_tiles(D, 4);
+  constexpr int NT = step_tiles(D, Form);
   constexpr int G = D / kGroup4;
+  constexpr int QC = Form == 1 ? 1 : 2;  // columns that a thread looks after
+  constexpr bool kTwice = Form <= 4;
   const int lane = threadIdx.x & 31, t = lane & 3, g = lane >> 2;
   auto& [m, l, acc] = sums;
-  // the queries' sums over each group
-  float qs[NB][G][2], rest[NB][G][2];
+  // the queries' sums over each group, times the scale
+  float qs[NB][G][QC], rest[NB][G][QC];
 #pragma unroll
   for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -339,11 +357,16 @@ __device__ __forceinline__ void attend_tiles4(const PagedCache& c, const Attend&
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        qs[b][v][i] = __shfl_sync(0xffffffffu, sum, 4 * (2 * t + i));
+      for (int i = 0; i < QC; ++i) {
+        qs[b][v][i] = __shfl_sync(0xffffffffu, sum, 4 * (2 * t + i)) * a.scale2;
         rest[b][v][i] = 0.f;
       }
     }
+  // where the thread's bytes are in a block: codes of keys g (and g + 8), of values 2t (2t + 1, 2t + 8, 2t + 9), pairs
+  const int64_t page_bytes = static_cast<int64_t>(c.layers) * 4 * c.kv_elems;
+  const unsigned char* blocks = block4(c, 0, a.layer, 0, head);
+  const int k_at = g * (D / 2) + 8 * t, v_at = 2 * static_cast<int>(c.kv_elems) + 2 * t * (D / 2) + 4 * g;
+  const int p_at = block4_codes(c) + g * (4 * G), pv_at = 2 * static_cast<int>(c.kv_elems);
   for (int base = t0; base < t1; base += NT) {
     // keys in reach: one per lane and pair of tiles
     uint32_t bits[NT / 2];
@@ -355,25 +378,26 @@ __device__ __forceinline__ void attend_tiles4(const PagedCache& c, const Attend&
       bits[u] = __ballot_sync(0xffffffffu, in);
     }
     uint2 kr[NT][2][G];
-    uint32_t vr[NT][4][G], kp[NT][2][G], vp[NT][2][G], on[NT];
+    uint32_t vr[NT][4][G], kp[NT][2][G], vp[NT][2][G];
+    bool on[NT][2];  // the thread's keys g, g + 8
 #pragma unroll
     for (int u = 0; u < NT; ++u) {
-      on[u] = c.is_page(page[u]) ? (bits[u >> 1] >> (16 * (u & 1))) & 0xffffu : 0u;
+      const bool there = c.is_page(page[u]);
+      const uint32_t mine = (there ? bits[u >> 1] : 0u) >> (16 * (u & 1) + g);
+      on[u][0] = (mine & 1u) != 0;
+      on[u][1] = (mine & 256u) != 0;
       const int in_page = (16 * seen.tile(base + u)) & (c.page_size - 1);
-      const unsigned char* kb = block4(c, page[u], a.layer, 0, head);
-      const unsigned char* vb = kb + 2 * c.kv_elems;
-      const int pairs = block4_codes(c);
+      const unsigned char* at = blocks + page[u] * page_bytes + in_page * (D / 2);
+      const unsigned char* pairs = blocks + page[u] * page_bytes + (p_at + in_page * (4 * G));
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int key = in_page + g + 8 * h;
-        const bool there = (on[u] >> (g + 8 * h)) & 1u;
 #pragma unroll
-        for (int v = 0; v < G; ++v) kr[u][h][v] = load8(kb + key * (D / 2) + 32 * v + 8 * t, there);
+        for (int v = 0; v < G; ++v) kr[u][h][v] = load8(at + k_at + 8 * h * (D / 2) + 32 * v, there);
         if constexpr (G == 1) {
-          kp[u][h][0] = load4(kb + pairs + 4 * key, there);
-          vp[u][h][0] = load4(vb + pairs + 4 * key, there);
+          kp[u][h][0] = load4(pairs + 8 * h * 4, there);
+          vp[u][h][0] = load4(pairs + pv_at + 8 * h * 4, there);
         } else {
-          const uint2 x = load8(kb + pairs + 8 * key, there), y = load8(vb + pairs + 8 * key, there);
+          const uint2 x = load8(pairs + 8 * h * 8, there), y = load8(pairs + pv_at + 8 * h * 8, there);
           kp[u][h][0] = x.x;
           kp[u][h][1] = x.y;
           vp[u][h][0] = y.x;
@@ -381,11 +405,9 @@ __device__ __forceinline__ void attend_tiles4(const PagedCache& c, const Attend&
         }
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int key = 2 * t + (i & 1) + 8 * (i >> 1);
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int v = 0; v < G; ++v) vr[u][i][v] = load4(vb + (in_page + key) * (D / 2) + 32 * v + 4 * g, (on[u] >> key) & 1u);
-      }
+        for (int v = 0; v < G; ++v) vr[u][i][v] = load4(at + v_at + ((i & 1) + 8 * (i >> 1)) * (D / 2) + 32 * v, there);
     }
     // the next step's pages, while this step's keys arrive
 #pragma unroll
@@ -395,11 +417,11 @@ __device__ __forceinline__ void attend_tiles4(const PagedCache& c, const Attend&
     }
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      float s[NT][4];
-      float top0 = m[b][0], top1 = m[b][1];
+      float s[NT][2][QC], top[QC];
+#pragma unroll
+      for (int i = 0; i < QC; ++i) top[i] = -CUDART_INF_F;
 #pragma unroll
       for (int u = 0; u < NT; ++u) {
-        s[u][0] = s[u][1] = s[u][2] = s[u][3] = 0.f;
 #pragma unroll
         for (int v = 0; v < G; ++v) {
           float x[4] = {0.f, 0.f, 0.f, 0.f};
@@ -410,64 +432,83 @@ __device__ __forceinline__ void attend_tiles4(const PagedCache& c, const Attend&
             Half16<T>::mma(x, codes2<T, 0>(w0), codes2<T, 0>(w1), codes2<T, 1>(w0), codes2<T, 1>(w1), y.x, y.y);
             Half16<T>::mma(x, codes2<T, 2>(w0), codes2<T, 2>(w1), codes2<T, 3>(w0), codes2<T, 3>(w1), y.z, y.w);
           }
-          const float2 lo = step_off(unpack2<T>(kp[u][0][v])), hi = step_off(unpack2<T>(kp[u][1][v]));
-          s[u][0] = fmaf(lo.x, x[0], fmaf(lo.y, qs[b][v][0], s[u][0]));
-          s[u][1] = fmaf(lo.x, x[1], fmaf(lo.y, qs[b][v][1], s[u][1]));
-          s[u][2] = fmaf(hi.x, x[2], fmaf(hi.y, qs[b][v][0], s[u][2]));
-          s[u][3] = fmaf(hi.x, x[3], fmaf(hi.y, qs[b][v][1], s[u][3]));
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float2 so = step_off(unpack2<T>(kp[u][h][v]));
+            const float step = so.x * a.scale2;
+#pragma unroll
+            for (int i = 0; i < QC; ++i)
+              s[u][h][i] = fmaf(step, x[2 * h + i], v == 0 ? so.y * qs[b][0][i] : fmaf(so.y, qs[b][v][i], s[u][h][i]));
+          }
         }
-        const bool lo = (on[u] >> g) & 1u, hi = (on[u] >> (g + 8)) & 1u;
-        s[u][0] = lo ? s[u][0] * a.scale2 : -CUDART_INF_F;
-        s[u][1] = lo ? s[u][1] * a.scale2 : -CUDART_INF_F;
-        s[u][2] = hi ? s[u][2] * a.scale2 : -CUDART_INF_F;
-        s[u][3] = hi ? s[u][3] * a.scale2 : -CUDART_INF_F;
-        top0 = fmaxf(top0, fmaxf(s[u][0], s[u][2]));
-        top1 = fmaxf(top1, fmaxf(s[u][1], s[u][3]));
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < QC; ++i) {
+            s[u][h][i] = on[u][h] ? s[u][h][i] : -CUDART_INF_F;
+            top[i] = fmaxf(top[i], s[u][h][i]);
+          }
       }
+      bool more = false;
 #pragma unroll
-      for (int o = 4; o < 32; o <<= 1) {
-        top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, o));
-        top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, o));
-      }
-      const float z0 = top0 == -CUDART_INF_F ? 0.f : top0, z1 = top1 == -CUDART_INF_F ? 0.f : top1;
-      const float keep0 = ex2(m[b][0] - z0), keep1 = ex2(m[b][1] - z1);
-      m[b][0] = top0;
-      m[b][1] = top1;
-      l[b][0] *= keep0;
-      l[b][1] *= keep1;
+      for (int i = 0; i < QC; ++i) more = more || top[i] > m[b][i];
+      if (__any_sync(0xffffffffu, more)) {
 #pragma unroll
-      for (int v = 0; v < G; ++v) {
-        rest[b][v][0] *= keep0;
-        rest[b][v][1] *= keep1;
+        for (int i = 0; i < QC; ++i) {
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          acc[b][v][w][0] *= keep0;
-          acc[b][v][w][1] *= keep1;
-          acc[b][v][w][2] *= keep0;
-          acc[b][v][w][3] *= keep1;
+          for (int o = 4; o < 32; o <<= 1) top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
+          top[i] = fmaxf(top[i], m[b][i]);
+          const float keep = top[i] == -CUDART_INF_F ? 1.f : ex2(m[b][i] - top[i]);
+          m[b][i] = top[i];
+          l[b][i] *= keep;
+#pragma unroll
+          for (int v = 0; v < G; ++v) {
+            rest[b][v][i] *= keep;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              acc[b][v][w][i] *= keep;
+              acc[b][v][w][2 + i] *= keep;
+            }
+          }
         }
       }
+      float z[QC];
+#pragma unroll
+      for (int i = 0; i < QC; ++i) z[i] = m[b][i] == -CUDART_INF_F ? 0.f : m[b][i];
 #pragma unroll
       for (int u = 0; u < NT; ++u) {
-        const float p0 = ex2(s[u][0] - z0), p1 = ex2(s[u][1] - z1), p2 = ex2(s[u][2] - z0), p3 = ex2(s[u][3] - z1);
-        l[b][0] += p0 + p2;
-        l[b][1] += p1 + p3;
+        float w[2][2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < QC; ++i) {
+            w[h][i] = ex2(s[u][h][i] - z[i]);
+            l[b][i] += w[h][i];
+          }
 #pragma unroll
         for (int v = 0; v < G; ++v) {
-          const float2 lo = step_off(unpack2<T>(vp[u][0][v])), hi = step_off(unpack2<T>(vp[u][1][v]));
-          rest[b][v][0] = fmaf(p0, lo.y, fmaf(p2, hi.y, rest[b][v][0]));
-          rest[b][v][1] = fmaf(p1, lo.y, fmaf(p3, hi.y, rest[b][v][1]));
-          const uint2 w0 = Half16<B>::split(p0 * lo.x, p1 * lo.x), w1 = Half16<B>::split(p2 * hi.x, p3 * hi.x);
-          const uint32_t b0 = transpose8x8(w0.x), b1 = transpose8x8(w1.x);
-          const uint32_t rest0 = transpose8x8(w0.y), rest1 = transpose8x8(w1.y);
+          uint2 parts[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float2 so = step_off(unpack2<T>(on[u][h] ? vp[u][h][v] : 0u));
+#pragma unroll
+            for (int i = 0; i < QC; ++i) rest[b][v][i] = fmaf(w[h][i], so.y, rest[b][v][i]);
+            parts[h] = Half16<B>::split(w[h][0] * so.x, QC == 2 ? w[h][1] * so.x : 0.f);
+          }
           const uint32_t near[2] = {__byte_perm(vr[u][0][v], vr[u][1][v], 0x5410), __byte_perm(vr[u][0][v], vr[u][1][v], 0x7632)};
           const uint32_t far[2] = {__byte_perm(vr[u][2][v], vr[u][3][v], 0x5410), __byte_perm(vr[u][2][v], vr[u][3][v], 0x7632)};
-          auto dims = [&](auto w) {  // 8g + 2w (row g of the product) and 8g + 2w + 1 (row g + 8)
-            constexpr int W = decltype(w)::value;
+          uint32_t first[2], second[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            first[h] = transpose8x8(kTwice && t >= 2 ? parts[h].y : parts[h].x);
+            if constexpr (!kTwice) second[h] = transpose8x8(parts[h].y);
+          }
+          auto dims = [&](auto which) {  // 8g + 2w (row g of the product) and 8g + 2w + 1 (row g + 8)
+            constexpr int W = decltype(which)::value;
             const uint32_t v0 = codes2<B, W>(near[0]), v1 = codes2<B, W>(near[1]);
             const uint32_t v2 = codes2<B, W>(far[0]), v3 = codes2<B, W>(far[1]);
-            Half16<B>::mma(acc[b][v][W], v0, v1, v2, v3, b0, b1);
-            Half16<B>::mma(acc[b][v][W], v0, v1, v2, v3, rest0, rest1);
+            Half16<B>::mma(acc[b][v][W], v0, v1, v2, v3, first[0], first[1]);
+            if constexpr (!kTwice) Half16<B>::mma(acc[b][v][W], v0, v1, v2, v3, second[0], second[1]);
           };
           dims(std::integral_constant<int, 0>{});
           dims(std::integral_constant<int, 1>{});
@@ -483,33 +524,36 @@ __device__ __forceinline__ void attend_tiles4(const PagedCache& c, const Attend&
 #pragma unroll
     for (int v = 0; v < G; ++v)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < QC; ++i) {
         float x = rest[b][v][i];
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          acc[b][v][w][i] += x;
-          acc[b][v][w][2 + i] += x;
-        }
+        for (int w = 0; w < 4; ++w)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            float& o = acc[b][v][w][2 * k + i];
+            if constexpr (kTwice) o += __shfl_xor_sync(0xffffffffu, o, 2);
+            o += x;
+          }
       }
 }
 
-template <typename T, int D, int NB, int Bits>
+template <typename T, int D, int NB, int Form>
 __device__ __forceinline__ void attend_tiles_of(const PagedCache& c, const Attend& a, const SeenTiles& seen,
                                                 const int32_t* row, const bool* mask, int head, int t0, int t1,
-                                                const uint4 (&q)[NB][D / 32], int (&page)[step_tiles(D, Bits)],
+                                                const uint4 (&q)[NB][D / 32], int (&page)[step_tiles(D, Form)],
                                                 StepSums<D, NB>& sums) {
-  if constexpr (Bits == 4)
-    attend_tiles4<T, D, NB>(c, a, seen, row, mask, head, t0, t1, q, page, sums);
+  if constexpr (Form != 16)
+    attend_tiles4<T, D, NB, Form>(c, a, seen, row, mask, head, t0, t1, q, page, sums);
   else
     attend_tiles<T, D, NB>(c, a, seen, row, mask, static_cast<int64_t>(head) * c.page_size * D, t0, t1, q, page, sums);
 }
 
-template <typename T, int D, int NB, int Bits>
+template <typename T, int D, int NB, int Form>
 __global__ void __launch_bounds__(kStepThreads, step_ctas(D, NB))
     step_kernel(PagedCache c, Attend a, SharedPrefix shared, StepSpace ws, int blocks, int min_tiles) {
-  constexpr int NT = step_tiles(D, Bits);
+  constexpr int NT = step_tiles(D, Form);
   constexpr int NQ = 8 * NB;   // query rows of a unit
   constexpr int KC = D / 32, VC = D / 64;
   extern __shared__ int tiles_before[];  // [rows + 1]: tiles of a key head of the slots before
@@ -601,11 +645,12 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(D, NB))
     t0 = static_cast<int>(max(x - unit_x - kUnitCost, static_cast<int64_t>(0)));
     t1 = static_cast<int>(max(min(static_cast<int64_t>(seen.n), x_end - unit_x - kUnitCost), static_cast<int64_t>(0)));
     const int queries = min(NQ, a.group - block * NQ);
-    const int64_t q_at = slot * a.q_row + static_cast<int64_t>(head * a.group + block * NQ + g) * D;
+    const int col = step_column<Form>(g);
+    const int64_t q_at = slot * a.q_row + static_cast<int64_t>(head * a.group + block * NQ + col) * D;
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
-      for (int k = 0; k < KC; ++k) q[b][k] = load16(a.q + q_at + 8 * b * D + step_dims<Bits>(t, k), 8 * b + g < queries);
+      for (int k = 0; k < KC; ++k) q[b][k] = load16(a.q + q_at + 8 * b * D + step_dims<Form>(t, k), 8 * b + col < queries);
     const int32_t* row = c.table + static_cast<int64_t>(slot) * c.table_pages;
 #pragma unroll
     for (int u = 0; u < NT; ++u) page[u] = t0 + u < t1 ? row[(16 * seen.tile(t0 + u)) >> c.page_shift] : -1;
@@ -618,7 +663,7 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(D, NB))
     const bool* mask = a.key_mask != nullptr ? a.key_mask + slot * a.mask_stride : nullptr;
     StepSums<D, NB> sums;
     sums.clear();
-    attend_tiles_of<T, D, NB, Bits>(c, a, seen, row, mask, head, t0, t1, q, page, sums);
+    attend_tiles_of<T, D, NB, Form>(c, a, seen, row, mask, head, t0, t1, q, page, sums);
     auto& [m, l, acc] = sums;
 
     // a thread holds queries 2t, 2t + 1 and dims 8g .. 8g + 7 of each 64
@@ -774,9 +819,9 @@ constexpr int kMaxSpread = 8, kFewSteps = 4;
 
 // 4 CTAs of 4 warps an SM, as head_dim 64 has by itself: 132 registers instead of
 // 128 would let one cluster in four go.
-template <typename T, int D, int NB, int W, int Bits>
+template <typename T, int D, int NB, int W, int Form>
 __global__ void __launch_bounds__(32 * W, D == 128 && NB == 1 && W == 4 ? 4 : 0) step_few_kernel(PagedCache c, Attend a, int blocks, int spread) {
-  constexpr int NT = step_tiles(D, Bits);
+  constexpr int NT = step_tiles(D, Form);
   constexpr int NQ = 8 * NB, KC = D / 32, VC = D / 64;
   constexpr int kRow = D + 2;  // weighted values, maximum, sum
   extern __shared__ float few_smem[];
@@ -800,14 +845,15 @@ __global__ void __launch_bounds__(32 * W, D == 128 && NB == 1 && W == 4 ? 4 : 0)
   int page[NT];
 #pragma unroll
   for (int u = 0; u < NT; ++u) page[u] = t0 + u < t1 ? row[(16 * seen.tile(t0 + u)) >> c.page_shift] : -1;
-  const int64_t q_at = slot * a.q_row + static_cast<int64_t>(q_head + g) * D;
+  const int col = step_column<Form>(g);
+  const int64_t q_at = slot * a.q_row + static_cast<int64_t>(q_head + col) * D;
 #pragma unroll
   for (int b = 0; b < NB; ++b)
 #pragma unroll
-    for (int k = 0; k < KC; ++k) q[b][k] = load16(a.q + q_at + 8 * b * D + step_dims<Bits>(t, k), 8 * b + g < queries);
+    for (int k = 0; k < KC; ++k) q[b][k] = load16(a.q + q_at + 8 * b * D + step_dims<Form>(t, k), 8 * b + col < queries);
   StepSums<D, NB> sums;
   sums.clear();
-  attend_tiles_of<T, D, NB, Bits>(c, a, seen, row, a.key_mask != nullptr ? a.key_mask + slot * a.mask_stride : nullptr, head,
+  attend_tiles_of<T, D, NB, Form>(c, a, seen, row, a.key_mask != nullptr ? a.key_mask + slot * a.mask_stride : nullptr, head,
                                   t0, t1, q, page, sums);
   auto& [m, l, acc] = sums;
 #pragma unroll
@@ -892,13 +938,13 @@ struct FewLaunch {
 
 // Clusters of `Spread` CTAs of the kernel that the current device runs at once
 // (0: cannot be queried).  Nothing here allocates or throws.
-template <typename T, int D, int NB, int W, int Spread, int Bits>
+template <typename T, int D, int NB, int W, int Spread, int Form>
 int few_clusters() {
   static std::atomic<int> known[64];  // by device ordinal, plus 1; the opt-in below is per device
   int dev = -1, clusters = 0;
   if (cudaGetDevice(&dev) == cudaSuccess) {
     if (dev >= 0 && dev < 64 && (clusters = known[dev].load(std::memory_order_relaxed)) > 0) return clusters - 1;
-    const auto kernel = step_few_kernel<T, D, NB, W, Bits>;
+    const auto kernel = step_few_kernel<T, D, NB, W, Form>;
     FewLaunch launch(1, Spread, W, few_bytes(D, NB, W), nullptr);
     launch.cfg.numAttrs = 1;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -945,7 +991,8 @@ cudaError_t launch_step(const PagedCache& c, int dtype, const Attend& a, const S
   if (sms <= 0 || sms > kMaxSms) return cudaErrorInvalidValue;
   const size_t smem = 4 * (static_cast<size_t>(a.rows) + 1);
   const int grid = sms * step_ctas(c.head_dim, nb), shares = grid * kStepWarps;
-  const int min_tiles = kUnitCost + step_tiles(c.head_dim, c.bits);
+  const int form = step_form(c.bits, a.group);
+  const int min_tiles = kUnitCost + step_tiles(c.head_dim, form);
   const int pairs = std::min(8 * nb, a.group) * c.head_dim / 2;
   auto go = [&](auto kernel, auto join) {
     if (smem > 40 * 1024) {
@@ -968,25 +1015,30 @@ cudaError_t launch_step(const PagedCache& c, int dtype, const Attend& a, const S
     const FewLaunch launch(static_cast<int>(units), spread, warps, few_bytes(c.head_dim, nb, warps), stream);
     return cudaLaunchKernelEx(&launch.cfg, kernel, c, a, blocks, spread);
   };
-  auto with_bits = [&](auto type, auto dim, auto bs, auto bits) {
+  auto with_form = [&](auto type, auto dim, auto bs, auto f) {
     using T = decltype(type);
-    constexpr int D = decltype(dim)::value, NB = decltype(bs)::value, Bits = decltype(bits)::value;
+    constexpr int D = decltype(dim)::value, NB = decltype(bs)::value, Form = decltype(f)::value;
     auto fits = [&](int warps, int clusters) {
-      return units <= clusters && reach <= static_cast<int64_t>(kFewSteps) * warps * 16 * step_tiles(D, Bits);
+      return units <= clusters && reach <= static_cast<int64_t>(kFewSteps) * warps * 16 * step_tiles(D, Form);
     };
     if (shared.base == nullptr) {
-      if (reach > 32 * 16 * step_tiles(D, Bits) && fits(64, few_clusters<T, D, NB, 8, 8, Bits>()))
-        return few(step_few_kernel<T, D, NB, 8, Bits>, 8, 8);
-      if (fits(32, few_clusters<T, D, NB, 4, 8, Bits>())) return few(step_few_kernel<T, D, NB, 4, Bits>, 4, 8);
-      if (fits(16, few_clusters<T, D, NB, 4, 4, Bits>())) return few(step_few_kernel<T, D, NB, 4, Bits>, 4, 4);
-      if (fits(8, few_clusters<T, D, NB, 4, 2, Bits>())) return few(step_few_kernel<T, D, NB, 4, Bits>, 4, 2);
-      if (fits(4, few_clusters<T, D, NB, 4, 1, Bits>())) return few(step_few_kernel<T, D, NB, 4, Bits>, 4, 1);
+      if (reach > 32 * 16 * step_tiles(D, Form) && fits(64, few_clusters<T, D, NB, 8, 8, Form>()))
+        return few(step_few_kernel<T, D, NB, 8, Form>, 8, 8);
+      if (fits(32, few_clusters<T, D, NB, 4, 8, Form>())) return few(step_few_kernel<T, D, NB, 4, Form>, 4, 8);
+      if (fits(16, few_clusters<T, D, NB, 4, 4, Form>())) return few(step_few_kernel<T, D, NB, 4, Form>, 4, 4);
+      if (fits(8, few_clusters<T, D, NB, 4, 2, Form>())) return few(step_few_kernel<T, D, NB, 4, Form>, 4, 2);
+      if (fits(4, few_clusters<T, D, NB, 4, 1, Form>())) return few(step_few_kernel<T, D, NB, 4, Form>, 4, 1);
     }
-    return go(step_kernel<T, D, NB, Bits>, step_join_kernel<T, D>);
+    return go(step_kernel<T, D, NB, Form>, step_join_kernel<T, D>);
   };
   auto run = [&](auto type, auto dim, auto bs) {
-    return c.bits == 4 ? with_bits(type, dim, bs, std::integral_constant<int, 4>{})
-                       : with_bits(type, dim, bs, std::integral_constant<int, 16>{});
+    using std::integral_constant;
+    if (form == 16) return with_form(type, dim, bs, integral_constant<int, 16>{});
+    if constexpr (decltype(bs)::value == 1) {
+      if (form == 1) return with_form(type, dim, bs, integral_constant<int, 1>{});
+      if (form == 4) return with_form(type, dim, bs, integral_constant<int, 4>{});
+    }
+    return with_form(type, dim, bs, integral_constant<int, 8>{});
   };
   auto pick = [&](auto type) {
     using std::integral_constant;
