@@ -52,7 +52,9 @@ constexpr int step_form(int bits, int group) { return bits == 16 ? 16 : group ==
 
 // 16-key tiles per warp and step
 constexpr int step_tiles(int head_dim, int form) { return (head_dim == 64 ? 2 : 1) * (form == 16 ? 1 : 2); }
-constexpr int step_ctas(int head_dim, int nb) { return (head_dim == 64 ? 4 : 3) - (nb == 2 ? 1 : 0); }  // per SM (registers)
+constexpr int step_ctas(int head_dim, int nb, int form) {  // per SM (registers)
+  return (head_dim == 64 ? 4 : 3) - (nb == 2 ? 1 : 0);
+}
 
 // A unit's place on the line: its tiles, and before them what entering and
 // leaving it costs, in tiles.  (2052 slots with 1 to 249 keys each, prefix pass
@@ -328,15 +330,15 @@ __device__ __forceinline__ int step_column(int g) {
 template <typename T, int D, int NB, int Form>
 __device__ __forceinline__ void attend_tiles4(const PagedCache& c, const Attend& a, const SeenTiles& seen,
                                               const int32_t* row, const bool* mask, int head, int t0, int t1,
-                                              const uint4 (&q)[NB][D / 32], int (&page)[step_tiles(D, Form)],
-                                              StepSums<D, NB>& sums) {
+                                              const uint4 (&q)[NB][D / 32], StepSums<D, NB>& sums) {
   using B = __nv_bfloat16;
   constexpr int NT = step_tiles(D, Form);
   constexpr int G = D / kGroup4;
   constexpr int QC = Form == 1 ? 1 : 2;  // columns that a thread looks after
   constexpr bool kTwice = Form <= 4;
   const int lane = threadIdx.x & 31, t = lane & 3, g = lane >> 2;
-  auto& [m, l, acc] = sums;
+  auto &m = sums.m, &l = sums.l;
+  auto& acc = sums.acc;
   // the queries' sums over each group, times the scale
   float qs[NB][G][QC], rest[NB][G][QC];
 #pragma unroll
@@ -367,13 +369,21 @@ __device__ __forceinline__ void attend_tiles4(const PagedCache& c, const Attend&
   const unsigned char* blocks = block4(c, 0, a.layer, 0, head);
   const int k_at = g * (D / 2) + 8 * t, v_at = 2 * static_cast<int>(c.kv_elems) + 2 * t * (D / 2) + 4 * g;
   const int p_at = block4_codes(c) + g * (4 * G), pv_at = 2 * static_cast<int>(c.kv_elems);
+  // Lane u (of each NT) looks up tile u of the step and tells the others.
+  const int mine = lane & (NT - 1);
+  const float lower = t >= 2 ? -1.f : 0.f;
+  auto lookup = [&](int tile) { return tile < t1 ? row[(16 * seen.tile(tile)) >> c.page_shift] : -1; };
+  int my_page = lookup(t0 + mine);
   for (int base = t0; base < t1; base += NT) {
+    const int my_key = 16 * seen.tile(base + mine), my_in = c.is_page(my_page) ? my_key & (c.page_size - 1) : -1;
+    const int64_t my_at = reinterpret_cast<int64_t>(blocks) + my_page * page_bytes + my_in * (D / 2);
+    const int next_page = lookup(base + NT + mine);  // on its way while this step's keys arrive
     // keys in reach: one per lane and pair of tiles
     uint32_t bits[NT / 2];
 #pragma unroll
     for (int u = 0; u < NT / 2; ++u) {
-      const int my_tile = base + 2 * u + (lane >> 4), j = 16 * seen.tile(my_tile) + (lane & 15);
-      bool in = my_tile < t1 && j < seen.len && (j >= seen.low || j < a.sinks);
+      const int j = __shfl_sync(0xffffffffu, my_key, 2 * u + (lane >> 4)) + (lane & 15);
+      bool in = base + 2 * u + (lane >> 4) < t1 && j < seen.len && (j >= seen.low || j < a.sinks);
       if (in && mask != nullptr) in = mask[j];
       bits[u] = __ballot_sync(0xffffffffu, in);
     }
@@ -382,13 +392,13 @@ __device__ __forceinline__ void attend_tiles4(const PagedCache& c, const Attend&
     bool on[NT][2];  // the thread's keys g, g + 8
 #pragma unroll
     for (int u = 0; u < NT; ++u) {
-      const bool there = c.is_page(page[u]);
-      const uint32_t mine = (there ? bits[u >> 1] : 0u) >> (16 * (u & 1) + g);
-      on[u][0] = (mine & 1u) != 0;
-      on[u][1] = (mine & 256u) != 0;
-      const int in_page = (16 * seen.tile(base + u)) & (c.page_size - 1);
-      const unsigned char* at = blocks + page[u] * page_bytes + in_page * (D / 2);
-      const unsigned char* pairs = blocks + page[u] * page_bytes + (p_at + in_page * (4 * G));
+      const int in_page = __shfl_sync(0xffffffffu, my_in, u);
+      const bool there = in_page >= 0;
+      const uint32_t my_bits = (there ? bits[u >> 1] : 0u) >> (16 * (u & 1) + g);
+      on[u][0] = (my_bits & 1u) != 0;
+      on[u][1] = (my_bits & 256u) != 0;
+      const unsigned char* at = reinterpret_cast<const unsigned char*>(__shfl_sync(0xffffffffu, my_at, u));
+      const unsigned char* pairs = at + (p_at - in_page * (D / 2 - 4 * G));
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
 #pragma unroll
@@ -409,12 +419,7 @@ __device__ __forceinline__ void attend_tiles4(const PagedCache& c, const Attend&
 #pragma unroll
         for (int v = 0; v < G; ++v) vr[u][i][v] = load4(at + v_at + ((i & 1) + 8 * (i >> 1)) * (D / 2) + 32 * v, there);
     }
-    // the next step's pages, while this step's keys arrive
-#pragma unroll
-    for (int u = 0; u < NT; ++u) {
-      const int tt = base + NT + u;
-      page[u] = tt < t1 ? row[(16 * seen.tile(tt)) >> c.page_shift] : -1;
-    }
+    my_page = next_page;
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       float s[NT][2][QC], top[QC];
@@ -487,22 +492,24 @@ __device__ __forceinline__ void attend_tiles4(const PagedCache& c, const Attend&
           }
 #pragma unroll
         for (int v = 0; v < G; ++v) {
-          uint2 parts[2];
+          uint32_t first[2], second[2];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const float2 so = step_off(unpack2<T>(on[u][h] ? vp[u][h][v] : 0u));
 #pragma unroll
             for (int i = 0; i < QC; ++i) rest[b][v][i] = fmaf(w[h][i], so.y, rest[b][v][i]);
-            parts[h] = Half16<B>::split(w[h][0] * so.x, QC == 2 ? w[h][1] * so.x : 0.f);
+            const float x0 = w[h][0] * so.x, x1 = QC == 2 ? w[h][1] * so.x : 0.f;
+            if constexpr (kTwice) {  // threads 2 and 3 take what the rounding leaves
+              const float2 r = unpack2<B>(Half16<B>::pack(x0, x1));
+              first[h] = transpose8x8(Half16<B>::pack(fmaf(lower, r.x, x0), QC == 2 ? fmaf(lower, r.y, x1) : 0.f));
+            } else {
+              const uint2 x = Half16<B>::split(x0, x1);
+              first[h] = transpose8x8(x.x);
+              second[h] = transpose8x8(x.y);
+            }
           }
           const uint32_t near[2] = {__byte_perm(vr[u][0][v], vr[u][1][v], 0x5410), __byte_perm(vr[u][0][v], vr[u][1][v], 0x7632)};
           const uint32_t far[2] = {__byte_perm(vr[u][2][v], vr[u][3][v], 0x5410), __byte_perm(vr[u][2][v], vr[u][3][v], 0x7632)};
-          uint32_t first[2], second[2];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            first[h] = transpose8x8(kTwice && t >= 2 ? parts[h].y : parts[h].x);
-            if constexpr (!kTwice) second[h] = transpose8x8(parts[h].y);
-          }
           auto dims = [&](auto which) {  // 8g + 2w (row g of the product) and 8g + 2w + 1 (row g + 8)
             constexpr int W = decltype(which)::value;
             const uint32_t v0 = codes2<B, W>(near[0]), v1 = codes2<B, W>(near[1]);
@@ -545,13 +552,13 @@ __device__ __forceinline__ void attend_tiles_of(const PagedCache& c, const Atten
                                                 const uint4 (&q)[NB][D / 32], int (&page)[step_tiles(D, Form)],
                                                 StepSums<D, NB>& sums) {
   if constexpr (Form != 16)
-    attend_tiles4<T, D, NB, Form>(c, a, seen, row, mask, head, t0, t1, q, page, sums);
+    attend_tiles4<T, D, NB, Form>(c, a, seen, row, mask, head, t0, t1, q, sums);
   else
     attend_tiles<T, D, NB>(c, a, seen, row, mask, static_cast<int64_t>(head) * c.page_size * D, t0, t1, q, page, sums);
 }
 
 template <typename T, int D, int NB, int Form>
-__global__ void __launch_bounds__(kStepThreads, step_ctas(D, NB))
+__global__ void __launch_bounds__(kStepThreads, step_ctas(D, NB, Form))
     step_kernel(PagedCache c, Attend a, SharedPrefix shared, StepSpace ws, int blocks, int min_tiles) {
   constexpr int NT = step_tiles(D, Form);
   constexpr int NQ = 8 * NB;   // query rows of a unit
@@ -969,29 +976,30 @@ void step_blocks(int group, int* nb, int* blocks) {
 // cut records, then parts; sized for the largest device this library runs on
 // (kMaxSms SMs), so that the size does not depend on the current one
 constexpr int kMaxSms = 160;
-size_t cut_bytes(int head_dim, int nb) {
-  return static_cast<size_t>(kMaxSms) * step_ctas(head_dim, nb) * kStepWarps * sizeof(int4);
+size_t cut_bytes(int head_dim, int nb, int form) {
+  return static_cast<size_t>(kMaxSms) * step_ctas(head_dim, nb, form) * kStepWarps * sizeof(int4);
 }
 
 size_t step_workspace(const mtt_b200_paged_cache_t& c, int q_heads) {
   int nb, blocks;
   step_blocks(q_heads / c.kv_heads, &nb, &blocks);
-  const size_t shares = static_cast<size_t>(kMaxSms) * step_ctas(c.head_dim, nb) * kStepWarps;
-  return cut_bytes(c.head_dim, nb) + (shares * 2 * 8 * nb * (c.head_dim + 2) * 4 + 255) / 256 * 256;
+  const int form = step_form((c.dtype & MTT_B200_CACHE_4BIT) != 0 ? 4 : 16, q_heads / c.kv_heads);
+  const size_t shares = static_cast<size_t>(kMaxSms) * step_ctas(c.head_dim, nb, form) * kStepWarps;
+  return cut_bytes(c.head_dim, nb, form) + (shares * 2 * 8 * nb * (c.head_dim + 2) * 4 + 255) / 256 * 256;
 }
 
 cudaError_t launch_step(const PagedCache& c, int dtype, const Attend& a, const SharedPrefix& shared, void* space,
                         cudaStream_t stream) {
   int nb, blocks;
   step_blocks(a.group, &nb, &blocks);
+  const int form = step_form(c.bits, a.group);
   StepSpace ws;
   ws.cut = static_cast<int4*>(space);
-  ws.part = reinterpret_cast<float*>(static_cast<char*>(space) + cut_bytes(c.head_dim, nb));
+  ws.part = reinterpret_cast<float*>(static_cast<char*>(space) + cut_bytes(c.head_dim, nb, form));
   const int sms = cache_sm_count();
   if (sms <= 0 || sms > kMaxSms) return cudaErrorInvalidValue;
   const size_t smem = 4 * (static_cast<size_t>(a.rows) + 1);
-  const int grid = sms * step_ctas(c.head_dim, nb), shares = grid * kStepWarps;
-  const int form = step_form(c.bits, a.group);
+  const int grid = sms * step_ctas(c.head_dim, nb, form), shares = grid * kStepWarps;
   const int min_tiles = kUnitCost + step_tiles(c.head_dim, form);
   const int pairs = std::min(8 * nb, a.group) * c.head_dim / 2;
   auto go = [&](auto kernel, auto join) {
