@@ -47,11 +47,13 @@ constexpr int kStepWarps = 4;
 constexpr int kStepThreads = 32 * kStepWarps;
 
 // Forms of the kernels: 16 for a pool in 16 bits; for one in 4 bits how many query
-// heads a key head has at most: 1, 4 or more (8).
-constexpr int step_form(int bits, int group) { return bits == 16 ? 16 : group == 1 ? 1 : group <= 4 ? 4 : 8; }
+// heads a key head has at most: 1, 2, 4 or more (8).
+constexpr int step_form(int bits, int group) { return bits == 16 ? 16 : group <= 2 ? group : group <= 4 ? 4 : 8; }
 
 // 16-key tiles per warp and step
-constexpr int step_tiles(int head_dim, int form) { return (head_dim == 64 ? 2 : 1) * (form == 16 ? 1 : 2); }
+constexpr int step_tiles(int head_dim, int form) {
+  return form == 16 ? (head_dim == 64 ? 2 : 1) : form == 8 && head_dim == 128 ? 2 : 4;
+}
 constexpr int step_ctas(int head_dim, int nb, int form) {  // per SM (registers)
   return (head_dim == 64 ? 4 : 3) - (nb == 2 ? 1 : 0);
 }
@@ -311,7 +313,7 @@ __device__ __forceinline__ int step_dims(int t, int k) {
 // The query of a product's column.
 template <int Form>
 __device__ __forceinline__ int step_column(int g) {
-  return Form == 16 || Form == 8 ? g : g & 3;
+  return Form == 16 ? g : g & (Form == 1 ? 1 : Form - 1);  // (with one query the odd columns are empty)
 }
 
 // attend_tiles for a pool in 4 bits.  Nothing is rounded on the way into the
@@ -319,14 +321,23 @@ __device__ __forceinline__ int step_column(int g) {
 // pairs come in afterwards, in f32,
 //   q.k = sum over groups: step (q.(16 + c)) + off sum q,   off = low - 16 step;
 // the values' weights are p step, in two bf16 numbers each (their range is not
-// f16's), and p off is summed by itself.  Up to four queries take the product's
-// columns twice, the weights' first numbers in columns 0 to 3 and what their
-// rounding leaves in 4 to 7: one product for both, the halves added at the end.
+// f16's), and p off is summed by itself.
 //
-// What bounds it is instructions, a third of them the codes' way into 16 bits, so
-// the rest is kept few: addresses are one sum a tile, all 16 keys of a tile are
-// loaded (a masked key's pair is taken as zero), and the maximum is looked after
-// only when a key passes it.
+// What bounds it is instructions, above all the logic and shift unit's: the codes'
+// way into 16 bits takes two for each pair of codes, 64 a tile of 16 keys and 64
+// dims, and so the rest has to be few.
+//  * A product has 8 columns.  Few queries take them several times, each time for
+//    another tile: with one or two queries (Form 1, 2) a thread's two columns are
+//    those of tile t of four, with up to four of tile t / 2 of two.  Scores of the
+//    other tiles are passed over, so that a thread has two scores a query in four
+//    (two) tiles, and loads, weighs and masks two pairs instead of eight.  For the
+//    values the weights go through one transposition for all of them and are
+//    cleared outside the tile's own columns; the columns are added up at the end.
+//    With one query the second column holds what the first one's rounding leaves.
+//  * Addresses are 64-byte units in 32 bits, found by one lane a tile.
+//  * All 16 keys of a tile are loaded; a key that is not in reach counts by its
+//    weight of zero alone (its pair, which may be anything, is taken as zero).
+//  * The maximum is looked after only when a key passes it.
 template <typename T, int D, int NB, int Form>
 __device__ __forceinline__ void attend_tiles4(const PagedCache& c, const Attend& a, const SeenTiles& seen,
                                               const int32_t* row, const bool* mask, int head, int t0, int t1,
@@ -334,9 +345,12 @@ __device__ __forceinline__ void attend_tiles4(const PagedCache& c, const Attend&
   using B = __nv_bfloat16;
   constexpr int NT = step_tiles(D, Form);
   constexpr int G = D / kGroup4;
-  constexpr int QC = Form == 1 ? 1 : 2;  // columns that a thread looks after
-  constexpr bool kTwice = Form <= 4;
+  constexpr int QC = Form == 1 ? 1 : 2;                        // queries of a thread
+  constexpr int TP = Form <= 2 ? 4 : Form == 4 ? 2 : 1;        // tiles that share the columns
+  constexpr int NP = NT / TP, kTileShift = TP == 4 ? 0 : TP == 2 ? 1 : 2;
   const int lane = threadIdx.x & 31, t = lane & 3, g = lane >> 2;
+  const int my = t >> kTileShift;         // the thread's tile of each TP
+  const int col_tile = g >> (kTileShift + 1);  // the tile of column g
   auto &m = sums.m, &l = sums.l;
   auto& acc = sums.acc;
   // the queries' sums over each group, times the scale
@@ -364,95 +378,110 @@ __device__ __forceinline__ void attend_tiles4(const PagedCache& c, const Attend&
         rest[b][v][i] = 0.f;
       }
     }
-  // where the thread's bytes are in a block: codes of keys g (and g + 8), of values 2t (2t + 1, 2t + 8, 2t + 9), pairs
-  const int64_t page_bytes = static_cast<int64_t>(c.layers) * 4 * c.kv_elems;
-  const unsigned char* blocks = block4(c, 0, a.layer, 0, head);
-  const int k_at = g * (D / 2) + 8 * t, v_at = 2 * static_cast<int>(c.kv_elems) + 2 * t * (D / 2) + 4 * g;
-  const int p_at = block4_codes(c) + g * (4 * G), pv_at = 2 * static_cast<int>(c.kv_elems);
-  // Lane u (of each NT) looks up tile u of the step and tells the others.
+  // the thread's bytes in page 0's block: codes of keys g (and g + 8), of values 2t (2t + 1, 2t + 8, 2t + 9), pairs of keys g
+  const unsigned char* k_base = block4(c, 0, a.layer, 0, head);
+  const unsigned char* p_base = k_base + block4_codes(c) + g * (4 * G);
+  const unsigned char* vp_base = p_base + 2 * c.kv_elems;
+  const unsigned char* v_base = k_base + 2 * c.kv_elems + 2 * t * (D / 2) + 4 * g;
+  k_base += g * (D / 2) + 8 * t;
+  const uint32_t page_units = static_cast<uint32_t>(c.layers * c.kv_elems / 16);  // of 64 bytes: a pool of 256 GB at most
+  // lane u (of each NT) looks up tile u of the step
   const int mine = lane & (NT - 1);
-  const float lower = t >= 2 ? -1.f : 0.f;
   auto lookup = [&](int tile) { return tile < t1 ? row[(16 * seen.tile(tile)) >> c.page_shift] : -1; };
   int my_page = lookup(t0 + mine);
   for (int base = t0; base < t1; base += NT) {
-    const int my_key = 16 * seen.tile(base + mine), my_in = c.is_page(my_page) ? my_key & (c.page_size - 1) : -1;
-    const int64_t my_at = reinterpret_cast<int64_t>(blocks) + my_page * page_bytes + my_in * (D / 2);
+    const int my_key = 16 * seen.tile(base + mine);
+    // the tile's place in its page in tiles (-1: there is none), and where its codes begin
+    const int my_in = c.is_page(my_page) ? (my_key & (c.page_size - 1)) >> 4 : -1;
+    const uint32_t my_at = my_page * page_units + my_in * (D / 8);
     const int next_page = lookup(base + NT + mine);  // on its way while this step's keys arrive
-    // keys in reach: one per lane and pair of tiles
-    uint32_t bits[NT / 2];
-#pragma unroll
-    for (int u = 0; u < NT / 2; ++u) {
-      const int j = __shfl_sync(0xffffffffu, my_key, 2 * u + (lane >> 4)) + (lane & 15);
-      bool in = base + 2 * u + (lane >> 4) < t1 && j < seen.len && (j >= seen.low || j < a.sinks);
-      if (in && mask != nullptr) in = mask[j];
-      bits[u] = __ballot_sync(0xffffffffu, in);
-    }
     uint2 kr[NT][2][G];
-    uint32_t vr[NT][4][G], kp[NT][2][G], vp[NT][2][G];
-    bool on[NT][2];  // the thread's keys g, g + 8
+    uint32_t vr[NT][4][G];
 #pragma unroll
     for (int u = 0; u < NT; ++u) {
-      const int in_page = __shfl_sync(0xffffffffu, my_in, u);
-      const bool there = in_page >= 0;
-      const uint32_t my_bits = (there ? bits[u >> 1] : 0u) >> (16 * (u & 1) + g);
-      on[u][0] = (my_bits & 1u) != 0;
-      on[u][1] = (my_bits & 256u) != 0;
-      const unsigned char* at = reinterpret_cast<const unsigned char*>(__shfl_sync(0xffffffffu, my_at, u));
-      const unsigned char* pairs = at + (p_at - in_page * (D / 2 - 4 * G));
+      const bool there = __shfl_sync(0xffffffffu, my_in, u) >= 0;
+      const int64_t at = static_cast<int64_t>(__shfl_sync(0xffffffffu, my_at, u)) * 64;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int v = 0; v < G; ++v) kr[u][h][v] = load8(at + k_at + 8 * h * (D / 2) + 32 * v, there);
-        if constexpr (G == 1) {
-          kp[u][h][0] = load4(pairs + 8 * h * 4, there);
-          vp[u][h][0] = load4(pairs + pv_at + 8 * h * 4, there);
-        } else {
-          const uint2 x = load8(pairs + 8 * h * 8, there), y = load8(pairs + pv_at + 8 * h * 8, there);
-          kp[u][h][0] = x.x;
-          kp[u][h][1] = x.y;
-          vp[u][h][0] = y.x;
-          vp[u][h][1] = y.y;
-        }
-      }
+        for (int v = 0; v < G; ++v) kr[u][h][v] = load8(k_base + at + 8 * h * (D / 2) + 32 * v, there);
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int v = 0; v < G; ++v) vr[u][i][v] = load4(at + v_at + ((i & 1) + 8 * (i >> 1)) * (D / 2) + 32 * v, there);
+        for (int v = 0; v < G; ++v) vr[u][i][v] = load4(v_base + at + ((i & 1) + 8 * (i >> 1)) * (D / 2) + 32 * v, there);
+    }
+    uint32_t kp[NP][2][G], vp[NP][2][G];
+    bool on[NP][2];  // the thread's keys g, g + 8 of its tiles
+#pragma unroll
+    for (int n = 0; n < NP; ++n) {
+      const int u = n * TP + my;
+      const int key = TP == NT ? my_key : __shfl_sync(0xffffffffu, my_key, u);
+      const int in = TP == NT ? my_in : __shfl_sync(0xffffffffu, my_in, u);
+      const uint32_t first = TP == NT ? my_at : __shfl_sync(0xffffffffu, my_at, u);
+      const int64_t at = static_cast<int64_t>(first - in * (D / 8 - G)) * 64;  // pairs lie in 64-byte units, too
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int j = key + g + 8 * h;
+        on[n][h] = in >= 0 && j < seen.len && (j >= seen.low || j < a.sinks);
+        if constexpr (G == 1) {
+          kp[n][h][0] = load4(p_base + at + 32 * h, in >= 0);
+          vp[n][h][0] = load4(vp_base + at + 32 * h, in >= 0);
+        } else {
+          const uint2 x = load8(p_base + at + 64 * h, in >= 0), y = load8(vp_base + at + 64 * h, in >= 0);
+          kp[n][h][0] = x.x;
+          kp[n][h][1] = x.y;
+          vp[n][h][0] = y.x;
+          vp[n][h][1] = y.y;
+        }
+      }
+      if (mask != nullptr) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          if (on[n][h]) on[n][h] = mask[key + g + 8 * h];
+      }
     }
     my_page = next_page;
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      float s[NT][2][QC], top[QC];
+      float s[NP][2][QC], top[QC];
 #pragma unroll
       for (int i = 0; i < QC; ++i) top[i] = -CUDART_INF_F;
 #pragma unroll
-      for (int u = 0; u < NT; ++u) {
+      for (int n = 0; n < NP; ++n) {
+        float x[G][4];
 #pragma unroll
-        for (int v = 0; v < G; ++v) {
-          float x[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int u = 0; u < TP; ++u)
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const uint32_t w0 = k == 0 ? kr[u][0][v].x : kr[u][0][v].y, w1 = k == 0 ? kr[u][1][v].x : kr[u][1][v].y;
-            const uint4& y = q[b][2 * v + k];
-            Half16<T>::mma(x, codes2<T, 0>(w0), codes2<T, 0>(w1), codes2<T, 1>(w0), codes2<T, 1>(w1), y.x, y.y);
-            Half16<T>::mma(x, codes2<T, 2>(w0), codes2<T, 2>(w1), codes2<T, 3>(w0), codes2<T, 3>(w1), y.z, y.w);
+          for (int v = 0; v < G; ++v) {
+            float y[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const uint2 &r0 = kr[n * TP + u][0][v], &r1 = kr[n * TP + u][1][v];
+              const uint32_t w0 = k == 0 ? r0.x : r0.y, w1 = k == 0 ? r1.x : r1.y;
+              const uint4& z = q[b][2 * v + k];
+              Half16<T>::mma(y, codes2<T, 0>(w0), codes2<T, 0>(w1), codes2<T, 1>(w0), codes2<T, 1>(w1), z.x, z.y);
+              Half16<T>::mma(y, codes2<T, 2>(w0), codes2<T, 2>(w1), codes2<T, 3>(w0), codes2<T, 3>(w1), z.z, z.w);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (QC == 2 || i % 2 == 0) x[v][i] = u == 0 || my == u ? y[i] : x[v][i];
           }
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float2 so = step_off(unpack2<T>(kp[u][h][v]));
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int v = 0; v < G; ++v) {
+            const float2 so = step_off(unpack2<T>(kp[n][h][v]));
             const float step = so.x * a.scale2;
 #pragma unroll
             for (int i = 0; i < QC; ++i)
-              s[u][h][i] = fmaf(step, x[2 * h + i], v == 0 ? so.y * qs[b][0][i] : fmaf(so.y, qs[b][v][i], s[u][h][i]));
+              s[n][h][i] = fmaf(step, x[v][2 * h + i], v == 0 ? so.y * qs[b][0][i] : fmaf(so.y, qs[b][v][i], s[n][h][i]));
           }
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int i = 0; i < QC; ++i) {
-            s[u][h][i] = on[u][h] ? s[u][h][i] : -CUDART_INF_F;
-            top[i] = fmaxf(top[i], s[u][h][i]);
+            s[n][h][i] = on[n][h] ? s[n][h][i] : -CUDART_INF_F;
+            top[i] = fmaxf(top[i], s[n][h][i]);
           }
+        }
       }
       bool more = false;
 #pragma unroll
@@ -460,8 +489,9 @@ __device__ __forceinline__ void attend_tiles4(const PagedCache& c, const Attend&
       if (__any_sync(0xffffffffu, more)) {
 #pragma unroll
         for (int i = 0; i < QC; ++i) {
+          // over the keys and, where the columns are shared, over the tiles
 #pragma unroll
-          for (int o = 4; o < 32; o <<= 1) top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
+          for (int o = TP == 4 ? 1 : TP == 2 ? 2 : 4; o < 32; o <<= 1) top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
           top[i] = fmaxf(top[i], m[b][i]);
           const float keep = top[i] == -CUDART_INF_F ? 1.f : ex2(m[b][i] - top[i]);
           m[b][i] = top[i];
@@ -473,6 +503,10 @@ __device__ __forceinline__ void attend_tiles4(const PagedCache& c, const Attend&
             for (int w = 0; w < 4; ++w) {
               acc[b][v][w][i] *= keep;
               acc[b][v][w][2 + i] *= keep;
+              if constexpr (QC == 1) {
+                acc[b][v][w][1] *= keep;
+                acc[b][v][w][3] *= keep;
+              }
             }
           }
         }
@@ -481,13 +515,13 @@ __device__ __forceinline__ void attend_tiles4(const PagedCache& c, const Attend&
 #pragma unroll
       for (int i = 0; i < QC; ++i) z[i] = m[b][i] == -CUDART_INF_F ? 0.f : m[b][i];
 #pragma unroll
-      for (int u = 0; u < NT; ++u) {
-        float w[2][2];
+      for (int n = 0; n < NP; ++n) {
+        float w[2][QC];
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int i = 0; i < QC; ++i) {
-            w[h][i] = ex2(s[u][h][i] - z[i]);
+            w[h][i] = ex2(s[n][h][i] - z[i]);
             l[b][i] += w[h][i];
           }
 #pragma unroll
@@ -495,55 +529,67 @@ __device__ __forceinline__ void attend_tiles4(const PagedCache& c, const Attend&
           uint32_t first[2], second[2];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const float2 so = step_off(unpack2<T>(on[u][h] ? vp[u][h][v] : 0u));
+            const float2 so = step_off(unpack2<T>(on[n][h] ? vp[n][h][v] : 0u));
 #pragma unroll
             for (int i = 0; i < QC; ++i) rest[b][v][i] = fmaf(w[h][i], so.y, rest[b][v][i]);
-            const float x0 = w[h][0] * so.x, x1 = QC == 2 ? w[h][1] * so.x : 0.f;
-            if constexpr (kTwice) {  // threads 2 and 3 take what the rounding leaves
-              const float2 r = unpack2<B>(Half16<B>::pack(x0, x1));
-              first[h] = transpose8x8(Half16<B>::pack(fmaf(lower, r.x, x0), QC == 2 ? fmaf(lower, r.y, x1) : 0.f));
+            const float x0 = w[h][0] * so.x;
+            if constexpr (QC == 1) {
+              first[h] = transpose8x8(Half16<B>::pack(x0, x0 - unpack2<B>(Half16<B>::pack(x0, 0.f)).x));
             } else {
-              const uint2 x = Half16<B>::split(x0, x1);
+              const uint2 x = Half16<B>::split(x0, w[h][1] * so.x);
               first[h] = transpose8x8(x.x);
               second[h] = transpose8x8(x.y);
             }
           }
-          const uint32_t near[2] = {__byte_perm(vr[u][0][v], vr[u][1][v], 0x5410), __byte_perm(vr[u][0][v], vr[u][1][v], 0x7632)};
-          const uint32_t far[2] = {__byte_perm(vr[u][2][v], vr[u][3][v], 0x5410), __byte_perm(vr[u][2][v], vr[u][3][v], 0x7632)};
-          auto dims = [&](auto which) {  // 8g + 2w (row g of the product) and 8g + 2w + 1 (row g + 8)
-            constexpr int W = decltype(which)::value;
-            const uint32_t v0 = codes2<B, W>(near[0]), v1 = codes2<B, W>(near[1]);
-            const uint32_t v2 = codes2<B, W>(far[0]), v3 = codes2<B, W>(far[1]);
-            Half16<B>::mma(acc[b][v][W], v0, v1, v2, v3, first[0], first[1]);
-            if constexpr (!kTwice) Half16<B>::mma(acc[b][v][W], v0, v1, v2, v3, second[0], second[1]);
-          };
-          dims(std::integral_constant<int, 0>{});
-          dims(std::integral_constant<int, 1>{});
-          dims(std::integral_constant<int, 2>{});
-          dims(std::integral_constant<int, 3>{});
+#pragma unroll
+          for (int u = 0; u < TP; ++u) {
+            const uint32_t(&r)[4][G] = vr[n * TP + u];
+            const uint32_t near[2] = {__byte_perm(r[0][v], r[1][v], 0x5410), __byte_perm(r[0][v], r[1][v], 0x7632)};
+            const uint32_t far[2] = {__byte_perm(r[2][v], r[3][v], 0x5410), __byte_perm(r[2][v], r[3][v], 0x7632)};
+            const bool mine = TP == 1 || col_tile == u;
+            const uint32_t b0 = mine ? first[0] : 0u, b1 = mine ? first[1] : 0u;
+            auto dims = [&](auto which) {  // 8g + 2w (row g of the product) and 8g + 2w + 1 (row g + 8)
+              constexpr int W = decltype(which)::value;
+              const uint32_t v0 = codes2<B, W>(near[0]), v1 = codes2<B, W>(near[1]);
+              const uint32_t v2 = codes2<B, W>(far[0]), v3 = codes2<B, W>(far[1]);
+              Half16<B>::mma(acc[b][v][W], v0, v1, v2, v3, b0, b1);
+              if constexpr (QC == 2) Half16<B>::mma(acc[b][v][W], v0, v1, v2, v3, mine ? second[0] : 0u, mine ? second[1] : 0u);
+            };
+            dims(std::integral_constant<int, 0>{});
+            dims(std::integral_constant<int, 1>{});
+            dims(std::integral_constant<int, 2>{});
+            dims(std::integral_constant<int, 3>{});
+          }
         }
       }
     }
   }
-  // the weights' part that belongs to no code is the same for all dims of a group
+  // shared columns are added up; the weights' part that belongs to no code is the same for all dims of a group
+  auto over_tiles = [&](float x) {
+    if constexpr (TP == 4) x += __shfl_xor_sync(0xffffffffu, x, 1);
+    if constexpr (TP >= 2) x += __shfl_xor_sync(0xffffffffu, x, 2);
+    return x;
+  };
 #pragma unroll
   for (int b = 0; b < NB; ++b)
 #pragma unroll
-    for (int v = 0; v < G; ++v)
+    for (int i = 0; i < QC; ++i) {
+      l[b][i] = over_tiles(l[b][i]);
 #pragma unroll
-      for (int i = 0; i < QC; ++i) {
+      for (int v = 0; v < G; ++v) {
         float x = rest[b][v][i];
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+        x = over_tiles(x);
 #pragma unroll
         for (int w = 0; w < 4; ++w)
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
             float& o = acc[b][v][w][2 * k + i];
-            if constexpr (kTwice) o += __shfl_xor_sync(0xffffffffu, o, 2);
-            o += x;
+            o = over_tiles(QC == 1 ? o + acc[b][v][w][2 * k + 1] : o) + x;
           }
       }
+    }
 }
 
 template <typename T, int D, int NB, int Form>
@@ -1044,6 +1090,7 @@ cudaError_t launch_step(const PagedCache& c, int dtype, const Attend& a, const S
     if (form == 16) return with_form(type, dim, bs, integral_constant<int, 16>{});
     if constexpr (decltype(bs)::value == 1) {
       if (form == 1) return with_form(type, dim, bs, integral_constant<int, 1>{});
+      if (form == 2) return with_form(type, dim, bs, integral_constant<int, 2>{});
       if (form == 4) return with_form(type, dim, bs, integral_constant<int, 4>{});
     }
     return with_form(type, dim, bs, integral_constant<int, 8>{});
