@@ -52,7 +52,7 @@ constexpr int step_form(int bits, int group) { return bits == 16 ? 16 : group <=
 
 // 16-key tiles per warp and step
 constexpr int step_tiles(int head_dim, int form) {
-  return form == 16 ? (head_dim == 64 ? 2 : 1) : form == 8 && head_dim == 128 ? 2 : 4;
+  return form == 16 ? (head_dim == 64 ? 2 : 1) : form >= 4 && head_dim == 128 ? 2 : 4;
 }
 constexpr int step_ctas(int head_dim, int nb, int form) {  // per SM (registers)
   return (head_dim == 64 ? 4 : 3) - (nb == 2 ? 1 : 0);
@@ -61,7 +61,8 @@ constexpr int step_ctas(int head_dim, int nb, int form) {  // per SM (registers)
 // A unit's place on the line: its tiles, and before them what entering and
 // leaving it costs, in tiles.  (2052 slots with 1 to 249 keys each, prefix pass
 // included: 134 us with 0, 96 with 2, 104 with 4, 116 with 8.)
-constexpr int kUnitCost = 2;
+// (512 sessions over a 4-bit pool: 113 us with 2, 109 with 4.)
+constexpr int unit_cost(int form) { return form == 16 ? 2 : 4; }
 
 // Probabilities are held 2^15 times as large where the cache is f16, so that what
 // is small beside the largest (1) stays in that type's range; sums and weighted
@@ -293,15 +294,15 @@ __device__ __forceinline__ void attend_tiles(const PagedCache& c, const Attend& 
   }
 }
 
-// 4 or 8 bytes, as load16.
-__device__ __forceinline__ uint32_t load4(const unsigned char* p, bool on) {
-  uint32_t v = 0;
-  if (on) asm volatile("ld.global.L1::no_allocate.u32 %0, [%1];" : "=r"(v) : "l"(p));
+// 4 or 8 bytes, as load16, without a condition: a register that a load may leave as it is costs an instruction to clear.
+__device__ __forceinline__ uint32_t load4(const unsigned char* p) {
+  uint32_t v;
+  asm volatile("ld.global.L1::no_allocate.u32 %0, [%1];" : "=r"(v) : "l"(p));
   return v;
 }
-__device__ __forceinline__ uint2 load8(const unsigned char* p, bool on) {
-  uint2 v = make_uint2(0, 0);
-  if (on) asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+__device__ __forceinline__ uint2 load8(const unsigned char* p) {
+  uint2 v;
+  asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
   return v;
 }
 
@@ -385,54 +386,62 @@ __device__ __forceinline__ void attend_tiles4(const PagedCache& c, const Attend&
   const unsigned char* v_base = k_base + 2 * c.kv_elems + 2 * t * (D / 2) + 4 * g;
   k_base += g * (D / 2) + 8 * t;
   const uint32_t page_units = static_cast<uint32_t>(c.layers * c.kv_elems / 16);  // of 64 bytes: a pool of 256 GB at most
-  // lane u (of each NT) looks up tile u of the step
+  // Lane u (of each NT) looks up tile u of a step: its first key, its place in its page in tiles (-1: there is none), and
+  // where its codes begin.
   const int mine = lane & (NT - 1);
-  auto lookup = [&](int tile) { return tile < t1 ? row[(16 * seen.tile(tile)) >> c.page_shift] : -1; };
-  int my_page = lookup(t0 + mine);
-  for (int base = t0; base < t1; base += NT) {
-    const int my_key = 16 * seen.tile(base + mine);
-    // the tile's place in its page in tiles (-1: there is none), and where its codes begin
-    const int my_in = c.is_page(my_page) ? (my_key & (c.page_size - 1)) >> 4 : -1;
-    const uint32_t my_at = my_page * page_units + my_in * (D / 8);
-    const int next_page = lookup(base + NT + mine);  // on its way while this step's keys arrive
-    uint2 kr[NT][2][G];
-    uint32_t vr[NT][4][G];
+  auto lookup = [&](int base) { return base + mine < t1 ? row[(16 * seen.tile(base + mine)) >> c.page_shift] : -1; };
+  struct Place {
+    int key, in;
+    uint32_t at;
+  };
+  auto place = [&](int base, int page) {
+    Place p;
+    p.key = 16 * seen.tile(base + mine);
+    p.in = c.is_page(page) ? (p.key & (c.page_size - 1)) >> 4 : -1;
+    p.at = page * page_units + p.in * (D / 8);
+    return p;
+  };
+  auto at64 = [](const unsigned char* from, uint32_t units) {  // from + 64 units
+    uint64_t r;
+    asm("mad.wide.u32 %0, %1, 64, %2;" : "=l"(r) : "r"(units), "l"(from));
+    return reinterpret_cast<const unsigned char*>(r);
+  };
+  // (a tile that is not there leaves its registers as they are: codes are numbers whatever they are, pairs are looked at
+  // only where a key is in reach)
+  uint2 kr[NT][2][G] = {};
+  uint32_t vr[NT][4][G] = {}, kp[NP][2][G] = {}, vp[NP][2][G] = {};
+  auto load_pair = [](uint32_t (&to)[G], const unsigned char* at) {
+    if constexpr (G == 1) {
+      to[0] = load4(at);
+    } else {
+      const uint2 x = load8(at);
+      to[0] = x.x;
+      to[1] = x.y;
+    }
+  };
+  auto load_keys = [&](const Place& p, bool (&on)[NP][2]) {  // on: whether the thread's keys g, g + 8 of its tiles are in reach
 #pragma unroll
     for (int u = 0; u < NT; ++u) {
-      const bool there = __shfl_sync(0xffffffffu, my_in, u) >= 0;
-      const int64_t at = static_cast<int64_t>(__shfl_sync(0xffffffffu, my_at, u)) * 64;
+      const bool there = __shfl_sync(0xffffffffu, p.in, u) >= 0;
+      const unsigned char* at = at64(k_base, __shfl_sync(0xffffffffu, p.at, u));
+      if (there) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int v = 0; v < G; ++v) kr[u][h][v] = load8(k_base + at + 8 * h * (D / 2) + 32 * v, there);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int v = 0; v < G; ++v) vr[u][i][v] = load4(v_base + at + ((i & 1) + 8 * (i >> 1)) * (D / 2) + 32 * v, there);
+          for (int v = 0; v < G; ++v) kr[u][h][v] = load8(at + 8 * h * (D / 2) + 32 * v);
+      }
     }
-    uint32_t kp[NP][2][G], vp[NP][2][G];
-    bool on[NP][2];  // the thread's keys g, g + 8 of its tiles
 #pragma unroll
     for (int n = 0; n < NP; ++n) {
       const int u = n * TP + my;
-      const int key = TP == NT ? my_key : __shfl_sync(0xffffffffu, my_key, u);
-      const int in = TP == NT ? my_in : __shfl_sync(0xffffffffu, my_in, u);
-      const uint32_t first = TP == NT ? my_at : __shfl_sync(0xffffffffu, my_at, u);
-      const int64_t at = static_cast<int64_t>(first - in * (D / 8 - G)) * 64;  // pairs lie in 64-byte units, too
+      const int key = TP == 4 ? p.key : __shfl_sync(0xffffffffu, p.key, u), in = TP == 4 ? p.in : __shfl_sync(0xffffffffu, p.in, u);
+      const uint32_t first = TP == 4 ? p.at : __shfl_sync(0xffffffffu, p.at, u);
+      const unsigned char* at = at64(p_base, first - in * (D / 8 - G));  // pairs lie in 64-byte units, too
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int j = key + g + 8 * h;
         on[n][h] = in >= 0 && j < seen.len && (j >= seen.low || j < a.sinks);
-        if constexpr (G == 1) {
-          kp[n][h][0] = load4(p_base + at + 32 * h, in >= 0);
-          vp[n][h][0] = load4(vp_base + at + 32 * h, in >= 0);
-        } else {
-          const uint2 x = load8(p_base + at + 64 * h, in >= 0), y = load8(vp_base + at + 64 * h, in >= 0);
-          kp[n][h][0] = x.x;
-          kp[n][h][1] = x.y;
-          vp[n][h][0] = y.x;
-          vp[n][h][1] = y.y;
-        }
+        if (in >= 0) load_pair(kp[n][h], at + 32 * G * h);
       }
       if (mask != nullptr) {
 #pragma unroll
@@ -440,12 +449,44 @@ __device__ __forceinline__ void attend_tiles4(const PagedCache& c, const Attend&
           if (on[n][h]) on[n][h] = mask[key + g + 8 * h];
       }
     }
-    my_page = next_page;
+  };
+  auto load_values = [&](const Place& p) {
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+      const bool there = __shfl_sync(0xffffffffu, p.in, u) >= 0;
+      const unsigned char* at = at64(v_base, __shfl_sync(0xffffffffu, p.at, u));
+      if (there) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int v = 0; v < G; ++v) vr[u][i][v] = load4(at + ((i & 1) + 8 * (i >> 1)) * (D / 2) + 32 * v);
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < NP; ++n) {
+      const int u = n * TP + my;
+      const int in = TP == 4 ? p.in : __shfl_sync(0xffffffffu, p.in, u);
+      const uint32_t first = TP == 4 ? p.at : __shfl_sync(0xffffffffu, p.at, u);
+      const unsigned char* at = at64(vp_base, first - in * (D / 8 - G));
+      if (in >= 0) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) load_pair(vp[n][h], at + 32 * G * h);
+      }
+    }
+  };
+  bool on[NP][2];
+  Place here = place(t0, lookup(t0));
+  int next_page = lookup(t0 + NT);
+  load_keys(here, on);
+  load_values(here);
+  for (int base = t0; base < t1; base += NT) {
+    const Place next = place(base + NT, next_page);
+    next_page = lookup(base + 2 * NT);
+    float s[NB][NP][2][QC], top[NB][QC];
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      float s[NP][2][QC], top[QC];
 #pragma unroll
-      for (int i = 0; i < QC; ++i) top[i] = -CUDART_INF_F;
+      for (int i = 0; i < QC; ++i) top[b][i] = -CUDART_INF_F;
 #pragma unroll
       for (int n = 0; n < NP; ++n) {
         float x[G][4];
@@ -453,13 +494,16 @@ __device__ __forceinline__ void attend_tiles4(const PagedCache& c, const Attend&
         for (int u = 0; u < TP; ++u)
 #pragma unroll
           for (int v = 0; v < G; ++v) {
-            float y[4] = {0.f, 0.f, 0.f, 0.f};
+            float y[4];
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
               const uint2 &r0 = kr[n * TP + u][0][v], &r1 = kr[n * TP + u][1][v];
               const uint32_t w0 = k == 0 ? r0.x : r0.y, w1 = k == 0 ? r1.x : r1.y;
               const uint4& z = q[b][2 * v + k];
-              Half16<T>::mma(y, codes2<T, 0>(w0), codes2<T, 0>(w1), codes2<T, 1>(w0), codes2<T, 1>(w1), z.x, z.y);
+              if (k == 0)
+                Half16<T>::mma0(y, codes2<T, 0>(w0), codes2<T, 0>(w1), codes2<T, 1>(w0), codes2<T, 1>(w1), z.x, z.y);
+              else
+                Half16<T>::mma(y, codes2<T, 0>(w0), codes2<T, 0>(w1), codes2<T, 1>(w0), codes2<T, 1>(w1), z.x, z.y);
               Half16<T>::mma(y, codes2<T, 2>(w0), codes2<T, 2>(w1), codes2<T, 3>(w0), codes2<T, 3>(w1), z.z, z.w);
             }
 #pragma unroll
@@ -474,27 +518,32 @@ __device__ __forceinline__ void attend_tiles4(const PagedCache& c, const Attend&
             const float step = so.x * a.scale2;
 #pragma unroll
             for (int i = 0; i < QC; ++i)
-              s[n][h][i] = fmaf(step, x[v][2 * h + i], v == 0 ? so.y * qs[b][0][i] : fmaf(so.y, qs[b][v][i], s[n][h][i]));
+              s[b][n][h][i] = fmaf(step, x[v][2 * h + i], v == 0 ? so.y * qs[b][0][i] : fmaf(so.y, qs[b][v][i], s[b][n][h][i]));
           }
 #pragma unroll
           for (int i = 0; i < QC; ++i) {
-            s[n][h][i] = on[n][h] ? s[n][h][i] : -CUDART_INF_F;
-            top[i] = fmaxf(top[i], s[n][h][i]);
+            s[b][n][h][i] = on[n][h] ? s[b][n][h][i] : -CUDART_INF_F;
+            top[b][i] = fmaxf(top[b][i], s[b][n][h][i]);
           }
         }
       }
+    }
+    bool next_on[NP][2];
+    load_keys(next, next_on);  // under the softmax and the values' product
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
       bool more = false;
 #pragma unroll
-      for (int i = 0; i < QC; ++i) more = more || top[i] > m[b][i];
+      for (int i = 0; i < QC; ++i) more = more || top[b][i] > m[b][i];
       if (__any_sync(0xffffffffu, more)) {
 #pragma unroll
         for (int i = 0; i < QC; ++i) {
           // over the keys and, where the columns are shared, over the tiles
 #pragma unroll
-          for (int o = TP == 4 ? 1 : TP == 2 ? 2 : 4; o < 32; o <<= 1) top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
-          top[i] = fmaxf(top[i], m[b][i]);
-          const float keep = top[i] == -CUDART_INF_F ? 1.f : ex2(m[b][i] - top[i]);
-          m[b][i] = top[i];
+          for (int o = TP == 4 ? 1 : TP == 2 ? 2 : 4; o < 32; o <<= 1) top[b][i] = fmaxf(top[b][i], __shfl_xor_sync(0xffffffffu, top[b][i], o));
+          top[b][i] = fmaxf(top[b][i], m[b][i]);
+          const float keep = top[b][i] == -CUDART_INF_F ? 1.f : ex2(m[b][i] - top[b][i]);
+          m[b][i] = top[b][i];
           l[b][i] *= keep;
 #pragma unroll
           for (int v = 0; v < G; ++v) {
@@ -521,7 +570,7 @@ __device__ __forceinline__ void attend_tiles4(const PagedCache& c, const Attend&
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int i = 0; i < QC; ++i) {
-            w[h][i] = ex2(s[n][h][i] - z[i]);
+            w[h][i] = ex2(s[b][n][h][i] - z[i]);
             l[b][i] += w[h][i];
           }
 #pragma unroll
@@ -563,6 +612,11 @@ __device__ __forceinline__ void attend_tiles4(const PagedCache& c, const Attend&
         }
       }
     }
+    load_values(next);  // under the next step's scores
+#pragma unroll
+    for (int n = 0; n < NP; ++n)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) on[n][h] = next_on[n][h];
   }
   // shared columns are added up; the weights' part that belongs to no code is the same for all dims of a group
   auto over_tiles = [&](float x) {
@@ -606,7 +660,7 @@ __device__ __forceinline__ void attend_tiles_of(const PagedCache& c, const Atten
 template <typename T, int D, int NB, int Form>
 __global__ void __launch_bounds__(kStepThreads, step_ctas(D, NB, Form))
     step_kernel(PagedCache c, Attend a, SharedPrefix shared, StepSpace ws, int blocks, int min_tiles) {
-  constexpr int NT = step_tiles(D, Form);
+  constexpr int NT = step_tiles(D, Form), kUnitCost = unit_cost(Form);
   constexpr int NQ = 8 * NB;   // query rows of a unit
   constexpr int KC = D / 32, VC = D / 64;
   extern __shared__ int tiles_before[];  // [rows + 1]: tiles of a key head of the slots before
@@ -1046,7 +1100,7 @@ cudaError_t launch_step(const PagedCache& c, int dtype, const Attend& a, const S
   if (sms <= 0 || sms > kMaxSms) return cudaErrorInvalidValue;
   const size_t smem = 4 * (static_cast<size_t>(a.rows) + 1);
   const int grid = sms * step_ctas(c.head_dim, nb, form), shares = grid * kStepWarps;
-  const int min_tiles = kUnitCost + step_tiles(c.head_dim, form);
+  const int min_tiles = unit_cost(form) + step_tiles(c.head_dim, form);
   const int pairs = std::min(8 * nb, a.group) * c.head_dim / 2;
   auto go = [&](auto kernel, auto join) {
     if (smem > 40 * 1024) {
