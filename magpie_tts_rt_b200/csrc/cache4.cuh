@@ -95,34 +95,21 @@ struct Pair4 {
     const float step = unpack2<T>(bits).x;
     inverse = step >= 1.17549435e-38f ? __frcp_rn(step) : 0.f;
   }
-  // the codes of 8 values
+  // The codes of 8 values.  1.5 * 2^23 is added, which rounds to a whole number, half to even, and leaves the code in the
+  // lowest bits of 0x4b400000 + code; eight of them are put together by products, whose constant parts add up to one.
   __device__ __forceinline__ uint32_t codes(const uint4& x) const {
     const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    const float2 less = make_float2(-low, -low), by = make_float2(inverse, inverse), whole = make_float2(12582912.f, 12582912.f);
     uint32_t r = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float2 v = unpack2<T>(w[i]);
-      r |= code(v.x) << (4 * i) | code(v.y) << (4 * i + 16);
+      float2 v = mul2(add2(unpack2<T>(w[i]), less), by);
+      v = add2(make_float2(fminf(v.x, 15.f), fminf(v.y, 15.f)), whole);
+      r += __float_as_uint(v.x) * (1u << (4 * i)) + __float_as_uint(v.y) * (1u << (4 * i + 16));
     }
-    return r;
-  }
-  __device__ __forceinline__ uint32_t code(float x) const {
-    const float at = fminf(fmaxf(__fmul_rn(__fsub_rn(x, low), inverse), 0.f), 15.f);  // 0 for a NaN
-    return __float_as_uint(__fadd_rn(at, 12582912.f)) & 15u;  // 1.5 * 2^23: rounds to a whole number, half to even
+    return inverse == 0.f ? 0u : r - 0x4b400000u * 0x11111111u;  // (no step: the group is constant, or not finite)
   }
 };
-
-// The values of 8 codes, rounded to 16 bits.
-template <typename T>
-__device__ __forceinline__ uint4 values4(uint32_t codes, uint32_t pair) {
-  const float2 p = unpack2<T>(pair);
-  uint32_t r[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    r[i] = Half16<T>::pack(fmaf(static_cast<float>((codes >> (4 * i)) & 15u), p.x, p.y),
-                           fmaf(static_cast<float>((codes >> (4 * i + 16)) & 15u), p.x, p.y));
-  return make_uint4(r[0], r[1], r[2], r[3]);
-}
 
 // Codes of dims 2 I and 2 I + 1 of the eight in w, as 16 + code in 16 bits each:
 // the code goes into the upper mantissa bits of 16.0, so that it takes a shift and
@@ -158,6 +145,14 @@ __device__ __forceinline__ uint32_t value2<__half>(uint32_t c16, uint32_t step2,
   asm("{\n .reg .b32 c;\n add.rn.f16x2 c, %1, %4;\n fma.rn.f16x2 %0, c, %2, %3;\n}\n"
       : "=r"(r) : "r"(c16), "r"(step2), "r"(low2), "r"(0xcc00cc00u));
   return r;
+}
+
+// The values of 8 codes, rounded to 16 bits.
+template <typename T>
+__device__ __forceinline__ uint4 values4(uint32_t codes, uint32_t pair) {
+  const uint32_t step2 = __byte_perm(pair, 0, 0x1010), low2 = __byte_perm(pair, 0, 0x3232);
+  return make_uint4(value2<T>(codes2<T, 0>(codes), step2, low2), value2<T>(codes2<T, 1>(codes), step2, low2),
+                    value2<T>(codes2<T, 2>(codes), step2, low2), value2<T>(codes2<T, 3>(codes), step2, low2));
 }
 
 // Where a token's 8 dims from 8 * piece on, and the pair of its group, lie in its block.

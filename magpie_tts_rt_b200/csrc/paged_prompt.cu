@@ -425,34 +425,6 @@ __device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint32
       : "memory");
 }
 
-// Two f32 operations in one instruction.
-__device__ __forceinline__ uint64_t bits2(float2 v) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(v.x), "f"(v.y));
-  return r;
-}
-__device__ __forceinline__ float2 pair2(uint64_t v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(bits2(a)), "l"(bits2(b)), "l"(bits2(c)));
-  return pair2(d);
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits2(a)), "l"(bits2(b)));
-  return pair2(d);
-}
-
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits2(a)), "l"(bits2(b)));
-  return pair2(d);
-}
-
 // NaN if any of the three is.
 __device__ __forceinline__ float max_nan(float a, float b, float c) {
   float r;
@@ -550,13 +522,10 @@ struct Convert4 {
     for (int b = 0; b < DB; ++b) {
       const uint4 x = raw->codes[slot][b][lane];
       const uint32_t w[4] = {x.x, x.y, x.z, x.w}, p = raw->pair[slot][b][lane >> 1];
-      const uint32_t step2 = __byte_perm(p, 0, 0x1010), low2 = __byte_perm(p, 0, 0x3232);
       unsigned char* to = stage + b * (kKeys * 128) + row * 128;
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        *reinterpret_cast<uint4*>(to + 16 * ((4 * (lane & 1) + k) ^ (row & 7))) =
-            make_uint4(value2<T>(codes2<T, 0>(w[k]), step2, low2), value2<T>(codes2<T, 1>(w[k]), step2, low2),
-                       value2<T>(codes2<T, 2>(w[k]), step2, low2), value2<T>(codes2<T, 3>(w[k]), step2, low2));
+        *reinterpret_cast<uint4*>(to + 16 * ((4 * (lane & 1) + k) ^ (row & 7))) = values4<T>(w[k], p);
     }
   }
   // the rounded keys, and DB blocks on what that leaves

@@ -1,10 +1,10 @@
 // Rows into and out of the paged cache beside paged_cache.cu's 16-bit store:
 // store4 writes them in 4 bits, load reads them back.
 //
-// A token's head is held by head_dim / 16 lanes, 16 dims each as two 16-byte
-// pieces, so that a group's 64 dims lie in 4 lanes (head_dim 64: all of them) or
-// one piece of each of 8: minimum and maximum take two or three shuffles in
-// packed 16-bit pairs.  HBM bounds both kernels.
+// A token's head is held by head_dim / 16 lanes, 16 dims each (32 bytes, in one
+// load where the rows allow it), so that a group's 64 dims lie in 4 lanes: minimum and
+// maximum take two shuffles in packed 16-bit pairs.  HBM bounds both kernels as long
+// as instructions stay few: store4 has some 12 an element to spend.
 #include "cache4.cuh"
 
 namespace mtt {
@@ -15,38 +15,74 @@ constexpr int kRowsWarps = kRowsThreads / 32;
 
 struct RowsArgs {
   int layer, n_layers, rows, chunks;
+  bool wide;  // rows of k and v are 32-byte aligned
   uint16_t *k, *v;
   int64_t k_row, v_row, k_layer, v_layer;
   const int32_t* offsets;
 };
 
-// A warp's unit: part `chunk` of a row's (layer, keys or values, head) items.
+// A warp's unit: part `chunk` of a row's (layer, keys or values, head) items, a head
+// for each D / 16 lanes at a time.
 template <int D>
 struct RowUnit {
   static constexpr int L = D / 16, H = 32 / L;  // lanes of a head, heads of a warp
-  int row, i0, i1;
+  int row, i, end;                              // the lane's item
+  int block, head;                              // item i: 2 * layer + (keys or values), and head
+  int blocks_on, heads_on;                      // from an item to the lane's next
   __device__ __forceinline__ RowUnit(const PagedCache& c, const RowsArgs& in) {
     const int64_t unit = static_cast<int64_t>(blockIdx.x) * kRowsWarps + (threadIdx.x >> 5);
     row = static_cast<int>(unit / in.chunks);
     const int chunk = static_cast<int>(unit % in.chunks);
     const int items = 2 * in.n_layers * c.kv_heads, each = ((items + in.chunks - 1) / in.chunks + H - 1) / H * H;
-    i0 = chunk * each;
-    i1 = min(items, i0 + each);
+    i = chunk * each + (threadIdx.x & 31) / L;
+    end = min(items, (chunk + 1) * each);
+    block = i / c.kv_heads;
+    head = i - block * c.kv_heads;
+    blocks_on = H / c.kv_heads;
+    heads_on = H - blocks_on * c.kv_heads;
+  }
+  __device__ __forceinline__ bool on() const { return i < end; }
+  __device__ __forceinline__ void next(const PagedCache& c) {
+    i += H;
+    block += blocks_on;
+    head += heads_on;
+    if (head >= c.kv_heads) {
+      head -= c.kv_heads;
+      ++block;
+    }
+  }
+  // the lane's 16 dims of the item in k or v
+  __device__ __forceinline__ uint16_t* at(const RowsArgs& in) const {
+    const int layer = block >> 1, t = (threadIdx.x & 31) % L;
+    return ((block & 1) != 0 ? in.v + row * in.v_row + layer * in.v_layer : in.k + row * in.k_row + layer * in.k_layer) +
+           (head * D + 16 * t);
+  }
+  __device__ __forceinline__ unsigned char* place(const PagedCache& c, const RowsArgs& in, int page) const {
+    return reinterpret_cast<unsigned char*>(c.pool + c.block(page, in.layer + (block >> 1), block & 1));
   }
 };
 
-// An item's first element in k or v, and its place in the cache.
-struct RowItem {
-  int kv, layer, head;
-  uint16_t* at;
-  __device__ __forceinline__ RowItem(const PagedCache& c, const RowsArgs& in, int row, int item) {
-    const int b = item / c.kv_heads;
-    head = item - b * c.kv_heads;
-    kv = b & 1;
-    layer = b >> 1;
-    at = (kv ? in.v + row * in.v_row + layer * in.v_layer : in.k + row * in.k_row + layer * in.k_layer) +
-         static_cast<int64_t>(head) * c.head_dim;
-    layer += in.layer;
+struct Piece {
+  uint4 a, b;  // 16 values
+  __device__ __forceinline__ void load(const uint16_t* p, bool wide) {
+    if (wide) {
+      asm volatile("ld.global.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                   : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w), "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w)
+                   : "l"(p));
+    } else {
+      a = __ldcs(reinterpret_cast<const uint4*>(p));
+      b = __ldcs(reinterpret_cast<const uint4*>(p) + 1);
+    }
+  }
+  __device__ __forceinline__ void store(uint16_t* p, bool wide) const {
+    if (wide) {
+      asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w),
+                   "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w)
+                   : "memory");
+    } else {
+      __stcs(reinterpret_cast<uint4*>(p), a);
+      __stcs(reinterpret_cast<uint4*>(p) + 1, b);
+    }
   }
 };
 
@@ -54,9 +90,11 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kRowsThreads) store4_kernel(PagedCache c, RowsArgs in) {
   using U = RowUnit<D>;
   take_turn();
-  const U u(c, in);
+  U u(c, in);
   if (u.row >= in.rows) return;
   const int lane = threadIdx.x & 31, t = lane % U::L;
+  Piece next{};
+  if (u.on()) next.load(u.at(in), in.wide);
   const RowPlace at(c, in.offsets, in.rows, u.row);
   if (at.pos < 0 && at.unfit == 0) return;
   if (at.unfit != 2 && c.refused != nullptr && c.refused[at.slot] != 0) return;  // its last tokens are not the rows'
@@ -69,34 +107,21 @@ __global__ void __launch_bounds__(kRowsThreads) store4_kernel(PagedCache c, Rows
     if (lane == 0 && c.status != nullptr) c.status[at.slot] = bad;
     return;
   }
-  const int in_page = at.pos & (c.page_size - 1);
-  for (int i0 = u.i0; i0 < u.i1; i0 += U::H) {
-    const int i = i0 + lane / U::L;
-    const bool on = i < u.i1;
-    const RowItem item(c, in, u.row, on ? i : i0);
-    const uint4 a = __ldcs(reinterpret_cast<const uint4*>(item.at) + t);
-    const uint4 b = __ldcs(reinterpret_cast<const uint4*>(item.at) + t + U::L);
-    unsigned char* block = block4(c, page, item.layer, item.kv, item.head);
-    Extent4<T> e = Extent4<T>::of(a);
-    if constexpr (D == 64) {
-      e.take(b);
-      e.join(U::L);
-      const Pair4<T> p(e);
-      if (on) {
-        *codes_at(c, block, in_page, t) = p.codes(a);
-        *codes_at(c, block, in_page, t + U::L) = p.codes(b);
-        if (t == 0) *pair_at(c, block, in_page, 0) = p.bits;
-      }
-    } else {
-      Extent4<T> f = Extent4<T>::of(b);
-      e.join(U::L);
-      f.join(U::L);
-      const Pair4<T> p(e), q(f);
-      if (on) {
-        *codes_at(c, block, in_page, t) = p.codes(a);
-        *codes_at(c, block, in_page, t + U::L) = q.codes(b);
-        if (t < 2) *pair_at(c, block, in_page, t) = t == 0 ? p.bits : q.bits;
-      }
+  const int in_page = at.pos & (c.page_size - 1), head_bytes = block4_bytes(c);
+  const int codes = in_page * (D / 2) + 8 * t, pair = block4_codes(c) + (in_page * (D / kGroup4) + t / 4) * 4;
+  while (__any_sync(0xffffffffu, u.on())) {
+    const Piece x = next;
+    const bool on = u.on();
+    unsigned char* to = u.place(c, in, page) + u.head * head_bytes;
+    u.next(c);
+    if (u.on()) next.load(u.at(in), in.wide);
+    Extent4<T> e = Extent4<T>::of(x.a);
+    e.take(x.b);
+    e.join(4);
+    const Pair4<T> p(e);
+    if (on) {
+      *reinterpret_cast<uint2*>(to + codes) = make_uint2(p.codes(x.a), p.codes(x.b));
+      if (t % 4 == 0) *reinterpret_cast<uint32_t*>(to + pair) = p.bits;
     }
   }
 }
@@ -105,30 +130,47 @@ template <typename T, int D, int Bits>
 __global__ void __launch_bounds__(kRowsThreads) load_kernel(PagedCache c, RowsArgs in) {
   using U = RowUnit<D>;
   take_turn();
-  const U u(c, in);
+  U u(c, in);
   if (u.row >= in.rows) return;
-  const int lane = threadIdx.x & 31, t = lane % U::L;
+  const int t = (threadIdx.x & 31) % U::L;
   const RowPlace at(c, in.offsets, in.rows, u.row);
   const int page = at.pos < 0 ? -1 : c.table[static_cast<int64_t>(at.slot) * c.table_pages + (at.pos >> c.page_shift)];
   const bool there = c.is_page(page);
   const int in_page = at.pos & (c.page_size - 1);
-  for (int i = u.i0 + lane / U::L; i < u.i1; i += U::H) {
-    const RowItem item(c, in, u.row, i);
-    uint4 a = make_uint4(0, 0, 0, 0), b = a;
-    if (there) {
-      if constexpr (Bits == 4) {
-        unsigned char* block = block4(c, page, item.layer, item.kv, item.head);
-        a = values4<T>(*codes_at(c, block, in_page, t), *pair_at(c, block, in_page, t / 8));
-        b = values4<T>(*codes_at(c, block, in_page, t + U::L), *pair_at(c, block, in_page, (t + U::L) / 8));
-      } else {
-        const uint16_t* src = c.pool + c.block(page, item.layer, item.kv) +
-                              (static_cast<int64_t>(item.head) * c.page_size + in_page) * D;
-        a = *(reinterpret_cast<const uint4*>(src) + t);
-        b = *(reinterpret_cast<const uint4*>(src) + t + U::L);
-      }
+  if constexpr (Bits == 4) {
+    const int head_bytes = block4_bytes(c);
+    const int codes = in_page * (D / 2) + 8 * t, pair = block4_codes(c) + (in_page * (D / kGroup4) + t / 4) * 4;
+    uint2 w = make_uint2(0, 0);
+    uint32_t p = 0;
+    auto load = [&] {
+      if (!there || !u.on()) return;
+      const unsigned char* from = u.place(c, in, page) + u.head * head_bytes;
+      w = *reinterpret_cast<const uint2*>(from + codes);
+      p = *reinterpret_cast<const uint32_t*>(from + pair);
+    };
+    load();
+    while (u.on()) {
+      const Piece x{values4<T>(w.x, p), values4<T>(w.y, p)};
+      uint16_t* to = u.at(in);
+      u.next(c);
+      load();
+      x.store(to, in.wide);
     }
-    __stcs(reinterpret_cast<uint4*>(item.at) + t, a);
-    __stcs(reinterpret_cast<uint4*>(item.at) + t + U::L, b);
+  } else {
+    Piece next{};
+    auto load = [&] {
+      if (!there || !u.on()) return;
+      next.load(reinterpret_cast<const uint16_t*>(u.place(c, in, page)) +
+                    (static_cast<int64_t>(u.head) * c.page_size + in_page) * D + 16 * t, true);
+    };
+    load();
+    while (u.on()) {
+      const Piece x = next;
+      uint16_t* to = u.at(in);
+      u.next(c);
+      load();
+      x.store(to, in.wide);
+    }
   }
 }
 
@@ -142,7 +184,10 @@ cudaError_t for_type_and_dim(const PagedCache& c, Run run) {
 }
 
 RowsArgs rows_args(const PagedCache& c, const mtt_b200_cache_rows_t& r) {
-  RowsArgs in{r.layer, r.n_layers, r.rows, 1, static_cast<uint16_t*>(const_cast<void*>(r.k)),
+  const auto aligned32 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 31u) == 0; };
+  const bool wide = aligned32(r.k) && aligned32(r.v) &&
+                    (r.k_row_stride | r.v_row_stride | r.k_layer_stride | r.v_layer_stride) % 16 == 0;
+  RowsArgs in{r.layer, r.n_layers, r.rows, 1, wide, static_cast<uint16_t*>(const_cast<void*>(r.k)),
               static_cast<uint16_t*>(const_cast<void*>(r.v)), r.k_row_stride, r.v_row_stride, r.k_layer_stride,
               r.v_layer_stride, r.offsets};
   // few rows: a row's items are dealt to several warps

@@ -5,10 +5,15 @@
 //
 // HBM bounds it: every element is read and written once.  A head is held by
 // head_dim / 16 lanes as two 16-byte pieces each, chosen so that both dims of
-// every pair lie in the same lane and a lane has the same 8 pairs in every head:
-// a warp, which takes heads of one row, finds its row's cosines and sines once
-// (each lane a pair or two, exchanged through shared memory) and keeps them in
-// registers, as it does the weights.  The mean takes two or three shuffles.
+// every pair lie in the same lane and a lane has the same 8 pairs in every head.  A
+// warp takes a row's heads, a few at a time, and finds the row's cosines and sines
+// once (each lane a pair or two, exchanged through shared memory); a lane keeps
+// their products with the weights, so that norm and rotation are two products an
+// element, in pairs of f32, and a factor for the head.  The mean takes two or three
+// shuffles.  What hides the loads is warps: 32 an SM, for which a lane's coefficients
+// lie in shared memory (in registers, 16 warps with four passes' loads in flight
+// each: 45 us instead of 33 for 8192 rows of 32 and 8 heads of 128, which is 5.1
+// TB/s; their prompts' append, 6,600 rows, 41 us).
 //
 // The angle is position x turns in 64 bits, of which only the part past whole
 // turns is kept: exact to 2^-22 of a turn at positions up to 2^31, where a 32-bit
@@ -20,9 +25,9 @@
 namespace mtt {
 namespace {
 
-constexpr int kRotThreads = 256;
+constexpr int kRotThreads = 128;
 constexpr int kRotWarps = kRotThreads / 32;
-constexpr int kRotAhead = 4;  // passes whose loads are in flight together
+constexpr int kRotAhead = 1;  // passes whose loads are on their way while another is turned
 
 enum class Into { kRows, kCache16, kCache4 };
 
@@ -37,10 +42,56 @@ struct RotArgs {
   const int32_t *positions, *offsets;
 };
 
-template <typename T, int D, Into To>
-__global__ void __launch_bounds__(kRotThreads) rotate_kernel(PagedCache c, RotArgs in) {
+// A lane's share of a head is 16 values, 8 pairs y that lie beside each other, and
+// what turns them: z = y own + other (another pair).  Interleaved, y is a pair of the
+// rotation and the other one itself, swapped,
+//   own = (w0 c, w1 c),  other = (-w1 s, w0 s);
+// else the lane's first piece (pairs 0 to 3) is turned against the second,
+//   own = w c,  other = -+ its w s.
+// They lie in shared memory, for queries and for keys: in registers they would halve
+// the number of warps.  [own 0-1 .. own 6-7, other 0-1 .. other 6-7][lane of a head]
+template <int L>
+using Coefficients = float4[8][L];
+
+template <bool Interleaved, int L>
+__device__ __forceinline__ void make_coefficients(Coefficients<L>& to, int t, const float2* turn, const float* weight, int pa, int pb) {
+  float2 own[8], other[8];
+  float w[16];
+#pragma unroll
+  for (int i = 0; i < 16; i += 4) {
+    const float4 x = weight == nullptr ? make_float4(1.f, 1.f, 1.f, 1.f)
+                                       : *reinterpret_cast<const float4*>(weight + 8 * (i < 8 ? pa : pb) + i % 8);
+    w[i] = x.x;
+    w[i + 1] = x.y;
+    w[i + 2] = x.z;
+    w[i + 3] = x.w;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float2 v = turn[i];  // cosine, sine of the lane's pair i
+    if constexpr (Interleaved) {
+      own[i] = make_float2(w[2 * i] * v.x, w[2 * i + 1] * v.x);
+      other[i] = make_float2(-w[2 * i + 1] * v.y, w[2 * i] * v.y);
+    } else {
+      float2 &a = own[i / 2], &b = own[4 + i / 2], &c = other[i / 2], &d = other[4 + i / 2];
+      (i % 2 ? a.y : a.x) = w[i] * v.x;
+      (i % 2 ? b.y : b.x) = w[8 + i] * v.x;
+      (i % 2 ? c.y : c.x) = -w[8 + i] * v.y;
+      (i % 2 ? d.y : d.x) = w[i] * v.y;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    to[i][t] = make_float4(own[2 * i].x, own[2 * i].y, own[2 * i + 1].x, own[2 * i + 1].y);
+    to[4 + i][t] = make_float4(other[2 * i].x, other[2 * i].y, other[2 * i + 1].x, other[2 * i + 1].y);
+  }
+}
+
+template <typename T, int D, Into To, bool Interleaved>
+__global__ void __launch_bounds__(kRotThreads, To == Into::kCache4 ? 4 : 8) rotate_kernel(PagedCache c, RotArgs in) {
   constexpr int L = D / 16, H = 32 / L;  // lanes of a head, heads of a pass
   __shared__ float2 turn[kRotWarps][D / 2];
+  __shared__ Coefficients<L> coefficients[kRotWarps][2];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = lane % L, j = lane / L;
   const int64_t unit = static_cast<int64_t>(blockIdx.x) * kRotWarps + warp;
   const int row = static_cast<int>(unit / in.chunks), chunk = static_cast<int>(unit % in.chunks);
@@ -52,25 +103,29 @@ __global__ void __launch_bounds__(kRotThreads) rotate_kernel(PagedCache c, RotAr
   const int p0 = static_cast<int>(static_cast<int64_t>(passes) * chunk / in.chunks);
   const int p1 = static_cast<int>(static_cast<int64_t>(passes) * (chunk + 1) / in.chunks);
   // the lane's pieces of a query or key head
-  const bool turned = t < in.rotary_dim / 16;
-  const int pa = turned && !in.interleaved ? t : 2 * t;
-  const int pb = turned && !in.interleaved ? t + in.rotary_dim / 16 : 2 * t + 1;
+  const bool turned = t < in.rotary_dim / 16, all_turned = in.rotary_dim == D;
+  const int pa = turned && !Interleaved ? t : 2 * t;
+  const int pb = turned && !Interleaved ? t + in.rotary_dim / 16 : 2 * t + 1;
+  const uint16_t* q_src = in.q + row * in.q_row + j * D + 8 * pa;
+  const uint16_t* k_src = in.k + row * in.k_row + j * D + 8 * pa;
+  const uint16_t* v_src = in.v + row * in.v_row + j * D + 8 * t;
+  const int second = 8 * (pb - pa);  // from the first piece to the other
 
   uint4 x[kRotAhead][2];
   auto load = [&](int n, int p) {
-    const bool is_q = p < qp, is_k = !is_q && p < qp + kp;
-    const int h = (is_q ? p : is_k ? p - qp : p - qp - kp) * H + j;
-    if (p >= p1 || h >= (is_q ? in.q_heads : in.kv_heads)) {
-      x[n][0] = x[n][1] = make_uint4(0, 0, 0, 0);
-      return;
-    }
-    const uint16_t* src = is_q ? in.q + row * in.q_row : is_k ? in.k + row * in.k_row : in.v + row * in.v_row;
-    src += static_cast<int64_t>(h) * D;
-    x[n][0] = *(reinterpret_cast<const uint4*>(src) + (is_q || is_k ? pa : t));
-    x[n][1] = *(reinterpret_cast<const uint4*>(src) + (is_q || is_k ? pb : t + L));
+    if (p >= p1) return;
+    const bool is_v = To != Into::kRows && p >= qp + kp, is_q = p < qp;
+    const int h = (is_q ? p : is_v ? p - qp - kp : p - qp) * H;
+    if (h + j >= (is_q ? in.q_heads : in.kv_heads)) return;
+    const uint16_t* src = (is_q ? q_src : is_v ? v_src : k_src) + h * D;
+    x[n][0] = *reinterpret_cast<const uint4*>(src);
+    x[n][1] = *reinterpret_cast<const uint4*>(src + (is_v ? 8 * L : second));
   };
 #pragma unroll
-  for (int n = 0; n < kRotAhead; ++n) load(n, p0 + n);
+  for (int n = 0; n < kRotAhead; ++n) {
+    x[n][0] = x[n][1] = make_uint4(0, 0, 0, 0);
+    load(n, p0 + n);
+  }
 
   // where the row goes
   int page = -1, in_page = 0, position = 0;
@@ -93,145 +148,132 @@ __global__ void __launch_bounds__(kRotThreads) rotate_kernel(PagedCache c, RotAr
     }
     if (bad != 0 && chunk == 0 && lane == 0 && c.status != nullptr) c.status[at.slot] = bad;
   }
-  for (int i = lane; i < in.rotary_dim / 2; i += 32) {
-    const double turns = position * in.turns[i];
-    float s, cs;
-    sincospif(2.f * static_cast<float>(turns - rint(turns)), &s, &cs);
-    turn[warp][i] = make_float2(cs, s);
+#pragma unroll
+  for (int k = 0; k < D / 64; ++k) {
+    const int i = lane + 32 * k;  // pairs past rotary_dim: no turn
+    const double turns = i < in.rotary_dim / 2 ? position * in.turns[i] : 0.;
+    float sn, cs;
+    // within half a turn the fast functions are right to 2^-21, where the result is rounded to 2^-12 at best
+    __sincosf(6.283185307f * static_cast<float>(turns - rint(turns)), &sn, &cs);
+    turn[warp][i] = make_float2(cs, sn);
   }
   __syncwarp();
-  float cs[8], sn[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float2 v = turned ? turn[warp][8 * t + i] : make_float2(1.f, 0.f);
-    cs[i] = v.x;
-    sn[i] = v.y;
-  }
 
-  float w[16];
-  const float* weight = nullptr;
+  // the lanes of the pass's first head for the queries, of its second for the keys
+  if (j < 2) make_coefficients<Interleaved, L>(coefficients[warp][j], t, &turn[warp][8 * t], j == 0 ? in.q_weight : in.k_weight, pa, pb);
+  __syncwarp();
+  // head h: what becomes of it, in 16 bits
+  auto turn_head = [&](bool is_q, uint4& a, uint4& b) {
+    const float* weight = is_q ? in.q_weight : in.k_weight;
+    const Coefficients<L>& with = coefficients[warp][is_q ? 0 : 1];
+    float2 y[8];
+    {
+      const uint32_t u[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = unpack2<T>(u[i]);
+    }
+    float inv = 1.f;  // of the norm
+    if (weight != nullptr) {
+      float2 sums = mul2(y[0], y[0]);
+#pragma unroll
+      for (int i = 1; i < 8; ++i) sums = fma2(y[i], y[i], sums);
+      float sum = sums.x + sums.y;
+#pragma unroll
+      for (int o = 1; o < L; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      inv = rsqrtf(sum * (1.f / D) + in.eps);
+    }
+    uint32_t z[8];
+    const float2 inv2 = make_float2(inv, inv);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float4 own = with[i][t], other = with[4 + i][t];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const float2 mine = y[2 * i + k], far = Interleaved ? make_float2(mine.y, mine.x) : y[(2 * i + k + 4) % 8];
+        const float2 kept = mul2(mine, k == 0 ? make_float2(own.x, own.y) : make_float2(own.z, own.w));
+        float2 v = fma2(far, k == 0 ? make_float2(other.x, other.y) : make_float2(other.z, other.w), kept);
+        // a dim past rotary_dim is not turned: not by 0 either, which an infinite neighbour would make a NaN
+        if (!all_turned) v = turned ? v : kept;
+        if (weight != nullptr) v = mul2(v, inv2);
+        z[2 * i + k] = Half16<T>::pack(v.x, v.y);
+      }
+    }
+    if (turned || weight != nullptr) {  // else it keeps its bits
+      a = make_uint4(z[0], z[1], z[2], z[3]);
+      b = make_uint4(z[4], z[5], z[6], z[7]);
+    }
+  };
+  // keys or values of the row's token into the cache
+  auto put = [&](int kv, int h, int qa, int qb, const uint4& a, const uint4& b, bool on) {
+    if constexpr (To == Into::kCache16) {
+      if (on) {
+        uint4* out = reinterpret_cast<uint4*>(c.pool + c.block(page, in.layer, kv) +
+                                              (static_cast<int64_t>(h) * c.page_size + in_page) * D);
+        out[qa] = a;
+        out[qb] = b;
+      }
+    } else {
+      unsigned char* block = block4(c, page, in.layer, kv, on ? h : 0);
+      if constexpr (D == 64) {
+        Extent4<T> e = Extent4<T>::of(a);
+        e.take(b);
+        e.join(L);
+        const Pair4<T> g(e);
+        if (on) {
+          *codes_at(c, block, in_page, qa) = g.codes(a);
+          *codes_at(c, block, in_page, qb) = g.codes(b);
+          if (t == 0) *pair_at(c, block, in_page, 0) = g.bits;
+        }
+      } else {
+        // either piece may belong to either group: where a lane has none, an extent that changes nothing
+        const Extent4<T> ea = Extent4<T>::of(a), eb = Extent4<T>::of(b);
+        constexpr uint32_t kMost = std::is_same_v<T, __half> ? 0x7c007c00u : 0x7f807f80u;
+        const Extent4<T> none{kMost, kMost | 0x80008000u};
+        Extent4<T> e0 = qa < 8 ? ea : none, e1 = qa < 8 ? none : ea;
+        if (qb < 8) {
+          e0 = {min2<T>(e0.low, eb.low), max2<T>(e0.high, eb.high)};
+        } else {
+          e1 = {min2<T>(e1.low, eb.low), max2<T>(e1.high, eb.high)};
+        }
+        e0.join(L);
+        e1.join(L);
+        const Pair4<T> g0(e0), g1(e1);
+        if (on) {
+          *codes_at(c, block, in_page, qa) = (qa < 8 ? g0 : g1).codes(a);
+          *codes_at(c, block, in_page, qb) = (qb < 8 ? g0 : g1).codes(b);
+          if (t < 2) *pair_at(c, block, in_page, t) = t == 0 ? g0.bits : g1.bits;
+        }
+      }
+    }
+  };
   for (int base = p0; base < p1; base += kRotAhead) {
 #pragma unroll
     for (int n = 0; n < kRotAhead; ++n) {
       const int p = base + n;
       if (p >= p1) break;
-      const bool is_q = p < qp, is_k = !is_q && p < qp + kp;
-      const int h = (is_q ? p : is_k ? p - qp : p - qp - kp) * H + j;
-      const bool on = h < (is_q ? in.q_heads : in.kv_heads);
       uint4 a = x[n][0], b = x[n][1];
-      if (is_q || is_k) {
-        const float* mine = is_q ? in.q_weight : in.k_weight;
-        float y[16];
-        {
-          const uint32_t u[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float2 v = unpack2<T>(u[i]);
-            y[2 * i] = v.x;
-            y[2 * i + 1] = v.y;
-          }
-        }
-        if (mine != nullptr) {
-          if (mine != weight) {  // once for the queries, once for the keys
-            weight = mine;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              *reinterpret_cast<float4*>(w + 4 * i) = *(reinterpret_cast<const float4*>(mine + 8 * pa) + i);
-              *reinterpret_cast<float4*>(w + 8 + 4 * i) = *(reinterpret_cast<const float4*>(mine + 8 * pb) + i);
-            }
-          }
-          float sum = 0.f;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) sum = fmaf(y[i], y[i], sum);
-#pragma unroll
-          for (int o = 1; o < L; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-          const float inv = rsqrtf(sum * (1.f / D) + in.eps);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) y[i] = y[i] * inv * w[i];
-        }
-        float z[16];
-        if (in.interleaved) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            z[2 * i] = fmaf(y[2 * i], cs[i], -y[2 * i + 1] * sn[i]);
-            z[2 * i + 1] = fmaf(y[2 * i + 1], cs[i], y[2 * i] * sn[i]);
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            z[i] = fmaf(y[i], cs[i], -y[8 + i] * sn[i]);
-            z[8 + i] = fmaf(y[8 + i], cs[i], y[i] * sn[i]);
-          }
-        }
-        // a dim past rotary_dim is not turned: not by 0 either, which an infinite neighbour would make a NaN
-#pragma unroll
-        for (int i = 0; i < 16; ++i) z[i] = turned ? z[i] : y[i];
-        if (turned || mine != nullptr) {  // else it keeps its bits
-          a = make_uint4(Half16<T>::pack(z[0], z[1]), Half16<T>::pack(z[2], z[3]), Half16<T>::pack(z[4], z[5]),
-                         Half16<T>::pack(z[6], z[7]));
-          b = make_uint4(Half16<T>::pack(z[8], z[9]), Half16<T>::pack(z[10], z[11]), Half16<T>::pack(z[12], z[13]),
-                         Half16<T>::pack(z[14], z[15]));
-        }
+      load(n, p + kRotAhead);
+      if (To != Into::kRows && p >= qp + kp) {
+        const int h = (p - qp - kp) * H + j;
+        if (page >= 0) put(1, h, t, t + L, a, b, h < in.kv_heads);
+        continue;
       }
-      if (is_q) {
+      const bool is_q = p < qp;
+      const int h = (is_q ? p : p - qp) * H + j;
+      const bool on = h < (is_q ? in.q_heads : in.kv_heads);
+      turn_head(is_q, a, b);
+      if (is_q || To == Into::kRows) {
         if (!known) a = b = make_uint4(0, 0, 0, 0);
         if (on) {
-          uint4* out = reinterpret_cast<uint4*>(in.q_out + row * in.q_out_row + static_cast<int64_t>(h) * D);
-          out[pa] = a;
-          out[pb] = b;
-        }
-      } else if constexpr (To == Into::kRows) {
-        if (on) {
-          uint4* out = reinterpret_cast<uint4*>(in.k_out + row * in.k_out_row + static_cast<int64_t>(h) * D);
+          uint4* out = reinterpret_cast<uint4*>((is_q ? in.q_out + row * in.q_out_row : in.k_out + row * in.k_out_row) +
+                                                static_cast<int64_t>(h) * D);
           out[pa] = a;
           out[pb] = b;
         }
       } else if (page >= 0) {
-        const int qa = is_k ? pa : t, qb = is_k ? pb : t + L;  // the pieces' numbers
-        if constexpr (To == Into::kCache16) {
-          if (on) {
-            uint4* out = reinterpret_cast<uint4*>(c.pool + c.block(page, in.layer, is_k ? 0 : 1) +
-                                                  (static_cast<int64_t>(h) * c.page_size + in_page) * D);
-            out[qa] = a;
-            out[qb] = b;
-          }
-        } else {
-          unsigned char* block = block4(c, page, in.layer, is_k ? 0 : 1, on ? h : 0);
-          if constexpr (D == 64) {
-            Extent4<T> e = Extent4<T>::of(a);
-            e.take(b);
-            e.join(L);
-            const Pair4<T> g(e);
-            if (on) {
-              *codes_at(c, block, in_page, qa) = g.codes(a);
-              *codes_at(c, block, in_page, qb) = g.codes(b);
-              if (t == 0) *pair_at(c, block, in_page, 0) = g.bits;
-            }
-          } else {
-            // either piece may belong to either group: where a lane has none, an extent that changes nothing
-            const Extent4<T> ea = Extent4<T>::of(a), eb = Extent4<T>::of(b);
-            constexpr uint32_t kMost = std::is_same_v<T, __half> ? 0x7c007c00u : 0x7f807f80u;
-            const Extent4<T> none{kMost, kMost | 0x80008000u};
-            Extent4<T> e0 = qa < 8 ? ea : none, e1 = qa < 8 ? none : ea;
-            if (qb < 8) {
-              e0 = {min2<T>(e0.low, eb.low), max2<T>(e0.high, eb.high)};
-            } else {
-              e1 = {min2<T>(e1.low, eb.low), max2<T>(e1.high, eb.high)};
-            }
-            e0.join(L);
-            e1.join(L);
-            const Pair4<T> g0(e0), g1(e1);
-            if (on) {
-              *codes_at(c, block, in_page, qa) = (qa < 8 ? g0 : g1).codes(a);
-              *codes_at(c, block, in_page, qb) = (qb < 8 ? g0 : g1).codes(b);
-              if (t < 2) *pair_at(c, block, in_page, t) = t == 0 ? g0.bits : g1.bits;
-            }
-          }
-        }
+        put(0, h, pa, pb, a, b, on);
       }
     }
-#pragma unroll
-    for (int n = 0; n < kRotAhead; ++n) load(n, base + kRotAhead + n);
   }
 }
 
@@ -266,10 +308,14 @@ int run(const PagedCache& c, const mtt_b200_rotation_t& rot, const mtt_b200_rota
   auto go = [&](auto type, auto dim) {
     using T = decltype(type);
     constexpr int D = decltype(dim)::value;
-    const auto kernel = to == Into::kRows      ? rotate_kernel<T, D, Into::kRows>
-                        : to == Into::kCache16 ? rotate_kernel<T, D, Into::kCache16>
-                                               : rotate_kernel<T, D, Into::kCache4>;
-    return launch_serialized(kernel, grid, dim3(kRotThreads), 0, stream, c, in);
+    auto kernel = [&](auto interleaved) {
+      constexpr bool I = decltype(interleaved)::value;
+      return to == Into::kRows      ? rotate_kernel<T, D, Into::kRows, I>
+             : to == Into::kCache16 ? rotate_kernel<T, D, Into::kCache16, I>
+                                    : rotate_kernel<T, D, Into::kCache4, I>;
+    };
+    return launch_serialized(in.interleaved != 0 ? kernel(std::true_type{}) : kernel(std::false_type{}), grid, dim3(kRotThreads),
+                             0, stream, c, in);
   };
   auto pick = [&](auto type) {
     return rot.head_dim == 64 ? go(type, std::integral_constant<int, 64>{}) : go(type, std::integral_constant<int, 128>{});
