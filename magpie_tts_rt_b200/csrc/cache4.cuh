@@ -90,10 +90,18 @@ struct Pair4 {
     const float high = unpack2<T>(max2<T>(e.high, e.high >> 16 | e.high << 16)).x;
     const float spread = __fsub_rn(high, low);
     // not finite: the whole group reads as NaN
-    const float wide = spread <= 3.402823466e38f ? __fdiv_rn(spread, 15.f) : CUDART_NAN_F;
+    const float wide = spread <= 3.402823466e38f ? fifteenth(spread) : CUDART_NAN_F;
     bits = Half16<T>::pack(wide, low);
     const float step = unpack2<T>(bits).x;
     inverse = step >= 1.17549435e-38f ? __frcp_rn(step) : 0.f;
+  }
+  // x / 15 rounded to nearest: the product with the rounded reciprocal, and one step with what is left (Markstein 1990);
+  // numbers so small that what is left could be lost are divided
+  static __device__ __forceinline__ float fifteenth(float x) {
+    constexpr float kBy = 1.f / 15.f;
+    if (x < 1e-25f) return __fdiv_rn(x, 15.f);
+    const float q = x * kBy;
+    return fmaf(fmaf(-15.f, q, x), kBy, q);
   }
   // The codes of 8 values.  1.5 * 2^23 is added, which rounds to a whole number, half to even, and leaves the code in the
   // lowest bits of 0x4b400000 + code; eight of them are put together by products, whose constant parts add up to one.

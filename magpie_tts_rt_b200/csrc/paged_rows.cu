@@ -51,14 +51,13 @@ struct RowUnit {
       ++block;
     }
   }
-  // the lane's 16 dims of the item in k or v
-  __device__ __forceinline__ uint16_t* at(const RowsArgs& in) const {
-    const int layer = block >> 1, t = (threadIdx.x & 31) % L;
-    return ((block & 1) != 0 ? in.v + row * in.v_row + layer * in.v_layer : in.k + row * in.k_row + layer * in.k_layer) +
-           (head * D + 16 * t);
+  // the lane's 16 dims of the item in k or v (`k`, `v`: those of the row's first head and layer)
+  __device__ __forceinline__ uint16_t* at(uint16_t* k, uint16_t* v, const RowsArgs& in) const {
+    return ((block & 1) != 0 ? v + (block >> 1) * in.v_layer : k + (block >> 1) * in.k_layer) + head * D;
   }
-  __device__ __forceinline__ unsigned char* place(const PagedCache& c, const RowsArgs& in, int page) const {
-    return reinterpret_cast<unsigned char*>(c.pool + c.block(page, in.layer + (block >> 1), block & 1));
+  // the item's keys or values in its page (`first`: those of the call's first layer), all heads
+  __device__ __forceinline__ unsigned char* place(const PagedCache& c, unsigned char* first) const {
+    return first + static_cast<uint64_t>(static_cast<uint32_t>(block)) * static_cast<uint32_t>(2 * c.kv_elems);
   }
 };
 
@@ -93,8 +92,9 @@ __global__ void __launch_bounds__(kRowsThreads) store4_kernel(PagedCache c, Rows
   U u(c, in);
   if (u.row >= in.rows) return;
   const int lane = threadIdx.x & 31, t = lane % U::L;
+  uint16_t *k = in.k + u.row * in.k_row + 16 * t, *v = in.v + u.row * in.v_row + 16 * t;
   Piece next{};
-  if (u.on()) next.load(u.at(in), in.wide);
+  if (u.on()) next.load(u.at(k, v, in), in.wide);
   const RowPlace at(c, in.offsets, in.rows, u.row);
   if (at.pos < 0 && at.unfit == 0) return;
   if (at.unfit != 2 && c.refused != nullptr && c.refused[at.slot] != 0) return;  // its last tokens are not the rows'
@@ -109,12 +109,13 @@ __global__ void __launch_bounds__(kRowsThreads) store4_kernel(PagedCache c, Rows
   }
   const int in_page = at.pos & (c.page_size - 1), head_bytes = block4_bytes(c);
   const int codes = in_page * (D / 2) + 8 * t, pair = block4_codes(c) + (in_page * (D / kGroup4) + t / 4) * 4;
+  unsigned char* first = reinterpret_cast<unsigned char*>(c.pool + c.block(page, in.layer, 0));
   while (__any_sync(0xffffffffu, u.on())) {
     const Piece x = next;
     const bool on = u.on();
-    unsigned char* to = u.place(c, in, page) + u.head * head_bytes;
+    unsigned char* to = u.place(c, first) + u.head * head_bytes;
     u.next(c);
-    if (u.on()) next.load(u.at(in), in.wide);
+    if (u.on()) next.load(u.at(k, v, in), in.wide);
     Extent4<T> e = Extent4<T>::of(x.a);
     e.take(x.b);
     e.join(4);
@@ -137,6 +138,8 @@ __global__ void __launch_bounds__(kRowsThreads) load_kernel(PagedCache c, RowsAr
   const int page = at.pos < 0 ? -1 : c.table[static_cast<int64_t>(at.slot) * c.table_pages + (at.pos >> c.page_shift)];
   const bool there = c.is_page(page);
   const int in_page = at.pos & (c.page_size - 1);
+  uint16_t *k = in.k + u.row * in.k_row + 16 * t, *v = in.v + u.row * in.v_row + 16 * t;
+  unsigned char* first = reinterpret_cast<unsigned char*>(c.pool + c.block(page, in.layer, 0));
   if constexpr (Bits == 4) {
     const int head_bytes = block4_bytes(c);
     const int codes = in_page * (D / 2) + 8 * t, pair = block4_codes(c) + (in_page * (D / kGroup4) + t / 4) * 4;
@@ -144,14 +147,14 @@ __global__ void __launch_bounds__(kRowsThreads) load_kernel(PagedCache c, RowsAr
     uint32_t p = 0;
     auto load = [&] {
       if (!there || !u.on()) return;
-      const unsigned char* from = u.place(c, in, page) + u.head * head_bytes;
+      const unsigned char* from = u.place(c, first) + u.head * head_bytes;
       w = *reinterpret_cast<const uint2*>(from + codes);
       p = *reinterpret_cast<const uint32_t*>(from + pair);
     };
     load();
     while (u.on()) {
       const Piece x{values4<T>(w.x, p), values4<T>(w.y, p)};
-      uint16_t* to = u.at(in);
+      uint16_t* to = u.at(k, v, in);
       u.next(c);
       load();
       x.store(to, in.wide);
@@ -160,13 +163,13 @@ __global__ void __launch_bounds__(kRowsThreads) load_kernel(PagedCache c, RowsAr
     Piece next{};
     auto load = [&] {
       if (!there || !u.on()) return;
-      next.load(reinterpret_cast<const uint16_t*>(u.place(c, in, page)) +
+      next.load(reinterpret_cast<const uint16_t*>(u.place(c, first)) +
                     (static_cast<int64_t>(u.head) * c.page_size + in_page) * D + 16 * t, true);
     };
     load();
     while (u.on()) {
       const Piece x = next;
-      uint16_t* to = u.at(in);
+      uint16_t* to = u.at(k, v, in);
       u.next(c);
       load();
       x.store(to, in.wide);
