@@ -22,7 +22,8 @@ from typing import Optional
 import torch
 
 from magpie_tts_rt_b200 import _lib as L
-from magpie_tts_rt_b200.paged_cache import _DTYPES, HEAD_DIMS, MAX_ROWS, _check, _current_device, _raw_stream, _rows_of
+from magpie_tts_rt_b200 import paged_cache as _cache
+from magpie_tts_rt_b200.paged_cache import _DTYPES, HEAD_DIMS, MAX_ROWS, _check, _raw_stream, _rows_of
 
 MAX_HEADS = 1 << 16
 
@@ -131,7 +132,7 @@ class Rotation:
             outs.append(out)
         self._on_stream(handle, stream)
         call = L.lib.mtt_b200_launch_rotate_heads
-        if _current_device() == index:
+        if _cache._current_device() == index:
             rc = call(self._c[dtype][1], ctypes.byref(args), handle)
         else:
             with torch.cuda.device(index):
