@@ -1,6 +1,6 @@
 """Many speech sessions from a few prefilled voices, on one paged cache.
 
-    python examples/voice_sessions.py [--sessions 64] [--steps 48] [--window 64]
+    python examples/voice_sessions.py [--sessions 64] [--steps 48] [--window 64] [--bits 4]
 
 The decoder here is the self-attention part of the Main Decoder's layers (its
 width, heads and weights; LayerNorm and projections in torch): what matters is
@@ -33,12 +33,13 @@ class VoiceServer:
     """Slots 0..3: voices 0 and 1, conditional and unconditional rows; session
     i: slots 4 + 2 i (conditional) and 5 + 2 i."""
 
-    def __init__(self, sessions: int, max_tokens: int, layers: int = 4, window: int = 0, seed: int = 0, page_size=16):
+    def __init__(self, sessions: int, max_tokens: int, layers: int = 4, window: int = 0, seed: int = 0, page_size=16,
+                 bits: int = 16):
         self.sessions, self.layers, self.window = sessions, layers, window
         slots = 4 + 2 * sessions
         # the voices once, and for each slot its own tokens and a copy of a partial page
         pages = 4 * -(-REFERENCE_PREFIX // page_size) + 2 * sessions * (2 + (max_tokens - REFERENCE_PREFIX) // page_size)
-        self.cache = PagedCache.allocate(pages, slots, max_tokens, layers, HEADS, HEAD_DIM, page_size)
+        self.cache = PagedCache.allocate(pages, slots, max_tokens, layers, HEADS, HEAD_DIM, page_size, bits=bits)
         self.weights = make_main_decoder_weights(seed, positions=8, layers=layers).to(device="cuda")
         self.open = [False] * sessions
         self.voice = [0] * sessions
@@ -115,8 +116,9 @@ def main() -> None:
     ap.add_argument("--sessions", type=int, default=64)
     ap.add_argument("--steps", type=int, default=48)
     ap.add_argument("--window", type=int, default=64)
+    ap.add_argument("--bits", type=int, default=16, choices=(4, 16), help="of a key or value in the cache")
     a = ap.parse_args()
-    server = VoiceServer(a.sessions, REFERENCE_PREFIX + a.steps + 1, window=a.window)
+    server = VoiceServer(a.sessions, REFERENCE_PREFIX + a.steps + 1, window=a.window, bits=a.bits)
     g = torch.Generator(device="cuda").manual_seed(1)
     draw = lambda *s: torch.randn(*s, WIDTH, generator=g, device="cuda").to(torch.bfloat16)  # noqa: E731
     server.prefill(draw(4, REFERENCE_PREFIX))

@@ -396,3 +396,32 @@ def test_shared_prefix(pc, d, group, known):
     fin = torch.isfinite(ref_lse)
     assert ((lse.cpu().double() - ref_lse).abs()[fin] <= 1e-3 + 2 * (plain[1] - ref_lse).abs()[fin]).all()
     assert (alone.cpu().double() - plain[0]).abs().max() < 0.05
+
+
+def test_voice_sessions_in_4_bits(pc):
+    """The example on a 4-bit cache: prefill, forks, shared-prefix steps, sessions ended, compaction, new ones; no call is
+    refused, and a prefix stays to the bit what it was when it was stored."""
+    import os
+    import sys
+    sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples"))
+    from voice_sessions import REFERENCE_PREFIX, WIDTH, VoiceServer
+    server = VoiceServer(6, REFERENCE_PREFIX + 32, layers=2, window=24, bits=4)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    draw = lambda *s: torch.randn(*s, WIDTH, generator=g, device="cuda").to(torch.bfloat16)  # noqa: E731
+    server.prefill(draw(4, REFERENCE_PREFIX))
+    cache, n = server.cache, REFERENCE_PREFIX
+    offsets = i32([n * min(s, 4) for s in range(cache.slots + 1)])
+    before = cache.load(4 * n, offsets=offsets)
+    server.start(range(6), [s % 2 for s in range(6)])
+    x = draw(cache.slots)
+    for step in range(10):
+        if step == 5:
+            server.end([0, 2, 4])
+            server.start([0, 4], [1, 1])
+        x = server.step(x)
+    torch.cuda.synchronize()
+    assert cache.bits == 4 and (cache.status == 0).all()
+    live = torch.tensor([s for s in range(4, cache.slots) if server.open[(s - 4) // 2]], device="cuda")
+    assert torch.isfinite(x[live].float()).all()
+    after = cache.load(4 * n, offsets=offsets)
+    assert torch.equal(before[0], after[0]) and torch.equal(before[1], after[1])
