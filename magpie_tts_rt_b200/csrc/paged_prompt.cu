@@ -938,21 +938,23 @@ __global__ void __launch_bounds__(PromptCfg<D, Bits>::kThreads, 1)
                   if (ok && t == last[i]) commit(&o_full[i]);
                 }
               }
-              if (next) {
-                if (i == 0) {
-                  ok = ok && patience.wait(&ready[ks], (it / S) & 1);
-                  if (ok) tmem_fence_after_sync();
-                }
-                if (ok && seen[i].at(j1)) {
-                  scores4(i, ks, h);
+            }
+            // the values' stage is given back before the next scores, which would hold it up
+            if (ok && h == 1) commit(&kv_empty[vs]);
+            if (next) {
+              ok = ok && patience.wait(&ready[ks], (it / S) & 1);
+              ++it;
+              if (ok) {
+                tmem_fence_after_sync();
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                  if (seen[i].at(j1)) scores4(i, ks, h);
                   if (h == 1 && t + 1 == last[i]) commit(&q_free[i]);
                 }
+                commit(&kv_empty[ks]);
               }
             }
-            if (ok && next) commit(&kv_empty[ks]);
-            if (next) ++it;
           }
-          if (ok) commit(&kv_empty[vs]);
         }
         if (!ok) *errv = 1;
         continue;
