@@ -597,9 +597,11 @@ __global__ void __launch_bounds__(PromptCfg<D, Bits>::kThreads, 1)
       mbar_init(&half_done[i], 1);
       mbar_init(&o_full[i], 1);
       mbar_init(&q_free[i], 1);
-      for (int h = 0; h < 2; ++h) {
-        mbar_init(&s_half[i][h], 1);
-        mbar_init(&pv_done[i][h], 1);
+      if constexpr (Bits == 4) {
+        for (int h = 0; h < 2; ++h) {
+          mbar_init(&s_half[i][h], 1);
+          mbar_init(&pv_done[i][h], 1);
+        }
       }
     }
     mbar_init(&fin, 1);

@@ -22,6 +22,7 @@ import torch
 
 from oracle import paged_cache as O
 from test_gpu_paged_cache import agree, i32, pc, queries  # noqa: F401
+from test_gpu_paged_waits import call
 
 pytestmark = pytest.mark.gpu
 
@@ -425,3 +426,74 @@ def test_voice_sessions_in_4_bits(pc):
     assert torch.isfinite(x[live].float()).all()
     after = cache.load(4 * n, offsets=offsets)
     assert torch.equal(before[0], after[0]) and torch.equal(before[1], after[1])
+
+
+# ---------------------------------------------------------------------------
+# bounded waits (the converters' among them)
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_prompt_that_gives_up(pc, d):
+    """No key tile is ever converted: all slots with rows are marked, no other, and the next call is right."""
+    new = [1, 0, 300, 40, 0, 129, 7]
+    lengths = [n + 100 * (i % 3) for i, n in enumerate(new)]
+    cache, pool, table = make4(pc, lengths, 2, d)
+    q = queries(sum(new), 4, d, torch.bfloat16)
+    offsets = [0] + np.cumsum(new).tolist()
+    call(cache, q.cuda(), 2_000_000, i32(offsets), starve=True)
+    assert cache.status.tolist() == [4 if n else 0 for n in new]
+    cache.status.zero_()
+    got, lse = call(cache, q.cuda(), 200_000_000, i32(offsets))
+    agree(got, lse, O.attention(values_rounded(O.held(pool, torch.bfloat16), torch.bfloat16), table, lengths, 0, q, offsets),
+          torch.bfloat16, max(lengths))
+    assert (cache.status == 0).all()
+
+
+def test_prefix_pass_that_gives_up(pc):
+    """Its members are attended on their own: marked, and right."""
+    cache = pc.PagedCache.allocate(60, 5, 320, 1, 2, 64, bits=4)
+    cache.extend(i32([160, 0, 0, 0, 0]))
+    x = values((160, 2, 64), torch.bfloat16, 2).cuda()
+    cache.store(x, -x, layer=0, offsets=i32([0] + [160] * 5))
+    cache.fork(i32([-1, 0, 0, 0, -1]))
+    cache.extend(i32([0, 3, 1, 20, 0]))
+    y = values((24, 2, 64), torch.bfloat16, 3).cuda()
+    cache.store(y, y, layer=0, offsets=i32([0, 0, 3, 4, 24, 24]))
+    plan = pc.PrefixGroups(cache, [(0, 160, [1, 2, 3])], q_heads=4)
+    plan._c.shared_tokens = 0
+    q = queries(5, 4, 64, torch.bfloat16).cuda()
+    for starve, status in ((True, [0, 4, 4, 4, 0]), (False, [0] * 5)):
+        cache.status.zero_()
+        got, lse = call(cache, q, 2_000_000, groups=plan, starve=starve)
+        assert cache.status.tolist() == status
+        held = O.held(cache.pool.cpu(), torch.bfloat16)
+        ref = O.attention(held, cache.page_table.cpu(), cache.lengths.tolist(), 0, q.cpu(), list(range(6)))
+        # a prefix's values are rounded once more (2^-8 of the weight), as are its weights and the result
+        assert ((got.cpu().double() - ref[0]).abs() <= 1.1 * 2.0 ** -8 * (ref[0].abs() + 2 * ref[2]) + 1e-4).all()
+        if starve:      # single tokens: the result's rounding, scores and weights right to 2^-12 (see above)
+            assert ((got.cpu().double() - ref[0]).abs() <= 2.0 ** -8 * ref[0].abs() + 2.0 ** -12 * (ref[2] + 1)).all()
+
+
+def test_units_longer_than_the_limit(pc):
+    """As in test_gpu_paged_waits.py: a unit lasts far longer than a bound that would not grow with the share."""
+    d, hkv, ps, distinct, rows, length, dtype = 128, 4, 128, 64, 4096, 700_000, torch.bfloat16
+    used = -(-length // ps)
+    g = torch.Generator().manual_seed(4)
+    pool = torch.randint(0, 256, (distinct, 1, 2, hkv, ps, token_bytes(d)), generator=g, dtype=torch.uint8)
+    pairs = torch.stack([torch.full((2,), 0.25), torch.full((2,), -2.0)], -1).to(dtype)     # values -2 .. 1.75
+    pool.view(distinct, 1, 2, hkv, -1)[..., ps * d // 2:] = pairs.view(torch.uint8).flatten().repeat(ps)
+    table = torch.randint(0, distinct, (1, used), generator=g, dtype=torch.int32)
+    cache = pc.PagedCache(pool.cuda(), table.cuda(), i32([length]), torch.ones(distinct, dtype=torch.int32, device="cuda"), dtype=dtype)
+    q = queries(rows, hkv, d, dtype)
+    out, lse = call(cache, q.cuda(), 2_000_000, i32([0, rows]))
+    assert int(cache.status) == 0
+    k, v = (x.permute(1, 0, 2, 3).reshape(hkv, distinct * ps, d) for x in O.held(pool, dtype)[:, 0].unbind(1))
+    for r in (0, 255, 256, rows // 2 + 3, rows - 1):
+        p = length - rows + r
+        full = p // ps
+        times = torch.bincount(table[0, :full].long(), minlength=distinct).double()[:, None].expand(distinct, ps).clone()
+        times[table[0, full], :p % ps + 1] += 1
+        s = torch.einsum("hd,hkd->hk", q[r].double(), k) * d ** -0.5 + times.reshape(-1).log()
+        w = torch.softmax(s, -1)
+        ref = tuple(torch.einsum("hk,hkd->hd", w, x)[None] for x in (v, v.abs()))
+        agree(out[r:r + 1], lse[r:r + 1], (ref[0], torch.logsumexp(s, -1)[None], ref[1]), dtype, 1)
