@@ -290,7 +290,8 @@ class PagedCache:
             _check(0 <= rows <= MAX_ROWS, f"at most {MAX_ROWS} rows")
             shape = (rows, self.kv_heads, self.head_dim) if layer is not None else (self.layers, rows, self.kv_heads, self.head_dim)
             with self._on(stream):
-                k, v = torch.empty((2, *shape), dtype=self.dtype, device=self.device)
+                k = torch.empty(shape, dtype=self.dtype, device=self.device)
+                v = torch.empty(shape, dtype=self.dtype, device=self.device)
         args = self._cache_rows(k, v, layer, offsets)
         _check(args.rows == rows, "k and v have other rows than asked for")
         self._call("mtt_b200_launch_paged_cache_load", self._ref, ctypes.byref(args), self._handle(stream))
@@ -304,30 +305,40 @@ class PagedCache:
         ``rotation.rotate`` and ``store``, bit for bit, in one pass.  A token's
         position is its place in its slot, or positions [rows] int32.  A row that no
         slot has, or whose tokens ``extend`` has refused, gets a query of 0."""
-        _check(rotation._index == self._index and rotation.head_dim == self.head_dim,
-               "the rotation is for another head_dim or device than the cache")
-        rows = L.RotateRows()
-        args = self._cache_rows(k, v, layer, offsets)
-        rows.rows, rows.kv_heads, rows.layer, rows.k, rows.v = args.rows, self.kv_heads, layer, args.k, args.v
-        rows.k_row_stride, rows.v_row_stride, rows.offsets = args.k_row_stride, args.v_row_stride, args.offsets
-        _check(args.rows <= MAX_ROWS, f"at most {MAX_ROWS} rows")
-        if positions is not None:
-            rows.positions = self._vector(positions, args.rows, torch.int32, "positions")
+        shape, d, heads = k.shape, self.head_dim, self.kv_heads
+        if rotation._index != self._index or rotation.head_dim != d:
+            raise ValueError("the rotation is for another head_dim or device than the cache")
+        if not 0 <= layer < self.layers:
+            raise ValueError("no such layer")
+        if len(shape) != 3 or v.shape != shape or shape[1] != heads or shape[2] != d:
+            raise ValueError("k and v must be [rows, kv_heads, head_dim], with the cache's heads")
+        n = shape[0]
+        if n > MAX_ROWS or (offsets is None and n > self.slots):
+            raise ValueError(f"at most {MAX_ROWS} rows, and without offsets one for each slot")
+        k_row, v_row = self._rows_of(k, shape, k.stride(), "k"), self._rows_of(v, shape, v.stride(), "v")
+        at = None if offsets is None else self._vector(offsets, self.slots + 1, torch.int32, "offsets")
+        places = None if positions is None else self._vector(positions, n, torch.int32, "positions")
+        q_heads, q_at, q_row, out_at, out_row = 0, None, 0, None, 0
         if q is not None:
-            shape = q.shape
-            if len(shape) != 3 or shape[0] != args.rows or shape[2] != self.head_dim or not 1 <= shape[1] <= MAX_GROUP * self.kv_heads:
+            q_shape = q.shape
+            if len(q_shape) != 3 or q_shape[0] != n or q_shape[2] != d or not 1 <= q_shape[1] <= MAX_GROUP * heads:
                 raise ValueError("q must be [rows, q_heads, head_dim], with the rows of k and v")
-            rows.q_heads, rows.q, rows.q_row_stride = shape[1], q.data_ptr(), self._rows_of(q, shape, q.stride(), "q")
+            q_heads, q_at, q_row = q_shape[1], q.data_ptr(), self._rows_of(q, q_shape, q.stride(), "q")
             if q_out is None:
                 with self._on(stream):
-                    q_out = torch.empty(shape, dtype=self.dtype, device=self.device)
-            elif q_out.shape != shape:
-                raise ValueError("q_out must have q's shape")
-            rows.q_out, rows.q_out_row_stride = q_out.data_ptr(), self._rows_of(q_out, shape, q_out.stride(), "q_out")
+                    q_out = torch.empty(q_shape, dtype=self.dtype, device=self.device)
+                out_row = q_heads * d
+            else:
+                _check(q_out.shape == q_shape, "q_out must have q's shape")
+                out_row = self._rows_of(q_out, q_shape, q_out.stride(), "q_out")
+            out_at = q_out.data_ptr()
         else:
             _check(q_out is None, "q_out without q")
+        rows = L.RotateRows(n, q_heads, heads, layer, q_at, k.data_ptr(), v.data_ptr(), out_at, None, q_row, k_row, v_row, out_row,
+                            0, places, at)
         handle = self._handle(stream)
-        rotation._on_stream(handle, stream)
+        if handle not in rotation._streams:
+            rotation._on_stream(handle, stream)
         self._call("mtt_b200_launch_paged_cache_append", self._ref, rotation._c[self.dtype][1], ctypes.byref(rows), handle)
         return q_out
 

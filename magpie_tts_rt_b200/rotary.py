@@ -87,50 +87,27 @@ class Rotation:
         head_dim] bf16 or f16 (either may be None), rows of any stride with
         contiguous heads, positions [rows] int32.  q_out and k_out may be q and k;
         otherwise they must not overlap what the call reads."""
-        _check(q is not None or k is not None, "a rotation needs queries or keys")
-        first = q if q is not None else k
-        dtype, index = first.dtype, first.get_device()
-        _check(dtype in _DTYPES, "q and k must be bfloat16 or float16")
-        _check(index == self._index, "q and k must be on the rotation's device")
-        _check(first.dim() == 3, "q and k must be [rows, heads, head_dim]")
-        rows = first.shape[0]
-        _check(rows <= MAX_ROWS, f"at most {MAX_ROWS} rows")
+        first = k if q is None else q
+        if first is None or first.dim() != 3:
+            raise ValueError("a rotation needs queries or keys, [rows, heads, head_dim]")
+        index, dtype, rows = self._index, first.dtype, first.shape[0]
+        if dtype not in _DTYPES or rows > MAX_ROWS:
+            raise ValueError(f"q and k must be bfloat16 or float16, of at most {MAX_ROWS} rows")
         if positions.dtype is not torch.int32 or positions.shape != (rows,) or positions.get_device() != index or \
                 not positions.is_contiguous():
             raise ValueError(f"positions must be a contiguous int32 vector of {rows} on the rotation's device")
-        args = L.RotateRows()
-        args.rows, args.positions = rows, positions.data_ptr()
         if stream is None:
-            handle, ctx = self._raw(index), None
+            handle = self._raw(index)
+        elif stream.device.index == index:
+            handle = stream.cuda_stream
         else:
-            _check(stream.device.index == index, "the stream belongs to another device than the rotation")
-            handle, ctx = stream.cuda_stream, torch.cuda.stream(stream)
-        outs = []
-        for name, x, out in (("q", q, q_out), ("k", k, k_out)):
-            if x is None:
-                _check(out is None, f"{name}_out without {name}")
-                outs.append(None)
-                continue
-            _check(x.dim() == 3 and x.shape[0] == rows and x.shape[2] == self.head_dim and x.shape[1] <= MAX_HEADS,
-                   "q and k must be [rows, heads, head_dim]")
-            stride = _rows_of(x, x.shape, x.stride(), name, dtype, index)
-            if out is None:
-                if ctx is None:
-                    out = torch.empty(x.shape, dtype=dtype, device=self.device)
-                else:
-                    with ctx:
-                        out = torch.empty(x.shape, dtype=dtype, device=self.device)
-            else:
-                _check(out.shape == x.shape, f"{name}_out must have {name}'s shape")
-            out_stride = _rows_of(out, x.shape, out.stride(), name + "_out", dtype, index)
-            if name == "q":
-                args.q_heads, args.q, args.q_row_stride = x.shape[1], x.data_ptr(), stride
-                args.q_out, args.q_out_row_stride = out.data_ptr(), out_stride
-            else:
-                args.kv_heads, args.k, args.k_row_stride = x.shape[1], x.data_ptr(), stride
-                args.k_out, args.k_out_row_stride = out.data_ptr(), out_stride
-            outs.append(out)
-        self._on_stream(handle, stream)
+            raise ValueError("the stream belongs to another device than the rotation")
+        q_heads, q_at, q_row, q_to, q_to_row, q_out = self._side(q, q_out, "q", rows, dtype, stream)
+        k_heads, k_at, k_row, k_to, k_to_row, k_out = self._side(k, k_out, "k", rows, dtype, stream)
+        args = L.RotateRows(rows, q_heads, k_heads, 0, q_at, k_at, None, q_to, k_to, q_row, k_row, 0, q_to_row, k_to_row,
+                            positions.data_ptr())
+        if handle not in self._streams:
+            self._on_stream(handle, stream)
         call = L.lib.mtt_b200_launch_rotate_heads
         if _cache._current_device() == index:
             rc = call(self._c[dtype][1], ctypes.byref(args), handle)
@@ -139,4 +116,23 @@ class Rotation:
                 rc = call(self._c[dtype][1], ctypes.byref(args), handle)
         if rc != L.STATUS_OK:
             raise RuntimeError(f"mtt_b200_launch_rotate_heads failed with status {rc}")
-        return tuple(outs)
+        return q_out, k_out
+
+    def _side(self, x, out, name, rows, dtype, stream):
+        """(heads, address, row stride, out's address and row stride, out) of queries or keys."""
+        if x is None:
+            _check(out is None, f"{name}_out without {name}")
+            return 0, None, 0, None, 0, None
+        shape = x.shape
+        if len(shape) != 3 or shape[0] != rows or shape[2] != self.head_dim or shape[1] > MAX_HEADS:
+            raise ValueError("q and k must be [rows, heads, head_dim]")
+        stride = _rows_of(x, shape, x.stride(), name, dtype, self._index)
+        if out is None:
+            if stream is None:
+                out = torch.empty(shape, dtype=dtype, device=self.device)
+            else:
+                with torch.cuda.stream(stream):
+                    out = torch.empty(shape, dtype=dtype, device=self.device)
+            return shape[1], x.data_ptr(), stride, out.data_ptr(), shape[1] * shape[2], out
+        _check(out.shape == shape, f"{name}_out must have {name}'s shape")
+        return shape[1], x.data_ptr(), stride, out.data_ptr(), _rows_of(out, shape, out.stride(), name + "_out", dtype, self._index), out
