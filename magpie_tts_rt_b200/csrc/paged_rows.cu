@@ -53,11 +53,11 @@ struct RowUnit {
   }
   // the lane's 16 dims of the item in k or v (`k`, `v`: those of the row's first head and layer)
   __device__ __forceinline__ uint16_t* at(uint16_t* k, uint16_t* v, const RowsArgs& in) const {
-    return ((block & 1) != 0 ? v + (block >> 1) * in.v_layer : k + (block >> 1) * in.k_layer) + head * D;
+    return ((block & 1) != 0 ? v + (block >> 1) * in.v_layer : k + (block >> 1) * in.k_layer) + static_cast<int64_t>(head) * D;
   }
   // the item's keys or values in its page (`first`: those of the call's first layer), all heads
   __device__ __forceinline__ unsigned char* place(const PagedCache& c, unsigned char* first) const {
-    return first + static_cast<uint64_t>(static_cast<uint32_t>(block)) * static_cast<uint32_t>(2 * c.kv_elems);
+    return first + static_cast<uint64_t>(static_cast<uint32_t>(block)) * static_cast<uint64_t>(2 * c.kv_elems);
   }
 };
 
@@ -113,7 +113,7 @@ __global__ void __launch_bounds__(kRowsThreads) store4_kernel(PagedCache c, Rows
   while (__any_sync(0xffffffffu, u.on())) {
     const Piece x = next;
     const bool on = u.on();
-    unsigned char* to = u.place(c, first) + u.head * head_bytes;
+    unsigned char* to = u.place(c, first) + static_cast<int64_t>(u.head) * head_bytes;
     u.next(c);
     if (u.on()) next.load(u.at(k, v, in), in.wide);
     Extent4<T> e = Extent4<T>::of(x.a);
@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(kRowsThreads) load_kernel(PagedCache c, RowsAr
     uint32_t p = 0;
     auto load = [&] {
       if (!there || !u.on()) return;
-      const unsigned char* from = u.place(c, first) + u.head * head_bytes;
+      const unsigned char* from = u.place(c, first) + static_cast<int64_t>(u.head) * head_bytes;
       w = *reinterpret_cast<const uint2*>(from + codes);
       p = *reinterpret_cast<const uint32_t*>(from + pair);
     };

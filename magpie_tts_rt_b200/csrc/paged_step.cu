@@ -47,12 +47,22 @@ constexpr int kStepWarps = 4;
 constexpr int kStepThreads = 32 * kStepWarps;
 
 // Forms of the kernels: 16 for a pool in 16 bits; for one in 4 bits how many query
-// heads a key head has at most: 1, 2, 4 or more (8).
-constexpr int step_form(int bits, int group) { return bits == 16 ? 16 : group <= 2 ? group : group <= 4 ? 4 : 8; }
+// heads a key head has at most: 1, 2, 4, 8 or more (9).  (Two heads of 128 dims take
+// form 4, whose two tiles a step leave registers: 16 slots of 16,384 keys, 8 key
+// heads, 101 us instead of 107.  Heads of 64 dims: 115 instead of 99.)
+constexpr int step_form(int bits, int head_dim, int group) {
+  if (bits == 16) return 16;
+  if (group > 4) return group > 8 ? 9 : 8;
+  return group > 2 || (group == 2 && head_dim == 128) ? 4 : group;
+}
 
-// 16-key tiles per warp and step
+// 16-key tiles per warp and step.  (4 bits, the same keys, or twice as many with 64
+// dims, in us with 4 / 2 / 1 tiles: 4 heads of 64 116 / 113 / -, 8 of 64 177 / 129 /
+// 143, 8 of 128 - / 124 / 129, 16 of 64 490 / 190 / 191, 16 of 128 - / 263 / 185:
+// what does not fit the registers is what costs.)
 constexpr int step_tiles(int head_dim, int form) {
-  return form == 16 ? (head_dim == 64 ? 2 : 1) : form >= 4 && head_dim == 128 ? 2 : 4;
+  if (form == 16) return head_dim == 64 ? 2 : 1;
+  return form == 9 ? 1 : form >= 4 ? 2 : 4;
 }
 constexpr int step_ctas(int head_dim, int nb, int form) {  // per SM (registers)
   return (head_dim == 64 ? 4 : 3) - (nb == 2 ? 1 : 0);
@@ -314,7 +324,7 @@ __device__ __forceinline__ int step_dims(int t, int k) {
 // The query of a product's column.
 template <int Form>
 __device__ __forceinline__ int step_column(int g) {
-  return Form == 16 ? g : g & (Form == 1 ? 1 : Form - 1);  // (with one query the odd columns are empty)
+  return Form >= 8 ? g : g & (Form == 1 ? 1 : Form - 1);  // (with one query the odd columns are empty)
 }
 
 // attend_tiles for a pool in 4 bits.  Nothing is rounded on the way into the
@@ -1083,7 +1093,7 @@ size_t cut_bytes(int head_dim, int nb, int form) {
 size_t step_workspace(const mtt_b200_paged_cache_t& c, int q_heads) {
   int nb, blocks;
   step_blocks(q_heads / c.kv_heads, &nb, &blocks);
-  const int form = step_form((c.dtype & MTT_B200_CACHE_4BIT) != 0 ? 4 : 16, q_heads / c.kv_heads);
+  const int form = step_form((c.dtype & MTT_B200_CACHE_4BIT) != 0 ? 4 : 16, c.head_dim, q_heads / c.kv_heads);
   const size_t shares = static_cast<size_t>(kMaxSms) * step_ctas(c.head_dim, nb, form) * kStepWarps;
   return cut_bytes(c.head_dim, nb, form) + (shares * 2 * 8 * nb * (c.head_dim + 2) * 4 + 255) / 256 * 256;
 }
@@ -1092,7 +1102,7 @@ cudaError_t launch_step(const PagedCache& c, int dtype, const Attend& a, const S
                         cudaStream_t stream) {
   int nb, blocks;
   step_blocks(a.group, &nb, &blocks);
-  const int form = step_form(c.bits, a.group);
+  const int form = step_form(c.bits, c.head_dim, a.group);
   StepSpace ws;
   ws.cut = static_cast<int4*>(space);
   ws.part = reinterpret_cast<float*>(static_cast<char*>(space) + cut_bytes(c.head_dim, nb, form));
@@ -1144,10 +1154,12 @@ cudaError_t launch_step(const PagedCache& c, int dtype, const Attend& a, const S
     if (form == 16) return with_form(type, dim, bs, integral_constant<int, 16>{});
     if constexpr (decltype(bs)::value == 1) {
       if (form == 1) return with_form(type, dim, bs, integral_constant<int, 1>{});
-      if (form == 2) return with_form(type, dim, bs, integral_constant<int, 2>{});
+      if constexpr (decltype(dim)::value == 64) {
+        if (form == 2) return with_form(type, dim, bs, integral_constant<int, 2>{});
+      }
       if (form == 4) return with_form(type, dim, bs, integral_constant<int, 4>{});
     }
-    return with_form(type, dim, bs, integral_constant<int, 8>{});
+    return with_form(type, dim, bs, integral_constant<int, decltype(bs)::value == 1 ? 8 : 9>{});
   };
   auto pick = [&](auto type) {
     using std::integral_constant;
