@@ -92,6 +92,14 @@ def _rows_of(t, shape, st, name, dtype, index) -> int:
     return row
 
 
+def _written_rows(t, shape, name, dtype, index) -> int:
+    """_rows_of a tensor that a call writes: rows must not overlap."""
+    row = _rows_of(t, shape, t.stride(), name, dtype, index)
+    if shape[0] > 1 and abs(row) < shape[1] * shape[2]:
+        raise ValueError(f"rows of {name} overlap")
+    return row
+
+
 def _token_bytes(head_dim: int) -> int:
     """Of one token's keys, or values, of one head in a 4-bit pool."""
     return head_dim // 2 + head_dim // 16
@@ -286,7 +294,8 @@ class PagedCache:
         that no slot has, or whose slot has fewer tokens than rows, is 0.  k and v:
         where they go, if given."""
         _check((k is None) == (v is None), "k and v are given together")
-        if k is None:
+        given = k is not None
+        if not given:
             _check(0 <= rows <= MAX_ROWS, f"at most {MAX_ROWS} rows")
             shape = (rows, self.kv_heads, self.head_dim) if layer is not None else (self.layers, rows, self.kv_heads, self.head_dim)
             with self._on(stream):
@@ -294,6 +303,12 @@ class PagedCache:
                 v = torch.empty(shape, dtype=self.dtype, device=self.device)
         args = self._cache_rows(k, v, layer, offsets)
         _check(args.rows == rows, "k and v have other rows than asked for")
+        if given:
+            for x, name in ((k, "k"), (v, "v")):
+                one = x if layer is not None else x[0]
+                _written_rows(one, one.shape, name, self.dtype, self._index)
+                _check(layer is not None or len(x) == 1 or abs(x.stride(0)) >= self.kv_heads * self.head_dim,
+                       f"layers of {name} overlap")
         self._call("mtt_b200_launch_paged_cache_load", self._ref, ctypes.byref(args), self._handle(stream))
         return k, v
 
@@ -330,7 +345,7 @@ class PagedCache:
                 out_row = q_heads * d
             else:
                 _check(q_out.shape == q_shape, "q_out must have q's shape")
-                out_row = self._rows_of(q_out, q_shape, q_out.stride(), "q_out")
+                out_row = _written_rows(q_out, q_shape, "q_out", self.dtype, self._index)
             out_at = q_out.data_ptr()
         else:
             _check(q_out is None, "q_out without q")

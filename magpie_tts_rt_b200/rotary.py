@@ -23,7 +23,7 @@ import torch
 
 from magpie_tts_rt_b200 import _lib as L
 from magpie_tts_rt_b200 import paged_cache as _cache
-from magpie_tts_rt_b200.paged_cache import _DTYPES, HEAD_DIMS, MAX_ROWS, _check, _raw_stream, _rows_of
+from magpie_tts_rt_b200.paged_cache import _DTYPES, HEAD_DIMS, MAX_ROWS, _check, _raw_stream, _rows_of, _written_rows
 
 MAX_HEADS = 1 << 16
 
@@ -35,8 +35,8 @@ class Rotation:
         """rotary_dim (a multiple of 16, all of head_dim if not given) dims of a
         head are turned, pair i by base^(-2 i / rotary_dim) radians a position, or
         by frequencies [rotary_dim / 2] (any real type).  q_norm, k_norm [head_dim]:
-        weights of the norms.  All of it is copied: later changes of the tensors do
-        not reach the rotation."""
+        weights of the norms.  All of it is copied, which is waited for: later changes of
+        the tensors do not reach the rotation, and any stream may use it."""
         _check(head_dim in HEAD_DIMS, f"head_dim must be one of {HEAD_DIMS}")
         rotary_dim = head_dim if rotary_dim is None else rotary_dim
         _check(16 <= rotary_dim <= head_dim and rotary_dim % 16 == 0, "rotary_dim must be a multiple of 16, at most head_dim")
@@ -55,6 +55,8 @@ class Rotation:
         self._index = self.device.index if self.device.type == "cuda" else -1
         self.turns = (frequencies.detach().double() / (2 * math.pi)).to(self.device)
         self.q_norm, self.k_norm = (self._weight(w, n) for w, n in ((q_norm, "q_norm"), (k_norm, "k_norm")))
+        if self.device.type == "cuda":  # any stream may be the first to use them
+            torch.cuda.current_stream(self.device).synchronize()
         self._raw = _raw_stream(self.device)
         self._streams = set()
         self._c = {}
@@ -135,4 +137,4 @@ class Rotation:
                     out = torch.empty(shape, dtype=dtype, device=self.device)
             return shape[1], x.data_ptr(), stride, out.data_ptr(), shape[1] * shape[2], out
         _check(out.shape == shape, f"{name}_out must have {name}'s shape")
-        return shape[1], x.data_ptr(), stride, out.data_ptr(), _rows_of(out, shape, out.stride(), name + "_out", dtype, self._index), out
+        return shape[1], x.data_ptr(), stride, out.data_ptr(), _written_rows(out, shape, name + "_out", dtype, self._index), out

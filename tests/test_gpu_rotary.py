@@ -3,8 +3,8 @@ rotates (PagedCache.append) on the GPU.
 
 Tolerance of a rotated value, derived: f32 arithmetic on a pair (a, b) loses at
 most (D + 24) 2^-24 (|a| + |b|): the mean of D squares in f32, a reciprocal square root
-and two products (8 roundings), cosine and sine (off by 2^-22 from the reduction
-and 2 ulp of their own), two products and a sum.  The result is rounded once:
+and two products (8 roundings), cosine and sine (the reduced angle right to 2^-22, the
+functions to 2^-21: 12 of these units), two products and a sum.  The result is rounded once:
 u |y|, u = finfo.eps / 2."""
 import math
 
@@ -106,6 +106,21 @@ def test_rotate_values_beside_infinities(rotary):
     bad = ~torch.isfinite(got)
     assert bad.nonzero().tolist() == [[1, 0, 3], [1, 0, 19], [1, 1, 40], [2, 0, 63]]
     assert torch.equal(got[..., 32:].view(torch.int16), x[..., 32:].view(torch.int16))
+
+
+def test_rotation_made_on_a_busy_stream(rotary):
+    """Weights that a stream has yet to write: the rotation is there for any stream at once."""
+    side = torch.cuda.Stream()
+    x, pos = values((4, 2, 64), torch.bfloat16, 1).cuda(), i32([0, 1, 2, 3])
+    weight, given = torch.ones(64, device="cuda"), torch.rand(64, device="cuda") + 0.5
+    ref, _ = rotary.Rotation(64, q_norm=given).rotate(x, None, pos)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(100_000_000)
+        weight.copy_(given)
+        r = rotary.Rotation(64, q_norm=weight)
+    got, _ = r.rotate(x, None, pos)
+    assert torch.equal(got, ref)
 
 
 # ---------------------------------------------------------------------------

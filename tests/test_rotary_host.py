@@ -210,6 +210,24 @@ def test_append_and_load_refuse(lib, call):  # noqa: F811
     assert lib.calls == []
 
 
+def test_overlapping_rows_are_not_written(lib):  # noqa: F811
+    """Outputs whose rows (or layers) share memory are refused; inputs may be broadcast."""
+    cache, r = on_host(), turner()
+    one, x = heads(1).expand(3, 2, 64), heads()
+    layers = torch.zeros(1, 3, 2, 64, dtype=torch.bfloat16).expand(2, 3, 2, 64)
+    for call in (lambda: r.rotate(x, None, POS, q_out=one), lambda: r.rotate(x, x, POS, k_out=one),
+                 lambda: cache.append(0, x, x, x, r, q_out=one), lambda: cache.load(3, layer=0, k=one, v=x),
+                 lambda: cache.load(3, layer=0, k=x, v=one), lambda: cache.load(3, k=layers, v=torch.zeros(2, 3, 2, 64, dtype=torch.bfloat16))):
+        with pytest.raises(ValueError):
+            call()
+    assert lib.calls == []
+    r.rotate(one, one, POS)
+    cache.append(0, one, one, one, r)
+    rows = torch.zeros(3, 2, 2, 64, dtype=torch.bfloat16).transpose(0, 1)  # layers side by side in a row
+    cache.load(3, k=rows, v=rows)
+    assert len(lib.calls) == 3
+
+
 def test_4bit_pools_are_looked_at():
     """Without a GPU a cache cannot be made; that a pool is on a CUDA device is the first thing asked for."""
     pool = torch.zeros(2, 1, 2, 1, 16, 36, dtype=torch.uint8)
