@@ -12,6 +12,8 @@ namespace {
 
 constexpr int kRowsThreads = 256;
 constexpr int kRowsWarps = kRowsThreads / 32;
+template <int Bits>
+constexpr int kLoadAhead = Bits == 4 ? 4 : 2;  // heads of a load that a lane has on their way
 
 struct RowsArgs {
   int layer, n_layers, rows, chunks;
@@ -140,39 +142,60 @@ __global__ void __launch_bounds__(kRowsThreads) load_kernel(PagedCache c, RowsAr
   const int in_page = at.pos & (c.page_size - 1);
   uint16_t *k = in.k + u.row * in.k_row + 16 * t, *v = in.v + u.row * in.v_row + 16 * t;
   unsigned char* first = reinterpret_cast<unsigned char*>(c.pool + c.block(page, in.layer, 0));
+  U ahead = u;  // the item that is asked for next
   if constexpr (Bits == 4) {
     const int head_bytes = block4_bytes(c);
     const int codes = in_page * (D / 2) + 8 * t, pair = block4_codes(c) + (in_page * (D / kGroup4) + t / 4) * 4;
-    uint2 w = make_uint2(0, 0);
-    uint32_t p = 0;
-    auto load = [&] {
-      if (!there || !u.on()) return;
-      const unsigned char* from = u.place(c, first) + static_cast<int64_t>(u.head) * head_bytes;
-      w = *reinterpret_cast<const uint2*>(from + codes);
-      p = *reinterpret_cast<const uint32_t*>(from + pair);
+    uint2 w[kLoadAhead<Bits>];
+    uint32_t p[kLoadAhead<Bits>];
+    auto load = [&](int n) {
+      if (there && ahead.on()) {
+        const unsigned char* from = ahead.place(c, first) + static_cast<int64_t>(ahead.head) * head_bytes;
+        w[n] = __ldcs(reinterpret_cast<const uint2*>(from + codes));
+        p[n] = __ldcs(reinterpret_cast<const uint32_t*>(from + pair));
+      }
+      ahead.next(c);
     };
-    load();
+#pragma unroll
+    for (int n = 0; n < kLoadAhead<Bits>; ++n) {
+      w[n] = make_uint2(0, 0);
+      p[n] = 0;
+      load(n);
+    }
     while (u.on()) {
-      const Piece x{values4<T>(w.x, p), values4<T>(w.y, p)};
-      uint16_t* to = u.at(k, v, in);
-      u.next(c);
-      load();
-      x.store(to, in.wide);
+#pragma unroll
+      for (int n = 0; n < kLoadAhead<Bits>; ++n) {
+        if (!u.on()) break;
+        const Piece x{values4<T>(w[n].x, p[n]), values4<T>(w[n].y, p[n])};
+        uint16_t* to = u.at(k, v, in);
+        u.next(c);
+        load(n);
+        x.store(to, in.wide);
+      }
     }
   } else {
-    Piece next{};
-    auto load = [&] {
-      if (!there || !u.on()) return;
-      next.load(reinterpret_cast<const uint16_t*>(u.place(c, first)) +
-                    (static_cast<int64_t>(u.head) * c.page_size + in_page) * D + 16 * t, true);
+    Piece x[kLoadAhead<Bits>];
+    auto load = [&](int n) {
+      if (there && ahead.on())
+        x[n].load(reinterpret_cast<const uint16_t*>(ahead.place(c, first)) +
+                      (static_cast<int64_t>(ahead.head) * c.page_size + in_page) * D + 16 * t, true);
+      ahead.next(c);
     };
-    load();
+#pragma unroll
+    for (int n = 0; n < kLoadAhead<Bits>; ++n) {
+      x[n] = Piece{};
+      load(n);
+    }
     while (u.on()) {
-      const Piece x = next;
-      uint16_t* to = u.at(k, v, in);
-      u.next(c);
-      load();
-      x.store(to, in.wide);
+#pragma unroll
+      for (int n = 0; n < kLoadAhead<Bits>; ++n) {
+        if (!u.on()) break;
+        const Piece y = x[n];
+        uint16_t* to = u.at(k, v, in);
+        u.next(c);
+        load(n);
+        y.store(to, in.wide);
+      }
     }
   }
 }
