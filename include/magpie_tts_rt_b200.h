@@ -759,7 +759,9 @@ MTT_B200_API int mtt_b200_session_engine_collect(mtt_b200_session_engine_t* engi
  *   value = low + step * code,
  * with spread, spread / 15 and the code's operations each rounded to single
  * precision, and step then to the type.  A group with a value that is not
- * finite, or a spread that single precision does not hold, reads as NaN.
+ * finite, or a spread that single precision does not hold, reads as NaN; a code
+ * that step's rounding takes past the type's largest number (within 2^-7 of it)
+ * reads as infinite, or NaN where it is a prompt's key.
  *   pool [pages][layers][2][kv_heads] blocks of page_size * (head_dim / 2 +
  *   head_dim / 16) bytes: the codes of the block's tokens (head_dim / 2 bytes
  *   each), then their pairs, step first ([page_size][head_dim / 64][2]).  Every
@@ -856,7 +858,8 @@ MTT_B200_API int mtt_b200_launch_paged_cache_load(const mtt_b200_paged_cache_t* 
  * for i in [0, rotary_dim / 2), a = i, b = i + rotary_dim / 2, or, interleaved,
  * a = 2 i, b = 2 i + 1; dims from rotary_dim on are not turned.  The angle is
  * taken in 64 bits and reduced to one turn, the rest is f32, and each result is
- * rounded once. */
+ * rounded once.  (A head whose squares add up past f32's range is normed as by an
+ * infinite sum.) */
 typedef struct mtt_b200_rotation {
   int32_t head_dim;        /* 64 or 128 */
   int32_t rotary_dim;      /* a multiple of 16, at most head_dim */
@@ -926,10 +929,10 @@ MTT_B200_API int mtt_b200_launch_paged_cache_append(const mtt_b200_paged_cache_t
  * before the first slot's and after the last one's.  Offsets that are not
  * ascending within [0, rows] are not to be given: which rows are then written is
  * not said (none outside [0, rows]).
- * A 4-bit cache is attended to as if it held the values its codes stand for;
- * keys as they are, and values too for single tokens; prompts and shared
- * prefixes round each value once to the cache's type (a further u sum_j p_j
- * |v_j|).
+ * A 4-bit cache is attended to as if it held the values its codes stand for.
+ * Single tokens take keys and values as they are; prompts and shared prefixes
+ * take a key as two numbers of the cache's type (right to 2^-16 of it) and
+ * round each value once (a further u sum_j p_j |v_j|).
  * status[i] becomes 4 when a bounded wait inside the prompt kernel gave up (the
  * bounds grow with the keys that the call has to read): the outputs of slot i's
  * rows are then not to be used. */

@@ -105,6 +105,7 @@ struct Pair4 {
   }
   // The codes of 8 values.  1.5 * 2^23 is added, which rounds to a whole number, half to even, and leaves the code in the
   // lowest bits of 0x4b400000 + code; eight of them are put together by products, whose constant parts add up to one.
+  // (The minimum holds back what a step far below f16's normal range asks for, and keeps product and sum two operations.)
   __device__ __forceinline__ uint32_t codes(const uint4& x) const {
     const uint32_t w[4] = {x.x, x.y, x.z, x.w};
     const float2 less = make_float2(-low, -low), by = make_float2(inverse, inverse), whole = make_float2(12582912.f, 12582912.f);

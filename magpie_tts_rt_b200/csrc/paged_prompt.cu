@@ -62,6 +62,26 @@
 // issuing warp per Q tile, two threads per row, a register split with setmaxnreg
 // (230 bytes spilled in the loop), a quarter of the exponentials as polynomials on
 // the FMA pipe (5 to 10%: it is instructions that bound the loop).
+//
+// A pool in 4 bits (Bits = 4) has 512 threads: warps 9, 10 and 12 to 15 convert
+// (Convert4) instead of TMA and clearing, and the ring holds, of each key tile, the
+// two halves of its keys and its values.  Values are rounded once to 16 bits; a key
+// is two 16-bit numbers, both of which the product takes, half a tile (N = 64) at a
+// time.  A half's scores have columns of their own and are made as soon as P V of
+// the same half of the tile before is under way.  8192 tokens as above take 880 us
+// (0.62 PFLOP/s, the second pass not counted; 925 with inputs that change), 24 ragged
+// prompts of 1 to 509 tokens, 12 heads of 64, window 512, masked keys, 78 us.  A
+// tile's products take 4032 cycles (those of 64 keys 47 each instead of 32: the
+// queries come from shared memory every time), the converter warps are busy for some
+// 4900 of 5900, and the softmax shares their schedulers: without the conversion the
+// first case takes 853 us, with half of the scores' products 822, with neither 674.
+// Tried: keys rounded once (log-sum-exps off by 2^-9 of their scores' terms); codes
+// as they are, steps and offsets joined by the softmax (1020 us; unrolled, 2600: the
+// code did not fit the instruction cache); a tile's values kept until the next scores
+// were made (1047 us); keys split in 16-bit arithmetic on a grid of each group's
+// largest (868 us, with a second path for large values); scores of both numbers
+// beside each other, one N = 128 product and a single buffer (with that split 852
+// us, but the ragged prompts 86 instead of 78).
 #include <algorithm>
 #include <atomic>
 #include <type_traits>

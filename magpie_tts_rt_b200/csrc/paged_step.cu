@@ -34,6 +34,10 @@
 // warps of a CTA side by side in a unit (187 and 247 us, 389 us for the short ones,
 // when the line took 162 and 238); a unit's further tiles prefetched into L2 when
 // it is entered (249 -> 253 us, the short ones 10 us more).
+//
+// A pool in 4 bits (attend_tiles4) takes 9/32 of the bytes, and instructions bound
+// it: the same 512 slots 109 us (306 MB, 2.8 TB/s), the same 8 slots in f16 136 us
+// (422 MB, 3.1 TB/s), the logic pipe busy 66 and 64% of the time, the schedulers 51 and 52.
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -349,6 +353,10 @@ __device__ __forceinline__ int step_column(int g) {
 //  * All 16 keys of a tile are loaded; a key that is not in reach counts by its
 //    weight of zero alone (its pair, which may be anything, is taken as zero).
 //  * The maximum is looked after only when a key passes it.
+//  * A step's keys are loaded under the softmax of the one before, its values under
+//    the next scores (113 -> 109 and 147 -> 136 us of the head comment's cases).
+// Tried and slower: shifts as high halves of products, for another pipe (118, 152
+// us), another number of tiles a step or CTAs an SM.
 template <typename T, int D, int NB, int Form>
 __device__ __forceinline__ void attend_tiles4(const PagedCache& c, const Attend& a, const SeenTiles& seen,
                                               const int32_t* row, const bool* mask, int head, int t0, int t1,
