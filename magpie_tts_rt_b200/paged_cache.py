@@ -229,6 +229,14 @@ class PagedCache:
         """Where a call's own tensors are allocated: the stream that the caller gave, if any."""
         return contextlib.nullcontext() if stream is None else torch.cuda.stream(stream)
 
+    @staticmethod
+    def _new(like, shape, stream, dtype=None):
+        """An output of a call that reads `like` (torch.empty, which looks the type and device up, takes a microsecond more)."""
+        if stream is None:
+            return like.new_empty(shape, dtype=dtype)
+        with torch.cuda.stream(stream):
+            return like.new_empty(shape, dtype=dtype)
+
     def _vector(self, t: torch.Tensor, n: int, dtype: torch.dtype, name: str) -> int:
         if t.dtype is not dtype or t.shape != (n,) or t.get_device() != self._index or not t.is_contiguous():
             raise ValueError(f"{name} must be a contiguous {dtype} vector of {n} on the pool's device")
@@ -300,7 +308,7 @@ class PagedCache:
             shape = (rows, self.kv_heads, self.head_dim) if layer is not None else (self.layers, rows, self.kv_heads, self.head_dim)
             with self._on(stream):
                 k = torch.empty(shape, dtype=self.dtype, device=self.device)
-                v = torch.empty(shape, dtype=self.dtype, device=self.device)
+                v = torch.empty_like(k)
         args = self._cache_rows(k, v, layer, offsets)
         _check(args.rows == rows, "k and v have other rows than asked for")
         if given:
@@ -321,8 +329,8 @@ class PagedCache:
         position is its place in its slot, or positions [rows] int32.  A row that no
         slot has, or whose tokens ``extend`` has refused, gets a query of 0."""
         shape, d, heads = k.shape, self.head_dim, self.kv_heads
-        if rotation._index != self._index or rotation.head_dim != d:
-            raise ValueError("the rotation is for another head_dim or device than the cache")
+        if getattr(rotation, "_index", None) != self._index or rotation.head_dim != d:
+            raise ValueError("the rotation must be a rotary.Rotation of the cache's head_dim and device")
         if not 0 <= layer < self.layers:
             raise ValueError("no such layer")
         if len(shape) != 3 or v.shape != shape or shape[1] != heads or shape[2] != d:
@@ -340,8 +348,7 @@ class PagedCache:
                 raise ValueError("q must be [rows, q_heads, head_dim], with the rows of k and v")
             q_heads, q_at, q_row = q_shape[1], q.data_ptr(), self._rows_of(q, q_shape, q.stride(), "q")
             if q_out is None:
-                with self._on(stream):
-                    q_out = torch.empty(q_shape, dtype=self.dtype, device=self.device)
+                q_out = self._new(q, q_shape, stream)
                 out_row = q_heads * d
             else:
                 _check(q_out.shape == q_shape, "q_out must have q's shape")
@@ -407,8 +414,7 @@ class PagedCache:
         elif not 0 < scale < float("inf"):
             raise ValueError("scale must be positive")
         if out is None:
-            with self._on(stream):
-                out = torch.empty(shape, dtype=self.dtype, device=self.device)
+            out = self._new(q, shape, stream)
             out_row = q_heads * d
         else:
             if out.shape != shape:
@@ -418,8 +424,7 @@ class PagedCache:
         lse = None
         args = L.CacheAttention(layer, q_heads, rows, window, sinks, scale, q.data_ptr(), q_row, out.data_ptr(), out_row)
         if return_lse:
-            with self._on(stream):
-                lse = torch.empty((rows, q_heads), dtype=torch.float32, device=self.device)
+            lse = self._new(q, (rows, q_heads), stream, torch.float32)
             args.lse = lse.data_ptr()
         return args, out, lse
 

@@ -131,10 +131,10 @@ class Rotation:
         stride = _rows_of(x, shape, x.stride(), name, dtype, self._index)
         if out is None:
             if stream is None:
-                out = torch.empty(shape, dtype=dtype, device=self.device)
+                out = x.new_empty(shape)
             else:
                 with torch.cuda.stream(stream):
-                    out = torch.empty(shape, dtype=dtype, device=self.device)
+                    out = x.new_empty(shape)
             return shape[1], x.data_ptr(), stride, out.data_ptr(), shape[1] * shape[2], out
         _check(out.shape == shape, f"{name}_out must have {name}'s shape")
         return shape[1], x.data_ptr(), stride, out.data_ptr(), _written_rows(out, shape, name + "_out", dtype, self._index), out

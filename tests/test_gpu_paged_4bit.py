@@ -399,6 +399,30 @@ def test_shared_prefix(pc, d, group, known):
     assert (alone.cpu().double() - plain[0]).abs().max() < 0.05
 
 
+@pytest.mark.parametrize("d,ps", [(64, 16), (128, 128)])
+def test_places_past_32_bits(pc, d, ps):
+    """A pool of more than 4 GB whose last pages are in use: what a small pool gives, bit for bit."""
+    hkv, group, dtype, lengths = 8, 2, torch.bfloat16, [300, 1, 77]
+    block = 2 * hkv * ps * (d // 2 + d // 16)
+    many = (5 << 30) // block
+    x = values((2, sum(lengths), hkv, d), dtype, 1).cuda()
+    q, rows = queries(3, hkv * group, d, dtype, 2).cuda(), queries(sum(lengths), hkv * group, d, dtype, 3).cuda()
+    offsets = i32([0] + np.cumsum(lengths).tolist())
+    got = []
+    for pages in (64, many):
+        cache = pc.PagedCache.allocate(pages, 3, 320, 1, hkv, d, ps, dtype, bits=4)
+        cache.refs[:pages - 64] = 1                      # all but the last are taken
+        cache.extend(i32(lengths))
+        cache.store(x[0], x[1], layer=0, offsets=offsets)
+        first = cache.page_table[0, 0].item()
+        assert first == pages - 64
+        got.append([*cache.load(sum(lengths), layer=0, offsets=offsets), cache.attend(0, q), cache.attend(0, q, window=40, sinks=3),
+                    cache.attend(0, rows, offsets=offsets), cache.status])
+        torch.cuda.synchronize()
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+
+
 def test_voice_sessions_in_4_bits(pc):
     """The example on a 4-bit cache: prefill, forks, shared-prefix steps, sessions ended, compaction, new ones; no call is
     refused, and a prefix stays to the bit what it was when it was stored."""
