@@ -44,7 +44,11 @@ bool attend_args(const PagedCache& c, const mtt_b200_cache_attention_t* args, At
 // own against shared: 101 MB (12 heads of 64, 1024 tokens, 32 slots) 19 against
 // 30 us; 134 MB (8 of 128, 16384, 2) 38 / 62; 302 MB (12 of 64, 192, 512) 43 / 34;
 // 403 MB (12 of 64, 16384, 8) 66 / 60; 2.1 GB (8 of 128, 4096, 128) 244 / 43.
-constexpr double kSharedBytesWorth = 220e6;
+// In 4 bits the pass takes some 7 us more and its alternative less: of as many values
+// (counted as in 16 bits) 285 MB (8 of 128, 4096, 17) 35 against 42 us; 247 MB (12 of
+// 64, 208, 388) 43 / 47; 329 MB (the same, 516) 54 / 52; 405 MB (12 of 64, 1024, 129)
+// 42 / 40; 545 MB (8 of 128, 512, 260) 73 / 62.
+constexpr double kSharedBytesWorth = 220e6, kSharedBytesWorth4 = 350e6;
 
 // Bytes of the prefix pass's results: base and state (SharedPrefix).
 size_t base_bytes(const mtt_b200_paged_cache_t& c) { return (4 * static_cast<size_t>(c.slots) + 255) / 256 * 256; }
@@ -84,7 +88,7 @@ int attend_shared(const mtt_b200_paged_cache_t* cache, const mtt_b200_cache_atte
   SharedPrefix shared{};
   const double shared_bytes = 4.0 * groups->shared_tokens * c.kv_heads * c.head_dim;
   if (groups->n_groups > 0 && groups->n_members > 0 &&
-      (groups->shared_tokens <= 0 || shared_bytes >= kSharedBytesWorth)) {
+      (groups->shared_tokens <= 0 || shared_bytes >= (c.bits == 4 ? kSharedBytesWorth4 : kSharedBytesWorth))) {
     if (groups->voice == nullptr || groups->tokens == nullptr || groups->offsets == nullptr ||
         groups->members == nullptr)
       return MTT_B200_STATUS_INVALID_ARGUMENT;

@@ -924,7 +924,7 @@ __global__ void __launch_bounds__(kStepThreads)
 // cluster's warps, which join their parts through shared memory: one launch and
 // no workspace.  The largest cluster is taken with which all units run at once
 // (8 CTAs of 8 warps only where a slot can have more than one step for each of 32
-// warps), if a slot cannot be longer than kFewSteps steps of each of its warps.
+// warps), if a slot cannot be longer than few_steps steps of each of its warps.
 // There this saves the scan, the second launch and the parts' way through L2;
 // past either limit the line of tiles is faster, as it fills the device and
 // balances it.  How long a slot can be is the table's width, which the host knows,
@@ -940,7 +940,15 @@ __global__ void __launch_bounds__(kStepThreads)
 //   32/8   128   16    14.5 /  7.4  17.8 / 12.0  23.7 / 18.3 (34.8 / 30.8)
 //   32/8   128   48    18.3 / 12.5 (29.1 / 27.4) (45.9 / 48.6)
 //   16/1   128    6    21.2 /  7.9  21.8 /  8.1  22.8 /  9.9  27.1 / 14.8
-constexpr int kMaxSpread = 8, kFewSteps = 4;
+// Over 4 bits twice as many steps are taken (in brackets what is not):
+//   heads  dim  slots    128 keys      467         1000         2000         4000         8000
+//   12/12   64    2     8.0 /  4.7  10.2 /  4.8  11.8 /  5.0  12.4 /  5.7  13.9 /  7.2  15.3 /  9.7
+//   12/12   64   24    10.8 /  5.2  13.6 /  7.1  15.8 /  9.8  19.7 / 14.7  31.8 / 26.6 (54.3 / 48.7)
+//   32/8   128    4    11.8 /  6.8  12.2 /  7.6  13.3 /  8.5  15.0 / 11.4  19.2 / 17.0  25.0 / 27.3
+//   32/8   128   16    12.3 /  7.3  14.5 /  9.5  18.4 / 13.0  23.3 / 19.6  35.4 / 34.9 (58.4 / 66.0)
+//   16/1   128    6    19.4 /  5.9  20.1 /  6.0  20.7 /  7.5  21.9 /  8.8  23.9 / 11.3  29.3 / 16.4
+constexpr int kMaxSpread = 8;
+constexpr int few_steps(int form) { return form == 16 ? 4 : 8; }
 
 // 4 CTAs of 4 warps an SM, as head_dim 64 has by itself: 132 registers instead of
 // 128 would let one cluster in four go.
@@ -1145,7 +1153,7 @@ cudaError_t launch_step(const PagedCache& c, int dtype, const Attend& a, const S
     using T = decltype(type);
     constexpr int D = decltype(dim)::value, NB = decltype(bs)::value, Form = decltype(f)::value;
     auto fits = [&](int warps, int clusters) {
-      return units <= clusters && reach <= static_cast<int64_t>(kFewSteps) * warps * 16 * step_tiles(D, Form);
+      return units <= clusters && reach <= static_cast<int64_t>(few_steps(Form)) * warps * 16 * step_tiles(D, Form);
     };
     if (shared.base == nullptr) {
       if (reach > 32 * 16 * step_tiles(D, Form) && fits(64, few_clusters<T, D, NB, 8, 8, Form>()))
