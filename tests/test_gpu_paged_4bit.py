@@ -321,7 +321,15 @@ def some_keys(n, keys):
 @pytest.mark.parametrize("window", [0, 50])
 def test_step_masks(pc, dtype, d, wide, window):
     check(pc, [70, 33, 129, 16, 0, 1], d=d, mask=some_keys, window=window, sinks=8 if window else 0, dtype=dtype, hkv=3,
-          group=3, table_pages=1024 if wide else None)
+          group=3, table_pages=4096 if wide else None)
+
+
+@pytest.mark.parametrize("d,group,window,sinks", [(64, 1, 17, 3), (64, 2, 40, 33), (64, 8, 100, 0), (128, 2, 64, 16), (128, 4, 1, 20),
+                                                  (128, 1, 90, 5)])
+def test_step_windows_of_many_slots(pc, d, group, window, sinks):
+    """More slots and heads than there are clusters: the line of tiles, whose shares begin and end inside windows."""
+    lengths = np.random.default_rng(window).integers(0, 260, 330).tolist()
+    check(pc, lengths, d=d, group=group, window=window, sinks=sinks, seed=window, dtype=TYPES[window % 2])
 
 
 def test_step_many_slots_and_scale(pc):
