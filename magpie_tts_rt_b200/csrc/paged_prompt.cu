@@ -1131,6 +1131,19 @@ __global__ void __launch_bounds__(PromptCfg<D, Bits>::kThreads, 1)
                   float top = m;
 #pragma unroll
                   for (int k = 0; k < 32; k += 2) top = max_nan(top, __uint_as_float(s[k]), __uint_as_float(s[k + 1]));
+                  // The chunk before waits in P, rounded: the maximum then rises by a whole power of two of the weights, short
+                  // of the largest by less than one, so that P by it is exact and a weight is rounded once.  (In f16 but
+                  // for what falls below its normal range, as a weight does that was that small at once.)
+                  float rescale = 1.f;
+                  if (x > 0 && m != -CUDART_INF_F) {
+                    const float up = floorf((top - m) * a.scale2);
+                    if (up < 126.f) {  // (past that, and where a score is not a number, nothing is left of P)
+                      rescale = __uint_as_float(static_cast<uint32_t>(127 - static_cast<int>(up)) << 23);
+                      top = up > 0.f ? m + up / a.scale2 : m;
+                    } else {
+                      rescale = up >= 126.f ? 0.f : CUDART_NAN_F;
+                    }
+                  }
                   const float f = m == -CUDART_INF_F ? 1.f : ex2((m - top) * a.scale2);
                   l *= f;
                   if (started || h == 1) {
@@ -1147,14 +1160,14 @@ __global__ void __launch_bounds__(PromptCfg<D, Bits>::kThreads, 1)
                       tmem_st16(o_col + 16 * b, o);
                     }
                   }
-                  if (x > 0) {  // the chunk before, whose weights wait in P: at most 2^-15 of these, so that rounding them again is nothing
+                  if (x > 0) {
                     uint32_t p[16];
                     tmem_wait_st();
                     tmem_ld16(p, h_col);
 #pragma unroll
                     for (int k = 0; k < 16; ++k) {
                       const float2 v = unpack2<T>(p[k]);
-                      p[k] = Half16<T>::pack(v.x * f, v.y * f);
+                      p[k] = Half16<T>::pack(v.x * rescale, v.y * rescale);
                     }
                     tmem_st16(h_col, p);
                   }
