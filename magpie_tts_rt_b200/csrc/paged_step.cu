@@ -36,7 +36,7 @@
 // it is entered (249 -> 253 us, the short ones 10 us more).
 //
 // A pool in 4 bits (attend_tiles4) takes 9/32 of the bytes, and instructions bound
-// it: the same 512 slots 109 us (306 MB, 2.8 TB/s), the same 8 slots in f16 136 us
+// it: the same 512 slots 109 us (306 MB, 2.8 TB/s), the same 8 slots in f16 138 us
 // (422 MB, 3.1 TB/s), the logic pipe busy 66 and 64% of the time, the schedulers 51 and 52.
 #include <algorithm>
 #include <atomic>
@@ -334,9 +334,12 @@ __device__ __forceinline__ int step_column(int g) {
 // attend_tiles for a pool in 4 bits.  Nothing is rounded on the way into the
 // products: a code is a small whole number, exact in either 16-bit type, and the
 // pairs come in afterwards, in f32,
-//   q.k = sum over groups: step (q.(16 + c)) + off sum q,   off = low - 16 step;
+//   q.k = sum over groups: step (q.(16 + c) - 16 sum q) + low sum q;
 // the values' weights are p step, in two bf16 numbers each (their range is not
-// f16's), and p off is summed by itself.
+// f16's), and p low - 16 p step is summed by itself.  A weight is so right to 2^-16, and
+// a value to 2^-16 of p 31 step.  (step itself is not multiplied, and probabilities are
+// an eighth of what they are: 16 or 31 times the step of bf16's largest groups would
+// leave f32.)
 //
 // What bounds it is instructions, above all the logic and shift unit's: the codes'
 // way into 16 bits takes two for each pair of codes, 64 a tile of 16 keys and 64
@@ -372,7 +375,8 @@ __device__ __forceinline__ void attend_tiles4(const PagedCache& c, const Attend&
   const int col_tile = g >> (kTileShift + 1);  // the tile of column g
   auto &m = sums.m, &l = sums.l;
   auto& acc = sums.acc;
-  // the queries' sums over each group, times the scale
+  constexpr float kLess = 3.f;            // probabilities are held 2^3 times smaller
+  // the queries' sums over each group
   float qs[NB][G][QC], rest[NB][G][QC];
 #pragma unroll
   for (int b = 0; b < NB; ++b)
@@ -393,7 +397,7 @@ __device__ __forceinline__ void attend_tiles4(const PagedCache& c, const Attend&
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
 #pragma unroll
       for (int i = 0; i < QC; ++i) {
-        qs[b][v][i] = __shfl_sync(0xffffffffu, sum, 4 * (2 * t + i)) * a.scale2;
+        qs[b][v][i] = __shfl_sync(0xffffffffu, sum, 4 * (2 * t + i));
         rest[b][v][i] = 0.f;
       }
     }
@@ -532,15 +536,15 @@ __device__ __forceinline__ void attend_tiles4(const PagedCache& c, const Attend&
         for (int h = 0; h < 2; ++h) {
 #pragma unroll
           for (int v = 0; v < G; ++v) {
-            const float2 so = step_off(unpack2<T>(kp[n][h][v]));
-            const float step = so.x * a.scale2;
+            const float2 pair = unpack2<T>(kp[n][h][v]);  // step, low
 #pragma unroll
             for (int i = 0; i < QC; ++i)
-              s[b][n][h][i] = fmaf(step, x[v][2 * h + i], v == 0 ? so.y * qs[b][0][i] : fmaf(so.y, qs[b][v][i], s[b][n][h][i]));
+              s[b][n][h][i] = fmaf(pair.x, fmaf(-16.f, qs[b][v][i], x[v][2 * h + i]),
+                                   v == 0 ? pair.y * qs[b][0][i] : fmaf(pair.y, qs[b][v][i], s[b][n][h][i]));
           }
 #pragma unroll
           for (int i = 0; i < QC; ++i) {
-            s[b][n][h][i] = on[n][h] ? s[b][n][h][i] : -CUDART_INF_F;
+            s[b][n][h][i] = on[n][h] ? s[b][n][h][i] * a.scale2 : -CUDART_INF_F;
             top[b][i] = fmaxf(top[b][i], s[b][n][h][i]);
           }
         }
@@ -580,7 +584,7 @@ __device__ __forceinline__ void attend_tiles4(const PagedCache& c, const Attend&
       }
       float z[QC];
 #pragma unroll
-      for (int i = 0; i < QC; ++i) z[i] = m[b][i] == -CUDART_INF_F ? 0.f : m[b][i];
+      for (int i = 0; i < QC; ++i) z[i] = m[b][i] == -CUDART_INF_F ? 0.f : m[b][i] + kLess;
 #pragma unroll
       for (int n = 0; n < NP; ++n) {
         float w[2][QC];
@@ -596,14 +600,17 @@ __device__ __forceinline__ void attend_tiles4(const PagedCache& c, const Attend&
           uint32_t first[2], second[2];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const float2 so = step_off(unpack2<T>(on[n][h] ? vp[n][h][v] : 0u));
+            const float2 pair = unpack2<T>(on[n][h] ? vp[n][h][v] : 0u);
+            float ws[QC];
 #pragma unroll
-            for (int i = 0; i < QC; ++i) rest[b][v][i] = fmaf(w[h][i], so.y, rest[b][v][i]);
-            const float x0 = w[h][0] * so.x;
+            for (int i = 0; i < QC; ++i) {
+              ws[i] = w[h][i] * pair.x;
+              rest[b][v][i] = fmaf(-16.f, ws[i], fmaf(w[h][i], pair.y, rest[b][v][i]));
+            }
             if constexpr (QC == 1) {
-              first[h] = transpose8x8(Half16<B>::pack(x0, x0 - unpack2<B>(Half16<B>::pack(x0, 0.f)).x));
+              first[h] = transpose8x8(Half16<B>::pack(ws[0], ws[0] - unpack2<B>(Half16<B>::pack(ws[0], 0.f)).x));
             } else {
-              const uint2 x = Half16<B>::split(x0, w[h][1] * so.x);
+              const uint2 x = Half16<B>::split(ws[0], ws[1]);
               first[h] = transpose8x8(x.x);
               second[h] = transpose8x8(x.y);
             }
@@ -646,6 +653,7 @@ __device__ __forceinline__ void attend_tiles4(const PagedCache& c, const Attend&
   for (int b = 0; b < NB; ++b)
 #pragma unroll
     for (int i = 0; i < QC; ++i) {
+      m[b][i] += kLess;
       l[b][i] = over_tiles(l[b][i]);
 #pragma unroll
       for (int v = 0; v < G; ++v) {
