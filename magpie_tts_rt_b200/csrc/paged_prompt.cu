@@ -555,9 +555,24 @@ struct Convert4 {
     for (int b = 0; b < DB; ++b) {
       const uint4 x = raw->codes[slot][b][lane];
       const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-      const float2 so = step_off(unpack2<T>(raw->pair[slot][b][lane >> 1]));
+      const float2 pair = unpack2<T>(raw->pair[slot][b][lane >> 1]), so = step_off(pair);
       const float2 step = make_float2(so.x, so.x), off = make_float2(so.y, so.y);
       unsigned char* to = stage + b * (kHalf * 128) + row * 128;
+      if (std::is_same_v<T, __nv_bfloat16> && !(fabsf(so.y) <= 3.402823466e38f)) {
+        // the largest steps, 16 of which leave f32 (or a pair that is not finite): code by code
+#pragma unroll 1
+        for (int n = 0; n < 16; ++n) {
+          const uint32_t w2 = reinterpret_cast<const uint32_t*>(&raw->codes[slot][b][lane])[n >> 2] >> (4 * (n & 3));
+          const float2 v = make_float2(fmaf(static_cast<float>(w2 & 15u), pair.x, pair.y),
+                                       fmaf(static_cast<float>(w2 >> 16 & 15u), pair.x, pair.y));
+          const uint32_t hi = Half16<T>::pack(v.x, v.y);
+          const float2 near = unpack2<T>(hi);
+          const int at = 16 * ((4 * (lane & 1) + (n >> 2)) ^ (row & 7)) + 4 * (n & 3);
+          *reinterpret_cast<uint32_t*>(to + at) = hi;
+          *reinterpret_cast<uint32_t*>(to + DB * kHalf * 128 + at) = Half16<T>::pack(v.x - near.x, v.y - near.y);
+        }
+        continue;
+      }
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         uint32_t hi[4], lo[4];

@@ -122,7 +122,7 @@ def test_large_values(pc, dtype, new, table_pages, d, group):  # noqa: F811
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("new,table_pages", WAYS[:2], ids=["clusters", "line"])
+@pytest.mark.parametrize("new,table_pages", WAYS, ids=["clusters", "line", "prompt"])
 @pytest.mark.parametrize("d,group", [(64, 1), (64, 2), (64, 4), (64, 8), (64, 16), (128, 1), (128, 4), (128, 8), (128, 16)])
 def test_large_keys(pc, dtype, new, table_pages, d, group):  # noqa: F811
     """Queries so small that scores of the largest keys are ordinary ones."""
