@@ -147,3 +147,34 @@ def test_awkward_groups(pc, dtype, new, table_pages, d, group):  # noqa: F811
     put(pool, table, 2, 0, 1, x[1])
     cache.pool.copy_(pool)
     check(cache, pool, table, LENGTHS, queries(sum(new) if new else len(LENGTHS), 2 * group, d, dtype, 4), new, dtype)
+
+
+@pytest.mark.parametrize("table_pages", [None, 4096], ids=["clusters", "line"])
+@pytest.mark.parametrize("d,group", [(64, 1), (64, 2), (64, 4), (64, 8), (64, 16), (128, 1), (128, 4), (128, 8), (128, 16)])
+def test_small_values_of_wide_groups(pc, table_pages, d, group):  # noqa: F811
+    """Dims that are 0 beside -8 and 7: their error goes by the steps, u |out| + 2^-16 sum_j p_j 31 step_j as the header
+    says (in f16, whose u is small), scores and f32 sums apart; of 2^-16 sum_j p_j |v_j| nothing would be left for them."""
+    dtype, scale = torch.float16, d ** -0.5
+    cache, pool, table = filled(pc, d, 2, dtype, table_pages)
+    g = torch.Generator().manual_seed(2)
+    for i, n in enumerate(LENGTHS):
+        for token in range(n):
+            x = torch.randint(-8, 8, (2, d), generator=g).to(dtype)
+            x[:, ::8], x[:, 1::64], x[:, 2::64] = 0, -8, 7
+            put(pool, table, i, token, 1, x)
+    cache.pool.copy_(pool)
+    q = (0.05 * queries(len(LENGTHS), 2 * group, d, torch.float32, 4)).to(dtype)
+    held, (step, low) = O.held(pool, dtype), pairs_of(pool, dtype)
+    assert (held[table[1, 0], 1, 1, 0, 0, ::8] == 0).all() and step[table[1, 0], 1, 1, 0, 0, 0] == 1
+    out, _, weight = O.attention(held, table, LENGTHS, 1, q, list(range(len(LENGTHS) + 1)))
+    got = cache.attend(1, q.cuda()).cpu().double()
+    for i, n in enumerate(LENGTHS):
+        if n == 0:
+            continue
+        j = np.arange(n)
+        page = torch.as_tensor(np.asarray(table[i])[j // 16], dtype=torch.long)
+        size = 47 * step[page, 1, 0, :, j % 16] + low[page, 1, 0, :, j % 16].abs()
+        delta = (2 * d + 16) * 2.0 ** -24 * scale * torch.einsum("hgd,khd->hgk", q[i].double().reshape(2, -1, d).abs(), size).amax()
+        sums = 2.0 ** -20 * 39                          # exponentials and sums in f32, of p (31 step + |low|)
+        tol = 1.1 * (2.0 ** -16 * 31 + 2.0 ** -11 * out[i].abs()) + torch.expm1(2 * delta) * weight[i] + sums
+        assert ((got[i] - out[i]).abs() <= tol).all()
