@@ -100,6 +100,16 @@ def _written_rows(t, shape, name, dtype, index) -> int:
     return row
 
 
+def _layers_overlap(layers: int, layer: int, rows: int, row: int, block: int) -> bool:
+    """Whether blocks of `block` elements at i layer + j row, i < layers, j < rows, share
+    memory.  (Rows of one layer do not: _written_rows.)"""
+    for d in range(layer, layers * layer, layer) if layer > 0 else [0] * (layers - 1):
+        j = min(d // row, rows - 1) if rows > 1 else 0   # the row that begins last at or before d
+        if d - j * row < block or (j + 1 < rows and (j + 1) * row - d < block):
+            return True
+    return False
+
+
 def _token_bytes(head_dim: int) -> int:
     """Of one token's keys, or values, of one head in a 4-bit pool."""
     return head_dim // 2 + head_dim // 16
@@ -314,8 +324,8 @@ class PagedCache:
         if given:
             for x, name in ((k, "k"), (v, "v")):
                 one = x if layer is not None else x[0]
-                _written_rows(one, one.shape, name, self.dtype, self._index)
-                _check(layer is not None or len(x) == 1 or abs(x.stride(0)) >= self.kv_heads * self.head_dim,
+                row = _written_rows(one, one.shape, name, self.dtype, self._index)
+                _check(layer is not None or rows == 0 or not _layers_overlap(len(x), x.stride(0), rows, row, self.kv_heads * self.head_dim),
                        f"layers of {name} overlap")
         self._call("mtt_b200_launch_paged_cache_load", self._ref, ctypes.byref(args), self._handle(stream))
         return k, v
