@@ -845,7 +845,8 @@ MTT_B200_API int mtt_b200_launch_paged_cache_store(const mtt_b200_paged_cache_t*
                                                    const mtt_b200_cache_rows_t* rows, void* stream);
 
 /* The reverse of store: reads the keys and values of each slot's last tokens
- * into rows of k and v (written; the same fields).  A row that no slot has, or
+ * into rows of k and v (written; the same fields; no two rows of the two may
+ * share memory).  A row that no slot has, or
  * whose slot has fewer tokens than rows, gets zeros, and so does one without a
  * page.  Of a 4-bit cache it gives the values that the codes stand for, rounded
  * once to the type. */

@@ -110,6 +110,28 @@ def _layers_overlap(layers: int, layer: int, rows: int, row: int, block: int) ->
     return False
 
 
+def _share(x: int, y: int, block_x: int, block_y: int, rows: int, row, layers: int = 1, layer=(0, 0)) -> bool:
+    """Whether two tensors' rows share memory: blocks of block_x elements at x + i layer[0] +
+    j row[0], of block_y at y + i layer[1] + j row[1], i < layers, j < rows."""
+    if rows == 0 or block_x == 0 or block_y == 0:
+        return False
+    row, layer = (0, 0) if rows == 1 else row, (0, 0) if layers == 1 else layer
+    ends = [(layers - 1) * l + (rows - 1) * r for l, r in zip(layer, row)]
+    if x + ends[0] + block_x <= y or y + ends[1] + block_y <= x:
+        return False
+    if row[0] == row[1] and layer[0] == layer[1]:   # views of one buffer: by the differences of i and j
+        for i in range(1 - layers, layers):
+            d = y - x + i * layer[0]                # a difference of j must bring it above -block_y and below block_x
+            j = max((-block_y - d) // row[0] + 1, 1 - rows) if rows > 1 else 0
+            if j < rows and -block_y < d + j * row[0] < block_x:
+                return True
+        return False
+    xs, ys = (at + (torch.arange(layers)[:, None] * l + torch.arange(rows) * r).flatten().sort().values
+              for at, l, r in zip((x, y), layer, row))
+    next_y = torch.searchsorted(ys, xs - block_y, right=True)
+    return bool((ys[next_y.clamp(max=len(ys) - 1)] < xs + block_x)[next_y < len(ys)].any())
+
+
 def _token_bytes(head_dim: int) -> int:
     """Of one token's keys, or values, of one head in a 4-bit pool."""
     return head_dim // 2 + head_dim // 16
@@ -310,7 +332,8 @@ class PagedCache:
         """(k, v): the keys and values of each slot's last tokens, in rows laid out
         as for ``store`` (of a 4-bit cache the values its codes stand for).  A row
         that no slot has, or whose slot has fewer tokens than rows, is 0.  k and v:
-        where they go, if given."""
+        where they go, if given; they must not share memory, but that one tensor may be given
+        for both, which then holds the values."""
         _check((k is None) == (v is None), "k and v are given together")
         given = k is not None
         if not given:
@@ -322,11 +345,20 @@ class PagedCache:
         args = self._cache_rows(k, v, layer, offsets)
         _check(args.rows == rows, "k and v have other rows than asked for")
         if given:
+            rows_at, layers_at = [], (0, 0) if layer is not None else (k.stride(0), v.stride(0))
             for x, name in ((k, "k"), (v, "v")):
                 one = x if layer is not None else x[0]
                 row = _written_rows(one, one.shape, name, self.dtype, self._index)
+                rows_at.append(row)
                 _check(layer is not None or rows == 0 or not _layers_overlap(len(x), x.stride(0), rows, row, self.kv_heads * self.head_dim),
                        f"layers of {name} overlap")
+            block = self.kv_heads * self.head_dim
+            if k.data_ptr() == v.data_ptr() and k.stride() == v.stride() and rows > 0:
+                with self._on(stream):
+                    apart = torch.empty(k.shape, dtype=self.dtype, device=self.device)
+                args = self._cache_rows(apart, v, layer, offsets)
+            elif _share(k.data_ptr() // 2, v.data_ptr() // 2, block, block, rows, rows_at, 1 if layer is not None else len(k), layers_at):
+                raise ValueError("k and v share memory")
         self._call("mtt_b200_launch_paged_cache_load", self._ref, ctypes.byref(args), self._handle(stream))
         return k, v
 

@@ -58,3 +58,59 @@ def test_load_of_no_rows(lib):  # noqa: F811
     none = torch.zeros(1, 0, H, D, dtype=torch.bfloat16).expand(2, 0, H, D)
     cache.load(0, k=none, v=none)
     assert len(lib.calls) == 1
+
+
+def two_layouts(n):
+    """Pairs of layouts in one storage whose own rows are apart: most of them views of a buffer of wider rows."""
+    rng, found = random.Random(5), []
+    while len(found) < n:
+        layers, rows = rng.choice([(1, 1), (1, 4), (2, 3), (3, 2), (4, 1), (3, 5)])
+        strides = [8 * rng.randint(16, 60) if rng.random() < 0.5 else rng.choice([128, 256, 384, 512, 768, 1024, 1536]) for _ in range(2)]
+        other = strides if rng.random() < 0.7 else [8 * rng.randint(16, 100) for _ in range(2)]
+        at = 8 * rng.randint(0, 120) if rng.random() < 0.5 else 128 * rng.randint(0, 12)
+        a, b = covered(0, (layers, rows), strides), covered(at, (layers, rows), other)
+        if a is not None and b is not None:
+            found.append((layers, rows, strides, other, at, bool(a & b)))
+    return found
+
+
+@pytest.mark.parametrize("swap", [False, True])
+def test_keys_and_values_into_one_storage(lib, swap):  # noqa: F811
+    storage = torch.zeros(20000, dtype=torch.bfloat16)
+    storage = storage[(-storage.data_ptr() // 2) % 8:]
+    found = two_layouts(600)
+    assert 100 < sum(share for *_, share in found) < 500
+    for layers, rows, strides, other, at, share in found:
+        cache = on_host(slots=8, layers=layers)
+        x, y = strided(storage, 0, (layers, rows), strides), strided(storage, at, (layers, rows), other)
+        if at == 0 and x.stride() == y.stride():
+            continue                                    # one tensor: see below
+        k, v = (y, x) if swap else (x, y)
+        before = len(lib.calls)
+        if share:
+            with pytest.raises(ValueError):
+                cache.load(rows, k=k, v=v)
+        else:
+            cache.load(rows, k=k, v=v)
+        assert len(lib.calls) == before + (not share)
+        if layers == 1:                                 # the same, one layer by itself
+            if share:
+                with pytest.raises(ValueError):
+                    cache.load(rows, layer=0, k=k[0], v=v[0])
+            else:
+                cache.load(rows, layer=0, k=k[0], v=v[0])
+
+
+def test_one_tensor_for_keys_and_values(lib, monkeypatch):  # noqa: F811
+    """The values go there, the keys elsewhere."""
+    from magpie_tts_rt_b200 import paged_cache as pc
+    made = []
+    real = pc.L.CacheRows
+    monkeypatch.setattr(pc.L, "CacheRows", lambda: made.append(real()) or made[-1])
+    cache, x = on_host(), torch.zeros(2, 3, 2, H, D, dtype=torch.bfloat16)[:, :, 0]
+    k, v = cache.load(3, k=x, v=x)
+    assert k is x and v is x and made[-1].v == x.data_ptr() and made[-1].v_row_stride == x.stride(1)
+    low, high = x.data_ptr(), x.data_ptr() + 2 * (x.stride(0) + 2 * x.stride(1) + BLOCK)
+    size = 2 * (made[-1].k_layer_stride + 2 * made[-1].k_row_stride + BLOCK)
+    assert made[-1].k + size <= low or made[-1].k >= high
+    assert len(lib.calls) == 1
