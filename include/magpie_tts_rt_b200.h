@@ -884,7 +884,7 @@ typedef struct mtt_b200_rotate_rows {
   const void* k;
   const void* v;             /* append only */
   void* q_out;               /* may be q (with its stride) */
-  void* k_out;               /* rotate only; may be k (with its stride) */
+  void* k_out;               /* rotate only; may be k (with its stride); apart from q_out */
   int64_t q_row_stride;
   int64_t k_row_stride;
   int64_t v_row_stride;

@@ -23,7 +23,7 @@ import torch
 
 from magpie_tts_rt_b200 import _lib as L
 from magpie_tts_rt_b200 import paged_cache as _cache
-from magpie_tts_rt_b200.paged_cache import _DTYPES, HEAD_DIMS, MAX_ROWS, _check, _raw_stream, _rows_of, _written_rows
+from magpie_tts_rt_b200.paged_cache import _DTYPES, HEAD_DIMS, MAX_ROWS, _check, _raw_stream, _rows_of, _share, _written_rows
 
 MAX_HEADS = 1 << 16
 
@@ -88,7 +88,7 @@ class Rotation:
         """(q, k) normed and turned: q [rows, q_heads, head_dim], k [rows, kv_heads,
         head_dim] bf16 or f16 (either may be None), rows of any stride with
         contiguous heads, positions [rows] int32.  q_out and k_out may be q and k;
-        otherwise they must not overlap what the call reads."""
+        otherwise they must not overlap what the call reads, nor each other."""
         first = k if q is None else q
         if first is None or first.dim() != 3:
             raise ValueError("a rotation needs queries or keys, [rows, heads, head_dim]")
@@ -104,8 +104,11 @@ class Rotation:
             handle = stream.cuda_stream
         else:
             raise ValueError("the stream belongs to another device than the rotation")
+        given = q_out is not None and k_out is not None
         q_heads, q_at, q_row, q_to, q_to_row, q_out = self._side(q, q_out, "q", rows, dtype, stream)
         k_heads, k_at, k_row, k_to, k_to_row, k_out = self._side(k, k_out, "k", rows, dtype, stream)
+        if given and _share(q_to // 2, k_to // 2, q_heads * self.head_dim, k_heads * self.head_dim, rows, (q_to_row, k_to_row)):
+            raise ValueError("q_out and k_out share memory")
         args = L.RotateRows(rows, q_heads, k_heads, 0, q_at, k_at, None, q_to, k_to, q_row, k_row, 0, q_to_row, k_to_row,
                             positions.data_ptr())
         if handle not in self._streams:

@@ -114,3 +114,42 @@ def test_one_tensor_for_keys_and_values(lib, monkeypatch):  # noqa: F811
     size = 2 * (made[-1].k_layer_stride + 2 * made[-1].k_row_stride + BLOCK)
     assert made[-1].k + size <= low or made[-1].k >= high
     assert len(lib.calls) == 1
+
+
+def test_queries_and_keys_into_one_storage(lib):  # noqa: F811
+    """Of other numbers of heads, too."""
+    r, rng = turner(), random.Random(7)
+    storage = torch.zeros(20000, dtype=torch.bfloat16)
+    storage = storage[(-storage.data_ptr() // 2) % 8:]
+    shared = 0
+    for _ in range(600):
+        rows, heads = rng.choice([1, 2, 5]), (rng.choice([1, 2, 4]), rng.choice([1, 2]))
+        row = [rng.choice([64 * h, 256, 384, 8 * rng.randint(8 * h, 60)]) for h in heads]
+        row[1] = row[0] if rng.random() < 0.6 and row[0] >= 64 * heads[1] else row[1]
+        at = 8 * rng.randint(0, 80) if rng.random() < 0.5 else 64 * rng.randint(0, 12)
+        a, b = (covered(x, (rows,), (s,), 64 * h) for x, s, h in zip((0, at), row, heads))
+        if a is None or b is None:
+            continue
+        outs = [torch.as_strided(storage, (rows, h, D), (s, D, 1), x) for x, s, h in zip((0, at), row, heads)]
+        q, k = (torch.zeros(rows, h, D, dtype=torch.bfloat16) for h in heads)
+        before, pos = len(lib.calls), torch.zeros(rows, dtype=torch.int32)
+        if a & b:
+            shared += 1
+            with pytest.raises(ValueError):
+                r.rotate(q, k, pos, q_out=outs[0], k_out=outs[1])
+        else:
+            r.rotate(q, k, pos, q_out=outs[0], k_out=outs[1])
+        assert len(lib.calls) == before + (not a & b)
+    assert shared > 50
+
+
+def test_rotating_in_place(lib):  # noqa: F811
+    """Queries and keys of one projection's rows, where they are."""
+    y, r = torch.zeros(3, 5, D, dtype=torch.bfloat16), turner()
+    q, k = y[:, :3], y[:, 3:]
+    got = r.rotate(q, k, torch.zeros(3, dtype=torch.int32), q_out=q, k_out=k)
+    assert got[0] is q and got[1] is k and len(lib.calls) == 1
+    for bad in (y[:, 2:4], y[:, :2], q[:, 1:]):
+        with pytest.raises(ValueError):
+            r.rotate(q, k, torch.zeros(3, dtype=torch.int32), q_out=q, k_out=bad)
+    assert len(lib.calls) == 1
