@@ -54,7 +54,7 @@ def pairs_of(pool, dtype):
     return p[..., 0].repeat_interleave(64, -1), p[..., 1].repeat_interleave(64, -1)
 
 
-def step_tolerance(pool, table, lengths, layer, q, ref, dtype, scale):
+def step_tolerance(pool, table, lengths, layer, q, ref, dtype, scale, window=0, sinks=0):
     """(of each output, of each log-sum-exp); see above."""
     held, (step, low) = O.held(pool, dtype), pairs_of(pool, dtype)
     out, lse, weight = ref
@@ -64,6 +64,8 @@ def step_tolerance(pool, table, lengths, layer, q, ref, dtype, scale):
         if n == 0:
             continue
         j = np.arange(n)
+        if window:
+            j = j[(n - 1 - j < window) | (j < sinks)]
         page = torch.as_tensor(np.asarray(table[i])[j // ps], dtype=torch.long)
         at = lambda x, kv: x[page, layer, kv, :, j % ps]    # noqa: E731  [n, hkv, d]
         x = q[i].double().reshape(hkv, -1, d)
