@@ -860,7 +860,8 @@ MTT_B200_API int mtt_b200_launch_paged_cache_load(const mtt_b200_paged_cache_t* 
  * a = 2 i, b = 2 i + 1; dims from rotary_dim on are not turned.  The angle is
  * taken in 64 bits and reduced to one turn, the rest is f32, and each result is
  * rounded once.  (A head whose squares add up past f32's range is normed as by an
- * infinite sum.) */
+ * infinite sum.)  turns and the weights are read when a call runs, and at each
+ * replay of a CUDA graph that holds one. */
 typedef struct mtt_b200_rotation {
   int32_t head_dim;        /* 64 or 128 */
   int32_t rotary_dim;      /* a multiple of 16, at most head_dim */

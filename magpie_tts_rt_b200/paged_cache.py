@@ -36,7 +36,8 @@ call on another stream than its own is the caller's to keep until the call is
 done.  Every call can be captured into a CUDA graph after one such call on the
 capturing stream (which makes that stream's workspace).  A graph goes on using
 that workspace: its replays must be ordered with that stream's other calls, and
-with the replays of other graphs captured on it.
+with the replays of other graphs captured on it.  The cache, and the ``PrefixGroups``
+and rotations of its calls, must outlive the graph.
 """
 from __future__ import annotations
 

@@ -36,7 +36,9 @@ class Rotation:
         head are turned, pair i by base^(-2 i / rotary_dim) radians a position, or
         by frequencies [rotary_dim / 2] (any real type).  q_norm, k_norm [head_dim]:
         weights of the norms.  All of it is copied, which is waited for: later changes of
-        the tensors do not reach the rotation, and any stream may use it."""
+        the tensors do not reach the rotation, and any stream may use it.  A rotation may
+        be dropped while calls that use it are still queued, but must outlive CUDA graphs
+        captured with it (a graph reads frequencies and weights when it is replayed)."""
         _check(head_dim in HEAD_DIMS, f"head_dim must be one of {HEAD_DIMS}")
         rotary_dim = head_dim if rotary_dim is None else rotary_dim
         _check(16 <= rotary_dim <= head_dim and rotary_dim % 16 == 0, "rotary_dim must be a multiple of 16, at most head_dim")
