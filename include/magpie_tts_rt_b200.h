@@ -935,8 +935,8 @@ MTT_B200_API int mtt_b200_launch_paged_cache_append(const mtt_b200_paged_cache_t
  * all of them that load gives finite.  Single tokens take keys and values as they
  * are, and hold p_j step_j, with the step of the value's group, in two bf16 numbers:
  * u |out| + 2^-16 sum_j p_j 31 step_j, also where a group's values are far smaller
- * than its spread (31 |q| summed over 64 dims has to be in f32's range).  Prompts
- * and shared prefixes take a key as two numbers of the cache's type (right to
+ * than its spread (31 |q| and 12 scale |q|, summed over 64 dims, have to be in
+ * f32's range).  Prompts and shared prefixes take a key as two numbers of the cache's type (right to
  * 2^-16 of it, or 2^-134; f16: to 2^-22, or 2^-25) and round each value once (a
  * further u sum_j p_j |v_j|).
  * status[i] becomes 4 when a bounded wait inside the prompt kernel gave up (the

@@ -36,7 +36,7 @@
 // it is entered (249 -> 253 us, the short ones 10 us more).
 //
 // A pool in 4 bits (attend_tiles4) takes 9/32 of the bytes, and instructions bound
-// it: the same 512 slots 109 us (306 MB, 2.8 TB/s), the same 8 slots in f16 138 us
+// it: the same 512 slots 109 us (306 MB, 2.8 TB/s), the same 8 slots in f16 136 us
 // (422 MB, 3.1 TB/s), the logic pipe busy 66 and 64% of the time, the schedulers 51 and 52.
 #include <algorithm>
 #include <atomic>
@@ -63,7 +63,8 @@ constexpr int step_form(int bits, int head_dim, int group) {
 // 16-key tiles per warp and step.  (4 bits, the same keys, or twice as many with 64
 // dims, in us with 4 / 2 / 1 tiles: 4 heads of 64 116 / 113 / -, 8 of 64 177 / 129 /
 // 143, 8 of 128 - / 124 / 129, 16 of 64 490 / 190 / 191, 16 of 128 - / 263 / 185:
-// what does not fit the registers is what costs.)
+// what does not fit the registers is what costs.  Since bf16's off is held as an eighth
+// 16 of 64 take 196 us and 16 of 128 191, the others within 1% of these.)
 constexpr int step_tiles(int head_dim, int form) {
   if (form == 16) return head_dim == 64 ? 2 : 1;
   return form == 9 ? 1 : form >= 4 ? 2 : 4;
@@ -334,12 +335,11 @@ __device__ __forceinline__ int step_column(int g) {
 // attend_tiles for a pool in 4 bits.  Nothing is rounded on the way into the
 // products: a code is a small whole number, exact in either 16-bit type, and the
 // pairs come in afterwards, in f32,
-//   q.k = sum over groups: step (q.(16 + c) - 16 sum q) + low sum q;
+//   q.k = sum over groups: step (q.(16 + c)) + off sum q,   off = low - 16 step;
 // the values' weights are p step, in two bf16 numbers each (their range is not
-// f16's), and p low - 16 p step is summed by itself.  A weight is so right to 2^-16, and
-// a value to 2^-16 of p 31 step.  (step itself is not multiplied, and probabilities are
-// an eighth of what they are: 16 or 31 times the step of bf16's largest groups would
-// leave f32.)
+// f16's), and p off is summed by itself.  A weight is so right to 2^-16, and a value
+// to 2^-16 of p 31 step.  Of bf16's largest groups 16 and 31 steps would leave f32:
+// there off, and the values, are an eighth of themselves.
 //
 // What bounds it is instructions, above all the logic and shift unit's: the codes'
 // way into 16 bits takes two for each pair of codes, 64 a tile of 16 keys and 64
@@ -375,8 +375,12 @@ __device__ __forceinline__ void attend_tiles4(const PagedCache& c, const Attend&
   const int col_tile = g >> (kTileShift + 1);  // the tile of column g
   auto &m = sums.m, &l = sums.l;
   auto& acc = sums.acc;
-  constexpr float kLess = 3.f;            // probabilities are held 2^3 times smaller
-  // the queries' sums over each group
+  constexpr float kPart = std::is_same_v<T, B> ? 0.125f : 1.f;  // of off, and of the values
+  auto step_part = [](uint32_t bits) {  // step, and the part of off
+    const float2 pair = unpack2<T>(bits);
+    return make_float2(pair.x, fmaf(-16.f * kPart, pair.x, kPart * pair.y));
+  };
+  // the queries' sums over each group, times the scale
   float qs[NB][G][QC], rest[NB][G][QC];
 #pragma unroll
   for (int b = 0; b < NB; ++b)
@@ -397,7 +401,7 @@ __device__ __forceinline__ void attend_tiles4(const PagedCache& c, const Attend&
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
 #pragma unroll
       for (int i = 0; i < QC; ++i) {
-        qs[b][v][i] = __shfl_sync(0xffffffffu, sum, 4 * (2 * t + i));
+        qs[b][v][i] = __shfl_sync(0xffffffffu, sum, 4 * (2 * t + i)) * (a.scale2 / kPart);
         rest[b][v][i] = 0.f;
       }
     }
@@ -536,15 +540,15 @@ __device__ __forceinline__ void attend_tiles4(const PagedCache& c, const Attend&
         for (int h = 0; h < 2; ++h) {
 #pragma unroll
           for (int v = 0; v < G; ++v) {
-            const float2 pair = unpack2<T>(kp[n][h][v]);  // step, low
+            const float2 so = step_part(kp[n][h][v]);
+            const float step = so.x * a.scale2;
 #pragma unroll
             for (int i = 0; i < QC; ++i)
-              s[b][n][h][i] = fmaf(pair.x, fmaf(-16.f, qs[b][v][i], x[v][2 * h + i]),
-                                   v == 0 ? pair.y * qs[b][0][i] : fmaf(pair.y, qs[b][v][i], s[b][n][h][i]));
+              s[b][n][h][i] = fmaf(step, x[v][2 * h + i], v == 0 ? so.y * qs[b][0][i] : fmaf(so.y, qs[b][v][i], s[b][n][h][i]));
           }
 #pragma unroll
           for (int i = 0; i < QC; ++i) {
-            s[b][n][h][i] = on[n][h] ? s[b][n][h][i] * a.scale2 : -CUDART_INF_F;
+            s[b][n][h][i] = on[n][h] ? s[b][n][h][i] : -CUDART_INF_F;
             top[b][i] = fmaxf(top[b][i], s[b][n][h][i]);
           }
         }
@@ -584,7 +588,7 @@ __device__ __forceinline__ void attend_tiles4(const PagedCache& c, const Attend&
       }
       float z[QC];
 #pragma unroll
-      for (int i = 0; i < QC; ++i) z[i] = m[b][i] == -CUDART_INF_F ? 0.f : m[b][i] + kLess;
+      for (int i = 0; i < QC; ++i) z[i] = m[b][i] == -CUDART_INF_F ? 0.f : m[b][i];
 #pragma unroll
       for (int n = 0; n < NP; ++n) {
         float w[2][QC];
@@ -600,17 +604,15 @@ __device__ __forceinline__ void attend_tiles4(const PagedCache& c, const Attend&
           uint32_t first[2], second[2];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const float2 pair = unpack2<T>(on[n][h] ? vp[n][h][v] : 0u);
-            float ws[QC];
+            float2 so = step_part(on[n][h] ? vp[n][h][v] : 0u);
+            so.x *= kPart;
 #pragma unroll
-            for (int i = 0; i < QC; ++i) {
-              ws[i] = w[h][i] * pair.x;
-              rest[b][v][i] = fmaf(-16.f, ws[i], fmaf(w[h][i], pair.y, rest[b][v][i]));
-            }
+            for (int i = 0; i < QC; ++i) rest[b][v][i] = fmaf(w[h][i], so.y, rest[b][v][i]);
+            const float x0 = w[h][0] * so.x;
             if constexpr (QC == 1) {
-              first[h] = transpose8x8(Half16<B>::pack(ws[0], ws[0] - unpack2<B>(Half16<B>::pack(ws[0], 0.f)).x));
+              first[h] = transpose8x8(Half16<B>::pack(x0, x0 - unpack2<B>(Half16<B>::pack(x0, 0.f)).x));
             } else {
-              const uint2 x = Half16<B>::split(ws[0], ws[1]);
+              const uint2 x = Half16<B>::split(x0, w[h][1] * so.x);
               first[h] = transpose8x8(x.x);
               second[h] = transpose8x8(x.y);
             }
@@ -653,7 +655,6 @@ __device__ __forceinline__ void attend_tiles4(const PagedCache& c, const Attend&
   for (int b = 0; b < NB; ++b)
 #pragma unroll
     for (int i = 0; i < QC; ++i) {
-      m[b][i] += kLess;
       l[b][i] = over_tiles(l[b][i]);
 #pragma unroll
       for (int v = 0; v < G; ++v) {
@@ -666,7 +667,7 @@ __device__ __forceinline__ void attend_tiles4(const PagedCache& c, const Attend&
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
             float& o = acc[b][v][w][2 * k + i];
-            o = over_tiles(QC == 1 ? o + acc[b][v][w][2 * k + 1] : o) + x;
+            o = (over_tiles(QC == 1 ? o + acc[b][v][w][2 * k + 1] : o) + x) * (1.f / kPart);
           }
       }
     }
