@@ -42,7 +42,7 @@ class Rotation:
         _check(head_dim in HEAD_DIMS, f"head_dim must be one of {HEAD_DIMS}")
         rotary_dim = head_dim if rotary_dim is None else rotary_dim
         _check(16 <= rotary_dim <= head_dim and rotary_dim % 16 == 0, "rotary_dim must be a multiple of 16, at most head_dim")
-        _check(eps >= 0 and math.isfinite(eps), "eps must not be negative")
+        _check(0 <= eps <= torch.finfo(torch.float32).max, "eps must not be negative, and held by single precision")
         if frequencies is None:
             _check(base > 0 and math.isfinite(base), "base must be positive")
             radians = [base ** (-2.0 * i / rotary_dim) for i in range(rotary_dim // 2)]
