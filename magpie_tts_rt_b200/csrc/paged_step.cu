@@ -69,7 +69,7 @@ constexpr int step_tiles(int head_dim, int form) {
   if (form == 16) return head_dim == 64 ? 2 : 1;
   return form == 9 ? 1 : form >= 4 ? 2 : 4;
 }
-constexpr int step_ctas(int head_dim, int nb, int form) {  // per SM (registers)
+constexpr int step_ctas(int head_dim, int nb) {  // per SM (registers)
   return (head_dim == 64 ? 4 : 3) - (nb == 2 ? 1 : 0);
 }
 
@@ -685,7 +685,7 @@ __device__ __forceinline__ void attend_tiles_of(const PagedCache& c, const Atten
 }
 
 template <typename T, int D, int NB, int Form>
-__global__ void __launch_bounds__(kStepThreads, step_ctas(D, NB, Form))
+__global__ void __launch_bounds__(kStepThreads, step_ctas(D, NB))
     step_kernel(PagedCache c, Attend a, SharedPrefix shared, StepSpace ws, int blocks, int min_tiles) {
   constexpr int NT = step_tiles(D, Form), kUnitCost = unit_cost(Form);
   constexpr int NQ = 8 * NB;   // query rows of a unit
@@ -773,7 +773,7 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(D, NB, Form))
   SeenTiles seen = tiles_of(slot);
   int base_tokens = shared.base != nullptr ? shared.base[slot] : 0;
   uint4 q[NB][KC];
-  int page[NT];
+  int page[NT];  // (16 bits; attend_tiles4 looks its tiles' up by itself)
   // the unit's share, its queries and its first pages
   auto enter = [&] {
     t0 = static_cast<int>(max(x - unit_x - kUnitCost, static_cast<int64_t>(0)));
@@ -785,9 +785,11 @@ __global__ void __launch_bounds__(kStepThreads, step_ctas(D, NB, Form))
     for (int b = 0; b < NB; ++b)
 #pragma unroll
       for (int k = 0; k < KC; ++k) q[b][k] = load16(a.q + q_at + 8 * b * D + step_dims<Form>(t, k), 8 * b + col < queries);
-    const int32_t* row = c.table + static_cast<int64_t>(slot) * c.table_pages;
+    if constexpr (Form == 16) {
+      const int32_t* row = c.table + static_cast<int64_t>(slot) * c.table_pages;
 #pragma unroll
-    for (int u = 0; u < NT; ++u) page[u] = t0 + u < t1 ? row[(16 * seen.tile(t0 + u)) >> c.page_shift] : -1;
+      for (int u = 0; u < NT; ++u) page[u] = t0 + u < t1 ? row[(16 * seen.tile(t0 + u)) >> c.page_shift] : -1;
+    }
   };
   enter();
   while (true) {
@@ -985,8 +987,10 @@ __global__ void __launch_bounds__(32 * W, D == 128 && NB == 1 && W == 4 ? 4 : 0)
   const int32_t* row = c.table + static_cast<int64_t>(slot) * c.table_pages;
   uint4 q[NB][KC];
   int page[NT];
+  if constexpr (Form == 16) {
 #pragma unroll
-  for (int u = 0; u < NT; ++u) page[u] = t0 + u < t1 ? row[(16 * seen.tile(t0 + u)) >> c.page_shift] : -1;
+    for (int u = 0; u < NT; ++u) page[u] = t0 + u < t1 ? row[(16 * seen.tile(t0 + u)) >> c.page_shift] : -1;
+  }
   const int col = step_column<Form>(g);
   const int64_t q_at = slot * a.q_row + static_cast<int64_t>(q_head + col) * D;
 #pragma unroll
@@ -1111,16 +1115,15 @@ void step_blocks(int group, int* nb, int* blocks) {
 // cut records, then parts; sized for the largest device this library runs on
 // (kMaxSms SMs), so that the size does not depend on the current one
 constexpr int kMaxSms = 160;
-size_t cut_bytes(int head_dim, int nb, int form) {
-  return static_cast<size_t>(kMaxSms) * step_ctas(head_dim, nb, form) * kStepWarps * sizeof(int4);
+size_t cut_bytes(int head_dim, int nb) {
+  return static_cast<size_t>(kMaxSms) * step_ctas(head_dim, nb) * kStepWarps * sizeof(int4);
 }
 
 size_t step_workspace(const mtt_b200_paged_cache_t& c, int q_heads) {
   int nb, blocks;
   step_blocks(q_heads / c.kv_heads, &nb, &blocks);
-  const int form = step_form((c.dtype & MTT_B200_CACHE_4BIT) != 0 ? 4 : 16, c.head_dim, q_heads / c.kv_heads);
-  const size_t shares = static_cast<size_t>(kMaxSms) * step_ctas(c.head_dim, nb, form) * kStepWarps;
-  return cut_bytes(c.head_dim, nb, form) + (shares * 2 * 8 * nb * (c.head_dim + 2) * 4 + 255) / 256 * 256;
+  const size_t shares = static_cast<size_t>(kMaxSms) * step_ctas(c.head_dim, nb) * kStepWarps;
+  return cut_bytes(c.head_dim, nb) + (shares * 2 * 8 * nb * (c.head_dim + 2) * 4 + 255) / 256 * 256;
 }
 
 cudaError_t launch_step(const PagedCache& c, int dtype, const Attend& a, const SharedPrefix& shared, void* space,
@@ -1130,11 +1133,11 @@ cudaError_t launch_step(const PagedCache& c, int dtype, const Attend& a, const S
   const int form = step_form(c.bits, c.head_dim, a.group);
   StepSpace ws;
   ws.cut = static_cast<int4*>(space);
-  ws.part = reinterpret_cast<float*>(static_cast<char*>(space) + cut_bytes(c.head_dim, nb, form));
+  ws.part = reinterpret_cast<float*>(static_cast<char*>(space) + cut_bytes(c.head_dim, nb));
   const int sms = cache_sm_count();
   if (sms <= 0 || sms > kMaxSms) return cudaErrorInvalidValue;
   const size_t smem = 4 * (static_cast<size_t>(a.rows) + 1);
-  const int grid = sms * step_ctas(c.head_dim, nb, form), shares = grid * kStepWarps;
+  const int grid = sms * step_ctas(c.head_dim, nb), shares = grid * kStepWarps;
   const int min_tiles = unit_cost(form) + step_tiles(c.head_dim, form);
   const int pairs = std::min(8 * nb, a.group) * c.head_dim / 2;
   auto go = [&](auto kernel, auto join) {
