@@ -5,9 +5,10 @@
 // load where the rows allow it), so that a group's 64 dims lie in 4 lanes: minimum and
 // maximum take two shuffles in packed 16-bit pairs.  HBM bounds both kernels as long
 // as instructions stay few (store4: the schedulers are busy 78% of the time), and a
-// load's as long as enough of them are on their way.  26,208 rows of 8 layers, 8 heads
-// of 128: stored in 207 us (1.10 GB, 5.3 TB/s), loaded in 180 (6.1 TB/s; one head of a lane
-// ahead instead of four 216), from 16 bits 263 (6.5 TB/s; one ahead 264, four 274).
+// load's as long as enough of them are on their way.  16,892 rows (prompts of 96 slots) of 8
+// layers, 8 heads of 128, in a graph: stored in 142 us (709 MB, 5.0 TB/s), loaded in 120
+// (5.9 TB/s; one head of a lane ahead instead of four 141), from 16 bits 173 (1.11 GB, 6.4
+// TB/s; one ahead 172, four 179).
 #include "cache4.cuh"
 
 namespace mtt {

@@ -3,7 +3,9 @@
 //
 //   y = x w / sqrt(mean x^2 + eps);  (y_a, y_b) <- (y_a cos - y_b sin, y_b cos + y_a sin)
 //
-// HBM bounds it: every element is read and written once.  A head is held by
+// Every element is read and written once: HBM bounds many rows, latency few, and a
+// prompt's append (offsets, length, table and reference count follow one another
+// before a row's first use, one pass of loads on its way).  A head is held by
 // head_dim / 16 lanes as two 16-byte pieces each, chosen so that both dims of
 // every pair lie in the same lane and a lane has the same 8 pairs in every head.  A
 // warp takes a row's heads, a few at a time, and finds the row's cosines and sines
@@ -12,9 +14,9 @@
 // element, in pairs of f32, and a factor for the head.  The mean takes two or three
 // shuffles.  What hides the loads is warps: 32 an SM, for which a lane's coefficients
 // lie in shared memory (in registers, 16 warps with four passes' loads in flight
-// each: 45 us instead of 33 for 8192 rows of 32 and 8 heads of 128, which is 5.1
-// TB/s; the append of 6,600 such rows 34 us, into 4 bits 41, where 111 registers leave
-// 16 warps).
+// each: 45 us instead of 32 for 8192 rows of 32 and 8 heads of 128, which is 5.3
+// TB/s; the append of 7105 such rows, prompts of 24 slots, 39 us (4.5 TB/s), into 4 bits
+// 48 (3.2 TB/s), where 111 registers leave 16 warps).
 //
 // The angle is position x turns in 64 bits, of which only the part past whole
 // turns is kept: exact to 2^-22 of a turn at positions up to 2^31, where a 32-bit
@@ -28,7 +30,9 @@ namespace {
 
 constexpr int kRotThreads = 128;
 constexpr int kRotWarps = kRotThreads / 32;
-constexpr int kRotAhead = 1;  // passes whose loads are on their way while another is turned
+// Passes whose loads are on their way while another is turned.  (With the loops over it written out for one the compiler
+// spills 24 bytes instead of 0 to 16: 8192 rows 34 us instead of 32.)
+constexpr int kRotAhead = 1;
 
 enum class Into { kRows, kCache16, kCache4 };
 
