@@ -35,9 +35,11 @@
 // when the line took 162 and 238); a unit's further tiles prefetched into L2 when
 // it is entered (249 -> 253 us, the short ones 10 us more).
 //
-// A pool in 4 bits (attend_tiles4) takes 9/32 of the bytes, and instructions bound
-// it: the same 512 slots 109 us (306 MB, 2.8 TB/s), the same 8 slots in f16 136 us
-// (422 MB, 3.1 TB/s), the logic pipe busy 66 and 64% of the time, the schedulers 51 and 52.
+// A pool in 4 bits (attend_tiles4) takes 9/32 of the bytes: the same 512 slots 108 us
+// (306 MB, 2.8 TB/s), the same 8 slots in f16 135 us (422 MB, 3.1 TB/s).  Nothing is full
+// there: the logic pipe is busy 66 and 64% of the time, the schedulers 51 and 52, with 13
+// and 10 warps an SM (128 and 168 registers) to cover a step's chain of load, score,
+// maximum and weight.
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -341,9 +343,9 @@ __device__ __forceinline__ int step_column(int g) {
 // to 2^-16 of p 31 step.  Of bf16's largest groups 16 and 31 steps would leave f32:
 // there off, and the values, are an eighth of themselves.
 //
-// What bounds it is instructions, above all the logic and shift unit's: the codes'
-// way into 16 bits takes two for each pair of codes, 64 a tile of 16 keys and 64
-// dims, and so the rest has to be few.
+// What is busiest is the logic and shift unit: the codes' way into 16 bits takes two
+// instructions for each pair of codes, 64 a tile of 16 keys and 64 dims, and so the
+// rest has to be few; the other bound is registers, and with them warps.
 //  * A product has 8 columns.  Few queries take them several times, each time for
 //    another tile: with one or two queries (Form 1, 2) a thread's two columns are
 //    those of tile t of four, with up to four of tile t / 2 of two.  Scores of the
