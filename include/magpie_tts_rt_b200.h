@@ -936,9 +936,12 @@ MTT_B200_API int mtt_b200_launch_paged_cache_append(const mtt_b200_paged_cache_t
  * are, and hold p_j step_j, with the step of the value's group, in two bf16 numbers:
  * u |out| + 2^-16 sum_j p_j 31 step_j, also where a group's values are far smaller
  * than its spread (31 |q| and 12 scale |q|, summed over 64 dims, have to be in
- * f32's range).  Prompts and shared prefixes take a key as two numbers of the cache's type (right to
- * 2^-16 of it, or 2^-134; f16: to 2^-22, or 2^-25) and round each value once (a
- * further u sum_j p_j |v_j|).
+ * f32's range).  Prompts and shared prefixes take a key as two numbers of the
+ * cache's type (right to 2^-16 of it, or 2^-134; f16: to 2^-22, or 2^-25) and round
+ * each value once (a further u sum_j p_j |v_j|).
+ * Of either cache, values are summed in f32 before the division by the sum of their
+ * weights, which is at most n for the n keys that a single token sees, and 2^10 n in
+ * a prompt: bf16 values past 2^128 and 2^118 over that n may come out infinite.
  * status[i] becomes 4 when a bounded wait inside the prompt kernel gave up (the
  * bounds grow with the keys that the call has to read): the outputs of slot i's
  * rows are then not to be used. */
